@@ -60,6 +60,7 @@ extern "C" {
 /* KV pool element formats (va_kv_pool.kv_format) */
 #define VA_KV_NATIVE 0   /* the entry point's dtype (bf16 / f16 / f32)              */
 #define VA_KV_FP8_E4M3 1 /* OCP float8 e4m3 (float8_e4m3fn); element = code * scale */
+#define VA_KV_MXFP4 2    /* OCP MX e2m1 codes with e8m0 scales (the *_mx4 entry points) */
 
 /* how va_decode_args.lens is read */
 #define VA_LENS_PER_SEQ 0    /* lens[b] = context length of sequence b           */
@@ -330,6 +331,126 @@ size_t va_varlen_workspace_bytes(const va_varlen_args* args);
  * unsplit one up to rounding, and in its last bits depends on the launch's
  * other sequences.  Depends on the current device's compute-unit count. */
 size_t va_varlen_split_workspace_bytes(const va_varlen_args* args);
+
+/* ----------------------------------------------------------- MXFP4 pools */
+/*
+ * A pool of kv_format VA_KV_MXFP4 holds a row of D elements as D / 2 bytes of
+ * 4-bit e2m1 codes (element 2 i in the low half of byte i) and, in an array of
+ * its own, D / 32 e8m0 scale bytes, one per 32 elements: a code c with scale
+ * byte s stands for c * 2^(s - 127).  Its va_kv_pool gives the codes, strides
+ * counting bytes; va_mx4_scales gives the scales, addressed alike.  The pool's
+ * k_scale / v_scale are not read.  Rows of codes are 16-byte aligned, rows of
+ * scales aligned to D / 32 bytes where that is 2, 4 or 8.
+ *
+ * A store quantises 16-bit rows: the scale is the smallest 2^e with
+ * max |x| < 7 * 2^e over the group, with e in [-125, 125] for bf16 rows and
+ * [-23, 13] for f16 (6 * 2^e and 2^e / 2 are representable in the type), the
+ * codes are x / 2^e rounded to nearest, ties to even, saturating at 6.  A
+ * group that holds a NaN gets scale byte 255 and codes 0, and reads as NaN.
+ * A pool is read in the type it was written in, or in bf16: f16 does not hold
+ * every value that bf16 rows may have stored.
+ */
+typedef struct va_mx4_scales {
+  uint32_t struct_size; /* sizeof(va_mx4_scales)                         */
+  void* k;              /* scale bytes of the key pool                   */
+  void* v;              /* scale bytes of the value pool (same strides)  */
+  int64_t stride_block; /* bytes between consecutive blocks              */
+  int64_t stride_slot;  /* bytes between slots inside one block          */
+  int64_t stride_head;  /* bytes between kv heads                        */
+} va_mx4_scales;
+
+/* va_store_kvcache into an MXFP4 pool; 16-bit key / value rows, head_dim a
+ * multiple of 32. */
+int va_store_kvcache_mx4(const va_store_args* args, const va_mx4_scales* scales, void* stream);
+
+typedef struct va_load_args {
+  uint32_t struct_size;   /* sizeof(va_load_args)                        */
+  int32_t dtype;          /* VA_BF16 / VA_F16                            */
+  void* key;              /* [num_tokens, Hkv, D], written               */
+  void* value;
+  int64_t key_stride_tok, key_stride_head;
+  int64_t value_stride_tok, value_stride_head;
+  va_kv_pool pool;
+  const void* slot_mapping; /* [num_tokens]; slot < 0 or >= capacity reads as zeros */
+  int32_t slot_dtype;       /* VA_I32 / VA_I64                            */
+  int32_t num_tokens;
+  int32_t num_kv_heads;
+  int32_t head_dim;
+} va_load_args;
+
+/* The rows stored at slot_mapping, as 16-bit values (exact in the type they
+ * were stored from): the inverse of va_store_kvcache_mx4. */
+int va_load_kvcache_mx4(const va_load_args* args, const va_mx4_scales* scales, void* stream);
+
+/* va_paged_decode over an MXFP4 pool: bf16 / f16 q, head_dim 64 / 128 / 256,
+ * group 1 / 2 / 4 / 8, a block size that is a multiple of 16, scale > 0.  The
+ * current row is stored quantised and attended as stored. */
+int va_paged_decode_mx4(const va_decode_args* args, const va_mx4_scales* scales, void* stream);
+
+/* Bytes of workspace va_paged_decode_mx4 needs for these arguments; see
+ * va_paged_decode_workspace_bytes. */
+size_t va_paged_decode_mx4_workspace_bytes(const va_decode_args* args);
+
+/* va_varlen_attention over an MXFP4 pool: head_dim 64 / 128, no query
+ * prologue.  Prefix rows are converted inside the kernel; new rows are attended
+ * as given and stored quantised after the attention.  The workspace is
+ * va_varlen_split_workspace_bytes'. */
+int va_varlen_attention_mx4(const va_varlen_args* args, const va_mx4_scales* scales,
+                            void* stream);
+
+/* -------------------------------------------------------- step metadata */
+/*
+ * The metadata of one step over num_seqs requests, from their lengths on the
+ * device: request i's new tokens are positions [num_computed[i], lens[i]), its
+ * block table is row rows[i] (NULL: row i) of request_tables, and the outputs
+ * are those that the engine's host builders make
+ * (qwen_asr_vllm/engine/model_runner.py:183-233 and graph_runner.py:150-191).
+ * lens[i] is taken as 0 when negative and num_computed[i] held to
+ * [0, lens[i]].
+ *
+ * Rows num_seqs .. padded_seqs - 1 are padding as a captured decode graph has
+ * it: one token at position 0 with slot -1, table row 0, key length 1.  A
+ * request whose rows[i] is outside the table has slots and entries -1, and so
+ * has a token whose column is past the table's width or whose block id is
+ * negative.  Tokens past max_tokens are not written; entries of positions and
+ * slot_mapping behind the last token are 0 and -1.
+ *
+ * With free_count, request i holds the blocks of its computed tokens (columns
+ * below ceil(num_computed[i] / block_size)), and the blocks of its new columns
+ * are taken from the free list's end: the k-th block taken, in request order
+ * and ascending columns, is free_blocks[free_count - 1 - k].  They are written
+ * to the request's row of request_tables (rows[i] must then be distinct);
+ * columns past its width are not taken.  When the list runs out, the columns
+ * left get -1, and so the slots.  free_count is not written: totals
+ * says what is left, and a launch with the same inputs gives the same outputs.
+ */
+typedef struct va_batch_args {
+  uint32_t struct_size; /* sizeof(va_batch_args)                          */
+  int32_t index_dtype;  /* of lens and num_computed: VA_I32 / VA_I64      */
+  const void* lens;     /* [num_seqs] context lengths after the step      */
+  const void* num_computed; /* [num_seqs] tokens computed before it       */
+  int32_t* request_tables;  /* [num_requests, request_width]; read, and   */
+  int64_t request_stride;   /* written where blocks are taken             */
+  int32_t num_requests, request_width;
+  const int32_t* rows;      /* optional [num_seqs]                        */
+  int32_t num_seqs, padded_seqs; /* padded_seqs >= num_seqs               */
+  int32_t block_size;
+  int32_t max_tokens;       /* entries of positions and slot_mapping      */
+  int64_t* positions;       /* [max_tokens]                               */
+  int32_t* slot_mapping;    /* [max_tokens]                               */
+  int32_t* cu_seqlens_q;    /* [padded_seqs + 1]                          */
+  int32_t* cu_seqlens_k;    /* [padded_seqs + 1]                          */
+  int32_t* block_tables;    /* optional [padded_seqs, table_width]; -1    */
+  int64_t table_stride;     /* behind a request's last block              */
+  int32_t table_width;
+  int32_t* totals;          /* [5]: tokens, longest query, longest        */
+                            /* context, free blocks left, blocks missing  */
+  const int32_t* free_blocks; /* optional, with free_count                */
+  const int32_t* free_count;  /* [1] entries of free_blocks in use        */
+  int32_t free_capacity;      /* entries of free_blocks                   */
+} va_batch_args;
+
+int va_batch_metadata(const va_batch_args* args, void* stream);
 
 /* ----------------------------------------------------------------- misc */
 const char* va_last_error(void);

@@ -1,0 +1,195 @@
+"""ops.batch_metadata and the engine's device builders against plain integers,
+the host builders, and a served run over an MXFP4 pool."""
+
+import random
+
+import pytest
+import torch
+
+from oracle import mx4 as oracle
+from voiceagent_amd import ops
+from voiceagent_amd.engine import DecodeGraphMetadata, prepare_batch, prepare_batch_device
+from voiceagent_amd.layers.attention import PagedAttention
+from voiceagent_amd.layers.context import attention_context
+
+pytestmark = pytest.mark.gpu
+
+
+def run(dev, lens, done, *, block=16, requests=None, width=None, rows=True, padded=0, table_width=None,
+        alloc=False, lack=0, wide=False, extra=3, seed=0, max_tokens=None):
+    rng = random.Random(seed)
+    size = len(lens)
+    requests = size + 3 if requests is None else requests
+    width = max([-(-max(0, n) // block) for n in lens] + [1]) if width is None else width
+    ids = list(range(requests * width + 50))
+    rng.shuffle(ids)
+    tables = [[ids.pop() for _ in range(width)] for _ in range(requests)]
+    row = rng.sample(range(requests), size) if rows is True else rows
+    free = count = None
+    if alloc:
+        need = sum(-(-max(0, n) // block) for n in lens)
+        free = [1000 + i for i in range(need + 20)]
+        rng.shuffle(free)
+        count = max(0, need + 5 - lack)
+    index = torch.int64 if wide else torch.int32
+    t = torch.tensor(tables, dtype=torch.int32, device=dev).reshape(requests, width)
+    total = sum(max(0, n) - min(max(0, c), max(0, n)) for n, c in zip(lens, done)) + max(0, padded - size)
+    max_tokens = total + extra if max_tokens is None else max_tokens
+    vec = lambda v, d=torch.int32: torch.tensor(v, dtype=d, device=dev)  # noqa: E731
+    m = ops.batch_metadata(vec(lens, index), vec(done, index), t, block, max_tokens=max_tokens,
+                           rows=None if row is None else vec(row), padded_batch=padded,
+                           table_width=table_width, free_blocks=None if free is None else vec(free),
+                           free_count=None if free is None else vec([count]))
+    want = oracle.batch_metadata(lens, done, tables, block, max_tokens=max_tokens, rows=row, padded=padded,
+                                 width=table_width, free=free, count=count)
+    assert m.positions.tolist() == want["positions"]
+    assert m.slot_mapping.tolist() == want["slots"]
+    assert m.cu_seqlens_q.tolist() == want["cu_q"] and m.cu_seqlens_k.tolist() == want["cu_k"]
+    assert m.block_tables.tolist() == want["tables"]
+    assert m.totals.tolist() == want["totals"]
+    assert t.tolist() == want["request_tables"]
+    return m
+
+
+@pytest.mark.parametrize("wide", [False, True])
+@pytest.mark.parametrize("block", [1, 16, 24])
+@pytest.mark.parametrize("alloc", [False, True])
+def test_small_batches(dev, wide, block, alloc):
+    run(dev, [1], [0], wide=wide, block=block, alloc=alloc)
+    run(dev, [17, 0, 16, 33, 5, 100], [16, 0, 16, 0, 5, 1], wide=wide, block=block, alloc=alloc)
+    run(dev, [40, 7, 64], [39, 6, 63], padded=8, wide=wide, block=block, alloc=alloc, table_width=70)
+
+
+def test_no_requests(dev):
+    run(dev, [], [], requests=2, width=3)
+    run(dev, [], [], requests=2, width=3, padded=4)
+
+
+@pytest.mark.parametrize("size, hi", [(3, 9000), (250, 90), (1025, 20), (5000, 3), (2100, 40)])
+def test_large_batches(dev, size, hi):
+    rng = random.Random(size)
+    lens = [rng.randint(0, hi) for _ in range(size)]
+    done = [rng.choice([0, n, rng.randint(0, n), max(0, n - 1)]) for n in lens]
+    run(dev, lens, done, alloc=True, seed=size)
+    run(dev, lens, done, seed=size + 1, padded=size + 7)
+
+
+def test_the_free_list_runs_out(dev):
+    for lack in (1, 6, 9, 1000):
+        m = run(dev, [50, 40, 33], [10, 0, 32], alloc=True, lack=lack, seed=lack)
+    assert m.totals.tolist()[3] == 0 and m.free_count.item() == 0
+
+
+def test_bad_lengths_rows_and_narrow_tables(dev):
+    run(dev, [-5, 20, 30, 10], [0, -3, 99, 4], seed=1)
+    run(dev, [20, 30, 40], [0, 10, 0], rows=[7, -1, 1], requests=4, width=3, seed=2)
+    run(dev, [20, 90, 40], [0, 10, 39], requests=5, width=2, alloc=True, seed=3)
+    run(dev, [20, 90, 40], [0, 10, 39], table_width=1, seed=4)
+    run(dev, [20, 90, 40], [0, 10, 39], max_tokens=50, seed=5)
+    run(dev, [20, 90, 40], [0, 10, 39], max_tokens=0, seed=6)
+    run(dev, [20, 30], [4, 0], rows=None, seed=7)
+
+
+class Seq:
+    def __init__(self, n, done, table):
+        self.n, self.num_computed_tokens, self.block_table = n, done, table
+
+    def __len__(self):
+        return self.n
+
+
+def test_same_as_the_host_builders(dev):
+    rng = random.Random(4)
+    lens = [rng.randint(1, 200) for _ in range(30)]
+    done = [rng.randint(0, n - 1) for n in lens]
+    ids = list(range(1000))
+    rng.shuffle(ids)
+    tables = [[ids.pop() for _ in range(-(-n // 16))] for n in lens]
+    width = max(map(len, tables))
+    t = torch.tensor([x + [-1] * (width - len(x)) for x in tables], dtype=torch.int32, device=dev)
+    seqs = [Seq(*x) for x in zip(lens, done, tables)]
+    positions, ctx = prepare_batch(seqs, 16, dev)
+    vec = lambda v: torch.tensor(v, dtype=torch.int32, device=dev)  # noqa: E731
+    p2, c2, meta = prepare_batch_device(vec(lens), vec(done), t, 16, max_tokens=positions.numel(),
+                                        max_seqlen_q=ctx.max_seqlen_q, max_seqlen_k=ctx.max_seqlen_k,
+                                        max_seqlen_k_exact=True)
+    assert torch.equal(positions, p2)
+    for name in ("cu_seqlens_q", "cu_seqlens_k", "slot_mapping", "block_tables"):
+        assert torch.equal(getattr(ctx, name), getattr(c2, name)), name
+    assert meta.totals[:3].tolist() == [positions.numel(), ctx.max_seqlen_q, ctx.max_seqlen_k]
+
+    host, device = (DecodeGraphMetadata(64, 20, 16, 320, dev, buckets=[8, 32, 64]) for _ in range(2))
+    assert host.stage(seqs) == 32
+    assert device.stage_device(vec(lens), vec([n - 1 for n in lens]), t)[0] == 32
+    for name in ("positions", "slot_mapping", "cu_seqlens_k", "cu_seqlens_q"):
+        assert torch.equal(getattr(host, name), getattr(device, name)), name
+    live = torch.arange(20, device=dev) < torch.tensor([len(x) for x in tables], device=dev)[:, None]
+    assert torch.equal(host.block_tables[:30][live], device.block_tables[:30][live])
+    assert not device.block_tables[30:32].any()
+
+
+def test_captured_and_replayed(dev):
+    table = torch.randperm(64, device=dev).int().view(4, 16)
+    lens, done = (torch.tensor(v, dtype=torch.int32, device=dev) for v in ([20, 3, 40], [0, 0, 39]))
+    free = torch.arange(100, 200, dtype=torch.int32, device=dev)
+    count = torch.tensor([100], dtype=torch.int32, device=dev)
+    kw = {"max_tokens": 64, "padded_batch": 5, "free_blocks": free, "free_count": count}
+    out = ops.batch_metadata(lens, done, table.clone(), 16, **kw)
+    mine = table.clone()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        ops.batch_metadata(lens, done, mine, 16, out=out, **kw)
+    for step in range(3):
+        lens.copy_(torch.tensor([20 + step, 3 + 16 * step, 40]))
+        done.copy_(torch.tensor([step, step, 39 - step]))
+        count.fill_(100 - step)
+        other = mine.clone()
+        g.replay()
+        torch.cuda.synchronize()
+        want = ops.batch_metadata(lens, done, other, 16, **kw)
+        for name in ("positions", "slot_mapping", "cu_seqlens_q", "cu_seqlens_k", "block_tables", "totals"):
+            assert torch.equal(getattr(out, name), getattr(want, name)), name
+        assert torch.equal(mine, other)
+
+
+@pytest.mark.parametrize("layout", ["nhd", "hnd"])
+def test_serving_over_an_mxfp4_pool(dev, layout):
+    """Prompts in two chunks, then decode steps, blocks off the free list: the
+    layer over a 4-bit pool against float64 attention over the same stored rows."""
+    hq, hkv, d, block, blocks, limit = 8, 2, 128, 16, 64, 12
+    gen = torch.Generator().manual_seed(1)
+    k, v, ks, vs = ops.mxfp4_kv_pool(blocks, block, hkv, d, device=dev, layout=layout)
+    layer = PagedAttention(hq, d, d ** -0.5, hkv)
+    layer.kv_layout, layer.k_cache, layer.v_cache, layer.k_scale, layer.v_scale = layout, k, v, ks, vs
+    tables = torch.full((5, limit), -1, dtype=torch.int32, device=dev)
+    free = torch.randperm(blocks, generator=gen).int().to(dev)
+    count = torch.tensor([blocks], dtype=torch.int32, device=dev)
+    rows = torch.tensor([3, 0, 4], dtype=torch.int32, device=dev)
+    final = [70, 33, 101]
+    x = [torch.randn(n + 6, hq + 2 * hkv, d, generator=gen).to(torch.bfloat16) for n in final]
+    done = [0, 0, 0]
+    for new in ([40, 33, 64], [30, 1, 37]) + ([1, 1, 1],) * 4:
+        lens = [a + b for a, b in zip(done, new)]
+        vec = lambda z: torch.tensor(z, dtype=torch.int32, device=dev)  # noqa: E731
+        _, ctx, meta = prepare_batch_device(vec(lens), vec(done), tables, block, max_tokens=sum(new),
+                                            max_seqlen_q=max(new), max_seqlen_k=max(lens), rows=rows,
+                                            free_blocks=free, free_count=count)
+        count = meta.free_count
+        qkv = torch.cat([t[a:b] for t, a, b in zip(x, done, lens)])
+        gpu = qkv.to(dev)
+        with attention_context(ctx):
+            out = layer(gpu[:, :hq], gpu[:, hq:hq + hkv], gpu[:, hq + hkv:])
+        at = 0
+        for t, a, b in zip(x, done, lens):
+            q, kk, vv = t[a:b, :hq], t[:b, hq:hq + hkv], t[:b, hq + hkv:]
+            kq, vq = (oracle.values(*oracle.quantise(z)) for z in (kk, vv))
+            if new != [1, 1, 1]:  # a chunk's own rows are attended as given, a decode's as stored
+                kq[a:], vq[a:] = kk[a:].double(), vv[a:].double()
+            seen = torch.arange(b) <= torch.arange(a, b)[:, None]
+            ref, tol = oracle.attend(q, kq, vq, seen, d ** -0.5, torch.bfloat16, 13)
+            bad = (out[at:at + b - a].double().cpu() - ref).abs() > tol
+            assert not bad.any()
+            at += b - a
+        done = lens
+    assert meta.totals[4].item() == 0
+    assert count.item() == blocks - sum(-(-n // block) for n in done)

@@ -1,0 +1,428 @@
+"""MXFP4 KV pools on the GPU: store, load, paged decode and varlen attention
+against the float64 oracle (oracle/mx4.py), which also bounds the rounding."""
+
+import math
+
+import pytest
+import torch
+
+from oracle import mx4 as oracle
+from tests.mx4_common import Pool, close, cu, slots_of, tables_for
+from voiceagent_amd import ops
+
+pytestmark = pytest.mark.gpu
+
+BF16, F16 = torch.bfloat16, torch.float16
+# The decode's Q K^T runs on scaled matrix products, which align neighbouring
+# products to 13 bits before adding; the varlen kernel's on 16-bit ones.
+DECODE_BITS, VARLEN_BITS = 13, 17
+
+
+# ------------------------------------------------------------- store and load
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("hkv, d, block, layout, wide, n", [
+    (8, 128, 16, "nhd", False, 37), (8, 128, 16, "hnd", True, 700), (1, 64, 32, "nhd", False, 1),
+    (3, 256, 16, "hnd", False, 9), (2, 96, 7, "nhd", True, 50), (5, 32, 1, "hnd", False, 11)])
+def test_store_and_load_are_exact(dev, dtype, hkv, d, block, layout, wide, n):
+    gen = torch.Generator().manual_seed(n + d)
+    blocks = -(-n // block) + 3
+    pool = Pool(gen, blocks, block, hkv, d, layout, dtype, dev)
+    key = (torch.randn(n, hkv, d, generator=gen) * torch.exp(4 * torch.randn(n, hkv, 1, generator=gen))).to(dtype)
+    # Rows strided as a view of a fused projection.
+    value = torch.randn(n, hkv + 2, d, generator=gen).to(dtype)[:, 1:-1]
+    # The format's corners: ties, limits, subnormals, infinities, NaN.
+    special = torch.tensor([6.0, 0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0, -0.0, -0.25, 7.0, -7.0])
+    key[0, 0, :12] = special.to(dtype)
+    value[0, 0, :12] = (special * 2.0 ** -13).to(dtype)
+    tiny, most = torch.finfo(dtype).tiny, torch.finfo(dtype).max
+    if n > 8:
+        key[1, 0, :3] = torch.tensor([tiny / 4, tiny, -tiny / 2]).to(dtype)
+        key[1, 0, 3:] = 0
+        key[2] = 0
+        key[3, 0, 5] = math.inf
+        value[4, 0, 7] = math.nan
+        value[5, 0, :4] = torch.tensor([most, -most, most / 2, 1.0]).to(dtype)
+        key[6, 0, 1] = -math.inf
+    slots = torch.randperm(blocks * block, generator=gen)[:n].to(torch.int64 if wide else torch.int32)
+    if n > 8:
+        slots[7], slots[8] = -1, blocks * block  # padding, past the pool
+    (kc, vc), kw = pool.args()
+    gpu_value = value.to(dev)
+    fused = torch.zeros(n, hkv + 2, d, dtype=dtype, device=dev)
+    fused[:, 1:-1] = gpu_value
+    ops.store_kvcache(key.to(dev), fused[:, 1:-1], kc, vc, slots.to(dev), **kw)
+    oracle.store(key, value, pool.cpu, slots, block, layout)
+    assert pool.same()
+    k, v = ops.load_kvcache(kc, vc, slots.to(dev), dtype, **kw)
+    ok = (slots >= 0) & (slots < blocks * block)
+    ek, ev = pool.rows(slots.long().clamp(0, blocks * block - 1))
+    for got, want in ((k, ek), (v, ev)):
+        want[~ok] = 0
+        assert torch.equal(got.double().cpu().nan_to_num(nan=12345.0), want.nan_to_num(nan=12345.0))
+    assert pool.same()
+
+
+def test_store_of_nothing(dev):
+    gen = torch.Generator().manual_seed(0)
+    pool = Pool(gen, 2, 16, 2, 64, "nhd", BF16, dev)
+    (kc, vc), kw = pool.args()
+    x = torch.zeros(0, 2, 64, dtype=BF16, device=dev)
+    slots = torch.zeros(0, dtype=torch.int32, device=dev)
+    ops.store_kvcache(x, x, kc, vc, slots, **kw)
+    assert ops.load_kvcache(kc, vc, slots, **kw)[0].shape == (0, 2, 64)
+    assert pool.same()
+
+
+# --------------------------------------------------------------------- decode
+def run_decode(dev, lens, *, hq=16, hkv=8, d=128, block=16, layout="nhd", dtype=BF16, seed=0,
+               cumulative=True, table_dtype=torch.int32, split=0, bound=None, new=False, slots=None,
+               mask=None, key_limit=0, table_read_width=0, pad=-1, edit=None, scale=None):
+    gen = torch.Generator().manual_seed(seed)
+    B = len(lens)
+    blocks = sum(-(-n // block) for n in lens) + 5
+    pool = Pool(gen, blocks, block, hkv, d, layout, dtype, dev)
+    tables = tables_for(gen, lens, block, blocks, table_dtype, pad, extra=1)
+    if edit:
+        edit(pool, tables)
+        pool.gpu = [t.to(dev) for t in pool.cpu]
+    q = torch.randn(B, hq + 1, d, generator=gen).to(dtype)[:, :hq]
+    more = {}
+    if new:
+        nk = torch.randn(B, hkv, 2 * d, generator=gen).to(dtype)
+        nv = (torch.randn(B, hkv, d, generator=gen) * 3).to(dtype)
+        more = {"new_k": nk.to(dev)[..., :d], "new_v": nv.to(dev)}
+        if slots is not None:
+            more["new_slots"] = slots.to(dev)
+    if mask is not None:
+        more["valid_mask"] = mask.to(dev)
+    (kc, vc), kw = pool.args()
+    scale = d ** -0.5 if scale is None else scale
+    vec = cu(lens) if cumulative else torch.tensor(lens, dtype=torch.int64)
+    out = ops.paged_decode(q.to(dev), kc, vc, tables.to(dev), vec.to(dev), lens_cumulative=cumulative,
+                           max_seq_len=max(lens) if bound is None else bound, scale=scale,
+                           split_tokens=split, key_limit=key_limit,
+                           table_read_width=table_read_width, **more, **kw)
+    torch.cuda.synchronize()
+    # The oracle: the current row first, then one sequence at a time.
+    capacity = blocks * block
+    width = tables.shape[1]
+    read_width = min(table_read_width, width) if table_read_width else width
+    for b, n in enumerate(lens):
+        if not new or n < 1:
+            continue
+        col = (n - 1) // block
+        if slots is not None:
+            at = int(slots[b])
+        else:
+            blk = int(tables[b, col]) if col < width else 0
+            at = blk * block + (n - 1) % block if 0 <= blk < blocks else -1
+        if 0 <= at < capacity:
+            oracle.store(nk[b:b + 1, :, :d], nv[b:b + 1], pool.cpu, torch.tensor([at]), block, layout)
+    for b, n in enumerate(lens):
+        m = min(n, key_limit) if key_limit else n
+        if m <= 0:
+            assert not out[b].any()
+            continue
+        pos = torch.arange(m)
+        col = pos // block
+        blk = torch.where(col < read_width, tables[b].long()[col.clamp(max=width - 1)], 0)
+        seen = (blk >= 0) & (blk < blocks)
+        if mask is not None:
+            seen &= torch.where(pos < mask.shape[1], mask[b][pos.clamp(max=mask.shape[1] - 1)], True)
+        k, v = pool.rows(blk.clamp(0, blocks - 1) * block + pos % block)
+        if new and m == n and (slots is None or 0 <= int(slots[b]) < capacity) and \
+                ((n - 1) // block < read_width or slots is not None or (n - 1) // block >= width):
+            kq, ks = oracle.quantise(nk[b, :, :d])
+            vq, vs = oracle.quantise(nv[b])
+            k[-1], v[-1] = oracle.values(kq, ks), oracle.values(vq, vs)
+        ref, tol = oracle.attend(q[b:b + 1], k, v, seen[None], scale, dtype, DECODE_BITS)
+        close(out[b:b + 1], ref, tol)
+    assert pool.same()
+    return out
+
+
+LENS = [1, 2, 15, 16, 17, 31, 32, 33, 63, 100, 257, 600]
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("hq, hkv, d", [(16, 8, 128), (8, 8, 128), (8, 2, 64), (16, 2, 128), (4, 2, 256),
+                                        (8, 1, 256), (14, 14, 64)])
+@pytest.mark.parametrize("layout, block", [("nhd", 16), ("hnd", 16), ("nhd", 48)])
+def test_decode(dev, dtype, hq, hkv, d, layout, block):
+    run_decode(dev, LENS, hq=hq, hkv=hkv, d=d, dtype=dtype, layout=layout, block=block, seed=hq + d)
+
+
+@pytest.mark.parametrize("dtype, d", [(BF16, 128), (F16, 64), (BF16, 256)])
+@pytest.mark.parametrize("split, bound", [(0, None), (0, 32768), (ops.SPLIT_EXACT, None), (1, None), (700, None)])
+def test_decode_splits(dev, dtype, d, split, bound):
+    run_decode(dev, [4099, 1, 2050], hq=8, hkv=2, d=d, dtype=dtype, split=split, bound=bound, seed=5)
+
+
+def test_decode_many_steps_a_wave(dev):
+    # One partition: more than 64 steps for every wave (their block ids are read 32 steps at a time).
+    run_decode(dev, [17000, 8300], hq=2, hkv=1, split=1 << 20, seed=6)
+
+
+@pytest.mark.parametrize("new", [False, True])
+@pytest.mark.parametrize("cumulative, table_dtype", [(False, torch.int64), (True, torch.int64)])
+def test_decode_index_types(dev, new, cumulative, table_dtype):
+    run_decode(dev, [5, 40, 300, 0, 16], cumulative=cumulative, table_dtype=table_dtype, new=new, seed=7)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("hq, hkv, d, layout", [(16, 8, 128, "nhd"), (4, 1, 64, "hnd"), (4, 2, 256, "nhd")])
+@pytest.mark.parametrize("split", [0, 256])
+def test_decode_current_row(dev, dtype, hq, hkv, d, layout, split):
+    run_decode(dev, [1, 16, 17, 32, 33, 255, 900], hq=hq, hkv=hkv, d=d, layout=layout, dtype=dtype,
+               new=True, split=split, seed=8)
+
+
+def test_decode_current_row_slots(dev):
+    # Slots other than the position's own, none, and past the pool.
+    lens = [40, 33, 17, 1, 64]
+    blocks = sum(-(-n // 16) for n in lens) + 5
+    for values in ([-1] * 5, [blocks * 16, -1, -1, blocks * 16 + 5, -7]):
+        run_decode(dev, lens, new=True, slots=torch.tensor(values, dtype=torch.int64), seed=10)
+
+
+def test_decode_key_limit_and_read_width(dev):
+    lens = [200, 40, 16, 100]
+    run_decode(dev, lens, key_limit=50, seed=11)
+    run_decode(dev, lens, key_limit=50, new=True, seed=12)
+    run_decode(dev, lens, table_read_width=3, seed=13)
+    run_decode(dev, lens, table_read_width=3, new=True, seed=14)
+
+
+@pytest.mark.parametrize("split", [0, 256])
+def test_decode_mask(dev, split):
+    lens = [300, 40, 17, 1, 600]
+    gen = torch.Generator().manual_seed(15)
+    mask = torch.rand(5, 333, generator=gen) < 0.5  # narrower than a context: the rest is valid
+    mask[1] = False  # a row with nothing left
+    mask[0, :290] = False
+    run_decode(dev, lens, mask=mask, split=split, seed=16)
+    run_decode(dev, lens, mask=mask, new=True, split=split, seed=17, layout="hnd", dtype=F16)
+    run_decode(dev, lens, mask=mask[:, 1:], seed=18, hq=4, hkv=1, d=64)
+
+
+def test_decode_dead_places_hold_anything(dev):
+    # NaN groups, huge scales and garbage where a mask, the context's end or a
+    # missing block says that nothing is attended.
+    lens = [40, 70, 20]
+    mask = torch.ones(3, 80, dtype=torch.bool)
+    mask[0, 3:9] = False
+    mask[1, 64:] = False
+
+    def edit(pool, tables):
+        live = torch.zeros(pool.cpu[0].shape[0] * 16, dtype=torch.bool)
+        for b, n in enumerate(lens):
+            at = slots_of(tables[b], n, 16)
+            live[at[mask[b, :n]]] = True
+        live[slots_of(tables[2], 20, 16)[16:]] = False
+        for t in (2, 3):
+            pool.cpu[t].flatten(0, 1)[~live] = 255
+        for t in (0, 1):
+            pool.cpu[t].flatten(0, 1)[~live] = 0x7f
+        tables[2, 1] = 10 ** 6  # a block outside the pool
+
+    out = run_decode(dev, lens, mask=mask, edit=edit, seed=19)
+    assert out.isfinite().all()
+
+
+def test_decode_nan_reaches_its_own_sequence_only(dev):
+    gen = torch.Generator().manual_seed(20)
+    pool = Pool(gen, 8, 16, 2, 128, "nhd", BF16, dev)
+    tables = torch.tensor([[0, 1], [2, 3], [4, 5]], dtype=torch.int32)
+    pool.gpu[3][0, 3, 1, 2] = 255  # V, sequence 0, head 1, elements 64 .. 95
+    pool.gpu[2][2, 3, 0, 1] = 255  # K, sequence 1, head 0
+    (kc, vc), kw = pool.args()
+    q = torch.randn(3, 4, 128, generator=gen).to(BF16)
+    q[2, 3, 7] = math.inf
+    out = ops.paged_decode(q.to(dev), kc, vc, tables.to(dev), torch.tensor([20, 20, 20], device=dev),
+                           max_seq_len=20, scale=0.1, **kw).cpu()
+    assert out[0, 2:, 64:96].isnan().all() and out[0, 2:, :64].isfinite().all() and out[0, :2].isfinite().all()
+    assert out[1, :2].isnan().all() and out[1, 2:].isfinite().all()
+    assert out[2, 3].isnan().all() and out[2, :3].isfinite().all()
+
+
+@pytest.mark.parametrize("d, hq, hkv, dtype", [(128, 16, 8, BF16), (64, 8, 2, F16), (256, 8, 1, BF16)])
+@pytest.mark.parametrize("split", [0, 256])
+def test_decode_prologue_is_the_standalone_one(dev, d, hq, hkv, dtype, split):
+    lens = [1, 17, 300, 700]
+    gen = torch.Generator().manual_seed(21)
+    blocks = sum(-(-n // 16) for n in lens)
+    one, two = (Pool(torch.Generator().manual_seed(3), blocks, 16, hkv, d, "nhd", dtype, dev) for _ in range(2))
+    tables = tables_for(gen, lens, 16, blocks).to(dev)
+    q, k, v = (torch.randn(4, n, d, generator=gen).to(dtype).to(dev) for n in (hq, hkv, hkv))
+    pro = ops.QKPrologue(torch.rand(d, generator=gen).to(dtype).to(dev), torch.rand(d, generator=gen).to(dtype).to(dev),
+                         1e-6, torch.randn(800, d, generator=gen).to(dev),
+                         torch.tensor([n - 1 for n in lens], device=dev))
+    kw = {"max_seq_len": 700, "scale": d ** -0.5, "split_tokens": split}
+    vec = torch.tensor(lens, device=dev)
+    (kc, vc), more = one.args()
+    got = ops.paged_decode(q, kc, vc, tables, vec, new_k=k, new_v=v, prologue=pro, **kw, **more)
+    qn, kn = ops.qk_norm_rope(q, k, pro)
+    (kc, vc), more = two.args()
+    want = ops.paged_decode(qn, kc, vc, tables, vec, new_k=kn, new_v=v, **kw, **more)
+    assert torch.equal(got, want)
+    assert all(torch.equal(a, b) for a, b in zip(one.gpu, two.gpu))
+
+
+def test_decode_pool_past_4_gib(dev):
+    # Codes and scales of one pool past 2^32 bytes: blocks at its far end.
+    blocks, hkv, d = 540000, 8, 128
+    codes = torch.empty(2, blocks, 16, hkv, d // 2, dtype=torch.uint8, device=dev)
+    scales = torch.empty(2, blocks, 16, hkv, d // 32, dtype=torch.uint8, device=dev)
+    gen = torch.Generator().manual_seed(22)
+    small = Pool(gen, 6, 16, hkv, d, "nhd", BF16, dev)
+    at = torch.tensor([blocks - 1, 3, blocks - 7, 530000, 0, blocks - 2], device=dev)
+    for i in range(2):
+        codes[i, at], scales[i, at] = small.gpu[i], small.gpu[2 + i]
+    q = torch.randn(2, 16, d, generator=gen).to(BF16).to(dev)
+    near = torch.tensor([[0, 1, 2], [3, 4, 5]], dtype=torch.int32, device=dev)
+    (kc, vc), kw = small.args()
+    lens = torch.tensor([48, 41], device=dev)
+    want = ops.paged_decode(q, kc, vc, near, lens, max_seq_len=48, scale=0.1, **kw)
+    far = {"k_scale": scales[0].view(ops.MXFP4_SCALE_DTYPE), "v_scale": scales[1].view(ops.MXFP4_SCALE_DTYPE)}
+    big = (codes[0].view(ops.MXFP4_KV_DTYPE), codes[1].view(ops.MXFP4_KV_DTYPE))
+    got = ops.paged_decode(q, *big, at[near.long()].int(), lens, max_seq_len=48, scale=0.1, **far)
+    assert torch.equal(got, want)
+    cq = torch.tensor([0, 16, 25], dtype=torch.int32, device=dev)
+    ck = torch.tensor([0, 48, 89], dtype=torch.int32, device=dev)
+    qp = torch.randn(25, 16, d, generator=gen).to(BF16).to(dev)
+    a = ops.varlen_attention(qp, None, None, cq, ck, 16, 48, scale=0.1, causal=True, k_cache=big[0],
+                             v_cache=big[1], block_tables=at[near.long()].int(), **far)
+    b = ops.varlen_attention(qp, None, None, cq, ck, 16, 48, scale=0.1, causal=True, k_cache=kc, v_cache=vc,
+                             block_tables=near, **kw)
+    assert torch.equal(a, b)
+    # (stored last: these slots lie in blocks that the calls above read)
+    rows = torch.randn(3, hkv, d, generator=gen).to(BF16).to(dev)
+    slots = torch.tensor([blocks * 16 - 1, 5, blocks * 16 - 20], dtype=torch.int64, device=dev)
+    ops.store_kvcache(rows, rows, *big, slots, **far)
+    k, v = ops.load_kvcache(*big, slots, BF16, **far)
+    c, s = oracle.quantise(rows.cpu())
+    assert torch.equal(k.double().cpu(), oracle.values(c, s)) and torch.equal(k, v)
+
+
+def test_decode_on_a_side_stream_and_captured(dev):
+    gen = torch.Generator().manual_seed(23)
+    lens = [3000, 17, 900, 1]
+    blocks = sum(-(-n // 16) for n in lens) + 2
+    pool = Pool(gen, blocks, 16, 2, 128, "nhd", BF16, dev)
+    (kc, vc), kw = pool.args()
+    tables = tables_for(gen, lens, 16, blocks).to(dev)
+    vec = torch.tensor(lens, device=dev)
+    q = torch.randn(4, 8, 128, generator=gen).to(BF16).to(dev)
+    nk, nv = (torch.randn(4, 2, 128, generator=gen).to(BF16).to(dev) for _ in range(2))
+
+    def call(out=None):
+        return ops.paged_decode(q, kc, vc, tables, vec, max_seq_len=32768, scale=0.1, new_k=nk, new_v=nv,
+                                out=out, **kw)
+
+    want = call()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = call()
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(got, want)
+    outs = [torch.empty_like(q) for _ in range(2)]
+    graphs = []
+    for out in outs:  # two graphs, which share the capture stream's workspace
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            call(out)
+        graphs.append(g)
+    for i in range(3):
+        q.copy_(torch.randn(4, 8, 128, generator=gen).to(BF16))
+        nk.copy_(torch.randn(4, 2, 128, generator=gen).to(BF16))
+        vec.copy_(torch.tensor([3000 - 7 * i, 17, 900 - i, 1 + i]))
+        for out in outs:
+            out.fill_(7)
+        for g in graphs:
+            g.replay()
+        torch.cuda.synchronize()
+        got = [o.clone() for o in outs]
+        want = call()
+        assert torch.equal(got[0], want) and torch.equal(got[1], want)
+
+
+# --------------------------------------------------------------------- varlen
+def run_varlen(dev, prefixes, qlens, *, hq=16, hkv=8, d=128, block=16, layout="nhd", dtype=BF16, seed=0,
+               causal=True, fresh=True, table_dtype=torch.int32, tail=0, edit=None):
+    gen = torch.Generator().manual_seed(seed)
+    klens = [p + m for p, m in zip(prefixes, qlens)]
+    total = sum(qlens) + tail  # rows behind the last sequence
+    blocks = sum(-(-n // block) for n in klens) + 3
+    pool = Pool(gen, blocks, block, hkv, d, layout, dtype, dev)
+    tables = tables_for(gen, klens, block, blocks, table_dtype)
+    if edit:
+        edit(pool, tables)
+        pool.gpu = [t.to(dev) for t in pool.cpu]
+    qkv = torch.randn(total, hq + 2 * hkv, d, generator=gen).to(dtype)
+    q, k, v = qkv[:, :hq], qkv[:, hq:hq + hkv], qkv[:, hq + hkv:]
+    slots = torch.full((total,), -1, dtype=table_dtype)
+    at = 0
+    for b, (p, m) in enumerate(zip(prefixes, qlens)):
+        slots[at:at + m] = slots_of(tables[b], p + m, block)[p:].to(table_dtype)
+        at += m
+    (kc, vc), kw = pool.args()
+    gpu = qkv.to(dev)
+    out = torch.full((total, hq, d), 5.0, dtype=dtype, device=dev)
+    ops.varlen_attention(gpu[:, :hq], gpu[:, hq:hq + hkv] if fresh else None,
+                         gpu[:, hq + hkv:] if fresh else None, cu(qlens).to(dev), cu(klens).to(dev),
+                         max(qlens), max(klens), scale=d ** -0.5, causal=causal, k_cache=kc, v_cache=vc,
+                         block_tables=tables.to(dev), slot_mapping=slots.to(dev) if fresh else None,
+                         out=out, **kw)
+    torch.cuda.synchronize()
+    at = 0
+    for b, (p, m, n) in enumerate(zip(prefixes, qlens, klens)):
+        if m == 0:
+            continue
+        pos = torch.arange(n)
+        blk = tables[b].long()[pos // block]
+        ok = (blk >= 0) & (blk < blocks)
+        kk, vv = pool.rows(blk.clamp(0, blocks - 1) * block + pos % block)
+        kk[~ok], vv[~ok] = 0, 0  # rows of a block outside the pool read as zeros
+        if fresh:
+            kk[p:], vv[p:] = k[at:at + m].double(), v[at:at + m].double()
+        seen = pos <= torch.arange(p, n)[:, None] if causal else torch.ones(m, n, dtype=torch.bool)
+        ref, tol = oracle.attend(q[at:at + m], kk, vv, seen, d ** -0.5, dtype, VARLEN_BITS)
+        close(out[at:at + m], ref, tol)
+        at += m
+    assert (out[at:] == 5.0).all()
+    if fresh:
+        oracle.store(k, v, pool.cpu, slots, block, layout)
+    assert pool.same()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("hq, hkv, d", [(16, 8, 128), (8, 1, 128), (4, 4, 64), (8, 2, 64)])
+@pytest.mark.parametrize("layout, block", [("nhd", 16), ("hnd", 48)])
+def test_varlen(dev, dtype, hq, hkv, d, layout, block):
+    run_varlen(dev, [0, 1, 16, 63, 64, 100, 257, 40], [5, 1, 17, 64, 1, 70, 130, 0], hq=hq, hkv=hkv, d=d,
+               dtype=dtype, layout=layout, block=block, seed=d + hq, tail=3)
+
+
+@pytest.mark.parametrize("d, hq, hkv", [(128, 16, 8), (64, 8, 1), (128, 4, 4)])
+@pytest.mark.parametrize("prefixes, qlens", [([5000], [40]), ([3000, 10, 700], [20, 300, 1]),
+                                             ([0, 0], [333, 20]), ([2048] * 3, [1, 1, 1])])
+def test_varlen_long_prefixes(dev, d, hq, hkv, prefixes, qlens):
+    run_varlen(dev, prefixes, qlens, hq=hq, hkv=hkv, d=d, seed=len(prefixes))
+
+
+@pytest.mark.parametrize("causal", [True, False])
+def test_varlen_all_from_the_pool(dev, causal):
+    run_varlen(dev, [0, 30, 200], [20, 3, 100], fresh=False, causal=causal, seed=2, table_dtype=torch.int64)
+
+
+def test_varlen_not_causal(dev):
+    run_varlen(dev, [0, 100, 64], [70, 30, 64], causal=False, seed=3)
+
+
+def test_varlen_blocks_outside_the_pool(dev):
+    def edit(pool, tables):
+        tables[0, 2] = -1
+        tables[1, 0] = 10 ** 6
+
+    run_varlen(dev, [150, 90], [40, 10], edit=edit, seed=4)

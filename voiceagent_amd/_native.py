@@ -20,7 +20,7 @@ VA_OK = 0
 VA_BF16, VA_F16, VA_F32 = 0, 1, 2
 VA_I32, VA_I64 = 0, 1
 VA_LENS_PER_SEQ, VA_LENS_CUMULATIVE = 0, 1
-VA_KV_NATIVE, VA_KV_FP8_E4M3 = 0, 1
+VA_KV_NATIVE, VA_KV_FP8_E4M3, VA_KV_MXFP4 = 0, 1, 2
 ABI_VERSION = 7  # VA_ATTN_ABI_VERSION of the header these structs mirror
 DECODE_NOALLOC_SCRATCH_BYTES = 4 << 20  # VA_DECODE_NOALLOC_SCRATCH_BYTES
 VA_SPLIT_EXACT = -1  # split_tokens: automatic split, max_seq_len exact
@@ -193,6 +193,50 @@ class VarlenArgs(ctypes.Structure):
     ]
 
 
+class Mx4Scales(ctypes.Structure):
+    _fields_ = [
+        ("struct_size", c_uint32),
+        ("k", c_void_p),
+        ("v", c_void_p),
+        ("stride_block", c_int64),
+        ("stride_slot", c_int64),
+        ("stride_head", c_int64),
+    ]
+
+
+class LoadArgs(ctypes.Structure):
+    _fields_ = list(StoreArgs._fields_)
+
+
+class BatchArgs(ctypes.Structure):
+    _fields_ = [
+        ("struct_size", c_uint32),
+        ("index_dtype", c_int32),
+        ("lens", c_void_p),
+        ("num_computed", c_void_p),
+        ("request_tables", c_void_p),
+        ("request_stride", c_int64),
+        ("num_requests", c_int32),
+        ("request_width", c_int32),
+        ("rows", c_void_p),
+        ("num_seqs", c_int32),
+        ("padded_seqs", c_int32),
+        ("block_size", c_int32),
+        ("max_tokens", c_int32),
+        ("positions", c_void_p),
+        ("slot_mapping", c_void_p),
+        ("cu_seqlens_q", c_void_p),
+        ("cu_seqlens_k", c_void_p),
+        ("block_tables", c_void_p),
+        ("table_stride", c_int64),
+        ("table_width", c_int32),
+        ("totals", c_void_p),
+        ("free_blocks", c_void_p),
+        ("free_count", c_void_p),
+        ("free_capacity", c_int32),
+    ]
+
+
 # Every function include/voiceagent_attn.h declares, with its ctypes signature.
 SIGNATURES = {
     "va_store_kvcache": (c_int32, [ctypes.POINTER(StoreArgs), c_void_p]),
@@ -203,6 +247,16 @@ SIGNATURES = {
     "va_varlen_workspace_bytes": (c_size_t, [ctypes.POINTER(VarlenArgs)]),
     "va_varlen_split_workspace_bytes": (c_size_t, [ctypes.POINTER(VarlenArgs)]),
     "va_qk_norm_rope": (c_int32, [ctypes.POINTER(QkNormRopeArgs), c_void_p]),
+    "va_store_kvcache_mx4": (c_int32, [ctypes.POINTER(StoreArgs), ctypes.POINTER(Mx4Scales),
+                                       c_void_p]),
+    "va_load_kvcache_mx4": (c_int32, [ctypes.POINTER(LoadArgs), ctypes.POINTER(Mx4Scales),
+                                      c_void_p]),
+    "va_paged_decode_mx4": (c_int32, [ctypes.POINTER(DecodeArgs), ctypes.POINTER(Mx4Scales),
+                                      c_void_p]),
+    "va_paged_decode_mx4_workspace_bytes": (c_size_t, [ctypes.POINTER(DecodeArgs)]),
+    "va_varlen_attention_mx4": (c_int32, [ctypes.POINTER(VarlenArgs), ctypes.POINTER(Mx4Scales),
+                                          c_void_p]),
+    "va_batch_metadata": (c_int32, [ctypes.POINTER(BatchArgs), c_void_p]),
     "va_last_error": (ctypes.c_char_p, []),
     "va_abi_version": (c_int32, []),
 }

@@ -56,7 +56,7 @@ HIPCC_FLAGS = [
 # back on every tile.
 EXTRA_FLAGS = {
     f"paged_decode_{unit}.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=true"]
-    for unit in ("bf16", "f16", "bf16_f8", "f16_f8")
+    for unit in ("bf16", "f16", "bf16_f8", "f16_f8", "bf16_mx4", "f16_mx4")
 }
 
 

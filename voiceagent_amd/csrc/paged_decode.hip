@@ -1,11 +1,12 @@
 // Host side of the paged decode: argument checks, the context split and
-// launch dispatch (kernels in paged_decode_kernel.h and paged_decode_mfma.h,
-// instantiated per element type in paged_decode_{bf16,f16,f32}.hip).
+// launch dispatch (kernels in paged_decode_kernel.h, paged_decode_mfma.h and
+// paged_decode_mx4.h, instantiated per element type in
+// paged_decode_{bf16,f16,f32}*.hip).
 #include <cstdlib>
 #include <cstring>
 #include <mutex>
 
-#include "paged_decode_mfma.h"
+#include "paged_decode_mx4.h"
 
 namespace va {
 
@@ -95,18 +96,11 @@ static int nosplit_tokens_for(const va_decode_args* a) {
   return per_token > 0 ? (int)(kNoSplitBytes / per_token) : 0;
 }
 
-static DecodePlan plan_decode(const va_decode_args* a) {
+// The split of a launch whose workgroups take `unit` tokens a round, with
+// contexts of up to `nosplit` tokens (at 8 partitions a pair) kept whole.
+static DecodePlan plan_split(const va_decode_args* a, int unit, int64_t nosplit) {
   DecodePlan pl{};
-  if (small_head_decode(a)) {  // one workgroup per (sequence, query head), no split
-    pl.max_parts = 1;
-    pl.split_tokens = a->max_seq_len > 0 ? a->max_seq_len : 1;
-    pl.wg_tokens = pl.split_tokens;
-    return pl;
-  }
   const int G = a->num_kv_heads > 0 ? a->num_heads / a->num_kv_heads : 1;
-  int unit = use_mfma_decode(a) ? mfma_unit_for(a->head_dim)
-                                : decode_unit_for(a->dtype, a->head_dim, G);
-  if (unit <= 0) unit = 128;
   int max_len = a->max_seq_len > 0 ? a->max_seq_len : 1;
   if (a->key_limit > 0 && a->key_limit < max_len) max_len = a->key_limit;
   const bool exact = a->split_tokens == VA_SPLIT_EXACT;
@@ -131,7 +125,7 @@ static DecodePlan plan_decode(const va_decode_args* a) {
     const int64_t cus = current_device_cus();
     const int64_t want = pairs >= cus ? 1 : cus / (pairs > 0 ? pairs : 1);
     int64_t parts = want;
-    if (parts > 1 && (int64_t)max_len * (parts < 8 ? parts : 8) <= (int64_t)nosplit_tokens_for(a) * 8)
+    if (parts > 1 && (int64_t)max_len * (parts < 8 ? parts : 8) <= nosplit * 8)
       parts = 1;
     const int64_t by_len = (max_len + kDynGrain - 1) / kDynGrain;
     if (parts > by_len) parts = by_len;
@@ -181,6 +175,27 @@ static DecodePlan plan_decode(const va_decode_args* a) {
   return pl;
 }
 
+static DecodePlan plan_decode(const va_decode_args* a) {
+  if (small_head_decode(a)) {  // one workgroup per (sequence, query head), no split
+    DecodePlan pl{};
+    pl.max_parts = 1;
+    pl.split_tokens = a->max_seq_len > 0 ? a->max_seq_len : 1;
+    pl.wg_tokens = pl.split_tokens;
+    return pl;
+  }
+  const int G = a->num_kv_heads > 0 ? a->num_heads / a->num_kv_heads : 1;
+  const int unit = use_mfma_decode(a) ? mfma_unit_for(a->head_dim)
+                                      : decode_unit_for(a->dtype, a->head_dim, G);
+  return plan_split(a, unit > 0 ? unit : 128, nosplit_tokens_for(a));
+}
+
+// MXFP4 pools: contexts of up to this many tokens stay whole.
+constexpr int64_t kMx4NoSplitTokens = 1024;
+
+static DecodePlan plan_decode_mx4(const va_decode_args* a) {
+  return plan_split(a, 8 * kMx4Step, kMx4NoSplitTokens);
+}
+
 template <typename ET>
 static int unit_for_d(int D, int G) {
 #define VA_UNIT_G(DD)                                      \
@@ -222,8 +237,10 @@ extern "C" size_t va_paged_decode_workspace_bytes(const va_decode_args* a) {
 
 namespace va {
 
-// The body of va_paged_decode; the workspace comes from the arguments.
-static int paged_decode_impl(const va_decode_args* a, void* stream);
+// The body of va_paged_decode, and with scales of va_paged_decode_mx4; the
+// workspace comes from the arguments.
+static int paged_decode_impl(const va_decode_args* a, const va_mx4_scales* sc, const char* fn,
+                             void* stream);
 
 // ------------------------------------------------- allocation-free variant
 // Scratch memory of va_paged_decode_noalloc: the split-context partials,
@@ -294,99 +311,137 @@ extern "C" int va_paged_decode_noalloc(const va_decode_args* a, void* stream) {
       b.workspace_bytes = kDecodeScratchBytes;
     }
   }
-  return paged_decode_impl(&b, stream);
+  return paged_decode_impl(&b, nullptr, "va_paged_decode", stream);
 }
 
 extern "C" int va_paged_decode(const va_decode_args* a, void* stream) {
-  return va::paged_decode_impl(a, stream);
+  return va::paged_decode_impl(a, nullptr, "va_paged_decode", stream);
 }
 
-int va::paged_decode_impl(const va_decode_args* a, void* stream) {
+extern "C" int va_paged_decode_mx4(const va_decode_args* a, const va_mx4_scales* sc,
+                                   void* stream) {
   using namespace va;
-  VA_CHECK_ARG(a != nullptr, "va_paged_decode: null args");
+  VA_CHECK_ARG(sc != nullptr, "va_paged_decode_mx4: null scales");
+  return paged_decode_impl(a, sc, "va_paged_decode_mx4", stream);
+}
+
+extern "C" size_t va_paged_decode_mx4_workspace_bytes(const va_decode_args* a) {
+  if (a == nullptr || a->struct_size != sizeof(va_decode_args)) return 0;
+  return va::plan_decode_mx4(a).total_bytes;
+}
+
+int va::paged_decode_impl(const va_decode_args* a, const va_mx4_scales* sc, const char* fn,
+                          void* stream) {
+  using namespace va;
+  const bool mx4 = sc != nullptr;
+  VA_CHECK_ARG(a != nullptr, "%s: null args", fn);
   VA_CHECK_ARG(a->struct_size == sizeof(va_decode_args),
-               "va_paged_decode: struct_size %u != %zu (header/library mismatch)", a->struct_size,
+               "%s: struct_size %u != %zu (header/library mismatch)", fn, a->struct_size,
                sizeof(va_decode_args));
   const int eb = elem_bytes_of(a->dtype);
-  VA_CHECK_ARG(eb != 0, "va_paged_decode: unknown dtype %d", a->dtype);
+  VA_CHECK_ARG(eb != 0, "%s: unknown dtype %d", fn, a->dtype);
   const bool f8 = a->pool.kv_format == VA_KV_FP8_E4M3;
-  VA_CHECK_ARG(a->pool.kv_format == VA_KV_NATIVE || f8, "va_paged_decode: unknown kv_format %d",
+  VA_CHECK_ARG(a->pool.kv_format == VA_KV_NATIVE || f8 || mx4, "%s: unknown kv_format %d", fn,
                a->pool.kv_format);
   VA_CHECK_ARG(!f8 || (a->pool.k_scale > 0.f && a->pool.v_scale > 0.f),
-               "va_paged_decode: FP8 pool scales must be positive");
-  const int kv_eb = f8 ? 1 : eb;  // bytes per pool element
-  VA_CHECK_ARG(a->num_seqs >= 0, "va_paged_decode: num_seqs < 0");
+               "%s: FP8 pool scales must be positive", fn);
+  const int kv_eb = f8 || mx4 ? 1 : eb;  // bytes per unit of the pool's strides
+  VA_CHECK_ARG(a->num_seqs >= 0, "%s: num_seqs < 0", fn);
   if (a->num_seqs == 0) return VA_OK;
-  VA_CHECK_ARG(a->num_seqs <= 65535, "va_paged_decode: num_seqs > 65535");  // merge grid.y
+  VA_CHECK_ARG(a->num_seqs <= 65535, "%s: num_seqs > 65535", fn);  // merge grid.y
   VA_CHECK_ARG(a->q && a->out && a->pool.k && a->pool.v && a->block_tables && a->lens,
-               "va_paged_decode: null pointer argument");
+               "%s: null pointer argument", fn);
   VA_CHECK_ARG(a->num_kv_heads > 0 && a->num_heads > 0 && a->num_heads % a->num_kv_heads == 0,
-               "va_paged_decode: num_heads (%d) must be a positive multiple of num_kv_heads (%d)",
+               "%s: num_heads (%d) must be a positive multiple of num_kv_heads (%d)", fn,
                a->num_heads, a->num_kv_heads);
-  VA_CHECK_ARG(a->num_kv_heads <= 65535, "va_paged_decode: num_kv_heads > 65535");
+  VA_CHECK_ARG(a->num_kv_heads <= 65535, "%s: num_kv_heads > 65535", fn);
   const int G = a->num_heads / a->num_kv_heads;
-  VA_CHECK_ARG(a->pool.block_size > 0 && a->pool.num_blocks >= 0, "va_paged_decode: bad pool");
-  VA_CHECK_ARG(a->table_dtype == VA_I32 || a->table_dtype == VA_I64, "va_paged_decode: table_dtype");
-  VA_CHECK_ARG(a->lens_dtype == VA_I32 || a->lens_dtype == VA_I64, "va_paged_decode: lens_dtype");
+  VA_CHECK_ARG(a->pool.block_size > 0 && a->pool.num_blocks >= 0, "%s: bad pool", fn);
+  VA_CHECK_ARG(a->table_dtype == VA_I32 || a->table_dtype == VA_I64, "%s: table_dtype", fn);
+  VA_CHECK_ARG(a->lens_dtype == VA_I32 || a->lens_dtype == VA_I64, "%s: lens_dtype", fn);
   VA_CHECK_ARG(a->lens_kind == VA_LENS_PER_SEQ || a->lens_kind == VA_LENS_CUMULATIVE,
-               "va_paged_decode: lens_kind");
+               "%s: lens_kind", fn);
   VA_CHECK_ARG((a->new_k == nullptr) == (a->new_v == nullptr),
-               "va_paged_decode: new_k and new_v must be given together");
+               "%s: new_k and new_v must be given together", fn);
   VA_CHECK_ARG(a->new_slots == nullptr || a->new_k != nullptr,
-               "va_paged_decode: new_slots requires new_k/new_v");
+               "%s: new_slots requires new_k/new_v", fn);
   VA_CHECK_ARG(a->new_slots == nullptr || a->new_slots_dtype == VA_I32 ||
                    a->new_slots_dtype == VA_I64,
-               "va_paged_decode: new_slots_dtype");
-  VA_CHECK_ARG(a->max_seq_len >= 0, "va_paged_decode: max_seq_len < 0");
+               "%s: new_slots_dtype", fn);
+  VA_CHECK_ARG(a->max_seq_len >= 0, "%s: max_seq_len < 0", fn);
   VA_CHECK_ARG(a->split_tokens >= VA_SPLIT_EXACT,
-               "va_paged_decode: split_tokens %d (>= 0, or VA_SPLIT_EXACT)", a->split_tokens);
-  VA_CHECK_ARG(a->table_width >= 0, "va_paged_decode: table_width < 0");
+               "%s: split_tokens %d (>= 0, or VA_SPLIT_EXACT)", fn, a->split_tokens);
+  VA_CHECK_ARG(a->table_width >= 0, "%s: table_width < 0", fn);
   VA_CHECK_ARG(a->key_limit >= 0 && a->table_read_width >= 0,
-               "va_paged_decode: key_limit and table_read_width must be non-negative");
+               "%s: key_limit and table_read_width must be non-negative", fn);
   VA_CHECK_ARG(a->valid_mask == nullptr || (a->valid_len >= 0 && a->valid_stride_seq >= 0),
-               "va_paged_decode: valid_len and valid_stride_seq must be non-negative");
+               "%s: valid_len and valid_stride_seq must be non-negative", fn);
   // The vector kernels move 16-byte pieces; the small-head kernel moves
   // single elements.
   const bool small = small_head_decode(a);
   const int64_t align = small ? eb : 16, palign = small ? kv_eb : 16;
   VA_CHECK_ARG(!small || (a->head_dim >= 1 && a->head_dim <= kSmallMaxHeadDim),
-               "va_paged_decode: head_dim %d outside [1, %d]", a->head_dim, kSmallMaxHeadDim);
-  VA_CHECK_ARG(!small || (a->prologue == nullptr && !f8),
-               "va_paged_decode: the q/k prologue and FP8 pools need head_dim 64|128|256 and "
-               "group 1|2|4|8 (got head_dim %d, group %d)",
+               "%s: head_dim %d outside [1, %d]", fn, a->head_dim, kSmallMaxHeadDim);
+  VA_CHECK_ARG(!small || (a->prologue == nullptr && !f8 && !mx4),
+               "%s: the q/k prologue, FP8 and MXFP4 pools need head_dim 64|128|256 and "
+               "group 1|2|4|8 (got head_dim %d, group %d)", fn,
                a->head_dim, G);
   const int64_t strides[] = {a->q_stride_seq,      a->q_stride_head,     a->out_stride_seq,
                              a->out_stride_head,   a->new_k_stride_seq,  a->new_k_stride_head,
                              a->new_v_stride_seq,  a->new_v_stride_head};
   for (int64_t s : strides)
-    VA_CHECK_ARG((s * eb) % align == 0, "va_paged_decode: strides must be %lld-byte multiples",
+    VA_CHECK_ARG((s * eb) % align == 0, "%s: strides must be %lld-byte multiples", fn,
                  (long long)align);
   const int64_t pstrides[] = {a->pool.stride_block, a->pool.stride_slot, a->pool.stride_head};
   for (int64_t s : pstrides)
     VA_CHECK_ARG((s * kv_eb) % palign == 0,
-                 "va_paged_decode: pool strides must be %lld-byte multiples", (long long)palign);
+                 "%s: pool strides must be %lld-byte multiples", fn, (long long)palign);
   const uintptr_t ptrs[] = {(uintptr_t)a->q, (uintptr_t)a->out, (uintptr_t)a->new_k,
                             (uintptr_t)a->new_v};
   for (uintptr_t p : ptrs)
-    VA_CHECK_ARG(p % align == 0, "va_paged_decode: pointers must be %lld-byte aligned",
+    VA_CHECK_ARG(p % align == 0, "%s: pointers must be %lld-byte aligned", fn,
                  (long long)align);
   const uintptr_t pptrs[] = {(uintptr_t)a->pool.k, (uintptr_t)a->pool.v};
   for (uintptr_t p : pptrs)
-    VA_CHECK_ARG(p % palign == 0, "va_paged_decode: pool pointers must be %lld-byte aligned",
+    VA_CHECK_ARG(p % palign == 0, "%s: pool pointers must be %lld-byte aligned", fn,
                  (long long)palign);
 
-  const DecodePlan pl = plan_decode(a);
+  if (mx4) {
+    VA_CHECK_ARG(a->dtype == VA_BF16 || a->dtype == VA_F16,
+                 "%s: an MXFP4 pool needs bf16 or f16 q (got dtype %d)", fn, a->dtype);
+    if (const int rc = check_mx4(fn, a->pool, sc, a->head_dim)) return rc;
+    VA_CHECK_ARG(a->pool.block_size % kChunk == 0,
+                 "%s: an MXFP4 pool needs a block size that is a multiple of 16 (got %d)", fn,
+                 a->pool.block_size);
+    // Per-lane offsets inside a 16-row tile are 32-bit.
+    VA_CHECK_ARG(a->pool.stride_slot >= 0 && sc->stride_slot >= 0 &&
+                     (kChunk - 1) * a->pool.stride_slot + a->head_dim < ((int64_t)1 << 31) &&
+                     (kChunk - 1) * sc->stride_slot + a->head_dim < ((int64_t)1 << 31),
+                 "%s: slot strides must be non-negative and below 128 MiB", fn);
+    VA_CHECK_ARG(a->scale > 0.f && a->scale < INFINITY, "%s: scale must be > 0", fn);
+  }
+
+  const DecodePlan pl = mx4 ? plan_decode_mx4(a) : plan_decode(a);
   if (pl.total_bytes > 0) {
     if (a->workspace == nullptr || a->workspace_bytes < pl.total_bytes) {
-      set_error("va_paged_decode: workspace of %zu bytes needed, %zu given", pl.total_bytes,
+      set_error("%s: workspace of %zu bytes needed, %zu given", fn, pl.total_bytes,
                 a->workspace_bytes);
       return VA_ERR_WORKSPACE;
     }
-    VA_CHECK_ARG((uintptr_t)a->workspace % 16 == 0, "va_paged_decode: workspace alignment");
+    VA_CHECK_ARG((uintptr_t)a->workspace % 16 == 0, "%s: workspace alignment", fn);
   }
-  VA_CHECK_ARG(pl.max_parts <= kMaxParts, "va_paged_decode: too many context partitions");
+  VA_CHECK_ARG(pl.max_parts <= kMaxParts, "%s: too many context partitions", fn);
 
-  DecodeParams p;
+  DecodeMx4Params p;
+  p.ks = p.vs = nullptr;
+  p.sc_blk = p.sc_slot = p.sc_head = 0;
+  if (mx4) {
+    p.ks = (char*)sc->k;
+    p.vs = (char*)sc->v;
+    p.sc_blk = sc->stride_block;
+    p.sc_slot = sc->stride_slot;
+    p.sc_head = sc->stride_head;
+  }
   p.q = (const char*)a->q;
   p.q_sb = a->q_stride_seq * eb;
   p.q_sh = a->q_stride_head * eb;
@@ -460,16 +515,16 @@ int va::paged_decode_impl(const va_decode_args* a, void* stream) {
     const va_qk_prologue& pr = *a->prologue;
     VA_CHECK_ARG(pr.cos_sin_cache && pr.positions && pr.max_position > 0 &&
                      pr.cos_sin_stride >= a->head_dim,
-                 "va_paged_decode: prologue rotary cache / positions");
+                 "%s: prologue rotary cache / positions", fn);
     VA_CHECK_ARG(pr.q_norm_weight && (a->new_k == nullptr || pr.k_norm_weight),
-                 "va_paged_decode: prologue norm weights missing");
+                 "%s: prologue norm weights missing", fn);
     VA_CHECK_ARG(pr.weight_dtype == VA_BF16 || pr.weight_dtype == VA_F16 ||
                      pr.weight_dtype == VA_F32,
-                 "va_paged_decode: prologue weight_dtype");
+                 "%s: prologue weight_dtype", fn);
     VA_CHECK_ARG(pr.positions_dtype == VA_I32 || pr.positions_dtype == VA_I64,
-                 "va_paged_decode: prologue positions_dtype");
+                 "%s: prologue positions_dtype", fn);
     VA_CHECK_ARG((uintptr_t)pr.q_norm_weight % 16 == 0 && (uintptr_t)pr.k_norm_weight % 16 == 0,
-                 "va_paged_decode: prologue norm weights must be 16-byte aligned");
+                 "%s: prologue norm weights must be 16-byte aligned", fn);
     p.pro.q_w = pr.q_norm_weight;
     p.pro.k_w = pr.k_norm_weight;
     p.pro.w_dtype = pr.weight_dtype;
@@ -491,15 +546,25 @@ int va::paged_decode_impl(const va_decode_args* a, void* stream) {
     ok = launch_paged_decode_small(a->dtype, a->head_dim, G, p, dim3(a->num_seqs, a->num_heads),
                                    s);
     if (!ok) {
-      set_error("va_paged_decode: unsupported dtype %d / head_dim %d", a->dtype, a->head_dim);
+      set_error("%s: unsupported dtype %d / head_dim %d", fn, a->dtype, a->head_dim);
       return VA_ERR_UNSUPPORTED;
     }
-    return check_launch("va_paged_decode");
+    return check_launch(fn);
+  }
+  if (mx4) {
+    const dim3 hgrid(a->num_kv_heads, a->num_seqs, pl.max_parts);
+    ok = a->dtype == VA_BF16 ? launch_paged_decode_mx4<BF16>(a->head_dim, G, p, hgrid, s)
+                             : launch_paged_decode_mx4<F16>(a->head_dim, G, p, hgrid, s);
+    if (!ok) {
+      set_error("%s: unsupported head_dim %d / group size %d", fn, a->head_dim, G);
+      return VA_ERR_UNSUPPORTED;
+    }
+    return check_launch(fn);
   }
   if (f8 && !use_mfma_decode(a)) {
-    set_error("va_paged_decode: an FP8 pool needs bf16/f16 q, a block size that is a multiple "
+    set_error("%s: an FP8 pool needs bf16/f16 q, a block size that is a multiple "
               "of 16, head_dim 64|128|256 and group 1|2|4|8 (got dtype %d, block %d, head_dim %d, "
-              "group %d)",
+              "group %d)", fn,
               a->dtype, a->pool.block_size, a->head_dim, G);
     return VA_ERR_UNSUPPORTED;
   }
@@ -517,10 +582,10 @@ int va::paged_decode_impl(const va_decode_args* a, void* stream) {
     }
   }
   if (!ok) {
-    set_error("va_paged_decode: unsupported head_dim %d / group size %d (head_dim 64|128|256, "
-              "group 1|2|4|8)",
+    set_error("%s: unsupported head_dim %d / group size %d (head_dim 64|128|256, "
+              "group 1|2|4|8)", fn,
               a->head_dim, G);
     return VA_ERR_UNSUPPORTED;
   }
-  return check_launch("va_paged_decode");
+  return check_launch(fn);
 }

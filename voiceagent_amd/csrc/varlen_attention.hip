@@ -17,7 +17,21 @@ static bool dispatch_varlen(int D, int G, const VarlenParams& p, bool causal,
   }
 }
 
-static int varlen_native(const va_varlen_args* a, void* stream);
+template <bool kBF16>
+static bool dispatch_varlen_mx4(int D, int G, const VarlenParams& p, bool causal,
+                                int64_t items_per_xcd, hipStream_t st) {
+  switch (D) {
+    case 64: return launch_varlen_mx4_d<kBF16, 64>(G, p, causal, items_per_xcd, st);
+    case 128: return launch_varlen_mx4_d<kBF16, 128>(G, p, causal, items_per_xcd, st);
+    default: return false;
+  }
+}
+
+static va_store_args store_args_of(const va_varlen_args* a);
+
+// The attention alone over any pool (sc: an MXFP4 pool's scales); no codes are
+// stored.
+static int varlen_native(const va_varlen_args* a, const va_mx4_scales* sc, void* stream);
 
 }  // namespace va
 
@@ -179,7 +193,7 @@ extern "C" int va_varlen_attention(const va_varlen_args* a, void* stream) {
   VA_CHECK_ARG(!has_pool || a->pool.kv_format == VA_KV_NATIVE ||
                    a->pool.kv_format == VA_KV_FP8_E4M3,
                "va_varlen_attention: unknown kv_format %d", a->pool.kv_format);
-  if (!has_pool || a->pool.kv_format == VA_KV_NATIVE) return varlen_native(a, stream);
+  if (!has_pool || a->pool.kv_format == VA_KV_NATIVE) return varlen_native(a, nullptr, stream);
 
   // ---- FP8 pool: attention with the prefix converted in the kernel, then
   // the quantising store of the new rows ----
@@ -187,9 +201,41 @@ extern "C" int va_varlen_attention(const va_varlen_args* a, void* stream) {
                "va_varlen_attention: FP8 pool scales must be positive");
   va_varlen_args b = *a;
   b.slot_mapping = nullptr;
-  int rc = varlen_native(&b, stream);
+  int rc = varlen_native(&b, nullptr, stream);
   if (rc != VA_OK || a->slot_mapping == nullptr) return rc;
+  const va_store_args sa = va::store_args_of(a);
+  return va_store_kvcache(&sa, stream);
+}
 
+extern "C" int va_varlen_attention_mx4(const va_varlen_args* a, const va_mx4_scales* sc,
+                                       void* stream) {
+  using namespace va;
+  const char* const fn = "va_varlen_attention_mx4";
+  VA_CHECK_ARG(a != nullptr && sc != nullptr, "%s: null args or scales", fn);
+  VA_CHECK_ARG(a->struct_size == sizeof(va_varlen_args),
+               "%s: struct_size %u != %zu (header/library mismatch)", fn, a->struct_size,
+               sizeof(va_varlen_args));
+  VA_CHECK_ARG(a->num_seqs >= 0, "%s: num_seqs < 0", fn);
+  if (a->num_seqs == 0 || a->total_q == 0) return VA_OK;
+  VA_CHECK_ARG(a->pool.k != nullptr, "%s: an MXFP4 pool is needed", fn);
+  if (const int rc = check_mx4(fn, a->pool, sc, a->head_dim)) return rc;
+  VA_CHECK_ARG(a->pool.block_size > 0 && a->pool.block_size % 16 == 0,
+               "%s: an MXFP4 pool needs a block size that is a multiple of 16 (got %d)", fn,
+               a->pool.block_size);
+  VA_CHECK_ARG(a->pool.stride_slot >= 0 &&
+                   15 * a->pool.stride_slot + a->head_dim < ((int64_t)1 << 31),
+               "%s: the pool's slot stride must be non-negative and below 128 MiB", fn);
+  VA_CHECK_ARG(a->prologue == nullptr, "%s: no query prologue over an MXFP4 pool", fn);
+  va_varlen_args b = *a;
+  b.slot_mapping = nullptr;
+  const int rc = varlen_native(&b, sc, stream);
+  if (rc != VA_OK || a->slot_mapping == nullptr) return rc;
+  const va_store_args sa = store_args_of(a);
+  return va_store_kvcache_mx4(&sa, sc, stream);
+}
+
+// The store of a call's new rows, as a launch of its own.
+static va_store_args va::store_args_of(const va_varlen_args* a) {
   va_store_args sa{};
   sa.struct_size = sizeof(va_store_args);
   sa.dtype = a->dtype;
@@ -205,10 +251,10 @@ extern "C" int va_varlen_attention(const va_varlen_args* a, void* stream) {
   sa.num_tokens = a->total_q;
   sa.num_kv_heads = a->num_kv_heads;
   sa.head_dim = a->head_dim;
-  return va_store_kvcache(&sa, stream);
+  return sa;
 }
 
-int va::varlen_native(const va_varlen_args* a, void* stream) {
+int va::varlen_native(const va_varlen_args* a, const va_mx4_scales* sc, void* stream) {
   using namespace va;
   VA_CHECK_ARG(a->dtype == VA_BF16 || a->dtype == VA_F16,
                "va_varlen_attention: dtype must be VA_BF16 or VA_F16 (MFMA path)");
@@ -238,7 +284,8 @@ int va::varlen_native(const va_varlen_args* a, void* stream) {
   const bool f8 = has_pool && a->pool.kv_format == VA_KV_FP8_E4M3;
   VA_CHECK_ARG(!f8 || a->head_dim % 16 == 0,
                "va_varlen_attention: FP8 pool head_dim must be a multiple of 16");
-  const int64_t kv_eb = f8 ? 1 : 2;
+  const bool mx4 = sc != nullptr;
+  const int64_t kv_eb = f8 || mx4 ? 1 : 2;
   const int64_t strides[] = {a->q_stride_tok,  a->q_stride_head,      a->k_stride_tok,
                              a->k_stride_head, a->v_stride_tok,       a->v_stride_head,
                              a->out_stride_tok, a->out_stride_head};
@@ -305,6 +352,11 @@ int va::varlen_native(const va_varlen_args* a, void* stream) {
   p.kv_f8 = f8;
   p.k_scale = f8 ? a->pool.k_scale : 1.0f;
   p.v_scale = f8 ? a->pool.v_scale : 1.0f;
+  p.ks = mx4 ? (const uint8_t*)sc->k : nullptr;
+  p.vs = mx4 ? (const uint8_t*)sc->v : nullptr;
+  p.sc_blk = mx4 ? sc->stride_block : 0;
+  p.sc_slot = mx4 ? sc->stride_slot : 0;
+  p.sc_head = mx4 ? sc->stride_head : 0;
   p.has_pro = a->prologue != nullptr;
   p.pro = PrologueParams{};
   if (a->prologue != nullptr) {
@@ -375,7 +427,11 @@ int va::varlen_native(const va_varlen_args* a, void* stream) {
   const int64_t items_per_xcd = (npairs + kXcds - 1) / kXcds * nqb;
   const hipStream_t st = (hipStream_t)stream;
   const bool ok =
-      a->dtype == VA_BF16
+      mx4 ? (a->dtype == VA_BF16
+                 ? dispatch_varlen_mx4<true>(a->head_dim, G, p, a->causal != 0, items_per_xcd, st)
+                 : dispatch_varlen_mx4<false>(a->head_dim, G, p, a->causal != 0, items_per_xcd,
+                                              st))
+      : a->dtype == VA_BF16
           ? dispatch_varlen<true>(a->head_dim, G, p, a->causal != 0, items_per_xcd, st)
           : dispatch_varlen<false>(a->head_dim, G, p, a->causal != 0, items_per_xcd, st);
   if (!ok) {

@@ -49,6 +49,7 @@
 
 #include "common.h"
 #include "fastdiv.h"
+#include "mx4.h"
 #include "prologue.h"
 
 namespace va {
@@ -101,6 +102,9 @@ struct VarlenParams {
   int32_t* part_count;
   int32_t has_pro;          // the Qwen3 query prologue runs on every query row
   PrologueParams pro;
+  const uint8_t* ks;  // MXFP4 pool: the scale bytes
+  const uint8_t* vs;
+  int64_t sc_blk, sc_slot, sc_head;  // bytes
 };
 
 // The launch's arguments where they are needed once per item or on uncommon
@@ -236,13 +240,20 @@ constexpr int waves_per_simd(int d, bool half) { return d == 64 ? (half ? 4 : 3)
 // its own: the plan's state costs the others scalar registers, 1 us of 41 on
 // a launch of 32 prompts).
 //
+// kMx4 (with kPaged): the pool holds MXFP4 codes and scales (mx4.h), blocks of
+// a multiple of 16 tokens.  As over FP8 pools a tile's pool rows are copied as
+// codes, but a wave converts the rows it copied itself, in a code area of its
+// own, before the tile's barrier: no second barrier.  A lane converts whole
+// groups (16 bytes of codes), whose scale bytes it loaded when the tile was
+// requested.
+//
 // kHalf: 64 MFMA rows per item, one 16-row tile per wave.  A tile's body is
 // bound by the wave's own chain (S^T, softmax, O^T; ~1.5 us with two row tiles,
 // ~1.25 with one, alone on a CU), so a launch that leaves slots idle, or whose
 // blocks are short anyway, ends sooner on items of half the rows (the host's
 // rule: half_rows_wanted).
 template <bool kBF16, int D, int G, bool kCausal, bool kPaged, bool kOnce, bool kF8, bool kPro,
-          bool kSplit, bool kHalf>
+          bool kSplit, bool kHalf, bool kMx4>
 __global__ __launch_bounds__(kVarlenThreads, waves_per_simd(D, kHalf)) void
 varlen_attention_kernel(VarlenParams p) {
   constexpr int NR = kHalf ? 1 : 2;        // 16-row tiles per wave
@@ -266,13 +277,23 @@ varlen_attention_kernel(VarlenParams p) {
   __shared__ __align__(1024) char s_kv[kStages * 2 * TILE_B];
   // FP8 pool: the codes of one tile's pool rows (K, then V), row-major and
   // unswizzled: row r's 16-code chunk c at r D + 16 c.
-  static_assert(!kF8 || kPaged, "FP8 codes come from a pool");
-  constexpr int CODE_B = kKeyTile * D;     // bytes of one tile of codes, K or V
-  constexpr int CCPR = D / 16;             // 16-code chunks per code row
+  constexpr bool kCode = kF8 || kMx4;
+  static_assert(!kCode || kPaged, "codes come from a pool");
+  static_assert(!(kF8 && kMx4) && !(kMx4 && kPro), "one pool format, no query prologue");
+  constexpr int CROWB = kMx4 ? D / 2 : D;  // bytes of a code row
+  constexpr int CCPR = CROWB / 16;         // 16-byte chunks per code row
   constexpr int CRPI = 64 / CCPR;          // code rows per DMA instruction
-  constexpr int NIC = CODE_B / 1024 / 4;   // code DMA instructions per wave per tile, K or V
-  static_assert(!kF8 || NIC * 4 * 1024 == CODE_B, "code DMA split");
-  __shared__ __align__(1024) char s_code[kF8 ? 2 * CODE_B : 16];
+  // Code DMA instructions per wave per tile, K or V (MXFP4 at head_dim 64: the
+  // upper lanes copy the wave's 16 rows a second time).
+  constexpr int NIC = CRPI < 16 ? 16 / CRPI : 1;
+  constexpr int CODE_B = 4 * NIC * 1024;   // bytes of one tile of codes, K or V
+  static_assert(!kF8 || CODE_B == kKeyTile * D, "code DMA split");
+  __shared__ __align__(1024) char s_code[kCode ? 2 * CODE_B : 16];
+  // kMx4: a wave's 16 rows are 16 D / 32 groups of K and as many of V, NGL of
+  // them a lane's: group e = 64 i + lane is group e % NS of row e / NS (K's 16,
+  // then V's).
+  constexpr int NS = D / kMx4Group;
+  constexpr int NGL = 2 * 16 * NS / 64;
   // kPro: the query norm weights as fp32, written once per workgroup here and
   // read by every item's prologue (the first tile's barrier orders them).
   __shared__ __align__(16) float s_qw[kPro ? D : 4];
@@ -526,7 +547,13 @@ varlen_attention_kernel(VarlenParams p) {
   set_offsets(k_st, v_st);
   // FP8 pool: a wave's 16 code rows (unswizzled, CRPI rows an instruction).
   const uint32_t code_lane =
-      kF8 ? (uint32_t)(lane / CCPR) * (uint32_t)p.s_slot + (uint32_t)(lane % CCPR) * 16u : 0u;
+      kF8 ? (uint32_t)(lane / CCPR) * (uint32_t)p.s_slot + (uint32_t)(lane % CCPR) * 16u
+      : kMx4 ? (uint32_t)(lane / CCPR % 16) * (uint32_t)p.s_slot + (uint32_t)(lane % CCPR) * 16u
+             : 0u;
+  // kMx4: the scales of the lane's groups of the tile requested last.
+  uint32_t gsc[kMx4 ? NGL : 1];
+#pragma unroll
+  for (int i = 0; i < (kMx4 ? NGL : 1); ++i) gsc[i] = 0;
   const uint32_t code_dst = code_base + (uint32_t)(wave * NIC * 1024);
 
   // The cursor of the tiles being requested, one step ahead of the tiles
@@ -551,6 +578,7 @@ varlen_attention_kernel(VarlenParams p) {
     cu.vb += (uint64_t)v_st * kKeyTile;
   };
   int64_t rows = kNoRow;
+  int64_t srows = 0;  // kMx4: the scales' offset beside `rows`
   uint2 pend = make_uint2(0u, 0u);  // raw block ids that `rows` takes next
   auto cursor_to = [&](const Item& it) {
     cu.t = it.t0;
@@ -600,6 +628,10 @@ varlen_attention_kernel(VarlenParams p) {
     if (bid >= 0 && bid < ca->num_blocks)
       rows = bid * ca->s_blk + (int64_t)fast_mod(tok, cold_div(ca->bs_div)) * ca->s_slot +
              cu.h * ca->s_head;
+    if constexpr (kMx4)
+      if (rows != kNoRow)
+        srows = bid * ca->sc_blk + (int64_t)fast_mod(tok, cold_div(ca->bs_div)) * ca->sc_slot +
+                cu.h * ca->sc_head;
   };
   // What `rows` will need next: the item's following 64 tiles, or the next
   // item's first.
@@ -664,12 +696,12 @@ varlen_attention_kernel(VarlenParams p) {
         }
       }
     };
-    const char* kc[kF8 ? NIC : 1];
-    const char* vc[kF8 ? NIC : 1];
-    if constexpr (kF8) {
+    const char* kc[kCode ? NIC : 1];
+    const char* vc[kCode ? NIC : 1];
+    if constexpr (kCode) {
       // The tile's pool rows as codes: lane l of code instruction i copies
       // chunk l % CCPR of code row (wave NIC + i) CRPI + l / CCPR.
-      int crow0 = 16 * wave + lane / CCPR;
+      int crow0 = 16 * wave + (kMx4 ? lane / CCPR % 16 : lane / CCPR);
       asm volatile("" : "+v"(crow0));
       uint2 craw[NIC];
 #pragma unroll
@@ -686,7 +718,7 @@ varlen_attention_kernel(VarlenParams p) {
 #pragma unroll
     for (int i = 0; i < NI; ++i) {
       braw[i] = make_uint2(0u, 0u);
-      if (kPaged && !kF8) raw_id(kb + row0 + i * RPI, braw[i]);
+      if (kPaged && !kCode) raw_id(kb + row0 + i * RPI, braw[i]);
     }
     const char* ka[NI];
     const char* va_[NI];
@@ -699,8 +731,8 @@ varlen_attention_kernel(VarlenParams p) {
       va_[i] = zero_row;
       if (j < cu.kend) {
         if (kPaged && j < cu.prefix) {
-          // An FP8 pool row is staged by the code copy and its conversion.
-          if constexpr (!kF8) pool_at(j, braw[i], chunk * 16, ka[i], va_[i]);
+          // A row of codes is staged by the code copy and its conversion.
+          if constexpr (!kCode) pool_at(j, braw[i], chunk * 16, ka[i], va_[i]);
         } else {
           const uint32_t r = row - 16 * wave;
           ka[i] = cu.kb + (r * k_st + chunk * 16);
@@ -715,7 +747,7 @@ varlen_attention_kernel(VarlenParams p) {
     // 300 14.6 -> 13.9, 9 of 60-594 22.5 -> 21.4, 28 decoding sequences with 4
     // prompts 20.6 -> 19.9; 64/8 heads, 32 of 50-450 69.7 -> 67.1.  (head_dim
     // 128 has other registers there and no such wait.)
-    if constexpr (kPaged && !kF8 && D == 64) {
+    if constexpr (kPaged && !kCode && D == 64) {
 #pragma unroll
       for (int i = 0; i < NI; ++i) asm volatile("" ::"v"(braw[i].x), "v"(braw[i].y));
     }
@@ -729,7 +761,7 @@ varlen_attention_kernel(VarlenParams p) {
         dma16(va_[i], dst0 + TILE_B + i * 1024);
       }
     }
-    if constexpr (kF8) {
+    if constexpr (kCode) {
       if (kb < cu.prefix) {
 #pragma unroll
         for (int i = 0; i < NIC; ++i) {
@@ -748,7 +780,7 @@ varlen_attention_kernel(VarlenParams p) {
     const int kb = cu.t * kKeyTile;
     if (kb >= cu.prefix && kb + kKeyTile <= cu.kend) {
       e.kind = kRows;
-      if (kPaged && !kF8 && off_pool) {
+      if (kPaged && !kCode && off_pool) {
         set_offsets(k_st, v_st);
         off_pool = false;
       }
@@ -761,9 +793,29 @@ varlen_attention_kernel(VarlenParams p) {
       const int l = cu.t - cu.row0;
       row = (int64_t)(((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(rows >> 32), l) << 32) |
                       (uint32_t)__builtin_amdgcn_readlane((int)rows, l));
+      if constexpr (kMx4) {
+        // The scales of the lane's groups: loaded whatever the row, so that no
+        // load sits behind a branch (a row that is not there takes a zero).
+        const int64_t srow =
+            (int64_t)(((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(srows >> 32), l) << 32) |
+                      (uint32_t)__builtin_amdgcn_readlane((int)srows, l));
+        const ColdArgs ca = cold_args();
+        const char* at[NGL];
+#pragma unroll
+        for (int i = 0; i < NGL; ++i) {
+          const int g = 64 * i + lane, rc = g % (16 * NS);
+          const int j = kb + 16 * wave + rc / NS;
+          at[i] = zero_row;
+          if (row != kNoRow && j < cu.prefix && j < cu.kend)
+            at[i] = reinterpret_cast<const char*>(g >= 16 * NS ? ca->vs : ca->ks) + srow +
+                    (rc / NS) * ca->sc_slot + rc % NS;
+        }
+#pragma unroll
+        for (int i = 0; i < NGL; ++i) gsc[i] = *reinterpret_cast<const uint8_t*>(at[i]);
+      }
       if (kb + kKeyTile <= min(cu.prefix, cu.kend) && row != kNoRow && p.block16) {
-        e.kind = kF8 ? kCodes : kRows;
-        if (!kF8 && !off_pool) {
+        e.kind = kCode ? kCodes : kRows;
+        if (!kCode && !off_pool) {
           const uint32_t slot = (uint32_t)cold_args()->s_slot;
           set_offsets(slot, slot);
           off_pool = true;
@@ -796,7 +848,7 @@ varlen_attention_kernel(VarlenParams p) {
 #pragma unroll
       for (int i = 0; i < NI; ++i) easy_issue(e, i, dst);
     }
-    if constexpr (kF8) {
+    if constexpr (kCode) {
       if (e.kind == kCodes) {
 #pragma unroll
         for (int i = 0; i < NIC; ++i) easy_codes(e, i);
@@ -845,7 +897,7 @@ varlen_attention_kernel(VarlenParams p) {
   constexpr int RPS = 64 / CPR;  // rows per store step
   constexpr int NSTEP = (BQ * CPR + kVarlenThreads - 1) / kVarlenThreads;
   static_assert(NSTEP * RPS <= 64, "one slot lane per row");
-  const bool fused_store = kPaged && !kF8 && p.slots != nullptr;  // FP8: a launch of its own
+  const bool fused_store = kPaged && !kCode && p.slots != nullptr;  // codes: a launch of its own
   auto st_base = [&](int k) {  // first block row of store step k (BQ: none)
     const int e0 = k * kVarlenThreads + 64 * wave;
     return e0 < BQ * CPR ? e0 / CPR : BQ;
@@ -928,6 +980,33 @@ varlen_attention_kernel(VarlenParams p) {
       // which then takes the next tile: this item's tile t + 1, or the next
       // item's first tile.
       wait_vmcnt<0>();
+      // MXFP4 pool: the wave's rows of this tile from its code area into the
+      // stage, at their swizzled positions; then the code area and `gsc` may
+      // take the next tile.
+      if constexpr (kMx4) {
+#pragma unroll
+        for (int i = 0; i < NGL; ++i) asm volatile("" ::"v"(gsc[i]));
+        if (kb < prefix) {
+          char* const s_kt = s_kv + stage * 2 * TILE_B;
+#pragma unroll
+          for (int i = 0; i < NGL; ++i) {
+            const int g = 64 * i + lane, rc = g % (16 * NS);
+            const int is_v = g >= 16 * NS ? 1 : 0;
+            const int r = 16 * wave + rc / NS, c = rc % NS;
+            if (kb + r < prefix) {
+              const uint4 codes = lds_read16(
+                  s_code + is_v * CODE_B + wave * NIC * 1024, (rc / NS) * CROWB + c * 16);
+              char* const dst = s_kt + is_v * TILE_B + r * ROWB;
+              const uint32_t w[4] = {codes.x, codes.y, codes.z, codes.w};
+#pragma unroll
+              for (int q = 0; q < 4; ++q)
+                *reinterpret_cast<uint4*>(dst + (((4 * c + q) ^ swz<D>(r)) << 4)) =
+                    mx4_values8<ET>(w[q], gsc[i]);
+            }
+          }
+          wait_lgkmcnt0();
+        }
+      }
       __syncthreads();
       // The query rows, the slot and block ids were loaded before the wait:
       // make the compiler's own wait for them fall here, before the next
@@ -1170,7 +1249,7 @@ varlen_attention_kernel(VarlenParams p) {
 #pragma unroll
             for (int j = 0; j < PAIRS; ++j) easy_issue(e, (kt / EVERY) * PAIRS + j, n_dst);
           }
-          if constexpr (kF8) {
+          if constexpr (kCode) {
             if (kt < NIC && e.kind == kCodes) easy_codes(e, kt);
           }
         }
@@ -1372,7 +1451,8 @@ varlen_attention_kernel(VarlenParams p) {
 // of the item whose first piece is XCD x % 8's piece x / 8 (the XCD that wrote
 // it), and ends at once when there is no such item.
 //   out = sum_j 2^(m_j - M) o_j / sum_j 2^(m_j - M) l_j,  M = max_j m_j.
-template <bool kBF16, int D, int G, bool kHalf>
+// kMx4 only separates the names of two translation units' instantiations.
+template <bool kBF16, int D, int G, bool kHalf, bool kMx4>
 __global__ __launch_bounds__(256) void varlen_merge_kernel(VarlenParams p) {
   constexpr int LPR = D / 4;       // lanes per row, four outputs each
   constexpr int RPP = 256 / LPR;   // rows per pass
@@ -1421,9 +1501,10 @@ __global__ __launch_bounds__(256) void varlen_merge_kernel(VarlenParams p) {
 // keeps resident on one XCD's CUs, or fewer when the XCD's item list (at
 // most items_per_xcd long) is shorter.
 template <bool kBF16, int D, int G, bool kCausal, bool kPaged, bool kOnce, bool kF8, bool kPro,
-          bool kSplit, bool kHalf>
+          bool kSplit, bool kHalf, bool kMx4>
 static void launch_grid(const VarlenParams& p, int64_t items_per_xcd, hipStream_t st) {
-  const auto kern = varlen_attention_kernel<kBF16, D, G, kCausal, kPaged, kOnce, kF8, kPro, kSplit, kHalf>;
+  const auto kern = varlen_attention_kernel<kBF16, D, G, kCausal, kPaged, kOnce, kF8, kPro, kSplit,
+                                            kHalf, kMx4>;
   // Resident workgroups per CU, queried once (a failed query is not cached:
   // the launch then assumes 1, which is correct but leaves slots idle).
   static std::atomic<int> cached{0};
@@ -1445,26 +1526,27 @@ static void launch_grid(const VarlenParams& p, int64_t items_per_xcd, hipStream_
   if (per_xcd < 1) per_xcd = 1;
   hipLaunchKernelGGL(kern, dim3((unsigned)(per_xcd * kXcds)), dim3(kVarlenThreads), 0, st, p);
   if constexpr (kSplit)
-    hipLaunchKernelGGL((varlen_merge_kernel<kBF16, D, G, kHalf>),
+    hipLaunchKernelGGL((varlen_merge_kernel<kBF16, D, G, kHalf, kMx4>),
                        dim3(p.split_slots * kXcds, kHalf ? 2 : 4), dim3(256), 0, st, p);
 }
 
 template <bool kBF16, int D, int G, bool kCausal, bool kPaged, bool kOnce = false,
-          bool kF8 = false, bool kPro = false>
+          bool kF8 = false, bool kPro = false, bool kMx4 = false>
 static void launch_persistent(const VarlenParams& p, int64_t items_per_xcd, hipStream_t st) {
   if constexpr (kCausal && !kPro) {
     if (p.half)
-      return p.split ? launch_grid<kBF16, D, G, true, kPaged, false, kF8, false, true, true>(
+      return p.split ? launch_grid<kBF16, D, G, true, kPaged, false, kF8, false, true, true, kMx4>(
                            p, items_per_xcd, st)
-                     : launch_grid<kBF16, D, G, true, kPaged, false, kF8, false, false, true>(
+                     : launch_grid<kBF16, D, G, true, kPaged, false, kF8, false, false, true, kMx4>(
                            p, items_per_xcd, st);
   }
   if constexpr (!kOnce) {
     if (p.split)
-      return launch_grid<kBF16, D, G, kCausal, kPaged, false, kF8, kPro, true, false>(
+      return launch_grid<kBF16, D, G, kCausal, kPaged, false, kF8, kPro, true, false, kMx4>(
           p, items_per_xcd, st);
   }
-  launch_grid<kBF16, D, G, kCausal, kPaged, kOnce, kF8, kPro, false, false>(p, items_per_xcd, st);
+  launch_grid<kBF16, D, G, kCausal, kPaged, kOnce, kF8, kPro, false, false, kMx4>(
+      p, items_per_xcd, st);
 }
 
 template <bool kBF16, int D, int G, bool kCausal>
@@ -1513,6 +1595,40 @@ template <>
 bool launch_varlen_d<false, 64>(int, const VarlenParams&, bool, int64_t, hipStream_t);
 template <>
 bool launch_varlen_d<false, 128>(int, const VarlenParams&, bool, int64_t, hipStream_t);
+
+// The same over MXFP4 pools, in varlen_<type>_d<D>_mx4.hip.
+template <bool kBF16, int D>
+bool launch_varlen_mx4_d(int G, const VarlenParams& p, bool causal, int64_t items_per_xcd,
+                         hipStream_t st);
+template <>
+bool launch_varlen_mx4_d<true, 64>(int, const VarlenParams&, bool, int64_t, hipStream_t);
+template <>
+bool launch_varlen_mx4_d<true, 128>(int, const VarlenParams&, bool, int64_t, hipStream_t);
+template <>
+bool launch_varlen_mx4_d<false, 64>(int, const VarlenParams&, bool, int64_t, hipStream_t);
+template <>
+bool launch_varlen_mx4_d<false, 128>(int, const VarlenParams&, bool, int64_t, hipStream_t);
+
+template <bool kBF16, int D, int G>
+static void launch_varlen_mx4(const VarlenParams& p, bool causal, int64_t items_per_xcd,
+                              hipStream_t st) {
+  if (causal)
+    launch_persistent<kBF16, D, G, true, true, false, false, false, true>(p, items_per_xcd, st);
+  else
+    launch_persistent<kBF16, D, G, false, true, false, false, false, true>(p, items_per_xcd, st);
+}
+
+template <bool kBF16, int D>
+static bool dispatch_varlen_mx4_g(int G, const VarlenParams& p, bool causal, int64_t items_per_xcd,
+                                  hipStream_t st) {
+  switch (G) {
+    case 1: launch_varlen_mx4<kBF16, D, 1>(p, causal, items_per_xcd, st); return true;
+    case 2: launch_varlen_mx4<kBF16, D, 2>(p, causal, items_per_xcd, st); return true;
+    case 4: launch_varlen_mx4<kBF16, D, 4>(p, causal, items_per_xcd, st); return true;
+    case 8: launch_varlen_mx4<kBF16, D, 8>(p, causal, items_per_xcd, st); return true;
+    default: return false;
+  }
+}
 
 template <bool kBF16, int D>
 static bool dispatch_varlen_g(int G, const VarlenParams& p, bool causal, int64_t items_per_xcd,

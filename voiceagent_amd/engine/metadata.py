@@ -19,6 +19,12 @@ driven exactly as the engine drives them:
   skipped (:150-191).  ``max_seqlen_k`` is baked in at ``max_model_len``
   (:81-94).
 
+Both also exist for an engine that keeps its requests' state on the GPU (block
+tables a row per request, lengths a step's kernels may have advanced, a free
+list): :func:`prepare_batch_device` and :meth:`DecodeGraphMetadata.stage_device`
+build the same metadata there in one launch, with no host copy
+(:func:`voiceagent_amd.ops.batch_metadata`).
+
 A sequence is any object with ``num_computed_tokens``, ``block_table`` (a list
 of block ids) and ``len()``, the three attributes the reference builders read.
 """
@@ -29,6 +35,7 @@ from typing import Protocol, Sequence
 
 import torch
 
+from voiceagent_amd import ops
 from voiceagent_amd.layers.context import AttentionContext
 
 
@@ -83,6 +90,42 @@ def prepare_batch(
     return torch.tensor(positions, dtype=torch.int64, device=device), context
 
 
+def prepare_batch_device(
+    lens: torch.Tensor,
+    num_computed: torch.Tensor,
+    request_tables: torch.Tensor,
+    block_size: int,
+    *,
+    max_tokens: int,
+    max_seqlen_q: int,
+    max_seqlen_k: int,
+    max_seqlen_k_exact: bool = False,
+    rows: torch.Tensor | None = None,
+    free_blocks: torch.Tensor | None = None,
+    free_count: torch.Tensor | None = None,
+) -> tuple[torch.Tensor, AttentionContext, ops.BatchMetadata]:
+    """:func:`prepare_batch` for requests whose lengths and block tables are on
+    the GPU: positions, the attention context, and the metadata they come from
+    (its totals and, with a free list, the count left).
+
+    The host gives what it has to know: ``max_tokens`` rows (the step's tokens,
+    or more: rows behind the last token have slot -1 and belong to no sequence)
+    and bounds of the query and context lengths."""
+    meta = ops.batch_metadata(lens, num_computed, request_tables, block_size,
+                              max_tokens=max_tokens, rows=rows, free_blocks=free_blocks,
+                              free_count=free_count)
+    context = AttentionContext(
+        cu_seqlens_q=meta.cu_seqlens_q,
+        cu_seqlens_k=meta.cu_seqlens_k,
+        max_seqlen_q=max_seqlen_q,
+        max_seqlen_k=max_seqlen_k,
+        slot_mapping=meta.slot_mapping,
+        block_tables=meta.block_tables,
+        max_seqlen_k_exact=max_seqlen_k_exact,
+    )
+    return meta.positions, context, meta
+
+
 class DecodeGraphMetadata:
     """Static decode metadata for captured graphs (graph_runner.py:60-191)."""
 
@@ -116,6 +159,36 @@ class DecodeGraphMetadata:
         self.host_slot_mapping = torch.full((size,), -1, dtype=torch.int32, **pinned)
         self.host_cu_seqlens_k = torch.zeros(size + 1, dtype=torch.int32, **pinned)
         self.host_block_tables = torch.zeros(size, max_blocks, dtype=torch.int32, **pinned)
+
+    def stage_device(
+        self,
+        lens: torch.Tensor,
+        num_computed: torch.Tensor,
+        request_tables: torch.Tensor,
+        *,
+        rows: torch.Tensor | None = None,
+        free_blocks: torch.Tensor | None = None,
+        free_count: torch.Tensor | None = None,
+    ) -> tuple[int, ops.BatchMetadata]:
+        """:meth:`stage` for requests whose state is on the GPU: one launch
+        fills the static buffers of the bucket that holds the batch.  Every
+        request contributes its last token (``num_computed = lens - 1``); the
+        result's totals say how many tokens there were and, with a free list,
+        what is left of it.  Returns the bucket and the metadata."""
+        batch = int(lens.numel())
+        bucket = self.bucket_for(batch)
+        if bucket is None:
+            raise ValueError(f"no bucket for a batch of {batch}")
+        i32 = {"dtype": torch.int32, "device": self.device}
+        # cu_seqlens_q stays the static 0, 1, 2, ... whatever the lengths say.
+        out = ops.BatchMetadata(self.positions[:bucket], self.slot_mapping[:bucket],
+                                torch.empty(bucket + 1, **i32), self.cu_seqlens_k[: bucket + 1],
+                                self.block_tables[:bucket], torch.empty(5, **i32))
+        meta = ops.batch_metadata(lens, num_computed, request_tables, self.block_size,
+                                  max_tokens=bucket, rows=rows, padded_batch=bucket,
+                                  table_width=self.max_blocks, free_blocks=free_blocks,
+                                  free_count=free_count, out=out)
+        return bucket, meta
 
     def context(self, batch_size: int) -> AttentionContext:
         """The context a graph of ``batch_size`` rows captures (graph_runner.py:81-94)."""

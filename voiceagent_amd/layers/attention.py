@@ -46,6 +46,10 @@ the layer's ``k_scale`` / ``v_scale`` (vLLM's per-tensor convention, 1.0 by
 default) give each code's value, every store quantises and every read
 dequantises.  The engine allocates the cache in that dtype
 (model_runner.py:119) and sets the scales on the layers.
+
+Or MXFP4 (``torch.float4_e2m1fn_x2``, about a quarter of bf16's bytes;
+``ops.mxfp4_kv_pool``): the layer's ``k_scale`` / ``v_scale`` are then the
+layer's slices of the pool's scale tensors.  Blocks of a multiple of 16 tokens.
 """
 
 from __future__ import annotations
@@ -64,8 +68,8 @@ def store_kvcache(
     v_cache: torch.Tensor,
     slot_mapping: torch.Tensor,
     *,
-    k_scale: float = 1.0,
-    v_scale: float = 1.0,
+    k_scale: float | torch.Tensor = 1.0,
+    v_scale: float | torch.Tensor = 1.0,
 ) -> None:
     """Scatter key/value rows [N, Hkv, D] into an NHD pool [nb, bs, Hkv, D].
 
@@ -73,13 +77,15 @@ def store_kvcache(
     contract (assertions :61-64): rows may be strided (the engine's ``v`` is a
     view of the fused qkv output) but each row's heads are contiguous.  An FP8
     (float8_e4m3fn) pool receives the codes of key / k_scale and
-    value / v_scale; the scales are ignored for a 16-bit or fp32 pool.
+    value / v_scale; the scales are ignored for a 16-bit or fp32 pool.  An
+    MXFP4 pool (two codes an element) comes with its scale tensors.
     """
     num_tokens, num_heads, head_dim = key.shape
     hidden = num_heads * head_dim
     assert key.stride(-1) == 1 and value.stride(-1) == 1
     assert key.stride(1) == head_dim and value.stride(1) == head_dim
-    assert k_cache.stride(1) == hidden and v_cache.stride(1) == hidden
+    packed = 2 if k_cache.dtype == ops.MXFP4_KV_DTYPE else 1
+    assert k_cache.stride(1) * packed == hidden and v_cache.stride(1) * packed == hidden
     assert slot_mapping.numel() == num_tokens
     ops.store_kvcache(key, value, k_cache, v_cache, slot_mapping, layout=ops.LAYOUT_NHD,
                       k_scale=k_scale, v_scale=v_scale)
@@ -104,7 +110,7 @@ class PagedAttention(nn.Module):
     varlen_fuse_prologue = False
     kv_layout = ops.LAYOUT_NHD
     k_scale = 1.0  # FP8 pools: value of a key code = code * k_scale
-    v_scale = 1.0
+    v_scale = 1.0  # (MXFP4 pools: the layer's scale tensors)
 
     def __init__(self, num_heads: int, head_dim: int, scale: float, num_kv_heads: int):
         super().__init__()
@@ -233,7 +239,8 @@ class PagedAttention(nn.Module):
     def _store(self, k: torch.Tensor, v: torch.Tensor, slot_mapping: torch.Tensor) -> None:
         """Unfused store: the reference's store_kvcache (and its stride
         contract) for an NHD pool, the same scatter by layout otherwise."""
-        if self.kv_layout == ops.LAYOUT_NHD and self.k_cache.dtype != ops.FP8_KV_DTYPE:
+        if (self.kv_layout == ops.LAYOUT_NHD and
+                self.k_cache.dtype not in (ops.FP8_KV_DTYPE, ops.MXFP4_KV_DTYPE)):
             store_kvcache(k, v, self.k_cache, self.v_cache, slot_mapping)
         else:
             ops.store_kvcache(k, v, self.k_cache, self.v_cache, slot_mapping,

@@ -77,10 +77,13 @@ class Qwen3AttentionCore(PagedAttention):
                 lens_cumulative=True,
                 max_seq_len=context.max_seqlen_k,
                 scale=self.scale,
+                layout=self.kv_layout,
                 new_k=k,
                 new_v=v,
                 new_slots=context.slot_mapping,
                 prologue=pro,
+                k_scale=self.k_scale,
+                v_scale=self.v_scale,
             )
         if self.fuse_prologue:
             # Prefill batches: the varlen launch applies the query prologue.

@@ -25,6 +25,13 @@ LAYOUT_HND = "hnd"  # [pages, Hkv, page_size, D]        (TTS, qwen_tts_outer_pag
 # An FP8 KV pool holds OCP e4m3 codes (torch.float8_e4m3fn); an element's
 # value is code * k_scale (keys) or code * v_scale (values).
 FP8_KV_DTYPE = torch.float8_e4m3fn
+# An MXFP4 KV pool holds 4-bit e2m1 codes, two to a byte (the even element in
+# the low half): a float4_e2m1fn_x2 pool whose last dimension is head_dim / 2.
+# k_scale / v_scale are then float8_e8m0fnu tensors of the pool's shape with a
+# last dimension of head_dim / 32: one power of two per 32 elements of a row.
+MXFP4_KV_DTYPE = torch.float4_e2m1fn_x2
+MXFP4_SCALE_DTYPE = torch.float8_e8m0fnu
+MXFP4_GROUP = 32
 
 
 class AttentionArgumentError(ValueError):
@@ -111,11 +118,71 @@ def kv_pool(k_cache: torch.Tensor, v_cache: torch.Tensor, layout: str = LAYOUT_N
     return pool
 
 
+def mxfp4_kv_pool(num_blocks: int, block_size: int, num_kv_heads: int, head_dim: int, *,
+                  device: torch.device | str, layout: str = LAYOUT_NHD
+                  ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    """An MXFP4 pool of zeros: (k_cache, v_cache, k_scale, v_scale)."""
+    _require(head_dim % MXFP4_GROUP == 0, "head_dim must be a multiple of 32")
+    _require(layout in (LAYOUT_NHD, LAYOUT_HND), f"unknown pool layout {layout!r}")
+    dims = ((num_blocks, block_size, num_kv_heads) if layout == LAYOUT_NHD
+            else (num_blocks, num_kv_heads, block_size))
+
+    def zeros(width: int, dtype: torch.dtype) -> torch.Tensor:
+        return torch.zeros(2, *dims, width, dtype=torch.uint8, device=device).view(dtype)
+
+    codes = zeros(head_dim // 2, MXFP4_KV_DTYPE)
+    scales = zeros(head_dim // MXFP4_GROUP, MXFP4_SCALE_DTYPE)
+    return codes[0], codes[1], scales[0], scales[1]
+
+
+def _mx4_structs(k_cache: torch.Tensor, v_cache: torch.Tensor, layout: str, k_scale, v_scale,
+                 dtype: torch.dtype) -> tuple[N.KvPool, N.Mx4Scales]:
+    """The pool and scale descriptions of an MXFP4 pool that `dtype` rows go
+    to or come from."""
+    _require(k_cache.dtype == MXFP4_KV_DTYPE and v_cache.dtype == MXFP4_KV_DTYPE,
+             f"tensor scales need an MXFP4 (float4_e2m1fn_x2) pool, got {k_cache.dtype}")
+    _require(dtype in (torch.bfloat16, torch.float16), "an MXFP4 pool needs 16-bit rows")
+    _require(isinstance(k_scale, torch.Tensor) and isinstance(v_scale, torch.Tensor)
+             and k_scale.dtype == v_scale.dtype == MXFP4_SCALE_DTYPE,
+             "an MXFP4 pool needs k_scale and v_scale tensors of float8_e8m0fnu")
+    _check_gpu(k_cache, v_cache, k_scale, v_scale)
+    _require(k_cache.dim() == 4, "KV pool must be 4-D")
+    _require(v_cache.shape == k_cache.shape and v_cache.stride() == k_cache.stride(),
+             "key and value pools must have identical shapes and strides")
+    _require(k_scale.shape == k_cache.shape[:3] + (k_cache.shape[3] * 2 // MXFP4_GROUP,)
+             and k_cache.shape[3] * 2 % MXFP4_GROUP == 0,
+             "k_scale must have the pool's shape with a last dimension of head_dim / 32")
+    _require(v_scale.shape == k_scale.shape and v_scale.stride() == k_scale.stride(),
+             "k_scale and v_scale must have identical shapes and strides")
+    _rows(k_cache, "KV pool")
+    _require(k_scale.stride(3) == 1 or k_scale.shape[3] == 1,
+             "k_scale: the last dimension must be contiguous")
+    _require(layout in (LAYOUT_NHD, LAYOUT_HND), f"unknown pool layout {layout!r}")
+    slot, head = (1, 2) if layout == LAYOUT_NHD else (2, 1)
+    pool = N.KvPool(k=k_cache.data_ptr(), v=v_cache.data_ptr(), stride_block=k_cache.stride(0),
+                    stride_slot=k_cache.stride(slot), stride_head=k_cache.stride(head),
+                    block_size=k_cache.shape[slot], num_blocks=k_cache.shape[0],
+                    kv_format=N.VA_KV_MXFP4, k_scale=1.0, v_scale=1.0)
+    scales = N.Mx4Scales(struct_size=ctypes.sizeof(N.Mx4Scales), k=k_scale.data_ptr(),
+                         v=v_scale.data_ptr(), stride_block=k_scale.stride(0),
+                         stride_slot=k_scale.stride(slot), stride_head=k_scale.stride(head))
+    return pool, scales
+
+
+def _mx4_call(name: str, args, scales: N.Mx4Scales, device: torch.device) -> None:
+    """Launch an MXFP4 entry point on the current stream of `device`."""
+    index = _device_index(device)
+    with _current(index):
+        N.check(name, getattr(N.lib(), name)(ctypes.byref(args), ctypes.byref(scales),
+                                             _raw_stream(index)))
+
+
 def pool_heads(k_cache: torch.Tensor, layout: str) -> tuple[int, int]:
     """(num_kv_heads, head_dim) of a pool."""
+    d = int(k_cache.shape[3]) * (2 if k_cache.dtype == MXFP4_KV_DTYPE else 1)
     if layout == LAYOUT_NHD:
-        return int(k_cache.shape[2]), int(k_cache.shape[3])
-    return int(k_cache.shape[1]), int(k_cache.shape[3])
+        return int(k_cache.shape[2]), d
+    return int(k_cache.shape[1]), d
 
 
 # --------------------------------------------------------------------- store
@@ -126,11 +193,15 @@ def store_kvcache(
     v_cache: torch.Tensor,
     slot_mapping: torch.Tensor,
     layout: str = LAYOUT_NHD,
-    k_scale: float = 1.0,
-    v_scale: float = 1.0,
+    k_scale: float | torch.Tensor = 1.0,
+    v_scale: float | torch.Tensor = 1.0,
 ) -> None:
     """Write key[i] / value[i] ([N, Hkv, D]) to pool slot slot_mapping[i]; -1 skips.
-    An FP8 pool receives e4m3 codes of key / k_scale and value / v_scale."""
+    An FP8 pool receives e4m3 codes of key / k_scale and value / v_scale.  An
+    MXFP4 pool receives e2m1 codes, and k_scale / v_scale (its scale tensors)
+    the groups' scales: the smallest power of two 2^e with max |x| < 7 * 2^e."""
+    if isinstance(k_scale, torch.Tensor):
+        return _store_mx4(key, value, k_cache, v_cache, slot_mapping, layout, k_scale, v_scale)
     fast = _FAST if _FAST_LOADED else _fast_calls()
     if fast is not None and layout in (LAYOUT_NHD, LAYOUT_HND):
         index = key.get_device()
@@ -166,6 +237,65 @@ def store_kvcache(
     args.num_kv_heads = hkv
     args.head_dim = d
     N.call("va_store_kvcache", args, device)
+
+
+def _rows_args(args, key, value, pool, slot_mapping, hkv, d):
+    """Fill the fields that the store's and the load's arguments share."""
+    _require(key.dim() == 3 and value.shape == key.shape, "key/value must be [N, Hkv, D]")
+    _rows(key, "key")
+    _rows(value, "value")
+    _require(key.shape[1] == hkv and key.shape[2] == d, "key/value heads must match the pool")
+    _require(key.dtype == value.dtype, "key and value must share a dtype")
+    _require(slot_mapping.dim() == 1 and slot_mapping.numel() == key.shape[0],
+             "slot_mapping must have one entry per token")
+    _require(slot_mapping.is_contiguous(), "slot_mapping must be contiguous")
+    args.dtype = _dtype_code(key)
+    args.key = key.data_ptr()
+    args.value = value.data_ptr()
+    args.key_stride_tok, args.key_stride_head = key.stride(0), key.stride(1)
+    args.value_stride_tok, args.value_stride_head = value.stride(0), value.stride(1)
+    args.pool = pool
+    args.slot_mapping = slot_mapping.data_ptr()
+    args.slot_dtype = _index_code(slot_mapping, "slot_mapping")
+    args.num_tokens = int(key.shape[0])
+    args.num_kv_heads = hkv
+    args.head_dim = d
+    return args
+
+
+def _store_mx4(key, value, k_cache, v_cache, slot_mapping, layout, k_scale, v_scale) -> None:
+    device = _check_gpu(key, value, k_cache, v_cache, slot_mapping)
+    pool, scales = _mx4_structs(k_cache, v_cache, layout, k_scale, v_scale, key.dtype)
+    _check_gpu(key, k_scale)
+    hkv, d = pool_heads(k_cache, layout)
+    args = _rows_args(N.new_args(N.StoreArgs), key, value, pool, slot_mapping, hkv, d)
+    _mx4_call("va_store_kvcache_mx4", args, scales, device)
+
+
+def load_kvcache(
+    k_cache: torch.Tensor,
+    v_cache: torch.Tensor,
+    slot_mapping: torch.Tensor,
+    dtype: torch.dtype = torch.bfloat16,
+    *,
+    layout: str = LAYOUT_NHD,
+    k_scale: torch.Tensor,
+    v_scale: torch.Tensor,
+) -> tuple[torch.Tensor, torch.Tensor]:
+    """The K and V rows [N, Hkv, D] that an MXFP4 pool holds at slot_mapping,
+    as values of `dtype` (exact in the type they were stored from); slots
+    outside the pool read as zeros.  A 16-bit or FP8 pool's rows are read by
+    indexing it."""
+    device = _check_gpu(k_cache, v_cache, slot_mapping, k_scale, v_scale)
+    pool, scales = _mx4_structs(k_cache, v_cache, layout, k_scale, v_scale, dtype)
+    hkv, d = pool_heads(k_cache, layout)
+    _require(slot_mapping.dim() == 1, "slot_mapping must be a vector")
+    shape = (int(slot_mapping.numel()), hkv, d)
+    key = torch.empty(shape, dtype=dtype, device=device)
+    value = torch.empty(shape, dtype=dtype, device=device)
+    args = _rows_args(N.new_args(N.LoadArgs), key, value, pool, slot_mapping, hkv, d)
+    _mx4_call("va_load_kvcache_mx4", args, scales, device)
+    return key, value
 
 
 # ---------------------------------------------------------- q/k prologue
@@ -491,8 +621,8 @@ def paged_decode(
     key_limit: int = 0,
     table_read_width: int = 0,
     no_alloc: bool = False,
-    k_scale: float = 1.0,
-    v_scale: float = 1.0,
+    k_scale: float | torch.Tensor = 1.0,
+    v_scale: float | torch.Tensor = 1.0,
 ) -> torch.Tensor:
     """One-token paged GQA attention.
 
@@ -514,13 +644,17 @@ def paged_decode(
     (on the GPU, outside graph capture; under capture the caller must order
     them).
     An FP8 (float8_e4m3fn) pool is read as code * k_scale / v_scale, and the
-    current row is stored into it quantised.  ``split_tokens``: 0 splits
+    current row is stored into it quantised; so is an MXFP4 pool, with its
+    scale tensors as k_scale / v_scale (16-bit q, head_dim 64 / 128 / 256,
+    groups of 1 / 2 / 4 / 8, blocks of a multiple of 16 tokens, not with
+    ``no_alloc``).  ``split_tokens``: 0 splits
     contexts automatically; ``SPLIT_EXACT`` does too, for a ``max_seq_len``
     that is the batch's exact longest context (partitions fixed from it); a
     positive value fixes the partition size.
     """
+    mx4 = isinstance(k_scale, torch.Tensor)
     fast = _FAST if _FAST_LOADED else _fast_calls()
-    if fast is not None and not no_alloc and layout in (LAYOUT_NHD, LAYOUT_HND):
+    if fast is not None and not no_alloc and not mx4 and layout in (LAYOUT_NHD, LAYOUT_HND):
         index = q.get_device()
         if index >= 0 and index == torch.cuda.current_device():
             if out is None:
@@ -548,6 +682,7 @@ def paged_decode(
         _check_gpu(q, prologue.q_norm_weight, prologue.k_norm_weight, prologue.cos_sin_cache,
                    prologue.positions)
     _require(not no_alloc or out is not None, "no_alloc needs the output tensor (out=...)")
+    _require(not no_alloc or not mx4, "no_alloc takes no MXFP4 pool")
     _require(q.dim() == 3, "q must be [num_seqs, num_heads, head_dim]")
     qs = q.stride()
     _require(qs[2] == 1, "q: the last dimension must be contiguous")
@@ -555,8 +690,13 @@ def paged_decode(
     hkv, pd = pool_heads(k_cache, layout)
     _require(pd == d, f"head_dim mismatch: q {d}, pool {pd}")
     _require(hq % hkv == 0, "num_heads must be a multiple of num_kv_heads")
-    _require(_pool_matches(k_cache, q.dtype),
-             "q and the KV pool must share a dtype (or the pool be FP8 for 16-bit q)")
+    if mx4:
+        pool, scales = _mx4_structs(k_cache, v_cache, layout, k_scale, v_scale, q.dtype)
+        _check_gpu(q, k_scale)
+    else:
+        _require(_pool_matches(k_cache, q.dtype),
+                 "q and the KV pool must share a dtype (or the pool be FP8 for 16-bit q)")
+        pool = _pool_struct(k_cache, v_cache, layout, k_scale, v_scale)
     bts = block_tables.stride()
     _require(block_tables.dim() == 2 and block_tables.shape[0] >= B,
              "block_tables must be [num_seqs, width]")
@@ -574,7 +714,7 @@ def paged_decode(
     fields = dict(
         struct_size=_DECODE_ARGS_SIZE, dtype=_dtype_code(q), q=q.data_ptr(),
         q_stride_seq=qs[0], q_stride_head=qs[1], out=out.data_ptr(), out_stride_seq=os_[0],
-        out_stride_head=os_[1], pool=_pool_struct(k_cache, v_cache, layout, k_scale, v_scale),
+        out_stride_head=os_[1], pool=pool,
         block_tables=block_tables.data_ptr(),
         table_dtype=_index_code(block_tables, "block_tables"), table_stride_seq=bts[0],
         table_width=block_tables.shape[1], lens=lens.data_ptr(),
@@ -617,12 +757,18 @@ def paged_decode(
             N.check("va_paged_decode_noalloc",
                     lib.va_paged_decode_noalloc(ctypes.byref(args), _raw_stream(index)))
             return out
-        nbytes = lib.va_paged_decode_workspace_bytes(ctypes.byref(args))
+        nbytes = (lib.va_paged_decode_mx4_workspace_bytes if mx4
+                  else lib.va_paged_decode_workspace_bytes)(ctypes.byref(args))
         if nbytes:
             ws = decode_workspace(device, nbytes, floor=decode_workspace_bound(device, hq, hkv, d))
             args.workspace = ws.data_ptr()
             args.workspace_bytes = ws.numel()
-        N.check("va_paged_decode", lib.va_paged_decode(ctypes.byref(args), _raw_stream(index)))
+        if mx4:
+            N.check("va_paged_decode_mx4",
+                    lib.va_paged_decode_mx4(ctypes.byref(args), ctypes.byref(scales),
+                                            _raw_stream(index)))
+        else:
+            N.check("va_paged_decode", lib.va_paged_decode(ctypes.byref(args), _raw_stream(index)))
     return out
 
 
@@ -644,8 +790,8 @@ def varlen_attention(
     slot_mapping: torch.Tensor | None = None,
     layout: str = LAYOUT_NHD,
     out: torch.Tensor | None = None,
-    k_scale: float = 1.0,
-    v_scale: float = 1.0,
+    k_scale: float | torch.Tensor = 1.0,
+    v_scale: float | torch.Tensor = 1.0,
     prologue: QKPrologue | None = None,
 ) -> torch.Tensor:
     """Packed variable-length attention (flash_attn_varlen_func semantics).
@@ -661,14 +807,15 @@ def varlen_attention(
     launch's choice of items (the block table may be wider).  An FP8 pool
     (float8_e4m3fn codes, values code * k_scale / v_scale) is converted tile
     by tile inside the kernel (no workspace); its new rows are stored
-    quantised after the attention.  With a ``prologue`` (causal, head_dim
+    quantised after the attention.  So is an MXFP4 pool, with its scale tensors
+    as k_scale / v_scale (blocks of a multiple of 16 tokens).  With a ``prologue`` (causal, head_dim
     128, a 16-bit pool or none), q holds the raw query projections and the
     launch normalises and rotates them at ``prologue.positions`` (one per
     query token); k and the pool must hold processed keys.
     """
     fast = _FAST if _FAST_LOADED else _fast_calls()
     if (fast is not None and prologue is None and layout in (LAYOUT_NHD, LAYOUT_HND) and
-            (k_cache is None or k_cache.dtype != FP8_KV_DTYPE)):
+            (k_cache is None or k_cache.dtype not in (FP8_KV_DTYPE, MXFP4_KV_DTYPE))):
         index = q.get_device()
         if index >= 0 and index == torch.cuda.current_device():
             if out is None:
@@ -695,17 +842,23 @@ def varlen_attention(
              "cu_seqlens must be contiguous")
     num_seqs = cu_seqlens_q.numel() - 1
     fields = {}
+    scales = None  # an MXFP4 pool's
     if k_cache is not None:
         _require(v_cache is not None and block_tables is not None,
                  "a KV pool needs v_cache and block_tables")
         hkv, pd = pool_heads(k_cache, layout)
         _require(pd == d, "pool head_dim must match q")
-        _require(_pool_matches(k_cache, q.dtype),
-                 "pool dtype must match q (or the pool be FP8 for 16-bit q)")
+        if isinstance(k_scale, torch.Tensor):
+            pool, scales = _mx4_structs(k_cache, v_cache, layout, k_scale, v_scale, q.dtype)
+            _check_gpu(q, k_scale)
+        else:
+            _require(_pool_matches(k_cache, q.dtype),
+                     "pool dtype must match q (or the pool be FP8 for 16-bit q)")
+            pool = _pool_struct(k_cache, v_cache, layout, k_scale, v_scale)
         bts = block_tables.stride()
         _require(block_tables.dim() == 2 and block_tables.shape[0] >= num_seqs and bts[1] == 1,
                  "block_tables must be [num_seqs, width]")
-        fields.update(pool=_pool_struct(k_cache, v_cache, layout, k_scale, v_scale),
+        fields.update(pool=pool,
                       block_tables=block_tables.data_ptr(),
                       table_dtype=_index_code(block_tables, "block_tables"),
                       table_stride_seq=bts[0], table_width=block_tables.shape[1])
@@ -760,8 +913,131 @@ def varlen_attention(
                 args.workspace_bytes = nbytes
             except torch.OutOfMemoryError:
                 pass
-        N.check("va_varlen_attention",
-                lib.va_varlen_attention(ctypes.byref(args), _raw_stream(index)))
+        if scales is not None:
+            N.check("va_varlen_attention_mx4",
+                    lib.va_varlen_attention_mx4(ctypes.byref(args), ctypes.byref(scales),
+                                                _raw_stream(index)))
+        else:
+            N.check("va_varlen_attention",
+                    lib.va_varlen_attention(ctypes.byref(args), _raw_stream(index)))
+    return out
+
+
+# ------------------------------------------------------------- step metadata
+@dataclass(frozen=True)
+class BatchMetadata:
+    """A step's attention metadata on the GPU (see :func:`batch_metadata`)."""
+
+    positions: torch.Tensor  # [max_tokens] int64
+    slot_mapping: torch.Tensor  # [max_tokens] int32
+    cu_seqlens_q: torch.Tensor  # [rows + 1] int32
+    cu_seqlens_k: torch.Tensor  # [rows + 1] int32
+    block_tables: torch.Tensor  # [rows, table_width] int32
+    totals: torch.Tensor
+    """[5] int32: tokens, longest query, longest context, free blocks left, blocks missing."""
+
+    @property
+    def free_count(self) -> torch.Tensor:
+        """[1] int32: the free list's count after the step."""
+        return self.totals[3:4]
+
+
+def batch_metadata(
+    lens: torch.Tensor,
+    num_computed: torch.Tensor,
+    request_tables: torch.Tensor,
+    block_size: int,
+    *,
+    max_tokens: int,
+    rows: torch.Tensor | None = None,
+    padded_batch: int = 0,
+    table_width: int | None = None,
+    free_blocks: torch.Tensor | None = None,
+    free_count: torch.Tensor | None = None,
+    out: BatchMetadata | None = None,
+) -> BatchMetadata:
+    """Positions, slots, cumulative lengths and block tables of a step, built
+    on the GPU from the requests' lengths (engine/model_runner.py:183-233,
+    engine/graph_runner.py:150-191 build them on the host).
+
+    Request i has ``num_computed[i]`` tokens behind it and ``lens[i]`` after the
+    step (int32 or int64 [B]); its block table is row ``rows[i]`` (int32; row i
+    without it) of ``request_tables`` ([requests, width] int32).  Its new tokens'
+    positions and slots follow those of the requests before it; entries up to
+    ``max_tokens`` behind the last token are 0 and -1, and tokens past it are
+    not written.  ``block_tables`` row i holds the request's blocks, then -1
+    (``table_width`` columns, request_tables' width by default).  Rows B ..
+    ``padded_batch`` - 1 are a captured decode graph's padding: one token at
+    position 0 with slot -1, table row 0, key length 1.  A row or column outside
+    request_tables, or a negative block id, gives slot -1.
+
+    With ``free_blocks`` ([n] int32) and ``free_count`` ([1] int32), requests
+    hold the blocks of their computed tokens, and the blocks of their new
+    columns are taken from the list's end, in request order: the k-th taken is
+    ``free_blocks[free_count - 1 - k]``.  They are written into request_tables
+    (``rows`` must be distinct); columns that the list does not reach get -1
+    there, and so do their slots.  ``free_count`` itself is not changed: the
+    count left is ``totals[3]`` (``result.free_count``), the blocks that were
+    missing ``totals[4]``.
+
+    ``out``: tensors of an earlier result of the same sizes to write into (a
+    captured graph's static buffers)."""
+    device = _check_gpu(lens, num_computed, request_tables, rows, free_blocks, free_count)
+    _require(lens.dim() == 1 and num_computed.shape == lens.shape and lens.is_contiguous()
+             and num_computed.is_contiguous(), "lens and num_computed must be [B] vectors")
+    _require(lens.dtype == num_computed.dtype, "lens and num_computed must share a dtype")
+    _require(request_tables.dim() == 2 and request_tables.dtype == torch.int32
+             and request_tables.stride(1) == 1, "request_tables must be int32 [requests, width]")
+    _require(block_size > 0, "block_size must be positive")
+    B = int(lens.numel())
+    if rows is not None:
+        _require(rows.dtype == torch.int32 and rows.dim() == 1 and rows.numel() >= B
+                 and rows.is_contiguous(), "rows must be a contiguous int32 [B] vector")
+    _require((free_blocks is None) == (free_count is None),
+             "free_blocks and free_count must be given together")
+    if free_blocks is not None:
+        _require(free_blocks.dtype == torch.int32 and free_blocks.dim() == 1
+                 and free_blocks.is_contiguous(), "free_blocks must be a contiguous int32 vector")
+        _require(free_count.dtype == torch.int32 and free_count.numel() == 1,
+                 "free_count must be one int32")
+    size = max(B, int(padded_batch))
+    width = int(request_tables.shape[1]) if table_width is None else int(table_width)
+    _require(max_tokens >= 0 and width >= 0, "max_tokens and table_width must be non-negative")
+    if out is None:
+        i32 = {"dtype": torch.int32, "device": device}
+        out = BatchMetadata(torch.empty(max_tokens, dtype=torch.int64, device=device),
+                            torch.empty(max_tokens, **i32), torch.empty(size + 1, **i32),
+                            torch.empty(size + 1, **i32), torch.empty(size, width, **i32),
+                            torch.empty(5, **i32))
+    else:
+        _check_gpu(lens, out.positions, out.slot_mapping, out.cu_seqlens_q, out.cu_seqlens_k,
+                   out.block_tables, out.totals)
+        for t, n, dtype in ((out.positions, max_tokens, torch.int64),
+                            (out.slot_mapping, max_tokens, torch.int32),
+                            (out.cu_seqlens_q, size + 1, torch.int32),
+                            (out.cu_seqlens_k, size + 1, torch.int32),
+                            (out.totals, 5, torch.int32)):
+            _require(t.dim() == 1 and t.numel() == n and t.dtype == dtype and t.is_contiguous(),
+                     "out: tensors must have the sizes and types of this call's result")
+        _require(out.block_tables.shape == (size, width) and out.block_tables.dtype == torch.int32
+                 and out.block_tables.stride(1) == 1,
+                 "out: block_tables must be int32 [rows, table_width]")
+    args = N.BatchArgs(
+        struct_size=ctypes.sizeof(N.BatchArgs), index_dtype=_index_code(lens, "lens"),
+        lens=lens.data_ptr(), num_computed=num_computed.data_ptr(),
+        request_tables=request_tables.data_ptr(), request_stride=request_tables.stride(0),
+        num_requests=request_tables.shape[0], request_width=request_tables.shape[1],
+        rows=N.ptr(rows), num_seqs=B, padded_seqs=size, block_size=int(block_size),
+        max_tokens=int(max_tokens), positions=out.positions.data_ptr(),
+        slot_mapping=out.slot_mapping.data_ptr(), cu_seqlens_q=out.cu_seqlens_q.data_ptr(),
+        cu_seqlens_k=out.cu_seqlens_k.data_ptr(), block_tables=out.block_tables.data_ptr(),
+        table_stride=out.block_tables.stride(0), table_width=width,
+        totals=out.totals.data_ptr(), free_blocks=N.ptr(free_blocks), free_count=N.ptr(free_count),
+        free_capacity=0 if free_blocks is None else free_blocks.numel())
+    index = _device_index(device)
+    with _current(index):
+        N.check("va_batch_metadata",
+                N.lib().va_batch_metadata(ctypes.byref(args), _raw_stream(index)))
     return out
 
 
