@@ -1,5 +1,5 @@
-// Host fast path of ops.paged_decode, ops.varlen_attention, ops.store_kvcache
-// and ops.qk_norm_rope.
+// Host fast path of ops.paged_decode, ops.varlen_attention, ops.store_kvcache,
+// ops.qk_norm_rope, ops.load_kvcache and ops.batch_metadata.
 //
 // The Python wrappers validate every argument and fill a ctypes struct on
 // each call, about 10 us of host time, which an eager engine step pays once
@@ -18,6 +18,8 @@
 
 #include <cstdint>
 #include <limits>
+#include <tuple>
+#include <vector>
 
 #include "voiceagent_attn.h"
 
@@ -36,6 +38,19 @@ VarlenFn g_varlen = nullptr;
 VarlenWsFn g_varlen_ws = nullptr;
 StoreFn g_store = nullptr;
 RopeFn g_rope = nullptr;
+
+// The entry points over MXFP4 pools, and the step metadata.
+using StoreMx4Fn = int (*)(const va_store_args*, const va_mx4_scales*, void*);
+using LoadMx4Fn = int (*)(const va_load_args*, const va_mx4_scales*, void*);
+using DecodeMx4Fn = int (*)(const va_decode_args*, const va_mx4_scales*, void*);
+using VarlenMx4Fn = int (*)(const va_varlen_args*, const va_mx4_scales*, void*);
+using BatchFn = int (*)(const va_batch_args*, void*);
+StoreMx4Fn g_store_mx4 = nullptr;
+LoadMx4Fn g_load_mx4 = nullptr;
+DecodeMx4Fn g_decode_mx4 = nullptr;
+DecodeWsFn g_decode_mx4_ws = nullptr;
+VarlenMx4Fn g_varlen_mx4 = nullptr;
+BatchFn g_batch = nullptr;
 
 constexpr int64_t kNotTaken = -1000;
 
@@ -94,6 +109,44 @@ bool fill_pool(const at::Tensor& kc, const at::Tensor& vc, bool hnd, double k_sc
   return true;
 }
 
+// The pool and scale descriptions of _mx4_structs(): an MXFP4 pool (two codes
+// a byte) and its e8m0 scale tensors, of the same geometry.  False when any
+// check fails.
+bool fill_pool_mx4(const at::Tensor& kc, const at::Tensor& vc, const at::Tensor& ks,
+                   const at::Tensor& vs, bool hnd, int64_t device, va_kv_pool* pool,
+                   va_mx4_scales* sc) {
+  if (!on(kc, device) || !on(vc, device) || !on(ks, device) || !on(vs, device)) return false;
+  if (kc.scalar_type() != at::kFloat4_e2m1fn_x2 || vc.scalar_type() != at::kFloat4_e2m1fn_x2 ||
+      ks.scalar_type() != at::kFloat8_e8m0fnu || vs.scalar_type() != at::kFloat8_e8m0fnu)
+    return false;
+  if (kc.dim() != 4 || vc.sizes() != kc.sizes() || vc.strides() != kc.strides() ||
+      kc.stride(3) != 1 || ks.dim() != 4 || vs.sizes() != ks.sizes() ||
+      vs.strides() != ks.strides())
+    return false;
+  const int64_t d = kc.size(3) * 2;
+  if (d % 32 != 0 || ks.size(0) != kc.size(0) || ks.size(1) != kc.size(1) ||
+      ks.size(2) != kc.size(2) || ks.size(3) != d / 32 || (ks.stride(3) != 1 && ks.size(3) != 1))
+    return false;
+  const int slot = hnd ? 2 : 1, head = hnd ? 1 : 2;
+  if (!fits_i32(kc.size(slot)) || !fits_i32(kc.size(0))) return false;
+  pool->k = kc.data_ptr();
+  pool->v = vc.data_ptr();
+  pool->stride_block = kc.stride(0);
+  pool->stride_slot = kc.stride(slot);
+  pool->stride_head = kc.stride(head);
+  pool->block_size = (int32_t)kc.size(slot);
+  pool->num_blocks = (int32_t)kc.size(0);
+  pool->kv_format = VA_KV_MXFP4;
+  pool->k_scale = pool->v_scale = 1.0f;
+  sc->struct_size = sizeof(*sc);
+  sc->k = ks.data_ptr();
+  sc->v = vs.data_ptr();
+  sc->stride_block = ks.stride(0);
+  sc->stride_slot = ks.stride(slot);
+  sc->stride_head = ks.stride(head);
+  return true;
+}
+
 // q's dtype for the pool: the pool's own, or FP8 codes for 16-bit q.
 bool pool_matches(const at::Tensor& pool, c10::ScalarType dt) {
   return pool.scalar_type() == dt ||
@@ -103,6 +156,16 @@ bool pool_matches(const at::Tensor& pool, c10::ScalarType dt) {
 // A contiguous index vector of at least n entries.
 bool index_vector(const at::Tensor& t, int64_t n) {
   return t.dim() == 1 && t.numel() >= n && t.is_contiguous() && index_code(t.scalar_type()) >= 0;
+}
+
+void set_mx4_entries(int64_t store, int64_t load, int64_t decode, int64_t decode_ws,
+                     int64_t varlen, int64_t batch) {
+  g_store_mx4 = reinterpret_cast<StoreMx4Fn>(static_cast<intptr_t>(store));
+  g_load_mx4 = reinterpret_cast<LoadMx4Fn>(static_cast<intptr_t>(load));
+  g_decode_mx4 = reinterpret_cast<DecodeMx4Fn>(static_cast<intptr_t>(decode));
+  g_decode_mx4_ws = reinterpret_cast<DecodeWsFn>(static_cast<intptr_t>(decode_ws));
+  g_varlen_mx4 = reinterpret_cast<VarlenMx4Fn>(static_cast<intptr_t>(varlen));
+  g_batch = reinterpret_cast<BatchFn>(static_cast<intptr_t>(batch));
 }
 
 void set_entries(int64_t decode, int64_t decode_ws, int64_t varlen, int64_t varlen_ws,
@@ -146,7 +209,7 @@ bool fill_prologue(const at::Tensor& qw, const at::Tensor& kw, double eps, const
 // prologue is given by its four tensors and eps, all or none).  0: launched;
 // > 0: workspace bytes needed, nothing launched; VA_ERR_*: the library's
 // status; kNotTaken: nothing done.
-int64_t paged_decode(const at::Tensor& q, const at::Tensor& kc, const at::Tensor& vc,
+int64_t decode_call(const at::Tensor& q, const at::Tensor& kc, const at::Tensor& vc,
                      const at::Tensor& tables, const at::Tensor& lens, const at::Tensor& out,
                      const c10::optional<at::Tensor>& new_k,
                      const c10::optional<at::Tensor>& new_v,
@@ -158,9 +221,12 @@ int64_t paged_decode(const at::Tensor& q, const at::Tensor& kc, const at::Tensor
                      const c10::optional<at::Tensor>& pro_positions,
                      const c10::optional<at::Tensor>& workspace, bool cumulative, bool layout_hnd,
                      int64_t max_seq_len, double scale, int64_t split_tokens, int64_t key_limit,
-                     int64_t table_read_width, double k_scale, double v_scale, int64_t device,
-                     int64_t stream) {
+                     int64_t table_read_width, double k_scale, double v_scale,
+                     const c10::optional<at::Tensor>& k_scales,
+                     const c10::optional<at::Tensor>& v_scales, int64_t device, int64_t stream) {
   if (g_decode == nullptr || g_decode_ws == nullptr) return kNotTaken;
+  const bool mx4 = k_scales.has_value();
+  if (mx4 && (g_decode_mx4 == nullptr || !v_scales.has_value())) return kNotTaken;
   if (!on(q, device) || !on(kc, device) || !on(vc, device) || !on(tables, device) ||
       !on(lens, device) || !on(out, device))
     return kNotTaken;
@@ -168,10 +234,10 @@ int64_t paged_decode(const at::Tensor& q, const at::Tensor& kc, const at::Tensor
   const int64_t B = q.size(0), hq = q.size(1), d = q.size(2);
   if (kc.dim() != 4) return kNotTaken;
   const int64_t hkv = layout_hnd ? kc.size(1) : kc.size(2);
-  if (kc.size(3) != d || hkv <= 0 || hq % hkv != 0) return kNotTaken;
-  if (!pool_matches(kc, q.scalar_type())) return kNotTaken;
+  if (kc.size(3) * (mx4 ? 2 : 1) != d || hkv <= 0 || hq % hkv != 0) return kNotTaken;
+  if (!mx4 && !pool_matches(kc, q.scalar_type())) return kNotTaken;
   const int dt = dtype_code(q.scalar_type());
-  if (dt < 0) return kNotTaken;
+  if (dt < 0 || (mx4 && dt == VA_F32)) return kNotTaken;
   if (tables.dim() != 2 || tables.size(0) < B || tables.stride(1) != 1 ||
       index_code(tables.scalar_type()) < 0)
     return kNotTaken;
@@ -194,7 +260,10 @@ int64_t paged_decode(const at::Tensor& q, const at::Tensor& kc, const at::Tensor
   a.out = out.data_ptr();
   a.out_stride_seq = out.stride(0);
   a.out_stride_head = out.stride(1);
-  if (!fill_pool(kc, vc, layout_hnd, k_scale, v_scale, &a.pool)) return kNotTaken;
+  va_mx4_scales sc{};
+  if (mx4 ? !fill_pool_mx4(kc, vc, *k_scales, *v_scales, layout_hnd, device, &a.pool, &sc)
+          : !fill_pool(kc, vc, layout_hnd, k_scale, v_scale, &a.pool))
+    return kNotTaken;
   a.block_tables = tables.data_ptr();
   a.table_dtype = index_code(tables.scalar_type());
   a.table_stride_seq = tables.stride(0);
@@ -250,7 +319,7 @@ int64_t paged_decode(const at::Tensor& q, const at::Tensor& kc, const at::Tensor
   a.key_limit = (int32_t)key_limit;
   a.table_read_width = (int32_t)table_read_width;
 
-  const size_t need = g_decode_ws(&a);
+  const size_t need = mx4 ? g_decode_mx4_ws(&a) : g_decode_ws(&a);
   if (need > 0) {
     if (!workspace.has_value()) return (int64_t)need;
     const at::Tensor& ws = *workspace;
@@ -259,21 +328,28 @@ int64_t paged_decode(const at::Tensor& q, const at::Tensor& kc, const at::Tensor
     a.workspace = ws.data_ptr();
     a.workspace_bytes = (size_t)ws.numel() * ws.element_size();
   }
-  return g_decode(&a, reinterpret_cast<void*>(static_cast<intptr_t>(stream)));
+  void* const st = reinterpret_cast<void*>(static_cast<intptr_t>(stream));
+  return mx4 ? g_decode_mx4(&a, &sc, st) : g_decode(&a, st);
 }
 
 // ops.varlen_attention over a 16-bit pool or none (an FP8 pool needs a
 // workspace: not taken).  0: launched; VA_ERR_*: the library's status;
 // kNotTaken: nothing done.
-int64_t varlen_attention(const at::Tensor& q, const c10::optional<at::Tensor>& k,
+int64_t varlen_call(const at::Tensor& q, const c10::optional<at::Tensor>& k,
                          const c10::optional<at::Tensor>& v, const at::Tensor& cu_q,
                          const at::Tensor& cu_k, int64_t max_seqlen_q, int64_t max_seqlen_k,
                          double scale, bool causal, const c10::optional<at::Tensor>& k_cache,
                          const c10::optional<at::Tensor>& v_cache,
                          const c10::optional<at::Tensor>& tables,
                          const c10::optional<at::Tensor>& slot_mapping, const at::Tensor& out,
-                         bool layout_hnd, int64_t device, int64_t stream) {
+                         bool layout_hnd, const c10::optional<at::Tensor>& k_scales,
+                         const c10::optional<at::Tensor>& v_scales, int64_t device,
+                         int64_t stream) {
   if (g_varlen == nullptr) return kNotTaken;
+  const bool mx4 = k_scales.has_value();
+  if (mx4 && (g_varlen_mx4 == nullptr || !v_scales.has_value() || !k_cache.has_value()))
+    return kNotTaken;
+  va_mx4_scales sc{};
   if (!on(q, device) || !on(cu_q, device) || !on(cu_k, device) || !on(out, device))
     return kNotTaken;
   if (q.dim() != 3 || q.stride(2) != 1) return kNotTaken;
@@ -296,12 +372,16 @@ int64_t varlen_attention(const at::Tensor& q, const c10::optional<at::Tensor>& k
       return kNotTaken;
     if (kc.dim() != 4) return kNotTaken;
     hkv = layout_hnd ? kc.size(1) : kc.size(2);
-    if (kc.size(3) != d || kc.scalar_type() != q.scalar_type()) return kNotTaken;
+    if (kc.size(3) * (mx4 ? 2 : 1) != d || (!mx4 && kc.scalar_type() != q.scalar_type()) ||
+        (mx4 && dt == VA_F32))
+      return kNotTaken;
     const at::Tensor& t = *tables;
     if (t.dim() != 2 || t.size(0) < num_seqs || t.stride(1) != 1 ||
         index_code(t.scalar_type()) < 0 || !fits_i32(t.size(1)))
       return kNotTaken;
-    if (!fill_pool(kc, *v_cache, layout_hnd, 1.0, 1.0, &a.pool)) return kNotTaken;
+    if (mx4 ? !fill_pool_mx4(kc, *v_cache, *k_scales, *v_scales, layout_hnd, device, &a.pool, &sc)
+            : !fill_pool(kc, *v_cache, layout_hnd, 1.0, 1.0, &a.pool))
+      return kNotTaken;
     a.block_tables = t.data_ptr();
     a.table_dtype = index_code(t.scalar_type());
     a.table_stride_seq = t.stride(0);
@@ -369,7 +449,8 @@ int64_t varlen_attention(const at::Tensor& q, const c10::optional<at::Tensor>& k
     } catch (const c10::OutOfMemoryError&) {
     }
   }
-  return g_varlen(&a, reinterpret_cast<void*>(static_cast<intptr_t>(stream)));
+  void* const st = reinterpret_cast<void*>(static_cast<intptr_t>(stream));
+  return mx4 ? g_varlen_mx4(&a, &sc, st) : g_varlen(&a, st);
 }
 
 // ops.store_kvcache.  0: launched; VA_ERR_*: the library's status;
@@ -409,6 +490,134 @@ int64_t store_kvcache(const at::Tensor& key, const at::Tensor& value, const at::
   a.num_kv_heads = (int32_t)hkv;
   a.head_dim = (int32_t)key.size(2);
   return g_store(&a, reinterpret_cast<void*>(static_cast<intptr_t>(stream)));
+}
+
+// What ops.store_kvcache and ops.load_kvcache share over an MXFP4 pool; false
+// when a check fails.
+template <typename Args>
+bool fill_rows(const at::Tensor& key, const at::Tensor& value, const at::Tensor& kc,
+               const at::Tensor& slots, bool layout_hnd, int64_t device, Args* a) {
+  if (!on(key, device) || !on(value, device) || !on(slots, device)) return false;
+  if (key.dim() != 3 || value.sizes() != key.sizes() || key.stride(2) != 1 ||
+      value.stride(2) != 1 || key.scalar_type() != value.scalar_type())
+    return false;
+  const int dt = dtype_code(key.scalar_type());
+  if (dt != VA_BF16 && dt != VA_F16) return false;
+  const int64_t hkv = layout_hnd ? kc.size(1) : kc.size(2);
+  if (key.size(1) != hkv || key.size(2) != kc.size(3) * 2) return false;
+  if (slots.dim() != 1 || slots.numel() != key.size(0) || !slots.is_contiguous() ||
+      index_code(slots.scalar_type()) < 0 || !fits_i32(key.size(0)) || !fits_i32(hkv) ||
+      !fits_i32(key.size(2)))
+    return false;
+  a->struct_size = sizeof(*a);
+  a->dtype = dt;
+  a->key = key.data_ptr();
+  a->value = value.data_ptr();
+  a->key_stride_tok = key.stride(0);
+  a->key_stride_head = key.stride(1);
+  a->value_stride_tok = value.stride(0);
+  a->value_stride_head = value.stride(1);
+  a->slot_mapping = slots.data_ptr();
+  a->slot_dtype = index_code(slots.scalar_type());
+  a->num_tokens = (int32_t)key.size(0);
+  a->num_kv_heads = (int32_t)hkv;
+  a->head_dim = (int32_t)key.size(2);
+  return true;
+}
+
+// ops.store_kvcache into an MXFP4 pool: as store_kvcache.
+int64_t store_kvcache_mx4(const at::Tensor& key, const at::Tensor& value, const at::Tensor& kc,
+                          const at::Tensor& vc, const at::Tensor& slots, bool layout_hnd,
+                          const at::Tensor& ks, const at::Tensor& vs, int64_t device,
+                          int64_t stream) {
+  if (g_store_mx4 == nullptr) return kNotTaken;
+  va_store_args a{};
+  va_mx4_scales sc{};
+  if (!fill_pool_mx4(kc, vc, ks, vs, layout_hnd, device, &a.pool, &sc) ||
+      !fill_rows(key, value, kc, slots, layout_hnd, device, &a))
+    return kNotTaken;
+  return g_store_mx4(&a, &sc, reinterpret_cast<void*>(static_cast<intptr_t>(stream)));
+}
+
+// ops.load_kvcache: the status and the rows.
+std::tuple<int64_t, at::Tensor, at::Tensor> load_kvcache_mx4(
+    const at::Tensor& kc, const at::Tensor& vc, const at::Tensor& slots, bool half,
+    bool layout_hnd, const at::Tensor& ks, const at::Tensor& vs, int64_t device, int64_t stream) {
+  at::Tensor key, value;
+  va_load_args a{};
+  va_mx4_scales sc{};
+  if (g_load_mx4 == nullptr ||
+      !fill_pool_mx4(kc, vc, ks, vs, layout_hnd, device, &a.pool, &sc) || !on(slots, device))
+    return {kNotTaken, key, value};
+  const auto opts = kc.options().dtype(half ? at::kHalf : at::kBFloat16);
+  const int64_t hkv = layout_hnd ? kc.size(1) : kc.size(2);
+  key = at::empty({slots.numel(), hkv, kc.size(3) * 2}, opts);
+  value = at::empty({slots.numel(), hkv, kc.size(3) * 2}, opts);
+  if (!fill_rows(key, value, kc, slots, layout_hnd, device, &a)) return {kNotTaken, key, value};
+  return {g_load_mx4(&a, &sc, reinterpret_cast<void*>(static_cast<intptr_t>(stream))), key, value};
+}
+
+// ops.batch_metadata without `out`: the status and the result's tensors
+// (positions, slot_mapping, cu_seqlens_q, cu_seqlens_k, block_tables, totals).
+std::tuple<int64_t, std::vector<at::Tensor>> batch_metadata(
+    const at::Tensor& lens, const at::Tensor& done, const at::Tensor& req, int64_t block_size,
+    int64_t max_tokens, const c10::optional<at::Tensor>& rows, int64_t padded, int64_t width,
+    const c10::optional<at::Tensor>& free_blocks, const c10::optional<at::Tensor>& free_count,
+    int64_t device, int64_t stream) {
+  std::vector<at::Tensor> out;
+  const auto no = [&]() { return std::make_tuple(kNotTaken, out); };
+  if (g_batch == nullptr || !on(lens, device) || !on(done, device) || !on(req, device)) return no();
+  if (lens.dim() != 1 || done.sizes() != lens.sizes() || !lens.is_contiguous() ||
+      !done.is_contiguous() || lens.scalar_type() != done.scalar_type() ||
+      index_code(lens.scalar_type()) < 0)
+    return no();
+  if (req.dim() != 2 || req.scalar_type() != at::kInt || req.stride(1) != 1) return no();
+  const int64_t B = lens.numel(), size = padded > B ? padded : B;
+  if (width < 0) width = req.size(1);
+  if (block_size <= 0 || max_tokens < 0 || !fits_i32(size) || !fits_i32(block_size) ||
+      !fits_i32(max_tokens) || !fits_i32(width) || !fits_i32(req.size(0)) || !fits_i32(req.size(1)))
+    return no();
+  if (rows.has_value() && (!on(*rows, device) || rows->scalar_type() != at::kInt ||
+                           rows->dim() != 1 || rows->numel() < B || !rows->is_contiguous()))
+    return no();
+  if (free_blocks.has_value() != free_count.has_value()) return no();
+  va_batch_args a{};
+  if (free_blocks.has_value()) {
+    if (!on(*free_blocks, device) || !on(*free_count, device) ||
+        free_blocks->scalar_type() != at::kInt || free_blocks->dim() != 1 ||
+        !free_blocks->is_contiguous() || !fits_i32(free_blocks->numel()) ||
+        free_count->scalar_type() != at::kInt || free_count->numel() != 1)
+      return no();
+    a.free_blocks = static_cast<const int32_t*>(free_blocks->data_ptr());
+    a.free_count = static_cast<const int32_t*>(free_count->data_ptr());
+    a.free_capacity = (int32_t)free_blocks->numel();
+  }
+  const auto i32 = req.options();
+  out = {at::empty({max_tokens}, i32.dtype(at::kLong)), at::empty({max_tokens}, i32),
+         at::empty({size + 1}, i32), at::empty({size + 1}, i32), at::empty({size, width}, i32),
+         at::empty({5}, i32)};
+  a.struct_size = sizeof(a);
+  a.index_dtype = index_code(lens.scalar_type());
+  a.lens = lens.data_ptr();
+  a.num_computed = done.data_ptr();
+  a.request_tables = static_cast<int32_t*>(req.data_ptr());
+  a.request_stride = req.stride(0);
+  a.num_requests = (int32_t)req.size(0);
+  a.request_width = (int32_t)req.size(1);
+  a.rows = rows.has_value() ? static_cast<const int32_t*>(rows->data_ptr()) : nullptr;
+  a.num_seqs = (int32_t)B;
+  a.padded_seqs = (int32_t)size;
+  a.block_size = (int32_t)block_size;
+  a.max_tokens = (int32_t)max_tokens;
+  a.positions = static_cast<int64_t*>(out[0].data_ptr());
+  a.slot_mapping = static_cast<int32_t*>(out[1].data_ptr());
+  a.cu_seqlens_q = static_cast<int32_t*>(out[2].data_ptr());
+  a.cu_seqlens_k = static_cast<int32_t*>(out[3].data_ptr());
+  a.block_tables = static_cast<int32_t*>(out[4].data_ptr());
+  a.table_stride = width;
+  a.table_width = (int32_t)width;
+  a.totals = static_cast<int32_t*>(out[5].data_ptr());
+  return {g_batch(&a, reinterpret_cast<void*>(static_cast<intptr_t>(stream))), out};
 }
 
 // ops.qk_norm_rope with both outputs given.  0: launched; VA_ERR_*: the
@@ -453,6 +662,55 @@ int64_t qk_norm_rope(const at::Tensor& q, const at::Tensor& k, const at::Tensor&
   return g_rope(&a, reinterpret_cast<void*>(static_cast<intptr_t>(stream)));
 }
 
+// ops.paged_decode over a 16-bit, fp32 or FP8 pool; ..._mx4: with an MXFP4
+// pool's scale tensors.  The same for ops.varlen_attention.
+using Opt = const c10::optional<at::Tensor>&;
+int64_t paged_decode(const at::Tensor& q, const at::Tensor& kc, const at::Tensor& vc,
+                     const at::Tensor& tables, const at::Tensor& lens, const at::Tensor& out,
+                     Opt new_k, Opt new_v, Opt new_slots, Opt valid_mask, Opt pro_q_w,
+                     Opt pro_k_w, double pro_eps, Opt pro_cos_sin, Opt pro_positions,
+                     Opt workspace, bool cumulative, bool layout_hnd, int64_t max_seq_len,
+                     double scale, int64_t split_tokens, int64_t key_limit,
+                     int64_t table_read_width, double k_scale, double v_scale, int64_t device,
+                     int64_t stream) {
+  return decode_call(q, kc, vc, tables, lens, out, new_k, new_v, new_slots, valid_mask, pro_q_w,
+                     pro_k_w, pro_eps, pro_cos_sin, pro_positions, workspace, cumulative,
+                     layout_hnd, max_seq_len, scale, split_tokens, key_limit, table_read_width,
+                     k_scale, v_scale, c10::nullopt, c10::nullopt, device, stream);
+}
+int64_t paged_decode_mx4(const at::Tensor& q, const at::Tensor& kc, const at::Tensor& vc,
+                         const at::Tensor& tables, const at::Tensor& lens, const at::Tensor& out,
+                         Opt new_k, Opt new_v, Opt new_slots, Opt valid_mask, Opt pro_q_w,
+                         Opt pro_k_w, double pro_eps, Opt pro_cos_sin, Opt pro_positions,
+                         Opt workspace, bool cumulative, bool layout_hnd, int64_t max_seq_len,
+                         double scale, int64_t split_tokens, int64_t key_limit,
+                         int64_t table_read_width, const at::Tensor& k_scale,
+                         const at::Tensor& v_scale, int64_t device, int64_t stream) {
+  return decode_call(q, kc, vc, tables, lens, out, new_k, new_v, new_slots, valid_mask, pro_q_w,
+                     pro_k_w, pro_eps, pro_cos_sin, pro_positions, workspace, cumulative,
+                     layout_hnd, max_seq_len, scale, split_tokens, key_limit, table_read_width,
+                     1.0, 1.0, k_scale, v_scale, device, stream);
+}
+int64_t varlen_attention(const at::Tensor& q, Opt k, Opt v, const at::Tensor& cu_q,
+                         const at::Tensor& cu_k, int64_t max_seqlen_q, int64_t max_seqlen_k,
+                         double scale, bool causal, Opt k_cache, Opt v_cache, Opt tables,
+                         Opt slot_mapping, const at::Tensor& out, bool layout_hnd, int64_t device,
+                         int64_t stream) {
+  return varlen_call(q, k, v, cu_q, cu_k, max_seqlen_q, max_seqlen_k, scale, causal, k_cache,
+                     v_cache, tables, slot_mapping, out, layout_hnd, c10::nullopt, c10::nullopt,
+                     device, stream);
+}
+int64_t varlen_attention_mx4(const at::Tensor& q, Opt k, Opt v, const at::Tensor& cu_q,
+                             const at::Tensor& cu_k, int64_t max_seqlen_q, int64_t max_seqlen_k,
+                             double scale, bool causal, Opt k_cache, Opt v_cache, Opt tables,
+                             Opt slot_mapping, const at::Tensor& out, bool layout_hnd,
+                             const at::Tensor& k_scale, const at::Tensor& v_scale, int64_t device,
+                             int64_t stream) {
+  return varlen_call(q, k, v, cu_q, cu_k, max_seqlen_q, max_seqlen_k, scale, causal, k_cache,
+                     v_cache, tables, slot_mapping, out, layout_hnd, k_scale, v_scale, device,
+                     stream);
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_fast_calls, m) {
@@ -463,4 +721,10 @@ PYBIND11_MODULE(_fast_calls, m) {
   m.def("varlen_attention", &varlen_attention);
   m.def("store_kvcache", &store_kvcache);
   m.def("qk_norm_rope", &qk_norm_rope);
+  m.def("set_mx4_entries", &set_mx4_entries);
+  m.def("paged_decode_mx4", &paged_decode_mx4);
+  m.def("varlen_attention_mx4", &varlen_attention_mx4);
+  m.def("store_kvcache_mx4", &store_kvcache_mx4);
+  m.def("load_kvcache_mx4", &load_kvcache_mx4);
+  m.def("batch_metadata", &batch_metadata);
 }

@@ -98,7 +98,8 @@ static int nosplit_tokens_for(const va_decode_args* a) {
 
 // The split of a launch whose workgroups take `unit` tokens a round, with
 // contexts of up to `nosplit` tokens (at 8 partitions a pair) kept whole.
-static DecodePlan plan_split(const va_decode_args* a, int unit, int64_t nosplit) {
+static DecodePlan plan_split(const va_decode_args* a, int unit, int64_t nosplit,
+                             int grain = kDynGrain) {
   DecodePlan pl{};
   const int G = a->num_kv_heads > 0 ? a->num_heads / a->num_kv_heads : 1;
   int max_len = a->max_seq_len > 0 ? a->max_seq_len : 1;
@@ -127,7 +128,7 @@ static DecodePlan plan_split(const va_decode_args* a, int unit, int64_t nosplit)
     int64_t parts = want;
     if (parts > 1 && (int64_t)max_len * (parts < 8 ? parts : 8) <= nosplit * 8)
       parts = 1;
-    const int64_t by_len = (max_len + kDynGrain - 1) / kDynGrain;
+    const int64_t by_len = (max_len + grain - 1) / grain;
     if (parts > by_len) parts = by_len;
     if (parts > kMaxParts) parts = kMaxParts;
     if (parts > 1 && (exact || max_len <= kStaticSplitMax)) {
@@ -189,11 +190,18 @@ static DecodePlan plan_decode(const va_decode_args* a) {
   return plan_split(a, unit > 0 ? unit : 128, nosplit_tokens_for(a));
 }
 
-// MXFP4 pools: contexts of up to this many tokens stay whole.
-constexpr int64_t kMx4NoSplitTokens = 1024;
+// MXFP4 pools: contexts of up to this many tokens (at 8 partitions a pair or
+// more; twice as many at 4, four times at 2) stay whole, and an automatic
+// partition has at least kMx4MinPart tokens, two waves' steps.  16 query / 8 kv
+// heads of 128, whole against split, us: one context of 512 7.9 / 8.0, of 768
+// 9.5 / 8.1; 8 (4 partitions) of 768 9.8 / 10.4, of 1536 13.0 / 12.0; 16 (2) of
+// 1536 13.3 / 14.4, of 4096 34.1 / 26.0.  Partitions of at least 128 tokens took
+// 0.2 us more, of 256 0.9.
+constexpr int64_t kMx4NoSplitTokens = 512;
+constexpr int kMx4MinPart = 64;
 
 static DecodePlan plan_decode_mx4(const va_decode_args* a) {
-  return plan_split(a, 8 * kMx4Step, kMx4NoSplitTokens);
+  return plan_split(a, 8 * kMx4Step, kMx4NoSplitTokens, kMx4MinPart);
 }
 
 template <typename ET>
@@ -506,6 +514,19 @@ int va::paged_decode_impl(const va_decode_args* a, const va_mx4_scales* sc, cons
             : wgs > current_device_cus()      ? 4
             : f8 && pl.wg_tokens <= kWave12Tokens ? 12
                                               : 0;
+  if (mx4) {
+    // Several small workgroups a CU where there are more than CUs (256 x
+    // U[60,600]: 54 us with eight waves, 30 with four, 28 with two, which are
+    // slower for longer contexts), one large one otherwise (32: 8.8 against
+    // 10.6 with four).
+    p.waves = wgs > current_device_cus() ? 4 : 8;
+    p.num_seqs = a->num_seqs;
+    p.min_part = kMx4MinPart;
+    p.hkv_div = make_fastdiv((uint32_t)a->num_kv_heads);
+    p.seq_div = make_fastdiv((uint32_t)a->num_seqs);
+    p.by_token = a->num_kv_heads > 1 && a->pool.stride_head < a->pool.stride_slot &&
+                 wgs + 8 * (int64_t)a->num_kv_heads < INT32_MAX;
+  }
   p.v_scale = f8 ? a->pool.v_scale : 1.0f;
   p.inv_k = f8 ? 1.0f / a->pool.k_scale : 1.0f;
   p.inv_v = f8 ? 1.0f / a->pool.v_scale : 1.0f;

@@ -34,11 +34,24 @@ struct DecodeMx4Params : DecodeParams {
   char* ks;  // scale bytes
   char* vs;
   int64_t sc_blk, sc_slot, sc_head;  // bytes
+  int32_t num_seqs;
+  int32_t by_token;  // the grid keeps a sequence's heads together (see the kernel)
+  FastDiv hkv_div, seq_div;
+  int32_t min_part;  // dyn_split: fewest tokens of a partition
 };
 
 typedef int mx_i32x8 __attribute__((ext_vector_type(8)));
 
 constexpr int kMx4Step = 32;  // tokens a wave reduces at a time: two 16-token tiles
+
+// Tokens of a context partition: fixed, or with dyn_split an even share of the
+// context's L tokens, in whole tiles.
+__device__ inline int mx4_partition(const DecodeMx4Params& p, int L) {
+  if (!p.dyn_split) return p.split_tokens;
+  int P = (L + p.max_parts - 1) / p.max_parts;
+  P = (P + kChunk - 1) / kChunk * kChunk;
+  return P > p.min_part ? P : p.min_part;
+}
 
 // S^T += K Q^T: e2m1 codes of 16 tokens against e4m3 queries.
 __device__ inline mf_f32x4 mx4_qk(uint4 k, int ks, const mx_i32x8& q, int qs, mf_f32x4 c) {
@@ -53,106 +66,350 @@ __device__ inline mf_f32x4 mx4_pv(uint4 v, uint4 p, mf_f32x4 c) {
   return DecodeMma<ET>::qk(v, p, c);
 }
 
-// N e4m3 terms of 16 floats: term t takes what the terms before it left, times
-// 16 each time, so its unit is 2^-4 of the one before.  x is consumed.
-template <int N>
-__device__ inline void mx4_split16(float (&x)[16], uint4 (&term)[N]) {
+// N e4m3 terms of 16 elements of ET (two words of 8), for the power of two
+// `unit`: term 0 rounds x / unit to e4m3, term t what the terms before it left,
+// in units of 2^-4t.  The conversions divide by their scale themselves.
+template <typename ET, int N>
+__device__ inline void mx4_split16(const uint4 (&u)[2], float unit, uint4 (&term)[N]) {
+  typedef short s16x2 __attribute__((ext_vector_type(2)));
+  const uint32_t in[8] = {u[0].x, u[0].y, u[0].z, u[0].w, u[1].x, u[1].y, u[1].z, u[1].w};
+  uint32_t w[4];
 #pragma unroll
-  for (int t = 0; t < N; ++t) {
-    int w[4];
+  for (int i = 0; i < 4; ++i) {
+    s16x2 r = {0, 0};
+    if constexpr (ET::kIsBF16) {
+      r = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(r, __builtin_bit_cast(bf16x2_t, in[2 * i]), unit,
+                                                    false);
+      r = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(r, __builtin_bit_cast(bf16x2_t, in[2 * i + 1]),
+                                                    unit, true);
+    } else {
+      r = __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(r, __builtin_bit_cast(f16x2_t, in[2 * i]), unit,
+                                                   false);
+      r = __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(r, __builtin_bit_cast(f16x2_t, in[2 * i + 1]),
+                                                   unit, true);
+    }
+    w[i] = __builtin_bit_cast(uint32_t, r);
+  }
+  term[0] = make_uint4(w[0], w[1], w[2], w[3]);
+  float x[16];
+  float(&x0)[8] = *reinterpret_cast<float(*)[8]>(&x[0]);
+  float(&x1)[8] = *reinterpret_cast<float(*)[8]>(&x[8]);
+  ET::unpack(u[0], x0);
+  ET::unpack(u[1], x1);
+#pragma unroll
+  for (int t = 1; t < N; ++t) {
+    const float before = t == 1 ? unit : unit * 0.0625f;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      w[i] = __builtin_amdgcn_cvt_pk_fp8_f32(x[4 * i], x[4 * i + 1], 0, false);
-      w[i] = __builtin_amdgcn_cvt_pk_fp8_f32(x[4 * i + 2], x[4 * i + 3], w[i], true);
+      const auto lo = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(w[i], before, false);
+      const auto hi = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(w[i], before, true);
+      x[4 * i] -= lo[0];
+      x[4 * i + 1] -= lo[1];
+      x[4 * i + 2] -= hi[0];
+      x[4 * i + 3] -= hi[1];
+      s16x2 r = {0, 0};
+      r = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(r, x[4 * i], x[4 * i + 1], before * 0.0625f,
+                                                   false);
+      r = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(r, x[4 * i + 2], x[4 * i + 3], before * 0.0625f,
+                                                   true);
+      w[i] = __builtin_bit_cast(uint32_t, r);
     }
     term[t] = make_uint4(w[0], w[1], w[2], w[3]);
-    if (t + 1 < N) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8(w[i], false);
-        const auto hi = __builtin_amdgcn_cvt_pk_f32_fp8(w[i], true);
-        x[4 * i] = (x[4 * i] - lo[0]) * 16.0f;
-        x[4 * i + 1] = (x[4 * i + 1] - lo[1]) * 16.0f;
-        x[4 * i + 2] = (x[4 * i + 2] - hi[0]) * 16.0f;
-        x[4 * i + 3] = (x[4 * i + 3] - hi[1]) * 16.0f;
-      }
-    }
   }
 }
 
 template <int D>
 struct Mx4DecodeShape {
-  static constexpr int ROWB = D / 2;               // bytes of a row's codes
-  static constexpr int NS = D / kMx4Group;         // scales of a row
+  static constexpr int ROWB = D / 2;                 // bytes of a row's codes
+  static constexpr int CPR = ROWB / 16;              // 16-byte chunks of a row
   static constexpr int CH = D <= 128 ? 1 : D / 128;  // 128-element chunks of a row
-  static constexpr int NV = D / 16;                // V elements of a lane and token
+  static constexpr int NV = D / 16;                  // V elements of a lane and token
+  static constexpr int TILE_B = 16 * ROWB;           // codes of a 16-token tile, K or V
+  static constexpr int SCW = D <= 128 ? 4 : 8;       // staged bytes of a row's scales
+  // A stage: K codes of both tiles, V codes, K scales, V scales.
+  static constexpr int V_OFF = 2 * TILE_B, KS_OFF = 4 * TILE_B, VS_OFF = KS_OFF + 32 * SCW;
+  static constexpr int STAGE_B = VS_OFF + 32 * SCW;
+  static constexpr int NDMA = 4 * TILE_B / 1024 + 2 * 32 * SCW / 256;  // requests of a step
   using V = std::conditional_t<D == 64, uint16_t, std::conditional_t<D == 128, uint32_t, uint2>>;
-  using S = std::conditional_t<D == 64, uint16_t, std::conditional_t<D == 128, uint32_t, uint2>>;
 };
 
-// What a lane (r16 = lane % 16, c4 = lane / 16) holds of a step: K codes of
-// token r16 of each tile, their scale, V codes (elements NV r16 ..) of tokens
-// 4 c4 .. 4 c4 + 3 of both tiles, and all scales of token 4 c4 + r16 % 4.
+// LDS place of a staged tile's token and of a row's chunk.  Tokens 4 c + r lie
+// at row 4 r + c, so that the V reads of one r (four rows, each read whole by
+// 16 lanes) are consecutive, and a row's chunks are XORed so that the K reads
+// (one chunk of 16 rows) cover all banks.
+__device__ inline int mx4_slot(int token) { return (token & 3) * 4 + (token >> 2); }
 template <int D>
-struct Mx4Step {
-  using Sh = Mx4DecodeShape<D>;
-  uint4 k[2][Sh::CH];
-  uint32_t ks[2][Sh::CH];
-  typename Sh::V v[2][4];
-  typename Sh::S vs[2];
-  uint32_t mask[2];
-  uint32_t ok;  // bit t: tile t's block is in the pool and it holds tokens (uniform)
-};
+__device__ inline int mx4_swz(int slot) {
+  return (slot / (256 / Mx4DecodeShape<D>::ROWB)) & (Mx4DecodeShape<D>::CPR - 1);
+}
 
-template <typename ET, int D, int G, bool kProlog, bool kMask, int W>
-__global__ __launch_bounds__(W * 64, 2) void paged_decode_mx4_kernel(DecodeMx4Params p) {
+// One 4-byte global -> LDS copy per lane (lane l's word lands at lds + 4 l).
+__device__ inline void dma4(const void* src, uint32_t lds) {
+  asm volatile("s_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(src), "{m0}"(lds) : "memory");
+}
+
+template <typename ET, int D, int G, bool kProlog, bool kMask, int W, int S>
+__global__ __launch_bounds__(W * 64, W == 4 && D <= 128 ? 4 : 2) void paged_decode_mx4_kernel(DecodeMx4Params p) {
   using Sh = Mx4DecodeShape<D>;
   using M = DecodeMma<ET>;
   using VT = typename Sh::V;
-  using ST = typename Sh::S;
-  constexpr int CH = Sh::CH, NV = Sh::NV;
+  constexpr int CH = Sh::CH, NV = Sh::NV, CPR = Sh::CPR, ROWB = Sh::ROWB, SCW = Sh::SCW;
+  constexpr int TILE_B = Sh::TILE_B, STAGE_B = Sh::STAGE_B, NDMA = Sh::NDMA;
   constexpr int NT = W * 64, ROW16 = D * 2;
   constexpr int TERMS = ET::kIsBF16 ? 2 : 3;        // e4m3 terms of a query
   constexpr int QM = D == 64 ? (TERMS + 1) / 2 : TERMS;  // products per chunk (two terms share one at 64)
   constexpr int LPR = D / 8, RPL = 64 / LPR, E = 8;  // the row layout of prologue.h
   constexpr int QROWS = (G + RPL - 1) / RPL;
+  constexpr int LPS = kMx4Group / NV;  // lanes that share a V scale
   static_assert(W % 4 == 0, "the wave merge reads (m, l) of four waves at a time");
 
-  __shared__ __align__(16) float s_o[W * G * D];
-  __shared__ __align__(16) float s_ml[2 * G * W];
+  // The waves' partial results: o [W][G][D], then m and l [G][W]; in LDS of
+  // their own where two workgroups a CU have room for it, else in the ring.
+  constexpr int MERGE_B = W * G * D * 4 + 2 * G * W * 4;
+  constexpr int Q_B = kProlog ? W * (G + 1) * ROW16 : 16;
+  constexpr bool kOwnMerge = W * S * STAGE_B + MERGE_B + Q_B <= (D == 256 ? 80 : W == 4 ? 40 : 160) * 1024;
+  static_assert(kOwnMerge || MERGE_B <= W * S * STAGE_B, "merge scratch");
+  __shared__ __align__(1024) char s_ring[W * S * STAGE_B];
+  __shared__ __align__(16) char s_mrg[kOwnMerge ? MERGE_B : 16];
   // kProlog: each wave's processed query rows and current key row.
-  __shared__ __align__(16) char s_q[kProlog ? W * (G + 1) * ROW16 : 16];
+  __shared__ __align__(16) char s_q[Q_B];
 
-  // Grid (kv head, sequence, partition), as the other decode kernels.
-  const int b = blockIdx.y, h = blockIdx.x, part = blockIdx.z;
+  // Workgroup i runs on XCD i % 8.  Grid (kv head, sequence, partition), as the
+  // other decode kernels', gives each XCD its heads of every sequence.  Where a
+  // token's heads are neighbours (NHD pools), that would have every XCD read
+  // every 128-byte line: a head's 64 bytes of codes are half of one, its 4 bytes
+  // of scales a small part.  There (by_token) the heads of a (sequence,
+  // partition) pair u follow one another on XCD u % 8 (32 contexts of 7000 tokens:
+  // 92 -> 67 us; the requests to HBM then equal an HND pool's).
+  int b = blockIdx.y, h = blockIdx.x, part = blockIdx.z;
+  if (p.by_token) {
+    const uint32_t j = blockIdx.x >> 3, r = fast_div(j, p.hkv_div);
+    const uint32_t u = r * 8 + (blockIdx.x & 7);
+    h = (int)(j - r * p.hkv_div.d);
+    part = (int)fast_div(u, p.seq_div);
+    b = (int)(u - (uint32_t)part * p.seq_div.d);
+    if (part >= p.max_parts) return;
+  }
   const int tid = threadIdx.x;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int lane = tid & 63;
   const int r16 = lane & 15, c4 = lane >> 4;
   const int rg = lane / LPR, col = lane % LPR;
   const int64_t table_row = (int64_t)b * p.t_sb;
+  int P = p.split_tokens;  // a placeholder with dyn_split, fixed below from L
+  int start = part * P;
+  const bool last_part = part == p.max_parts - 1;
 
-  // ---- lengths and the partition ----
+  // ---- independent loads, all requested before the first wait: block ids,
+  // the query, the current row, the mask, the length and the slot ----
+  // Lane l holds tile l % 2 of the wave's step 32 i + l / 2: the block id, from
+  // which its byte offsets are formed 32 steps at a time.
+  const uint32_t* const tabw = reinterpret_cast<const uint32_t*>(p.table);
+  auto tile_tok = [&](int k0) {
+    return start + kMx4Step * (wave + W * (k0 + (lane >> 1))) + 16 * (lane & 1);
+  };
+  uint2 ids = make_uint2(0u, 0u);  // raw words of a block id
+  auto load_ids = [&](int k0, int limit) {
+    const int tok = tile_tok(k0);
+    const int idx = (int)fast_div((uint32_t)tok, p.bs_div);
+    ids = make_uint2(0u, 0u);  // columns past the table read as block 0
+    if (tok < limit && idx < p.table_width) {
+      const int64_t at = (table_row + idx) << p.table_i64;
+      ids.x = tabw[at];
+      ids.y = tabw[at + p.table_i64];
+    }
+  };
+  const bool early = !p.dyn_split;
+  const int early_limit = last_part ? INT32_MAX : start + P;
+  if (early) load_ids(0, early_limit);
+  constexpr int PC = D == 64 ? 1 : 2;  // 16-element pieces of a chunk
+  // Queries in the order of the products' B operand: lane (r16, c4) holds
+  // elements 128 c + 64 f + 16 c4 .. + 15 (f = 0, 1) of head r16; with the
+  // prologue as rows first.
+  uint4 qraw[CH][PC][2];
+  uint4 qrow[QROWS];
+  if constexpr (!kProlog) {
+#pragma unroll
+    for (int c = 0; c < CH; ++c)
+#pragma unroll
+      for (int f = 0; f < PC; ++f)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          // Columns past the group read head 0's row; their scores are unused.
+          const int g = r16 < G ? r16 : 0;
+          qraw[c][f][i] = ld16(p.q + b * p.q_sb + (int64_t)(h * G + g) * p.q_sh +
+                               (128 * c + 64 * f + 16 * c4) * 2 + 16 * i);
+        }
+  } else {
+#pragma unroll
+    for (int i = 0; i < QROWS; ++i) {
+      const int g = rg + RPL * i;
+      qrow[i] = ld16(p.q + b * p.q_sb + (int64_t)(h * G + (g < G ? g : 0)) * p.q_sh + col * 16);
+    }
+  }
+  // key_valid_mask: lane l holds its tile's 16 tokens as bits (the words that
+  // cover its bytes; see paged_decode_mfma.h, which reads them the same way).
+  const int mlen = kMask ? p.valid_len : 0;
+  const uint8_t* const mrow = p.valid + (kMask ? (int64_t)b * p.valid_sb : 0);
+  const int moff = (int)((uintptr_t)mrow & 3);
+  const uint32_t* const mwords = reinterpret_cast<const uint32_t*>(mrow - moff);
+  uint32_t mraw[5] = {~0u, ~0u, ~0u, ~0u, ~0u};
+  int mtb = 0;
+  auto mask_load = [&](int k0) {
+    mtb = tile_tok(k0);
+#pragma unroll
+    for (int j = 0; j < 5; ++j) {
+      const int rb = mtb + 4 * j - moff;
+      mraw[j] = rb < mlen && (j < 4 || moff != 0) ? mwords[(mtb >> 2) + j] : 0xffffffffu;
+    }
+  };
+  auto mask_bits = [&]() -> uint32_t {
+    uint32_t bits = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      uint32_t x = __builtin_amdgcn_alignbyte(mraw[j + 1], mraw[j], (uint32_t)moff);
+      x |= x >> 4;
+      x |= x >> 2;
+      x |= x >> 1;
+      x &= 0x01010101u;
+      bits |= ((x * 0x01020408u) >> 24) << (4 * j);
+    }
+    const int rem = mlen - mtb;
+    if (rem < 16) bits |= rem <= 0 ? 0xffffu : (0xffffu << rem) & 0xffffu;
+    return bits;
+  };
+  uint32_t mbits = 0xffffu;
+  if (kMask && early) mask_load(0);
   const uint32_t* const lensw = reinterpret_cast<const uint32_t*>(p.lens);
   const uint32_t len_hi = lensw[(int64_t)(b + p.lens_cum) << p.lens_i64];
   const uint32_t len_lo = lensw[(int64_t)b << p.lens_i64];
+  uint32_t slot_lo = ~0u, slot_hi = ~0u;  // new_slots[b] (-1 without one)
+  if (p.new_slots != nullptr) {
+    const uint32_t* const sw = reinterpret_cast<const uint32_t*>(p.new_slots);
+    slot_lo = sw[(int64_t)b << p.new_slots_i64];
+    slot_hi = sw[((int64_t)b << p.new_slots_i64) + p.new_slots_i64];
+  }
+
+  // ---- the wave's ring: S stages of a step each, filled by DMA ----
+  char* const s_wave = s_ring + wave * S * STAGE_B;
+  const uint32_t lds_wave = __builtin_amdgcn_readfirstlane(
+      (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)s_wave);
+  // Codes: request i of a tile fills LDS rows i RPI ..; lane l's chunk is
+  // position l % CPR of row i RPI + l / CPR.  At head_dim 64 one request takes
+  // both tiles, 32 lanes each.
+  constexpr int RPI = 64 / CPR, NI = TILE_B >= 1024 ? TILE_B / 1024 : 1;
+  uint32_t loff[NI];
+#pragma unroll
+  for (int i = 0; i < NI; ++i) {
+    const int slot = (i * RPI + lane / CPR) & 15, pos = lane % CPR;
+    const int token = (slot & 3) * 4 + (slot >> 2);
+    loff[i] = (uint32_t)(token * (int)p.s_slot) + (uint32_t)((pos ^ mx4_swz<D>(slot)) << 4);
+  }
+  const int64_t head_off = (int64_t)h * p.s_head, head_sc = (int64_t)h * p.sc_head;
+  int64_t toff = head_off, tsc = head_sc;  // of the lane's tile (block 0 where there is none)
+  uint64_t tiles_ok = 0;                   // bit l: lane l's tile has a block of the pool
+  auto take_ids = [&](int k0) {
+    const int64_t bid = p.table_i64 ? (int64_t)(((uint64_t)ids.y << 32) | ids.x)
+                                    : (int64_t)(int32_t)ids.x;
+    const bool ok = bid >= 0 && bid < p.num_blocks;
+    const int in = ok ? (int)fast_mod((uint32_t)tile_tok(k0), p.bs_div) : 0;
+    toff = (ok ? bid : 0) * p.s_blk + (int64_t)in * p.s_slot + head_off;
+    tsc = (ok ? bid : 0) * p.sc_blk + (int64_t)in * p.sc_slot + head_sc;
+    tiles_ok = __builtin_amdgcn_ballot_w64(ok);
+  };
+  auto lane64 = [&](int64_t x, int l) -> int64_t {
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)x, l);
+    const uint32_t hi = (uint32_t)__builtin_amdgcn_readlane((int)(x >> 32), l);
+    return (int64_t)(((uint64_t)hi << 32) | lo);
+  };
+  // Requests step k (of the 32 whose offsets the lanes hold) into stage k % S.
+  auto issue = [&](int k) {
+    const uint32_t dst = lds_wave + (uint32_t)((k % S) * STAGE_B);
+    const int l = 2 * (k & 31);
+    const int64_t o0 = lane64(toff, l), o1 = lane64(toff, l + 1);
+    const int64_t c0 = lane64(tsc, l), c1 = lane64(tsc, l + 1);
+    if constexpr (D == 64) {
+      const int64_t o = (lane < 32 ? o0 : o1) + loff[0];
+      dma16_nt(p.kp + o, dst);
+      dma16_nt(p.vp + o, dst + Sh::V_OFF);
+    } else {
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        const char* const kb = uniform_ptr(p.kp + (t ? o1 : o0));
+        const char* const vb = uniform_ptr(p.vp + (t ? o1 : o0));
+#pragma unroll
+        for (int i = 0; i < NI; ++i) {
+          // Lines that other heads share stay in L2; others stream past it (32
+          // contexts of 7000, us: NHD 66.9 / 69.6, HND 55.9 / 52.0 without / with nt).
+          if (p.by_token) {
+            dma16(loff[i], kb, dst + t * TILE_B + i * 1024);
+            dma16(loff[i], vb, dst + Sh::V_OFF + t * TILE_B + i * 1024);
+          } else {
+            dma16_nt(loff[i], kb, dst + t * TILE_B + i * 1024);
+            dma16_nt(loff[i], vb, dst + Sh::V_OFF + t * TILE_B + i * 1024);
+          }
+        }
+      }
+    }
+    // Scales, a word a lane: at head_dim 64 the aligned word that holds the
+    // row's two.
+    if constexpr (D <= 128) {
+      const char* src = (lane < 32 ? p.ks : p.vs) + ((lane & 16) ? c1 : c0) +
+                        (int64_t)r16 * p.sc_slot;
+      if constexpr (D == 64) src = (const char*)((uintptr_t)src & ~(uintptr_t)3);
+      dma4(src, dst + Sh::KS_OFF);
+    } else {
+      const int64_t at = (lane < 32 ? c0 : c1) + (int64_t)((lane >> 1) & 15) * p.sc_slot + (lane & 1) * 4;
+      dma4(p.ks + at, dst + Sh::KS_OFF);
+      dma4(p.vs + at, dst + Sh::VS_OFF);
+    }
+  };
+
+  // With fixed partitions the first steps are requested before the length is
+  // known, once what was loaded above is there (a wait left to a first use
+  // behind the DMA would wait for the DMA too).  Tokens past the context are
+  // masked.
+  if (early) {
+    asm volatile("" ::"v"(ids.x), "v"(ids.y));
+    take_ids(0);
+    if constexpr (!kProlog) {
+#pragma unroll
+      for (int c = 0; c < CH; ++c)
+#pragma unroll
+        for (int f = 0; f < PC; ++f)
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+            asm volatile("" ::"v"(qraw[c][f][i].x), "v"(qraw[c][f][i].y), "v"(qraw[c][f][i].z),
+                         "v"(qraw[c][f][i].w));
+    }
+    if constexpr (kMask)
+      asm volatile("" ::"v"(mraw[0]), "v"(mraw[1]), "v"(mraw[2]), "v"(mraw[3]), "v"(mraw[4]));
+    if (p.num_blocks > 0)
+      for (int k = 0; k < S; ++k)
+        if (last_part || (wave + W * k) * kMx4Step < P) issue(k);
+  }
+
+  // ---- the length and the partition ----
   int L = __builtin_amdgcn_readfirstlane((int)(p.lens_cum ? len_hi - len_lo : len_lo));
   const int Lr = L;
   L = attend_len(p, L);
   if (p.num_blocks <= 0) L = 0;
   const int col_new = Lr >= 1 ? (int)fast_div((uint32_t)(Lr - 1), p.bs_div) : 0;
   const bool detached = current_row_detached(p, Lr, L, col_new);
-  int64_t new_slot = -1;
-  if (p.new_slots != nullptr) new_slot = load_index(p.new_slots, b, p.new_slots_i64);
-  const int P = partition_tokens(p, L > 0 ? L : 1);
-  const int start = part * P;
-  const bool last_part = part == p.max_parts - 1;
+  const int64_t new_slot = p.new_slots_i64 ? (int64_t)(((uint64_t)slot_hi << 32) | slot_lo)
+                                           : (int64_t)(int32_t)slot_lo;
+  if (p.dyn_split) {
+    P = mx4_partition(p, L > 0 ? L : 1);
+    start = part * P;
+  }
   const int end = L <= 0 ? 0 : (last_part ? L : min(start + P, L));
   const bool writes_row = detached && part == 0;  // this workgroup writes the detached row
-  if (start >= L && !writes_row && !(part == 0 && L <= 0)) return;
+  if (start >= L && !writes_row && !(part == 0 && L <= 0)) {
+    wait_vmcnt<0>();  // early steps land before the workgroup's LDS is released
+    return;
+  }
   int nparts = L > 0 ? (L + P - 1) / P : 1;
   if (nparts > p.max_parts) nparts = p.max_parts;  // the last partition absorbs the rest
-
   const int nsteps = end > start ? (end - start + kMx4Step - 1) / kMx4Step : 0;
   const int ntw = nsteps > wave ? (nsteps - wave + W - 1) / W : 0;  // steps of this wave
   const int new_tok =
@@ -160,106 +417,27 @@ __global__ __launch_bounds__(W * 64, 2) void paged_decode_mx4_kernel(DecodeMx4Pa
   const int new_step = new_tok >= 0 ? (new_tok - start) / kMx4Step : -1;
   const bool owns_new = new_step >= 0 && new_step % W == wave;
   const int64_t cap = (int64_t)p.num_blocks * p.block_size;
-
-  // ---- block ids: lane l holds tile l % 2 of the wave's step 32 i + l / 2,
-  // turned into the tile's byte offsets 32 steps at a time; the ids of the
-  // next 32 steps are requested then ----
-  const int64_t head_off = (int64_t)h * p.s_head, head_sc = (int64_t)h * p.sc_head;
-  auto tile_tok = [&](int k0) { return start + kMx4Step * (wave + W * (k0 + (lane >> 1))) + 16 * (lane & 1); };
-  auto load_ids = [&](int k0) -> int {
-    const int tok = tile_tok(k0);
-    if (tok >= end) return -1;
-    const int idx = (int)fast_div((uint32_t)tok, p.bs_div);
-    if (idx >= p.table_width) return 0;
-    // Both words of a 64-bit id (the same word twice of a 32-bit one).
-    const int32_t* const w = reinterpret_cast<const int32_t*>(p.table) + ((table_row + idx) << p.table_i64);
-    const int lo = w[0], hi = w[p.table_i64];
-    return p.table_i64 && hi != 0 ? -1 : lo;
-  };
-  int64_t toff = 0, tsc = 0;
-  uint64_t tok_ok = 0;
-  auto take_ids = [&](int k0, int blk) {
-    const bool ok = blk >= 0 && blk < p.num_blocks;
-    const int64_t bl = ok ? blk : 0;  // tiles without a block read block 0 and are masked
-    const int in = ok ? (int)fast_mod((uint32_t)tile_tok(k0), p.bs_div) : 0;
-    toff = bl * p.s_blk + (int64_t)in * p.s_slot + head_off;
-    tsc = bl * p.sc_blk + (int64_t)in * p.sc_slot + head_sc;
-    tok_ok = __builtin_amdgcn_ballot_w64(ok);
-  };
-  int ids = -1;
-  if (ntw > 0) {
-    ids = load_ids(0);
-    take_ids(0, ids);
-    if (ntw > 32) ids = load_ids(32);
-  }
-
-  // ---- a step's loads ----
-  const uint32_t k_lane = (uint32_t)(r16 * (int)p.s_slot + (D == 64 ? (c4 & 1) : c4) * 16);
-  const uint32_t ks_lane = (uint32_t)(r16 * (int)p.sc_slot + (D == 64 ? (c4 & 1) : c4));
-  const uint32_t v_lane = (uint32_t)(4 * c4 * (int)p.s_slot + r16 * (NV / 2));
-  const uint32_t vs_lane = (uint32_t)((4 * c4 + (r16 & 3)) * (int)p.sc_slot);
-  auto lane64 = [&](int64_t x, int l) -> int64_t {
-    const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)x, l);
-    const uint32_t hi = (uint32_t)__builtin_amdgcn_readlane((int)(x >> 32), l);
-    return (int64_t)(((uint64_t)hi << 32) | lo);
-  };
-  const uint8_t* const mrow = p.valid + (kMask ? (int64_t)b * p.valid_sb : 0);
-  auto load = [&](Mx4Step<D>& s, int k) {
-    if (k > 0 && (k & 31) == 0) {
-      take_ids(k, ids);
-      if (k + 32 < ntw) ids = load_ids(k + 32);
-    }
-    s.ok = (uint32_t)(tok_ok >> (2 * (k & 31))) & 3u;
-#pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      const int l = 2 * (k & 31) + t;
-      const int64_t off = lane64(toff, l), sc = lane64(tsc, l);
-      const char* const kb = p.kp + off;
-      const char* const vb = p.vp + off;
-      const char* const ksb = p.ks + sc;
-      const char* const vsb = p.vs + sc;
-#pragma unroll
-      for (int c = 0; c < CH; ++c) {
-        s.k[t][c] = *reinterpret_cast<const uint4*>(kb + (k_lane + 64u * c));
-        s.ks[t][c] = *reinterpret_cast<const uint8_t*>(ksb + (ks_lane + 4u * c));
-      }
-      s.vs[t] = *reinterpret_cast<const ST*>(vsb + vs_lane);
-#pragma unroll
-      for (int r = 0; r < 4; ++r)
-        s.v[t][r] = *reinterpret_cast<const VT*>(vb + r * p.s_slot + v_lane);
-      if constexpr (kMask) {
-        const int tok = start + kMx4Step * (wave + W * k) + 16 * t + 4 * c4 + (r16 & 3);
-        s.mask[t] = tok < p.valid_len && tok < end ? mrow[tok] : 1u;
-      }
-    }
-  };
-
-  // ---- queries: 16-element pieces of row r16 in the order of the products'
-  // B operand (lane (r16, c4): elements 128 c + 64 f + 16 c4 .. + 15, f = 0, 1) ----
-  constexpr int PC = D == 64 ? 1 : 2;  // pieces per chunk
-  uint4 qraw[CH][PC][2];
-  float pro_c[E], pro_s[E];
   const bool has_new = p.new_k != nullptr && (owns_new || (writes_row && wave == 0));
-  if constexpr (!kProlog) {
-#pragma unroll
-    for (int c = 0; c < CH; ++c)
-#pragma unroll
-      for (int f = 0; f < PC; ++f)
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-          qraw[c][f][i] = r16 < G ? ld16(p.q + b * p.q_sb + (int64_t)(h * G + r16) * p.q_sh +
-                                         (128 * c + 64 * f + 16 * c4) * 2 + 16 * i)
-                                  : make_uint4(0, 0, 0, 0);
+  if (!early && ntw > 0) {
+    load_ids(0, end);
+    if (kMask) mask_load(0);
+    asm volatile("" ::"v"(ids.x), "v"(ids.y));
+    if constexpr (kMask)
+      asm volatile("" ::"v"(mraw[0]), "v"(mraw[1]), "v"(mraw[2]), "v"(mraw[3]), "v"(mraw[4]));
+    take_ids(0);
+    for (int k = 0; k < S; ++k)
+      if (k < ntw) issue(k);
   }
-
-  Mx4Step<D> s0, s1;
-  if (ntw > 0) load(s0, 0);
-  if (ntw > 1) load(s1, 1);
+  if (kMask) mbits = mask_bits();
+  uint32_t mbits_k = mbits;   // of the step being reduced; the others are of the step requested
+  uint64_t tiles_ok_k = tiles_ok;
+  uint32_t tsc_k = (uint32_t)tsc;
 
   if constexpr (kProlog) {
     // Rows in the row layout, then through LDS (the wave's own part of it).
     int64_t pos = load_index(p.pro.pos, b, p.pro.pos_i64);
     pos = pos < 0 ? 0 : (pos >= p.pro.max_pos ? p.pro.max_pos - 1 : pos);
+    float pro_c[E], pro_s[E];
     load_rotary<E, LPR>(p.pro, pos, col, D, pro_c, pro_s);
     char* const s_w = s_q + wave * (G + 1) * ROW16;
     float w[E], x[E];
@@ -267,9 +445,7 @@ __global__ __launch_bounds__(W * 64, 2) void paged_decode_mx4_kernel(DecodeMx4Pa
 #pragma unroll
     for (int i = 0; i < QROWS; ++i) {
       const int g = rg + RPL * i;
-      const uint4 u = g < G ? ld16(p.q + b * p.q_sb + (int64_t)(h * G + g) * p.q_sh + col * 16)
-                            : make_uint4(0, 0, 0, 0);
-      ET::unpack(u, x);
+      ET::unpack(qrow[i], x);
       qk_prologue<ET, LPR, E>(x, w, p.pro.eps, D, pro_c, pro_s);
       if (g < G) st16(s_w + g * ROW16 + col * 16, ET::pack(x));
     }
@@ -279,19 +455,15 @@ __global__ __launch_bounds__(W * 64, 2) void paged_decode_mx4_kernel(DecodeMx4Pa
       qk_prologue<ET, LPR, E>(x, w, p.pro.eps, D, pro_c, pro_s);
       if (rg == 0) st16(s_w + G * ROW16 + col * 16, ET::pack(x));
     }
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
     __builtin_amdgcn_wave_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 #pragma unroll
     for (int c = 0; c < CH; ++c)
 #pragma unroll
       for (int f = 0; f < PC; ++f)
 #pragma unroll
         for (int i = 0; i < 2; ++i)
-          qraw[c][f][i] =
-              r16 < G ? *reinterpret_cast<const uint4*>(s_w + r16 * ROW16 +
-                                                        (128 * c + 64 * f + 16 * c4) * 2 + 16 * i)
-                      : make_uint4(0, 0, 0, 0);
+          qraw[c][f][i] = *reinterpret_cast<const uint4*>(s_w + (r16 < G ? r16 : 0) * ROW16 +
+                                                          (128 * c + 64 * f + 16 * c4) * 2 + 16 * i);
   }
 
   // ---- the current row, quantised: lane (., c4) the K group its step
@@ -393,9 +565,13 @@ __global__ __launch_bounds__(W * 64, 2) void paged_decode_mx4_kernel(DecodeMx4Pa
         st16(p.out + b * p.o_sb + (int64_t)(h * G + g) * p.o_sh + d * 2, make_uint4(0, 0, 0, 0));
       }
     }
+    wait_vmcnt<0>();
     return;
   }
-  if (start >= L) return;
+  if (start >= L) {
+    wait_vmcnt<0>();
+    return;
+  }
 
   // ---- the queries' e4m3 terms: the row's largest magnitude goes to
   // [2^7, 2^8), so a term's unit is at most 2^-9 of it ----
@@ -423,21 +599,14 @@ __global__ __launch_bounds__(W * 64, 2) void paged_decode_mx4_kernel(DecodeMx4Pa
     // row with an infinity or a NaN scores NaN.
     int e = (int)(bits >> 23) - 7;
     e = e < 27 ? 27 : e;
-    const float inv = __uint_as_float((uint32_t)(254 - e) << 23);
+    const float unit = __uint_as_float((uint32_t)e << 23);
     const bool bad = bits >= 0x7f800000u;
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
       uint4 term[PC][TERMS];
 #pragma unroll
       for (int f = 0; f < PC; ++f) {
-        float x[16];
-        float(&x0)[8] = *reinterpret_cast<float(*)[8]>(&x[0]);
-        float(&x1)[8] = *reinterpret_cast<float(*)[8]>(&x[8]);
-        ET::unpack(qraw[c][f][0], x0);
-        ET::unpack(qraw[c][f][1], x1);
-#pragma unroll
-        for (int i = 0; i < 16; ++i) x[i] *= inv;
-        mx4_split16<TERMS>(x, term[f]);
+        mx4_split16<ET, TERMS>(qraw[c][f], unit, term[f]);
       }
       auto join = [](uint4 lo, uint4 hi) {
         return mx_i32x8{(int)lo.x, (int)lo.y, (int)lo.z, (int)lo.w,
@@ -464,51 +633,131 @@ __global__ __launch_bounds__(W * 64, 2) void paged_decode_mx4_kernel(DecodeMx4Pa
 #pragma unroll
   for (int i = 0; i < NV; ++i) o[i] = mf_f32x4{0.f, 0.f, 0.f, 0.f};
 
-  auto reduce = [&](Mx4Step<D>& s, int k) {
+  // Byte offsets of the lane's reads inside a stage.
+  const int kslot = mx4_slot(r16);
+  const int koff = kslot * ROWB + (((D == 64 ? c4 & 1 : c4) ^ mx4_swz<D>(kslot)) << 4);
+  const int ksoff = Sh::KS_OFF + r16 * SCW + (D == 64 ? c4 & 1 : c4);
+  int voff[4];  // of token 4 c4 + i
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int slot = 4 * i + c4, byte = r16 * (NV / 2);
+    voff[i] = Sh::V_OFF + slot * ROWB + (((byte >> 4) ^ mx4_swz<D>(slot)) << 4) + (byte & 15);
+  }
+  const int vsoff = Sh::VS_OFF + 4 * c4 * SCW + r16 / LPS;
+
+  for (int k = 0; k < ntw; ++k) {
+    if (k + S - 1 < ntw)
+      wait_vmcnt<NDMA*(S - 1)>();  // the steps after it may stay in flight
+    else
+      wait_vmcnt<0>();
+    if (k > 0 && (k & 31) == 0) {
+      tiles_ok_k = tiles_ok;
+      mbits_k = mbits;
+      tsc_k = (uint32_t)tsc;
+    }
+    char* const st = s_wave + (k % S) * STAGE_B;
     const int c = wave + W * k;
     const int tb = start + kMx4Step * c;
+    uint32_t tpar[2] = {0u, 0u};
+    if constexpr (D == 64) {
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+        tpar[t] = (uint32_t)__builtin_amdgcn_readlane((int)tsc_k, 2 * (k & 31) + t);
+    }
+    // Byte offset (0 or 2) of row `row`'s scales in its staged word.
+    auto half = [&](int t, const char* base, int row) -> int {
+      return D == 64 ? (int)((uint32_t)(uintptr_t)base + tpar[t] + (uint32_t)(row * (int)p.sc_slot)) & 2 : 0;
+    };
     if (c == new_step && dst_off != INT64_MIN) {
       // The current row in place of the pool's.
-      const int r = new_tok - tb;
+      const int t = (new_tok - tb) >> 4, r = (new_tok - tb) & 15, slot = mx4_slot(r);
+      if (r16 == 0 && (D > 64 || c4 < 2)) {
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        if (r16 == r - 16 * t) {
-#pragma unroll
-          for (int cc = 0; cc < CH; ++cc) {
-            s.k[t][cc] = kq[cc];
-            s.ks[t][cc] = kqs[cc];
-          }
+        for (int cc = 0; cc < CH; ++cc) {
+          *reinterpret_cast<uint4*>(st + t * TILE_B + slot * ROWB +
+                                    (((4 * cc + c4) ^ mx4_swz<D>(slot)) << 4)) = kq[cc];
+          st[Sh::KS_OFF + (t * 16 + r) * SCW + half(t, p.ks, r) + 4 * cc + c4] = (char)kqs[cc];
         }
-        const int j = r - 16 * t - 4 * c4;  // the lane's token, when 0 .. 3
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (j == i) s.v[t][i] = vq;
       }
+      if (c4 == 0) {
+        const int byte = r16 * (NV / 2);
+        *reinterpret_cast<VT*>(st + Sh::V_OFF + t * TILE_B + slot * ROWB +
+                               (((byte >> 4) ^ mx4_swz<D>(slot)) << 4) + (byte & 15)) = vq;
+        if (r16 % LPS == 0)
+          st[Sh::VS_OFF + (t * 16 + r) * SCW + half(t, p.vs, r) + r16 / LPS] = (char)vqs;
+      }
+      __builtin_amdgcn_wave_barrier();
     }
     // S^T: the lane's scores are tokens 4 c4 + i of both tiles, head r16.
+    uint4 kk[2][CH];
+    uint32_t kks[2][CH];
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int cc = 0; cc < CH; ++cc) {
+        // (a row's chunks 4 .. 7 are its chunks 0 .. 3 with the third bit flipped)
+        kk[t][cc] = *reinterpret_cast<const uint4*>(st + t * TILE_B + (koff ^ (cc << 6)));
+        kks[t][cc] = (uint8_t)st[ksoff + t * 16 * SCW + 4 * cc + half(t, p.ks, r16)];
+      }
+    VT vv[8];
+    uint32_t vb[8];
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        vv[4 * t + i] = *reinterpret_cast<const VT*>(st + t * TILE_B + voff[i]);
+        vb[4 * t + i] = (uint8_t)st[vsoff + (t * 16 + i) * SCW + half(t, p.vs, 4 * c4 + i)];
+      }
     mf_f32x4 sc[2];
-    uint32_t live[2];
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
       sc[t] = mf_f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int cc = 0; cc < CH; ++cc)
 #pragma unroll
-        for (int q = 0; q < QM; ++q) sc[t] = mx4_qk(s.k[t][cc], s.ks[t][cc], qf[q][cc], qs[q], sc[t]);
-      const int rel = (s.ok >> t) & 1u ? end - tb - 16 * t - 4 * c4 : 0;
-      live[t] = rel >= 4 ? 15u : (rel <= 0 ? 0u : (1u << rel) - 1u);
-      if constexpr (kMask)  // lane (i, c4) holds token 4 c4 + i's byte
-        live[t] &= (uint32_t)(__builtin_amdgcn_ballot_w64(s.mask[t] != 0) >> (16 * c4));
+        for (int q = 0; q < QM; ++q) sc[t] = mx4_qk(kk[t][cc], kks[t][cc], qf[q][cc], qs[q], sc[t]);
+    }
+    // The stage has been read: it takes the wave's step k + S.
+    wait_lgkmcnt0();
+    if (k + S < ntw) {
+      const int n = k + S;
+      if ((n & 31) == 0) {
+        // The offsets of the next 32 steps.
+        load_ids(n, end);
+        if (kMask) mask_load(n);
+        asm volatile("" ::"v"(ids.x), "v"(ids.y));
+        take_ids(n);
+        if (kMask) mbits = mask_bits();
+      }
+      issue(n);
     }
     float sv[8];
-    float mx = -INFINITY;
 #pragma unroll
     for (int t = 0; t < 2; ++t)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        sv[4 * t + i] = (live[t] >> i) & 1u ? sc[t][i] : -INFINITY;
-        mx = fmaxf(mx, sv[4 * t + i]);
+      for (int i = 0; i < 4; ++i) sv[4 * t + i] = sc[t][i];
+    const uint32_t ok = (uint32_t)(tiles_ok_k >> (2 * (k & 31))) & 3u;
+    if (kMask || ok != 3u || end - tb < kMx4Step) {
+      // Tokens that are not attended: their scores are -inf, and their V
+      // scales 0, so that nothing their rows may hold (a NaN scale) meets
+      // their P of 0.
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        const int rel = (ok >> t) & 1u ? end - tb - 16 * t - 4 * c4 : 0;
+        uint32_t live = rel >= 4 ? 15u : (rel <= 0 ? 0u : (1u << rel) - 1u);
+        if constexpr (kMask)
+          live &= (uint32_t)__builtin_amdgcn_readlane((int)mbits_k, 2 * (k & 31) + t) >> (4 * c4);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const bool on = (live >> i) & 1u;
+          sv[4 * t + i] = on ? sv[4 * t + i] : -INFINITY;
+          vb[4 * t + i] = on ? vb[4 * t + i] : 0u;
+        }
       }
+    }
+    float mx = sv[0];
+#pragma unroll
+    for (int i = 1; i < 8; ++i) mx = fmaxf(mx, sv[i]);
     mx = max_xor16(mx);
     mx = max_xor32(mx);
     const float mxs = mx * p.scale_log2;
@@ -528,43 +777,8 @@ __global__ __launch_bounds__(W * 64, 2) void paged_decode_mx4_kernel(DecodeMx4Pa
     }
     const uint4 pb = make_uint4(M::pack2(pr[0], pr[1]), M::pack2(pr[2], pr[3]),
                                 M::pack2(pr[4], pr[5]), M::pack2(pr[6], pr[7]));
-
-    // V's scales as floats: token i of a tile from lane i of each quad, then
-    // the byte of the lane's elements.  A dead token's scale is 0, so that
-    // nothing its row may hold (a NaN scale) meets its P of 0.
-    float vsc[8];
-#pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      uint32_t w;
-      if constexpr (D == 256)
-        w = 0;
-      else
-        w = s.vs[t];
-      auto bcast = [&](uint32_t x, int i) -> uint32_t {
-        switch (i) {
-          case 0: return (uint32_t)__builtin_amdgcn_mov_dpp((int)x, 0x00, 0xF, 0xF, false);
-          case 1: return (uint32_t)__builtin_amdgcn_mov_dpp((int)x, 0x55, 0xF, 0xF, false);
-          case 2: return (uint32_t)__builtin_amdgcn_mov_dpp((int)x, 0xAA, 0xF, 0xF, false);
-          default: return (uint32_t)__builtin_amdgcn_mov_dpp((int)x, 0xFF, 0xF, 0xF, false);
-        }
-      };
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        uint32_t x;
-        if constexpr (D == 256) {
-          const uint32_t lo = bcast(s.vs[t].x, i), hi = bcast(s.vs[t].y, i);
-          x = r16 >= 8 ? hi : lo;
-        } else {
-          x = bcast(w, i);
-        }
-        constexpr int LPS = kMx4Group / NV;  // lanes per scale
-        const uint32_t byte = (x >> (((r16 / LPS) & 3) * 8)) & 0xffu;
-        uint32_t f = byte << 23;
-        if (c == new_step && dst_off != INT64_MIN && new_tok - tb - 16 * t - 4 * c4 == i)
-          f = vqs << 23;
-        vsc[4 * t + i] = __uint_as_float((live[t] >> i) & 1u ? f : 0u);
-      }
-    }
+    // O^T += V^T P^T, two d's at a time: eight tokens' pairs, then the tokens
+    // of each d together.
     auto word = [&](const VT& v, int i) -> uint32_t {  // codes 8 i .. of the lane's elements
       if constexpr (D == 256)
         return i == 0 ? v.x : v.y;
@@ -575,7 +789,8 @@ __global__ __launch_bounds__(W * 64, 2) void paged_decode_mx4_kernel(DecodeMx4Pa
       constexpr int B = decltype(BB)::value;
       uint32_t x[8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) x[j] = mx4_pair<ET, B>(word(s.v[j >> 2][j & 3], i), vsc[j]);
+      for (int j = 0; j < 8; ++j)
+        x[j] = mx4_pair<ET, B>(word(vv[j], i), __uint_as_float(vb[j] << 23));
       const uint4 lo = make_uint4(__builtin_amdgcn_perm(x[1], x[0], 0x05040100u),
                                   __builtin_amdgcn_perm(x[3], x[2], 0x05040100u),
                                   __builtin_amdgcn_perm(x[5], x[4], 0x05040100u),
@@ -597,22 +812,16 @@ __global__ __launch_bounds__(W * 64, 2) void paged_decode_mx4_kernel(DecodeMx4Pa
         product(std::integral_constant<int, 3>{}, i);
       }
     }
-  };
-
-  for (int k = 0; k < ntw; k += 2) {
-    reduce(s0, k);
-    if (k + 2 < ntw) load(s0, k + 2);
-    if (k + 1 < ntw) {
-      reduce(s1, k + 1);
-      if (k + 3 < ntw) load(s1, k + 3);
-    }
   }
+  wait_vmcnt<0>();  // steps requested early past the wave's last one
 
   // ---- merge the waves through LDS ----
   l = sum_xor16(l);
   l = sum_xor32(l);
-  float* const s_m = s_ml;          // [G][W]
-  float* const s_l = s_ml + G * W;  // [G][W]
+  if constexpr (!kOwnMerge) __syncthreads();  // every wave is done with its stages
+  float* const s_o = reinterpret_cast<float*>(kOwnMerge ? s_mrg : s_ring);  // [W][G][D]
+  float* const s_m = s_o + W * G * D;                                        // [G][W]
+  float* const s_l = s_m + G * W;                                            // [G][W]
   if (r16 < G) {
     // Lane (r16, c4) holds o of head r16 at d = NV (4 c4 + r) + i.
 #pragma unroll
@@ -670,27 +879,115 @@ __global__ __launch_bounds__(W * 64, 2) void paged_decode_mx4_kernel(DecodeMx4Pa
   if (owns_new) store_row();
 }
 
+// Merge of a split launch's partitions: one workgroup for each query head of a
+// sequence, 4 outputs a lane, the partitions dealt to the NG = 1024 / D groups
+// of D / 4 lanes, which meet in LDS.  (One workgroup for a whole group of
+// heads, each wave going through every partition, took 25 us over 64 heads'
+// worth of partitions at group 8.)  The first kFirst partitions of a group are
+// requested before the length is known.
+//   out = sum_q 2^(m_q - M) o_q / sum_q 2^(m_q - M) l_q,  M = max_q m_q.
+template <typename ET, int D>
+__global__ __launch_bounds__(256) void paged_decode_mx4_merge_kernel(DecodeMx4Params p, int G) {
+  constexpr int LPO = D / 4, NG = 256 / LPO, kFirst = 4;
+  __shared__ __align__(16) float s_o[NG * D];
+  __shared__ float s_m[NG], s_l[NG];
+  const int b = blockIdx.y, hq = blockIdx.x;
+  const int col = threadIdx.x % LPO, grp = threadIdx.x / LPO;
+  const int64_t slot0 = ((int64_t)b * p.num_kv_heads + hq / G) * p.max_parts * G + hq % G;
+  const uint32_t* const lensw = reinterpret_cast<const uint32_t*>(p.lens);
+  const uint32_t len_hi = lensw[(int64_t)(b + p.lens_cum) << p.lens_i64];
+  const uint32_t len_lo = lensw[(int64_t)b << p.lens_i64];
+  mf_f32x4 oq[kFirst];
+  float2 ml[kFirst];
+  auto request = [&](int q0) {  // partitions q0 + grp + NG j (past the last: the last)
+#pragma unroll
+    for (int j = 0; j < kFirst; ++j) {
+      const int q = q0 + grp + NG * j;
+      const int64_t slot = slot0 + (int64_t)(q < p.max_parts ? q : p.max_parts - 1) * G;
+      ml[j] = *reinterpret_cast<const float2*>(p.part_ml + slot * 2);
+      oq[j] = *reinterpret_cast<const mf_f32x4*>(p.part_o + slot * D + 4 * col);
+    }
+  };
+  request(0);
+  int L = (int)(p.lens_cum ? len_hi - len_lo : len_lo);
+  L = attend_len(p, __builtin_amdgcn_readfirstlane(L));
+  if (L <= 0 || p.num_blocks <= 0) return;
+  const int P = mx4_partition(p, L);
+  int nparts = (L + P - 1) / P;
+  if (nparts > p.max_parts) nparts = p.max_parts;
+  if (nparts <= 1) return;  // the attention kernel wrote the output itself
+  float M = kNegBig, Lt = 0.f;
+  mf_f32x4 acc = mf_f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int q0 = 0; q0 < nparts; q0 += NG * kFirst) {
+    if (q0 > 0) request(q0);
+#pragma unroll
+    for (int j = 0; j < kFirst; ++j) {
+      if (q0 + grp + NG * j < nparts) {
+        const float mn = fmaxf(M, ml[j].x);
+        const float a = fast_exp2(M - mn), c = fast_exp2(ml[j].x - mn);
+        acc = acc * a + oq[j] * c;
+        Lt = Lt * a + ml[j].y * c;
+        M = mn;
+      }
+    }
+  }
+  *reinterpret_cast<mf_f32x4*>(s_o + grp * D + 4 * col) = acc;
+  if (col == 0) {
+    s_m[grp] = M;
+    s_l[grp] = Lt;
+  }
+  __syncthreads();
+  if (grp != 0) return;
+  M = kNegBig;
+#pragma unroll
+  for (int g = 0; g < NG; ++g) M = fmaxf(M, s_m[g]);
+  Lt = 0.f;
+  acc = mf_f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int g = 0; g < NG; ++g) {
+    const float f = fast_exp2(s_m[g] - M);
+    Lt += s_l[g] * f;
+    acc += f * *reinterpret_cast<const mf_f32x4*>(s_o + g * D + 4 * col);
+  }
+  const float inv = Lt > 0.f ? 1.0f / Lt : (Lt == 0.f ? 0.f : Lt);  // a NaN stays one
+  uint2 u;
+  u.x = DecodeMma<ET>::pack2(acc[0] * inv, acc[1] * inv);
+  u.y = DecodeMma<ET>::pack2(acc[2] * inv, acc[3] * inv);
+  *reinterpret_cast<uint2*>(p.out + b * p.o_sb + (int64_t)hq * p.o_sh + col * 8) = u;
+}
+
 // ------------------------------------------------------------- launching
-template <typename ET, int D, int G, int W>
+template <typename ET, int D, int G, int W, int S>
 static void launch_decode_mx4_w(const DecodeMx4Params& p, dim3 grid, hipStream_t s) {
+  if (p.by_token) {
+    const int64_t units = (int64_t)p.num_seqs * p.max_parts;
+    grid = dim3((unsigned)((units + 7) / 8 * 8 * p.num_kv_heads));
+  }
   const dim3 nt(W * 64);
   const bool mask = p.valid != nullptr && p.valid_len > 0;
   if (p.has_pro && mask)
-    hipLaunchKernelGGL((paged_decode_mx4_kernel<ET, D, G, true, true, W>), grid, nt, 0, s, p);
+    hipLaunchKernelGGL((paged_decode_mx4_kernel<ET, D, G, true, true, W, S>), grid, nt, 0, s, p);
   else if (p.has_pro)
-    hipLaunchKernelGGL((paged_decode_mx4_kernel<ET, D, G, true, false, W>), grid, nt, 0, s, p);
+    hipLaunchKernelGGL((paged_decode_mx4_kernel<ET, D, G, true, false, W, S>), grid, nt, 0, s, p);
   else if (mask)
-    hipLaunchKernelGGL((paged_decode_mx4_kernel<ET, D, G, false, true, W>), grid, nt, 0, s, p);
+    hipLaunchKernelGGL((paged_decode_mx4_kernel<ET, D, G, false, true, W, S>), grid, nt, 0, s, p);
   else
-    hipLaunchKernelGGL((paged_decode_mx4_kernel<ET, D, G, false, false, W>), grid, nt, 0, s, p);
+    hipLaunchKernelGGL((paged_decode_mx4_kernel<ET, D, G, false, false, W, S>), grid, nt, 0, s, p);
 }
 
 template <typename ET, int D, int G>
 static void launch_decode_mx4(const DecodeMx4Params& p, dim3 grid, hipStream_t s) {
-  launch_decode_mx4_w<ET, D, G, 8>(p, grid, s);
+  if constexpr (D == 256) {
+    launch_decode_mx4_w<ET, D, G, 4, 2>(p, grid, s);
+  } else {
+    if (p.waves == 4)
+      launch_decode_mx4_w<ET, D, G, 4, 2>(p, grid, s);
+    else
+      launch_decode_mx4_w<ET, D, G, 8, 3>(p, grid, s);
+  }
   if (p.max_parts > 1)
-    hipLaunchKernelGGL((paged_decode_merge_kernel<ET, D, G, 2>), dim3(grid.x, grid.y), dim3(256),
-                       0, s, p);
+    hipLaunchKernelGGL((paged_decode_mx4_merge_kernel<ET, D>), dim3(grid.x * G, grid.y), dim3(256),
+                       0, s, p, G);
 }
 
 template <typename ET, int D>

@@ -263,7 +263,27 @@ def _rows_args(args, key, value, pool, slot_mapping, hkv, d):
     return args
 
 
+def _fast_on(t: torch.Tensor, layout: str):
+    """(fast-path module, device index) for a call on t's device when that is
+    the current one, else (None, -1)."""
+    fast = _FAST if _FAST_LOADED else _fast_calls()
+    if fast is not None and layout in (LAYOUT_NHD, LAYOUT_HND):
+        index = t.get_device()
+        if index >= 0 and index == torch.cuda.current_device():
+            return fast, index
+    return None, -1
+
+
 def _store_mx4(key, value, k_cache, v_cache, slot_mapping, layout, k_scale, v_scale) -> None:
+    fast, index = _fast_on(key, layout)
+    if fast is not None and isinstance(v_scale, torch.Tensor):
+        rc = fast.store_kvcache_mx4(key, value, k_cache, v_cache, slot_mapping,
+                                    layout == LAYOUT_HND, k_scale, v_scale, index,
+                                    _raw_stream(index))
+        if rc == 0:
+            return
+        if _FAST_NOT_TAKEN < rc < 0:
+            N.check("va_store_kvcache_mx4", rc)
     device = _check_gpu(key, value, k_cache, v_cache, slot_mapping)
     pool, scales = _mx4_structs(k_cache, v_cache, layout, k_scale, v_scale, key.dtype)
     _check_gpu(key, k_scale)
@@ -286,6 +306,15 @@ def load_kvcache(
     as values of `dtype` (exact in the type they were stored from); slots
     outside the pool read as zeros.  A 16-bit or FP8 pool's rows are read by
     indexing it."""
+    fast, index = _fast_on(k_cache, layout)
+    if fast is not None and dtype in (torch.bfloat16, torch.float16):
+        rc, key, value = fast.load_kvcache_mx4(k_cache, v_cache, slot_mapping,
+                                               dtype == torch.float16, layout == LAYOUT_HND,
+                                               k_scale, v_scale, index, _raw_stream(index))
+        if rc == 0:
+            return key, value
+        if _FAST_NOT_TAKEN < rc < 0:
+            N.check("va_load_kvcache_mx4", rc)
     device = _check_gpu(k_cache, v_cache, slot_mapping, k_scale, v_scale)
     pool, scales = _mx4_structs(k_cache, v_cache, layout, k_scale, v_scale, dtype)
     hkv, d = pool_heads(k_cache, layout)
@@ -475,7 +504,8 @@ _VARLEN_ARGS_SIZE = ctypes.sizeof(N.VarlenArgs)
 
 # Host fast path (csrc/host/fast_calls.cpp, the ``_fast_calls`` module next
 # to the library): the same checks and the same C-ABI call in C++, for the
-# common paged_decode / varlen_attention / store_kvcache / qk_norm_rope calls.  It launches nothing for a
+# common paged_decode / varlen_attention / store_kvcache / qk_norm_rope /
+# load_kvcache / batch_metadata calls.  It launches nothing for a
 # call it does not take, and the Python path below then runs (and raises the
 # error for a bad argument), so results and errors are the same either way.
 _FAST_NOT_TAKEN = -1000
@@ -509,6 +539,10 @@ def _fast_calls():
                             addr(lib.va_varlen_attention),
                             addr(lib.va_varlen_split_workspace_bytes), addr(lib.va_store_kvcache),
                             addr(lib.va_qk_norm_rope))
+            mod.set_mx4_entries(addr(lib.va_store_kvcache_mx4), addr(lib.va_load_kvcache_mx4),
+                                addr(lib.va_paged_decode_mx4),
+                                addr(lib.va_paged_decode_mx4_workspace_bytes),
+                                addr(lib.va_varlen_attention_mx4), addr(lib.va_batch_metadata))
             _FAST = mod
     return _FAST
 _POOLS: dict[tuple, N.KvPool] = {}  # pool descriptions by tensor identity and geometry
@@ -654,14 +688,15 @@ def paged_decode(
     """
     mx4 = isinstance(k_scale, torch.Tensor)
     fast = _FAST if _FAST_LOADED else _fast_calls()
-    if fast is not None and not no_alloc and not mx4 and layout in (LAYOUT_NHD, LAYOUT_HND):
+    if (fast is not None and not no_alloc and layout in (LAYOUT_NHD, LAYOUT_HND) and
+            mx4 == isinstance(v_scale, torch.Tensor)):
         index = q.get_device()
         if index >= 0 and index == torch.cuda.current_device():
             if out is None:
                 out = torch.empty_like(q)
             stream = _raw_stream(index)
             pro = prologue
-            rc = fast.paged_decode(
+            rc = (fast.paged_decode_mx4 if mx4 else fast.paged_decode)(
                 q, k_cache, v_cache, block_tables, lens, out, new_k, new_v, new_slots,
                 valid_mask, None if pro is None else pro.q_norm_weight,
                 None if pro is None else pro.k_norm_weight,
@@ -670,11 +705,12 @@ def paged_decode(
                 None if pro is None else pro.positions, _WORKSPACES.get((index, stream)),
                 lens_cumulative, layout == LAYOUT_HND,
                 int(max_seq_len), float(scale), int(split_tokens), int(key_limit),
-                int(table_read_width), float(k_scale), float(v_scale), index, stream)
+                int(table_read_width), k_scale if mx4 else float(k_scale),
+                v_scale if mx4 else float(v_scale), index, stream)
             if rc == 0:
                 return out
             if _FAST_NOT_TAKEN < rc < 0:
-                N.check("va_paged_decode", rc)
+                N.check("va_paged_decode_mx4" if mx4 else "va_paged_decode", rc)
             # Not taken, or a workspace is needed first: the path below.
     device = _check_gpu(q, k_cache, v_cache, block_tables, lens, valid_mask, new_k, new_v,
                         new_slots, out)
@@ -813,21 +849,27 @@ def varlen_attention(
     launch normalises and rotates them at ``prologue.positions`` (one per
     query token); k and the pool must hold processed keys.
     """
+    mx4 = isinstance(k_scale, torch.Tensor)
     fast = _FAST if _FAST_LOADED else _fast_calls()
     if (fast is not None and prologue is None and layout in (LAYOUT_NHD, LAYOUT_HND) and
-            (k_cache is None or k_cache.dtype not in (FP8_KV_DTYPE, MXFP4_KV_DTYPE))):
+            (k_cache is None or k_cache.dtype != FP8_KV_DTYPE) and
+            mx4 == isinstance(v_scale, torch.Tensor)):
         index = q.get_device()
         if index >= 0 and index == torch.cuda.current_device():
             if out is None:
                 out = torch.empty_like(q)
-            rc = fast.varlen_attention(
-                q, k, v, cu_seqlens_q, cu_seqlens_k, int(max_seqlen_q), int(max_seqlen_k),
-                float(scale), bool(causal), k_cache, v_cache, block_tables, slot_mapping, out,
-                layout == LAYOUT_HND, index, _raw_stream(index))
+            args = (q, k, v, cu_seqlens_q, cu_seqlens_k, int(max_seqlen_q), int(max_seqlen_k),
+                    float(scale), bool(causal), k_cache, v_cache, block_tables, slot_mapping, out,
+                    layout == LAYOUT_HND)
+            stream = _raw_stream(index)
+            if mx4:
+                rc = fast.varlen_attention_mx4(*args, k_scale, v_scale, index, stream)
+            else:
+                rc = fast.varlen_attention(*args, index, stream)
             if rc == 0:
                 return out
             if _FAST_NOT_TAKEN < rc < 0:
-                N.check("va_varlen_attention", rc)
+                N.check("va_varlen_attention_mx4" if mx4 else "va_varlen_attention", rc)
     device = _check_gpu(q, k, v, cu_seqlens_q, cu_seqlens_k, k_cache, v_cache, block_tables,
                         slot_mapping, out)
     _require(q.dim() == 3, "q must be [total_q, num_heads, head_dim]")
@@ -848,7 +890,7 @@ def varlen_attention(
                  "a KV pool needs v_cache and block_tables")
         hkv, pd = pool_heads(k_cache, layout)
         _require(pd == d, "pool head_dim must match q")
-        if isinstance(k_scale, torch.Tensor):
+        if mx4:
             pool, scales = _mx4_structs(k_cache, v_cache, layout, k_scale, v_scale, q.dtype)
             _check_gpu(q, k_scale)
         else:
@@ -982,6 +1024,17 @@ def batch_metadata(
 
     ``out``: tensors of an earlier result of the same sizes to write into (a
     captured graph's static buffers)."""
+    if out is None and (table_width is None or table_width >= 0):
+        fast, index = _fast_on(lens, LAYOUT_NHD)
+        if fast is not None:
+            rc, made = fast.batch_metadata(lens, num_computed, request_tables, int(block_size),
+                                           int(max_tokens), rows, int(padded_batch),
+                                           -1 if table_width is None else int(table_width),
+                                           free_blocks, free_count, index, _raw_stream(index))
+            if rc == 0:
+                return BatchMetadata(*made)
+            if _FAST_NOT_TAKEN < rc < 0:
+                N.check("va_batch_metadata", rc)
     device = _check_gpu(lens, num_computed, request_tables, rows, free_blocks, free_count)
     _require(lens.dim() == 1 and num_computed.shape == lens.shape and lens.is_contiguous()
              and num_computed.is_contiguous(), "lens and num_computed must be [B] vectors")
