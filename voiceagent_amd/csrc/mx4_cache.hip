@@ -74,14 +74,6 @@ __device__ inline bool mx4_place(const Mx4CacheParams& p, const Mx4Word& r, int6
   return true;
 }
 
-// Largest of the values of four neighbouring lanes.
-__device__ inline uint32_t quad_max(uint32_t x) {
-  const uint32_t a = (uint32_t)__builtin_amdgcn_mov_dpp((int)x, kDppQuadXor1, 0xF, 0xF, false);
-  x = x > a ? x : a;
-  const uint32_t b = (uint32_t)__builtin_amdgcn_mov_dpp((int)x, kDppQuadXor2, 0xF, 0xF, false);
-  return x > b ? x : b;
-}
-
 template <typename ET, int kWords>
 __global__ __launch_bounds__(kMx4Threads) void store_mx4_kernel(Mx4CacheParams p) {
   const uint32_t total = p.total_words;
@@ -163,6 +155,10 @@ int check_mx4(const char* fn, const va_kv_pool& pool, const va_mx4_scales* sc, i
   const int64_t sstrides[] = {sc->stride_block, sc->stride_slot, sc->stride_head};
   for (int64_t s : sstrides)
     VA_CHECK_ARG(s % align == 0, "%s: scale strides must be multiples of head_dim / 32 bytes", fn);
+  // (The attention finds head_dim 64's pairs of scales in words of 4 bytes, which
+  // blocks must not shift.)
+  VA_CHECK_ARG(word != 2 || sc->stride_block % 4 == 0,
+               "%s: the scales' block stride must be a multiple of 4 bytes", fn);
   VA_CHECK_ARG((uintptr_t)sc->k % align == 0 && (uintptr_t)sc->v % align == 0,
                "%s: scale pointers must be aligned to head_dim / 32 bytes", fn);
   return VA_OK;

@@ -40,8 +40,6 @@ struct DecodeMx4Params : DecodeParams {
   int32_t min_part;  // dyn_split: fewest tokens of a partition
 };
 
-typedef int mx_i32x8 __attribute__((ext_vector_type(8)));
-
 constexpr int kMx4Step = 32;  // tokens a wave reduces at a time: two 16-token tiles
 
 // Tokens of a context partition: fixed, or with dyn_split an even share of the
@@ -53,69 +51,10 @@ __device__ inline int mx4_partition(const DecodeMx4Params& p, int L) {
   return P > p.min_part ? P : p.min_part;
 }
 
-// S^T += K Q^T: e2m1 codes of 16 tokens against e4m3 queries.
-__device__ inline mf_f32x4 mx4_qk(uint4 k, int ks, const mx_i32x8& q, int qs, mf_f32x4 c) {
-  const mx_i32x8 a = {(int)k.x, (int)k.y, (int)k.z, (int)k.w, 0, 0, 0, 0};
-  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, q, c, 4 /* e2m1 */, 0 /* e4m3 */, 0,
-                                                          ks, 0, qs);
-}
-
 // O^T += V^T P^T over 32 tokens, 16-bit.
 template <typename ET>
 __device__ inline mf_f32x4 mx4_pv(uint4 v, uint4 p, mf_f32x4 c) {
   return DecodeMma<ET>::qk(v, p, c);
-}
-
-// N e4m3 terms of 16 elements of ET (two words of 8), for the power of two
-// `unit`: term 0 rounds x / unit to e4m3, term t what the terms before it left,
-// in units of 2^-4t.  The conversions divide by their scale themselves.
-template <typename ET, int N>
-__device__ inline void mx4_split16(const uint4 (&u)[2], float unit, uint4 (&term)[N]) {
-  typedef short s16x2 __attribute__((ext_vector_type(2)));
-  const uint32_t in[8] = {u[0].x, u[0].y, u[0].z, u[0].w, u[1].x, u[1].y, u[1].z, u[1].w};
-  uint32_t w[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    s16x2 r = {0, 0};
-    if constexpr (ET::kIsBF16) {
-      r = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(r, __builtin_bit_cast(bf16x2_t, in[2 * i]), unit,
-                                                    false);
-      r = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(r, __builtin_bit_cast(bf16x2_t, in[2 * i + 1]),
-                                                    unit, true);
-    } else {
-      r = __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(r, __builtin_bit_cast(f16x2_t, in[2 * i]), unit,
-                                                   false);
-      r = __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(r, __builtin_bit_cast(f16x2_t, in[2 * i + 1]),
-                                                   unit, true);
-    }
-    w[i] = __builtin_bit_cast(uint32_t, r);
-  }
-  term[0] = make_uint4(w[0], w[1], w[2], w[3]);
-  float x[16];
-  float(&x0)[8] = *reinterpret_cast<float(*)[8]>(&x[0]);
-  float(&x1)[8] = *reinterpret_cast<float(*)[8]>(&x[8]);
-  ET::unpack(u[0], x0);
-  ET::unpack(u[1], x1);
-#pragma unroll
-  for (int t = 1; t < N; ++t) {
-    const float before = t == 1 ? unit : unit * 0.0625f;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const auto lo = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(w[i], before, false);
-      const auto hi = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(w[i], before, true);
-      x[4 * i] -= lo[0];
-      x[4 * i + 1] -= lo[1];
-      x[4 * i + 2] -= hi[0];
-      x[4 * i + 3] -= hi[1];
-      s16x2 r = {0, 0};
-      r = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(r, x[4 * i], x[4 * i + 1], before * 0.0625f,
-                                                   false);
-      r = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(r, x[4 * i + 2], x[4 * i + 3], before * 0.0625f,
-                                                   true);
-      w[i] = __builtin_bit_cast(uint32_t, r);
-    }
-    term[t] = make_uint4(w[0], w[1], w[2], w[3]);
-  }
 }
 
 template <int D>
@@ -715,7 +654,7 @@ __global__ __launch_bounds__(W * 64, W == 4 && D <= 128 ? 4 : 2) void paged_deco
 #pragma unroll
       for (int cc = 0; cc < CH; ++cc)
 #pragma unroll
-        for (int q = 0; q < QM; ++q) sc[t] = mx4_qk(kk[t][cc], kks[t][cc], qf[q][cc], qs[q], sc[t]);
+        for (int q = 0; q < QM; ++q) sc[t] = mx4_mfma(kk[t][cc], kks[t][cc], qf[q][cc], qs[q], sc[t]);
     }
     // The stage has been read: it takes the wave's step k + S.
     wait_lgkmcnt0();

@@ -226,12 +226,7 @@ extern "C" int va_varlen_attention_mx4(const va_varlen_args* a, const va_mx4_sca
                    15 * a->pool.stride_slot + a->head_dim < ((int64_t)1 << 31),
                "%s: the pool's slot stride must be non-negative and below 128 MiB", fn);
   VA_CHECK_ARG(a->prologue == nullptr, "%s: no query prologue over an MXFP4 pool", fn);
-  va_varlen_args b = *a;
-  b.slot_mapping = nullptr;
-  const int rc = varlen_native(&b, sc, stream);
-  if (rc != VA_OK || a->slot_mapping == nullptr) return rc;
-  const va_store_args sa = store_args_of(a);
-  return va_store_kvcache_mx4(&sa, sc, stream);
+  return varlen_native(a, sc, stream);
 }
 
 // The store of a call's new rows, as a launch of its own.
@@ -352,8 +347,8 @@ int va::varlen_native(const va_varlen_args* a, const va_mx4_scales* sc, void* st
   p.kv_f8 = f8;
   p.k_scale = f8 ? a->pool.k_scale : 1.0f;
   p.v_scale = f8 ? a->pool.v_scale : 1.0f;
-  p.ks = mx4 ? (const uint8_t*)sc->k : nullptr;
-  p.vs = mx4 ? (const uint8_t*)sc->v : nullptr;
+  p.ks = mx4 ? (uint8_t*)sc->k : nullptr;
+  p.vs = mx4 ? (uint8_t*)sc->v : nullptr;
   p.sc_blk = mx4 ? sc->stride_block : 0;
   p.sc_slot = mx4 ? sc->stride_slot : 0;
   p.sc_head = mx4 ? sc->stride_head : 0;

@@ -44,6 +44,7 @@
 // from the lengths: every workgroup of an XCD computes the same one.
 #pragma once
 
+#include <algorithm>
 #include <atomic>
 #include <type_traits>
 
@@ -102,8 +103,8 @@ struct VarlenParams {
   int32_t* part_count;
   int32_t has_pro;          // the Qwen3 query prologue runs on every query row
   PrologueParams pro;
-  const uint8_t* ks;  // MXFP4 pool: the scale bytes
-  const uint8_t* vs;
+  uint8_t* ks;  // MXFP4 pool: the scale bytes
+  uint8_t* vs;
   int64_t sc_blk, sc_slot, sc_head;  // bytes
 };
 
@@ -244,8 +245,13 @@ constexpr int waves_per_simd(int d, bool half) { return d == 64 ? (half ? 4 : 3)
 // a multiple of 16 tokens.  As over FP8 pools a tile's pool rows are copied as
 // codes, but a wave converts the rows it copied itself, in a code area of its
 // own, before the tile's barrier: no second barrier.  A lane converts whole
-// groups (16 bytes of codes), whose scale bytes it loaded when the tile was
-// requested.
+// groups (16 bytes of codes).
+// (Measured and dropped: S^T of whole pool tiles from the codes themselves, on
+// scaled products against the queries' e4m3 terms, with V converted beside them:
+// four prompts over 2K-8K 91.9 us against 91.3, a chunk of 61 over 16K 45.1
+// against 40.9, 32 prompts over 1K 108 against 99.8.  The loop is bound by a
+// wave's chain, which a second barrier and the terms' set-up lengthen, not by LDS
+// traffic.)
 //
 // kHalf: 64 MFMA rows per item, one 16-row tile per wave.  A tile's body is
 // bound by the wave's own chain (S^T, softmax, O^T; ~1.5 us with two row tiles,
@@ -283,17 +289,20 @@ varlen_attention_kernel(VarlenParams p) {
   constexpr int CROWB = kMx4 ? D / 2 : D;  // bytes of a code row
   constexpr int CCPR = CROWB / 16;         // 16-byte chunks per code row
   constexpr int CRPI = 64 / CCPR;          // code rows per DMA instruction
-  // Code DMA instructions per wave per tile, K or V (MXFP4 at head_dim 64: the
-  // upper lanes copy the wave's 16 rows a second time).
+  // Code DMA instructions per wave per tile, K or V (kBoth: K and V together,
+  // half the lanes each).
+  constexpr bool kBoth = kMx4 && D == 64;
   constexpr int NIC = CRPI < 16 ? 16 / CRPI : 1;
-  constexpr int CODE_B = 4 * NIC * 1024;   // bytes of one tile of codes, K or V
+  constexpr int CODE_B = kBoth ? 512 : 4 * NIC * 1024;  // from a wave's K codes to its V codes
   static_assert(!kF8 || CODE_B == kKeyTile * D, "code DMA split");
-  __shared__ __align__(1024) char s_code[kCode ? 2 * CODE_B : 16];
+  __shared__ __align__(1024) char s_code[kBoth ? 4 * 1024 : kCode ? 2 * CODE_B : 16];
   // kMx4: a wave's 16 rows are 16 D / 32 groups of K and as many of V, NGL of
   // them a lane's: group e = 64 i + lane is group e % NS of row e / NS (K's 16,
-  // then V's).
+  // then V's).  Beside the codes the wave's scales are copied, a word a row
+  // (K's 16, then V's; at head_dim 64 the aligned word that holds the row's two).
   constexpr int NS = D / kMx4Group;
   constexpr int NGL = 2 * 16 * NS / 64;
+  __shared__ __align__(16) char s_scale[kMx4 ? 4 * 256 : 16];
   // kPro: the query norm weights as fp32, written once per workgroup here and
   // read by every item's prologue (the first tile's barrier orders them).
   __shared__ __align__(16) float s_qw[kPro ? D : 4];
@@ -545,15 +554,34 @@ varlen_attention_kernel(VarlenParams p) {
   uint32_t k_st = (uint32_t)p.k_st, v_st = (uint32_t)p.v_st;
   asm volatile("" : "+s"(k_st), "+s"(v_st));
   set_offsets(k_st, v_st);
+  // MXFP4 codes: chunk c of row r sits at position c ^ code_swz(r), so that 16
+  // rows' chunks c (an S^T operand) cover all banks.
+  auto code_swz = [&](int row) { return (row / (256 / CROWB)) & (CCPR - 1); };
   // FP8 pool: a wave's 16 code rows (unswizzled, CRPI rows an instruction).
   const uint32_t code_lane =
       kF8 ? (uint32_t)(lane / CCPR) * (uint32_t)p.s_slot + (uint32_t)(lane % CCPR) * 16u
-      : kMx4 ? (uint32_t)(lane / CCPR % 16) * (uint32_t)p.s_slot + (uint32_t)(lane % CCPR) * 16u
+      : kMx4 ? (uint32_t)(lane / CCPR % 16) * (uint32_t)p.s_slot +
+                   (uint32_t)((lane % CCPR) ^ code_swz(lane / CCPR)) * 16u
              : 0u;
-  // kMx4: the scales of the lane's groups of the tile requested last.
-  uint32_t gsc[kMx4 ? NGL : 1];
-#pragma unroll
-  for (int i = 0; i < (kMx4 ? NGL : 1); ++i) gsc[i] = 0;
+  // kMx4: the scale array and row of the lane's word; the lanes past the 32nd
+  // copy the same words again.
+  const char* const sc_lane =
+      kMx4 ? reinterpret_cast<const char*>((lane & 16) ? p.vs : p.ks) + (int64_t)(lane & 15) * p.sc_slot
+           : nullptr;
+  const uint32_t sc_dst = kMx4 ? (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)s_scale +
+                                     (uint32_t)(wave * 256)
+                               : 0u;
+  auto scale_copy = [&](const char* src, uint32_t dst) {  // (head_dim 64: down to a word)
+    if constexpr (D == 64) src = (const char*)((uintptr_t)src & ~(uintptr_t)3);
+    asm volatile("s_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(src), "{m0}"(dst) : "memory");
+  };
+  // head_dim 64: which half of its word a row's two scales are (blocks and tiles
+  // lie a multiple of 4 bytes apart: host check).
+  auto scale_half = [&](const uint8_t* base, int row, int h) -> int {
+    return D == 64 ? (int)((uint32_t)(uintptr_t)base + (uint32_t)h * (uint32_t)p.sc_head +
+                           (uint32_t)row * (uint32_t)p.sc_slot) & 2
+                   : 0;
+  };
   const uint32_t code_dst = code_base + (uint32_t)(wave * NIC * 1024);
 
   // The cursor of the tiles being requested, one step ahead of the tiles
@@ -648,9 +676,10 @@ varlen_attention_kernel(VarlenParams p) {
     int kind;
     const char* kb;  // the wave's first row
     const char* vb;
+    int64_t srow;    // kMx4: the offset of its scales
   };
   const char* zero_row = reinterpret_cast<const char*>(&kZeroRow);
-  auto issue_hard = [&](int64_t row, int st) {
+  auto issue_hard = [&](int64_t row, int64_t srow, int st) {
     const ColdArgs ca = cold_args();
     const uint32_t dst0 = lds_base + (uint32_t)(st * 2 * TILE_B + wave * NI * 1024);
     const int kb = cu.t * kKeyTile;
@@ -711,7 +740,8 @@ varlen_attention_kernel(VarlenParams p) {
         const int j = kb + crow0 + i * CRPI;
         kc[i] = zero_row;
         vc[i] = zero_row;
-        if (j < cu.prefix && j < cu.kend) pool_at(j, craw[i], (lane % CCPR) * 16, kc[i], vc[i]);
+        const int c = kMx4 ? (lane % CCPR) ^ code_swz(lane / CCPR) : lane % CCPR;
+        if (j < cu.prefix && j < cu.kend) pool_at(j, craw[i], c * 16, kc[i], vc[i]);
       }
     }
     uint2 braw[NI];
@@ -765,9 +795,14 @@ varlen_attention_kernel(VarlenParams p) {
       if (kb < cu.prefix) {
 #pragma unroll
         for (int i = 0; i < NIC; ++i) {
-          dma16(kc[i], code_dst + i * 1024);
-          dma16(vc[i], code_dst + CODE_B + i * 1024);
+          if constexpr (kBoth) {
+            dma16(lane < 32 ? kc[i] : vc[i], code_dst);
+          } else {
+            dma16(kc[i], code_dst + i * 1024);
+            dma16(vc[i], code_dst + CODE_B + i * 1024);
+          }
         }
+        if constexpr (kMx4) scale_copy(row != kNoRow ? sc_lane + srow : zero_row, sc_dst);
       }
     }
   };
@@ -777,6 +812,7 @@ varlen_attention_kernel(VarlenParams p) {
     Easy e;
     e.kind = kNone;
     e.kb = e.vb = nullptr;
+    e.srow = 0;
     const int kb = cu.t * kKeyTile;
     if (kb >= cu.prefix && kb + kKeyTile <= cu.kend) {
       e.kind = kRows;
@@ -794,24 +830,9 @@ varlen_attention_kernel(VarlenParams p) {
       row = (int64_t)(((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(rows >> 32), l) << 32) |
                       (uint32_t)__builtin_amdgcn_readlane((int)rows, l));
       if constexpr (kMx4) {
-        // The scales of the lane's groups: loaded whatever the row, so that no
-        // load sits behind a branch (a row that is not there takes a zero).
-        const int64_t srow =
+        e.srow =
             (int64_t)(((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(srows >> 32), l) << 32) |
                       (uint32_t)__builtin_amdgcn_readlane((int)srows, l));
-        const ColdArgs ca = cold_args();
-        const char* at[NGL];
-#pragma unroll
-        for (int i = 0; i < NGL; ++i) {
-          const int g = 64 * i + lane, rc = g % (16 * NS);
-          const int j = kb + 16 * wave + rc / NS;
-          at[i] = zero_row;
-          if (row != kNoRow && j < cu.prefix && j < cu.kend)
-            at[i] = reinterpret_cast<const char*>(g >= 16 * NS ? ca->vs : ca->ks) + srow +
-                    (rc / NS) * ca->sc_slot + rc % NS;
-        }
-#pragma unroll
-        for (int i = 0; i < NGL; ++i) gsc[i] = *reinterpret_cast<const uint8_t*>(at[i]);
       }
       if (kb + kKeyTile <= min(cu.prefix, cu.kend) && row != kNoRow && p.block16) {
         e.kind = kCode ? kCodes : kRows;
@@ -825,7 +846,7 @@ varlen_attention_kernel(VarlenParams p) {
         return e;
       }
     }
-    issue_hard(row, st);
+    issue_hard(row, e.srow, st);
     return e;
   };
   auto easy_issue = [&](const Easy& e, int i, uint32_t dst) {  // 16-bit rows
@@ -838,9 +859,15 @@ varlen_attention_kernel(VarlenParams p) {
     }
   };
   auto easy_codes = [&](const Easy& e, int i) {
+    if constexpr (kBoth) {
+      dma16((lane < 32 ? e.kb : e.vb) + code_lane, code_dst);
+      scale_copy(sc_lane + e.srow, sc_dst);
+      return;
+    }
     const int64_t step = (int64_t)(i * CRPI) * p.s_slot;
     dma16(code_lane, e.kb + step, code_dst + i * 1024);
     dma16(code_lane, e.vb + step, code_dst + CODE_B + i * 1024);
+    if constexpr (kMx4) scale_copy(sc_lane + e.srow, sc_dst);
   };
   auto issue_now = [&](const Easy& e, int st) {  // all of an easy tile at once
     const uint32_t dst = lds_base + (uint32_t)(st * 2 * TILE_B + wave * NI * 1024);
@@ -897,7 +924,10 @@ varlen_attention_kernel(VarlenParams p) {
   constexpr int RPS = 64 / CPR;  // rows per store step
   constexpr int NSTEP = (BQ * CPR + kVarlenThreads - 1) / kVarlenThreads;
   static_assert(NSTEP * RPS <= 64, "one slot lane per row");
-  const bool fused_store = kPaged && !kCode && p.slots != nullptr;  // codes: a launch of its own
+  // (FP8 codes: a launch of its own.)  MXFP4: a row's groups are four neighbouring
+  // lanes' chunks, quantised as va_store_kvcache_mx4 does (a launch after the
+  // attention took 4-5 us).
+  const bool fused_store = kPaged && !kF8 && p.slots != nullptr;
   auto st_base = [&](int k) {  // first block row of store step k (BQ: none)
     const int e0 = k * kVarlenThreads + 64 * wave;
     return e0 < BQ * CPR ? e0 / CPR : BQ;
@@ -981,27 +1011,30 @@ varlen_attention_kernel(VarlenParams p) {
       // item's first tile.
       wait_vmcnt<0>();
       // MXFP4 pool: the wave's rows of this tile from its code area into the
-      // stage, at their swizzled positions; then the code area and `gsc` may
-      // take the next tile.
+      // stage, at their swizzled positions; then the area may take the next
+      // tile.
+      // MXFP4 pool: the wave's rows of this tile from its code area into the
+      // stage, at their swizzled positions; then the area may take the next
+      // tile.
       if constexpr (kMx4) {
-#pragma unroll
-        for (int i = 0; i < NGL; ++i) asm volatile("" ::"v"(gsc[i]));
         if (kb < prefix) {
-          char* const s_kt = s_kv + stage * 2 * TILE_B;
 #pragma unroll
           for (int i = 0; i < NGL; ++i) {
             const int g = 64 * i + lane, rc = g % (16 * NS);
             const int is_v = g >= 16 * NS ? 1 : 0;
-            const int r = 16 * wave + rc / NS, c = rc % NS;
+            const int row = rc / NS, r = 16 * wave + row, c = rc % NS;
             if (kb + r < prefix) {
-              const uint4 codes = lds_read16(
-                  s_code + is_v * CODE_B + wave * NIC * 1024, (rc / NS) * CROWB + c * 16);
-              char* const dst = s_kt + is_v * TILE_B + r * ROWB;
+              const uint4 codes = lds_read16(s_code + is_v * CODE_B + wave * NIC * 1024,
+                                             row * CROWB + ((c ^ code_swz(row)) << 4));
+              // (A row without a block is zeros whatever its scale word.)
+              const uint32_t scale = (uint8_t)s_scale[wave * 256 + is_v * 64 + row * 4 +
+                                                      scale_half(is_v ? p.vs : p.ks, row, cur.h) + c];
+              char* const dst = s_kv + stage * 2 * TILE_B + is_v * TILE_B + r * ROWB;
               const uint32_t w[4] = {codes.x, codes.y, codes.z, codes.w};
 #pragma unroll
               for (int q = 0; q < 4; ++q)
                 *reinterpret_cast<uint4*>(dst + (((4 * c + q) ^ swz<D>(r)) << 4)) =
-                    mx4_values8<ET>(w[q], gsc[i]);
+                    mx4_values8<ET>(w[q], scale);
             }
           }
           wait_lgkmcnt0();
@@ -1160,6 +1193,7 @@ varlen_attention_kernel(VarlenParams p) {
       Easy e;
       e.kind = kNone;
       e.kb = e.vb = nullptr;
+      e.srow = 0;
       if (req) {
         e = issue(stage ^ 1);
         advance();
@@ -1177,12 +1211,16 @@ varlen_attention_kernel(VarlenParams p) {
         const int64_t cap = (int64_t)p.num_blocks * p.block_size;
         const int64_t slot = p.slot_i64 ? (int64_t)(((uint64_t)st_slot.y << 32) | st_slot.x)
                                           : (int64_t)(int32_t)st_slot.x;
-        int64_t at = kNoRow;
+        int64_t at = kNoRow, sat = 0;  // sat: kMx4, of the row's scales
         if (slot >= 0 && slot < cap) {
           const int64_t blk = p.slot_small
                                   ? (int64_t)fast_div((uint32_t)slot, p.bs_div)
                                   : slot / p.block_size;
           at = blk * p.s_blk + (slot - blk * p.block_size) * p.s_slot + cur.h * p.s_head;
+          if constexpr (kMx4) {
+            const ColdArgs ca = cold_args();
+            sat = blk * ca->sc_blk + (slot - blk * p.block_size) * ca->sc_slot + cur.h * ca->sc_head;
+          }
         }
         const int c = lane % CPR;
 #pragma unroll 4
@@ -1190,14 +1228,35 @@ varlen_attention_kernel(VarlenParams p) {
           const int holder = k * RPS + lane / CPR;
           const uint32_t lo = (uint32_t)__shfl((int)(uint32_t)at, holder, 64);
           const int hi = __shfl((int)(at >> 32), holder, 64);
+          uint32_t slo = 0;
+          int shi = 0;
+          if constexpr (kMx4) {
+            slo = (uint32_t)__shfl((int)(uint32_t)sat, holder, 64);
+            shi = __shfl((int)(sat >> 32), holder, 64);
+          }
           const int row = st_base(k) + lane / CPR;
           const int key = st_key0 + row;
           if (row < BQ && hi != (int)(kNoRow >> 32) && key >= kb && key < kb + kKeyTile) {
-            const int64_t dst = (int64_t)(((uint64_t)(uint32_t)hi << 32) | lo) + c * 16;
+            const int64_t dst =
+                (int64_t)(((uint64_t)(uint32_t)hi << 32) | lo) + c * (kMx4 ? 4 : 16);
             const int r = key - kb;
             const int off = r * ROWB + ((c ^ swz<D>(r)) << 4);
-            st16_nt(p.kp + dst, lds_read16(s_k, off));
-            st16_nt(p.vp + dst, lds_read16(s_v, off));
+            if constexpr (kMx4) {
+              const ColdArgs ca = cold_args();
+              const int64_t sdst = (int64_t)(((uint64_t)(uint32_t)shi << 32) | slo) + (c >> 2);
+              const uint4 kr = lds_read16(s_k, off), vr = lds_read16(s_v, off);
+              const uint32_t ksc = mx4_scale<ET>(quad_max(mx4_absmax8(kr)));
+              const uint32_t vsc = mx4_scale<ET>(quad_max(mx4_absmax8(vr)));
+              *reinterpret_cast<uint32_t*>(p.kp + dst) = mx4_codes8<ET>(kr, ksc);
+              *reinterpret_cast<uint32_t*>(p.vp + dst) = mx4_codes8<ET>(vr, vsc);
+              if ((c & 3) == 0) {
+                ca->ks[sdst] = (uint8_t)ksc;
+                ca->vs[sdst] = (uint8_t)vsc;
+              }
+            } else {
+              st16_nt(p.kp + dst, lds_read16(s_k, off));
+              st16_nt(p.vp + dst, lds_read16(s_v, off));
+            }
           }
         }
       }
@@ -1451,8 +1510,7 @@ varlen_attention_kernel(VarlenParams p) {
 // of the item whose first piece is XCD x % 8's piece x / 8 (the XCD that wrote
 // it), and ends at once when there is no such item.
 //   out = sum_j 2^(m_j - M) o_j / sum_j 2^(m_j - M) l_j,  M = max_j m_j.
-// kMx4 only separates the names of two translation units' instantiations.
-template <bool kBF16, int D, int G, bool kHalf, bool kMx4>
+template <bool kBF16, int D, int G, bool kHalf>
 __global__ __launch_bounds__(256) void varlen_merge_kernel(VarlenParams p) {
   constexpr int LPR = D / 4;       // lanes per row, four outputs each
   constexpr int RPP = 256 / LPR;   // rows per pass
@@ -1497,6 +1555,96 @@ __global__ __launch_bounds__(256) void varlen_merge_kernel(VarlenParams p) {
   }
 }
 
+// The merge of a launch over an MXFP4 pool: the same sum, with a row's pieces
+// dealt to NG groups of lanes that meet in LDS.  Workgroup (x, y) serves
+// kMergeRows rows of split item x / 8 of XCD x % 8, found among the pieces'
+// heads (the first piece of an item names it).  With one workgroup a piece, 32
+// rows and all of a row's pieces, few long items (61 tokens over 16K: 8 items of
+// 64 pieces) left the chip to 32 workgroups, 70 us; with two rows a workgroup
+// and one for every piece that there may be, 52K workgroups took 16 us to come
+// and go.
+constexpr int kMergeRows = 4;
+template <bool kBF16, int D, int G, bool kHalf>
+__global__ __launch_bounds__(256) void varlen_mx4_merge_kernel(VarlenParams p) {
+  constexpr int LPR = D / 4, NG = 4, ROWS = 256 / LPR / NG;  // rows per pass
+  constexpr int rows = kHalf ? kRowsPerWG / 2 : kRowsPerWG;  // of a piece's partials
+  static_assert(split_pieces(kSplitOver) <= 128, "two heads a lane");
+  __shared__ __align__(16) float s_o[ROWS * NG * D];
+  __shared__ float2 s_ml[ROWS * NG];
+  const int xcd = (int)blockIdx.x % kXcds, item = (int)blockIdx.x / kXcds;
+  const int lane = threadIdx.x & 63;
+  // The heads were written for slots below the count alone; the others are read
+  // as they are.
+  const int count = p.part_count[xcd];
+  const int4* const heads = p.part_head + (int64_t)xcd * p.split_slots;
+  const int h0 = lane < p.split_slots ? heads[lane].x : 0;
+  const int h1 = lane + 64 < p.split_slots ? heads[lane + 64].x : 0;
+  const uint64_t f0 = __builtin_amdgcn_ballot_w64(lane < count && h0 > 0);
+  const uint64_t f1 = __builtin_amdgcn_ballot_w64(lane + 64 < count && h1 > 0);
+  const int n0 = __popcll(f0);
+  if (item >= n0 + __popcll(f1)) return;
+  const uint64_t f = item < n0 ? f0 : f1;
+  const int nth = item < n0 ? item : item - n0;
+  const int below = __builtin_amdgcn_mbcnt_hi((uint32_t)(f >> 32),
+                                              __builtin_amdgcn_mbcnt_lo((uint32_t)f, 0));
+  const int slot = __builtin_ctzll(__builtin_amdgcn_ballot_w64((f >> lane & 1) && below == nth)) +
+                   (item < n0 ? 0 : 64);
+  const int64_t ps = (int64_t)xcd * p.split_slots + slot;
+  const int4 hd = p.part_head[ps];
+  const int col = threadIdx.x % LPR, grp = threadIdx.x / LPR % NG, rw = threadIdx.x / LPR / NG;
+  for (int row0 = (int)blockIdx.y * kMergeRows;
+       row0 < min((int)blockIdx.y * kMergeRows + kMergeRows, hd.z); row0 += ROWS) {
+    const int row = row0 + rw;
+    float M = -1.0e30f, L = 0.f;
+    f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
+    if (row < hd.z) {
+      const float* po = p.part_o + (ps * rows + row) * D + 4 * col;
+      const float2* pm = p.part_ml + ps * rows + row;
+      for (int j0 = grp; j0 < hd.x; j0 += 4 * NG) {
+        f32x4_t oj[4];
+        float2 ml[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int64_t at = min(j0 + j * NG, hd.x - 1) * (int64_t)rows;
+          ml[j] = pm[at];
+          oj[j] = *reinterpret_cast<const f32x4_t*>(po + at * D);
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          if (j0 + j * NG >= hd.x) break;
+          const float mn = fmaxf(M, ml[j].x);
+          const float a = fast_exp2(M - mn), b = fast_exp2(ml[j].x - mn);
+          acc = acc * a + oj[j] * b;
+          L = L * a + ml[j].y * b;
+          M = mn;
+        }
+      }
+    }
+    __syncthreads();  // the last pass's sums have been read
+    *reinterpret_cast<f32x4_t*>(s_o + (rw * NG + grp) * D + 4 * col) = acc;
+    if (col == 0) s_ml[rw * NG + grp] = make_float2(M, L);
+    __syncthreads();
+    if (grp != 0 || row >= hd.z) continue;
+    M = -1.0e30f;
+#pragma unroll
+    for (int g = 0; g < NG; ++g) M = fmaxf(M, s_ml[rw * NG + g].x);
+    L = 0.f;
+    acc = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int g = 0; g < NG; ++g) {
+      const float b = fast_exp2(s_ml[rw * NG + g].x - M);
+      L += s_ml[rw * NG + g].y * b;
+      acc += b * *reinterpret_cast<const f32x4_t*>(s_o + (rw * NG + g) * D + 4 * col);
+    }
+    const float inv = L > 0.f ? 1.f / L : 0.f;
+    uint2 w;
+    w.x = Mma<kBF16>::pack2(acc[0] * inv, acc[1] * inv);
+    w.y = Mma<kBF16>::pack2(acc[2] * inv, acc[3] * inv);
+    *reinterpret_cast<uint2*>(p.out + (int64_t)(hd.y + row / G) * p.o_st +
+                              (int64_t)(hd.w * G + row % G) * p.o_sh + col * 8) = w;
+  }
+}
+
 // Launch the persistent grid: per XCD, as many workgroups as the kernel
 // keeps resident on one XCD's CUs, or fewer when the XCD's item list (at
 // most items_per_xcd long) is shorter.
@@ -1521,12 +1669,19 @@ static void launch_grid(const VarlenParams& p, int64_t items_per_xcd, hipStream_
   }
   int64_t cus_per_xcd = current_device_cus() / kXcds;
   if (cus_per_xcd < 1) cus_per_xcd = 1;
+  const int64_t list_per_xcd = std::max<int64_t>(items_per_xcd, 1);
   int64_t per_xcd = (int64_t)per_cu * cus_per_xcd;
   if (per_xcd > items_per_xcd && !kSplit) per_xcd = items_per_xcd;
   if (per_xcd < 1) per_xcd = 1;
   hipLaunchKernelGGL(kern, dim3((unsigned)(per_xcd * kXcds)), dim3(kVarlenThreads), 0, st, p);
-  if constexpr (kSplit)
-    hipLaunchKernelGGL((varlen_merge_kernel<kBF16, D, G, kHalf, kMx4>),
+  if constexpr (kSplit && kMx4) {
+    // Split items of an XCD: two pieces each at least, and no more than its items.
+    const int64_t items = std::min<int64_t>(p.split_slots / 2, list_per_xcd);
+    hipLaunchKernelGGL((varlen_mx4_merge_kernel<kBF16, D, G, kHalf>),
+                       dim3((unsigned)items * kXcds, (kHalf ? 64 : 128) / kMergeRows), dim3(256),
+                       0, st, p);
+  } else if constexpr (kSplit)
+    hipLaunchKernelGGL((varlen_merge_kernel<kBF16, D, G, kHalf>),
                        dim3(p.split_slots * kXcds, kHalf ? 2 : 4), dim3(256), 0, st, p);
 }
 
