@@ -413,7 +413,7 @@ int va_varlen_attention_mx4(const va_varlen_args* args, const va_mx4_scales* sca
  * request whose rows[i] is outside the table has slots and entries -1, and so
  * has a token whose column is past the table's width or whose block id is
  * negative.  Tokens past max_tokens are not written; entries of positions and
- * slot_mapping behind the last token are 0 and -1.
+ * slot_mapping behind the last token are 0 and -1.  Sums stop at 2^31 - 1.
  *
  * With free_count, request i holds the blocks of its computed tokens (columns
  * below ceil(num_computed[i] / block_size)), and the blocks of its new columns
@@ -421,8 +421,9 @@ int va_varlen_attention_mx4(const va_varlen_args* args, const va_mx4_scales* sca
  * and ascending columns, is free_blocks[free_count - 1 - k].  They are written
  * to the request's row of request_tables (rows[i] must then be distinct);
  * columns past its width are not taken.  When the list runs out, the columns
- * left get -1, and so the slots.  free_count is not written: totals
- * says what is left, and a launch with the same inputs gives the same outputs.
+ * left get -1, and so the slots.  free_count is not written, nor may it lie in
+ * totals: totals says what is left, and a launch with the same inputs gives the
+ * same outputs.
  */
 typedef struct va_batch_args {
   uint32_t struct_size; /* sizeof(va_batch_args)                          */

@@ -8,6 +8,7 @@ import torch
 
 from oracle import mx4 as oracle
 from voiceagent_amd import ops
+from voiceagent_amd._native import NativeError
 from voiceagent_amd.engine import DecodeGraphMetadata, prepare_batch, prepare_batch_device
 from voiceagent_amd.layers.attention import PagedAttention
 from voiceagent_amd.layers.context import attention_context
@@ -193,3 +194,46 @@ def test_serving_over_an_mxfp4_pool(dev, layout):
         done = lens
     assert meta.totals[4].item() == 0
     assert count.item() == blocks - sum(-(-n // block) for n in done)
+
+
+def test_sums_past_31_bits(dev):
+    """Lengths whose sums do not fit: cumulative lengths stop at 2^31 - 1, and the
+    rows that there are room for are those of the first request."""
+    top, block = 2 ** 31 - 1, 16
+    t = torch.tensor([[5, 6], [7, 8], [9, 10]], dtype=torch.int32, device=dev)
+    lens = torch.tensor([2 ** 31 - 100, 2 ** 40, 2 ** 31 - 1], device=dev)
+    for done in ([0, 0, 0], [2 ** 31 - 110, 0, 0]):
+        free = torch.arange(20, dtype=torch.int32, device=dev)
+        m = ops.batch_metadata(lens, torch.tensor(done, device=dev), t, block, max_tokens=40,
+                               free_blocks=free, free_count=free[7:8].clone())
+        first = 2 ** 31 - 100 - done[0]
+        most = top - block
+        assert m.cu_seqlens_k.tolist() == [0, 2 ** 31 - 100, top, top]
+        assert m.cu_seqlens_q.tolist() == [0, first, min(top, first + most), top]
+        pos = (list(range(done[0], 2 ** 31 - 100)) if first < 40 else list(range(40)))
+        want = (pos + list(range(40)))[:40]
+        assert m.positions.tolist() == want
+        assert m.totals.tolist()[:3] == [top, most if first < 40 else max(first, most), most]
+
+
+def test_refusals_of_the_wrapper(dev):
+    vec = lambda n, dtype=torch.int32: torch.ones(n, dtype=dtype, device=dev)  # noqa: E731
+    t = torch.zeros(4, 3, dtype=torch.int32, device=dev)
+
+    def call(lens=vec(3), done=vec(3), t=t, block=16, max_tokens=8, **kw):
+        return ops.batch_metadata(lens, done, t, block, max_tokens=max_tokens, **kw)
+
+    out = call()
+    narrow = ops.BatchMetadata(*(getattr(out, f) for f in ("positions", "slot_mapping", "cu_seqlens_q",
+                                                           "cu_seqlens_k")), out.block_tables[:, :2], out.totals)
+    for bad in (dict(lens=vec(3, torch.float32)), dict(done=vec(2)), dict(done=vec(3, torch.int64)),
+                dict(t=t.long()), dict(t=t.t()), dict(t=t[0]), dict(block=0), dict(max_tokens=-1),
+                dict(rows=vec(2)), dict(rows=vec(3, torch.int64)), dict(free_blocks=vec(4)),
+                dict(free_blocks=vec(4), free_count=vec(2)), dict(free_blocks=vec(4, torch.int64), free_count=vec(1)),
+                dict(table_width=-2), dict(lens=vec(3).cpu()), dict(out=narrow), dict(max_tokens=9, out=out),
+                dict(padded_batch=4, out=out),
+                dict(free_blocks=vec(4), free_count=out.free_count, out=out)):
+        with pytest.raises((ops.AttentionArgumentError, NativeError, TypeError)):
+            call(**bad)
+            pytest.fail(f"{list(bad)} was taken")
+    assert call(out=out) is out

@@ -70,20 +70,24 @@ __device__ inline Request load_request(const BatchParams& p, int i) {
   return r;
 }
 
+// Sums of lengths stop at 2^31 - 1, so that no lengths, however wrong, give an
+// index that wraps (the sum of non-negative terms stays associative).
+__device__ inline int sat_add(int a, int b) { return __builtin_elementwise_add_sat(a, b); }
+
 // Sum (or maximum) of x over the workgroup, in every lane.
 template <bool kMax>
 __device__ inline int block_all(int x, int* s) {
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) {
     const int y = __shfl_xor(x, o, 64);
-    x = kMax ? max(x, y) : x + y;
+    x = kMax ? max(x, y) : sat_add(x, y);
   }
   __syncthreads();  // s may still be read from its last use
   if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = x;
   __syncthreads();
   int r = s[0];
 #pragma unroll
-  for (int w = 1; w < kBatchThreads / 64; ++w) r = kMax ? max(r, s[w]) : r + s[w];
+  for (int w = 1; w < kBatchThreads / 64; ++w) r = kMax ? max(r, s[w]) : sat_add(r, s[w]);
   return r;
 }
 
@@ -102,9 +106,9 @@ __global__ __launch_bounds__(kBatchThreads) void batch_metadata_kernel(BatchPara
   int q0 = 0, k0 = 0, take0 = 0, mq = 0, mk = 0;
   for (int i = tid; i < r0; i += kBatchThreads) {
     const Request r = load_request(p, i);
-    q0 += r.len - r.done;
-    k0 += r.len;
-    take0 += r.cols - r.held;
+    q0 = sat_add(q0, r.len - r.done);
+    k0 = sat_add(k0, r.len);
+    take0 = sat_add(take0, r.cols - r.held);
     mq = max(mq, r.len - r.done);
     mk = max(mk, r.len);
   }
@@ -126,9 +130,9 @@ __global__ __launch_bounds__(kBatchThreads) void batch_metadata_kernel(BatchPara
   for (int o = 1; o < 64; o <<= 1) {
     const int a = __shfl_up(q, o, 64), b = __shfl_up(k, o, 64), c = __shfl_up(take, o, 64);
     if (lane >= o) {
-      q += a;
-      k += b;
-      take += c;
+      q = sat_add(q, a);
+      k = sat_add(k, b);
+      take = sat_add(take, c);
     }
   }
   if (lane == 63) {
@@ -138,9 +142,9 @@ __global__ __launch_bounds__(kBatchThreads) void batch_metadata_kernel(BatchPara
   }
   __syncthreads();
   for (int w = 0; w < wave; ++w) {
-    q += s_scan[0][w];
-    k += s_scan[1][w];
-    take += s_scan[2][w];
+    q = sat_add(q, s_scan[0][w]);
+    k = sat_add(k, s_scan[1][w]);
+    take = sat_add(take, s_scan[2][w]);
   }
   if (tid == 0) s_q[0] = s_take[0] = 0;
   if (tid < nr) {
@@ -151,8 +155,8 @@ __global__ __launch_bounds__(kBatchThreads) void batch_metadata_kernel(BatchPara
     s_cols[tid] = mine.cols;
     s_row[tid] = r0 + tid >= p.num_seqs ? -2 : (row >= 0 && row < p.num_req ? row : -1);
     if (stripe == 0) {
-      p.cu_q[r0 + tid + 1] = q0 + q;
-      p.cu_k[r0 + tid + 1] = k0 + k;
+      p.cu_q[r0 + tid + 1] = sat_add(q0, q);
+      p.cu_k[r0 + tid + 1] = sat_add(k0, k);
     }
   }
   if (blockIdx.x == 0 && stripe == 0 && tid == 0) p.cu_q[0] = p.cu_k[0] = 0;
@@ -162,8 +166,8 @@ __global__ __launch_bounds__(kBatchThreads) void batch_metadata_kernel(BatchPara
     mq = block_all<true>(max(mq, mine.len - mine.done), s_red);
     mk = block_all<true>(max(mk, mine.len), s_red);
     if (tid == 0) {
-      const int taken = take0 + s_take[nr];
-      p.totals[0] = q0 + total;
+      const int taken = sat_add(take0, s_take[nr]);
+      p.totals[0] = sat_add(q0, total);
       p.totals[1] = mq;
       p.totals[2] = mk;
       p.totals[3] = max(0, count - taken);
@@ -175,13 +179,14 @@ __global__ __launch_bounds__(kBatchThreads) void batch_metadata_kernel(BatchPara
   auto block_at = [&](int r, int c) -> int {
     if (s_row[r] < 0 || c >= s_cols[r]) return -1;
     if (c < s_held[r]) return p.req[(int64_t)s_row[r] * p.req_stride + c];
-    const int at = count - 1 - (take0 + s_take[r] + c - s_held[r]);
+    const int64_t at = count - 1 - ((int64_t)take0 + s_take[r] + c - s_held[r]);
     return at >= 0 ? p.free_blocks[at] : -1;
   };
 
   // Tokens.
-  for (int t = stripe * kBatchThreads + tid; t < total; t += stripes * kBatchThreads) {
-    if (q0 + t >= p.max_tokens) break;
+  const int room = p.max_tokens > q0 ? min(total, p.max_tokens - q0) : 0;
+  for (int64_t i = stripe * kBatchThreads + tid; i < room; i += stripes * kBatchThreads) {
+    const int t = (int)i;
     int lo = 0, hi = nr;  // the last request whose first token is at most t
     while (hi - lo > 1) {
       const int mid = (lo + hi) >> 1;
@@ -252,6 +257,9 @@ extern "C" int va_batch_metadata(const va_batch_args* a, void* stream) {
   VA_CHECK_ARG(a->free_count ? a->free_blocks != nullptr || a->free_capacity == 0
                              : a->free_blocks == nullptr,
                "va_batch_metadata: free_blocks and free_count must be given together");
+  VA_CHECK_ARG(!a->free_count || (uintptr_t)a->free_count + 4 <= (uintptr_t)a->totals ||
+                   (uintptr_t)a->free_count >= (uintptr_t)(a->totals + 5),
+               "va_batch_metadata: free_count must not lie in totals (which the launch writes)");
 
   BatchParams p;
   p.lens = a->lens;

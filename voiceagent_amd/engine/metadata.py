@@ -172,7 +172,8 @@ class DecodeGraphMetadata:
     ) -> tuple[int, ops.BatchMetadata]:
         """:meth:`stage` for requests whose state is on the GPU: one launch
         fills the static buffers of the bucket that holds the batch.  Every
-        request contributes its last token (``num_computed = lens - 1``); the
+        request contributes its last token (``lens >= 1`` and ``num_computed =
+        lens - 1``); the
         result's totals say how many tokens there were and, with a free list,
         what is left of it.  Returns the bucket and the metadata."""
         batch = int(lens.numel())
