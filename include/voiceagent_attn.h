@@ -340,7 +340,9 @@ size_t va_varlen_split_workspace_bytes(const va_varlen_args* args);
  * byte s stands for c * 2^(s - 127).  Its va_kv_pool gives the codes, strides
  * counting bytes; va_mx4_scales gives the scales, addressed alike.  The pool's
  * k_scale / v_scale are not read.  Rows of codes are 16-byte aligned, rows of
- * scales aligned to D / 32 bytes where that is 2, 4 or 8.
+ * scales aligned to D / 32 bytes where that is 2, 4 or 8.  At head_dim 64 the
+ * scales' block stride is a multiple of 4: attention finds a row's pair in an
+ * aligned 4-byte word.
  *
  * A store quantises 16-bit rows: the scale is the smallest 2^e with
  * max |x| < 7 * 2^e over the group, with e in [-125, 125] for bf16 rows and
@@ -379,7 +381,8 @@ typedef struct va_load_args {
 } va_load_args;
 
 /* The rows stored at slot_mapping, as 16-bit values (exact in the type they
- * were stored from): the inverse of va_store_kvcache_mx4. */
+ * were stored from): the inverse of va_store_kvcache_mx4.  The pool has a block
+ * at least. */
 int va_load_kvcache_mx4(const va_load_args* args, const va_mx4_scales* scales, void* stream);
 
 /* va_paged_decode over an MXFP4 pool: bf16 / f16 q, head_dim 64 / 128 / 256,
@@ -393,7 +396,7 @@ size_t va_paged_decode_mx4_workspace_bytes(const va_decode_args* args);
 
 /* va_varlen_attention over an MXFP4 pool: head_dim 64 / 128, no query
  * prologue.  Prefix rows are converted inside the kernel; new rows are attended
- * as given and stored quantised after the attention.  The workspace is
+ * as given and stored quantised in the same launch.  The workspace is
  * va_varlen_split_workspace_bytes'. */
 int va_varlen_attention_mx4(const va_varlen_args* args, const va_mx4_scales* scales,
                             void* stream);

@@ -9,6 +9,10 @@ import torch
 from oracle import mx4 as oracle
 from tests.mx4_common import Pool, close, cu, slots_of, tables_for
 from voiceagent_amd import ops
+from voiceagent_amd._native import NativeError
+from voiceagent_amd.layers.attention import PagedAttention
+from voiceagent_amd.layers.context import AttentionContext, attention_context
+from voiceagent_amd.layers.qwen3 import Qwen3AttentionCore
 
 pytestmark = pytest.mark.gpu
 
@@ -426,3 +430,208 @@ def test_varlen_blocks_outside_the_pool(dev):
         tables[1, 0] = 10 ** 6
 
     run_varlen(dev, [150, 90], [40, 10], edit=edit, seed=4)
+
+
+@pytest.mark.parametrize("d, hq, hkv", [(128, 8, 2), (64, 4, 1)])
+def test_varlen_dead_places_hold_anything(dev, d, hq, hkv):
+    # NaN groups in every place that no prefix row holds, the ends of the
+    # prefixes' last blocks (inside a tile) among them.
+    prefixes = [1, 70, 0, 129]
+
+    def edit(pool, tables):
+        live = torch.zeros(pool.cpu[0].shape[0] * 16, dtype=torch.bool)
+        for b, n in enumerate(prefixes):
+            live[slots_of(tables[b], n, 16)] = True
+        for t in (2, 3):
+            pool.cpu[t].flatten(0, 1)[~live] = 255
+        for t in (0, 1):
+            pool.cpu[t].flatten(0, 1)[~live] = 0x7f
+
+    run_varlen(dev, prefixes, [3, 40, 20, 1], hq=hq, hkv=hkv, d=d, edit=edit, seed=5)
+
+
+# ------------------------------------------------------- heads, views, streams
+@pytest.mark.parametrize("hq, hkv, d", [(14, 7, 64), (3, 3, 64), (6, 3, 128), (5, 5, 256)])
+@pytest.mark.parametrize("layout", ["nhd", "hnd"])
+def test_odd_head_counts(dev, hq, hkv, d, layout):
+    # At head_dim 64 every second row's scales start inside a word.
+    run_decode(dev, [1, 33, 200, 16], hq=hq, hkv=hkv, d=d, layout=layout, new=True, seed=hkv)
+    if d <= 128:
+        run_varlen(dev, [0, 33, 100], [5, 3, 70], hq=hq, hkv=hkv, d=d, layout=layout, seed=hkv)
+
+
+@pytest.mark.parametrize("shift", [-100, 100])
+def test_scales_of_any_size(dev, shift):
+    # Key groups near both ends of the scales' range.
+    def edit(pool, tables):
+        pool.cpu[2] = (pool.cpu[2].int() + shift).clamp(2, 252).to(torch.uint8)
+
+    run_decode(dev, [40, 300], edit=edit, scale=128 ** -0.5 * 2.0 ** -shift, seed=30)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+def test_pools_inside_larger_tensors(dev, d):
+    """Keys and values side by side in one tensor a block, and a pool whose heads
+    and slots are transposed: the same results as from a pool of their own."""
+    gen = torch.Generator().manual_seed(31)
+    blocks, hkv, n = 12, 2, 90
+    own = Pool(gen, blocks, 16, hkv, d, "nhd", BF16, dev)
+    both = [torch.zeros(blocks, 2, 16, hkv, w, dtype=torch.uint8, device=dev) for w in (d // 2, d // 32)]
+    turned = [torch.zeros(2, blocks, hkv, 16, w, dtype=torch.uint8, device=dev).transpose(2, 3)
+              for w in (d // 2, d // 32)]
+    table = torch.randperm(blocks, generator=gen)[:6].int()[None].to(dev)
+    slots = slots_of(table[0].cpu(), n, 16).to(dev)
+    rows = [torch.randn(n, hkv, d, generator=gen).to(BF16).to(dev) for _ in range(2)]
+    new = [torch.randn(1, hkv, d, generator=gen).to(BF16).to(dev) for _ in range(2)]
+    q = torch.randn(40, 8, d, generator=gen).to(BF16).to(dev)
+
+    def run(kc, vc, ks, vs):
+        kc, vc = (t.view(ops.MXFP4_KV_DTYPE) for t in (kc, vc))
+        kw = {"k_scale": ks.view(ops.MXFP4_SCALE_DTYPE), "v_scale": vs.view(ops.MXFP4_SCALE_DTYPE)}
+        ops.store_kvcache(rows[0], rows[1], kc, vc, slots, **kw)
+        loaded = ops.load_kvcache(kc, vc, slots, **kw)
+        one = ops.paged_decode(q[:1], kc, vc, table, torch.tensor([n + 1], device=dev), max_seq_len=n + 1,
+                               scale=0.1, new_k=new[0], new_v=new[1], **kw)
+        cq, ck = cu([40]).to(dev), cu([n]).to(dev)
+        many = ops.varlen_attention(q, None, None, cq, ck, 40, n, scale=0.1, causal=True, k_cache=kc,
+                                    v_cache=vc, block_tables=table, **kw)
+        return (*loaded, one, many, *(t[slots // 16, slots % 16] for t in (kc.view(torch.uint8), ks.view(torch.uint8))))
+
+    want = run(own.gpu[0], own.gpu[1], own.gpu[2], own.gpu[3])
+    for c, s in ((both[0].unbind(1), both[1].unbind(1)), (turned[0], turned[1])):
+        for a, b in zip(run(c[0], c[1], s[0], s[1]), want):
+            assert torch.equal(a, b)
+
+
+def test_wrappers_refuse(dev):
+    k, v, ks, vs = ops.mxfp4_kv_pool(4, 16, 2, 128, device=dev)
+    kw = {"k_scale": ks, "v_scale": vs}
+    x = torch.zeros(3, 2, 128, dtype=BF16, device=dev)
+    q = torch.zeros(3, 4, 128, dtype=BF16, device=dev)
+    slots = torch.zeros(3, dtype=torch.int32, device=dev)
+    table = torch.zeros(3, 2, dtype=torch.int32, device=dev)
+    vec = cu([1, 1, 1]).to(dev)
+
+    def store(x=x, k=k, v=v, **more):
+        ops.store_kvcache(x, x, k, v, slots, **{**kw, **more})
+
+    def load(k=k, v=v, slots=slots, dtype=BF16, **more):
+        ops.load_kvcache(k, v, slots, dtype, **{**kw, **more})
+
+    def decode(q=q, k=k, v=v, **more):
+        ops.paged_decode(q, k, v, table, vec, lens_cumulative=True, max_seq_len=20, scale=1.0, **{**kw, **more})
+
+    def varlen(q=q, k=k, v=v, **more):
+        ops.varlen_attention(q, None, None, vec, vec, 1, 1, scale=1.0, causal=True, k_cache=k, v_cache=v,
+                             block_tables=table, **{**kw, **more})
+
+    wide = torch.zeros(4, 16, 2, 128, dtype=BF16, device=dev)
+    odd = [t[:, :, :1] for t in (ks, vs)]
+    small = ops.mxfp4_kv_pool(4, 8, 2, 128, device=dev)
+    calls = [lambda f=f, m=m: f(**m) for f in (store, load, decode, varlen) for m in (
+        {"k_scale": 1.0, "v_scale": 1.0}, {"v_scale": 1.0}, {"k_scale": ks.view(torch.uint8)},
+        {"k_scale": odd[0], "v_scale": odd[1]}, {"k": wide, "v": wide}, {"k_scale": ks.cpu(), "v_scale": vs.cpu()},
+        {"layout": "dhn"})]
+    calls += [lambda: store(x=x.float()), lambda: load(dtype=torch.float32), lambda: decode(q=q.float()),
+              lambda: varlen(q=q.float()), lambda: load(slots=slots[None]),
+              lambda: decode(no_alloc=True, out=torch.empty_like(q)), lambda: decode(q=q[:, :3]),
+              lambda: decode(k=small[0], v=small[1], k_scale=small[2], v_scale=small[3]),
+              lambda: varlen(k=small[0], v=small[1], k_scale=small[2], v_scale=small[3]),
+              lambda: decode(q=torch.zeros(3, 6, 128, dtype=BF16, device=dev))]
+    for i, call in enumerate(calls):
+        with pytest.raises((ops.AttentionArgumentError, NativeError, TypeError)):
+            call()
+            pytest.fail(f"call {i} was taken")
+    torch.cuda.synchronize()
+
+
+def test_two_streams_at_once(dev):
+    gen = torch.Generator().manual_seed(33)
+    lens = [5000, 300, 20]
+    pool = Pool(gen, 340, 16, 2, 128, "nhd", BF16, dev)
+    (kc, vc), kw = pool.args()
+    tables = tables_for(gen, lens, 16, 340).to(dev)
+    vec = torch.tensor(lens, device=dev)
+    qs = [torch.randn(3, 8, 128, generator=gen).to(BF16).to(dev) for _ in range(4)]
+
+    def call(q):
+        return ops.paged_decode(q, kc, vc, tables, vec, max_seq_len=5000, scale=0.1, **kw)
+
+    want = [call(q) for q in qs]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    got = []
+    for i, q in enumerate(qs * 3):
+        with torch.cuda.stream(streams[i % 2]):
+            got.append(call(q))
+    torch.cuda.synchronize()
+    for i, o in enumerate(got):
+        assert torch.equal(o, want[i % 4])
+
+
+@pytest.mark.parametrize("layout", ["nhd", "hnd"])
+def test_layer_without_the_fused_store(dev, layout):
+    """The layer's unfused path (store, then attention over the pool) against its
+    fused one: a decode step is the same; a prompt then attends its rows as stored."""
+    gen = torch.Generator().manual_seed(34)
+    hq, hkv, d, block = 8, 2, 128, 16
+    outs, pools = [], []
+    lens = [20, 35]
+    pre = torch.randn(55, hq + 2 * hkv, d, generator=gen).to(BF16)
+    step = torch.randn(2, hq + 2 * hkv, d, generator=gen).to(BF16)
+    tables = torch.tensor([[4, 1, 0], [2, 5, 3]], dtype=torch.int32)
+    for fused in (True, False):
+        layer = PagedAttention(hq, d, d ** -0.5, hkv)
+        pool = ops.mxfp4_kv_pool(6, block, hkv, d, device=dev, layout=layout)
+        layer.kv_layout, layer.fuse_store = layout, fused
+        layer.k_cache, layer.v_cache, layer.k_scale, layer.v_scale = pool
+        for qkv, q, k in ((pre, lens, lens), (step, [1, 1], [21, 36])):
+            slots = torch.cat([slots_of(t, n, block)[n - m:] for t, n, m in zip(tables, k, q)])
+            gpu = qkv.to(dev)
+            with attention_context(AttentionContext(
+                    cu_seqlens_q=cu(q).to(dev), cu_seqlens_k=cu(k).to(dev), max_seqlen_q=max(q),
+                    max_seqlen_k=max(k), slot_mapping=slots.int().to(dev), block_tables=tables.to(dev))):
+                out = layer(gpu[:, :hq], gpu[:, hq:hq + hkv], gpu[:, hq + hkv:])
+            outs.append(out)
+        pools.append([t.view(torch.uint8).cpu() for t in pool])
+    assert all(torch.equal(a, b) for a, b in zip(*pools))
+    assert torch.equal(outs[1], outs[3])
+    at = 0
+    for n in lens:  # the unfused prompt
+        q = pre[at:at + n, :hq]
+        k, v = (oracle.values(*oracle.quantise(pre[at:at + n, i:i + hkv])) for i in (hq, hq + hkv))
+        seen = torch.ones(n, n).tril().bool()
+        ref, tol = oracle.attend(q, k, v, seen, d ** -0.5, BF16, VARLEN_BITS)
+        close(outs[2][at:at + n], ref, tol)
+        at += n
+
+
+def test_qwen3_core_over_an_mxfp4_pool(dev):
+    """The fused decode step is the standalone prologue and the plain layer's step."""
+    gen = torch.Generator().manual_seed(35)
+    hq, hkv, d, block = 16, 8, 128, 16
+    k_lens = [21, 36]
+    tables = torch.tensor([[4, 1, 0], [2, 5, 3]], dtype=torch.int32)
+    x = torch.randn(2, hq + 2 * hkv, d, generator=gen).to(BF16).to(dev)
+    positions = torch.tensor([20, 35], device=dev)
+    slots = torch.cat([slots_of(t, n, block)[-1:] for t, n in zip(tables, k_lens)]).int().to(dev)
+    context = AttentionContext(cu_seqlens_q=cu([1, 1]).to(dev), cu_seqlens_k=cu(k_lens).to(dev),
+                               max_seqlen_q=1, max_seqlen_k=36, slot_mapping=slots,
+                               block_tables=tables.to(dev))
+    got = []
+    for core in (True, False):
+        pool = Pool(torch.Generator().manual_seed(36), 6, block, hkv, d, "nhd", BF16, dev)
+        (kc, vc), kw = pool.args()
+        layer = Qwen3AttentionCore(hq, d, hkv, max_position=64).to(dev)
+        layer.k_cache, layer.v_cache, layer.k_scale, layer.v_scale = kc, vc, kw["k_scale"], kw["v_scale"]
+        q, k, v = x[:, :hq], x[:, hq:hq + hkv], x[:, hq + hkv:]
+        with attention_context(context):
+            if core:
+                out = layer(positions, q, k, v)
+            else:
+                qn, kn = ops.qk_norm_rope(q, k, layer.prologue(positions))
+                out = PagedAttention.forward(layer, qn, kn, v)
+        got.append((out.reshape(2, -1), pool.gpu))
+    assert torch.equal(got[0][0], got[1][0])
+    assert all(torch.equal(a, b) for a, b in zip(got[0][1], got[1][1]))

@@ -189,3 +189,50 @@ def test_wrappers_refuse_cpu_tensors():
         ops.load_kvcache(k, v, slots, k_scale=ks, v_scale=vs)
     with pytest.raises(ops.AttentionArgumentError):
         ops.batch_metadata(slots, slots, slots.view(1, 3), 16, max_tokens=3)
+
+
+def test_batch_metadata_refuses_a_count_inside_its_totals():
+    lib = N.lib()
+    a = N.new_args(N.BatchArgs)
+    a.positions = a.slot_mapping = a.cu_seqlens_q = a.cu_seqlens_k = a.lens = a.num_computed = 1 << 16
+    a.totals, a.free_blocks, a.free_capacity = 1 << 17, 1 << 18, 4
+    a.num_seqs = a.padded_seqs = 1
+    a.block_size = 16
+    for entry in range(5):
+        a.free_count = (1 << 17) + 4 * entry
+        assert lib.va_batch_metadata(ctypes.byref(a), None) == -1
+        assert "totals" in N.last_error()
+
+
+def test_head_dim_64_scale_blocks_start_on_words():
+    lib = N.lib()
+    for fn, make in CALLS.items():
+        a, s = make()
+        a.head_dim = 64
+        s.stride_head, s.stride_slot, s.stride_block = 2, 6, 16 * 6 + 2
+        assert getattr(lib, fn)(ctypes.byref(a), ctypes.byref(s), None) < 0
+        assert "block stride" in N.last_error()
+
+
+def test_load_refusals():
+    lib = N.lib()
+
+    def call(change):
+        p, s = _pool()
+        a = N.new_args(N.LoadArgs)
+        a.dtype, a.key, a.value, a.pool = 0, 1 << 16, 1 << 16, p
+        a.key_stride_tok = a.value_stride_tok = 1024
+        a.key_stride_head = a.value_stride_head = 128
+        a.slot_mapping, a.num_tokens, a.num_kv_heads, a.head_dim = 1 << 16, 4, 8, 128
+        change(a, s)
+        assert lib.va_load_kvcache_mx4(ctypes.byref(a), ctypes.byref(s), None) < 0
+        return N.last_error()
+
+    assert "struct_size" in call(lambda a, s: setattr(a, "struct_size", 8))
+    assert "empty pool" in call(lambda a, s: setattr(a.pool, "num_blocks", 0))
+    assert "kv_format" in call(lambda a, s: setattr(a.pool, "kv_format", N.VA_KV_NATIVE))
+    assert "slot_dtype" in call(lambda a, s: setattr(a, "slot_dtype", 9))
+    assert "16-byte" in call(lambda a, s: setattr(a, "key", (1 << 16) + 2))
+    assert "16-byte" in call(lambda a, s: setattr(a, "value_stride_tok", 1028))
+    assert "null" in call(lambda a, s: setattr(a, "slot_mapping", None))
+    assert "dtype" in call(lambda a, s: setattr(a, "dtype", N.VA_F32))

@@ -110,11 +110,6 @@ __device__ inline mx_f32x4 mx4_mfma(uint4 a, int as, const mx_i32x8& b, int bs, 
   return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(av, b, c, 4 /* e2m1 */, 0 /* e4m3 */, 0,
                                                           as, 0, bs);
 }
-__device__ inline mx_f32x4 mx4_mfma(uint4 a, int as, uint4 b0, uint4 b1, int bs, mx_f32x4 c) {
-  const mx_i32x8 bv = {(int)b0.x, (int)b0.y, (int)b0.z, (int)b0.w,
-                       (int)b1.x, (int)b1.y, (int)b1.z, (int)b1.w};
-  return mx4_mfma(a, as, bv, bs, c);
-}
 
 // N e4m3 terms of 16 elements of ET (two words of 8), for the power of two
 // `unit`: term 0 rounds x / unit to e4m3, term t what the terms before it left,

@@ -14,15 +14,18 @@
 //     of two of its own, so that the products lose nothing of it.  The
 //     instruction aligns the products of neighbouring k before adding: sums
 //     came out within 4.2e-5 of the norm of the products (rms 4e-6 over 12800
-//     sums), against 2^-9 by which P is rounded below.
-//   * O^T += V^T P^T takes V in 16 bits.  A lane holds D / 16 neighbouring
-//     elements of eight tokens (one load a token), converts them with their
-//     scales (two elements an instruction) and pairs tokens with v_perm: no
-//     LDS and no transposing read.  P^T is the S^T accumulator packed in place.
+//     sums), against 2^-8 of each P, its rounding below.
+//   * O^T += V^T P^T takes V in 16 bits.  A lane reads D / 16 neighbouring
+//     elements of eight tokens, converts them with their scales (two elements
+//     an instruction) and pairs tokens with v_perm: no transposing read.  P^T
+//     is the S^T accumulator packed in place, rounded to the rows' type (the
+//     type of the matrix product; its row sum adds the unrounded values).
 //
 // A workgroup is W waves; wave w takes the partition's 32-token steps w, w + W,
-// ... with no barrier, its loads going straight to registers, one step or more
-// ahead.  The waves merge through LDS at the end.
+// ... with no barrier, through a ring of S steps in LDS of its own that DMA
+// fills S - 1 steps ahead.  (Loads to registers made the compiler wait for each
+// at the joins of the branches behind them.)  The waves merge through LDS at
+// the end.
 #pragma once
 
 #include "mx4.h"

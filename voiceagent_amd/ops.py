@@ -843,10 +843,12 @@ def varlen_attention(
     launch's choice of items (the block table may be wider).  An FP8 pool
     (float8_e4m3fn codes, values code * k_scale / v_scale) is converted tile
     by tile inside the kernel (no workspace); its new rows are stored
-    quantised after the attention.  So is an MXFP4 pool, with its scale tensors
-    as k_scale / v_scale (blocks of a multiple of 16 tokens).  With a ``prologue`` (causal, head_dim
-    128, a 16-bit pool or none), q holds the raw query projections and the
-    launch normalises and rotates them at ``prologue.positions`` (one per
+    quantised after the attention.  An MXFP4 pool (:func:`mxfp4_kv_pool`, blocks
+    of a multiple of 16 tokens), with its scale tensors as k_scale / v_scale, is
+    converted inside the kernel too, which also stores the new rows; the new
+    rows themselves are attended as given.  With a ``prologue`` (causal,
+    head_dim 128, a 16-bit pool or none), q holds the raw query projections and
+    the launch normalises and rotates them at ``prologue.positions`` (one per
     query token); k and the pool must hold processed keys.
     """
     mx4 = isinstance(k_scale, torch.Tensor)
@@ -1020,7 +1022,8 @@ def batch_metadata(
     (``rows`` must be distinct); columns that the list does not reach get -1
     there, and so do their slots.  ``free_count`` itself is not changed: the
     count left is ``totals[3]`` (``result.free_count``), the blocks that were
-    missing ``totals[4]``.
+    missing ``totals[4]`` (an ``out`` that free_count lies in is refused: copy
+    the count left into it after the launch).
 
     ``out``: tensors of an earlier result of the same sizes to write into (a
     captured graph's static buffers)."""
