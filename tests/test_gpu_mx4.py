@@ -635,3 +635,64 @@ def test_qwen3_core_over_an_mxfp4_pool(dev):
         got.append((out.reshape(2, -1), pool.gpu))
     assert torch.equal(got[0][0], got[1][0])
     assert all(torch.equal(a, b) for a, b in zip(got[0][1], got[1][1]))
+
+
+# ------------------------------- decode of long contexts, two heads a workgroup
+@pytest.mark.parametrize("dtype, hq, hkv", [(BF16, 4, 2), (F16, 2, 2), (BF16, 16, 2)])
+@pytest.mark.parametrize("new", [False, True])
+def test_decode_two_long_contexts(dev, dtype, hq, hkv, new):
+    run_decode(dev, [16500, 16420], hq=hq, hkv=hkv, dtype=dtype, split=ops.SPLIT_EXACT, new=new, seed=40)
+
+
+@pytest.mark.parametrize("dtype, hq, hkv, split", [(BF16, 8, 2, 0), (F16, 32, 4, 0), (BF16, 4, 4, 300), (BF16, 16, 8, 0)])
+@pytest.mark.parametrize("mask", [False, True])
+def test_decode_many_contexts_under_a_bound(dev, dtype, hq, hkv, split, mask):
+    # Lengths from none to several partitions; the current rows at their ends.
+    lens = [0, 1, 31, 32, 33, 127, 128, 129, 1300, 2500] + [16 * i + 5 for i in range(20)]
+    gen = torch.Generator().manual_seed(41)
+    m = torch.rand(30, 1400, generator=gen) > 0.3 if mask else None
+    if mask:
+        m[5] = False
+    run_decode(dev, lens, hq=hq, hkv=hkv, dtype=dtype, bound=32768, split=split, new=True, mask=m, seed=42)
+
+
+def test_decode_pairs_agree_with_single_heads(dev):
+    """A pool of 128-byte rows of head pairs against the same rows head-major,
+    with the prologue, the current row and two replays of one graph."""
+    gen = torch.Generator().manual_seed(43)
+    lens = [3000, 17, 900, 1] * 8
+    blocks = sum(-(-n // 16) for n in lens)
+    pool = Pool(gen, blocks, 16, 2, 128, "nhd", BF16, dev)
+    hnd = [t.transpose(1, 2).contiguous() for t in pool.gpu]
+    tables = tables_for(gen, lens, 16, blocks).to(dev)
+    q, k, v = (torch.randn(32, n, 128, generator=gen).to(BF16).to(dev) for n in (8, 2, 2))
+    pro = ops.QKPrologue(torch.rand(128, generator=gen).to(BF16).to(dev),
+                         torch.rand(128, generator=gen).to(BF16).to(dev), 1e-6,
+                         torch.randn(3000, 128, generator=gen).to(dev),
+                         torch.tensor([n - 1 for n in lens], device=dev))
+    vec = torch.tensor(lens, device=dev)
+
+    def call(pools, layout, out=None):
+        kc, vc = (t.view(ops.MXFP4_KV_DTYPE) for t in pools[:2])
+        ks, vs = (t.view(ops.MXFP4_SCALE_DTYPE) for t in pools[2:])
+        return ops.paged_decode(q, kc, vc, tables, vec, max_seq_len=32768, scale=0.08, new_k=k, new_v=v,
+                                prologue=pro, layout=layout, k_scale=ks, v_scale=vs, out=out)
+
+    one, two = call(hnd, "hnd"), call(pool.gpu, "nhd")
+    # (partitions differ, so sums are in another order: half a step of the
+    # output each, and P's and the sums' rounding, at values below 4)
+    assert (one.float() - two.float()).abs().max() <= 2 * 2.0 ** -8 * 4 + 2 * 2.0 ** -8 * 4
+    assert all(torch.equal(a, b.transpose(1, 2)) for a, b in zip(hnd, pool.gpu))
+    out = torch.empty_like(q)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        call(pool.gpu, "nhd", out)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        call(pool.gpu, "nhd", out)
+    for _ in range(3):
+        out.zero_()
+        graph.replay()
+        assert torch.equal(out, two)

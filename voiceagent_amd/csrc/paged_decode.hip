@@ -99,7 +99,7 @@ static int nosplit_tokens_for(const va_decode_args* a) {
 // The split of a launch whose workgroups take `unit` tokens a round, with
 // contexts of up to `nosplit` tokens (at 8 partitions a pair) kept whole.
 static DecodePlan plan_split(const va_decode_args* a, int unit, int64_t nosplit,
-                             int grain = kDynGrain) {
+                             int grain = kDynGrain, int heads_per_wg = 1) {
   DecodePlan pl{};
   const int G = a->num_kv_heads > 0 ? a->num_heads / a->num_kv_heads : 1;
   int max_len = a->max_seq_len > 0 ? a->max_seq_len : 1;
@@ -124,7 +124,8 @@ static DecodePlan plan_split(const va_decode_args* a, int unit, int64_t nosplit,
     // above 768, B = 16 (2 partitions) above 1536.  A max_seq_len that is
     // only an upper bound (max_model_len) keeps the split.
     const int64_t cus = current_device_cus();
-    const int64_t want = pairs >= cus ? 1 : cus / (pairs > 0 ? pairs : 1);
+    const int64_t most = cus * heads_per_wg;
+    const int64_t want = pairs >= most ? 1 : most / (pairs > 0 ? pairs : 1);
     int64_t parts = want;
     if (parts > 1 && (int64_t)max_len * (parts < 8 ? parts : 8) <= nosplit * 8)
       parts = 1;
@@ -200,8 +201,35 @@ static DecodePlan plan_decode(const va_decode_args* a) {
 constexpr int64_t kMx4NoSplitTokens = 512;
 constexpr int kMx4MinPart = 64;
 
+// Whether a workgroup serves two kv heads.  At head_dim 128 their codes of a
+// token in an NHD pool are one 128-byte line, which two workgroups would each
+// request whole; together they need half as many workgroups, and as many more
+// partitions.  One head / two, us (16 query / 8 kv heads, contexts within 10% of
+// the length): 2 x 4096 11.2 / 9.7, 8 x 8192 25 / 21, 64 x 1024 25 / 18, 64 x 2048
+// 35 / 31, 128 x 2048 80 / 57, 256 x 2048 147 / 107; but 1 x 4096 8.7 / 10.1, 16 x
+// 1024 11.3 / 12.3, 64 x 512 12.8 / 12.2, 256 x 512 39 / 44 (and of contexts spread
+// over U[60, 600] 33.6 / 39.4).  So: contexts past 1024 tokens, and 128 of them or
+// more a CU and pair.  Where the heads alone fill the CUs unsplit and the pairs
+// have to be split, only long ones: 32 x 2048 22.7 / 21.2, 4096 33.4 / 33.9, 8192
+// 72 / 57.  A max_seq_len that is only a bound counts as kMx4PairBound at most
+// (8 x 768 10.2 / 9.8, 1024 11.0 / 10.0; but 256 7.9 / 9.1).
+constexpr int64_t kMx4PairTokens = 1024, kMx4PairPerCu = 128, kMx4PairSplit = 4096;
+constexpr int64_t kMx4PairBound = 1280;
+static bool mx4_head_pairs(const va_decode_args* a) {
+  const int64_t heads = (int64_t)a->num_seqs * a->num_kv_heads;
+  if (a->head_dim != 128 || a->num_kv_heads % 2 != 0 || a->pool.stride_head != 64 ||
+      a->pool.stride_slot < 128 || heads > INT32_MAX / (2 * kMaxParts))
+    return false;
+  int64_t tokens = a->max_seq_len;
+  if (a->key_limit > 0 && a->key_limit < tokens) tokens = a->key_limit;
+  if (a->split_tokens != VA_SPLIT_EXACT && tokens > kMx4PairBound) tokens = kMx4PairBound;
+  const int64_t cus = current_device_cus();
+  if (tokens <= (heads < 2 * cus && heads >= cus ? kMx4PairSplit : kMx4PairTokens)) return false;
+  return heads / 2 * tokens >= kMx4PairPerCu * cus;
+}
+
 static DecodePlan plan_decode_mx4(const va_decode_args* a) {
-  return plan_split(a, 8 * kMx4Step, kMx4NoSplitTokens, kMx4MinPart);
+  return plan_split(a, 8 * kMx4Step, kMx4NoSplitTokens, kMx4MinPart, mx4_head_pairs(a) ? 2 : 1);
 }
 
 template <typename ET>
@@ -522,7 +550,8 @@ int va::paged_decode_impl(const va_decode_args* a, const va_mx4_scales* sc, cons
     p.waves = wgs > current_device_cus() ? 4 : 8;
     p.num_seqs = a->num_seqs;
     p.min_part = kMx4MinPart;
-    p.hkv_div = make_fastdiv((uint32_t)a->num_kv_heads);
+    p.head_pairs = mx4_head_pairs(a);
+    p.hkv_div = make_fastdiv((uint32_t)a->num_kv_heads / (p.head_pairs ? 2 : 1));
     p.seq_div = make_fastdiv((uint32_t)a->num_seqs);
     p.by_token = a->num_kv_heads > 1 && a->pool.stride_head < a->pool.stride_slot &&
                  wgs + 8 * (int64_t)a->num_kv_heads < INT32_MAX;

@@ -40,6 +40,7 @@ struct DecodeMx4Params : DecodeParams {
   int32_t num_seqs;
   int32_t by_token;  // the grid keeps a sequence's heads together (see the kernel)
   FastDiv hkv_div, seq_div;
+  int32_t head_pairs;  // a workgroup serves two kv heads (see the kernel)
   int32_t min_part;  // dyn_split: fewest tokens of a partition
 };
 
@@ -66,22 +67,19 @@ struct Mx4DecodeShape {
   static constexpr int CPR = ROWB / 16;              // 16-byte chunks of a row
   static constexpr int CH = D <= 128 ? 1 : D / 128;  // 128-element chunks of a row
   static constexpr int NV = D / 16;                  // V elements of a lane and token
-  static constexpr int TILE_B = 16 * ROWB;           // codes of a 16-token tile, K or V
   static constexpr int SCW = D <= 128 ? 4 : 8;       // staged bytes of a row's scales
-  // A stage: K codes of both tiles, V codes, K scales, V scales.
-  static constexpr int V_OFF = 2 * TILE_B, KS_OFF = 4 * TILE_B, VS_OFF = KS_OFF + 32 * SCW;
-  static constexpr int STAGE_B = VS_OFF + 32 * SCW;
-  static constexpr int NDMA = 4 * TILE_B / 1024 + 2 * 32 * SCW / 256;  // requests of a step
   using V = std::conditional_t<D == 64, uint16_t, std::conditional_t<D == 128, uint32_t, uint2>>;
 };
 
 // LDS place of a staged tile's token and of a row's chunk.  Tokens 4 c + r lie
 // at row 4 r + c, so that the V reads of one r (four rows, each read whole by
 // 16 lanes) are consecutive, and a row's chunks are XORed so that the K reads
-// (one chunk of 16 rows) cover all banks.
+// (one chunk of 16 rows) cover all banks.  kPair: a row is two heads' (see the
+// kernel), whose V reads are half of each of four rows.
 __device__ inline int mx4_slot(int token) { return (token & 3) * 4 + (token >> 2); }
-template <int D>
+template <int D, bool kPair>
 __device__ inline int mx4_swz(int slot) {
+  if constexpr (kPair) return ((slot >> 2) & 3) | ((slot & 2) << 1);
   return (slot / (256 / Mx4DecodeShape<D>::ROWB)) & (Mx4DecodeShape<D>::CPR - 1);
 }
 
@@ -90,28 +88,38 @@ __device__ inline void dma4(const void* src, uint32_t lds) {
   asm volatile("s_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(src), "{m0}"(lds) : "memory");
 }
 
-template <typename ET, int D, int G, bool kProlog, bool kMask, int W, int S>
+template <typename ET, int D, int G, bool kProlog, bool kMask, int W, int S, int HP>
 __global__ __launch_bounds__(W * 64, W == 4 && D <= 128 ? 4 : 2) void paged_decode_mx4_kernel(DecodeMx4Params p) {
   using Sh = Mx4DecodeShape<D>;
   using M = DecodeMma<ET>;
   using VT = typename Sh::V;
   constexpr int CH = Sh::CH, NV = Sh::NV, CPR = Sh::CPR, ROWB = Sh::ROWB, SCW = Sh::SCW;
-  constexpr int TILE_B = Sh::TILE_B, STAGE_B = Sh::STAGE_B, NDMA = Sh::NDMA;
   constexpr int NT = W * 64, ROW16 = D * 2;
   constexpr int TERMS = ET::kIsBF16 ? 2 : 3;        // e4m3 terms of a query
   constexpr int QM = D == 64 ? (TERMS + 1) / 2 : TERMS;  // products per chunk (two terms share one at 64)
   constexpr int LPR = D / 8, RPL = 64 / LPR, E = 8;  // the row layout of prologue.h
   constexpr int QROWS = (G + RPL - 1) / RPL;
   constexpr int LPS = kMx4Group / NV;  // lanes that share a V scale
-  static_assert(W % 4 == 0, "the wave merge reads (m, l) of four waves at a time");
+  constexpr bool kPair = HP == 2;
+  constexpr int TW = W / HP, HG = HP * G;  // a head's waves; the workgroup's query heads
+  static_assert(TW % 4 == 0, "the wave merge reads (m, l) of four waves at a time");
+  static_assert(HP == 1 || (kPair && D == 128), "a line holds two heads' 64 bytes");
+  // A stage: K codes of both tiles, V codes, K scales, V scales.
+  constexpr int PITCH = HP * ROWB, SCP = HP * SCW;  // of a staged row of codes, of scales
+  constexpr int TILE_B = 16 * PITCH;
+  constexpr int V_OFF = 2 * TILE_B, KS_OFF = 4 * TILE_B, VS_OFF = KS_OFF + 32 * SCP;
+  constexpr int STAGE_B = VS_OFF + 32 * SCP;
+  // Requests of a wave for a step (of a pair's, half).
+  constexpr int NDMA = kPair ? 5 : 4 * TILE_B / 1024 + 2 * 32 * SCW / 256;
+  constexpr int RING_B = TW * S * STAGE_B;
 
   // The waves' partial results: o [W][G][D], then m and l [G][W]; in LDS of
   // their own where two workgroups a CU have room for it, else in the ring.
   constexpr int MERGE_B = W * G * D * 4 + 2 * G * W * 4;
   constexpr int Q_B = kProlog ? W * (G + 1) * ROW16 : 16;
-  constexpr bool kOwnMerge = W * S * STAGE_B + MERGE_B + Q_B <= (D == 256 ? 80 : W == 4 ? 40 : 160) * 1024;
-  static_assert(kOwnMerge || MERGE_B <= W * S * STAGE_B, "merge scratch");
-  __shared__ __align__(1024) char s_ring[W * S * STAGE_B];
+  constexpr bool kOwnMerge = RING_B + MERGE_B + Q_B <= (D == 256 ? 80 : W == 4 ? 40 : 160) * 1024;
+  static_assert(kOwnMerge || MERGE_B <= RING_B, "merge scratch");
+  __shared__ __align__(1024) char s_ring[RING_B];
   __shared__ __align__(16) char s_mrg[kOwnMerge ? MERGE_B : 16];
   // kProlog: each wave's processed query rows and current key row.
   __shared__ __align__(16) char s_q[Q_B];
@@ -123,6 +131,14 @@ __global__ __launch_bounds__(W * 64, W == 4 && D <= 128 ? 4 : 2) void paged_deco
   // of scales a small part.  There (by_token) the heads of a (sequence,
   // partition) pair u follow one another on XCD u % 8 (32 contexts of 7000 tokens:
   // 92 -> 67 us; the requests to HBM then equal an HND pool's).
+  //
+  // That leaves each line going to two CUs, 2.2 times the requests of an HND
+  // pool from L2.  With HP = 2 a workgroup serves two heads, wave w and w + W / 2
+  // the same tokens for one head each, through a ring that they share: a request
+  // takes 8 whole lines, half of a tile's for both, and a barrier a step says
+  // that the halves are there (67 -> 57 us, against 52 over an HND pool).  Two
+  // heads a workgroup with rings of their own did not help (87: the second
+  // request for a line finds it in L2, not in the CU).
   int b = blockIdx.y, h = blockIdx.x, part = blockIdx.z;
   if (p.by_token) {
     const uint32_t j = blockIdx.x >> 3, r = fast_div(j, p.hkv_div);
@@ -134,6 +150,10 @@ __global__ __launch_bounds__(W * 64, W == 4 && D <= 128 ? 4 : 2) void paged_deco
   }
   const int tid = threadIdx.x;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int tw = kPair ? wave % TW : wave;
+  const int h0 = h * HP;  // the workgroup's first kv head
+  const int hd = kPair ? wave / TW : 0;
+  h = h0 + hd;
   const int lane = tid & 63;
   const int r16 = lane & 15, c4 = lane >> 4;
   const int rg = lane / LPR, col = lane % LPR;
@@ -148,7 +168,7 @@ __global__ __launch_bounds__(W * 64, W == 4 && D <= 128 ? 4 : 2) void paged_deco
   // which its byte offsets are formed 32 steps at a time.
   const uint32_t* const tabw = reinterpret_cast<const uint32_t*>(p.table);
   auto tile_tok = [&](int k0) {
-    return start + kMx4Step * (wave + W * (k0 + (lane >> 1))) + 16 * (lane & 1);
+    return start + kMx4Step * (tw + TW * (k0 + (lane >> 1))) + 16 * (lane & 1);
   };
   uint2 ids = make_uint2(0u, 0u);  // raw words of a block id
   auto load_ids = [&](int k0, int limit) {
@@ -232,31 +252,35 @@ __global__ __launch_bounds__(W * 64, W == 4 && D <= 128 ? 4 : 2) void paged_deco
     slot_hi = sw[((int64_t)b << p.new_slots_i64) + p.new_slots_i64];
   }
 
-  // ---- the wave's ring: S stages of a step each, filled by DMA ----
-  char* const s_wave = s_ring + wave * S * STAGE_B;
+  // ---- the wave's (the pair's) ring: S stages of a step each, filled by DMA ----
+  char* const s_wave = s_ring + tw * S * STAGE_B;
   const uint32_t lds_wave = __builtin_amdgcn_readfirstlane(
       (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)s_wave);
   // Codes: request i of a tile fills LDS rows i RPI ..; lane l's chunk is
   // position l % CPR of row i RPI + l / CPR.  At head_dim 64 one request takes
   // both tiles, 32 lanes each.
-  constexpr int RPI = 64 / CPR, NI = TILE_B >= 1024 ? TILE_B / 1024 : 1;
+  // A pair's wave hd takes LDS rows 8 hd .. of each tile.
+  constexpr int RPI = 1024 / PITCH, CPP = PITCH / 16;
+  constexpr int NI = kPair || TILE_B < 1024 ? 1 : TILE_B / 1024;
   uint32_t loff[NI];
+  auto swz = [](int slot) { return mx4_swz<D, kPair>(slot); };
 #pragma unroll
   for (int i = 0; i < NI; ++i) {
-    const int slot = (i * RPI + lane / CPR) & 15, pos = lane % CPR;
+    const int slot = ((kPair ? hd : i) * RPI + lane / CPP) & 15, pos = lane % CPP;
     const int token = (slot & 3) * 4 + (slot >> 2);
-    loff[i] = (uint32_t)(token * (int)p.s_slot) + (uint32_t)((pos ^ mx4_swz<D>(slot)) << 4);
+    loff[i] = (uint32_t)(token * (int)p.s_slot) + (uint32_t)((pos ^ swz(slot)) << 4);
   }
   const int64_t head_off = (int64_t)h * p.s_head, head_sc = (int64_t)h * p.sc_head;
-  int64_t toff = head_off, tsc = head_sc;  // of the lane's tile (block 0 where there is none)
+  const int64_t ring_off = (int64_t)h0 * p.s_head, ring_sc = (int64_t)h0 * p.sc_head;
+  int64_t toff = ring_off, tsc = ring_sc;  // of the lane's tile (block 0 where there is none)
   uint64_t tiles_ok = 0;                   // bit l: lane l's tile has a block of the pool
   auto take_ids = [&](int k0) {
     const int64_t bid = p.table_i64 ? (int64_t)(((uint64_t)ids.y << 32) | ids.x)
                                     : (int64_t)(int32_t)ids.x;
     const bool ok = bid >= 0 && bid < p.num_blocks;
     const int in = ok ? (int)fast_mod((uint32_t)tile_tok(k0), p.bs_div) : 0;
-    toff = (ok ? bid : 0) * p.s_blk + (int64_t)in * p.s_slot + head_off;
-    tsc = (ok ? bid : 0) * p.sc_blk + (int64_t)in * p.sc_slot + head_sc;
+    toff = (ok ? bid : 0) * p.s_blk + (int64_t)in * p.s_slot + ring_off;
+    tsc = (ok ? bid : 0) * p.sc_blk + (int64_t)in * p.sc_slot + ring_sc;
     tiles_ok = __builtin_amdgcn_ballot_w64(ok);
   };
   auto lane64 = [&](int64_t x, int l) -> int64_t {
@@ -270,10 +294,17 @@ __global__ __launch_bounds__(W * 64, W == 4 && D <= 128 ? 4 : 2) void paged_deco
     const int l = 2 * (k & 31);
     const int64_t o0 = lane64(toff, l), o1 = lane64(toff, l + 1);
     const int64_t c0 = lane64(tsc, l), c1 = lane64(tsc, l + 1);
-    if constexpr (D == 64) {
+    if constexpr (kPair) {
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        const uint32_t at = dst + t * TILE_B + hd * 1024;
+        dma16_nt(loff[0], uniform_ptr(p.kp + (t ? o1 : o0)), at);
+        dma16_nt(loff[0], uniform_ptr(p.vp + (t ? o1 : o0)), at + V_OFF);
+      }
+    } else if constexpr (D == 64) {
       const int64_t o = (lane < 32 ? o0 : o1) + loff[0];
       dma16_nt(p.kp + o, dst);
-      dma16_nt(p.vp + o, dst + Sh::V_OFF);
+      dma16_nt(p.vp + o, dst + V_OFF);
     } else {
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
@@ -285,25 +316,29 @@ __global__ __launch_bounds__(W * 64, W == 4 && D <= 128 ? 4 : 2) void paged_deco
           // contexts of 7000, us: NHD 66.9 / 69.6, HND 55.9 / 52.0 without / with nt).
           if (p.by_token) {
             dma16(loff[i], kb, dst + t * TILE_B + i * 1024);
-            dma16(loff[i], vb, dst + Sh::V_OFF + t * TILE_B + i * 1024);
+            dma16(loff[i], vb, dst + V_OFF + t * TILE_B + i * 1024);
           } else {
             dma16_nt(loff[i], kb, dst + t * TILE_B + i * 1024);
-            dma16_nt(loff[i], vb, dst + Sh::V_OFF + t * TILE_B + i * 1024);
+            dma16_nt(loff[i], vb, dst + V_OFF + t * TILE_B + i * 1024);
           }
         }
       }
     }
     // Scales, a word a lane: at head_dim 64 the aligned word that holds the
-    // row's two.
-    if constexpr (D <= 128) {
+    // row's two.  A pair's wave 0 takes both heads' K scales, wave 1 the V's.
+    if constexpr (kPair) {
+      const int64_t at = (lane < 32 ? c0 : c1) + (int64_t)((lane >> 1) & 15) * p.sc_slot +
+                         (lane & 1) * p.sc_head;
+      dma4((hd ? p.vs : p.ks) + at, dst + (hd ? VS_OFF : KS_OFF));
+    } else if constexpr (D <= 128) {
       const char* src = (lane < 32 ? p.ks : p.vs) + ((lane & 16) ? c1 : c0) +
                         (int64_t)r16 * p.sc_slot;
       if constexpr (D == 64) src = (const char*)((uintptr_t)src & ~(uintptr_t)3);
-      dma4(src, dst + Sh::KS_OFF);
+      dma4(src, dst + KS_OFF);
     } else {
       const int64_t at = (lane < 32 ? c0 : c1) + (int64_t)((lane >> 1) & 15) * p.sc_slot + (lane & 1) * 4;
-      dma4(p.ks + at, dst + Sh::KS_OFF);
-      dma4(p.vs + at, dst + Sh::VS_OFF);
+      dma4(p.ks + at, dst + KS_OFF);
+      dma4(p.vs + at, dst + VS_OFF);
     }
   };
 
@@ -327,8 +362,8 @@ __global__ __launch_bounds__(W * 64, W == 4 && D <= 128 ? 4 : 2) void paged_deco
     if constexpr (kMask)
       asm volatile("" ::"v"(mraw[0]), "v"(mraw[1]), "v"(mraw[2]), "v"(mraw[3]), "v"(mraw[4]));
     if (p.num_blocks > 0)
-      for (int k = 0; k < S; ++k)
-        if (last_part || (wave + W * k) * kMx4Step < P) issue(k);
+      for (int k = 0; k < S - kPair; ++k)
+        if (last_part || (tw + TW * k) * kMx4Step < P) issue(k);
   }
 
   // ---- the length and the partition ----
@@ -353,13 +388,13 @@ __global__ __launch_bounds__(W * 64, W == 4 && D <= 128 ? 4 : 2) void paged_deco
   int nparts = L > 0 ? (L + P - 1) / P : 1;
   if (nparts > p.max_parts) nparts = p.max_parts;  // the last partition absorbs the rest
   const int nsteps = end > start ? (end - start + kMx4Step - 1) / kMx4Step : 0;
-  const int ntw = nsteps > wave ? (nsteps - wave + W - 1) / W : 0;  // steps of this wave
+  const int ntw = nsteps > tw ? (nsteps - tw + TW - 1) / TW : 0;  // steps of this wave
   const int new_tok =
       (!detached && p.new_k != nullptr && L - 1 >= start && L - 1 < end) ? L - 1 : -1;
   const int new_step = new_tok >= 0 ? (new_tok - start) / kMx4Step : -1;
-  const bool owns_new = new_step >= 0 && new_step % W == wave;
+  const bool owns_new = new_step >= 0 && new_step % TW == tw;
   const int64_t cap = (int64_t)p.num_blocks * p.block_size;
-  const bool has_new = p.new_k != nullptr && (owns_new || (writes_row && wave == 0));
+  const bool has_new = p.new_k != nullptr && (owns_new || (writes_row && tw == 0));
   if (!early && ntw > 0) {
     load_ids(0, end);
     if (kMask) mask_load(0);
@@ -367,7 +402,7 @@ __global__ __launch_bounds__(W * 64, W == 4 && D <= 128 ? 4 : 2) void paged_deco
     if constexpr (kMask)
       asm volatile("" ::"v"(mraw[0]), "v"(mraw[1]), "v"(mraw[2]), "v"(mraw[3]), "v"(mraw[4]));
     take_ids(0);
-    for (int k = 0; k < S; ++k)
+    for (int k = 0; k < S - kPair; ++k)
       if (k < ntw) issue(k);
   }
   if (kMask) mbits = mask_bits();
@@ -498,13 +533,13 @@ __global__ __launch_bounds__(W * 64, W == 4 && D <= 128 ? 4 : 2) void paged_deco
       if (r16 % (kMx4Group / NV) == 0) p.vs[dst_sc + r16 * NV / kMx4Group] = (char)vqs;
     }
   };
-  if (writes_row && wave == 0) store_row();
+  if (writes_row && tw == 0) store_row();
   if (L <= 0) {
     // Nothing to attend: the output is defined as 0.
     if (part == 0) {
-      for (int idx = tid; idx < G * D / E; idx += NT) {
+      for (int idx = tid; idx < HG * D / E; idx += NT) {
         const int g = idx / (D / E), d = (idx % (D / E)) * E;
-        st16(p.out + b * p.o_sb + (int64_t)(h * G + g) * p.o_sh + d * 2, make_uint4(0, 0, 0, 0));
+        st16(p.out + b * p.o_sb + (int64_t)(h0 * G + g) * p.o_sh + d * 2, make_uint4(0, 0, 0, 0));
       }
     }
     wait_vmcnt<0>();
@@ -577,28 +612,37 @@ __global__ __launch_bounds__(W * 64, W == 4 && D <= 128 ? 4 : 2) void paged_deco
 
   // Byte offsets of the lane's reads inside a stage.
   const int kslot = mx4_slot(r16);
-  const int koff = kslot * ROWB + (((D == 64 ? c4 & 1 : c4) ^ mx4_swz<D>(kslot)) << 4);
-  const int ksoff = Sh::KS_OFF + r16 * SCW + (D == 64 ? c4 & 1 : c4);
+  const int hc = CPR * hd, hs = SCW * hd;  // the head's chunks and scales of a staged row
+  const int koff = kslot * PITCH + (((hc + (D == 64 ? c4 & 1 : c4)) ^ swz(kslot)) << 4);
+  const int ksoff = KS_OFF + r16 * SCP + hs + (D == 64 ? c4 & 1 : c4);
   int voff[4];  // of token 4 c4 + i
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int slot = 4 * i + c4, byte = r16 * (NV / 2);
-    voff[i] = Sh::V_OFF + slot * ROWB + (((byte >> 4) ^ mx4_swz<D>(slot)) << 4) + (byte & 15);
+    voff[i] = V_OFF + slot * PITCH + (((hc + (byte >> 4)) ^ swz(slot)) << 4) + (byte & 15);
   }
-  const int vsoff = Sh::VS_OFF + 4 * c4 * SCW + r16 / LPS;
+  const int vsoff = VS_OFF + 4 * c4 * SCP + hs + r16 / LPS;
 
-  for (int k = 0; k < ntw; ++k) {
-    if (k + S - 1 < ntw)
-      wait_vmcnt<NDMA*(S - 1)>();  // the steps after it may stay in flight
+  const int nloop = kPair ? (nsteps + TW - 1) / TW : ntw;
+  for (int k = 0; k < nloop; ++k) {
+    constexpr int kAhead = S - 1 - kPair;  // steps that may stay in flight
+    if (k + kAhead < ntw)
+      wait_vmcnt<NDMA * kAhead>();
     else
       wait_vmcnt<0>();
+    if constexpr (kPair) {
+      // Both waves' halves of step k are there, and both are done with the
+      // stage before it, which takes step k + S - 1 below.
+      asm volatile("s_barrier" ::: "memory");
+      if (k >= ntw) continue;
+    }
     if (k > 0 && (k & 31) == 0) {
       tiles_ok_k = tiles_ok;
       mbits_k = mbits;
       tsc_k = (uint32_t)tsc;
     }
     char* const st = s_wave + (k % S) * STAGE_B;
-    const int c = wave + W * k;
+    const int c = tw + TW * k;
     const int tb = start + kMx4Step * c;
     uint32_t tpar[2] = {0u, 0u};
     if constexpr (D == 64) {
@@ -616,17 +660,17 @@ __global__ __launch_bounds__(W * 64, W == 4 && D <= 128 ? 4 : 2) void paged_deco
       if (r16 == 0 && (D > 64 || c4 < 2)) {
 #pragma unroll
         for (int cc = 0; cc < CH; ++cc) {
-          *reinterpret_cast<uint4*>(st + t * TILE_B + slot * ROWB +
-                                    (((4 * cc + c4) ^ mx4_swz<D>(slot)) << 4)) = kq[cc];
-          st[Sh::KS_OFF + (t * 16 + r) * SCW + half(t, p.ks, r) + 4 * cc + c4] = (char)kqs[cc];
+          *reinterpret_cast<uint4*>(st + t * TILE_B + slot * PITCH +
+                                    (((4 * cc + hc + c4) ^ swz(slot)) << 4)) = kq[cc];
+          st[KS_OFF + (t * 16 + r) * SCP + hs + half(t, p.ks, r) + 4 * cc + c4] = (char)kqs[cc];
         }
       }
       if (c4 == 0) {
         const int byte = r16 * (NV / 2);
-        *reinterpret_cast<VT*>(st + Sh::V_OFF + t * TILE_B + slot * ROWB +
-                               (((byte >> 4) ^ mx4_swz<D>(slot)) << 4) + (byte & 15)) = vq;
+        *reinterpret_cast<VT*>(st + V_OFF + t * TILE_B + slot * PITCH +
+                               (((hc + (byte >> 4)) ^ swz(slot)) << 4) + (byte & 15)) = vq;
         if (r16 % LPS == 0)
-          st[Sh::VS_OFF + (t * 16 + r) * SCW + half(t, p.vs, r) + r16 / LPS] = (char)vqs;
+          st[VS_OFF + (t * 16 + r) * SCP + hs + half(t, p.vs, r) + r16 / LPS] = (char)vqs;
       }
       __builtin_amdgcn_wave_barrier();
     }
@@ -639,7 +683,7 @@ __global__ __launch_bounds__(W * 64, W == 4 && D <= 128 ? 4 : 2) void paged_deco
       for (int cc = 0; cc < CH; ++cc) {
         // (a row's chunks 4 .. 7 are its chunks 0 .. 3 with the third bit flipped)
         kk[t][cc] = *reinterpret_cast<const uint4*>(st + t * TILE_B + (koff ^ (cc << 6)));
-        kks[t][cc] = (uint8_t)st[ksoff + t * 16 * SCW + 4 * cc + half(t, p.ks, r16)];
+        kks[t][cc] = (uint8_t)st[ksoff + t * 16 * SCP + 4 * cc + half(t, p.ks, r16)];
       }
     VT vv[8];
     uint32_t vb[8];
@@ -648,7 +692,7 @@ __global__ __launch_bounds__(W * 64, W == 4 && D <= 128 ? 4 : 2) void paged_deco
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         vv[4 * t + i] = *reinterpret_cast<const VT*>(st + t * TILE_B + voff[i]);
-        vb[4 * t + i] = (uint8_t)st[vsoff + (t * 16 + i) * SCW + half(t, p.vs, 4 * c4 + i)];
+        vb[4 * t + i] = (uint8_t)st[vsoff + (t * 16 + i) * SCP + half(t, p.vs, 4 * c4 + i)];
       }
     mf_f32x4 sc[2];
 #pragma unroll
@@ -659,10 +703,10 @@ __global__ __launch_bounds__(W * 64, W == 4 && D <= 128 ? 4 : 2) void paged_deco
 #pragma unroll
         for (int q = 0; q < QM; ++q) sc[t] = mx4_mfma(kk[t][cc], kks[t][cc], qf[q][cc], qs[q], sc[t]);
     }
-    // The stage has been read: it takes the wave's step k + S.
+    // The stage has been read: it takes the wave's step k + S (a pair's, once
+    // both have read it: the stage before it takes step k + S - 1).
     wait_lgkmcnt0();
-    if (k + S < ntw) {
-      const int n = k + S;
+    if (const int n = k + S - kPair; n < ntw) {
       if ((n & 31) == 0) {
         // The offsets of the next 32 steps.
         load_ids(n, end);
@@ -761,31 +805,31 @@ __global__ __launch_bounds__(W * 64, W == 4 && D <= 128 ? 4 : 2) void paged_deco
   l = sum_xor16(l);
   l = sum_xor32(l);
   if constexpr (!kOwnMerge) __syncthreads();  // every wave is done with its stages
-  float* const s_o = reinterpret_cast<float*>(kOwnMerge ? s_mrg : s_ring);  // [W][G][D]
-  float* const s_m = s_o + W * G * D;                                        // [G][W]
-  float* const s_l = s_m + G * W;                                            // [G][W]
+  float* const s_o = reinterpret_cast<float*>(kOwnMerge ? s_mrg : s_ring);  // [TW][HG][D]
+  float* const s_m = s_o + W * G * D;                                        // [HG][TW]
+  float* const s_l = s_m + G * W;                                            // [HG][TW]
+  const int row0 = hd * G;  // the wave's first row of HG
   if (r16 < G) {
     // Lane (r16, c4) holds o of head r16 at d = NV (4 c4 + r) + i.
 #pragma unroll
     for (int r = 0; r < 4; ++r)
 #pragma unroll
       for (int i = 0; i < NV; i += 4)
-        *reinterpret_cast<mf_f32x4*>(s_o + (wave * G + r16) * D + NV * (4 * c4 + r) + i) =
+        *reinterpret_cast<mf_f32x4*>(s_o + (tw * HG + row0 + r16) * D + NV * (4 * c4 + r) + i) =
             mf_f32x4{o[i][r], o[i + 1][r], o[i + 2][r], o[i + 3][r]};
     if (c4 == 0) {
-      s_m[r16 * W + wave] = ntw > 0 ? m : kNegBig;
-      s_l[r16 * W + wave] = ntw > 0 ? l : 0.f;
+      s_m[(row0 + r16) * TW + tw] = ntw > 0 ? m : kNegBig;
+      s_l[(row0 + r16) * TW + tw] = ntw > 0 ? l : 0.f;
     }
   }
   __syncthreads();
-  const int64_t pair = (int64_t)b * p.num_kv_heads + h;
-  for (int qd = tid; qd < G * D / 4; qd += NT) {
+  for (int qd = tid; qd < HG * D / 4; qd += NT) {
     const int g = qd / (D / 4), d = (qd % (D / 4)) * 4;
-    float mw[W], lw[W];
+    float mw[TW], lw[TW];
 #pragma unroll
-    for (int w = 0; w < W; w += 4) {
-      const mf_f32x4 mv = *reinterpret_cast<const mf_f32x4*>(s_m + g * W + w);
-      const mf_f32x4 lv = *reinterpret_cast<const mf_f32x4*>(s_l + g * W + w);
+    for (int w = 0; w < TW; w += 4) {
+      const mf_f32x4 mv = *reinterpret_cast<const mf_f32x4*>(s_m + g * TW + w);
+      const mf_f32x4 lv = *reinterpret_cast<const mf_f32x4*>(s_l + g * TW + w);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         mw[w + i] = mv[i];
@@ -794,23 +838,24 @@ __global__ __launch_bounds__(W * 64, W == 4 && D <= 128 ? 4 : 2) void paged_deco
     }
     float Mx = kNegBig;
 #pragma unroll
-    for (int w = 0; w < W; ++w) Mx = fmaxf(Mx, mw[w]);
+    for (int w = 0; w < TW; ++w) Mx = fmaxf(Mx, mw[w]);
     float Lt = 0.f;
     mf_f32x4 acc = mf_f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int w = 0; w < W; ++w) {
+    for (int w = 0; w < TW; ++w) {
       const float f = fast_exp2(mw[w] - Mx);
       Lt += lw[w] * f;
-      acc += f * *reinterpret_cast<const mf_f32x4*>(s_o + (w * G + g) * D + d);
+      acc += f * *reinterpret_cast<const mf_f32x4*>(s_o + (w * HG + g) * D + d);
     }
     if (nparts == 1) {
       const float inv = Lt > 0.f ? 1.0f / Lt : (Lt == 0.f ? 0.f : Lt);  // a NaN stays one
       uint2 u;
       u.x = M::pack2(acc[0] * inv, acc[1] * inv);
       u.y = M::pack2(acc[2] * inv, acc[3] * inv);
-      *reinterpret_cast<uint2*>(p.out + b * p.o_sb + (int64_t)(h * G + g) * p.o_sh + d * 2) = u;
+      *reinterpret_cast<uint2*>(p.out + b * p.o_sb + (int64_t)(h0 * G + g) * p.o_sh + d * 2) = u;
     } else {
-      const int64_t slot = (pair * p.max_parts + part) * G + g;
+      const int64_t pair = (int64_t)b * p.num_kv_heads + h0 + g / G;
+      const int64_t slot = (pair * p.max_parts + part) * G + g % G;
       *reinterpret_cast<mf_f32x4*>(p.part_o + slot * D + d) = acc;
       if (d == 0) {
         p.part_ml[slot * 2] = Mx;
@@ -899,22 +944,22 @@ __global__ __launch_bounds__(256) void paged_decode_mx4_merge_kernel(DecodeMx4Pa
 }
 
 // ------------------------------------------------------------- launching
-template <typename ET, int D, int G, int W, int S>
+template <typename ET, int D, int G, int W, int S, int HP = 1>
 static void launch_decode_mx4_w(const DecodeMx4Params& p, dim3 grid, hipStream_t s) {
   if (p.by_token) {
     const int64_t units = (int64_t)p.num_seqs * p.max_parts;
-    grid = dim3((unsigned)((units + 7) / 8 * 8 * p.num_kv_heads));
+    grid = dim3((unsigned)((units + 7) / 8 * 8 * (p.num_kv_heads / HP)));
   }
   const dim3 nt(W * 64);
   const bool mask = p.valid != nullptr && p.valid_len > 0;
   if (p.has_pro && mask)
-    hipLaunchKernelGGL((paged_decode_mx4_kernel<ET, D, G, true, true, W, S>), grid, nt, 0, s, p);
+    hipLaunchKernelGGL((paged_decode_mx4_kernel<ET, D, G, true, true, W, S, HP>), grid, nt, 0, s, p);
   else if (p.has_pro)
-    hipLaunchKernelGGL((paged_decode_mx4_kernel<ET, D, G, true, false, W, S>), grid, nt, 0, s, p);
+    hipLaunchKernelGGL((paged_decode_mx4_kernel<ET, D, G, true, false, W, S, HP>), grid, nt, 0, s, p);
   else if (mask)
-    hipLaunchKernelGGL((paged_decode_mx4_kernel<ET, D, G, false, true, W, S>), grid, nt, 0, s, p);
+    hipLaunchKernelGGL((paged_decode_mx4_kernel<ET, D, G, false, true, W, S, HP>), grid, nt, 0, s, p);
   else
-    hipLaunchKernelGGL((paged_decode_mx4_kernel<ET, D, G, false, false, W, S>), grid, nt, 0, s, p);
+    hipLaunchKernelGGL((paged_decode_mx4_kernel<ET, D, G, false, false, W, S, HP>), grid, nt, 0, s, p);
 }
 
 template <typename ET, int D, int G>
@@ -922,7 +967,9 @@ static void launch_decode_mx4(const DecodeMx4Params& p, dim3 grid, hipStream_t s
   if constexpr (D == 256) {
     launch_decode_mx4_w<ET, D, G, 4, 2>(p, grid, s);
   } else {
-    if (p.waves == 4)
+    if (p.head_pairs) {
+      if constexpr (D == 128) launch_decode_mx4_w<ET, D, G, 8, 3, 2>(p, grid, s);
+    } else if (p.waves == 4)
       launch_decode_mx4_w<ET, D, G, 4, 2>(p, grid, s);
     else
       launch_decode_mx4_w<ET, D, G, 8, 3>(p, grid, s);
