@@ -696,3 +696,25 @@ def test_decode_pairs_agree_with_single_heads(dev):
         out.zero_()
         graph.replay()
         assert torch.equal(out, two)
+
+
+@pytest.mark.parametrize("hq, hkv, lens", [(16, 8, [2000] * 8), (16, 2, [16500, 30]), (8, 8, [1500] * 31)])
+@pytest.mark.parametrize("split", [0, ops.SPLIT_EXACT])
+def test_reserved_workspace_holds_every_automatic_split(dev, hq, hkv, lens, split):
+    gen = torch.Generator().manual_seed(44)
+    blocks = sum(-(-n // 16) for n in lens)
+    pool = Pool(gen, blocks, 16, hkv, 128, "nhd", BF16, dev)
+    (kc, vc), kw = pool.args()
+    tables = tables_for(gen, lens, 16, blocks).to(dev)
+    q = torch.randn(len(lens), hq, 128, generator=gen).to(BF16).to(dev)
+    vec = torch.tensor(lens, device=dev)
+    stream = torch.cuda.Stream()
+    ops.reserve_decode_workspace(dev, hq, hkv, 128, stream=stream)
+    key = (dev.index or 0, stream.cuda_stream)
+    before = ops._WORKSPACES[key]
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        ops.paged_decode(q, kc, vc, tables, vec, max_seq_len=max(lens) if split else 32768, scale=0.1,
+                         split_tokens=split, **kw)
+    torch.cuda.synchronize()
+    assert ops._WORKSPACES[key] is before

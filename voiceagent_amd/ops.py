@@ -567,14 +567,15 @@ def decode_workspace_bound(device: torch.device, num_heads: int, num_kv_heads: i
                            head_dim: int) -> int:
     """Bytes that covers every automatic split (split_tokens = 0) of a decode
     with these heads on `device`, whatever the batch and lengths: the split
-    gives at most one partition per compute unit over all (sequence, kv head)
-    pairs, each holding (m, l) and head_dim floats per query head of the
+    gives at most one partition per compute unit (over an MXFP4 pool two) over
+    all (sequence, kv head) pairs, each holding (m, l) and head_dim floats per query head of the
     group, with the (m, l) block rounded to 256 bytes."""
     index = _device_index(device)
     cus = _CUS.get(index)
     if cus is None:
         cus = _CUS[index] = torch.cuda.get_device_properties(index).multi_processor_count
     group = max(1, num_heads // max(1, num_kv_heads))
+    cus *= 2  # (MXFP4: workgroups that serve two kv heads each, twice the partitions)
     return (cus * group * 2 * 4 + 255) // 256 * 256 + cus * group * head_dim * 4
 
 
