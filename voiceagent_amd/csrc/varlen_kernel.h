@@ -1013,9 +1013,6 @@ varlen_attention_kernel(VarlenParams p) {
       // MXFP4 pool: the wave's rows of this tile from its code area into the
       // stage, at their swizzled positions; then the area may take the next
       // tile.
-      // MXFP4 pool: the wave's rows of this tile from its code area into the
-      // stage, at their swizzled positions; then the area may take the next
-      // tile.
       if constexpr (kMx4) {
         if (kb < prefix) {
 #pragma unroll
