@@ -718,3 +718,24 @@ def test_reserved_workspace_holds_every_automatic_split(dev, hq, hkv, lens, spli
                          split_tokens=split, **kw)
     torch.cuda.synchronize()
     assert ops._WORKSPACES[key] is before
+
+
+def test_fp8_pools_take_scales_of_one_number_as_tensors(dev):
+    gen = torch.Generator().manual_seed(45)
+    rows = [torch.randn(40, 2, 128, generator=gen).to(BF16).to(dev) for _ in range(2)]
+    q = torch.randn(40, 4, 128, generator=gen).to(BF16).to(dev)
+    slots = torch.arange(40, dtype=torch.int32, device=dev)
+    table = torch.tensor([[0, 1, 2]], dtype=torch.int32, device=dev)
+    lens, cu40 = torch.tensor([40], device=dev), cu([40]).to(dev)
+    got = []
+    for scale in (0.5, torch.tensor(0.5), torch.tensor([0.5], device=dev)):
+        kc, vc = (torch.zeros(4, 16, 2, 128, dtype=torch.uint8, device=dev).view(ops.FP8_KV_DTYPE)
+                  for _ in range(2))
+        kw = {"k_scale": scale, "v_scale": scale}
+        ops.store_kvcache(rows[0], rows[1], kc, vc, slots, **kw)
+        one = ops.paged_decode(q[:1], kc, vc, table, lens, max_seq_len=40, scale=0.1, **kw)
+        many = ops.varlen_attention(q, None, None, cu40, cu40, 40, 40, scale=0.1, causal=True, k_cache=kc,
+                                    v_cache=vc, block_tables=table, **kw)
+        got.append((kc.view(torch.uint8), one, many))
+    for other in got[1:]:
+        assert all(torch.equal(a, b) for a, b in zip(got[0], other))

@@ -169,6 +169,16 @@ def _mx4_structs(k_cache: torch.Tensor, v_cache: torch.Tensor, layout: str, k_sc
     return pool, scales
 
 
+_NUMBERS = (float, int)
+
+
+def _number(scale: float | torch.Tensor) -> float:
+    """An FP8 pool's scale (other pools ignore theirs)."""
+    _require(not isinstance(scale, torch.Tensor) or scale.numel() == 1,
+             "tensor scales need an MXFP4 (float4_e2m1fn_x2) pool, or hold one number")
+    return float(scale)
+
+
 def _mx4_call(name: str, args, scales: N.Mx4Scales, device: torch.device) -> None:
     """Launch an MXFP4 entry point on the current stream of `device`."""
     index = _device_index(device)
@@ -200,15 +210,17 @@ def store_kvcache(
     An FP8 pool receives e4m3 codes of key / k_scale and value / v_scale.  An
     MXFP4 pool receives e2m1 codes, and k_scale / v_scale (its scale tensors)
     the groups' scales: the smallest power of two 2^e with max |x| < 7 * 2^e."""
-    if isinstance(k_scale, torch.Tensor):
+    if k_cache.dtype is MXFP4_KV_DTYPE:
         return _store_mx4(key, value, k_cache, v_cache, slot_mapping, layout, k_scale, v_scale)
     fast = _FAST if _FAST_LOADED else _fast_calls()
     if fast is not None and layout in (LAYOUT_NHD, LAYOUT_HND):
         index = key.get_device()
         if index >= 0 and index == torch.cuda.current_device():
             rc = fast.store_kvcache(key, value, k_cache, v_cache, slot_mapping,
-                                    layout == LAYOUT_HND, float(k_scale), float(v_scale), index,
-                                    _raw_stream(index))
+                                    layout == LAYOUT_HND,
+                                    k_scale if k_scale.__class__ is float else _number(k_scale),
+                                    v_scale if v_scale.__class__ is float else _number(v_scale),
+                                    index, _raw_stream(index))
             if rc == 0:
                 return
             if _FAST_NOT_TAKEN < rc < 0:
@@ -230,7 +242,7 @@ def store_kvcache(
     args.value = value.data_ptr()
     args.key_stride_tok, args.key_stride_head = key.stride(0), key.stride(1)
     args.value_stride_tok, args.value_stride_head = value.stride(0), value.stride(1)
-    args.pool = kv_pool(k_cache, v_cache, layout, k_scale, v_scale)
+    args.pool = kv_pool(k_cache, v_cache, layout, _number(k_scale), _number(v_scale))
     args.slot_mapping = slot_mapping.data_ptr()
     args.slot_dtype = _index_code(slot_mapping, "slot_mapping")
     args.num_tokens = int(key.shape[0])
@@ -276,7 +288,7 @@ def _fast_on(t: torch.Tensor, layout: str):
 
 def _store_mx4(key, value, k_cache, v_cache, slot_mapping, layout, k_scale, v_scale) -> None:
     fast, index = _fast_on(key, layout)
-    if fast is not None and isinstance(v_scale, torch.Tensor):
+    if fast is not None and isinstance(k_scale, torch.Tensor) and isinstance(v_scale, torch.Tensor):
         rc = fast.store_kvcache_mx4(key, value, k_cache, v_cache, slot_mapping,
                                     layout == LAYOUT_HND, k_scale, v_scale, index,
                                     _raw_stream(index))
@@ -553,10 +565,10 @@ def _pool_struct(k_cache, v_cache, layout, k_scale, v_scale) -> N.KvPool:
     description depends only on the key's fields."""
     key = (k_cache.data_ptr(), v_cache.data_ptr(), k_cache.shape, k_cache.stride(),
            v_cache.shape, v_cache.stride(), k_cache.dtype, v_cache.dtype, layout,
-           float(k_scale), float(v_scale))
+           _number(k_scale), _number(v_scale))
     pool = _POOLS.get(key)
     if pool is None:
-        pool = kv_pool(k_cache, v_cache, layout, k_scale, v_scale)
+        pool = kv_pool(k_cache, v_cache, layout, key[-2], key[-1])
         if len(_POOLS) >= 1024:
             _POOLS.clear()
         _POOLS[key] = pool
@@ -687,10 +699,10 @@ def paged_decode(
     that is the batch's exact longest context (partitions fixed from it); a
     positive value fixes the partition size.
     """
-    mx4 = isinstance(k_scale, torch.Tensor)
+    mx4 = k_cache.dtype is MXFP4_KV_DTYPE
     fast = _FAST if _FAST_LOADED else _fast_calls()
     if (fast is not None and not no_alloc and layout in (LAYOUT_NHD, LAYOUT_HND) and
-            mx4 == isinstance(v_scale, torch.Tensor)):
+            (not mx4 or (isinstance(k_scale, torch.Tensor) and isinstance(v_scale, torch.Tensor)))):
         index = q.get_device()
         if index >= 0 and index == torch.cuda.current_device():
             if out is None:
@@ -706,8 +718,9 @@ def paged_decode(
                 None if pro is None else pro.positions, _WORKSPACES.get((index, stream)),
                 lens_cumulative, layout == LAYOUT_HND,
                 int(max_seq_len), float(scale), int(split_tokens), int(key_limit),
-                int(table_read_width), k_scale if mx4 else float(k_scale),
-                v_scale if mx4 else float(v_scale), index, stream)
+                int(table_read_width),
+                k_scale if mx4 or k_scale.__class__ is float else _number(k_scale),
+                v_scale if mx4 or v_scale.__class__ is float else _number(v_scale), index, stream)
             if rc == 0:
                 return out
             if _FAST_NOT_TAKEN < rc < 0:
@@ -852,23 +865,22 @@ def varlen_attention(
     the launch normalises and rotates them at ``prologue.positions`` (one per
     query token); k and the pool must hold processed keys.
     """
-    mx4 = isinstance(k_scale, torch.Tensor)
+    pool_dtype = None if k_cache is None else k_cache.dtype
+    mx4 = pool_dtype is MXFP4_KV_DTYPE
     fast = _FAST if _FAST_LOADED else _fast_calls()
     if (fast is not None and prologue is None and layout in (LAYOUT_NHD, LAYOUT_HND) and
-            (k_cache is None or k_cache.dtype != FP8_KV_DTYPE) and
-            mx4 == isinstance(v_scale, torch.Tensor)):
+            pool_dtype is not FP8_KV_DTYPE and
+            (isinstance(k_scale, torch.Tensor) and isinstance(v_scale, torch.Tensor) if mx4 else
+             k_scale.__class__ in _NUMBERS and v_scale.__class__ in _NUMBERS)):
         index = q.get_device()
         if index >= 0 and index == torch.cuda.current_device():
             if out is None:
                 out = torch.empty_like(q)
-            args = (q, k, v, cu_seqlens_q, cu_seqlens_k, int(max_seqlen_q), int(max_seqlen_k),
-                    float(scale), bool(causal), k_cache, v_cache, block_tables, slot_mapping, out,
-                    layout == LAYOUT_HND)
-            stream = _raw_stream(index)
-            if mx4:
-                rc = fast.varlen_attention_mx4(*args, k_scale, v_scale, index, stream)
-            else:
-                rc = fast.varlen_attention(*args, index, stream)
+            more = (k_scale, v_scale, index) if mx4 else (index,)
+            rc = (fast.varlen_attention_mx4 if mx4 else fast.varlen_attention)(
+                q, k, v, cu_seqlens_q, cu_seqlens_k, int(max_seqlen_q), int(max_seqlen_k),
+                float(scale), bool(causal), k_cache, v_cache, block_tables, slot_mapping, out,
+                layout == LAYOUT_HND, *more, _raw_stream(index))
             if rc == 0:
                 return out
             if _FAST_NOT_TAKEN < rc < 0:
