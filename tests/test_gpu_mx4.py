@@ -739,3 +739,21 @@ def test_fp8_pools_take_scales_of_one_number_as_tensors(dev):
         got.append((kc.view(torch.uint8), one, many))
     for other in got[1:]:
         assert all(torch.equal(a, b) for a, b in zip(got[0], other))
+
+
+@pytest.mark.parametrize("d, split", [(64, 256), (128, 0)])
+def test_decode_of_more_workgroups_than_a_flat_grid_holds(dev, d, split):
+    # 65535 sequences of one token each; at split 256 a bound of 8192 makes 16.8 M workgroups.
+    n, hkv = 65535, 8
+    k, v, ks, vs = ops.mxfp4_kv_pool(2, 16, hkv, d, device=dev)
+    gen = torch.Generator().manual_seed(46)
+    rows = [torch.randn(1, hkv, d, generator=gen).to(BF16).to(dev) for _ in range(2)]
+    slot = torch.tensor([16], dtype=torch.int32, device=dev)
+    ops.store_kvcache(rows[0], rows[1], k, v, slot, k_scale=ks, v_scale=vs)
+    _, want = ops.load_kvcache(k, v, slot, k_scale=ks, v_scale=vs)
+    q = torch.randn(1, hkv, d, generator=gen).to(BF16).to(dev).expand(n, hkv, d)
+    table = torch.ones(1, 512, dtype=torch.int32, device=dev).expand(n, 512)
+    out = torch.zeros(n, hkv, d, dtype=BF16, device=dev)
+    ops.paged_decode(q, k, v, table, torch.ones(n, dtype=torch.int32, device=dev), max_seq_len=8192, scale=0.1,
+                     split_tokens=split, out=out, k_scale=ks, v_scale=vs)
+    assert torch.equal(out, want.expand(n, hkv, d))

@@ -215,10 +215,13 @@ constexpr int kMx4MinPart = 64;
 // (8 x 768 10.2 / 9.8, 1024 11.0 / 10.0; but 256 7.9 / 9.1).
 constexpr int64_t kMx4PairTokens = 1024, kMx4PairPerCu = 128, kMx4PairSplit = 4096;
 constexpr int64_t kMx4PairBound = 1280;
+// A grid of one dimension holds fewer than 2^32 lanes, 512 a workgroup.
+constexpr int64_t kMx4FlatWgs = (int64_t)1 << 23;
 static bool mx4_head_pairs(const va_decode_args* a) {
   const int64_t heads = (int64_t)a->num_seqs * a->num_kv_heads;
   if (a->head_dim != 128 || a->num_kv_heads % 2 != 0 || a->pool.stride_head != 64 ||
-      a->pool.stride_slot < 128 || heads > INT32_MAX / (2 * kMaxParts))
+      a->pool.stride_slot < 128 ||
+      heads * (a->split_tokens > 0 ? kMaxParts : 1) > kMx4FlatWgs / 2)
     return false;
   int64_t tokens = a->max_seq_len;
   if (a->key_limit > 0 && a->key_limit < tokens) tokens = a->key_limit;
@@ -554,7 +557,7 @@ int va::paged_decode_impl(const va_decode_args* a, const va_mx4_scales* sc, cons
     p.hkv_div = make_fastdiv((uint32_t)a->num_kv_heads / (p.head_pairs ? 2 : 1));
     p.seq_div = make_fastdiv((uint32_t)a->num_seqs);
     p.by_token = a->num_kv_heads > 1 && a->pool.stride_head < a->pool.stride_slot &&
-                 wgs + 8 * (int64_t)a->num_kv_heads < INT32_MAX;
+                 wgs + 8 * (int64_t)a->num_kv_heads < kMx4FlatWgs;
   }
   p.v_scale = f8 ? a->pool.v_scale : 1.0f;
   p.inv_k = f8 ? 1.0f / a->pool.k_scale : 1.0f;
