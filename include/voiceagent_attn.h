@@ -437,7 +437,7 @@ typedef struct va_batch_args {
   int64_t request_stride;   /* written where blocks are taken             */
   int32_t num_requests, request_width;
   const int32_t* rows;      /* optional [num_seqs]                        */
-  int32_t num_seqs, padded_seqs; /* padded_seqs >= num_seqs               */
+  int32_t num_seqs, padded_seqs; /* num_seqs <= padded_seqs <= 65535      */
   int32_t block_size;
   int32_t max_tokens;       /* entries of positions and slot_mapping      */
   int64_t* positions;       /* [max_tokens]                               */

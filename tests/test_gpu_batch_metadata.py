@@ -237,3 +237,36 @@ def test_refusals_of_the_wrapper(dev):
             call(**bad)
             pytest.fail(f"{list(bad)} was taken")
     assert call(out=out) is out
+
+
+def test_a_step_in_which_a_request_has_no_token(dev):
+    """Rows past the step's tokens, and a request without one: with a query bound
+    of 2 the layer goes by the cumulative lengths, and later rows stay with theirs."""
+    hq, hkv, d, block = 4, 2, 64, 16
+    gen = torch.Generator().manual_seed(2)
+    pool = ops.mxfp4_kv_pool(8, block, hkv, d, device=dev)
+    layer = PagedAttention(hq, d, d ** -0.5, hkv)
+    layer.k_cache, layer.v_cache, layer.k_scale, layer.v_scale = pool
+    tables = torch.tensor([[3, 1], [0, 2], [6, 5]], dtype=torch.int32, device=dev)
+    x = torch.randn(3, 20, hq + 2 * hkv, d, generator=gen).to(torch.bfloat16)
+    done = [17, 5, 9]
+    for i in range(3):
+        slots = torch.tensor([int(tables[i, p // block]) * block + p % block for p in range(done[i])])
+        rows = x[i, :done[i]].to(dev)
+        ops.store_kvcache(rows[:, hq:hq + hkv].contiguous(), rows[:, hq + hkv:].contiguous(), pool[0], pool[1],
+                          slots.to(dev), k_scale=pool[2], v_scale=pool[3])
+    lens = [18, 5, 10]
+    vec = lambda z: torch.tensor(z, dtype=torch.int32, device=dev)  # noqa: E731
+    _, ctx, _ = prepare_batch_device(vec(lens), vec(done), tables, block, max_tokens=3, max_seqlen_q=2,
+                                     max_seqlen_k=18)
+    qkv = torch.stack([x[0, 17], x[2, 9], x[1, 19]])  # the last row is nobody's
+    gpu = qkv.to(dev)
+    with attention_context(ctx):
+        out = layer(gpu[:, :hq], gpu[:, hq:hq + hkv], gpu[:, hq + hkv:])
+    for row, i in ((0, 0), (1, 2)):
+        n = lens[i]
+        kk, vv = (oracle.values(*oracle.quantise(x[i, :n, a:a + hkv])) for a in (hq, hq + hkv))
+        kk[-1], vv[-1] = x[i, n - 1, hq:hq + hkv].double(), x[i, n - 1, hq + hkv:].double()
+        ref, tol = oracle.attend(qkv[row:row + 1, :hq], kk, vv, torch.ones(1, n, dtype=torch.bool), d ** -0.5,
+                                 torch.bfloat16, 13)
+        assert not ((out[row:row + 1].double().cpu() - ref).abs() > tol).any()

@@ -757,3 +757,45 @@ def test_decode_of_more_workgroups_than_a_flat_grid_holds(dev, d, split):
     ops.paged_decode(q, k, v, table, torch.ones(n, dtype=torch.int32, device=dev), max_seq_len=8192, scale=0.1,
                      split_tokens=split, out=out, k_scale=ks, v_scale=vs)
     assert torch.equal(out, want.expand(n, hkv, d))
+
+
+@pytest.mark.parametrize("d, prefixes, qlens", [(128, [3000, 10, 700], [20, 300, 1]), (64, [2000, 0], [40, 64])])
+def test_a_captured_step_replays(dev, d, prefixes, qlens):
+    """Store, varlen attention with the fused store and load in one graph: each
+    replay, on other rows, is the eager calls' result."""
+    gen = torch.Generator().manual_seed(47)
+    hq, hkv = 8, 2
+    klens = [p + m for p, m in zip(prefixes, qlens)]
+    total, blocks = sum(qlens), sum(-(-n // 16) for n in klens)
+    pool = Pool(gen, blocks, 16, hkv, d, "nhd", BF16, dev)
+    (kc, vc), kw = pool.args()
+    tables = tables_for(gen, klens, 16, blocks)
+    slots = torch.cat([slots_of(t, n, 16)[p:] for t, n, p in zip(tables, klens, prefixes)]).int().to(dev)
+    tables, cq, ck = tables.to(dev), cu(qlens).to(dev), cu(klens).to(dev)
+    x = torch.randn(total, hq + 2 * hkv, d, generator=gen).to(BF16).to(dev)
+    first = torch.tensor([slots_of(tables[0].cpu(), 5, 16)[i] for i in range(5)], device=dev)
+
+    def step():
+        k, v = x[:, hq:hq + hkv], x[:, hq + hkv:]
+        ops.store_kvcache(k[:5], v[:5], kc, vc, first, **kw)  # new rows of the first prefix
+        out = ops.varlen_attention(x[:, :hq], k, v, cq, ck, max(qlens), max(klens), scale=d ** -0.5,
+                                   causal=True, k_cache=kc, v_cache=vc, block_tables=tables,
+                                   slot_mapping=slots, **kw)
+        return (out, *ops.load_kvcache(kc, vc, slots, **kw))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for i in range(3):
+        x.copy_(torch.randn(total, hq + 2 * hkv, d, generator=gen).to(BF16))
+        graph.replay()
+        mine = [t.clone() for t in got]
+        state = [t.clone() for t in pool.gpu]
+        want = step()
+        assert all(torch.equal(a, b) for a, b in zip(mine, want))
+        assert all(torch.equal(a, b) for a, b in zip(state, pool.gpu))

@@ -110,7 +110,10 @@ def prepare_batch_device(
 
     The host gives what it has to know: ``max_tokens`` rows (the step's tokens,
     or more: rows behind the last token have slot -1 and belong to no sequence)
-    and bounds of the query and context lengths."""
+    and bounds of the query and context lengths.  ``max_seqlen_q`` 1 with a row
+    per request makes it a decode step, in which the layers take row i as
+    request i's: every request has one new token then.  A step in which some
+    request may have none gives ``max_seqlen_q`` 2 or more."""
     meta = ops.batch_metadata(lens, num_computed, request_tables, block_size,
                               max_tokens=max_tokens, rows=rows, free_blocks=free_blocks,
                               free_count=free_count)
