@@ -1559,11 +1559,13 @@ __global__ __launch_bounds__(256) void varlen_merge_kernel(VarlenParams p) {
 // rows and all of a row's pieces, few long items (61 tokens over 16K: 8 items of
 // 64 pieces) left the chip to 32 workgroups, 70 us; with two rows a workgroup
 // and one for every piece that there may be, 52K workgroups took 16 us to come
-// and go.
+// and go.  NG is what makes kMergeRows one pass (launches at head_dim 128, two
+// passes of four groups against one of two, us: four prompts over 2K-8K 89.9 /
+// 88.6, 61 tokens over 16K 39.7 / 39.2; eight rows a workgroup 88.9, 48).
 constexpr int kMergeRows = 4;
 template <bool kBF16, int D, int G, bool kHalf>
 __global__ __launch_bounds__(256) void varlen_mx4_merge_kernel(VarlenParams p) {
-  constexpr int LPR = D / 4, NG = 4, ROWS = 256 / LPR / NG;  // rows per pass
+  constexpr int LPR = D / 4, NG = D == 128 ? 2 : 4, ROWS = 256 / LPR / NG;  // rows per pass
   constexpr int rows = kHalf ? kRowsPerWG / 2 : kRowsPerWG;  // of a piece's partials
   static_assert(split_pieces(kSplitOver) <= 128, "two heads a lane");
   __shared__ __align__(16) float s_o[ROWS * NG * D];
