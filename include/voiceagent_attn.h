@@ -418,6 +418,13 @@ int va_varlen_attention_mx4(const va_varlen_args* args, const va_mx4_scales* sca
  * negative.  Tokens past max_tokens are not written; entries of positions and
  * slot_mapping behind the last token are 0 and -1.  Sums stop at 2^31 - 1.
  *
+ * totals counts every token, max_tokens or not.  With cut the cumulative
+ * lengths are those of the tokens written: a request's queries end where
+ * max_tokens does, its keys with them, so attention over max_tokens rows stays
+ * inside them whatever the lengths say.  Without it they are the full sums,
+ * which attention may be given only where totals[0] <= max_tokens.  Blocks are
+ * taken for all of lens either way.
+ *
  * With free_count, request i holds the blocks of its computed tokens (columns
  * below ceil(num_computed[i] / block_size)), and the blocks of its new columns
  * are taken from the free list's end: the k-th block taken, in request order
@@ -452,6 +459,7 @@ typedef struct va_batch_args {
   const int32_t* free_blocks; /* optional, with free_count                */
   const int32_t* free_count;  /* [1] entries of free_blocks in use        */
   int32_t free_capacity;      /* entries of free_blocks                   */
+  int32_t cut;                /* cumulative lengths stop at max_tokens    */
 } va_batch_args;
 
 int va_batch_metadata(const va_batch_args* args, void* stream);

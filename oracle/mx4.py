@@ -114,14 +114,14 @@ def attend(q, k, v, seen, scale: float, dtype: torch.dtype, product_bits: float)
 
 
 def batch_metadata(lens, done, tables, block, *, max_tokens, rows=None, padded=0, width=None,
-                   free=None, count=None):
+                   free=None, count=None, cut=False):
     """Plain integers: dict of lists, and the request tables as they become."""
     tables = [list(t) for t in tables]
     wide = len(tables[0]) if tables else 0
     width = wide if width is None else width
     rows = list(range(len(lens))) if rows is None else rows
     taken = missing = 0
-    pos, slots, cu_q, cu_k, out = [], [], [0], [0], []
+    pos, slots, new, ctx, out = [], [], [], [], []
     for n, c, r in zip(lens, done, rows):
         n = max(0, n)
         c = min(max(0, c), n)
@@ -141,18 +141,21 @@ def batch_metadata(lens, done, tables, block, *, max_tokens, rows=None, padded=0
             blk = row[p // block] if p // block < len(row) else -1
             pos.append(p)
             slots.append(blk * block + p % block if blk >= 0 else -1)
-        cu_q.append(cu_q[-1] + n - c)
-        cu_k.append(cu_k[-1] + n)
+        new.append(n - c)
+        ctx.append(n)
         out.append((row + [-1] * width)[:width])
     for _ in range(max(0, padded - len(lens))):
         pos.append(0)
         slots.append(-1)
-        cu_q.append(cu_q[-1] + 1)
-        cu_k.append(cu_k[-1] + 1)
+        new.append(1)
+        ctx.append(1)
         out.append([0] * width)
-    totals = [cu_q[-1], max((b - a for a, b in zip(cu_q, cu_q[1:])), default=0),
-              max((b - a for a, b in zip(cu_k, cu_k[1:])), default=0),
-              max(0, (count or 0) - taken), missing]
+    totals = [sum(new), max(new, default=0), max(ctx, default=0), max(0, (count or 0) - taken), missing]
+    cu_q, cu_k = [0], [0]
+    for m, n in zip(new, ctx):
+        kept = min(m, max_tokens - cu_q[-1]) if cut else m
+        cu_q.append(cu_q[-1] + kept)
+        cu_k.append(cu_k[-1] + n - m + kept)
     fill = max(0, max_tokens - len(pos))
     return {"positions": (pos + [0] * fill)[:max_tokens], "slots": (slots + [-1] * fill)[:max_tokens],
             "cu_q": cu_q, "cu_k": cu_k, "tables": out, "totals": totals, "request_tables": tables}

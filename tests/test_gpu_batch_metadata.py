@@ -270,3 +270,92 @@ def test_a_step_in_which_a_request_has_no_token(dev):
         ref, tol = oracle.attend(qkv[row:row + 1, :hq], kk, vv, torch.ones(1, n, dtype=torch.bool), d ** -0.5,
                                  torch.bfloat16, 13)
         assert not ((out[row:row + 1].double().cpu() - ref).abs() > tol).any()
+
+
+@pytest.mark.parametrize("room", [0, 1, 9, 10, 11, 29, 30, 31, 60, 64, 100])
+@pytest.mark.parametrize("padded", [0, 6])
+def test_cut_lengths_stop_at_the_rows(dev, room, padded):
+    lens, done = [20, 30, 0, 40], [10, 10, 0, 10]
+    tables = [[5 * i + j for j in range(3)] for i in range(4)]
+    t = torch.tensor(tables, dtype=torch.int32, device=dev)
+    vec = lambda v: torch.tensor(v, dtype=torch.int32, device=dev)  # noqa: E731
+    kw = {"max_tokens": room, "padded_batch": padded, "cut": True}
+    m = ops.batch_metadata(vec(lens), vec(done), t, 16, **kw)
+    want = oracle.batch_metadata(lens, done, tables, 16, max_tokens=room, padded=padded, cut=True)
+    again = ops.batch_metadata(vec(lens), vec(done), t, 16, out=ops.BatchMetadata(
+        *(torch.full_like(getattr(m, f), 7) for f in ("positions", "slot_mapping", "cu_seqlens_q", "cu_seqlens_k",
+                                                      "block_tables", "totals"))), **kw)
+    for got in (m, again):
+        assert got.cu_seqlens_q.tolist() == want["cu_q"] and got.cu_seqlens_q[-1] <= room
+        assert got.cu_seqlens_k.tolist() == want["cu_k"]
+        assert got.positions.tolist() == want["positions"] and got.slot_mapping.tolist() == want["slots"]
+        assert got.block_tables.tolist() == want["tables"] and got.totals.tolist() == want["totals"]
+    whole = ops.batch_metadata(vec(lens), vec(done), t, 16, max_tokens=200, padded_batch=padded, cut=True)
+    assert whole.cu_seqlens_q.tolist() == oracle.batch_metadata(lens, done, tables, 16, max_tokens=200,
+                                                                padded=padded)["cu_q"]
+
+
+def test_cut_sums_of_many_requests_and_past_31_bits(dev):
+    rng = random.Random(11)
+    lens = [rng.randint(0, 90) for _ in range(3000)]
+    done = [rng.choice([0, n, rng.randint(0, n)]) for n in lens]
+    t = torch.zeros(3000, 6, dtype=torch.int32, device=dev)
+    vec = lambda v, d=torch.int32: torch.tensor(v, dtype=d, device=dev)  # noqa: E731
+    for room in (5, 20000, 10 ** 6):
+        m = ops.batch_metadata(vec(lens), vec(done), t, 16, max_tokens=room, cut=True)
+        want = oracle.batch_metadata(lens, done, [[0] * 6] * 3000, 16, max_tokens=room, cut=True)
+        assert m.cu_seqlens_q.tolist() == want["cu_q"] and m.cu_seqlens_k.tolist() == want["cu_k"]
+    big = vec([2 ** 31 - 100, 2 ** 40, 2 ** 31 - 1], torch.int64)
+    m = ops.batch_metadata(big, vec([0, 0, 0], torch.int64), t, 16, max_tokens=40, cut=True)
+    assert m.cu_seqlens_q.tolist() == m.cu_seqlens_k.tolist() == [0, 40, 40, 40]
+    m = ops.batch_metadata(big, vec([2 ** 31 - 110, 0, 0], torch.int64), t, 16, max_tokens=40, cut=True)
+    assert m.cu_seqlens_q.tolist() == [0, 10, 40, 40]
+    assert m.cu_seqlens_k.tolist() == [0, 2 ** 31 - 100, 2 ** 31 - 70, 2 ** 31 - 70]
+
+
+@pytest.mark.parametrize("fmt", ["bf16", "mxfp4"])
+def test_a_step_of_more_tokens_than_rows(dev, fmt):
+    """prepare_batch_device with 40 rows for 54 tokens: the layer attends and stores the
+    rows that there are, each as its request's next tokens, and touches nothing else."""
+    hq, hkv, d, block, room = 4, 2, 128, 16, 40
+    gen = torch.Generator().manual_seed(3)
+    lens, done = [20, 30, 33], [3, 10, 16]
+    tables = torch.tensor([[3, 1, 0], [2, 5, 4], [6, 8, 7]], dtype=torch.int32)
+    rows = torch.randn(3, 33, hq + 2 * hkv, d, generator=gen).to(torch.bfloat16)
+    layer = PagedAttention(hq, d, d ** -0.5, hkv)
+    if fmt == "mxfp4":
+        pool = ops.mxfp4_kv_pool(9, block, hkv, d, device=dev)
+        layer.k_cache, layer.v_cache, layer.k_scale, layer.v_scale = pool
+        scales = {"k_scale": pool[2], "v_scale": pool[3]}
+    else:
+        layer.k_cache, layer.v_cache = (torch.zeros(9, block, hkv, d, dtype=torch.bfloat16, device=dev)
+                                        for _ in range(2))
+        scales = {}
+    at = lambda i, p: int(tables[i, p // block]) * block + p % block  # noqa: E731
+    for i in range(3):
+        x = rows[i, :done[i]].to(dev)
+        ops.store_kvcache(x[:, hq:hq + hkv], x[:, hq + hkv:], layer.k_cache, layer.v_cache,
+                          torch.tensor([at(i, p) for p in range(done[i])], device=dev), **scales)
+    vec = lambda v: torch.tensor(v, dtype=torch.int32, device=dev)  # noqa: E731
+    _, ctx, meta = prepare_batch_device(vec(lens), vec(done), tables.to(dev), block, max_tokens=room,
+                                        max_seqlen_q=20, max_seqlen_k=33)
+    assert meta.totals[0] == 54 and ctx.cu_seqlens_q.tolist() == [0, 17, 37, 40]
+    assert ctx.cu_seqlens_k.tolist() == [0, 20, 50, 69]
+    kept = [20, 30, 19]  # the third request's tokens 16, 17 and 18
+    x = torch.cat([rows[i, done[i]:kept[i]] for i in range(3)]).to(dev)
+    byte = lambda t: t.view(torch.uint8).cpu().flatten(0, 1)  # noqa: E731
+    before = byte(layer.k_cache)
+    with attention_context(ctx):
+        out = layer(x[:, :hq], x[:, hq:hq + hkv], x[:, hq + hkv:])
+    changed = (byte(layer.k_cache) != before).flatten(1).any(-1).nonzero().flatten().tolist()
+    assert changed == sorted(at(i, p) for i in range(3) for p in range(done[i], kept[i]))
+    row = 0
+    for i in range(3):
+        a, n = done[i], kept[i]
+        k, v = (rows[i, :n, j:j + hkv] for j in (hq, hq + hkv))
+        kk, vv = ((oracle.values(*oracle.quantise(z)) if fmt == "mxfp4" else z.double()) for z in (k, v))
+        kk[a:], vv[a:] = k[a:].double(), v[a:].double()
+        seen = torch.arange(n) <= torch.arange(a, n)[:, None]
+        ref, tol = oracle.attend(rows[i, a:n, :hq], kk, vv, seen, d ** -0.5, torch.bfloat16, 17)
+        assert not ((out[row:row + n - a].double().cpu() - ref).abs() > tol).any()
+        row += n - a

@@ -234,6 +234,7 @@ class BatchArgs(ctypes.Structure):
         ("free_blocks", c_void_p),
         ("free_count", c_void_p),
         ("free_capacity", c_int32),
+        ("cut", c_int32),
     ]
 
 

@@ -3,7 +3,7 @@
 // list.
 //
 // Every output element follows from its request's lengths and three sums over
-// the requests before it (query tokens, context tokens, blocks taken), so one
+// the requests before it (query tokens, computed tokens, blocks taken), so one
 // launch does it all: a workgroup serves R consecutive requests, first sums
 // the requests before them (16 bytes each, from L2), scans its own, and then
 // writes their tokens and table rows, both striped over the grid's second
@@ -42,6 +42,7 @@ struct BatchParams {
   const int32_t* free_blocks;
   const int32_t* free_count;
   int32_t free_capacity;
+  int32_t cu_limit;  // cumulative query lengths stop here
 };
 
 // A request's computed and context lengths, and the table columns it holds and
@@ -103,11 +104,11 @@ __global__ __launch_bounds__(kBatchThreads) void batch_metadata_kernel(BatchPara
   const int count = p.free_count != nullptr ? max(0, min(*p.free_count, p.free_capacity)) : 0;
 
   // The requests before this workgroup's.
-  int q0 = 0, k0 = 0, take0 = 0, mq = 0, mk = 0;
+  int q0 = 0, done0 = 0, take0 = 0, mq = 0, mk = 0;
   for (int i = tid; i < r0; i += kBatchThreads) {
     const Request r = load_request(p, i);
     q0 = sat_add(q0, r.len - r.done);
-    k0 = sat_add(k0, r.len);
+    done0 = sat_add(done0, r.done);
     take0 = sat_add(take0, r.cols - r.held);
     mq = max(mq, r.len - r.done);
     mk = max(mk, r.len);
@@ -120,30 +121,30 @@ __global__ __launch_bounds__(kBatchThreads) void batch_metadata_kernel(BatchPara
     if (r0 + tid < p.num_seqs) row = p.rows != nullptr ? p.rows[r0 + tid] : r0 + tid;
   }
   q0 = block_all<false>(q0, s_red);
-  k0 = block_all<false>(k0, s_red);
+  done0 = block_all<false>(done0, s_red);
   take0 = block_all<false>(take0, s_red);
   // Inclusive scans over lanes, then over waves.
-  int q = mine.len - mine.done, k = mine.len, take = mine.cols - mine.held;
+  int q = mine.len - mine.done, done = mine.done, take = mine.cols - mine.held;
   const int lane = tid & 63, wave = tid >> 6;
   __shared__ int s_scan[3][kBatchThreads / 64];
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) {
-    const int a = __shfl_up(q, o, 64), b = __shfl_up(k, o, 64), c = __shfl_up(take, o, 64);
+    const int a = __shfl_up(q, o, 64), b = __shfl_up(done, o, 64), c = __shfl_up(take, o, 64);
     if (lane >= o) {
       q = sat_add(q, a);
-      k = sat_add(k, b);
+      done = sat_add(done, b);
       take = sat_add(take, c);
     }
   }
   if (lane == 63) {
     s_scan[0][wave] = q;
-    s_scan[1][wave] = k;
+    s_scan[1][wave] = done;
     s_scan[2][wave] = take;
   }
   __syncthreads();
   for (int w = 0; w < wave; ++w) {
     q = sat_add(q, s_scan[0][w]);
-    k = sat_add(k, s_scan[1][w]);
+    done = sat_add(done, s_scan[1][w]);
     take = sat_add(take, s_scan[2][w]);
   }
   if (tid == 0) s_q[0] = s_take[0] = 0;
@@ -155,8 +156,11 @@ __global__ __launch_bounds__(kBatchThreads) void batch_metadata_kernel(BatchPara
     s_cols[tid] = mine.cols;
     s_row[tid] = r0 + tid >= p.num_seqs ? -2 : (row >= 0 && row < p.num_req ? row : -1);
     if (stripe == 0) {
-      p.cu_q[r0 + tid + 1] = sat_add(q0, q);
-      p.cu_k[r0 + tid + 1] = sat_add(k0, k);
+      // Context tokens are computed ones and those of the queries that there
+      // is room for (sums of non-negative terms, saturated at the end alike).
+      const int cq = min(sat_add(q0, q), p.cu_limit);
+      p.cu_q[r0 + tid + 1] = cq;
+      p.cu_k[r0 + tid + 1] = sat_add(sat_add(done0, done), cq);
     }
   }
   if (blockIdx.x == 0 && stripe == 0 && tid == 0) p.cu_q[0] = p.cu_k[0] = 0;
@@ -274,6 +278,7 @@ extern "C" int va_batch_metadata(const va_batch_args* a, void* stream) {
   p.padded = a->padded_seqs;
   p.block_size = a->block_size;
   p.max_tokens = a->max_tokens;
+  p.cu_limit = a->cut ? a->max_tokens : INT32_MAX;
   p.bs_div = make_fastdiv((uint32_t)a->block_size);
   p.positions = a->positions;
   p.slots = a->slot_mapping;

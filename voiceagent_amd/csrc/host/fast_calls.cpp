@@ -589,7 +589,7 @@ std::tuple<int64_t, std::vector<at::Tensor>> batch_metadata(
     const at::Tensor& lens, const at::Tensor& done, const at::Tensor& req, int64_t block_size,
     int64_t max_tokens, const c10::optional<at::Tensor>& rows, int64_t padded, int64_t width,
     const c10::optional<at::Tensor>& free_blocks, const c10::optional<at::Tensor>& free_count,
-    int64_t device, int64_t stream) {
+    bool cut, int64_t device, int64_t stream) {
   std::vector<at::Tensor> out;
   const auto no = [&]() { return std::make_tuple(kNotTaken, out); };
   if (g_batch == nullptr || !on(lens, device) || !on(done, device) || !on(req, device)) return no();
@@ -638,6 +638,7 @@ std::tuple<int64_t, std::vector<at::Tensor>> batch_metadata(
   a.padded_seqs = (int32_t)size;
   a.block_size = (int32_t)block_size;
   a.max_tokens = (int32_t)max_tokens;
+  a.cut = cut;
   a.positions = static_cast<int64_t*>(out[0].data_ptr());
   a.slot_mapping = static_cast<int32_t*>(out[1].data_ptr());
   a.cu_seqlens_q = static_cast<int32_t*>(out[2].data_ptr());

@@ -110,13 +110,15 @@ def prepare_batch_device(
 
     The host gives what it has to know: ``max_tokens`` rows (the step's tokens,
     or more: rows behind the last token have slot -1 and belong to no sequence)
-    and bounds of the query and context lengths.  ``max_seqlen_q`` 1 with a row
+    and bounds of the query and context lengths.  A step with more tokens than
+    rows ends at the last row, in the middle of a request where it falls:
+    ``totals[0]`` counts the tokens that there were.  ``max_seqlen_q`` 1 with a row
     per request makes it a decode step, in which the layers take row i as
     request i's: every request has one new token then.  A step in which some
     request may have none gives ``max_seqlen_q`` 2 or more."""
     meta = ops.batch_metadata(lens, num_computed, request_tables, block_size,
                               max_tokens=max_tokens, rows=rows, free_blocks=free_blocks,
-                              free_count=free_count)
+                              free_count=free_count, cut=True)
     context = AttentionContext(
         cu_seqlens_q=meta.cu_seqlens_q,
         cu_seqlens_k=meta.cu_seqlens_k,

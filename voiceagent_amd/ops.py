@@ -1012,6 +1012,7 @@ def batch_metadata(
     free_blocks: torch.Tensor | None = None,
     free_count: torch.Tensor | None = None,
     out: BatchMetadata | None = None,
+    cut: bool = False,
 ) -> BatchMetadata:
     """Positions, slots, cumulative lengths and block tables of a step, built
     on the GPU from the requests' lengths (engine/model_runner.py:183-233,
@@ -1022,7 +1023,11 @@ def batch_metadata(
     without it) of ``request_tables`` ([requests, width] int32).  Its new tokens'
     positions and slots follow those of the requests before it; entries up to
     ``max_tokens`` behind the last token are 0 and -1, and tokens past it are
-    not written.  ``block_tables`` row i holds the request's blocks, then -1
+    not written.  The cumulative lengths count those tokens too, and attention
+    over ``max_tokens`` rows may be given them only where ``totals[0]``, the
+    step's tokens, is no more; with ``cut`` they stop at ``max_tokens`` (the
+    keys of a request that is cut end with its queries), and may be given to
+    attention whatever the lengths say.  ``block_tables`` row i holds the request's blocks, then -1
     (``table_width`` columns, request_tables' width by default).  Rows B ..
     ``padded_batch`` - 1 are a captured decode graph's padding: one token at
     position 0 with slot -1, table row 0, key length 1.  A row or column outside
@@ -1046,7 +1051,8 @@ def batch_metadata(
             rc, made = fast.batch_metadata(lens, num_computed, request_tables, int(block_size),
                                            int(max_tokens), rows, int(padded_batch),
                                            -1 if table_width is None else int(table_width),
-                                           free_blocks, free_count, index, _raw_stream(index))
+                                           free_blocks, free_count, bool(cut), index,
+                                           _raw_stream(index))
             if rc == 0:
                 return BatchMetadata(*made)
             if _FAST_NOT_TAKEN < rc < 0:
@@ -1102,7 +1108,7 @@ def batch_metadata(
         cu_seqlens_k=out.cu_seqlens_k.data_ptr(), block_tables=out.block_tables.data_ptr(),
         table_stride=out.block_tables.stride(0), table_width=width,
         totals=out.totals.data_ptr(), free_blocks=N.ptr(free_blocks), free_count=N.ptr(free_count),
-        free_capacity=0 if free_blocks is None else free_blocks.numel())
+        free_capacity=0 if free_blocks is None else free_blocks.numel(), cut=bool(cut))
     index = _device_index(device)
     with _current(index):
         N.check("va_batch_metadata",
