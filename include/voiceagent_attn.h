@@ -430,10 +430,10 @@ int va_varlen_attention_mx4(const va_varlen_args* args, const va_mx4_scales* sca
  * are taken from the free list's end: the k-th block taken, in request order
  * and ascending columns, is free_blocks[free_count - 1 - k].  They are written
  * to the request's row of request_tables (rows[i] must then be distinct);
- * columns past its width are not taken.  When the list runs out, the columns
- * left get -1, and so the slots.  free_count is not written, nor may it lie in
- * totals: totals says what is left, and a launch with the same inputs gives the
- * same outputs.
+ * columns past its width are not taken, and a request without a row in the
+ * table takes none.  When the list runs out, the columns left get -1, and so
+ * the slots.  free_count is not written, nor may it lie in totals: totals says
+ * what is left, and a launch with the same inputs gives the same outputs.
  */
 typedef struct va_batch_args {
   uint32_t struct_size; /* sizeof(va_batch_args)                          */

@@ -127,16 +127,15 @@ def batch_metadata(lens, done, tables, block, *, max_tokens, rows=None, padded=0
         c = min(max(0, c), n)
         here = 0 <= r < len(tables)
         cols = min(-(-n // block), wide)
-        held = min(-(-c // block), cols) if free is not None else cols
+        held = min(-(-c // block), cols) if free is not None and here else cols
         row = list(tables[r][:held]) if here else [-1] * held
         for col in range(held, cols):
             at = count - 1 - taken
             taken += 1
             blk = free[at] if at >= 0 else -1
             missing += at < 0
-            row.append(blk if here else -1)
-            if here:
-                tables[r][col] = blk
+            row.append(blk)
+            tables[r][col] = blk
         for p in range(c, n):
             blk = row[p // block] if p // block < len(row) else -1
             pos.append(p)

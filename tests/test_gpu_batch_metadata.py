@@ -359,3 +359,16 @@ def test_a_step_of_more_tokens_than_rows(dev, fmt):
         ref, tol = oracle.attend(rows[i, a:n, :hq], kk, vv, seen, d ** -0.5, torch.bfloat16, 17)
         assert not ((out[row:row + n - a].double().cpu() - ref).abs() > tol).any()
         row += n - a
+
+
+@pytest.mark.parametrize("lack", [0, 6])
+def test_a_row_outside_the_table_takes_no_blocks(dev, lack):
+    m = run(dev, [20, 30, 40, 17], [0, 10, 0, 3], rows=[7, -1, 1, 0], requests=4, width=3, alloc=True, lack=lack,
+            seed=8)
+    if not lack:
+        assert m.totals.tolist()[4] == 0
+    rng = random.Random(9)
+    lens = [rng.randint(0, 90) for _ in range(1025)]
+    done = [rng.choice([0, n, rng.randint(0, n)]) for n in lens]
+    rows = rng.sample(range(2000), 1025)  # about half outside
+    run(dev, lens, done, rows=rows, requests=1000, alloc=True, seed=10)

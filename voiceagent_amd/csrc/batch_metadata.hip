@@ -45,10 +45,12 @@ struct BatchParams {
   int32_t cu_limit;  // cumulative query lengths stop here
 };
 
-// A request's computed and context lengths, and the table columns it holds and
-// needs (padding rows: none).
+// A request's computed and context lengths, the table columns it holds and
+// needs (padding rows: none), and its row of the request table (-1: outside it,
+// -2: padding).  Without a row there is nowhere to write a block: such a request
+// takes none.
 struct Request {
-  int done, len, held, cols;
+  int done, len, held, cols, row;
 };
 __device__ inline Request load_request(const BatchParams& p, int i) {
   Request r;
@@ -56,6 +58,7 @@ __device__ inline Request load_request(const BatchParams& p, int i) {
     r.done = 0;
     r.len = 1;
     r.held = r.cols = 0;
+    r.row = -2;
     return r;
   }
   auto clamp = [](int64_t x, int64_t hi) { return (int)(x < 0 ? 0 : (x > hi ? hi : x)); };
@@ -67,7 +70,9 @@ __device__ inline Request load_request(const BatchParams& p, int i) {
     return c < p.req_width ? c : p.req_width;
   };
   r.cols = columns(r.len);
-  r.held = p.free_count != nullptr ? columns(r.done) : r.cols;
+  const int row = p.rows != nullptr ? p.rows[i] : i;
+  r.row = row >= 0 && row < p.num_req ? row : -1;
+  r.held = p.free_count != nullptr && r.row >= 0 ? columns(r.done) : r.cols;
   return r;
 }
 
@@ -114,12 +119,8 @@ __global__ __launch_bounds__(kBatchThreads) void batch_metadata_kernel(BatchPara
     mk = max(mk, r.len);
   }
   // Its own, one a lane.
-  Request mine = {0, 0, 0, 0};
-  int row = -1;
-  if (tid < nr) {
-    mine = load_request(p, r0 + tid);
-    if (r0 + tid < p.num_seqs) row = p.rows != nullptr ? p.rows[r0 + tid] : r0 + tid;
-  }
+  Request mine = {0, 0, 0, 0, -1};
+  if (tid < nr) mine = load_request(p, r0 + tid);
   q0 = block_all<false>(q0, s_red);
   done0 = block_all<false>(done0, s_red);
   take0 = block_all<false>(take0, s_red);
@@ -154,7 +155,7 @@ __global__ __launch_bounds__(kBatchThreads) void batch_metadata_kernel(BatchPara
     s_done[tid] = mine.done;
     s_held[tid] = mine.held;
     s_cols[tid] = mine.cols;
-    s_row[tid] = r0 + tid >= p.num_seqs ? -2 : (row >= 0 && row < p.num_req ? row : -1);
+    s_row[tid] = mine.row;
     if (stripe == 0) {
       // Context tokens are computed ones and those of the queries that there
       // is room for (sums of non-negative terms, saturated at the end alike).

@@ -1037,8 +1037,9 @@ def batch_metadata(
     hold the blocks of their computed tokens, and the blocks of their new
     columns are taken from the list's end, in request order: the k-th taken is
     ``free_blocks[free_count - 1 - k]``.  They are written into request_tables
-    (``rows`` must be distinct); columns that the list does not reach get -1
-    there, and so do their slots.  ``free_count`` itself is not changed: the
+    (``rows`` must be distinct; a request whose row is outside it takes none);
+    columns that the list does not reach get -1 there, and so do their slots.
+    ``free_count`` itself is not changed: the
     count left is ``totals[3]`` (``result.free_count``), the blocks that were
     missing ``totals[4]`` (an ``out`` that free_count lies in is refused: copy
     the count left into it after the launch).
