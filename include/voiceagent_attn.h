@@ -433,7 +433,11 @@ int va_varlen_attention_mx4(const va_varlen_args* args, const va_mx4_scales* sca
  * columns past its width are not taken, and a request without a row in the
  * table takes none.  When the list runs out, the columns left get -1, and so
  * the slots.  free_count is not written, nor may it lie in totals: totals says
- * what is left, and a launch with the same inputs gives the same outputs.
+ * what is left, and a launch with the same inputs gives the same outputs.  A
+ * step that lacked blocks, or had more tokens than max_tokens, is to be made
+ * again from the free_count and the num_computed it began with: columns below
+ * num_computed are held whatever the table says, so those that got -1 would
+ * stay without a block.  The output arrays may not overlap the input ones.
  */
 typedef struct va_batch_args {
   uint32_t struct_size; /* sizeof(va_batch_args)                          */

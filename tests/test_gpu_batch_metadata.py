@@ -372,3 +372,23 @@ def test_a_row_outside_the_table_takes_no_blocks(dev, lack):
     done = [rng.choice([0, n, rng.randint(0, n)]) for n in lens]
     rows = rng.sample(range(2000), 1025)  # about half outside
     run(dev, lens, done, rows=rows, requests=1000, alloc=True, seed=10)
+
+
+def test_a_step_that_lacked_blocks_is_made_again(dev):
+    """With the list that it began with and more blocks in it: the same requests take
+    the same blocks, and the columns that had got none are filled."""
+    lens, done = [40, 50, 17], [16, 0, 16]
+    start = [[70, -1, -1, -1], [-1, -1, -1, -1], [71, -1, -1, -1]]
+    t = torch.tensor(start, dtype=torch.int32, device=dev)
+    vec = lambda v: torch.tensor(v, dtype=torch.int32, device=dev)  # noqa: E731
+    short = ops.batch_metadata(vec(lens), vec(done), t, 16, max_tokens=75, free_blocks=vec([1, 2, 3, 4]),
+                               free_count=vec([4]))
+    assert short.totals.tolist()[3:] == [0, 3]
+    assert t.tolist() == [[70, 4, 3, -1], [2, 1, -1, -1], [71, -1, -1, -1]]
+    # Blocks that came back go under the list that was there.
+    free = [11, 12, 13, 14, 1, 2, 3, 4]
+    m = ops.batch_metadata(vec(lens), vec(done), t, 16, max_tokens=75, free_blocks=vec(free), free_count=vec([8]))
+    want = oracle.batch_metadata(lens, done, start, 16, max_tokens=75, free=free, count=8)
+    assert m.totals.tolist() == want["totals"] and m.totals.tolist()[3:] == [1, 0]
+    assert t.tolist() == want["request_tables"] == [[70, 4, 3, -1], [2, 1, 14, 13], [71, 12, -1, -1]]
+    assert m.slot_mapping.tolist() == want["slots"] and min(want["slots"]) >= 0

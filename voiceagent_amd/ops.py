@@ -1042,10 +1042,13 @@ def batch_metadata(
     ``free_count`` itself is not changed: the
     count left is ``totals[3]`` (``result.free_count``), the blocks that were
     missing ``totals[4]`` (an ``out`` that free_count lies in is refused: copy
-    the count left into it after the launch).
+    the count left into it after the launch).  A step that lacked blocks, or had
+    more tokens than ``max_tokens``, is to be made again from the list and the
+    ``num_computed`` it began with: columns below ``num_computed`` are held
+    whatever the table says, so those that got -1 would stay without a block.
 
     ``out``: tensors of an earlier result of the same sizes to write into (a
-    captured graph's static buffers)."""
+    captured graph's static buffers); they may not overlap the inputs."""
     if out is None and (table_width is None or table_width >= 0):
         fast, index = _fast_on(lens, LAYOUT_NHD)
         if fast is not None:
