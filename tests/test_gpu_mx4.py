@@ -799,3 +799,29 @@ def test_a_captured_step_replays(dev, d, prefixes, qlens):
         want = step()
         assert all(torch.equal(a, b) for a, b in zip(mine, want))
         assert all(torch.equal(a, b) for a, b in zip(state, pool.gpu))
+
+
+def test_varlen_over_a_16_bit_pool_reads_no_scales(dev):
+    """k_scale / v_scale belong to FP8 and MXFP4 pools: over a 16-bit pool a tensor
+    of any size, on any device, changes nothing and is not waited for."""
+    gen = torch.Generator().manual_seed(49)
+    kc, vc = (torch.randn(4, 16, 2, 128, generator=gen).to(BF16).to(dev) for _ in range(2))
+    q = torch.randn(40, 4, 128, generator=gen).to(BF16).to(dev)
+    table = torch.tensor([[0, 2, 1]], dtype=torch.int32, device=dev)
+    c40 = cu([40]).to(dev)
+
+    def call(prologue=None, **kw):
+        return ops.varlen_attention(q, None, None, c40, c40, 40, 40, scale=0.1, causal=True, k_cache=kc,
+                                    v_cache=vc, block_tables=table, prologue=prologue, **kw)
+
+    pro = ops.QKPrologue(*(torch.ones(128, dtype=BF16, device=dev) for _ in range(2)), 1e-6,
+                         torch.ones(64, 128, device=dev), torch.arange(40, device=dev))
+    want = call(), call(pro)
+    for scale in (2.0, None, torch.full((3,), 2.0, device=dev), torch.tensor(2.0, device=dev), torch.ones(2, 2)):
+        mode = torch.cuda.get_sync_debug_mode()
+        torch.cuda.set_sync_debug_mode("error")
+        try:
+            got = call(k_scale=scale, v_scale=scale), call(pro, k_scale=scale, v_scale=scale)
+        finally:
+            torch.cuda.set_sync_debug_mode(mode)
+        assert all(torch.equal(a, b) for a, b in zip(got, want))

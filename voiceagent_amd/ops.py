@@ -169,9 +169,6 @@ def _mx4_structs(k_cache: torch.Tensor, v_cache: torch.Tensor, layout: str, k_sc
     return pool, scales
 
 
-_NUMBERS = (float, int)
-
-
 def _number(scale: float | torch.Tensor) -> float:
     """An FP8 pool's scale (other pools ignore theirs)."""
     _require(not isinstance(scale, torch.Tensor) or scale.numel() == 1,
@@ -867,11 +864,18 @@ def varlen_attention(
     """
     pool_dtype = None if k_cache is None else k_cache.dtype
     mx4 = pool_dtype is MXFP4_KV_DTYPE
+    if not mx4 and pool_dtype is not FP8_KV_DTYPE:
+        # A 16-bit pool, or none, has no scales: whatever is given is not read,
+        # but an MXFP4 pool's belong to codes.
+        for scale_of in (k_scale, v_scale):
+            _require(scale_of.__class__ is float or
+                     getattr(scale_of, "dtype", None) is not MXFP4_SCALE_DTYPE,
+                     f"float8_e8m0fnu scales need an MXFP4 pool, got {pool_dtype}")
+        k_scale = v_scale = 1.0
     fast = _FAST if _FAST_LOADED else _fast_calls()
     if (fast is not None and prologue is None and layout in (LAYOUT_NHD, LAYOUT_HND) and
             pool_dtype is not FP8_KV_DTYPE and
-            (isinstance(k_scale, torch.Tensor) and isinstance(v_scale, torch.Tensor) if mx4 else
-             k_scale.__class__ in _NUMBERS and v_scale.__class__ in _NUMBERS)):
+            (not mx4 or (isinstance(k_scale, torch.Tensor) and isinstance(v_scale, torch.Tensor)))):
         index = q.get_device()
         if index >= 0 and index == torch.cuda.current_device():
             if out is None:
