@@ -825,3 +825,11 @@ def test_varlen_over_a_16_bit_pool_reads_no_scales(dev):
         finally:
             torch.cuda.set_sync_debug_mode(mode)
         assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_load_refuses_scales_that_are_no_tensors(dev):
+    k, v, ks, vs = ops.mxfp4_kv_pool(4, 16, 2, 128, device=dev)
+    slots = torch.zeros(3, dtype=torch.int32, device=dev)
+    for k_scale, v_scale in ((1.0, 1.0), (ks, 1.0), (None, vs)):
+        with pytest.raises(ops.AttentionArgumentError):
+            ops.load_kvcache(k, v, slots, k_scale=k_scale, v_scale=v_scale)

@@ -316,7 +316,8 @@ def load_kvcache(
     outside the pool read as zeros.  A 16-bit or FP8 pool's rows are read by
     indexing it."""
     fast, index = _fast_on(k_cache, layout)
-    if fast is not None and dtype in (torch.bfloat16, torch.float16):
+    if (fast is not None and dtype in (torch.bfloat16, torch.float16) and
+            isinstance(k_scale, torch.Tensor) and isinstance(v_scale, torch.Tensor)):
         rc, key, value = fast.load_kvcache_mx4(k_cache, v_cache, slot_mapping,
                                                dtype == torch.float16, layout == LAYOUT_HND,
                                                k_scale, v_scale, index, _raw_stream(index))
@@ -324,8 +325,9 @@ def load_kvcache(
             return key, value
         if _FAST_NOT_TAKEN < rc < 0:
             N.check("va_load_kvcache_mx4", rc)
-    device = _check_gpu(k_cache, v_cache, slot_mapping, k_scale, v_scale)
+    device = _check_gpu(k_cache, v_cache, slot_mapping)
     pool, scales = _mx4_structs(k_cache, v_cache, layout, k_scale, v_scale, dtype)
+    _check_gpu(k_cache, k_scale)
     hkv, d = pool_heads(k_cache, layout)
     _require(slot_mapping.dim() == 1, "slot_mapping must be a vector")
     shape = (int(slot_mapping.numel()), hkv, d)
