@@ -833,3 +833,26 @@ def test_load_refuses_scales_that_are_no_tensors(dev):
     for k_scale, v_scale in ((1.0, 1.0), (ks, 1.0), (None, vs)):
         with pytest.raises(ops.AttentionArgumentError):
             ops.load_kvcache(k, v, slots, k_scale=k_scale, v_scale=v_scale)
+
+
+def test_workspaces_of_other_pools_keep_their_size(dev):
+    """Two partitions a compute unit are an MXFP4 pool's at head_dim 128 with an even
+    number of kv heads; other decodes allocate for one."""
+    cus = torch.cuda.get_device_properties(dev).multi_processor_count
+    one = (cus * 2 * 2 * 4 + 255) // 256 * 256 + cus * 2 * 128 * 4
+    kc, vc = (torch.zeros(128, 16, 2, 128, dtype=BF16, device=dev) for _ in range(2))
+    q = torch.zeros(1, 4, 128, dtype=BF16, device=dev)
+    table = torch.arange(128, dtype=torch.int32, device=dev)[None]
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    ops._WORKSPACES.pop((dev.index or 0, stream.cuda_stream), None)
+    with torch.cuda.stream(stream):
+        ops.paged_decode(q, kc, vc, table, torch.tensor([2048], device=dev), max_seq_len=2048, scale=0.1)
+    torch.cuda.synchronize()
+    assert ops._WORKSPACES[(dev.index or 0, stream.cuda_stream)].numel() == one
+    assert ops.decode_workspace_bound(dev, 4, 2, 128, BF16) == one
+    assert ops.decode_workspace_bound(dev, 4, 2, 128, ops.MXFP4_KV_DTYPE) > one
+    for shape in ((4, 2, 64), (6, 3, 128)):
+        both = [ops.decode_workspace_bound(dev, *shape, t) for t in (BF16, ops.MXFP4_KV_DTYPE)]
+        assert both[0] == both[1]
+    assert ops.decode_workspace_bound(dev, 4, 2, 128) == ops.decode_workspace_bound(dev, 4, 2, 128, ops.MXFP4_KV_DTYPE)

@@ -575,18 +575,21 @@ def _pool_struct(k_cache, v_cache, layout, k_scale, v_scale) -> N.KvPool:
 
 
 def decode_workspace_bound(device: torch.device, num_heads: int, num_kv_heads: int,
-                           head_dim: int) -> int:
+                           head_dim: int, kv_dtype: torch.dtype | None = None) -> int:
     """Bytes that covers every automatic split (split_tokens = 0) of a decode
     with these heads on `device`, whatever the batch and lengths: the split
-    gives at most one partition per compute unit (over an MXFP4 pool two) over
-    all (sequence, kv head) pairs, each holding (m, l) and head_dim floats per query head of the
-    group, with the (m, l) block rounded to 256 bytes."""
+    gives at most one partition per compute unit over all (sequence, kv head)
+    pairs, each holding (m, l) and head_dim floats per query head of the
+    group, with the (m, l) block rounded to 256 bytes.  Over an MXFP4 pool at
+    head_dim 128 a workgroup may serve two kv heads, and there may be two
+    partitions per compute unit.  ``kv_dtype``: the pool's, or None for any."""
     index = _device_index(device)
     cus = _CUS.get(index)
     if cus is None:
         cus = _CUS[index] = torch.cuda.get_device_properties(index).multi_processor_count
     group = max(1, num_heads // max(1, num_kv_heads))
-    cus *= 2  # (MXFP4: workgroups that serve two kv heads each, twice the partitions)
+    if kv_dtype in (None, MXFP4_KV_DTYPE) and head_dim == 128 and num_kv_heads % 2 == 0:
+        cus *= 2
     return (cus * group * 2 * 4 + 255) // 256 * 256 + cus * group * head_dim * 4
 
 
@@ -636,13 +639,14 @@ def _order_noalloc(index: int) -> None:
 
 
 def reserve_decode_workspace(device: torch.device, num_heads: int, num_kv_heads: int,
-                             head_dim: int, stream: torch.cuda.Stream | None = None) -> None:
+                             head_dim: int, stream: torch.cuda.Stream | None = None,
+                             kv_dtype: torch.dtype | None = None) -> None:
     """Allocate the decode workspace of `stream` (torch's current stream by
-    default) up front, at the size every automatic split needs, e.g. before
-    HIP graph capture.  ``torch.cuda.graph`` captures on a stream of its own
+    default) up front, at the size every automatic split needs over a pool of
+    ``kv_dtype`` (None: over any), e.g. before HIP graph capture.  ``torch.cuda.graph`` captures on a stream of its own
     unless it is given one: pass that stream here to reserve for it."""
     device = torch.device(device)
-    bound = decode_workspace_bound(device, num_heads, num_kv_heads, head_dim)
+    bound = decode_workspace_bound(device, num_heads, num_kv_heads, head_dim, kv_dtype)
     decode_workspace(device, bound, floor=bound, stream=stream)
 
 
@@ -809,7 +813,8 @@ def paged_decode(
         nbytes = (lib.va_paged_decode_mx4_workspace_bytes if mx4
                   else lib.va_paged_decode_workspace_bytes)(ctypes.byref(args))
         if nbytes:
-            ws = decode_workspace(device, nbytes, floor=decode_workspace_bound(device, hq, hkv, d))
+            ws = decode_workspace(device, nbytes, floor=decode_workspace_bound(
+                device, hq, hkv, d, k_cache.dtype))
             args.workspace = ws.data_ptr()
             args.workspace_bytes = ws.numel()
         if mx4:
