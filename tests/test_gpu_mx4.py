@@ -856,3 +856,34 @@ def test_workspaces_of_other_pools_keep_their_size(dev):
         both = [ops.decode_workspace_bound(dev, *shape, t) for t in (BF16, ops.MXFP4_KV_DTYPE)]
         assert both[0] == both[1]
     assert ops.decode_workspace_bound(dev, 4, 2, 128) == ops.decode_workspace_bound(dev, 4, 2, 128, ops.MXFP4_KV_DTYPE)
+
+
+def test_qwen3_core_splits_as_the_plain_layer_does(dev):
+    """An eager step that says its exact longest context: the fused step's partitions
+    are those of the plain layer's, so the outputs are the same bits."""
+    gen = torch.Generator().manual_seed(50)
+    hq, hkv, d, block = 16, 8, 128, 16
+    k_lens = [9000, 5000, 8100]
+    blocks = sum(-(-n // block) for n in k_lens)
+    tables = tables_for(gen, k_lens, block, blocks)
+    x = torch.randn(3, hq + 2 * hkv, d, generator=gen).to(BF16).to(dev)
+    positions = torch.tensor([n - 1 for n in k_lens], device=dev)
+    slots = torch.cat([slots_of(t, n, block)[-1:] for t, n in zip(tables, k_lens)]).int().to(dev)
+    context = AttentionContext(cu_seqlens_q=cu([1, 1, 1]).to(dev), cu_seqlens_k=cu(k_lens).to(dev), max_seqlen_q=1,
+                               max_seqlen_k=9000, slot_mapping=slots, block_tables=tables.to(dev),
+                               max_seqlen_k_exact=True)
+    got = []
+    for core in (True, False):
+        pool = Pool(torch.Generator().manual_seed(51), blocks, block, hkv, d, "nhd", BF16, dev)
+        (kc, vc), kw = pool.args()
+        layer = Qwen3AttentionCore(hq, d, hkv, max_position=9000).to(dev)
+        layer.k_cache, layer.v_cache, layer.k_scale, layer.v_scale = kc, vc, kw["k_scale"], kw["v_scale"]
+        q, k, v = x[:, :hq], x[:, hq:hq + hkv], x[:, hq + hkv:]
+        with attention_context(context):
+            if core:
+                out = layer(positions, q, k, v)
+            else:
+                qn, kn = ops.qk_norm_rope(q, k, layer.prologue(positions))
+                out = PagedAttention.forward(layer, qn, kn, v)
+        got.append(out.reshape(3, -1))
+    assert torch.equal(got[0], got[1])

@@ -10,6 +10,9 @@ import torch
 from oracle import mx4 as oracle
 from voiceagent_amd import _native as N
 from voiceagent_amd import ops
+from voiceagent_amd.layers.attention import PagedAttention
+from voiceagent_amd.layers.context import AttentionContext, attention_context
+from voiceagent_amd.layers.qwen3 import Qwen3AttentionCore
 
 
 def _row(values, dtype=torch.bfloat16):
@@ -236,3 +239,30 @@ def test_load_refusals():
     assert "16-byte" in call(lambda a, s: setattr(a, "value_stride_tok", 1028))
     assert "null" in call(lambda a, s: setattr(a, "slot_mapping", None))
     assert "dtype" in call(lambda a, s: setattr(a, "dtype", N.VA_F32))
+
+
+@pytest.mark.parametrize("exact", [False, True])
+def test_qwen3_core_decodes_as_the_plain_layer_does(monkeypatch, exact):
+    """The fused decode step of the prologue's layer gives paged_decode the pool, the
+    layout, the scales and the split that the plain layer's gives it."""
+    calls = []
+    monkeypatch.setattr(ops, "paged_decode", lambda *args, **kw: calls.append((args, kw)) or args[0])
+    cu = torch.tensor([0, 5000, 14000], dtype=torch.int32)
+    context = AttentionContext(cu_seqlens_q=torch.arange(3, dtype=torch.int32), cu_seqlens_k=cu, max_seqlen_q=1,
+                               max_seqlen_k=9000, slot_mapping=torch.zeros(2, dtype=torch.int32),
+                               block_tables=torch.zeros(2, 600, dtype=torch.int32), max_seqlen_k_exact=exact)
+    layer = Qwen3AttentionCore(4, 128, 2, max_position=8)
+    layer.k_cache, layer.v_cache, layer.k_scale, layer.v_scale = ops.mxfp4_kv_pool(2, 16, 2, 128, device="cpu",
+                                                                                   layout=ops.LAYOUT_HND)
+    layer.kv_layout = ops.LAYOUT_HND
+    q, k, v = (torch.zeros(2, n, 128, dtype=torch.bfloat16) for n in (4, 2, 2))
+    positions = torch.tensor([4999, 8999])
+    with attention_context(context):
+        layer(positions, q, k, v)
+        PagedAttention.forward(layer, q, k, v, layer.prologue(positions))
+    (a, kw), (b, plain) = calls
+    assert all(x is y for x, y in zip(a, b)) and kw.keys() == plain.keys()
+    pro, other = kw.pop("prologue"), plain.pop("prologue")
+    assert pro.positions is other.positions and pro.eps == other.eps
+    assert all(kw[n] is plain[n] or kw[n] == plain[n] for n in kw)
+    assert kw["split_tokens"] == (ops.SPLIT_EXACT if exact else 0)

@@ -31,7 +31,6 @@ from torch import nn
 
 from voiceagent_amd import ops
 from voiceagent_amd.layers.attention import PagedAttention
-from voiceagent_amd.layers.context import get_attention_context
 
 
 def rotary_cos_sin_cache(head_dim: int, max_position: int, base: float) -> torch.Tensor:
@@ -63,30 +62,9 @@ class Qwen3AttentionCore(PagedAttention):
     def forward(self, positions: torch.Tensor, q: torch.Tensor, k: torch.Tensor,
                 v: torch.Tensor) -> torch.Tensor:
         """positions [T] (int64), q [T, Hq, D], k/v [T, Hkv, D]: raw projections."""
-        context = get_attention_context()
         pro = self.prologue(positions)
-        num_seqs = context.cu_seqlens_k.numel() - 1
-        decode = context.max_seqlen_q == 1 and q.shape[0] == num_seqs
-        if self.fuse_prologue and self.fuse_store and decode and self.k_cache.numel():
-            return ops.paged_decode(
-                q,
-                self.k_cache,
-                self.v_cache,
-                context.block_tables,
-                context.cu_seqlens_k,
-                lens_cumulative=True,
-                max_seq_len=context.max_seqlen_k,
-                scale=self.scale,
-                layout=self.kv_layout,
-                new_k=k,
-                new_v=v,
-                new_slots=context.slot_mapping,
-                prologue=pro,
-                k_scale=self.k_scale,
-                v_scale=self.v_scale,
-            )
         if self.fuse_prologue:
-            # Prefill batches: the varlen launch applies the query prologue.
+            # (a decode step in one launch; prefill batches as varlen_fuse_prologue says)
             return super().forward(q, k, v, prologue=pro)
         qn, kn = ops.qk_norm_rope(q, k, pro)
         return super().forward(qn, kn, v)
