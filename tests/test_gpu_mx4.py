@@ -887,3 +887,61 @@ def test_qwen3_core_splits_as_the_plain_layer_does(dev):
                 out = PagedAttention.forward(layer, qn, kn, v)
         got.append(out.reshape(3, -1))
     assert torch.equal(got[0], got[1])
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("d, hq, hkv, layout, lens", [(128, 16, 8, "nhd", [40, 300]), (64, 8, 2, "hnd", [40, 300]),
+                                                      (256, 4, 2, "nhd", [40, 300]),
+                                                      (128, 4, 2, "nhd", [16500, 16420])])
+def test_decode_keeps_small_terms_beside_large_ones(dev, dtype, d, hq, hkv, layout, lens):
+    """Two channels of the query far larger than the rest, whose products cancel in
+    every key: what is left is the other channels' sum.  Q K^T is summed in float32,
+    so a logit is off by at most 2^-17 of its products' magnitudes (d additions of a
+    step of 2^-24 each, and room), 2^-17 * 2 * 6 * 1024 * scale = 0.01 at d = 64."""
+    gen = torch.Generator().manual_seed(48)
+    blocks = sum(-(-n // 16) for n in lens)
+    pool = Pool(gen, blocks, 16, hkv, d, layout, dtype, dev)
+    pool.cpu[0][..., 0] = 7 + 16 * 15  # elements 0 and 1 of every key: 6 and -6
+    pool.cpu[2][:] = 127
+    pool.gpu = [t.to(dev) for t in pool.cpu]
+    tables = tables_for(gen, lens, 16, blocks)
+    q = torch.randn(len(lens), hq, d, generator=gen)
+    q[..., :2] = 1024.0
+    q = q.to(dtype)
+    (kc, vc), kw = pool.args()
+    scale = d ** -0.5
+    out = ops.paged_decode(q.to(dev), kc, vc, tables.to(dev), torch.tensor(lens, device=dev), max_seq_len=max(lens),
+                           scale=scale, split_tokens=ops.SPLIT_EXACT, **kw)
+    for b, n in enumerate(lens):
+        k, v = pool.rows(slots_of(tables[b], n, 16))
+        ref, tol = oracle.attend(q[b:b + 1], k, v, torch.ones(1, n, dtype=torch.bool), scale, dtype, VARLEN_BITS)
+        close(out[b:b + 1], ref, tol)
+
+
+@pytest.mark.parametrize("hq, hkv, d", [(16, 8, 128), (8, 2, 64), (4, 2, 256)])
+def test_decode_of_the_smallest_f16_values(dev, hq, hkv, d):
+    # Keys and values of f16's subnormals, 2^-24 to 2^-15: exact in the products.
+    def edit(pool, tables):
+        for t in (2, 3):
+            pool.cpu[t] = pool.cpu[t].clamp(104, 109)
+
+    run_decode(dev, [40, 300], hq=hq, hkv=hkv, d=d, dtype=F16, edit=edit, scale=2.0 ** 14, new=True, seed=52)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("bad", [math.inf, -math.inf, math.nan])
+def test_decode_of_a_query_that_is_not_finite(dev, dtype, bad):
+    # One key, whose element beside the bad one is positive, zero or negative.
+    k, v, ks, vs = ops.mxfp4_kv_pool(3, 16, 2, 128, device=dev)
+    rows = torch.ones(3, 2, 128, dtype=dtype)
+    rows[1, :, 5], rows[2, :, 5] = 0.0, -1.0
+    slots = torch.tensor([0, 16, 32], dtype=torch.int32, device=dev)
+    ops.store_kvcache(rows.to(dev), rows.to(dev), k, v, slots, k_scale=ks, v_scale=vs)
+    q = torch.ones(3, 4, 128, dtype=dtype)
+    q[:, 1, 5] = bad
+    out = ops.paged_decode(q.to(dev), k, v, torch.arange(3, dtype=torch.int32, device=dev)[:, None],
+                           torch.ones(3, dtype=torch.int32, device=dev), max_seq_len=1, scale=0.1, k_scale=ks,
+                           v_scale=vs).cpu()
+    assert out[:, 1].isnan().all()
+    for h in (0, 2, 3):
+        assert torch.equal(out[:, h], rows[:, h // 2])

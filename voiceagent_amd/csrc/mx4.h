@@ -96,73 +96,6 @@ __device__ inline uint4 mx4_values8(uint32_t codes, uint32_t scale) {
                     mx4_pair<ET, 2>(codes, s), mx4_pair<ET, 3>(codes, s));
 }
 
-// Scaled products of 16 rows of 128 e2m1 codes (lane (r, g): 16 bytes, group g of
-// row r, and its scale byte) with 16 rows of e4m3 (lane (r, g): elements
-// 16 g .. + 15 in the first 16 bytes and 64 + 16 g .. in the others; the scale
-// byte of elements 32 g .. + 31): c[4 g + i][r] += sum_k a[4 g + i][k] b[r][k].
-// The instruction aligns neighbouring products before adding them, to 13 bits of
-// the largest; over 12800 sums of 128 normal products the error was 4.2e-5 of
-// the norm of the products at most, 4e-6 rms.
-typedef int mx_i32x8 __attribute__((ext_vector_type(8)));
-typedef float mx_f32x4 __attribute__((ext_vector_type(4)));
-__device__ inline mx_f32x4 mx4_mfma(uint4 a, int as, const mx_i32x8& b, int bs, mx_f32x4 c) {
-  const mx_i32x8 av = {(int)a.x, (int)a.y, (int)a.z, (int)a.w, 0, 0, 0, 0};
-  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(av, b, c, 4 /* e2m1 */, 0 /* e4m3 */, 0,
-                                                          as, 0, bs);
-}
-
-// N e4m3 terms of 16 elements of ET (two words of 8), for the power of two
-// `unit`: term 0 rounds x / unit to e4m3, term t what the terms before it left,
-// in units of 2^-4t.  The conversions divide by their scale themselves.
-template <typename ET, int N>
-__device__ inline void mx4_split16(const uint4 (&u)[2], float unit, uint4 (&term)[N]) {
-  typedef short s16x2 __attribute__((ext_vector_type(2)));
-  const uint32_t in[8] = {u[0].x, u[0].y, u[0].z, u[0].w, u[1].x, u[1].y, u[1].z, u[1].w};
-  uint32_t w[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    s16x2 r = {0, 0};
-    if constexpr (ET::kIsBF16) {
-      r = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(r, __builtin_bit_cast(bf16x2_t, in[2 * i]), unit,
-                                                    false);
-      r = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(r, __builtin_bit_cast(bf16x2_t, in[2 * i + 1]),
-                                                    unit, true);
-    } else {
-      r = __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(r, __builtin_bit_cast(f16x2_t, in[2 * i]), unit,
-                                                   false);
-      r = __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(r, __builtin_bit_cast(f16x2_t, in[2 * i + 1]),
-                                                   unit, true);
-    }
-    w[i] = __builtin_bit_cast(uint32_t, r);
-  }
-  term[0] = make_uint4(w[0], w[1], w[2], w[3]);
-  float x[16];
-  float(&x0)[8] = *reinterpret_cast<float(*)[8]>(&x[0]);
-  float(&x1)[8] = *reinterpret_cast<float(*)[8]>(&x[8]);
-  ET::unpack(u[0], x0);
-  ET::unpack(u[1], x1);
-#pragma unroll
-  for (int t = 1; t < N; ++t) {
-    const float before = t == 1 ? unit : unit * 0.0625f;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const auto lo = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(w[i], before, false);
-      const auto hi = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(w[i], before, true);
-      x[4 * i] -= lo[0];
-      x[4 * i + 1] -= lo[1];
-      x[4 * i + 2] -= hi[0];
-      x[4 * i + 3] -= hi[1];
-      s16x2 r = {0, 0};
-      r = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(r, x[4 * i], x[4 * i + 1], before * 0.0625f,
-                                                   false);
-      r = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(r, x[4 * i + 2], x[4 * i + 3], before * 0.0625f,
-                                                   true);
-      w[i] = __builtin_bit_cast(uint32_t, r);
-    }
-    term[t] = make_uint4(w[0], w[1], w[2], w[3]);
-  }
-}
-
 // Host checks of a pool's scale arrays that every entry point makes, for rows
 // of head_dim elements: rows of scales are read as single words.
 int check_mx4(const char* fn, const va_kv_pool& pool, const va_mx4_scales* sc, int head_dim);

@@ -7,15 +7,16 @@
 // share of the HBM rate is a row every ~7 cycles and the work between the load
 // and the matrix cores is what has to be kept small:
 //
-//   * S^T = K Q^T takes the codes as they are: v_mfma_scale_f32_16x16x128
-//     multiplies e2m1 K rows (A: 16 bytes a lane, its scale byte beside them)
-//     by an fp8 Q.  A query is cut once into e4m3 terms, each holding four
-//     more of its significant bits (two for bf16, three for f16) with a power
-//     of two of its own, so that the products lose nothing of it.  The
-//     instruction aligns the products of neighbouring k before adding: sums
-//     came out within 4.2e-5 of the norm of the products (rms 4e-6 over 12800
-//     sums), against 2^-8 of each P, its rounding below.
-//   * O^T += V^T P^T takes V in 16 bits.  A lane reads D / 16 neighbouring
+//   * S^T = K Q^T takes K in 16 bits, which hold its values exactly, and sums
+//     the products in fp32, as over the other pools.  A lane reads 32
+//     neighbouring codes of a row, one scale's (16 at head_dim 64), and converts
+//     them two an instruction; the query's operand has the same order of k.
+//     (Codes as they are, on scaled 16x16x128 products against a query cut into
+//     e4m3 terms: that instruction aligns neighbouring products to 13 bits
+//     before adding.  Two query channels of 256 times the others' size, whose
+//     products cancel, put the output off by 0.6%, of 4096 times by 5.7%; fp32
+//     sums 0.16% at any size, which is P's and the output's rounding.)
+//   * O^T += V^T P^T takes V in 16 bits too.  A lane reads D / 16 neighbouring
 //     elements of eight tokens, converts them with their scales (two elements
 //     an instruction) and pairs tokens with v_perm: no transposing read.  P^T
 //     is the S^T accumulator packed in place, rounded to the rows' type (the
@@ -95,8 +96,7 @@ __global__ __launch_bounds__(W * 64, W == 4 && D <= 128 ? 4 : 2) void paged_deco
   using VT = typename Sh::V;
   constexpr int CH = Sh::CH, NV = Sh::NV, CPR = Sh::CPR, ROWB = Sh::ROWB, SCW = Sh::SCW;
   constexpr int NT = W * 64, ROW16 = D * 2;
-  constexpr int TERMS = ET::kIsBF16 ? 2 : 3;        // e4m3 terms of a query
-  constexpr int QM = D == 64 ? (TERMS + 1) / 2 : TERMS;  // products per chunk (two terms share one at 64)
+  constexpr int KP = D == 64 ? 2 : 4;               // products per chunk: 8 elements a lane each
   constexpr int LPR = D / 8, RPL = 64 / LPR, E = 8;  // the row layout of prologue.h
   constexpr int QROWS = (G + RPL - 1) / RPL;
   constexpr int LPS = kMx4Group / NV;  // lanes that share a V scale
@@ -184,24 +184,21 @@ __global__ __launch_bounds__(W * 64, W == 4 && D <= 128 ? 4 : 2) void paged_deco
   const bool early = !p.dyn_split;
   const int early_limit = last_part ? INT32_MAX : start + P;
   if (early) load_ids(0, early_limit);
-  constexpr int PC = D == 64 ? 1 : 2;  // 16-element pieces of a chunk
-  // Queries in the order of the products' B operand: lane (r16, c4) holds
-  // elements 128 c + 64 f + 16 c4 .. + 15 (f = 0, 1) of head r16; with the
-  // prologue as rows first.
-  uint4 qraw[CH][PC][2];
+  // Queries in the order of the products' B operand, K's: lane (r16, c4) holds
+  // elements 128 c + 8 KP c4 + 8 i .. + 7 of head r16; with the prologue as rows
+  // first.
+  uint4 qreg[CH][KP];
   uint4 qrow[QROWS];
+  constexpr int QL = 16 * KP;  // bytes of a lane's elements of a chunk
   if constexpr (!kProlog) {
 #pragma unroll
     for (int c = 0; c < CH; ++c)
 #pragma unroll
-      for (int f = 0; f < PC; ++f)
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          // Columns past the group read head 0's row; their scores are unused.
-          const int g = r16 < G ? r16 : 0;
-          qraw[c][f][i] = ld16(p.q + b * p.q_sb + (int64_t)(h * G + g) * p.q_sh +
-                               (128 * c + 64 * f + 16 * c4) * 2 + 16 * i);
-        }
+      for (int i = 0; i < KP; ++i) {
+        // Columns past the group read head 0's row; their scores are unused.
+        const int g = r16 < G ? r16 : 0;
+        qreg[c][i] = ld16(p.q + b * p.q_sb + (int64_t)(h * G + g) * p.q_sh + 256 * c + QL * c4 + 16 * i);
+      }
   } else {
 #pragma unroll
     for (int i = 0; i < QROWS; ++i) {
@@ -353,11 +350,8 @@ __global__ __launch_bounds__(W * 64, W == 4 && D <= 128 ? 4 : 2) void paged_deco
 #pragma unroll
       for (int c = 0; c < CH; ++c)
 #pragma unroll
-        for (int f = 0; f < PC; ++f)
-#pragma unroll
-          for (int i = 0; i < 2; ++i)
-            asm volatile("" ::"v"(qraw[c][f][i].x), "v"(qraw[c][f][i].y), "v"(qraw[c][f][i].z),
-                         "v"(qraw[c][f][i].w));
+        for (int i = 0; i < KP; ++i)
+          asm volatile("" ::"v"(qreg[c][i].x), "v"(qreg[c][i].y), "v"(qreg[c][i].z), "v"(qreg[c][i].w));
     }
     if constexpr (kMask)
       asm volatile("" ::"v"(mraw[0]), "v"(mraw[1]), "v"(mraw[2]), "v"(mraw[3]), "v"(mraw[4]));
@@ -436,11 +430,9 @@ __global__ __launch_bounds__(W * 64, W == 4 && D <= 128 ? 4 : 2) void paged_deco
 #pragma unroll
     for (int c = 0; c < CH; ++c)
 #pragma unroll
-      for (int f = 0; f < PC; ++f)
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-          qraw[c][f][i] = *reinterpret_cast<const uint4*>(s_w + (r16 < G ? r16 : 0) * ROW16 +
-                                                          (128 * c + 64 * f + 16 * c4) * 2 + 16 * i);
+      for (int i = 0; i < KP; ++i)
+        qreg[c][i] = *reinterpret_cast<const uint4*>(s_w + (r16 < G ? r16 : 0) * ROW16 + 256 * c +
+                                                     QL * c4 + 16 * i);
   }
 
   // ---- the current row, quantised: lane (., c4) the K group its step
@@ -550,59 +542,23 @@ __global__ __launch_bounds__(W * 64, W == 4 && D <= 128 ? 4 : 2) void paged_deco
     return;
   }
 
-  // ---- the queries' e4m3 terms: the row's largest magnitude goes to
-  // [2^7, 2^8), so a term's unit is at most 2^-9 of it ----
-  mx_i32x8 qf[QM][CH];
-  int qs[QM];
+  // A query row with an infinity or a NaN scores NaN, whatever the keys are: its
+  // scores start there.
+  float score0 = 0.f;
   {
     uint32_t mag = 0;
 #pragma unroll
     for (int c = 0; c < CH; ++c)
 #pragma unroll
-      for (int f = 0; f < PC; ++f)
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const uint32_t m8 = mx4_absmax8(qraw[c][f][i]);
-          mag = mag > m8 ? mag : m8;
-        }
+      for (int i = 0; i < KP; ++i) {
+        const uint32_t m8 = mx4_absmax8(qreg[c][i]);
+        mag = mag > m8 ? mag : m8;
+      }
     const uint32_t m16 = (uint32_t)__shfl_xor((int)mag, 16, 64);
     mag = mag > m16 ? mag : m16;
     const uint32_t m32 = (uint32_t)__shfl_xor((int)mag, 32, 64);
     mag = mag > m32 ? mag : m32;
-    const uint32_t bits = ET::kIsBF16
-                              ? mag << 16
-                              : __float_as_uint((float)__builtin_bit_cast(_Float16, (uint16_t)mag));
-    // Scale byte of the first term; a row below 2^-100 keeps fewer bits, a
-    // row with an infinity or a NaN scores NaN.
-    int e = (int)(bits >> 23) - 7;
-    e = e < 27 ? 27 : e;
-    const float unit = __uint_as_float((uint32_t)e << 23);
-    const bool bad = bits >= 0x7f800000u;
-#pragma unroll
-    for (int c = 0; c < CH; ++c) {
-      uint4 term[PC][TERMS];
-#pragma unroll
-      for (int f = 0; f < PC; ++f) {
-        mx4_split16<ET, TERMS>(qraw[c][f], unit, term[f]);
-      }
-      auto join = [](uint4 lo, uint4 hi) {
-        return mx_i32x8{(int)lo.x, (int)lo.y, (int)lo.z, (int)lo.w,
-                        (int)hi.x, (int)hi.y, (int)hi.z, (int)hi.w};
-      };
-#pragma unroll
-      for (int t = 0; t < QM; ++t) {
-        if constexpr (D == 64)
-          qf[t][c] = join(term[0][2 * t], 2 * t + 1 < TERMS ? term[0][2 * t + 1 < TERMS ? 2 * t + 1 : 0]
-                                                            : make_uint4(0, 0, 0, 0));
-        else
-          qf[t][c] = join(term[0][t], term[PC - 1][t]);
-      }
-    }
-#pragma unroll
-    for (int t = 0; t < QM; ++t) {
-      const int first = D == 64 ? 2 * t + (c4 >> 1) : t;
-      qs[t] = bad ? 255 : e - 4 * first;
-    }
+    if (mag >= (ET::kIsBF16 ? 0x7f80u : 0x7c00u)) score0 = __builtin_nanf("");
   }
 
   float m = kNegBig, l = 0.f;
@@ -610,11 +566,14 @@ __global__ __launch_bounds__(W * 64, W == 4 && D <= 128 ? 4 : 2) void paged_deco
 #pragma unroll
   for (int i = 0; i < NV; ++i) o[i] = mf_f32x4{0.f, 0.f, 0.f, 0.f};
 
-  // Byte offsets of the lane's reads inside a stage.
+  // Byte offsets of the lane's reads inside a stage (K: its 16 bytes of a chunk, or
+  // at head_dim 64 8, half a scale's).
+  typedef uint32_t KT __attribute__((ext_vector_type(KP)));
   const int kslot = mx4_slot(r16);
   const int hc = CPR * hd, hs = SCW * hd;  // the head's chunks and scales of a staged row
-  const int koff = kslot * PITCH + (((hc + (D == 64 ? c4 & 1 : c4)) ^ swz(kslot)) << 4);
-  const int ksoff = KS_OFF + r16 * SCP + hs + (D == 64 ? c4 & 1 : c4);
+  const int koff = D == 64 ? kslot * PITCH + (((c4 >> 1) ^ swz(kslot)) << 4) + 8 * (c4 & 1)
+                           : kslot * PITCH + (((hc + c4) ^ swz(kslot)) << 4);
+  const int ksoff = KS_OFF + r16 * SCP + hs + (D == 64 ? c4 >> 1 : c4);
   int voff[4];  // of token 4 c4 + i
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -675,14 +634,14 @@ __global__ __launch_bounds__(W * 64, W == 4 && D <= 128 ? 4 : 2) void paged_deco
       __builtin_amdgcn_wave_barrier();
     }
     // S^T: the lane's scores are tokens 4 c4 + i of both tiles, head r16.
-    uint4 kk[2][CH];
+    KT kk[2][CH];
     uint32_t kks[2][CH];
 #pragma unroll
     for (int t = 0; t < 2; ++t)
 #pragma unroll
       for (int cc = 0; cc < CH; ++cc) {
         // (a row's chunks 4 .. 7 are its chunks 0 .. 3 with the third bit flipped)
-        kk[t][cc] = *reinterpret_cast<const uint4*>(st + t * TILE_B + (koff ^ (cc << 6)));
+        kk[t][cc] = *reinterpret_cast<const KT*>(st + t * TILE_B + (koff ^ (cc << 6)));
         kks[t][cc] = (uint8_t)st[ksoff + t * 16 * SCP + 4 * cc + half(t, p.ks, r16)];
       }
     VT vv[8];
@@ -697,11 +656,12 @@ __global__ __launch_bounds__(W * 64, W == 4 && D <= 128 ? 4 : 2) void paged_deco
     mf_f32x4 sc[2];
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
-      sc[t] = mf_f32x4{0.f, 0.f, 0.f, 0.f};
+      sc[t] = mf_f32x4{score0, score0, score0, score0};
 #pragma unroll
       for (int cc = 0; cc < CH; ++cc)
 #pragma unroll
-        for (int q = 0; q < QM; ++q) sc[t] = mx4_mfma(kk[t][cc], kks[t][cc], qf[q][cc], qs[q], sc[t]);
+        for (int i = 0; i < KP; ++i)
+          sc[t] = M::qk(mx4_values8<ET>(kk[t][cc][i], kks[t][cc]), qreg[cc][i], sc[t]);
     }
     // The stage has been read: it takes the wave's step k + S (a pair's, once
     // both have read it: the stage before it takes step k + S - 1).
