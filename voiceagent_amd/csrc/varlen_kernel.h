@@ -554,14 +554,11 @@ varlen_attention_kernel(VarlenParams p) {
   uint32_t k_st = (uint32_t)p.k_st, v_st = (uint32_t)p.v_st;
   asm volatile("" : "+s"(k_st), "+s"(v_st));
   set_offsets(k_st, v_st);
-  // MXFP4 codes: chunk c of row r sits at position c ^ code_swz(r), so that 16
-  // rows' chunks c (an S^T operand) cover all banks.
-  auto code_swz = [&](int row) { return (row / (256 / CROWB)) & (CCPR - 1); };
-  // FP8 pool: a wave's 16 code rows (unswizzled, CRPI rows an instruction).
+  // A wave's 16 code rows (unswizzled, CRPI rows an instruction: a conversion
+  // reads whole rows, whose banks are all different).
   const uint32_t code_lane =
       kF8 ? (uint32_t)(lane / CCPR) * (uint32_t)p.s_slot + (uint32_t)(lane % CCPR) * 16u
-      : kMx4 ? (uint32_t)(lane / CCPR % 16) * (uint32_t)p.s_slot +
-                   (uint32_t)((lane % CCPR) ^ code_swz(lane / CCPR)) * 16u
+      : kMx4 ? (uint32_t)(lane / CCPR % 16) * (uint32_t)p.s_slot + (uint32_t)(lane % CCPR) * 16u
              : 0u;
   // kMx4: the scale array and row of the lane's word; the lanes past the 32nd
   // copy the same words again.
@@ -740,8 +737,7 @@ varlen_attention_kernel(VarlenParams p) {
         const int j = kb + crow0 + i * CRPI;
         kc[i] = zero_row;
         vc[i] = zero_row;
-        const int c = kMx4 ? (lane % CCPR) ^ code_swz(lane / CCPR) : lane % CCPR;
-        if (j < cu.prefix && j < cu.kend) pool_at(j, craw[i], c * 16, kc[i], vc[i]);
+        if (j < cu.prefix && j < cu.kend) pool_at(j, craw[i], (lane % CCPR) * 16, kc[i], vc[i]);
       }
     }
     uint2 braw[NI];
@@ -1022,7 +1018,7 @@ varlen_attention_kernel(VarlenParams p) {
             const int row = rc / NS, r = 16 * wave + row, c = rc % NS;
             if (kb + r < prefix) {
               const uint4 codes = lds_read16(s_code + is_v * CODE_B + wave * NIC * 1024,
-                                             row * CROWB + ((c ^ code_swz(row)) << 4));
+                                             row * CROWB + (c << 4));
               // (A row without a block is zeros whatever its scale word.)
               const uint32_t scale = (uint8_t)s_scale[wave * 256 + is_v * 64 + row * 4 +
                                                       scale_half(is_v ? p.vs : p.ks, row, cur.h) + c];
