@@ -1555,17 +1555,18 @@ __global__ __launch_bounds__(256) void varlen_merge_kernel(VarlenParams p) {
 // rows and all of a row's pieces, few long items (61 tokens over 16K: 8 items of
 // 64 pieces) left the chip to 32 workgroups, 70 us; with two rows a workgroup
 // and one for every piece that there may be, 52K workgroups took 16 us to come
-// and go.  NG is what makes kMergeRows one pass (launches at head_dim 128, two
-// passes of four groups against one of two, us: four prompts over 2K-8K 89.9 /
-// 88.6, 61 tokens over 16K 39.7 / 39.2; eight rows a workgroup 88.9, 48).
+// and go.  A workgroup's rows go through in one pass of NG groups (launches at
+// head_dim 128, two passes of four groups against one of two, us: four prompts
+// over 2K-8K 89.9 / 88.6, 61 tokens over 16K 39.7 / 39.2; eight rows a workgroup
+// 88.9, 48).
 constexpr int kMergeRows = 4;
 template <bool kBF16, int D, int G, bool kHalf>
 __global__ __launch_bounds__(256) void varlen_mx4_merge_kernel(VarlenParams p) {
-  constexpr int LPR = D / 4, NG = D == 128 ? 2 : 4, ROWS = 256 / LPR / NG;  // rows per pass
+  constexpr int LPR = D / 4, NG = 256 / LPR / kMergeRows;
   constexpr int rows = kHalf ? kRowsPerWG / 2 : kRowsPerWG;  // of a piece's partials
   static_assert(split_pieces(kSplitOver) <= 128, "two heads a lane");
-  __shared__ __align__(16) float s_o[ROWS * NG * D];
-  __shared__ float2 s_ml[ROWS * NG];
+  __shared__ __align__(16) float s_o[kMergeRows * NG * D];
+  __shared__ float2 s_ml[kMergeRows * NG];
   const int xcd = (int)blockIdx.x % kXcds, item = (int)blockIdx.x / kXcds;
   const int lane = threadIdx.x & 63;
   // The heads were written for slots below the count alone; the others are read
@@ -1587,57 +1588,54 @@ __global__ __launch_bounds__(256) void varlen_mx4_merge_kernel(VarlenParams p) {
   const int64_t ps = (int64_t)xcd * p.split_slots + slot;
   const int4 hd = p.part_head[ps];
   const int col = threadIdx.x % LPR, grp = threadIdx.x / LPR % NG, rw = threadIdx.x / LPR / NG;
-  for (int row0 = (int)blockIdx.y * kMergeRows;
-       row0 < min((int)blockIdx.y * kMergeRows + kMergeRows, hd.z); row0 += ROWS) {
-    const int row = row0 + rw;
-    float M = -1.0e30f, L = 0.f;
-    f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
-    if (row < hd.z) {
-      const float* po = p.part_o + (ps * rows + row) * D + 4 * col;
-      const float2* pm = p.part_ml + ps * rows + row;
-      for (int j0 = grp; j0 < hd.x; j0 += 4 * NG) {
-        f32x4_t oj[4];
-        float2 ml[4];
+  const int row = (int)blockIdx.y * kMergeRows + rw;
+  if (row - rw >= hd.z) return;
+  float M = -1.0e30f, L = 0.f;
+  f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
+  if (row < hd.z) {
+    const float* po = p.part_o + (ps * rows + row) * D + 4 * col;
+    const float2* pm = p.part_ml + ps * rows + row;
+    for (int j0 = grp; j0 < hd.x; j0 += 4 * NG) {
+      f32x4_t oj[4];
+      float2 ml[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int64_t at = min(j0 + j * NG, hd.x - 1) * (int64_t)rows;
-          ml[j] = pm[at];
-          oj[j] = *reinterpret_cast<const f32x4_t*>(po + at * D);
-        }
+      for (int j = 0; j < 4; ++j) {
+        const int64_t at = min(j0 + j * NG, hd.x - 1) * (int64_t)rows;
+        ml[j] = pm[at];
+        oj[j] = *reinterpret_cast<const f32x4_t*>(po + at * D);
+      }
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          if (j0 + j * NG >= hd.x) break;
-          const float mn = fmaxf(M, ml[j].x);
-          const float a = fast_exp2(M - mn), b = fast_exp2(ml[j].x - mn);
-          acc = acc * a + oj[j] * b;
-          L = L * a + ml[j].y * b;
-          M = mn;
-        }
+      for (int j = 0; j < 4; ++j) {
+        if (j0 + j * NG >= hd.x) break;
+        const float mn = fmaxf(M, ml[j].x);
+        const float a = fast_exp2(M - mn), b = fast_exp2(ml[j].x - mn);
+        acc = acc * a + oj[j] * b;
+        L = L * a + ml[j].y * b;
+        M = mn;
       }
     }
-    __syncthreads();  // the last pass's sums have been read
-    *reinterpret_cast<f32x4_t*>(s_o + (rw * NG + grp) * D + 4 * col) = acc;
-    if (col == 0) s_ml[rw * NG + grp] = make_float2(M, L);
-    __syncthreads();
-    if (grp != 0 || row >= hd.z) continue;
-    M = -1.0e30f;
-#pragma unroll
-    for (int g = 0; g < NG; ++g) M = fmaxf(M, s_ml[rw * NG + g].x);
-    L = 0.f;
-    acc = f32x4_t{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int g = 0; g < NG; ++g) {
-      const float b = fast_exp2(s_ml[rw * NG + g].x - M);
-      L += s_ml[rw * NG + g].y * b;
-      acc += b * *reinterpret_cast<const f32x4_t*>(s_o + (rw * NG + g) * D + 4 * col);
-    }
-    const float inv = L > 0.f ? 1.f / L : 0.f;
-    uint2 w;
-    w.x = Mma<kBF16>::pack2(acc[0] * inv, acc[1] * inv);
-    w.y = Mma<kBF16>::pack2(acc[2] * inv, acc[3] * inv);
-    *reinterpret_cast<uint2*>(p.out + (int64_t)(hd.y + row / G) * p.o_st +
-                              (int64_t)(hd.w * G + row % G) * p.o_sh + col * 8) = w;
   }
+  *reinterpret_cast<f32x4_t*>(s_o + (rw * NG + grp) * D + 4 * col) = acc;
+  if (col == 0) s_ml[rw * NG + grp] = make_float2(M, L);
+  __syncthreads();
+  if (grp != 0 || row >= hd.z) return;
+  M = -1.0e30f;
+#pragma unroll
+  for (int g = 0; g < NG; ++g) M = fmaxf(M, s_ml[rw * NG + g].x);
+  L = 0.f;
+  acc = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int g = 0; g < NG; ++g) {
+    const float b = fast_exp2(s_ml[rw * NG + g].x - M);
+    L += s_ml[rw * NG + g].y * b;
+    acc += b * *reinterpret_cast<const f32x4_t*>(s_o + (rw * NG + g) * D + 4 * col);
+  }
+  const float inv = L > 0.f ? 1.f / L : 0.f;
+  uint2 w;
+  w.x = Mma<kBF16>::pack2(acc[0] * inv, acc[1] * inv);
+  w.y = Mma<kBF16>::pack2(acc[2] * inv, acc[3] * inv);
+  *reinterpret_cast<uint2*>(p.out + (int64_t)(hd.y + row / G) * p.o_st +
+                            (int64_t)(hd.w * G + row % G) * p.o_sh + col * 8) = w;
 }
 
 // Launch the persistent grid: per XCD, as many workgroups as the kernel
