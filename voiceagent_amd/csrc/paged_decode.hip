@@ -194,10 +194,11 @@ static DecodePlan plan_decode(const va_decode_args* a) {
 // MXFP4 pools: contexts of up to this many tokens (at 8 partitions a pair or
 // more; twice as many at 4, four times at 2) stay whole, and an automatic
 // partition has at least kMx4MinPart tokens, two waves' steps.  16 query / 8 kv
-// heads of 128, whole against split, us: one context of 512 7.9 / 8.0, of 768
-// 9.5 / 8.1; 8 (4 partitions) of 768 9.8 / 10.4, of 1536 13.0 / 12.0; 16 (2) of
-// 1536 13.3 / 14.4, of 4096 34.1 / 26.0.  Partitions of at least 128 tokens took
-// 0.2 us more, of 256 0.9.
+// heads of 128, one head a workgroup, whole against split, us: one context of 512
+// 7.9 / 7.5, of 768 8.9 / 7.6; four (8 partitions) of 512 8.2 / 7.8; eight (4) of
+// 512 8.2 / 9.0, of 768 9.6 / 10.2, of 1024 10.8 / 10.3, of 1536 13.3 / 11.1; 16
+// (2) of 1024 11.1 / 12.1, of 1536 13.6 / 14.0, of 2048 17.3 / 16.2, of 4096 33.6 /
+// 25.2.
 constexpr int64_t kMx4NoSplitTokens = 512;
 constexpr int kMx4MinPart = 64;
 
@@ -205,14 +206,16 @@ constexpr int kMx4MinPart = 64;
 // token in an NHD pool are one 128-byte line, which two workgroups would each
 // request whole; together they need half as many workgroups, and as many more
 // partitions.  One head / two, us (16 query / 8 kv heads, contexts within 10% of
-// the length): 2 x 4096 11.2 / 9.7, 8 x 8192 25 / 21, 64 x 1024 25 / 18, 64 x 2048
-// 35 / 31, 128 x 2048 80 / 57, 256 x 2048 147 / 107; but 1 x 4096 8.7 / 10.1, 16 x
-// 1024 11.3 / 12.3, 64 x 512 12.8 / 12.2, 256 x 512 39 / 44 (and of contexts spread
-// over U[60, 600] 33.6 / 39.4).  So: contexts past 1024 tokens, and 128 of them or
-// more a CU and pair.  Where the heads alone fill the CUs unsplit and the pairs
-// have to be split, only long ones: 32 x 2048 22.7 / 21.2, 4096 33.4 / 33.9, 8192
-// 72 / 57.  A max_seq_len that is only a bound counts as kMx4PairBound at most
-// (8 x 768 10.2 / 9.8, 1024 11.0 / 10.0; but 256 7.9 / 9.1).
+// the length): 2 x 4096 10.1 / 9.3, 8 x 8192 25 / 21, 64 x 1024 25 / 19, 64 x 2048
+// 42 / 31, 128 x 2048 80 / 61, 256 x 2048 146 / 118; but 1 x 4096 9.1 / 9.3, 16 x
+// 1024 11.1 / 16.2, 64 x 512 14.0 / 12.3, 256 x 512 43.6 / 43.9 (and of contexts
+// spread over U[60, 600] 34.8 / 40.2).  So: contexts past 1024 tokens, and 128 of
+// them or more a CU and pair.  Where the heads alone fill the CUs unsplit and the
+// pairs have to be split, only long ones: 32 x 2048 (pairs unsplit) 22.1 / 27.6,
+// 2304 24.1 / 22.9, 4096 38.8 / 33.3, 8192 73 / 60 (the border was set where both
+// were level, before S^T took K in 16 bits).  A max_seq_len that is only a bound
+// counts as kMx4PairBound at most (8 x 768 9.6 / 9.3, 1024 10.1 / 9.5; but 256 7.4
+// / 8.5).
 constexpr int64_t kMx4PairTokens = 1024, kMx4PairPerCu = 128, kMx4PairSplit = 4096;
 constexpr int64_t kMx4PairBound = 1280;
 // A grid of one dimension holds fewer than 2^32 lanes, 512 a workgroup.
@@ -546,10 +549,10 @@ int va::paged_decode_impl(const va_decode_args* a, const va_mx4_scales* sc, cons
             : f8 && pl.wg_tokens <= kWave12Tokens ? 12
                                               : 0;
   if (mx4) {
-    // Several small workgroups a CU where there are more than CUs (256 x
-    // U[60,600]: 54 us with eight waves, 30 with four, 28 with two, which are
-    // slower for longer contexts), one large one otherwise (32: 8.8 against
-    // 10.6 with four).
+    // Several small workgroups a CU where there are more than CUs (16 / 8 heads,
+    // contexts of U[60,600], us with eight waves / four: 40 of them 13.7 / 11.8,
+    // 64 15.9 / 12.9, 256 58 / 35; 256 x 2048 151 / 146), one large one otherwise
+    // (32 9.2 / 10.5).
     p.waves = wgs > current_device_cus() ? 4 : 8;
     p.num_seqs = a->num_seqs;
     p.min_part = kMx4MinPart;

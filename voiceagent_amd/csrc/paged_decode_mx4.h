@@ -26,7 +26,11 @@
 // ... with no barrier, through a ring of S steps in LDS of its own that DMA
 // fills S - 1 steps ahead.  (Loads to registers made the compiler wait for each
 // at the joins of the branches behind them.)  The waves merge through LDS at
-// the end.
+// the end.  In the four-wave instances at head_dim 128, held to 128 registers so
+// that four workgroups share a CU, the ring does less: the compiler keeps 5-11
+// registers in scratch (not at group 8 with the prologue, where LDS admits
+// three), the lane's scale address among them, and its reload between a step's
+// requests waits for those already in flight.
 #pragma once
 
 #include "mx4.h"
@@ -130,13 +134,13 @@ __global__ __launch_bounds__(W * 64, W == 4 && D <= 128 ? 4 : 2) void paged_deco
   // every 128-byte line: a head's 64 bytes of codes are half of one, its 4 bytes
   // of scales a small part.  There (by_token) the heads of a (sequence,
   // partition) pair u follow one another on XCD u % 8 (32 contexts of 7000 tokens:
-  // 92 -> 67 us; the requests to HBM then equal an HND pool's).
+  // 92 -> 66 us; the requests to HBM then equal an HND pool's).
   //
   // That leaves each line going to two CUs, 2.2 times the requests of an HND
   // pool from L2.  With HP = 2 a workgroup serves two heads, wave w and w + W / 2
   // the same tokens for one head each, through a ring that they share: a request
   // takes 8 whole lines, half of a tile's for both, and a barrier a step says
-  // that the halves are there (67 -> 57 us, against 52 over an HND pool).  Two
+  // that the halves are there (66 -> 59 us, against 53 over an HND pool).  Two
   // heads a workgroup with rings of their own did not help (87: the second
   // request for a line finds it in L2, not in the CU).
   int b = blockIdx.y, h = blockIdx.x, part = blockIdx.z;
