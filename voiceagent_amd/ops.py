@@ -582,13 +582,13 @@ def decode_workspace_bound(device: torch.device, num_heads: int, num_kv_heads: i
     pairs, each holding (m, l) and head_dim floats per query head of the
     group, with the (m, l) block rounded to 256 bytes.  Over an MXFP4 pool at
     head_dim 128 a workgroup may serve two kv heads, and there may be two
-    partitions per compute unit.  ``kv_dtype``: the pool's, or None for any."""
+    partitions per compute unit.  ``kv_dtype``: the pool's (None: not MXFP4)."""
     index = _device_index(device)
     cus = _CUS.get(index)
     if cus is None:
         cus = _CUS[index] = torch.cuda.get_device_properties(index).multi_processor_count
     group = max(1, num_heads // max(1, num_kv_heads))
-    if kv_dtype in (None, MXFP4_KV_DTYPE) and head_dim == 128 and num_kv_heads % 2 == 0:
+    if kv_dtype is MXFP4_KV_DTYPE and head_dim == 128 and num_kv_heads % 2 == 0:
         cus *= 2
     return (cus * group * 2 * 4 + 255) // 256 * 256 + cus * group * head_dim * 4
 
@@ -643,10 +643,12 @@ def reserve_decode_workspace(device: torch.device, num_heads: int, num_kv_heads:
                              kv_dtype: torch.dtype | None = None) -> None:
     """Allocate the decode workspace of `stream` (torch's current stream by
     default) up front, at the size every automatic split needs over a pool of
-    ``kv_dtype`` (None: over any), e.g. before HIP graph capture.  ``torch.cuda.graph`` captures on a stream of its own
-    unless it is given one: pass that stream here to reserve for it."""
+    ``kv_dtype`` (None: over any), e.g. before HIP graph capture.
+    ``torch.cuda.graph`` captures on a stream of its own unless it is given
+    one: pass that stream here to reserve for it."""
     device = torch.device(device)
-    bound = decode_workspace_bound(device, num_heads, num_kv_heads, head_dim, kv_dtype)
+    bound = decode_workspace_bound(device, num_heads, num_kv_heads, head_dim,
+                                   MXFP4_KV_DTYPE if kv_dtype is None else kv_dtype)
     decode_workspace(device, bound, floor=bound, stream=stream)
 
 
