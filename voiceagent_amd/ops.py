@@ -873,13 +873,13 @@ def varlen_attention(
     """
     pool_dtype = None if k_cache is None else k_cache.dtype
     mx4 = pool_dtype is MXFP4_KV_DTYPE
-    if not mx4 and pool_dtype is not FP8_KV_DTYPE:
+    if (not mx4 and pool_dtype is not FP8_KV_DTYPE and
+            not (k_scale.__class__ is float and v_scale.__class__ is float)):
         # A 16-bit pool, or none, has no scales: whatever is given is not read,
         # but an MXFP4 pool's belong to codes.
-        for scale_of in (k_scale, v_scale):
-            _require(scale_of.__class__ is float or
-                     getattr(scale_of, "dtype", None) is not MXFP4_SCALE_DTYPE,
-                     f"float8_e8m0fnu scales need an MXFP4 pool, got {pool_dtype}")
+        _require(MXFP4_SCALE_DTYPE not in (getattr(k_scale, "dtype", None),
+                                           getattr(v_scale, "dtype", None)),
+                 f"float8_e8m0fnu scales need an MXFP4 pool, got {pool_dtype}")
         k_scale = v_scale = 1.0
     fast = _FAST if _FAST_LOADED else _fast_calls()
     if (fast is not None and prologue is None and layout in (LAYOUT_NHD, LAYOUT_HND) and
