@@ -845,11 +845,13 @@ def test_workspaces_of_other_pools_keep_their_size(dev):
     table = torch.arange(128, dtype=torch.int32, device=dev)[None]
     stream = torch.cuda.Stream()
     stream.wait_stream(torch.cuda.current_stream())
-    ops._WORKSPACES.pop((dev.index or 0, stream.cuda_stream), None)
+    key = (dev.index or 0, stream.cuda_stream)
+    if key in ops._WORKSPACES:  # another test's, whose graph may hold it
+        ops._RETIRED.append(ops._WORKSPACES.pop(key))
     with torch.cuda.stream(stream):
         ops.paged_decode(q, kc, vc, table, torch.tensor([2048], device=dev), max_seq_len=2048, scale=0.1)
     torch.cuda.synchronize()
-    assert ops._WORKSPACES[(dev.index or 0, stream.cuda_stream)].numel() == one
+    assert ops._WORKSPACES[key].numel() == one
     assert ops.decode_workspace_bound(dev, 4, 2, 128, BF16) == one
     assert ops.decode_workspace_bound(dev, 4, 2, 128, ops.MXFP4_KV_DTYPE) > one
     for shape in ((4, 2, 64), (6, 3, 128)):
