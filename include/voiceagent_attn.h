@@ -332,6 +332,52 @@ size_t va_varlen_workspace_bytes(const va_varlen_args* args);
  * other sequences.  Depends on the current device's compute-unit count. */
 size_t va_varlen_split_workspace_bytes(const va_varlen_args* args);
 
+/* --------------------------------------------------- varlen, backward */
+/* The gradient of va_varlen_attention without a pool: with P = softmax(scale
+ * q k^T) over the visible keys and delta_i = sum_d dout_i out_i,
+ *   dS_ij = P_ij (dout_i . v_j - delta_i),  dq_i = scale sum_j dS_ij k_j,
+ *   dk_j = scale sum_i dS_ij q_i,  dv_j = sum_i P_ij dout_i,
+ * dk and dv summed over the query heads of their group.  P is recomputed, in
+ * fp32; P and dS are rounded to the element type before the products with
+ * dout, q and k, whose sums are fp32 (f16: both scaled by powers of two first,
+ * so that small gradients do not fall among f16's subnormals).
+ * q, k, v, out and dout are as in the forward call (any group size); rows that
+ * belong to no sequence get a gradient of zeros, as do queries that see no key
+ * and keys that no query sees.  Lengths come from cu_seqlens alone, held to
+ * the rows there are.  No atomics: calls repeat bit for bit.  The gradients
+ * must not overlap the inputs or one another. */
+typedef struct va_varlen_bwd_args {
+  uint32_t struct_size;   /* sizeof(va_varlen_bwd_args)                   */
+  int32_t dtype;          /* VA_BF16 / VA_F16                             */
+  const void* q;          /* [total_q, Hq, D]                             */
+  int64_t q_stride_tok, q_stride_head;
+  const void* k;          /* [total_k, Hkv, D]                            */
+  int64_t k_stride_tok, k_stride_head;
+  const void* v;
+  int64_t v_stride_tok, v_stride_head;
+  const void* out;        /* [total_q, Hq, D], the forward's result       */
+  int64_t out_stride_tok, out_stride_head;
+  const void* dout;       /* [total_q, Hq, D]                             */
+  int64_t dout_stride_tok, dout_stride_head;
+  void* dq;               /* [total_q, Hq, D]                             */
+  int64_t dq_stride_tok, dq_stride_head;
+  void* dk;               /* [total_k, Hkv, D]                            */
+  int64_t dk_stride_tok, dk_stride_head;
+  void* dv;
+  int64_t dv_stride_tok, dv_stride_head;
+  const int32_t* cu_seqlens_q; /* [num_seqs + 1]                          */
+  const int32_t* cu_seqlens_k; /* [num_seqs + 1]                          */
+  int32_t num_seqs, total_q, total_k;
+  int32_t num_heads, num_kv_heads, head_dim; /* head_dim 64 or 128        */
+  int32_t causal;         /* 1: bottom-right aligned causal mask          */
+  float scale;
+  void* workspace;        /* of va_varlen_attention_backward_workspace_bytes */
+  size_t workspace_bytes; /* (written; needs no initialisation)           */
+} va_varlen_bwd_args;
+
+int va_varlen_attention_backward(const va_varlen_bwd_args* args, void* stream);
+size_t va_varlen_attention_backward_workspace_bytes(const va_varlen_bwd_args* args);
+
 /* ----------------------------------------------------------- MXFP4 pools */
 /*
  * A pool of kv_format VA_KV_MXFP4 holds a row of D elements as D / 2 bytes of

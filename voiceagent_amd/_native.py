@@ -193,6 +193,49 @@ class VarlenArgs(ctypes.Structure):
     ]
 
 
+class VarlenBwdArgs(ctypes.Structure):
+    _fields_ = [
+        ("struct_size", c_uint32),
+        ("dtype", c_int32),
+        ("q", c_void_p),
+        ("q_stride_tok", c_int64),
+        ("q_stride_head", c_int64),
+        ("k", c_void_p),
+        ("k_stride_tok", c_int64),
+        ("k_stride_head", c_int64),
+        ("v", c_void_p),
+        ("v_stride_tok", c_int64),
+        ("v_stride_head", c_int64),
+        ("out", c_void_p),
+        ("out_stride_tok", c_int64),
+        ("out_stride_head", c_int64),
+        ("dout", c_void_p),
+        ("dout_stride_tok", c_int64),
+        ("dout_stride_head", c_int64),
+        ("dq", c_void_p),
+        ("dq_stride_tok", c_int64),
+        ("dq_stride_head", c_int64),
+        ("dk", c_void_p),
+        ("dk_stride_tok", c_int64),
+        ("dk_stride_head", c_int64),
+        ("dv", c_void_p),
+        ("dv_stride_tok", c_int64),
+        ("dv_stride_head", c_int64),
+        ("cu_seqlens_q", c_void_p),
+        ("cu_seqlens_k", c_void_p),
+        ("num_seqs", c_int32),
+        ("total_q", c_int32),
+        ("total_k", c_int32),
+        ("num_heads", c_int32),
+        ("num_kv_heads", c_int32),
+        ("head_dim", c_int32),
+        ("causal", c_int32),
+        ("scale", c_float),
+        ("workspace", c_void_p),
+        ("workspace_bytes", c_size_t),
+    ]
+
+
 class Mx4Scales(ctypes.Structure):
     _fields_ = [
         ("struct_size", c_uint32),
@@ -247,6 +290,8 @@ SIGNATURES = {
     "va_varlen_attention": (c_int32, [ctypes.POINTER(VarlenArgs), c_void_p]),
     "va_varlen_workspace_bytes": (c_size_t, [ctypes.POINTER(VarlenArgs)]),
     "va_varlen_split_workspace_bytes": (c_size_t, [ctypes.POINTER(VarlenArgs)]),
+    "va_varlen_attention_backward": (c_int32, [ctypes.POINTER(VarlenBwdArgs), c_void_p]),
+    "va_varlen_attention_backward_workspace_bytes": (c_size_t, [ctypes.POINTER(VarlenBwdArgs)]),
     "va_qk_norm_rope": (c_int32, [ctypes.POINTER(QkNormRopeArgs), c_void_p]),
     "va_store_kvcache_mx4": (c_int32, [ctypes.POINTER(StoreArgs), ctypes.POINTER(Mx4Scales),
                                        c_void_p]),

@@ -1,0 +1,118 @@
+// Host side of the varlen attention's gradient: argument checks, workspace and
+// dispatch (kernels in varlen_backward_kernel.h, instantiated per element type
+// in varlen_backward_{bf16,f16}.hip).
+#include "varlen_backward_kernel.h"
+
+namespace va {
+
+// The first launch's results for the second: lse, delta and, for f16, the
+// rows' largest |dout|.
+static size_t backward_workspace(const va_varlen_bwd_args* a) {
+  const size_t rows = (size_t)a->num_heads * (size_t)a->total_q;
+  return rows * sizeof(float) * (a->dtype == VA_F16 ? 3 : 2);
+}
+
+}  // namespace va
+
+extern "C" size_t va_varlen_attention_backward_workspace_bytes(const va_varlen_bwd_args* a) {
+  if (a == nullptr || a->struct_size != sizeof(va_varlen_bwd_args)) return 0;
+  if (a->num_heads <= 0 || a->total_q <= 0) return 0;
+  return va::backward_workspace(a);
+}
+
+extern "C" int va_varlen_attention_backward(const va_varlen_bwd_args* a, void* stream) {
+  using namespace va;
+  const char* const fn = "va_varlen_attention_backward";
+  VA_CHECK_ARG(a != nullptr, "%s: null args", fn);
+  VA_CHECK_ARG(a->struct_size == sizeof(va_varlen_bwd_args),
+               "%s: struct_size %u != %zu (header/library mismatch)", fn, a->struct_size,
+               sizeof(va_varlen_bwd_args));
+  VA_CHECK_ARG(a->num_seqs >= 0 && a->total_q >= 0 && a->total_k >= 0,
+               "%s: negative num_seqs, total_q or total_k", fn);
+  if (a->total_q == 0 && a->total_k == 0) return VA_OK;
+  VA_CHECK_ARG(a->dtype == VA_BF16 || a->dtype == VA_F16,
+               "%s: dtype must be VA_BF16 or VA_F16 (MFMA path)", fn);
+  VA_CHECK_ARG(a->head_dim == 64 || a->head_dim == 128, "%s: head_dim %d (64 or 128)", fn,
+               a->head_dim);
+  VA_CHECK_ARG(a->num_kv_heads > 0 && a->num_heads > 0 && a->num_heads % a->num_kv_heads == 0,
+               "%s: num_heads (%d) must be a positive multiple of num_kv_heads (%d)", fn,
+               a->num_heads, a->num_kv_heads);
+  VA_CHECK_ARG(a->cu_seqlens_q && a->cu_seqlens_k, "%s: cu_seqlens missing", fn);
+  VA_CHECK_ARG(a->total_q == 0 || (a->q && a->out && a->dout && a->dq),
+               "%s: null pointer argument (query side)", fn);
+  VA_CHECK_ARG(a->total_k == 0 || (a->k && a->v && a->dk && a->dv),
+               "%s: null pointer argument (key side)", fn);
+  const int64_t strides[] = {a->q_stride_tok,    a->q_stride_head,    a->k_stride_tok,
+                             a->k_stride_head,   a->v_stride_tok,     a->v_stride_head,
+                             a->out_stride_tok,  a->out_stride_head,  a->dout_stride_tok,
+                             a->dout_stride_head, a->dq_stride_tok,   a->dq_stride_head,
+                             a->dk_stride_tok,   a->dk_stride_head,   a->dv_stride_tok,
+                             a->dv_stride_head};
+  for (int64_t s : strides)
+    VA_CHECK_ARG(s % 8 == 0, "%s: strides must be 16-byte multiples", fn);
+  const uintptr_t ptrs[] = {(uintptr_t)a->q,    (uintptr_t)a->k,  (uintptr_t)a->v,  (uintptr_t)a->out,
+                            (uintptr_t)a->dout, (uintptr_t)a->dq, (uintptr_t)a->dk, (uintptr_t)a->dv};
+  for (uintptr_t p : ptrs)
+    VA_CHECK_ARG(p % 16 == 0, "%s: pointers must be 16-byte aligned", fn);
+  VA_CHECK_ARG(a->scale > 0.f && a->scale < INFINITY, "%s: scale must be > 0", fn);
+  // A workgroup per block of every sequence; one more, which finds none, writes
+  // the zeros of rows outside the sequences.
+  const int64_t q_tiles = (int64_t)a->total_q / kBwdRows + a->num_seqs + 1;
+  const int64_t k_tiles = (int64_t)a->total_k / kBwdRows + a->num_seqs + 1;
+  VA_CHECK_ARG(q_tiles * a->num_heads <= INT32_MAX && k_tiles * a->num_kv_heads <= INT32_MAX,
+               "%s: too many (sequence, head, block) items", fn);
+  const size_t need = a->total_q > 0 ? backward_workspace(a) : 0;
+  if (need > 0 && (a->workspace == nullptr || a->workspace_bytes < need ||
+                   (uintptr_t)a->workspace % 16 != 0)) {
+    set_error("%s: needs a 16-byte aligned workspace of %zu bytes", fn, need);
+    return VA_ERR_WORKSPACE;
+  }
+
+  VarlenBwdParams p;
+  p.q = (const char*)a->q;
+  p.q_st = a->q_stride_tok * 2;
+  p.q_sh = a->q_stride_head * 2;
+  p.k = (const char*)a->k;
+  p.k_st = a->k_stride_tok * 2;
+  p.k_sh = a->k_stride_head * 2;
+  p.v = (const char*)a->v;
+  p.v_st = a->v_stride_tok * 2;
+  p.v_sh = a->v_stride_head * 2;
+  p.out = (const char*)a->out;
+  p.o_st = a->out_stride_tok * 2;
+  p.o_sh = a->out_stride_head * 2;
+  p.dout = (const char*)a->dout;
+  p.do_st = a->dout_stride_tok * 2;
+  p.do_sh = a->dout_stride_head * 2;
+  p.dq = (char*)a->dq;
+  p.dq_st = a->dq_stride_tok * 2;
+  p.dq_sh = a->dq_stride_head * 2;
+  p.dk = (char*)a->dk;
+  p.dk_st = a->dk_stride_tok * 2;
+  p.dk_sh = a->dk_stride_head * 2;
+  p.dv = (char*)a->dv;
+  p.dv_st = a->dv_stride_tok * 2;
+  p.dv_sh = a->dv_stride_head * 2;
+  p.cu_q = a->cu_seqlens_q;
+  p.cu_k = a->cu_seqlens_k;
+  p.scale = a->scale;
+  p.scale_log2 = a->scale * 1.4426950408889634f;
+  p.causal = a->causal;
+  p.num_seqs = a->num_seqs;
+  p.total_q = a->total_q;
+  p.total_k = a->total_k;
+  p.num_heads = a->num_heads;
+  p.num_kv_heads = a->num_kv_heads;
+  p.q_tiles = (int)q_tiles;
+  p.k_tiles = (int)k_tiles;
+  const size_t rows = (size_t)a->num_heads * (size_t)a->total_q;
+  p.lse = (float*)a->workspace;
+  p.delta = p.lse + rows;
+  p.top = p.delta + rows;
+  const hipStream_t st = (hipStream_t)stream;
+  if (a->dtype == VA_BF16)
+    a->head_dim == 64 ? launch_varlen_backward<true, 64>(p, st) : launch_varlen_backward<true, 128>(p, st);
+  else
+    a->head_dim == 64 ? launch_varlen_backward<false, 64>(p, st) : launch_varlen_backward<false, 128>(p, st);
+  return check_launch(fn);
+}

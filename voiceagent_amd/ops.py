@@ -512,6 +512,7 @@ class _current:
 
 _DECODE_ARGS_SIZE = ctypes.sizeof(N.DecodeArgs)
 _VARLEN_ARGS_SIZE = ctypes.sizeof(N.VarlenArgs)
+_VARLEN_BWD_ARGS_SIZE = ctypes.sizeof(N.VarlenBwdArgs)
 
 # Host fast path (csrc/host/fast_calls.cpp, the ``_fast_calls`` module next
 # to the library): the same checks and the same C-ABI call in C++, for the
@@ -870,7 +871,16 @@ def varlen_attention(
     head_dim 128, a 16-bit pool or none), q holds the raw query projections and
     the launch normalises and rotates them at ``prologue.positions`` (one per
     query token); k and the pool must hold processed keys.
+
+    Without a pool, a prologue or ``out`` the call is differentiable in q, k
+    and v (:func:`varlen_attention_backward`); the others return tensors without
+    a gradient.
     """
+    if (k_cache is None and out is None and prologue is None and k is not None and v is not None
+            and (q.requires_grad or k.requires_grad or v.requires_grad)
+            and torch.is_grad_enabled()):
+        return _VarlenAttention.apply(q, k, v, cu_seqlens_q, cu_seqlens_k, max_seqlen_q,
+                                      max_seqlen_k, scale, causal)
     pool_dtype = None if k_cache is None else k_cache.dtype
     mx4 = pool_dtype is MXFP4_KV_DTYPE
     if (not mx4 and pool_dtype is not FP8_KV_DTYPE and
@@ -991,6 +1001,142 @@ def varlen_attention(
             N.check("va_varlen_attention",
                     lib.va_varlen_attention(ctypes.byref(args), _raw_stream(index)))
     return out
+
+
+# ---------------------------------------------------------- varlen, backward
+def _whole_rows(t: torch.Tensor) -> torch.Tensor:
+    """t, or a copy of it whose rows the kernels can read: 16-byte aligned, the
+    last dimension contiguous (autograd hands on expanded and offset gradients)."""
+    step = 16 // t.element_size()
+    if (t.stride(-1) != 1 or t.data_ptr() % 16 or
+            any(st % step for st, n in zip(t.stride()[:-1], t.shape) if n > 1)):
+        return t.clone(memory_format=torch.contiguous_format)
+    return t
+
+
+def _row_strides(t: torch.Tensor) -> tuple[int, int]:
+    """Strides of tokens and heads; a dimension of one has none to speak of
+    (torch leaves any number there)."""
+    n, h, _ = t.shape
+    return (t.stride(0) if n > 1 else 0), (t.stride(1) if h > 1 else 0)
+
+
+def _apart(new: torch.Tensor, old: torch.Tensor) -> bool:
+    """Whether two tensors' memory, first to last element, does not overlap."""
+    def span(t):
+        reach = [(n - 1) * st * t.element_size() for n, st in zip(t.shape, t.stride())]
+        return (t.data_ptr() + sum(r for r in reach if r < 0),
+                t.data_ptr() + sum(r for r in reach if r > 0) + t.element_size())
+
+    if new.numel() == 0 or old.numel() == 0:
+        return True
+    (a, b), (c, d) = span(new), span(old)
+    return b <= c or d <= a
+
+
+def varlen_attention_backward(
+    dout: torch.Tensor,
+    q: torch.Tensor,
+    k: torch.Tensor,
+    v: torch.Tensor,
+    out: torch.Tensor,
+    cu_seqlens_q: torch.Tensor,
+    cu_seqlens_k: torch.Tensor,
+    max_seqlen_q: int,
+    max_seqlen_k: int,
+    *,
+    scale: float,
+    causal: bool,
+    dq: torch.Tensor | None = None,
+    dk: torch.Tensor | None = None,
+    dv: torch.Tensor | None = None,
+) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """(dq, dk, dv) of :func:`varlen_attention` without a pool, from the output's
+    gradient ``dout`` and the output itself ([total_q, Hq, D]).
+
+    q, k, v, cu_seqlens, scale and causal are those of the forward call (16-bit
+    rows, head_dim 64 or 128; any group size); k and v of ``cu_seqlens_k``'s
+    rows, [total_k, Hkv, D].  The probabilities are recomputed.  Lengths come
+    from the cumulative lengths alone (the maxima are there for the forward
+    call's arguments, and not read).  Rows outside every sequence, queries that
+    see no key and keys that no query sees get zeros.  ``dq``, ``dk``, ``dv``:
+    tensors to write into (views of one buffer, say); they may not overlap the
+    inputs.  Two launches on the current stream, no atomics: the results repeat
+    bit for bit."""
+    device = _check_gpu(dout, q, k, v, out, cu_seqlens_q, cu_seqlens_k, dq, dk, dv)
+    _require(q.dim() == 3, "q must be [total_q, num_heads, head_dim]")
+    _require(out.shape == q.shape and dout.shape == q.shape, "out and dout must match q")
+    _require(k.dim() == 3 and v.shape == k.shape and k.shape[2] == q.shape[2],
+             "k/v must be [total_k, num_kv_heads, head_dim]")
+    _require(q.dtype == k.dtype == v.dtype == out.dtype == dout.dtype,
+             "dout/q/k/v/out dtypes must match")
+    _require(q.dtype in (torch.bfloat16, torch.float16), "varlen attention needs 16-bit rows")
+    total_q, hq, d = q.shape
+    total_k, hkv, _ = k.shape
+    _require(hkv > 0 and hq % hkv == 0 and hq > 0, "num_heads must be a multiple of num_kv_heads")
+    _require(cu_seqlens_q.dtype == torch.int32 and cu_seqlens_k.dtype == torch.int32,
+             "cu_seqlens must be int32")
+    _require(cu_seqlens_q.dim() == 1 and cu_seqlens_q.numel() >= 2 and
+             cu_seqlens_k.shape == cu_seqlens_q.shape, "cu_seqlens must be [num_seqs + 1]")
+    _require(cu_seqlens_q.is_contiguous() and cu_seqlens_k.is_contiguous(),
+             "cu_seqlens must be contiguous")
+    given = []
+    for name, t, like in (("dq", dq, q), ("dk", dk, k), ("dv", dv, v)):
+        if t is not None:
+            _require(t.shape == like.shape and t.dtype == like.dtype, f"{name} must match {name[1]}")
+            given.append((name, t))
+    for name, t in given:
+        _require(all(_apart(t, x) for x in (dout, q, k, v, out)),
+                 f"{name} may not overlap the inputs")
+    dq = torch.empty(q.shape, dtype=q.dtype, device=device) if dq is None else dq
+    dk = torch.empty(k.shape, dtype=k.dtype, device=device) if dk is None else dk
+    dv = torch.empty(k.shape, dtype=k.dtype, device=device) if dv is None else dv
+    args = N.VarlenBwdArgs(
+        struct_size=_VARLEN_BWD_ARGS_SIZE, dtype=_dtype_code(q),
+        cu_seqlens_q=cu_seqlens_q.data_ptr(), cu_seqlens_k=cu_seqlens_k.data_ptr(),
+        num_seqs=cu_seqlens_q.numel() - 1, total_q=total_q, total_k=total_k, num_heads=hq,
+        num_kv_heads=hkv, head_dim=d, causal=1 if causal else 0, scale=float(scale))
+    for name, t in (("q", q), ("k", k), ("v", v), ("out", out), ("dout", dout), ("dq", dq),
+                    ("dk", dk), ("dv", dv)):
+        _require(t.stride(2) == 1, f"{name}: the last dimension must be contiguous")
+        tok, head = _row_strides(t)
+        setattr(args, name, t.data_ptr())
+        setattr(args, name + "_stride_tok", tok)
+        setattr(args, name + "_stride_head", head)
+    lib = N.lib()
+    index = _device_index(device)
+    with _current(index):
+        # Two or three floats a query row, for this call alone: torch's allocator
+        # hands them out again in the order of this stream (or captured graph).
+        nbytes = lib.va_varlen_attention_backward_workspace_bytes(ctypes.byref(args))
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
+        args.workspace = ws.data_ptr()
+        args.workspace_bytes = nbytes
+        N.check("va_varlen_attention_backward",
+                lib.va_varlen_attention_backward(ctypes.byref(args), _raw_stream(index)))
+    return dq, dk, dv
+
+
+class _VarlenAttention(torch.autograd.Function):
+    """varlen_attention without a pool, with its gradient."""
+
+    @staticmethod
+    def forward(ctx, q, k, v, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, max_seqlen_k, scale, causal):
+        out = varlen_attention(q, k, v, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, max_seqlen_k,
+                               scale=scale, causal=causal)
+        ctx.save_for_backward(q, k, v, out, cu_seqlens_q, cu_seqlens_k)
+        ctx.call = (max_seqlen_q, max_seqlen_k, scale, causal)
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dout):
+        q, k, v, out, cu_q, cu_k = ctx.saved_tensors
+        max_q, max_k, scale, causal = ctx.call
+        grads = varlen_attention_backward(_whole_rows(dout), q, k, v, out, cu_q, cu_k, max_q, max_k,
+                                          scale=scale, causal=causal)
+        wanted = (g if need else None for g, need in zip(grads, ctx.needs_input_grad))
+        return (*wanted, None, None, None, None, None, None)
 
 
 # ------------------------------------------------------------- step metadata
