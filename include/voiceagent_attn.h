@@ -159,6 +159,70 @@ typedef struct va_qk_norm_rope_args {
  * fused decode path does not take). */
 int va_qk_norm_rope(const va_qk_norm_rope_args* args, void* stream);
 
+/* ---------------------------------------------------- q/k prologue, backward */
+/* The gradient of va_qk_norm_rope.  With r = 1/sqrt(mean(x^2) + eps), n = x r,
+ * y = n weight and z the rotation of y, from dz: dy is the transposed rotation
+ * of dz, dweight = sum over tokens and heads of dy n,
+ *   dx = r (dy weight - n mean(dy weight n)).
+ * All in fp32, rounded once at the end; the forward's roundings to the element
+ * type count as the identity.  No atomics: calls repeat bit for bit.  dq and dk
+ * may be dq_out and dk_out or q and k themselves. */
+typedef struct va_qk_norm_rope_bwd_args {
+  uint32_t struct_size;   /* sizeof(va_qk_norm_rope_bwd_args)             */
+  int32_t dtype;          /* VA_BF16 / VA_F16 / VA_F32, all rows          */
+  const void* dq_out;     /* [num_tokens, Hq, D] gradient of q_out        */
+  int64_t dq_out_stride_tok, dq_out_stride_head;
+  const void* dk_out;     /* [num_tokens, Hkv, D] gradient of k_out       */
+  int64_t dk_out_stride_tok, dk_out_stride_head;
+  const void* q;          /* the forward's inputs                         */
+  int64_t q_stride_tok, q_stride_head;
+  const void* k;
+  int64_t k_stride_tok, k_stride_head;
+  void* dq;               /* [num_tokens, Hq, D]                          */
+  int64_t dq_stride_tok, dq_stride_head;
+  void* dk;               /* [num_tokens, Hkv, D]                         */
+  int64_t dk_stride_tok, dk_stride_head;
+  void* dq_weight;        /* [D] in the prologue's weight_dtype           */
+  void* dk_weight;
+  int32_t num_tokens, num_heads, num_kv_heads, head_dim; /* heads of a side may be 0 */
+  va_qk_prologue prologue;
+  void* workspace;        /* of va_qk_norm_rope_backward_workspace_bytes  */
+  size_t workspace_bytes; /* (written; needs no initialisation)           */
+} va_qk_norm_rope_bwd_args;
+
+int va_qk_norm_rope_backward(const va_qk_norm_rope_bwd_args* args, void* stream);
+size_t va_qk_norm_rope_backward_workspace_bytes(const va_qk_norm_rope_bwd_args* args);
+
+/* -------------------------------------------------------------- rotary */
+/* Rotary positions alone, in every form: of each head's first rotary_dim
+ * elements, pairs (2 i, 2 i + 1) (interleaved) or (i, i + rotary_dim / 2) turn,
+ *   a' = a cos[i] - b sin[i],  b' = b cos[i] + a sin[i]
+ * with the table's row [cos | sin] at the token's position; the others are
+ * copied.  inverse negates the sines: the transposed rotation, which is its
+ * gradient.  fp32, rounded once.  A scaled table (longer contexts) may carry a
+ * factor in its entries. */
+typedef struct va_rotary_args {
+  uint32_t struct_size;   /* sizeof(va_rotary_args)                       */
+  int32_t dtype;          /* VA_BF16 / VA_F16 / VA_F32                    */
+  const void* q;          /* [num_tokens, Hq, D]                          */
+  int64_t q_stride_tok, q_stride_head;
+  const void* k;          /* [num_tokens, Hkv, D]                         */
+  int64_t k_stride_tok, k_stride_head;
+  void* q_out;            /* may be q itself, k_out k itself (in place)   */
+  int64_t q_out_stride_tok, q_out_stride_head;
+  void* k_out;
+  int64_t k_out_stride_tok, k_out_stride_head;
+  int32_t num_tokens, num_heads, num_kv_heads, head_dim; /* heads of a side may be 0 */
+  int32_t rotary_dim, interleaved, inverse;
+  const float* cos_sin_cache; /* [max_position, rotary_dim]: cos | sin halves */
+  int64_t cos_sin_stride;
+  int32_t max_position;   /* positions are clamped to [0, max_position)   */
+  int32_t positions_dtype;
+  const void* positions;  /* [num_tokens]                                 */
+} va_rotary_args;
+
+int va_rotary(const va_rotary_args* args, void* stream);
+
 /* --------------------------------------------------------------- decode */
 typedef struct va_decode_args {
   uint32_t struct_size;   /* sizeof(va_decode_args)                       */

@@ -130,3 +130,122 @@ def test_overlap_is_seen():
     assert not ops._apart(x[:, :2], x[:, 2:])  # views of one buffer's rows: within one another
     assert ops._apart(x[:2], x[2:]) and not ops._apart(x[:3], x[2:])
     assert ops._apart(x[:0], x) and ops._apart(torch.zeros(3), x)
+
+
+def _rotary_args(**over):
+    a = N.new_args(N.RotaryArgs)
+    for name in ("q", "k", "q_out", "k_out", "cos_sin_cache", "positions"):
+        setattr(a, name, 1 << 20)  # never dereferenced
+    a.num_tokens, a.num_heads, a.num_kv_heads, a.head_dim, a.rotary_dim = 4, 2, 2, 64, 32
+    a.cos_sin_stride, a.max_position = 32, 10
+    for name, x in over.items():
+        setattr(a, name, x)
+    return a
+
+
+@pytest.mark.parametrize("over,says", [
+    (dict(num_tokens=-1), "num_tokens"), (dict(dtype=9), "dtype"), (dict(num_heads=0, num_kv_heads=0), "heads"),
+    (dict(num_heads=-1), "heads"), (dict(rotary_dim=31), "rotary_dim"), (dict(rotary_dim=66), "rotary_dim"),
+    (dict(rotary_dim=0), "rotary_dim"), (dict(q=None), "missing"), (dict(k_out=None), "missing"),
+    (dict(positions=None), "positions"), (dict(cos_sin_stride=31), "rotary cache"),
+    (dict(max_position=0), "rotary cache"), (dict(positions_dtype=2), "positions_dtype"),
+    (dict(q=(1 << 20) + 1), "aligned"), (dict(num_tokens=2 ** 31 - 1), "too many"),
+])
+def test_c_abi_refuses_bad_rotations(over, says):
+    assert N.lib().va_rotary(ctypes.byref(_rotary_args(**over)), None) == -1
+    assert says in N.last_error()
+
+
+def test_rotation_of_no_tokens_is_no_call():
+    a = _rotary_args(num_tokens=0)
+    assert N.lib().va_rotary(ctypes.byref(a), None) == 0
+    a.struct_size += 4
+    assert N.lib().va_rotary(ctypes.byref(a), None) == -1 and "struct_size" in N.last_error()
+
+
+def _prologue_args(**over):
+    a = N.new_args(N.QkNormRopeBwdArgs)
+    for name in ("dq_out", "dk_out", "q", "k", "dq", "dk", "dq_weight", "dk_weight", "workspace"):
+        setattr(a, name, 1 << 20)
+    a.num_tokens, a.num_heads, a.num_kv_heads, a.head_dim = 4, 2, 2, 64
+    pro = a.prologue
+    for name in ("q_norm_weight", "k_norm_weight", "cos_sin_cache", "positions"):
+        setattr(pro, name, 1 << 20)
+    pro.cos_sin_stride, pro.max_position = 64, 10
+    a.workspace_bytes = 1 << 30
+    for name, x in over.items():
+        setattr(pro if hasattr(pro, name) else a, name, x)
+    return a
+
+
+@pytest.mark.parametrize("over,says", [
+    (dict(dtype=7), "dtype"), (dict(num_tokens=-1), "num_tokens"), (dict(head_dim=96), "head_dim"),
+    (dict(num_heads=0, num_kv_heads=0), "head"), (dict(num_heads=70000), "head"), (dict(q=None), "query side"),
+    (dict(dk_weight=None), "key side"), (dict(cos_sin_stride=63), "rotary cache"),
+    (dict(q_norm_weight=None), "norm weights"), (dict(weight_dtype=5), "weight_dtype"),
+    (dict(positions_dtype=-1), "positions_dtype"), (dict(dk_stride_tok=4), "strides"),
+    (dict(dq=(1 << 20) + 4), "aligned"), (dict(workspace=None), "workspace"), (dict(workspace_bytes=8), "workspace"),
+])
+def test_c_abi_refuses_bad_prologue_gradients(over, says):
+    assert N.lib().va_qk_norm_rope_backward(ctypes.byref(_prologue_args(**over)), None) < 0
+    assert says in N.last_error()
+
+
+def test_prologue_gradient_workspace():
+    size = N.lib().va_qk_norm_rope_backward_workspace_bytes
+    assert size(ctypes.byref(_prologue_args(num_tokens=0))) == 0
+    assert size(ctypes.byref(_prologue_args(head_dim=96))) == 0
+    assert size(ctypes.byref(_prologue_args())) == 2 * 64 * 4  # one workgroup's sums
+    most = size(ctypes.byref(_prologue_args(num_tokens=1 << 20)))
+    assert most == 1024 * 2 * 64 * 4
+
+
+def test_cpu_tensors_of_the_prologue_and_the_rotation_are_refused():
+    x = torch.zeros(4, 2, 64)
+    pos, table, w = torch.zeros(4, dtype=torch.int64), torch.zeros(9, 64), torch.ones(64)
+    with pytest.raises(ops.AttentionArgumentError, match="GPU"):
+        ops.rotary_embedding(x, x, table, pos)
+    with pytest.raises(ops.AttentionArgumentError, match="GPU"):
+        ops.qk_norm_rope_backward(x, x, x, x, ops.QKPrologue(w, w, 1e-6, table, pos))
+
+
+# -------------------------------------------------------------------------------- the tables
+def test_rotary_tables():
+    import math
+
+    from oracle import attention as oracle
+    from voiceagent_amd.layers import RotaryScaling, rotary_cos_sin_cache as table
+
+    # As before without a part or a scaling; in float64 angles with one.
+    assert torch.equal(table(64, 100, 1e4), oracle.rope_cache(64, 100, 1e4))
+    part = table(128, 100, 1e4, rotary_dim=64)
+    assert part.shape == (100, 64) and (part - table(64, 100, 1e4)).abs().max() < 1e-4
+    i, p = 5, 77
+    angle = p * 1e4 ** (-2 * i / 64)
+    assert abs(part[p, i] - math.cos(angle)) < 1e-7 and abs(part[p, 32 + i] - math.sin(angle)) < 1e-7
+    # Linear: a position's angles are those of position / factor.
+    linear = table(64, 100, 1e4, scaling=RotaryScaling("linear", 4.0))
+    assert torch.equal(linear[::4], table(64, 25, 1e4, rotary_dim=64))
+    # By the base: the fastest pair as it was, the slowest slower by the factor.
+    base = table(64, 100, 1e4, scaling=RotaryScaling("base", 8.0))
+    assert torch.equal(base[:, 0], part[:, 0])
+    slow = 1e4 ** (-62 / 64) / 8
+    assert abs(base[90, 31] - math.cos(90 * slow)) < 1e-7
+    # By parts: pairs that turn often as they were, those that hardly turn slower, times a factor.
+    yarn = table(64, 100, 1e4, scaling=RotaryScaling("yarn", 8.0, original_max_position=4096))
+    factor = 0.1 * math.log(8.0) + 1
+    assert abs(yarn[50, 0] - math.cos(50.0) * factor) < 1e-6
+    assert abs(yarn[50, 63] - math.sin(50 * 1e4 ** (-62 / 64) / 8) * factor) < 1e-6
+    low = math.floor(64 * math.log(4096 / (64 * math.pi)) / (2 * math.log(1e4)))
+    high = math.ceil(64 * math.log(4096 / (2 * math.pi)) / (2 * math.log(1e4)))
+    j = (low + high) // 2
+    ramp = (j - low) / (high - low)
+    freq = 1e4 ** (-2 * j / 64) * (1 - ramp + ramp / 8)
+    assert abs(yarn[99, j] - math.cos(99 * freq) * factor) < 1e-6
+    plain = table(64, 100, 1e4, scaling=RotaryScaling("yarn", 8.0, 4096, attention_factor=1.0))
+    assert (plain * factor - yarn).abs().max() < 1e-6
+    for bad in (dict(scaling=RotaryScaling("other", 2.0)), dict(scaling=RotaryScaling("linear", 0.5)),
+                dict(scaling=RotaryScaling("yarn", 2.0)), dict(rotary_dim=63), dict(rotary_dim=66),
+                dict(rotary_dim=2, scaling=RotaryScaling("base", 2.0))):
+        with pytest.raises(ValueError):
+            table(64, 10, 1e4, **bad)

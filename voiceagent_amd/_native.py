@@ -109,6 +109,71 @@ class QkNormRopeArgs(ctypes.Structure):
     ]
 
 
+class QkNormRopeBwdArgs(ctypes.Structure):
+    _fields_ = [
+        ("struct_size", c_uint32),
+        ("dtype", c_int32),
+        ("dq_out", c_void_p),
+        ("dq_out_stride_tok", c_int64),
+        ("dq_out_stride_head", c_int64),
+        ("dk_out", c_void_p),
+        ("dk_out_stride_tok", c_int64),
+        ("dk_out_stride_head", c_int64),
+        ("q", c_void_p),
+        ("q_stride_tok", c_int64),
+        ("q_stride_head", c_int64),
+        ("k", c_void_p),
+        ("k_stride_tok", c_int64),
+        ("k_stride_head", c_int64),
+        ("dq", c_void_p),
+        ("dq_stride_tok", c_int64),
+        ("dq_stride_head", c_int64),
+        ("dk", c_void_p),
+        ("dk_stride_tok", c_int64),
+        ("dk_stride_head", c_int64),
+        ("dq_weight", c_void_p),
+        ("dk_weight", c_void_p),
+        ("num_tokens", c_int32),
+        ("num_heads", c_int32),
+        ("num_kv_heads", c_int32),
+        ("head_dim", c_int32),
+        ("prologue", QkPrologue),
+        ("workspace", c_void_p),
+        ("workspace_bytes", c_size_t),
+    ]
+
+
+class RotaryArgs(ctypes.Structure):
+    _fields_ = [
+        ("struct_size", c_uint32),
+        ("dtype", c_int32),
+        ("q", c_void_p),
+        ("q_stride_tok", c_int64),
+        ("q_stride_head", c_int64),
+        ("k", c_void_p),
+        ("k_stride_tok", c_int64),
+        ("k_stride_head", c_int64),
+        ("q_out", c_void_p),
+        ("q_out_stride_tok", c_int64),
+        ("q_out_stride_head", c_int64),
+        ("k_out", c_void_p),
+        ("k_out_stride_tok", c_int64),
+        ("k_out_stride_head", c_int64),
+        ("num_tokens", c_int32),
+        ("num_heads", c_int32),
+        ("num_kv_heads", c_int32),
+        ("head_dim", c_int32),
+        ("rotary_dim", c_int32),
+        ("interleaved", c_int32),
+        ("inverse", c_int32),
+        ("cos_sin_cache", c_void_p),
+        ("cos_sin_stride", c_int64),
+        ("max_position", c_int32),
+        ("positions_dtype", c_int32),
+        ("positions", c_void_p),
+    ]
+
+
 class DecodeArgs(ctypes.Structure):
     _fields_ = [
         ("struct_size", c_uint32),
@@ -293,6 +358,9 @@ SIGNATURES = {
     "va_varlen_attention_backward": (c_int32, [ctypes.POINTER(VarlenBwdArgs), c_void_p]),
     "va_varlen_attention_backward_workspace_bytes": (c_size_t, [ctypes.POINTER(VarlenBwdArgs)]),
     "va_qk_norm_rope": (c_int32, [ctypes.POINTER(QkNormRopeArgs), c_void_p]),
+    "va_qk_norm_rope_backward": (c_int32, [ctypes.POINTER(QkNormRopeBwdArgs), c_void_p]),
+    "va_qk_norm_rope_backward_workspace_bytes": (c_size_t, [ctypes.POINTER(QkNormRopeBwdArgs)]),
+    "va_rotary": (c_int32, [ctypes.POINTER(RotaryArgs), c_void_p]),
     "va_store_kvcache_mx4": (c_int32, [ctypes.POINTER(StoreArgs), ctypes.POINTER(Mx4Scales),
                                        c_void_p]),
     "va_load_kvcache_mx4": (c_int32, [ctypes.POINTER(LoadArgs), ctypes.POINTER(Mx4Scales),

@@ -5,12 +5,13 @@ from voiceagent_amd.layers.context import (
     get_attention_context,
     set_attention_context,
 )
-from voiceagent_amd.layers.qwen3 import Qwen3AttentionCore, rotary_cos_sin_cache
+from voiceagent_amd.layers.qwen3 import Qwen3AttentionCore, RotaryScaling, rotary_cos_sin_cache
 
 __all__ = [
     "AttentionContext",
     "PagedAttention",
     "Qwen3AttentionCore",
+    "RotaryScaling",
     "VarlenSelfAttention",
     "attention_context",
     "get_attention_context",

@@ -32,7 +32,14 @@ other batch runs ``ops.qk_norm_rope`` over both first.  (With
 none, runs it over the keys alone and lets the varlen launch normalise and
 rotate the queries.)
 Qwen3Attention then passes the prologue instead of calling q_norm, k_norm and
-rotary_emb itself.
+rotary_emb itself.  A :class:`voiceagent_amd.ops.Rotary` in its place rotates q
+and k alone (pairs interleaved or halves, a part of the head), in a launch of
+its own.
+
+Without a cache (a training pass over packed sequences, as the memory-profiling
+pass is) the attention, the prologue and the rotation are differentiable in q,
+k, v and the norm weights; with a bound cache nothing has a gradient.
+:class:`VarlenSelfAttention` is differentiable too.
 
 ``kv_layout`` names the pool layout: ``"nhd"`` ``[num_blocks, block_size,
 Hkv, D]`` as model_runner.py:116-131 allocates it (the default), or
@@ -123,19 +130,25 @@ class PagedAttention(nn.Module):
         self.v_cache = torch.tensor([])
 
     def forward(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
-                prologue: ops.QKPrologue | None = None) -> torch.Tensor:
+                prologue: ops.QKPrologue | ops.Rotary | None = None) -> torch.Tensor:
         context = get_attention_context()
         num_seqs = context.cu_seqlens_k.numel() - 1
         decode = context.max_seqlen_q == 1 and q.shape[0] == num_seqs
         q_pro = None  # the prologue the varlen launch applies to q itself
         if prologue is not None:
-            if self.k_cache.numel() and decode and self.fuse_store:
+            if (self.k_cache.numel() and decode and self.fuse_store and
+                    not isinstance(prologue, ops.Rotary)):
                 return self._decode_fused(q, k, v, context, prologue)
-            if not decode and self._varlen_takes_prologue(q):
-                _, k = ops.qk_norm_rope(None, k, prologue)
-                q_pro = prologue
-            else:
-                q, k = ops.qk_norm_rope(q, k, prologue)
+            # (Over a cache nothing has a gradient, whatever the weights ask for.)
+            with torch.set_grad_enabled(torch.is_grad_enabled() and not self.k_cache.numel()):
+                if isinstance(prologue, ops.Rotary):
+                    q, k = ops.rotary_embedding(q, k, prologue.cos_sin_cache, prologue.positions,
+                                                interleaved=prologue.interleaved)
+                elif not decode and self._varlen_takes_prologue(q, k, prologue):
+                    _, k = ops.qk_norm_rope(None, k, prologue)
+                    q_pro = prologue
+                else:
+                    q, k = ops.qk_norm_rope(q, k, prologue)
         if not self.k_cache.numel():
             # Memory-profiling pass before the cache exists: packed causal varlen.
             return ops.varlen_attention(
@@ -208,12 +221,18 @@ class PagedAttention(nn.Module):
             prologue=q_pro,
         )
 
-    def _varlen_takes_prologue(self, q: torch.Tensor) -> bool:
+    def _varlen_takes_prologue(self, q: torch.Tensor, k: torch.Tensor,
+                               prologue: ops.QKPrologue) -> bool:
         """Whether the varlen launch can apply the query prologue itself:
-        head_dim 128, 16-bit q, and a 16-bit pool or none."""
+        head_dim 128, 16-bit q, a 16-bit pool or none, and nothing that asks for
+        a gradient (called in the grad mode that the prologue runs in)."""
         return (self.varlen_fuse_prologue and q.shape[-1] == 128 and
                 q.dtype in (torch.bfloat16, torch.float16) and
-                (not self.k_cache.numel() or self.k_cache.dtype == q.dtype))
+                (not self.k_cache.numel() or self.k_cache.dtype == q.dtype) and
+                not (torch.is_grad_enabled() and
+                     (q.requires_grad or k.requires_grad or
+                      prologue.q_norm_weight.requires_grad or
+                      prologue.k_norm_weight.requires_grad)))
 
     def _decode_fused(self, q, k, v, context, prologue: ops.QKPrologue | None) -> torch.Tensor:
         """One launch: (prologue,) store of the new rows, paged decode."""

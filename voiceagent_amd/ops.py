@@ -395,7 +395,15 @@ def qk_norm_rope(
     position per token).  Outputs are allocated contiguous when not given and
     may be q / k themselves (in place).  ``q`` None: the keys alone (a
     prefill whose varlen launch applies the query prologue itself); the
-    first result is then None."""
+    first result is then None.  Without outputs the call is differentiable in q,
+    k and the norm weights (:func:`qk_norm_rope_backward`)."""
+    if q_out is None and k_out is None and torch.is_grad_enabled():
+        qw, kw = prologue.q_norm_weight, prologue.k_norm_weight
+        if q is None:
+            if k.requires_grad or kw.requires_grad:
+                return None, _KNormRope.apply(k, kw, prologue)
+        elif q.requires_grad or k.requires_grad or qw.requires_grad or kw.requires_grad:
+            return _QkNormRope.apply(q, k, qw, kw, prologue)
     if q is None:
         return None, _k_norm_rope(k, prologue, k_out)
     fast = _FAST if _FAST_LOADED else _fast_calls()
@@ -466,6 +474,207 @@ def _k_norm_rope(k: torch.Tensor, prologue: QKPrologue,
     args.prologue = _prologue_struct(prologue, d, T)
     N.call("va_qk_norm_rope", args, device)
     return k_out
+
+
+def qk_norm_rope_backward(
+    dq_out: torch.Tensor | None,
+    dk_out: torch.Tensor,
+    q: torch.Tensor | None,
+    k: torch.Tensor,
+    prologue: QKPrologue,
+    *,
+    dq: torch.Tensor | None = None,
+    dk: torch.Tensor | None = None,
+) -> tuple[torch.Tensor | None, torch.Tensor, torch.Tensor | None, torch.Tensor]:
+    """(dq, dk, dq_norm_weight, dk_norm_weight) of :func:`qk_norm_rope`, from the
+    gradients of its outputs and its inputs q [T, Hq, D], k [T, Hkv, D]; the
+    weights' sum over all tokens and heads.  fp32, rounded once: the forward's
+    roundings to the element type count as the identity.  ``dq`` / ``dk`` may be
+    dq_out / dk_out or q / k themselves.  ``dq_out`` and ``q`` None: the keys
+    alone (dq and dq_norm_weight are then None).  Two launches, no atomics."""
+    _require((q is None) == (dq_out is None), "q and dq_out must be given together")
+    device = _check_gpu(dq_out, dk_out, q, k, dq, dk, prologue.q_norm_weight,
+                        prologue.k_norm_weight, prologue.cos_sin_cache, prologue.positions)
+    sides = [("k", dk_out, k, dk)] if q is None else [("q", dq_out, q, dq), ("k", dk_out, k, dk)]
+    _require(k.dim() == 3, "k must be [T, Hkv, D]")
+    T, hkv, d = (int(x) for x in k.shape)
+    args = N.new_args(N.QkNormRopeBwdArgs)
+    args.dtype = _dtype_code(k)
+    args.num_tokens, args.num_kv_heads, args.head_dim = T, hkv, d
+    results = {"q": None, "k": None, "qw": None, "kw": None}
+    for name, dz, x, dx in sides:
+        _require(x.dim() == 3 and x.shape[0] == T and x.shape[2] == d and x.dtype == k.dtype,
+                 "q must be [T, Hq, D] and k [T, Hkv, D] of one dtype")
+        _require(dz.shape == x.shape and dz.dtype == x.dtype, f"d{name}_out must match {name}")
+        if dx is None:
+            dx = torch.empty(x.shape, dtype=x.dtype, device=device)
+        _require(dx.shape == x.shape and dx.dtype == x.dtype, f"d{name} must match {name}")
+        for field, t in ((f"d{name}_out", dz), (name, x), (f"d{name}", dx)):
+            _rows(t, field)
+            tok, head = _row_strides(t)
+            setattr(args, field, t.data_ptr())
+            setattr(args, field + "_stride_tok", tok)
+            setattr(args, field + "_stride_head", head)
+        weight = prologue.q_norm_weight if name == "q" else prologue.k_norm_weight
+        results[name], results[name + "w"] = dx, torch.empty(d, dtype=weight.dtype, device=device)
+        setattr(args, f"d{name}_weight", results[name + "w"].data_ptr())
+    args.num_heads = 0 if q is None else int(q.shape[1])
+    args.prologue = _prologue_struct(prologue, d, T)
+    lib = N.lib()
+    index = _device_index(device)
+    with _current(index):
+        nbytes = lib.va_qk_norm_rope_backward_workspace_bytes(ctypes.byref(args))
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=device)  # this call's alone
+        args.workspace = ws.data_ptr()
+        args.workspace_bytes = nbytes
+        N.check("va_qk_norm_rope_backward",
+                lib.va_qk_norm_rope_backward(ctypes.byref(args), _raw_stream(index)))
+    return results["q"], results["k"], results["qw"], results["kw"]
+
+
+class _QkNormRope(torch.autograd.Function):
+    """qk_norm_rope with its gradient."""
+
+    @staticmethod
+    def forward(ctx, q, k, q_norm_weight, k_norm_weight, prologue):
+        ctx.save_for_backward(q, k, q_norm_weight, k_norm_weight, prologue.cos_sin_cache,
+                              prologue.positions)
+        ctx.eps = prologue.eps
+        return qk_norm_rope(q, k, prologue)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dq_out, dk_out):
+        q, k, qw, kw, cos_sin, positions = ctx.saved_tensors
+        grads = qk_norm_rope_backward(_whole_rows(dq_out), _whole_rows(dk_out), q, k,
+                                      QKPrologue(qw, kw, ctx.eps, cos_sin, positions))
+        return (*(g if need else None for g, need in zip(grads, ctx.needs_input_grad)), None)
+
+
+class _KNormRope(torch.autograd.Function):
+    """The key side of qk_norm_rope alone, with its gradient."""
+
+    @staticmethod
+    def forward(ctx, k, k_norm_weight, prologue):
+        ctx.save_for_backward(k, prologue.q_norm_weight, k_norm_weight, prologue.cos_sin_cache,
+                              prologue.positions)
+        ctx.eps = prologue.eps
+        return _k_norm_rope(k, prologue, None)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dk_out):
+        k, qw, kw, cos_sin, positions = ctx.saved_tensors
+        _, dk, _, dkw = qk_norm_rope_backward(None, _whole_rows(dk_out), None, k,
+                                              QKPrologue(qw, kw, ctx.eps, cos_sin, positions))
+        return (*(g if need else None for g, need in zip((dk, dkw), ctx.needs_input_grad)), None)
+
+
+# -------------------------------------------------------------------- rotary
+@dataclass(frozen=True)
+class Rotary:
+    """Rotary positions without a norm, for attention layers' ``prologue``: see
+    :func:`rotary_embedding`."""
+
+    cos_sin_cache: torch.Tensor
+    positions: torch.Tensor
+    interleaved: bool = False
+
+
+def rotary_embedding(
+    q: torch.Tensor | None,
+    k: torch.Tensor | None,
+    cos_sin_cache: torch.Tensor,
+    positions: torch.Tensor,
+    *,
+    interleaved: bool = False,
+    inverse: bool = False,
+    q_out: torch.Tensor | None = None,
+    k_out: torch.Tensor | None = None,
+) -> tuple[torch.Tensor | None, torch.Tensor | None]:
+    """Rotate the first r elements of every head of q [T, Hq, D] and k [T, Hkv, D]
+    (either may be None) at the tokens' positions.  ``cos_sin_cache`` is an fp32
+    [max_position, (1,) r] table, cosines | sines, r even and at most D
+    (:func:`voiceagent_amd.layers.rotary_cos_sin_cache` makes one, scaled or
+    not); pairs are elements (i, i + r/2), or (2 i, 2 i + 1) when
+    ``interleaved``.  Elements from r on are copied.  ``inverse``: the
+    transposed rotation, the gradient of the other.  fp32, rounded once (16-bit
+    or fp32 rows, any head_dim and strides; rows of 16-byte multiples go 16
+    bytes at a time).  Positions are held to the table.  Outputs may be q / k
+    themselves; without outputs the call is differentiable in q and k."""
+    if (q_out is None and k_out is None and torch.is_grad_enabled() and
+            ((q is not None and q.requires_grad) or (k is not None and k.requires_grad))):
+        return _Rotary.apply(q, k, cos_sin_cache, positions, interleaved, inverse)
+    device = _check_gpu(q, k, cos_sin_cache, positions, q_out, k_out)
+    _require(q is not None or k is not None, "q or k must be given")
+    like = k if q is None else q
+    _require(like.dim() == 3, "q and k must be [T, heads, D]")
+    T, _, d = (int(x) for x in like.shape)
+    args = N.new_args(N.RotaryArgs)
+    args.dtype = _dtype_code(like)
+    args.num_tokens, args.head_dim = T, d
+    outs = []
+    for name, x, y in (("q", q, q_out), ("k", k, k_out)):
+        if x is None:
+            _require(y is None, f"{name}_out without {name}")
+            outs.append(None)
+            continue
+        _require(x.dim() == 3 and x.shape[0] == T and x.shape[2] == d and x.dtype == like.dtype,
+                 "q must be [T, Hq, D] and k [T, Hkv, D] of one dtype")
+        if y is None:
+            y = torch.empty(x.shape, dtype=x.dtype, device=device)
+        _require(y.shape == x.shape and y.dtype == x.dtype, f"{name}_out must match {name}")
+        for field, t in ((name, x), (name + "_out", y)):
+            _require(t.stride(2) == 1 or d == 1, f"{field}: the last dimension must be contiguous")
+            tok, head = _row_strides(t)
+            setattr(args, field, t.data_ptr())
+            setattr(args, field + "_stride_tok", tok)
+            setattr(args, field + "_stride_head", head)
+        outs.append(y)
+    args.num_heads = 0 if q is None else int(q.shape[1])
+    args.num_kv_heads = 0 if k is None else int(k.shape[1])
+    cs = cos_sin_cache
+    if cs.dim() == 3:
+        _require(cs.shape[1] == 1, "cos_sin_cache must be [max_position, (1,) rotary_dim]")
+        cs = cs[:, 0]
+    _require(cs.dim() == 2 and cs.dtype == torch.float32 and cs.stride(-1) == 1 and
+             0 < cs.shape[1] <= d and cs.shape[1] % 2 == 0,
+             "cos_sin_cache must be an fp32 [max_position, rotary_dim] table (cos | sin), "
+             "rotary_dim even and at most head_dim")
+    _require(positions.dim() == 1 and positions.numel() >= T and positions.is_contiguous(),
+             f"positions must be a contiguous vector of at least {T} entries")
+    args.rotary_dim, args.interleaved, args.inverse = cs.shape[1], bool(interleaved), bool(inverse)
+    args.cos_sin_cache, args.cos_sin_stride = cs.data_ptr(), cs.stride(0)
+    args.max_position = int(cs.shape[0])
+    args.positions_dtype = _index_code(positions, "positions")
+    args.positions = positions.data_ptr()
+    N.call("va_rotary", args, device)
+    return outs[0], outs[1]
+
+
+class _Rotary(torch.autograd.Function):
+    """rotary_embedding with its gradient, the transposed rotation."""
+
+    @staticmethod
+    def forward(ctx, q, k, cos_sin_cache, positions, interleaved, inverse):
+        ctx.save_for_backward(cos_sin_cache, positions)
+        ctx.form = (interleaved, inverse)
+        ctx.set_materialize_grads(False)
+        return rotary_embedding(q, k, cos_sin_cache, positions, interleaved=interleaved,
+                                inverse=inverse)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dq, dk):
+        cos_sin, positions = ctx.saved_tensors
+        interleaved, inverse = ctx.form
+        dq, dk = (g if g is not None and need else None
+                  for g, need in zip((dq, dk), ctx.needs_input_grad))
+        if dq is not None or dk is not None:
+            dq, dk = (g if g is None or g.stride(2) == 1 else g.contiguous() for g in (dq, dk))
+            dq, dk = rotary_embedding(dq, dk, cos_sin, positions, interleaved=interleaved,
+                                      inverse=not inverse)
+        return dq, dk, None, None, None, None
 
 
 # -------------------------------------------------------------------- decode
