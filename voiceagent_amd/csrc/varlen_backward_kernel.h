@@ -118,26 +118,27 @@ __device__ inline BwdBlock find_block(const int32_t* cu, int num_seqs, int total
 
 // Zeros for one head of the rows that belong to no sequence (in front of the
 // first and behind the last), shared among the workgroups that found no block.
-template <int D>
+template <int D, int kThreads>
 __device__ inline void zero_rest(const int32_t* cu, int num_seqs, int total, char* g, int64_t st,
                                  int64_t off, int nth, int of) {
   const int lo = num_seqs > 0 ? min(max(cu[0], 0), total) : 0;
   const int hi = num_seqs > 0 ? min(max(cu[num_seqs], lo), total) : 0;
   const int rest = lo + total - hi;
-  constexpr int CPR = D / 8, RPB = kBwdThreads / CPR;
+  constexpr int CPR = D / 8, RPB = kThreads / CPR;
   for (int64_t i = (int64_t)nth * RPB + threadIdx.x / CPR; i < rest; i += (int64_t)of * RPB) {
     const int64_t row = i < lo ? i : hi + (i - lo);
     st16(g + row * st + off + (threadIdx.x % CPR) * 16, make_uint4(0, 0, 0, 0));
   }
 }
 
-// Copies 64 rows of one tensor into an LDS tile, wave w's quarter of it: row r
+// Copies 64 rows of one tensor into an LDS tile, wave w's share of kWaves: row r
 // of the tile is row base + r of the sequence, zeros past `len`.
-template <int D>
+template <int D, int kWaves>
 __device__ inline void stage_rows(const char* src, int64_t st, int base, int len, uint32_t lds,
                                   int wave, int lane) {
   constexpr int ROWB = D * 2, CPR = ROWB / 16, RPI = 64 / CPR;
-  constexpr int NI = kBwdTile * ROWB / 1024 / 4;
+  constexpr int NI = kBwdTile * ROWB / 1024 / kWaves;
+  static_assert(NI >= 1, "a wave copies at least 1 KiB");
 #pragma unroll
   for (int i = 0; i < NI; ++i) {
     const int r = (wave * NI + i) * RPI + lane / CPR;
@@ -163,6 +164,9 @@ struct TileAt {
     tr = t * ROWB + ((r16 & 1) << 3);
     tr0 = ((2 * (g & 1) + ((r16 >> 1) & 1)) ^ swz<D>(t)) << 4;
   }
+  // Keeps what the reads below add to these from being held in registers through
+  // a loop, where it makes the compiler spill.
+  __device__ inline void rebuild() { asm volatile("" : "+v"(row0), "+v"(tr0), "+v"(row), "+v"(tr)); }
   // Rows 32 sub + l % 32, elements 16 step + 8 (l / 32) ... + 7.
   __device__ inline uint4 a(const char* tile, int sub, int step) const {
     return lds_read16(tile, sub * 32 * D * 2 + row + (row0 ^ (step << 5)));
@@ -244,7 +248,7 @@ __global__ __launch_bounds__(kBwdThreads, 2) void varlen_dq_kernel(VarlenBwdPara
   const int kv = pick % p.num_kv_heads, head = kv * group + pick / p.num_kv_heads;
   const BwdBlock blk = find_block(p.cu_q, p.num_seqs, p.total_q, tile);
   if (!blk.found) {
-    zero_rest<D>(p.cu_q, p.num_seqs, p.total_q, p.dq, p.dq_st, head * p.dq_sh, tile - blk.first,
+    zero_rest<D, kBwdThreads>(p.cu_q, p.num_seqs, p.total_q, p.dq, p.dq_st, head * p.dq_sh, tile - blk.first,
                  p.q_tiles - blk.first);
     return;
   }
@@ -261,8 +265,8 @@ __global__ __launch_bounds__(kBwdThreads, 2) void varlen_dq_kernel(VarlenBwdPara
       (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)s_kv);
   auto issue = [&](int t) {
     const uint32_t to = lds + (uint32_t)((t & 1) * 2 * TILE_B);
-    stage_rows<D>(kp, p.k_st, t * kBwdTile, ks.len, to, wave, lane);
-    stage_rows<D>(vp, p.v_st, t * kBwdTile, ks.len, to + TILE_B, wave, lane);
+    stage_rows<D, 4>(kp, p.k_st, t * kBwdTile, ks.len, to, wave, lane);
+    stage_rows<D, 4>(vp, p.v_st, t * kBwdTile, ks.len, to + TILE_B, wave, lane);
   };
   if (tiles > 0) issue(0);
 
@@ -378,13 +382,42 @@ __global__ __launch_bounds__(kBwdThreads, 2) void varlen_dq_kernel(VarlenBwdPara
 }
 
 // ------------------------------------------------------------------- dk, dv
+// Eight waves: four groups of 32 keys, twice, for the two halves of a tile's 64
+// queries; the halves' sums meet in LDS at the end.  (With four waves that take
+// both halves in turn the two waves of a SIMD belong to two workgroups, of which
+// a causal launch leaves the one with more queries alone for most of the time.)
+constexpr int kDkvThreads = 512;
+
+// A wave's accumulators to LDS, 16 bytes a lane at a time, and added from there.
+template <int DT>
+__device__ inline void put_acc(const f32x16_t (&acc)[DT], char* s, int lane) {
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      *reinterpret_cast<f32x4_t*>(s + ((dt * 4 + j) * 64 + lane) * 16) =
+          f32x4_t{acc[dt][4 * j], acc[dt][4 * j + 1], acc[dt][4 * j + 2], acc[dt][4 * j + 3]};
+}
+template <int DT>
+__device__ inline void add_acc(f32x16_t (&acc)[DT], const char* s, int lane) {
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const f32x4_t x = *reinterpret_cast<const f32x4_t*>(s + ((dt * 4 + j) * 64 + lane) * 16);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) acc[dt][4 * j + i] += x[i];
+    }
+}
+
 template <bool kBF16, int D>
-__global__ __launch_bounds__(kBwdThreads, 2) void varlen_dkv_kernel(VarlenBwdParams p) {
+__global__ __launch_bounds__(kDkvThreads, 2) void varlen_dkv_kernel(VarlenBwdParams p) {
   constexpr int ROWB = D * 2, TILE_B = kBwdTile * ROWB, DS = D / 16, DT = D / 32;
   __shared__ __align__(1024) char s_qd[2 * 2 * TILE_B];
   __shared__ __align__(16) float s_st[2 * 2 * kBwdTile];  // a stage's lse, delta
-  __shared__ float s_top[4];
+  __shared__ float s_top[8];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int sub = wave >> 2;  // the wave's half of a tile's queries
   const int lane = threadIdx.x & 63, l32 = lane & 31, half = lane >> 5;
   // (Under a causal mask a sequence's earlier blocks are seen by more queries.)
   const int tile = (int)(blockIdx.x / (unsigned)p.num_kv_heads);
@@ -392,10 +425,10 @@ __global__ __launch_bounds__(kBwdThreads, 2) void varlen_dkv_kernel(VarlenBwdPar
   const int group = p.num_heads / p.num_kv_heads;
   const BwdBlock blk = find_block(p.cu_k, p.num_seqs, p.total_k, tile);
   if (!blk.found) {
-    zero_rest<D>(p.cu_k, p.num_seqs, p.total_k, p.dk, p.dk_st, kv * p.dk_sh, tile - blk.first,
-                 p.k_tiles - blk.first);
-    zero_rest<D>(p.cu_k, p.num_seqs, p.total_k, p.dv, p.dv_st, kv * p.dv_sh, tile - blk.first,
-                 p.k_tiles - blk.first);
+    zero_rest<D, kDkvThreads>(p.cu_k, p.num_seqs, p.total_k, p.dk, p.dk_st, kv * p.dk_sh,
+                              tile - blk.first, p.k_tiles - blk.first);
+    zero_rest<D, kDkvThreads>(p.cu_k, p.num_seqs, p.total_k, p.dv, p.dv_st, kv * p.dv_sh,
+                              tile - blk.first, p.k_tiles - blk.first);
     return;
   }
   const SeqRows qs = seq_rows(p.cu_q, blk.seq, p.total_q);
@@ -413,16 +446,19 @@ __global__ __launch_bounds__(kBwdThreads, 2) void varlen_dkv_kernel(VarlenBwdPar
   // The tile requested next: head of the group, tile of its queries.
   int gi = 0, ti = 0;
   auto issue = [&](int stage) {
+    int at_lane = lane;  // (what follows from the lane is formed anew each step)
+    asm volatile("" : "+v"(at_lane));
     const int head = kv * group + gi, base = (t0 + ti) * kBwdTile;
     const uint32_t to = lds + (uint32_t)(stage * 2 * TILE_B);
-    stage_rows<D>(p.q + (int64_t)qs.row * p.q_st + head * p.q_sh, p.q_st, base, qs.len, to, wave, lane);
-    stage_rows<D>(p.dout + (int64_t)qs.row * p.do_st + head * p.do_sh, p.do_st, base, qs.len,
-                  to + TILE_B, wave, lane);
+    stage_rows<D, 8>(p.q + (int64_t)qs.row * p.q_st + head * p.q_sh, p.q_st, base, qs.len, to, wave,
+                     at_lane);
+    stage_rows<D, 8>(p.dout + (int64_t)qs.row * p.do_st + head * p.do_sh, p.do_st, base, qs.len,
+                     to + TILE_B, wave, at_lane);
     if (wave < 2) {
-      const int64_t w = (int64_t)head * p.total_q + qs.row + base + lane;
+      const int64_t w = (int64_t)head * p.total_q + qs.row + base + at_lane;
       const float* const at = (wave == 0 ? p.lse : p.delta) + w;
       const float* const none = wave == 0 ? &kInfRow : reinterpret_cast<const float*>(&kZeroRow);
-      dma4(base + lane < qs.len ? at : none,
+      dma4(base + at_lane < qs.len ? at : none,
            lds_st + (uint32_t)((stage * 2 + wave) * kBwdTile * 4));
     }
     if (++ti == nt) {
@@ -432,7 +468,7 @@ __global__ __launch_bounds__(kBwdThreads, 2) void varlen_dkv_kernel(VarlenBwdPar
   };
   if (steps > 0) issue(0);
 
-  const int wkey = j0 + 32 * wave, key = wkey + l32;
+  const int wkey = j0 + 32 * (wave & 3), key = wkey + l32;
   const int at = ks.row + min(key, ks.len - 1);
   uint4 kreg[DS], vreg[DS];
 #pragma unroll
@@ -445,17 +481,19 @@ __global__ __launch_bounds__(kBwdThreads, 2) void varlen_dkv_kernel(VarlenBwdPar
   if constexpr (!kBF16) {
     float top = 0.f;
     for (int g = 0; g < group; ++g)
-      for (int i = threadIdx.x; i < qs.len; i += kBwdThreads)
+      for (int i = threadIdx.x; i < qs.len; i += kDkvThreads)
         top = fmaxf(top, p.top[(int64_t)(kv * group + g) * p.total_q + qs.row + i]);
     top = group_max<64>(top);
     if (lane == 0) s_top[wave] = top;
     __syncthreads();
-    const int e = top_exponent(fmaxf(fmaxf(s_top[0], s_top[1]), fmaxf(s_top[2], s_top[3])));
+#pragma unroll
+    for (int w = 0; w < 8; ++w) top = fmaxf(top, s_top[w]);
+    const int e = top_exponent(top);
     lift = pow2(-e - kF16Lift);
     lower = pow2(e);
   }
 
-  const TileAt<D> ta(lane);
+  TileAt<D> ta(lane);
   f32x16_t dk[DT], dv[DT];
 #pragma unroll
   for (int dt = 0; dt < DT; ++dt) dk[dt] = dv[dt] = f32x16_t{};
@@ -466,57 +504,69 @@ __global__ __launch_bounds__(kBwdThreads, 2) void varlen_dkv_kernel(VarlenBwdPar
     if (it + 1 < steps) issue((it + 1) & 1);
     const char* const sq = s_qd + (it & 1) * 2 * TILE_B;
     const char* const sd = sq + TILE_B;
-    const float* const st = s_st + (it & 1) * 2 * kBwdTile;
+    const float* const st = s_st + (it & 1) * 2 * kBwdTile + 32 * sub + 4 * half;
+    const int i0 = tq * kBwdTile + 32 * sub;
+    if (++tq == t0 + nt) tq = t0;
+    // No query of these sees a key of the wave, or there are none.
+    if ((p.causal && i0 + 31 + ahead < wkey) || i0 >= qs.len) continue;
+    ta.rebuild();
+    f32x16_t s = {}, dp;
 #pragma unroll
-    for (int sub = 0; sub < 2; ++sub) {
-      const int i0 = tq * kBwdTile + 32 * sub;
-      // No query of these sees a key of the wave, or there are none.
-      if ((p.causal && i0 + 31 + ahead < wkey) || i0 >= qs.len) continue;
-      f32x16_t s = {}, dp;
+    for (int ds = 0; ds < DS; ++ds) s = mfma32<kBF16>(ta.a(sq, sub, ds), kreg[ds], s);
+    if (p.causal && i0 + ahead < wkey + 31) {
+      const int rel = key - ahead - i0 - 4 * half;  // query 8 (i / 4) + i % 4 sees it iff >= rel
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const f32x4_t d = *reinterpret_cast<const f32x4_t*>(st + kBwdTile + 32 * sub + 8 * j + 4 * half);
+      for (int i = 0; i < 16; ++i)
+        if (8 * (i / 4) + i % 4 < rel) s[i] = -INFINITY;
+    }
 #pragma unroll
-        for (int i = 0; i < 4; ++i) dp[4 * j + i] = -d[i];
-      }
+    for (int j = 0; j < 4; ++j) {
+      const f32x4_t lse = *reinterpret_cast<const f32x4_t*>(st + 8 * j);
+      const f32x4_t d = *reinterpret_cast<const f32x4_t*>(st + kBwdTile + 8 * j);
 #pragma unroll
-      for (int ds = 0; ds < DS; ++ds) s = mfma32<kBF16>(ta.a(sq, sub, ds), kreg[ds], s);
-#pragma unroll
-      for (int ds = 0; ds < DS; ++ds) dp = mfma32<kBF16>(ta.a(sd, sub, ds), vreg[ds], dp);
-      if (p.causal && i0 + ahead < wkey + 31) {
-        const int rel = key - ahead - i0 - 4 * half;  // query 8 (i / 4) + i % 4 sees it iff >= rel
-#pragma unroll
-        for (int i = 0; i < 16; ++i)
-          if (8 * (i / 4) + i % 4 < rel) s[i] = -INFINITY;
-      }
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const f32x4_t lse = *reinterpret_cast<const f32x4_t*>(st + 32 * sub + 8 * j + 4 * half);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float off = kBF16 ? lse[i] : lse[i] - (float)kF16Lift;
-          s[4 * j + i] = fast_exp2(fmaf(s[4 * j + i], p.scale_log2, -off));
-          dp[4 * j + i] *= kBF16 ? s[4 * j + i] : s[4 * j + i] * lift;
-        }
-      }
-#pragma unroll
-      for (int hf = 0; hf < 2; ++hf) {
-        const uint4 pb = pack_b<kBF16>(s, hf), db = pack_b<kBF16>(dp, hf);
-#pragma unroll
-        for (int dt = 0; dt < DT; ++dt) {
-          dv[dt] = mfma32<kBF16>(ta.at(sd, sub, hf, dt), pb, dv[dt]);
-          dk[dt] = mfma32<kBF16>(ta.at(sq, sub, hf, dt), db, dk[dt]);
-        }
+      for (int i = 0; i < 4; ++i) {
+        const float off = kBF16 ? lse[i] : lse[i] - (float)kF16Lift;
+        s[4 * j + i] = fast_exp2(fmaf(s[4 * j + i], p.scale_log2, -off));
+        dp[4 * j + i] = -d[i];
       }
     }
-    if (++tq == t0 + nt) tq = t0;
+#pragma unroll
+    for (int hf = 0; hf < 2; ++hf) {
+      const uint4 pb = pack_b<kBF16>(s, hf);
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) dv[dt] = mfma32<kBF16>(ta.at(sd, sub, hf, dt), pb, dv[dt]);
+    }
+    ta.rebuild();
+#pragma unroll
+    for (int ds = 0; ds < DS; ++ds) dp = mfma32<kBF16>(ta.a(sd, sub, ds), vreg[ds], dp);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) dp[i] *= kBF16 ? s[i] : s[i] * lift;
+#pragma unroll
+    for (int hf = 0; hf < 2; ++hf) {
+      const uint4 db = pack_b<kBF16>(dp, hf);
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) dk[dt] = mfma32<kBF16>(ta.at(sq, sub, hf, dt), db, dk[dt]);
+    }
   }
+  // The halves' sums: the first half's waves write dk, the second's dv.
+  char* const s_x = s_qd + (wave & 3) * (64 * D / 2 * 4);
   __syncthreads();  // every wave is done with the tiles
-  char* const s_w = s_qd + wave * 2 * 32 * ROWB;
-  write_rows<kBF16, D>(dk, p.scale * lower, s_w, p.dk + (int64_t)ks.row * p.dk_st + kv * p.dk_sh,
-                       p.dk_st, wkey, ks.len, lane);
-  write_rows<kBF16, D>(dv, kBF16 ? 1.f : pow2(-kF16Lift), s_w + 32 * ROWB,
-                       p.dv + (int64_t)ks.row * p.dv_st + kv * p.dv_sh, p.dv_st, wkey, ks.len, lane);
+  if (sub == 0) put_acc<DT>(dv, s_x, lane);
+  __syncthreads();
+  if (sub == 1) add_acc<DT>(dv, s_x, lane);
+  __syncthreads();
+  if (sub == 1) put_acc<DT>(dk, s_x, lane);
+  __syncthreads();
+  if (sub == 0) add_acc<DT>(dk, s_x, lane);
+  __syncthreads();
+  char* const s_w = s_qd + wave * 32 * ROWB;
+  if (sub == 0)
+    write_rows<kBF16, D>(dk, p.scale * lower, s_w, p.dk + (int64_t)ks.row * p.dk_st + kv * p.dk_sh,
+                         p.dk_st, wkey, ks.len, lane);
+  else
+    write_rows<kBF16, D>(dv, kBF16 ? 1.f : pow2(-kF16Lift), s_w,
+                         p.dv + (int64_t)ks.row * p.dv_st + kv * p.dv_sh, p.dv_st, wkey, ks.len,
+                         lane);
 }
 
 // Both launches for one 16-bit type and head_dim, instantiated in
@@ -529,7 +579,7 @@ static void launch_varlen_backward_d(const VarlenBwdParams& p, hipStream_t st) {
   hipLaunchKernelGGL((varlen_dq_kernel<kBF16, D>), dim3((unsigned)p.q_tiles * p.num_heads),
                      dim3(kBwdThreads), 0, st, p);
   hipLaunchKernelGGL((varlen_dkv_kernel<kBF16, D>), dim3((unsigned)p.k_tiles * p.num_kv_heads),
-                     dim3(kBwdThreads), 0, st, p);
+                     dim3(kDkvThreads), 0, st, p);
 }
 
 template <>
