@@ -1,23 +1,52 @@
 // Host side of the varlen attention's gradient: argument checks, workspace and
 // dispatch (kernels in varlen_backward_kernel.h, instantiated per element type
 // in varlen_backward_{bf16,f16}.hip).
+#include <algorithm>
+
 #include "varlen_backward_kernel.h"
 
 namespace va {
 
-// The first launch's results for the second: lse, delta and, for f16, the
-// rows' largest |dout|.
-static size_t backward_workspace(const va_varlen_bwd_args* a) {
-  const size_t rows = (size_t)a->num_heads * (size_t)a->total_q;
-  return rows * sizeof(float) * (a->dtype == VA_F16 ? 3 : 2);
+// How many workgroups share the queries that see a block of keys.  Few blocks,
+// each of them seen by many queries (long sequences, or several query heads to a
+// kv head), leave most of the chip idle otherwise.
+static int dkv_parts(const va_varlen_bwd_args* a) {
+  if (a->num_seqs <= 0 || a->num_kv_heads <= 0 || a->total_q <= 0 || a->total_k <= 0) return 1;
+  const int64_t blocks = ((int64_t)a->total_k / kDkvKeys + a->num_seqs) * a->num_kv_heads;
+  const int64_t slots = (a->head_dim == 64 ? 3 : 2) * (int64_t)current_device_cus();
+  const int64_t tiles = ((int64_t)a->total_q / a->num_seqs + kDkvTile - 1) / kDkvTile;
+  const int64_t steps = tiles * (a->num_heads / a->num_kv_heads) / (a->causal ? 2 : 1);
+  return (int)std::max<int64_t>(1, std::min<int64_t>({3 * slots / blocks, steps / 2, 16}));
+}
+
+// Workspace: the first launch's results for the second (lse, delta and, for f16,
+// the rows' largest |dout|), and the parts' sums.
+struct BwdLayout {
+  int64_t k_tiles;
+  int parts;
+  size_t rows, sums, total;  // bytes; sums: where they begin
+};
+static BwdLayout backward_layout(const va_varlen_bwd_args* a) {
+  BwdLayout l;
+  l.rows = (size_t)a->num_heads * (size_t)a->total_q * sizeof(float);
+  l.k_tiles = (int64_t)a->total_k / kDkvKeys + a->num_seqs + 1;
+  l.parts = dkv_parts(a);
+  l.sums = (l.rows * (a->dtype == VA_F16 ? 3 : 2) + 255) / 256 * 256;
+  l.total = l.sums;
+  if (l.parts > 1)
+    l.total += (size_t)l.k_tiles * l.parts * a->num_kv_heads * 2 * kDkvKeys * a->head_dim * sizeof(float);
+  return l;
 }
 
 }  // namespace va
 
 extern "C" size_t va_varlen_attention_backward_workspace_bytes(const va_varlen_bwd_args* a) {
   if (a == nullptr || a->struct_size != sizeof(va_varlen_bwd_args)) return 0;
-  if (a->num_heads <= 0 || a->total_q <= 0) return 0;
-  return va::backward_workspace(a);
+  if (a->num_heads <= 0 || a->num_kv_heads <= 0 || a->num_heads % a->num_kv_heads != 0 ||
+      a->num_seqs < 0 || a->total_q <= 0 || a->total_k < 0 ||
+      (a->head_dim != 64 && a->head_dim != 128))
+    return 0;
+  return va::backward_layout(a).total;
 }
 
 extern "C" int va_varlen_attention_backward(const va_varlen_bwd_args* a, void* stream) {
@@ -50,6 +79,11 @@ extern "C" int va_varlen_attention_backward(const va_varlen_bwd_args* a, void* s
                              a->dv_stride_head};
   for (int64_t s : strides)
     VA_CHECK_ARG(s % 8 == 0, "%s: strides must be 16-byte multiples", fn);
+  // (A tile's lane offsets are 32-bit.)
+  const int64_t toks[] = {a->q_stride_tok, a->dout_stride_tok, a->k_stride_tok, a->v_stride_tok};
+  for (int64_t s : toks)
+    VA_CHECK_ARG(s >= 0 && s * 2 < ((int64_t)1 << 25),
+                 "%s: token strides of q, k, v and dout must be non-negative and below 32 MiB", fn);
   const uintptr_t ptrs[] = {(uintptr_t)a->q,    (uintptr_t)a->k,  (uintptr_t)a->v,  (uintptr_t)a->out,
                             (uintptr_t)a->dout, (uintptr_t)a->dq, (uintptr_t)a->dk, (uintptr_t)a->dv};
   for (uintptr_t p : ptrs)
@@ -58,10 +92,11 @@ extern "C" int va_varlen_attention_backward(const va_varlen_bwd_args* a, void* s
   // A workgroup per block of every sequence; one more, which finds none, writes
   // the zeros of rows outside the sequences.
   const int64_t q_tiles = (int64_t)a->total_q / kBwdRows + a->num_seqs + 1;
-  const int64_t k_tiles = (int64_t)a->total_k / kBwdRows + a->num_seqs + 1;
-  VA_CHECK_ARG(q_tiles * a->num_heads <= INT32_MAX && k_tiles * a->num_kv_heads <= INT32_MAX,
+  const BwdLayout lay = backward_layout(a);
+  VA_CHECK_ARG(q_tiles * a->num_heads <= INT32_MAX &&
+                   lay.k_tiles * lay.parts * a->num_kv_heads <= INT32_MAX,
                "%s: too many (sequence, head, block) items", fn);
-  const size_t need = a->total_q > 0 ? backward_workspace(a) : 0;
+  const size_t need = a->total_q > 0 ? lay.total : 0;
   if (need > 0 && (a->workspace == nullptr || a->workspace_bytes < need ||
                    (uintptr_t)a->workspace % 16 != 0)) {
     set_error("%s: needs a 16-byte aligned workspace of %zu bytes", fn, need);
@@ -104,11 +139,12 @@ extern "C" int va_varlen_attention_backward(const va_varlen_bwd_args* a, void* s
   p.num_heads = a->num_heads;
   p.num_kv_heads = a->num_kv_heads;
   p.q_tiles = (int)q_tiles;
-  p.k_tiles = (int)k_tiles;
-  const size_t rows = (size_t)a->num_heads * (size_t)a->total_q;
+  p.k_tiles = (int)lay.k_tiles;
+  p.parts = lay.parts;
   p.lse = (float*)a->workspace;
-  p.delta = p.lse + rows;
-  p.top = p.delta + rows;
+  p.delta = (float*)((char*)a->workspace + lay.rows);
+  p.top = (float*)((char*)a->workspace + 2 * lay.rows);
+  p.part = (float*)((char*)a->workspace + lay.sums);
   const hipStream_t st = (hipStream_t)stream;
   if (a->dtype == VA_BF16)
     a->head_dim == 64 ? launch_varlen_backward<true, 64>(p, st) : launch_varlen_backward<true, 128>(p, st);

@@ -53,16 +53,16 @@ struct VarlenBwdParams {
   float scale, scale_log2;  // c, c log2 e
   int32_t causal;
   int32_t num_seqs, total_q, total_k, num_heads, num_kv_heads;
-  int32_t q_tiles, k_tiles;  // workgroups per head of the two launches
-  float* lse;                // [num_heads][total_q]
-  float* delta;              // [num_heads][total_q]
+  int32_t q_tiles, k_tiles;  // workgroups per head of the two launches (and part)
+  int32_t parts;             // workgroups that share a block of keys' queries
+  float* part;               // parts > 1: their sums, [tile][part][kv head][wave][D / 8][64] x 4
+  float* lse;                // [num_heads][total_q]: log2 sum 2^(c log2 e s), f16: - kF16Lift
+  float* delta;              // [num_heads][total_q]: -delta
   float* top;                // f16: [num_heads][total_q], largest |dout| of the row
 };
 
 constexpr int kBwdThreads = 256;
 constexpr int kBwdRows = 128;  // queries (keys) of a workgroup, 32 a wave
-constexpr int kBwdTile = 64;   // rows of the other side staged at a time
-
 template <bool kBF16>
 __device__ inline f32x16_t mfma32(uint4 a, uint4 b, f32x16_t c) {
   if constexpr (kBF16)
@@ -73,13 +73,11 @@ __device__ inline f32x16_t mfma32(uint4 a, uint4 b, f32x16_t c) {
                                                   __builtin_bit_cast(f16x8_t, b), c, 0, 0, 0);
 }
 
-// The lse of a staged row that is not there: its P is 2^-inf = 0.
-__device__ const float kInfRow = INFINITY;
-
 // One 4-byte global -> LDS copy per lane (lane l's word lands at lds + 4 l);
 // wait states as in dma16.
-__device__ inline void dma4(const void* src, uint32_t lds) {
-  asm volatile("s_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(src), "{m0}"(lds) : "memory");
+__device__ inline void dma4(uint32_t off, const void* base, uint32_t lds) {
+  asm volatile("s_nop 4\n\tglobal_load_lds_dword %0, %1" ::"v"(off), "s"(base), "{m0}"(lds)
+               : "memory");
 }
 
 // Sequence s's rows [row, row + len) of `total` packed rows: what cu says, held
@@ -92,18 +90,19 @@ __device__ inline SeqRows seq_rows(const int32_t* cu, int s, int total) {
   return {a, min(max(cu[s + 1], a), total) - a};
 }
 
-// The `tile`-th block of kBwdRows rows, counting every sequence's blocks in
+// The `tile`-th block of kRows rows, counting every sequence's blocks in
 // turn.  found: there is one; otherwise first is the number of blocks there are.
 struct BwdBlock {
   bool found;
   int seq, first;  // first: tile number of the sequence's first block
 };
+template <int kRows>
 __device__ inline BwdBlock find_block(const int32_t* cu, int num_seqs, int total, int tile) {
   const int lane = threadIdx.x & 63;
   int before = 0;
   for (int s0 = 0; s0 < num_seqs; s0 += 64) {
     int nb = 0;
-    if (s0 + lane < num_seqs) nb = (seq_rows(cu, s0 + lane, total).len + kBwdRows - 1) / kBwdRows;
+    if (s0 + lane < num_seqs) nb = (seq_rows(cu, s0 + lane, total).len + kRows - 1) / kRows;
     const int upto = wave_scan(nb);
     const uint64_t past = __builtin_amdgcn_ballot_w64(before + upto > tile);
     if (past != 0) {
@@ -131,23 +130,41 @@ __device__ inline void zero_rest(const int32_t* cu, int num_seqs, int total, cha
   }
 }
 
-// Copies 64 rows of one tensor into an LDS tile, wave w's share of kWaves: row r
-// of the tile is row base + r of the sequence, zeros past `len`.
-template <int D, int kWaves>
-__device__ inline void stage_rows(const char* src, int64_t st, int base, int len, uint32_t lds,
-                                  int wave, int lane) {
-  constexpr int ROWB = D * 2, CPR = ROWB / 16, RPI = 64 / CPR;
-  constexpr int NI = kBwdTile * ROWB / 1024 / kWaves;
-  static_assert(NI >= 1, "a wave copies at least 1 KiB");
-#pragma unroll
-  for (int i = 0; i < NI; ++i) {
-    const int r = (wave * NI + i) * RPI + lane / CPR;
-    const int chunk = (lane % CPR) ^ swz<D>(r);
-    const char* const at = src + (int64_t)(base + r) * st + chunk * 16;
-    dma16(base + r < len ? at : reinterpret_cast<const char*>(&kZeroRow),
-          lds + (uint32_t)((wave * NI + i) * 1024));
-  }
+// The tiles' swizzle: the 16-byte chunk c of row r sits at chunk c ^ this.  Both
+// kinds of reads below find their 256 bytes a cycle in distinct banks: 16 rows of
+// one chunk (A operands), and 4 rows of 4 chunks (transposed; with the forward
+// kernel's swizzle these take two cycles).  Depends on r % 16 only.
+template <int D>
+__device__ inline int bwd_swz(int r) {
+  if constexpr (D == 128) return ((r & 3) << 2) | ((r >> 2) & 3);
+  return ((r & 2) << 1) | ((r >> 1) & 2) | ((r >> 3) & 1);
 }
+
+// A wave's share of the copies of kRows rows of one tensor into an LDS tile: NI
+// copies of 1 KiB.  A copy holds up its wave for some 70 cycles (more when all of
+// a CU's waves issue theirs at once: 64 bytes a cycle go to a CU), so a step's are
+// spread among its matrix products.  Rows past the sequence's last repeat it; what
+// they make is masked.  Lane offsets are 32-bit, what is left of an address is
+// uniform (64-bit lane addresses, formed for each copy, took 300 cycles a step).
+template <int D, int kWaves, int kRows>
+struct TileCopy {
+  static constexpr int CPR = D / 8, RPI = 64 / CPR;
+  static constexpr int NI = kRows * D * 2 / 1024 / kWaves;
+  static_assert(NI >= 1 && NI <= 4, "a wave copies 1 to 4 KiB");
+  uint32_t chunk;  // the lane's, in bytes, in copy 0; copy i's differs by exactly i chunks' bits
+  int row;         // its row in copy 0
+  __device__ inline TileCopy(int wave, int lane) {
+    row = wave * NI * RPI + lane / CPR;
+    chunk = (uint32_t)(((lane % CPR) ^ bwd_swz<D>(row)) << 4);
+  }
+  // Copy i of the tile whose row 0 is at src (rows st bytes apart, row `last` the
+  // last one there is).
+  __device__ inline void one(int i, const char* src, int64_t st, int last, uint32_t lds,
+                             int wave) const {
+    const uint32_t r = (uint32_t)min(row + i * RPI, last);
+    dma16(r * (uint32_t)st + (chunk ^ (i << 4)), src, lds + (uint32_t)((wave * NI + i) * 1024));
+  }
+};
 
 // A wave's LDS offsets in a tile: of row l % 32's chunk for 8 elements of the
 // l / 32 half (A rows), and of the transposed reads.
@@ -159,10 +176,10 @@ struct TileAt {
     constexpr int ROWB = D * 2;
     const int r = lane & 31, h = lane >> 5, r16 = lane & 15, g = lane >> 4;
     row = r * ROWB;
-    row0 = (h ^ swz<D>(r)) << 4;
+    row0 = (h ^ bwd_swz<D>(r)) << 4;
     const int t = 4 * h + (r16 >> 2);
     tr = t * ROWB + ((r16 & 1) << 3);
-    tr0 = ((2 * (g & 1) + ((r16 >> 1) & 1)) ^ swz<D>(t)) << 4;
+    tr0 = ((2 * (g & 1) + ((r16 >> 1) & 1)) ^ bwd_swz<D>(t)) << 4;
   }
   // Keeps what the reads below add to these from being held in registers through
   // a loop, where it makes the compiler spill.
@@ -176,18 +193,31 @@ struct TileAt {
     const int off = (sub * 32 + half * 16) * D * 2 + tr;
     const uint2 lo = __builtin_bit_cast(uint2, lds_read_tr(tile, off + (tr0 ^ (dt << 6))));
     const uint2 hi =
-        __builtin_bit_cast(uint2, lds_read_tr(tile, off + 8 * D * 2 + (tr0 ^ 16 ^ (dt << 6))));
+        __builtin_bit_cast(uint2, lds_read_tr(tile, off + 8 * D * 2 + (tr0 ^ (D == 128 ? 32 : 16) ^ (dt << 6))));
     return make_uint4(lo.x, lo.y, hi.x, hi.y);
   }
 };
+
+// Two floats to a pair of 16-bit elements, rounded to nearest even, in one
+// instruction (f16 too).
+template <bool kBF16>
+__device__ inline uint32_t pack_pair(float lo, float hi) {
+  if constexpr (kBF16) {
+    return Mma<true>::pack2(lo, hi);
+  } else {
+    typedef float f32x2 __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{lo, hi}), f16x2_t));
+  }
+}
 
 // Eight accumulator values of one lane (rows 16 half + {0-3, 8-11} + 4 (l / 32))
 // as a B operand.
 template <bool kBF16>
 __device__ inline uint4 pack_b(const f32x16_t& x, int half) {
-  using M = Mma<kBF16>;
-  return make_uint4(M::pack2(x[8 * half], x[8 * half + 1]), M::pack2(x[8 * half + 2], x[8 * half + 3]),
-                    M::pack2(x[8 * half + 4], x[8 * half + 5]), M::pack2(x[8 * half + 6], x[8 * half + 7]));
+  return make_uint4(pack_pair<kBF16>(x[8 * half], x[8 * half + 1]),
+                    pack_pair<kBF16>(x[8 * half + 2], x[8 * half + 3]),
+                    pack_pair<kBF16>(x[8 * half + 4], x[8 * half + 5]),
+                    pack_pair<kBF16>(x[8 * half + 6], x[8 * half + 7]));
 }
 
 // Writes a wave's gradient, accumulators [D][32 rows] times `mul`, as rows of
@@ -196,15 +226,14 @@ __device__ inline uint4 pack_b(const f32x16_t& x, int half) {
 template <bool kBF16, int D>
 __device__ inline void write_rows(const f32x16_t (&acc)[D / 32], float mul, char* s, char* dst,
                                   int64_t st, int row0, int rows, int lane) {
-  using M = Mma<kBF16>;
   constexpr int ROWB = D * 2, CPR = ROWB / 16, RPS = 64 / CPR;
   const int r = lane & 31, h = lane >> 5;
 #pragma unroll
   for (int dt = 0; dt < D / 32; ++dt)
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const uint2 w = make_uint2(M::pack2(acc[dt][4 * j] * mul, acc[dt][4 * j + 1] * mul),
-                                 M::pack2(acc[dt][4 * j + 2] * mul, acc[dt][4 * j + 3] * mul));
+      const uint2 w = make_uint2(pack_pair<kBF16>(acc[dt][4 * j] * mul, acc[dt][4 * j + 1] * mul),
+                                 pack_pair<kBF16>(acc[dt][4 * j + 2] * mul, acc[dt][4 * j + 3] * mul));
       *reinterpret_cast<uint2*>(s + r * ROWB + (((4 * dt + j) ^ (r % CPR)) << 4) + h * 8) = w;
     }
   __builtin_amdgcn_wave_barrier();
@@ -235,7 +264,8 @@ constexpr int kF16Lift = 14;
 // and the maximum is followed without slack, which keeps dS near v's size.
 template <bool kBF16, int D>
 __global__ __launch_bounds__(kBwdThreads, 2) void varlen_dq_kernel(VarlenBwdParams p) {
-  constexpr int ROWB = D * 2, TILE_B = kBwdTile * ROWB, DS = D / 16, DT = D / 32;
+  constexpr int kTile = 64;  // keys
+  constexpr int ROWB = D * 2, TILE_B = kTile * ROWB, DS = D / 16, DT = D / 32;
   __shared__ __align__(1024) char s_kv[2 * 2 * TILE_B];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int lane = threadIdx.x & 63, l32 = lane & 31, half = lane >> 5;
@@ -246,7 +276,7 @@ __global__ __launch_bounds__(kBwdThreads, 2) void varlen_dq_kernel(VarlenBwdPara
   const int pick = (int)(blockIdx.x % (unsigned)p.num_heads);
   const int group = p.num_heads / p.num_kv_heads;
   const int kv = pick % p.num_kv_heads, head = kv * group + pick / p.num_kv_heads;
-  const BwdBlock blk = find_block(p.cu_q, p.num_seqs, p.total_q, tile);
+  const BwdBlock blk = find_block<kBwdRows>(p.cu_q, p.num_seqs, p.total_q, tile);
   if (!blk.found) {
     zero_rest<D, kBwdThreads>(p.cu_q, p.num_seqs, p.total_q, p.dq, p.dq_st, head * p.dq_sh, tile - blk.first,
                  p.q_tiles - blk.first);
@@ -258,17 +288,26 @@ __global__ __launch_bounds__(kBwdThreads, 2) void varlen_dq_kernel(VarlenBwdPara
   const int ahead = ks.len - qs.len;             // causal: query i sees keys j <= i + ahead
   const int kend =
       p.causal ? min(max(ahead + min(i0 + kBwdRows, qs.len), 0), ks.len) : ks.len;
-  const int tiles = (kend + kBwdTile - 1) / kBwdTile;
+  const int tiles = (kend + kTile - 1) / kTile;
   const char* const kp = p.k + (int64_t)ks.row * p.k_st + kv * p.k_sh;
   const char* const vp = p.v + (int64_t)ks.row * p.v_st + kv * p.v_sh;
   const uint32_t lds = __builtin_amdgcn_readfirstlane(
       (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)s_kv);
-  auto issue = [&](int t) {
+  using Copy = TileCopy<D, 4, kTile>;
+  const Copy copy(wave, lane);
+  // Copy n of tile t: K's, then V's.
+  auto issue = [&](int t, int n) {
     const uint32_t to = lds + (uint32_t)((t & 1) * 2 * TILE_B);
-    stage_rows<D, 4>(kp, p.k_st, t * kBwdTile, ks.len, to, wave, lane);
-    stage_rows<D, 4>(vp, p.v_st, t * kBwdTile, ks.len, to + TILE_B, wave, lane);
+    const int last = ks.len - 1 - t * kTile;
+    if (n < Copy::NI)
+      copy.one(n, kp + (int64_t)(t * kTile) * p.k_st, p.k_st, last, to, wave);
+    else
+      copy.one(n - Copy::NI, vp + (int64_t)(t * kTile) * p.v_st, p.v_st, last, to + TILE_B, wave);
   };
-  if (tiles > 0) issue(0);
+  if (tiles > 0) {
+#pragma unroll
+    for (int n = 0; n < 2 * Copy::NI; ++n) issue(0, n);
+  }
 
   // The wave's 32 queries (rows past the sequence repeat its last).
   const int wrow = i0 + 32 * wave;
@@ -308,7 +347,7 @@ __global__ __launch_bounds__(kBwdThreads, 2) void varlen_dq_kernel(VarlenBwdPara
     }
   }
 
-  const TileAt<D> ta(lane);
+  TileAt<D> ta(lane);
   const int lim = p.causal ? min(ks.len, ahead + row + 1) : ks.len;  // keys the lane's query sees
   const int lim_lo = p.causal ? min(ks.len, ahead + wrow + 1) : ks.len;
   const int lim_hi = p.causal ? min(ks.len, ahead + wrow + 32) : ks.len;
@@ -321,59 +360,82 @@ __global__ __launch_bounds__(kBwdThreads, 2) void varlen_dq_kernel(VarlenBwdPara
   for (int t = 0; t < tiles; ++t) {
     wait_vmcnt<0>();
     __syncthreads();
-    if (t + 1 < tiles) issue(t + 1);
+    const bool more = t + 1 < tiles;
     const char* const sk = s_kv + (t & 1) * 2 * TILE_B;
     const char* const sv = sk + TILE_B;
 #pragma unroll
     for (int sub = 0; sub < 2; ++sub) {
-      const int j0 = t * kBwdTile + 32 * sub;
-      if (j0 >= lim_hi) break;  // no query of the wave sees these
-      f32x16_t s = {}, dp;
+    const int j0 = t * kTile + 32 * sub;
+    if (j0 >= lim_hi) {  // no query of the wave sees these
+      if (more) {
 #pragma unroll
-      for (int i = 0; i < 16; ++i) dp[i] = -delta;
-#pragma unroll
-      for (int ds = 0; ds < DS; ++ds) s = mfma32<kBF16>(ta.a(sk, sub, ds), qreg[ds], s);
-#pragma unroll
-      for (int ds = 0; ds < DS; ++ds) dp = mfma32<kBF16>(ta.a(sv, sub, ds), doreg[ds], dp);
-      if (j0 + 32 > lim_lo) {
-        const int rel = lim - j0 - 4 * half;  // key 8 (i / 4) + i % 4 of the lane is seen iff < rel
-#pragma unroll
-        for (int i = 0; i < 16; ++i)
-          if (8 * (i / 4) + i % 4 >= rel) s[i] = -INFINITY;
+        for (int n = 0; n < Copy::NI; ++n) issue(t + 1, sub * Copy::NI + n);
       }
-      float mx = s[0];
+      continue;
+    }
+    ta.rebuild();
+    // S and dP in turn, operands requested kAhead products before their own, the
+    // next tile's copies (K's beside the first 32 keys, V's beside the others)
+    // between them.
+    constexpr int kAhead = 4;
+    uint4 op[kAhead];
+    auto request = [&](int n) {
+      if (n < 2 * DS) op[n % kAhead] = ta.a(n & 1 ? sv : sk, sub, n / 2);
+    };
 #pragma unroll
-      for (int i = 1; i < 16; ++i) mx = fmaxf(mx, s[i]);
-      mx = max_xor32(mx) * p.scale_log2;
-      if (__builtin_amdgcn_ballot_w64(mx > m + kSlack) != 0) {
-        const float mn = fmaxf(m, mx);
-        const float alpha = fast_exp2(m - mn);
-        m = mn;
-        l *= alpha;
+    for (int n = 0; n < kAhead; ++n) request(n);
+    f32x16_t s = {}, dp;
 #pragma unroll
-        for (int dt = 0; dt < DT; ++dt) acc[dt] *= alpha;
-      }
-      const float base = kBF16 ? m : m + (float)e;
+    for (int i = 0; i < 16; ++i) dp[i] = -delta;
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        s[i] = fast_exp2(fmaf(s[i], p.scale_log2, -base));
-        l += s[i];
-        dp[i] *= s[i];
-      }
+    for (int n = 0; n < 2 * DS; ++n) {
+      if (n & 1)
+        dp = mfma32<kBF16>(op[n % kAhead], doreg[n / 2], dp);
+      else
+        s = mfma32<kBF16>(op[n % kAhead], qreg[n / 2], s);
+      request(n + kAhead);
+      constexpr int kEvery = 2 * DS / Copy::NI;
+      if (n % kEvery == kEvery - 1 && more) issue(t + 1, sub * Copy::NI + n / kEvery);
+    }
+    if (j0 + 32 > lim_lo) {
+      const int rel = lim - j0 - 4 * half;  // key 8 (i / 4) + i % 4 of the lane is seen iff < rel
 #pragma unroll
-      for (int hf = 0; hf < 2; ++hf) {
-        const uint4 b = pack_b<kBF16>(dp, hf);
+      for (int i = 0; i < 16; ++i)
+        if (8 * (i / 4) + i % 4 >= rel) s[i] = -INFINITY;
+    }
+    float mx = s[0];
 #pragma unroll
-        for (int dt = 0; dt < DT; ++dt) acc[dt] = mfma32<kBF16>(ta.at(sk, sub, hf, dt), b, acc[dt]);
-      }
+    for (int i = 1; i < 16; ++i) mx = fmaxf(mx, s[i]);
+    mx = max_xor32(mx) * p.scale_log2;
+    if (__builtin_amdgcn_ballot_w64(mx > m + kSlack) != 0) {
+      const float mn = fmaxf(m, mx);
+      const float alpha = fast_exp2(m - mn);
+      m = mn;
+      l *= alpha;
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) acc[dt] *= alpha;
+    }
+    const float base = kBF16 ? m : m + (float)e;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      s[i] = fast_exp2(fmaf(s[i], p.scale_log2, -base));
+      l += s[i];
+      dp[i] *= s[i];
+    }
+#pragma unroll
+    for (int hf = 0; hf < 2; ++hf) {
+      const uint4 b = pack_b<kBF16>(dp, hf);
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) acc[dt] = mfma32<kBF16>(ta.at(sk, sub, hf, dt), b, acc[dt]);
+    }
     }
   }
   l = sum_xor32(l);
   const float base = kBF16 ? m : m + (float)e;
   if (half == 0 && row < qs.len) {
     const int64_t w = (int64_t)head * p.total_q + at;
-    p.lse[w] = l > 0.f ? base + __builtin_amdgcn_logf(l) : INFINITY;
-    p.delta[w] = delta;
+    p.lse[w] = l > 0.f ? base + __builtin_amdgcn_logf(l) - (kBF16 ? 0.f : (float)kF16Lift) : INFINITY;
+    p.delta[w] = -delta;
   }
   __syncthreads();  // every wave is done with the tiles
   write_rows<kBF16, D>(acc, l > 0.f ? p.scale / l : 0.f, s_kv + wave * 32 * ROWB,
@@ -382,93 +444,136 @@ __global__ __launch_bounds__(kBwdThreads, 2) void varlen_dq_kernel(VarlenBwdPara
 }
 
 // ------------------------------------------------------------------- dk, dv
-// Eight waves: four groups of 32 keys, twice, for the two halves of a tile's 64
-// queries; the halves' sums meet in LDS at the end.  (With four waves that take
-// both halves in turn the two waves of a SIMD belong to two workgroups, of which
-// a causal launch leaves the one with more queries alone for most of the time.)
-constexpr int kDkvThreads = 512;
-
-// A wave's accumulators to LDS, 16 bytes a lane at a time, and added from there.
-template <int DT>
-__device__ inline void put_acc(const f32x16_t (&acc)[DT], char* s, int lane) {
-#pragma unroll
-  for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-      *reinterpret_cast<f32x4_t*>(s + ((dt * 4 + j) * 64 + lane) * 16) =
-          f32x4_t{acc[dt][4 * j], acc[dt][4 * j + 1], acc[dt][4 * j + 2], acc[dt][4 * j + 3]};
-}
-template <int DT>
-__device__ inline void add_acc(f32x16_t (&acc)[DT], const char* s, int lane) {
-#pragma unroll
-  for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const f32x4_t x = *reinterpret_cast<const f32x4_t*>(s + ((dt * 4 + j) * 64 + lane) * 16);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) acc[dt][4 * j + i] += x[i];
-    }
-}
-
+// A wave's 32 keys of dv (role 0) or dk.
 template <bool kBF16, int D>
-__global__ __launch_bounds__(kDkvThreads, 2) void varlen_dkv_kernel(VarlenBwdParams p) {
-  constexpr int ROWB = D * 2, TILE_B = kBwdTile * ROWB, DS = D / 16, DT = D / 32;
+__device__ inline void write_dkv(const VarlenBwdParams& p, const f32x16_t (&acc)[D / 32], float mul,
+                                 char* s, int role, const SeqRows& ks, int kv, int key, int lane) {
+  if (role == 0)
+    write_rows<kBF16, D>(acc, mul, s, p.dv + (int64_t)ks.row * p.dv_st + kv * p.dv_sh, p.dv_st, key,
+                         ks.len, lane);
+  else
+    write_rows<kBF16, D>(acc, mul, s, p.dk + (int64_t)ks.row * p.dk_st + kv * p.dk_sh, p.dk_st, key,
+                         ks.len, lane);
+}
+
+// A workgroup's share of the gradients of a block of 64 keys of one kv head: the
+// tiles of 64 queries, head by head of the group, that see some of them.
+constexpr int kDkvKeys = 64;
+constexpr int kDkvTile = 64;
+struct DkvBlock {
+  bool found;
+  SeqRows qs, ks;
+  int j0;      // the block's first key
+  int t0, nt;  // tiles of queries that see it
+  int steps;   // nt, for every head of the group
+  int empty;   // not found: the tiles that are there
+};
+__device__ inline DkvBlock dkv_block(const VarlenBwdParams& p, int tile) {
+  const BwdBlock blk = find_block<kDkvKeys>(p.cu_k, p.num_seqs, p.total_k, tile);
+  DkvBlock b{};
+  b.found = blk.found;
+  b.empty = blk.first;
+  if (!blk.found) return b;
+  b.qs = seq_rows(p.cu_q, blk.seq, p.total_q);
+  b.ks = seq_rows(p.cu_k, blk.seq, p.total_k);
+  b.j0 = (tile - blk.first) * kDkvKeys;
+  b.t0 = p.causal ? max(b.j0 - (b.ks.len - b.qs.len), 0) / kDkvTile : 0;
+  b.nt = max((b.qs.len + kDkvTile - 1) / kDkvTile - b.t0, 0);
+  b.steps = b.nt * (p.num_heads / p.num_kv_heads);
+  return b;
+}
+// The first step of part n of `parts`.
+__device__ inline int part_begin(int steps, int n, int parts) {
+  return (int)((int64_t)steps * n / parts);
+}
+// Zeros for the rows outside the sequences, by the workgroups without a block.
+template <int D>
+__device__ inline void zero_rest_kv(const VarlenBwdParams& p, int kv, int nth, int of) {
+  zero_rest<D, 256>(p.cu_k, p.num_seqs, p.total_k, p.dk, p.dk_st, kv * p.dk_sh, nth, of);
+  zero_rest<D, 256>(p.cu_k, p.num_seqs, p.total_k, p.dv, p.dv_st, kv * p.dv_sh, nth, of);
+}
+
+// Two pairs of waves, 32 keys a pair.  Of a tile the first wave of a pair forms P and dS of the first 32 queries, the second of the
+// others; they exchange through LDS what the other one needs, and the first adds
+// up dv of all 64, the second dk.  So a wave holds one gradient beside its K and V
+// operands and has registers left for the next operands.  (A wave that adds up
+// both has none: at head_dim 128 its step of 32 queries took 3600 cycles for 1024
+// of matrix work, its operands requested one ahead.)
+//
+// kParts: the block's steps are shared among several workgroups, whose sums a
+// third launch adds up (varlen_dkv_sum_kernel).
+template <bool kBF16, int D, bool kParts>
+__global__ __launch_bounds__(256, D == 64 ? 3 : 2) void varlen_dkv_kernel(VarlenBwdParams p) {
+  constexpr int kWaves = 4, kThreads = 256;
+  constexpr int kTile = kDkvTile, ROWB = D * 2, TILE_B = kTile * ROWB, DS = D / 16, DT = D / 32;
+  constexpr int kAhead = D == 128 ? 8 : 4;
   __shared__ __align__(1024) char s_qd[2 * 2 * TILE_B];
-  __shared__ __align__(16) float s_st[2 * 2 * kBwdTile];  // a stage's lse, delta
-  __shared__ float s_top[8];
+  __shared__ __align__(16) float s_st[2 * 2 * kTile];  // a stage's lse, delta
+  __shared__ __align__(16) char s_ex[kWaves * 2048];   // what a wave hands over
+  __shared__ float s_top[kWaves];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int sub = wave >> 2;  // the wave's half of a tile's queries
   const int lane = threadIdx.x & 63, l32 = lane & 31, half = lane >> 5;
+  const int pair = wave >> 1, role = wave & 1;  // role 0: first 32 queries, dv
   // (Under a causal mask a sequence's earlier blocks are seen by more queries.)
-  const int tile = (int)(blockIdx.x / (unsigned)p.num_kv_heads);
   const int kv = (int)(blockIdx.x % (unsigned)p.num_kv_heads);
+  const int unit = (int)(blockIdx.x / (unsigned)p.num_kv_heads);
+  const int parts = kParts ? p.parts : 1;
+  const int tile = unit / parts, part = unit % parts;
   const int group = p.num_heads / p.num_kv_heads;
-  const BwdBlock blk = find_block(p.cu_k, p.num_seqs, p.total_k, tile);
+  const DkvBlock blk = dkv_block(p, tile);
   if (!blk.found) {
-    zero_rest<D, kDkvThreads>(p.cu_k, p.num_seqs, p.total_k, p.dk, p.dk_st, kv * p.dk_sh,
-                              tile - blk.first, p.k_tiles - blk.first);
-    zero_rest<D, kDkvThreads>(p.cu_k, p.num_seqs, p.total_k, p.dv, p.dv_st, kv * p.dv_sh,
-                              tile - blk.first, p.k_tiles - blk.first);
+    if constexpr (!kParts) zero_rest_kv<D>(p, kv, tile - blk.empty, p.k_tiles - blk.empty);
     return;
   }
-  const SeqRows qs = seq_rows(p.cu_q, blk.seq, p.total_q);
-  const SeqRows ks = seq_rows(p.cu_k, blk.seq, p.total_k);
-  const int j0 = (tile - blk.first) * kBwdRows;  // the block's first key
+  const SeqRows qs = blk.qs, ks = blk.ks;
+  const int j0 = blk.j0, t0 = blk.t0, nt = blk.nt;
   const int ahead = ks.len - qs.len;
-  const int t0 = p.causal ? max(j0 - ahead, 0) / kBwdTile : 0;  // the first tile of queries that see it
-  const int nt = max((qs.len + kBwdTile - 1) / kBwdTile - t0, 0);
-  const int steps = nt * group;
+  const int begin = kParts ? part_begin(blk.steps, part, parts) : 0;
+  const int steps = (kParts ? part_begin(blk.steps, part + 1, parts) : blk.steps) - begin;
+  if (kParts && steps == 0) return;
 
   const uint32_t lds = __builtin_amdgcn_readfirstlane(
       (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)s_qd);
   const uint32_t lds_st = __builtin_amdgcn_readfirstlane(
       (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)s_st);
-  // The tile requested next: head of the group, tile of its queries.
-  int gi = 0, ti = 0;
-  auto issue = [&](int stage) {
-    int at_lane = lane;  // (what follows from the lane is formed anew each step)
-    asm volatile("" : "+v"(at_lane));
-    const int head = kv * group + gi, base = (t0 + ti) * kBwdTile;
-    const uint32_t to = lds + (uint32_t)(stage * 2 * TILE_B);
-    stage_rows<D, 8>(p.q + (int64_t)qs.row * p.q_st + head * p.q_sh, p.q_st, base, qs.len, to, wave,
-                     at_lane);
-    stage_rows<D, 8>(p.dout + (int64_t)qs.row * p.do_st + head * p.do_sh, p.do_st, base, qs.len,
-                     to + TILE_B, wave, at_lane);
-    if (wave < 2) {
-      const int64_t w = (int64_t)head * p.total_q + qs.row + base + at_lane;
-      const float* const at = (wave == 0 ? p.lse : p.delta) + w;
-      const float* const none = wave == 0 ? &kInfRow : reinterpret_cast<const float*>(&kZeroRow);
-      dma4(base + at_lane < qs.len ? at : none,
-           lds_st + (uint32_t)((stage * 2 + wave) * kBwdTile * 4));
-    }
+  using Copy = TileCopy<D, kWaves, kTile>;
+  constexpr int kCopies = 2 * Copy::NI + 1;
+  const Copy copy(wave, lane);
+  // The tile requested next: head of the group, tile of its queries, its sources.
+  int gi = nt > 0 ? begin / nt : 0, ti = nt > 0 ? begin % nt : 0, last = 0;
+  const char *next_q = nullptr, *next_do = nullptr;
+  const float* next_st = nullptr;
+  auto next_tile = [&]() {
+    const int head = kv * group + gi, base = (t0 + ti) * kTile;
+    last = qs.len - 1 - base;
+    next_q = p.q + (int64_t)(qs.row + base) * p.q_st + head * p.q_sh;
+    next_do = p.dout + (int64_t)(qs.row + base) * p.do_st + head * p.do_sh;
+    next_st = (wave == 0 ? p.lse : p.delta) + (int64_t)head * p.total_q + qs.row + base;
     if (++ti == nt) {
       ti = 0;
       ++gi;
     }
   };
-  if (steps > 0) issue(0);
+  // Its copy n: lse (wave 0) or delta (wave 1), Q's, dO's.
+  auto issue = [&](int stage, int n) {
+    const uint32_t to = lds + (uint32_t)(stage * 2 * TILE_B);
+    if (n == 0) {
+      if (wave < 2)
+        dma4((uint32_t)min(lane, last) * 4, next_st,
+             lds_st + (uint32_t)((stage * 2 + wave) * kTile * 4));
+    } else if (n <= Copy::NI) {
+      copy.one(n - 1, next_q, p.q_st, last, to, wave);
+    } else {
+      copy.one(n - 1 - Copy::NI, next_do, p.do_st, last, to + TILE_B, wave);
+    }
+  };
+  if (steps > 0) {
+    next_tile();
+#pragma unroll
+    for (int n = 0; n < kCopies; ++n) issue(0, n);
+  }
 
-  const int wkey = j0 + 32 * (wave & 3), key = wkey + l32;
+  const int wkey = j0 + 32 * pair, key = wkey + l32;
   const int at = ks.row + min(key, ks.len - 1);
   uint4 kreg[DS], vreg[DS];
 #pragma unroll
@@ -481,92 +586,185 @@ __global__ __launch_bounds__(kDkvThreads, 2) void varlen_dkv_kernel(VarlenBwdPar
   if constexpr (!kBF16) {
     float top = 0.f;
     for (int g = 0; g < group; ++g)
-      for (int i = threadIdx.x; i < qs.len; i += kDkvThreads)
+      for (int i = threadIdx.x; i < qs.len; i += kThreads)
         top = fmaxf(top, p.top[(int64_t)(kv * group + g) * p.total_q + qs.row + i]);
     top = group_max<64>(top);
     if (lane == 0) s_top[wave] = top;
     __syncthreads();
 #pragma unroll
-    for (int w = 0; w < 8; ++w) top = fmaxf(top, s_top[w]);
+    for (int w = 0; w < kWaves; ++w) top = fmaxf(top, s_top[w]);
     const int e = top_exponent(top);
     lift = pow2(-e - kF16Lift);
     lower = pow2(e);
   }
 
   TileAt<D> ta(lane);
-  f32x16_t dk[DT], dv[DT];
+  f32x16_t acc[DT];  // dv (role 0) or dk
 #pragma unroll
-  for (int dt = 0; dt < DT; ++dt) dk[dt] = dv[dt] = f32x16_t{};
-  int tq = t0;  // the step's tile of queries
+  for (int dt = 0; dt < DT; ++dt) acc[dt] = f32x16_t{};
+  int tq = t0 + (nt > 0 ? begin % nt : 0);  // the step's tile of queries
   for (int it = 0; it < steps; ++it) {
     wait_vmcnt<0>();
     __syncthreads();
-    if (it + 1 < steps) issue((it + 1) & 1);
+    const bool more = it + 1 < steps;
+    const int to = (it + 1) & 1;
+    if (more) next_tile();
     const char* const sq = s_qd + (it & 1) * 2 * TILE_B;
     const char* const sd = sq + TILE_B;
-    const float* const st = s_st + (it & 1) * 2 * kBwdTile + 32 * sub + 4 * half;
-    const int i0 = tq * kBwdTile + 32 * sub;
+    const char* const sa = role == 0 ? sd : sq;  // dv += dO^T P, dk += Q^T dS
+    const int base = tq * kTile;
     if (++tq == t0 + nt) tq = t0;
-    // No query of these sees a key of the wave, or there are none.
-    if ((p.causal && i0 + 31 + ahead < wkey) || i0 >= qs.len) continue;
+    // Whether any of 32 queries sees a key of the pair.
+    auto seen = [&](int r) {
+      return base + 32 * r < qs.len && (!p.causal || base + 32 * r + 31 + ahead >= wkey);
+    };
     ta.rebuild();
-    f32x16_t s = {}, dp;
+    uint4 op[kAhead];  // A operands requested ahead
+    uint4 own[2];      // P (role 0) or dS of the wave's own queries, as B operands
+    const bool mine = seen(role);
+    if (mine) {
+      const int i0 = base + 32 * role;
+      const float* const st = s_st + (it & 1) * 2 * kTile + 32 * role + 4 * half;
+      // S and dP in turn, the next tile's copies between them.
+      auto request = [&](int n) {
+        if (n < 2 * DS) op[n % kAhead] = ta.a(n & 1 ? sd : sq, role, n / 2);
+      };
 #pragma unroll
-    for (int ds = 0; ds < DS; ++ds) s = mfma32<kBF16>(ta.a(sq, sub, ds), kreg[ds], s);
-    if (p.causal && i0 + ahead < wkey + 31) {
-      const int rel = key - ahead - i0 - 4 * half;  // query 8 (i / 4) + i % 4 sees it iff >= rel
+      for (int n = 0; n < kAhead; ++n) request(n);
+      f32x16_t s = {}, dp;
 #pragma unroll
-      for (int i = 0; i < 16; ++i)
-        if (8 * (i / 4) + i % 4 < rel) s[i] = -INFINITY;
+      for (int j = 0; j < 4; ++j) {
+        const f32x4_t d = *reinterpret_cast<const f32x4_t*>(st + kTile + 8 * j);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) dp[4 * j + i] = d[i];
+      }
+#pragma unroll
+      for (int n = 0; n < 2 * DS; ++n) {
+        if (n & 1)
+          dp = mfma32<kBF16>(op[n % kAhead], vreg[n / 2], dp);
+        else
+          s = mfma32<kBF16>(op[n % kAhead], kreg[n / 2], s);
+        request(n + kAhead);
+        constexpr int kEvery = (2 * DS) / (kCopies - 1);
+        if (more) {
+          if (n == 0) issue(to, 0);
+          if (n % kEvery == kEvery - 1) issue(to, 1 + n / kEvery);
+        }
+      }
+      // The first operands of the sums, past the exponentials.
+#pragma unroll
+      for (int n = 0; n < kAhead && n < 2 * DT; ++n) op[n] = ta.at(sa, role, n / DT, n % DT);
+      const bool edge = p.causal && i0 + ahead < wkey + 31;
+      if (edge || i0 + 32 > qs.len) {
+        // Query 8 (i / 4) + i % 4 sees the lane's key iff >= rel, and is there iff < end.
+        const int rel = edge ? key - ahead - i0 - 4 * half : 0, end = qs.len - i0 - 4 * half;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const int c = 8 * (i / 4) + i % 4;
+          if (c < rel || c >= end) s[i] = -INFINITY;
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const f32x4_t lse = *reinterpret_cast<const f32x4_t*>(st + 8 * j);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          s[4 * j + i] = fast_exp2(fmaf(s[4 * j + i], p.scale_log2, -lse[i]));
+          dp[4 * j + i] *= kBF16 ? s[4 * j + i] : s[4 * j + i] * lift;
+        }
+      }
+#pragma unroll
+      for (int hf = 0; hf < 2; ++hf) {
+        const uint4 pb = pack_b<kBF16>(s, hf), db = pack_b<kBF16>(dp, hf);
+        uint4* const over = reinterpret_cast<uint4*>(s_ex + wave * 2048 + hf * 1024 + lane * 16);
+        if (role == 0) {
+          own[hf] = pb;
+          *over = db;
+        } else {
+          own[hf] = db;
+          *over = pb;
+        }
+      }
+    } else if (more) {
+#pragma unroll
+      for (int n = 0; n < kCopies; ++n) issue(to, n);
     }
+    __syncthreads();
+    // The wave's own 32 queries, then its neighbour's.
+    if (mine) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const f32x4_t lse = *reinterpret_cast<const f32x4_t*>(st + 8 * j);
-      const f32x4_t d = *reinterpret_cast<const f32x4_t*>(st + kBwdTile + 8 * j);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float off = kBF16 ? lse[i] : lse[i] - (float)kF16Lift;
-        s[4 * j + i] = fast_exp2(fmaf(s[4 * j + i], p.scale_log2, -off));
-        dp[4 * j + i] = -d[i];
+      for (int n = 0; n < 2 * DT; ++n) {
+        acc[n % DT] = mfma32<kBF16>(op[n % kAhead], own[n / DT], acc[n % DT]);
+        if (n + kAhead < 2 * DT)
+          op[n % kAhead] = ta.at(sa, role, (n + kAhead) / DT, (n + kAhead) % DT);
       }
     }
+    if (seen(role ^ 1)) {
+      ta.rebuild();
+      uint4 b[2];
 #pragma unroll
-    for (int hf = 0; hf < 2; ++hf) {
-      const uint4 pb = pack_b<kBF16>(s, hf);
+      for (int hf = 0; hf < 2; ++hf)
+        b[hf] = lds_read16(s_ex, (wave ^ 1) * 2048 + hf * 1024 + lane * 16);
 #pragma unroll
-      for (int dt = 0; dt < DT; ++dt) dv[dt] = mfma32<kBF16>(ta.at(sd, sub, hf, dt), pb, dv[dt]);
-    }
-    ta.rebuild();
+      for (int n = 0; n < kAhead && n < 2 * DT; ++n) op[n] = ta.at(sa, role ^ 1, n / DT, n % DT);
 #pragma unroll
-    for (int ds = 0; ds < DS; ++ds) dp = mfma32<kBF16>(ta.a(sd, sub, ds), vreg[ds], dp);
-#pragma unroll
-    for (int i = 0; i < 16; ++i) dp[i] *= kBF16 ? s[i] : s[i] * lift;
-#pragma unroll
-    for (int hf = 0; hf < 2; ++hf) {
-      const uint4 db = pack_b<kBF16>(dp, hf);
-#pragma unroll
-      for (int dt = 0; dt < DT; ++dt) dk[dt] = mfma32<kBF16>(ta.at(sq, sub, hf, dt), db, dk[dt]);
+      for (int n = 0; n < 2 * DT; ++n) {
+        acc[n % DT] = mfma32<kBF16>(op[n % kAhead], b[n / DT], acc[n % DT]);
+        if (n + kAhead < 2 * DT)
+          op[n % kAhead] = ta.at(sa, role ^ 1, (n + kAhead) / DT, (n + kAhead) % DT);
+      }
     }
   }
-  // The halves' sums: the first half's waves write dk, the second's dv.
-  char* const s_x = s_qd + (wave & 3) * (64 * D / 2 * 4);
+  const float mul = role == 1 ? p.scale * lower : kBF16 ? 1.f : pow2(-kF16Lift);
+  if constexpr (kParts) {
+    float* const to = p.part + (((int64_t)unit * p.num_kv_heads + kv) * kWaves + wave) * (32 * D);
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        *reinterpret_cast<f32x4_t*>(to + ((dt * 4 + j) * 64 + lane) * 4) =
+            f32x4_t{acc[dt][4 * j] * mul, acc[dt][4 * j + 1] * mul, acc[dt][4 * j + 2] * mul,
+                    acc[dt][4 * j + 3] * mul};
+    return;
+  }
   __syncthreads();  // every wave is done with the tiles
-  if (sub == 0) put_acc<DT>(dv, s_x, lane);
-  __syncthreads();
-  if (sub == 1) add_acc<DT>(dv, s_x, lane);
-  __syncthreads();
-  if (sub == 1) put_acc<DT>(dk, s_x, lane);
-  __syncthreads();
-  if (sub == 0) add_acc<DT>(dk, s_x, lane);
-  __syncthreads();
-  char* const s_w = s_qd + wave * 32 * ROWB;
-  if (sub == 0)
-    write_rows<kBF16, D>(dk, p.scale * lower, s_w, p.dk + (int64_t)ks.row * p.dk_st + kv * p.dk_sh,
-                         p.dk_st, wkey, ks.len, lane);
-  else
-    write_rows<kBF16, D>(dv, kBF16 ? 1.f : pow2(-kF16Lift), s_w,
-                         p.dv + (int64_t)ks.row * p.dv_st + kv * p.dv_sh, p.dv_st, wkey, ks.len,
-                         lane);
+  write_dkv<kBF16, D>(p, acc, mul, s_qd + wave * 32 * ROWB, role, ks, kv, wkey, lane);
+}
+
+// Adds up the parts of a block's gradients, in their order: a wave the sums that
+// one wave of each part wrote.
+template <bool kBF16, int D>
+__global__ __launch_bounds__(256) void varlen_dkv_sum_kernel(VarlenBwdParams p) {
+  constexpr int DT = D / 32;
+  __shared__ __align__(16) char s_w[4 * 32 * D * 2];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63;
+  const int kv = (int)(blockIdx.x % (unsigned)p.num_kv_heads);
+  const int tile = (int)(blockIdx.x / (unsigned)p.num_kv_heads);
+  const DkvBlock blk = dkv_block(p, tile);
+  if (!blk.found) {
+    zero_rest_kv<D>(p, kv, tile - blk.empty, p.k_tiles - blk.empty);
+    return;
+  }
+  f32x16_t acc[DT];
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt) acc[dt] = f32x16_t{};
+  for (int n = 0; n < p.parts; ++n) {
+    if (part_begin(blk.steps, n, p.parts) == part_begin(blk.steps, n + 1, p.parts)) continue;
+    const float* const from =
+        p.part +
+        ((((int64_t)tile * p.parts + n) * p.num_kv_heads + kv) * 4 + wave) * (32 * D);
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const f32x4_t x = *reinterpret_cast<const f32x4_t*>(from + ((dt * 4 + j) * 64 + lane) * 4);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[dt][4 * j + i] += x[i];
+      }
+  }
+  write_dkv<kBF16, D>(p, acc, 1.f, s_w + wave * 32 * D * 2, wave & 1, blk.ks, kv,
+                      blk.j0 + 32 * (wave >> 1), lane);
 }
 
 // Both launches for one 16-bit type and head_dim, instantiated in
@@ -578,8 +776,14 @@ template <bool kBF16, int D>
 static void launch_varlen_backward_d(const VarlenBwdParams& p, hipStream_t st) {
   hipLaunchKernelGGL((varlen_dq_kernel<kBF16, D>), dim3((unsigned)p.q_tiles * p.num_heads),
                      dim3(kBwdThreads), 0, st, p);
-  hipLaunchKernelGGL((varlen_dkv_kernel<kBF16, D>), dim3((unsigned)p.k_tiles * p.num_kv_heads),
-                     dim3(kDkvThreads), 0, st, p);
+  const dim3 grid((unsigned)p.k_tiles * p.parts * p.num_kv_heads);
+  if (p.parts == 1) {
+    hipLaunchKernelGGL((varlen_dkv_kernel<kBF16, D, false>), grid, dim3(256), 0, st, p);
+    return;
+  }
+  hipLaunchKernelGGL((varlen_dkv_kernel<kBF16, D, true>), grid, dim3(256), 0, st, p);
+  hipLaunchKernelGGL((varlen_dkv_sum_kernel<kBF16, D>), dim3((unsigned)p.k_tiles * p.num_kv_heads),
+                     dim3(256), 0, st, p);
 }
 
 template <>
