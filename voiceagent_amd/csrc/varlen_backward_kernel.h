@@ -158,11 +158,16 @@ struct TileCopy {
     chunk = (uint32_t)(((lane % CPR) ^ bwd_swz<D>(row)) << 4);
   }
   // Copy i of the tile whose row 0 is at src (rows st bytes apart, row `last` the
-  // last one there is).
-  __device__ inline void one(int i, const char* src, int64_t st, int last, uint32_t lds,
-                             int wave) const {
-    const uint32_t r = (uint32_t)min(row + i * RPI, last);
-    dma16(r * (uint32_t)st + (chunk ^ (i << 4)), src, lds + (uint32_t)((wave * NI + i) * 1024));
+  // last one there is; row_st is row * st).
+  __device__ inline void one(int i, const char* src, uint32_t st, uint32_t row_st, int last,
+                             uint32_t lds, int wave) const {
+    if (last >= kRows - 1) {
+      dma16(row_st + (chunk ^ (i << 4)), src + (uint32_t)(i * RPI) * st,
+            lds + (uint32_t)((wave * NI + i) * 1024));
+    } else {
+      const uint32_t r = (uint32_t)min(row + i * RPI, last);
+      dma16(r * st + (chunk ^ (i << 4)), src, lds + (uint32_t)((wave * NI + i) * 1024));
+    }
   }
 };
 
@@ -295,14 +300,17 @@ __global__ __launch_bounds__(kBwdThreads, 2) void varlen_dq_kernel(VarlenBwdPara
       (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)s_kv);
   using Copy = TileCopy<D, 4, kTile>;
   const Copy copy(wave, lane);
+  const uint32_t k_row = (uint32_t)copy.row * (uint32_t)p.k_st;
+  const uint32_t v_row = (uint32_t)copy.row * (uint32_t)p.v_st;
   // Copy n of tile t: K's, then V's.
   auto issue = [&](int t, int n) {
     const uint32_t to = lds + (uint32_t)((t & 1) * 2 * TILE_B);
     const int last = ks.len - 1 - t * kTile;
     if (n < Copy::NI)
-      copy.one(n, kp + (int64_t)(t * kTile) * p.k_st, p.k_st, last, to, wave);
+      copy.one(n, kp + (int64_t)(t * kTile) * p.k_st, (uint32_t)p.k_st, k_row, last, to, wave);
     else
-      copy.one(n - Copy::NI, vp + (int64_t)(t * kTile) * p.v_st, p.v_st, last, to + TILE_B, wave);
+      copy.one(n - Copy::NI, vp + (int64_t)(t * kTile) * p.v_st, (uint32_t)p.v_st, v_row, last,
+               to + TILE_B, wave);
   };
   if (tiles > 0) {
 #pragma unroll
@@ -506,7 +514,7 @@ template <bool kBF16, int D, bool kParts>
 __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void varlen_dkv_kernel(VarlenBwdParams p) {
   constexpr int kWaves = 4, kThreads = 256;
   constexpr int kTile = kDkvTile, ROWB = D * 2, TILE_B = kTile * ROWB, DS = D / 16, DT = D / 32;
-  constexpr int kAhead = D == 128 ? 8 : 4;
+  constexpr int kAhead = D == 128 ? 6 : 4;
   __shared__ __align__(1024) char s_qd[2 * 2 * TILE_B];
   __shared__ __align__(16) float s_st[2 * 2 * kTile];  // a stage's lse, delta
   __shared__ __align__(16) char s_ex[kWaves * 2048];   // what a wave hands over
@@ -539,20 +547,29 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void varlen_dkv_kernel(Varlen
   using Copy = TileCopy<D, kWaves, kTile>;
   constexpr int kCopies = 2 * Copy::NI + 1;
   const Copy copy(wave, lane);
-  // The tile requested next: head of the group, tile of its queries, its sources.
-  int gi = nt > 0 ? begin / nt : 0, ti = nt > 0 ? begin % nt : 0, last = 0;
-  const char *next_q = nullptr, *next_do = nullptr;
-  const float* next_st = nullptr;
-  auto next_tile = [&]() {
-    const int head = kv * group + gi, base = (t0 + ti) * kTile;
-    last = qs.len - 1 - base;
-    next_q = p.q + (int64_t)(qs.row + base) * p.q_st + head * p.q_sh;
-    next_do = p.dout + (int64_t)(qs.row + base) * p.do_st + head * p.do_sh;
-    next_st = (wave == 0 ? p.lse : p.delta) + (int64_t)head * p.total_q + qs.row + base;
-    if (++ti == nt) {
-      ti = 0;
-      ++gi;
-    }
+  const uint32_t q_row = (uint32_t)copy.row * (uint32_t)p.q_st;
+  const uint32_t do_row = (uint32_t)copy.row * (uint32_t)p.do_st;
+  // The tile requested next: its number, the rows behind its first, its sources.
+  int ti = nt > 0 ? begin % nt : 0, last = 0;
+  const char *next_q, *next_do;
+  const float* next_st;  // lse (wave 0) or delta
+  {
+    const int head = kv * group + (nt > 0 ? begin / nt : 0), base = qs.row + (t0 + ti) * kTile;
+    next_q = p.q + (int64_t)base * p.q_st + head * p.q_sh;
+    next_do = p.dout + (int64_t)base * p.do_st + head * p.do_sh;
+    next_st = (wave == 0 ? p.lse : p.delta) + (int64_t)head * p.total_q + base;
+    last = qs.len - 1 - (t0 + ti) * kTile;
+  }
+  const int64_t q_step = kTile * p.q_st, do_step = kTile * p.do_st;
+  const int64_t q_head = p.q_sh - (nt - 1) * q_step, do_head = p.do_sh - (nt - 1) * do_step;
+  const int64_t st_head = (int64_t)p.total_q - (int64_t)(nt - 1) * kTile;
+  auto next_tile = [&]() {  // (behind a tile's copies)
+    const bool wrap = ++ti == nt;  // on to the next head's first tile
+    next_q += wrap ? q_head : q_step;
+    next_do += wrap ? do_head : do_step;
+    next_st += wrap ? st_head : kTile;
+    last = wrap ? qs.len - 1 - t0 * kTile : last - kTile;
+    ti = wrap ? 0 : ti;
   };
   // Its copy n: lse (wave 0) or delta (wave 1), Q's, dO's.
   auto issue = [&](int stage, int n) {
@@ -562,13 +579,12 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void varlen_dkv_kernel(Varlen
         dma4((uint32_t)min(lane, last) * 4, next_st,
              lds_st + (uint32_t)((stage * 2 + wave) * kTile * 4));
     } else if (n <= Copy::NI) {
-      copy.one(n - 1, next_q, p.q_st, last, to, wave);
+      copy.one(n - 1, next_q, (uint32_t)p.q_st, q_row, last, to, wave);
     } else {
-      copy.one(n - 1 - Copy::NI, next_do, p.do_st, last, to + TILE_B, wave);
+      copy.one(n - 1 - Copy::NI, next_do, (uint32_t)p.do_st, do_row, last, to + TILE_B, wave);
     }
   };
   if (steps > 0) {
-    next_tile();
 #pragma unroll
     for (int n = 0; n < kCopies; ++n) issue(0, n);
   }
@@ -598,36 +614,57 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void varlen_dkv_kernel(Varlen
     lower = pow2(e);
   }
 
-  TileAt<D> ta(lane);
+  // The lane's LDS addresses: of the 8 elements of step n of S's rows (dO's for dP
+  // lie TILE_B further on), and of the transposed reads for the wave's gradient
+  // (role 0: dO, dv), whose other 32 rows differ in one bit.  In registers, with a
+  // stage's offset in the instruction: formed for each read they took 600 cycles
+  // of a step.
+  static_assert((32 * ROWB & (32 * ROWB - 1)) == 0 && 64 * ROWB <= TILE_B, "the rows' bit");
+  int a_at[DS], t_lo[DT], t_hi[DT];
+  {
+    const TileAt<D> ta(lane);
+#pragma unroll
+    for (int n = 0; n < DS; ++n) a_at[n] = role * 32 * ROWB + ta.row + (ta.row0 ^ (n << 5));
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) {
+      const int of = role * 32 * ROWB + (role == 0 ? TILE_B : 0);
+      t_lo[dt] = of + ta.tr + (ta.tr0 ^ (dt << 6));
+      t_hi[dt] = of + ta.tr + 8 * ROWB + (ta.tr0 ^ (D == 128 ? 32 : 16) ^ (dt << 6));
+    }
+  }
   f32x16_t acc[DT];  // dv (role 0) or dk
 #pragma unroll
   for (int dt = 0; dt < DT; ++dt) acc[dt] = f32x16_t{};
-  int tq = t0 + (nt > 0 ? begin % nt : 0);  // the step's tile of queries
-  for (int it = 0; it < steps; ++it) {
+  int tq = nt > 0 ? begin % nt : 0;  // the step's tile of queries, from t0
+  const int st_at = 32 * role + 4 * half;
+  auto step = [&](auto stage_c, int it) {
+    constexpr int kStage = decltype(stage_c)::value;
+    constexpr int kAt = kStage * 2 * TILE_B;
     wait_vmcnt<0>();
     __syncthreads();
     const bool more = it + 1 < steps;
-    const int to = (it + 1) & 1;
     if (more) next_tile();
-    const char* const sq = s_qd + (it & 1) * 2 * TILE_B;
-    const char* const sd = sq + TILE_B;
-    const char* const sa = role == 0 ? sd : sq;  // dv += dO^T P, dk += Q^T dS
-    const int base = tq * kTile;
-    if (++tq == t0 + nt) tq = t0;
+    const int base = (t0 + tq) * kTile;
+    if (++tq == nt) tq = 0;
     // Whether any of 32 queries sees a key of the pair.
     auto seen = [&](int r) {
       return base + 32 * r < qs.len && (!p.causal || base + 32 * r + 31 + ahead >= wkey);
     };
-    ta.rebuild();
     uint4 op[kAhead];  // A operands requested ahead
-    uint4 own[2];      // P (role 0) or dS of the wave's own queries, as B operands
+    auto sums = [&](int n, int other) {  // operand n of the sum over 32 queries
+      const int x = other * 32 * ROWB;
+      const uint2 lo = __builtin_bit_cast(uint2, lds_read_tr(s_qd + kAt + n / DT * 16 * ROWB, t_lo[n % DT] ^ x));
+      const uint2 hi = __builtin_bit_cast(uint2, lds_read_tr(s_qd + kAt + n / DT * 16 * ROWB, t_hi[n % DT] ^ x));
+      return make_uint4(lo.x, lo.y, hi.x, hi.y);
+    };
+    uint4 own[2];  // P (role 0) or dS of the wave's own queries, as B operands
     const bool mine = seen(role);
     if (mine) {
       const int i0 = base + 32 * role;
-      const float* const st = s_st + (it & 1) * 2 * kTile + 32 * role + 4 * half;
+      const float* const st = s_st + kStage * 2 * kTile + st_at;
       // S and dP in turn, the next tile's copies between them.
       auto request = [&](int n) {
-        if (n < 2 * DS) op[n % kAhead] = ta.a(n & 1 ? sd : sq, role, n / 2);
+        if (n < 2 * DS) op[n % kAhead] = lds_read16(s_qd + kAt + (n & 1) * TILE_B, a_at[n / 2]);
       };
 #pragma unroll
       for (int n = 0; n < kAhead; ++n) request(n);
@@ -647,13 +684,13 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void varlen_dkv_kernel(Varlen
         request(n + kAhead);
         constexpr int kEvery = (2 * DS) / (kCopies - 1);
         if (more) {
-          if (n == 0) issue(to, 0);
-          if (n % kEvery == kEvery - 1) issue(to, 1 + n / kEvery);
+          if (n == 0) issue(kStage ^ 1, 0);
+          if (n % kEvery == kEvery - 1) issue(kStage ^ 1, 1 + n / kEvery);
         }
       }
       // The first operands of the sums, past the exponentials.
 #pragma unroll
-      for (int n = 0; n < kAhead && n < 2 * DT; ++n) op[n] = ta.at(sa, role, n / DT, n % DT);
+      for (int n = 0; n < kAhead && n < 2 * DT; ++n) op[n] = sums(n, 0);
       const bool edge = p.causal && i0 + ahead < wkey + 31;
       if (edge || i0 + 32 > qs.len) {
         // Query 8 (i / 4) + i % 4 sees the lane's key iff >= rel, and is there iff < end.
@@ -687,7 +724,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void varlen_dkv_kernel(Varlen
       }
     } else if (more) {
 #pragma unroll
-      for (int n = 0; n < kCopies; ++n) issue(to, n);
+      for (int n = 0; n < kCopies; ++n) issue(kStage ^ 1, n);
     }
     __syncthreads();
     // The wave's own 32 queries, then its neighbour's.
@@ -695,25 +732,26 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void varlen_dkv_kernel(Varlen
 #pragma unroll
       for (int n = 0; n < 2 * DT; ++n) {
         acc[n % DT] = mfma32<kBF16>(op[n % kAhead], own[n / DT], acc[n % DT]);
-        if (n + kAhead < 2 * DT)
-          op[n % kAhead] = ta.at(sa, role, (n + kAhead) / DT, (n + kAhead) % DT);
+        if (n + kAhead < 2 * DT) op[n % kAhead] = sums(n + kAhead, 0);
       }
     }
     if (seen(role ^ 1)) {
-      ta.rebuild();
       uint4 b[2];
 #pragma unroll
       for (int hf = 0; hf < 2; ++hf)
         b[hf] = lds_read16(s_ex, (wave ^ 1) * 2048 + hf * 1024 + lane * 16);
 #pragma unroll
-      for (int n = 0; n < kAhead && n < 2 * DT; ++n) op[n] = ta.at(sa, role ^ 1, n / DT, n % DT);
+      for (int n = 0; n < kAhead && n < 2 * DT; ++n) op[n] = sums(n, 1);
 #pragma unroll
       for (int n = 0; n < 2 * DT; ++n) {
         acc[n % DT] = mfma32<kBF16>(op[n % kAhead], b[n / DT], acc[n % DT]);
-        if (n + kAhead < 2 * DT)
-          op[n % kAhead] = ta.at(sa, role ^ 1, (n + kAhead) / DT, (n + kAhead) % DT);
+        if (n + kAhead < 2 * DT) op[n % kAhead] = sums(n + kAhead, 1);
       }
     }
+  };
+  for (int it = 0; it < steps; it += 2) {
+    step(std::integral_constant<int, 0>{}, it);
+    if (it + 1 < steps) step(std::integral_constant<int, 1>{}, it + 1);
   }
   const float mul = role == 1 ? p.scale * lower : kBF16 ? 1.f : pow2(-kF16Lift);
   if constexpr (kParts) {
