@@ -133,3 +133,34 @@ def test_store_rope_and_prologue_decode_agree_on_both_paths(dev, python_path):
     torch.cuda.synchronize()
     for a, b in zip(*res):
         assert torch.equal(a, b)
+
+
+def test_training_fast_and_python_paths_agree(dev, python_path):
+    """The gradients and the rotation through both paths, bit for bit; a call that the fast path
+    does not take leaves the error to the wrapper."""
+    g = torch.Generator(device=dev).manual_seed(3)
+    lens, hq, hkv, d = [70, 1, 33], 4, 2, 64
+    T = sum(lens)
+    make = lambda h, dt=torch.bfloat16: torch.randn(T, h, d, device=dev, generator=g).to(dt)  # noqa: E731
+    cu = torch.tensor([0, 70, 71, 104], dtype=torch.int32, device=dev)
+    q, dout, out, k, v = make(hq), make(hq), make(hq), make(hkv), make(hkv)
+    w = (torch.rand(d, device=dev, generator=g) + 0.5).to(torch.bfloat16)
+    table = oracle.rope_cache(d, 128, 1e4).to(dev)
+    pos = torch.arange(T, device=dev)
+    pro = ops.QKPrologue(w, w, 1e-6, table, pos)
+
+    def run():
+        return (*ops.varlen_attention_backward(dout, q, k, v, out, cu, cu, 70, 70, scale=0.125,
+                                               causal=True),
+                *ops.qk_norm_rope_backward(dout, k, q, v, pro),
+                *ops.rotary_embedding(q, k, table[:, None, :32], pos, interleaved=True,
+                                      inverse=True))
+
+    first = run()
+    assert ops._fast_calls().varlen_attention_backward(
+        dout, q, k.float(), v, out, cu, cu, 0.125, True, 0, 0)[0] == ops._FAST_NOT_TAKEN
+    with pytest.raises(ops.AttentionArgumentError):
+        ops.rotary_embedding(q, k.float(), table, pos)
+    python_path()
+    for a, b in zip(first, run()):
+        assert torch.equal(a, b)

@@ -113,9 +113,16 @@ def test_attention_gradient_without_rows_is_no_call():
     assert N.lib().va_varlen_attention_backward_workspace_bytes(ctypes.byref(a)) == 0
     a = _bwd_args()
     size = N.lib().va_varlen_attention_backward_workspace_bytes
-    assert size(ctypes.byref(a)) == 2 * 4 * 8 * 4
+    assert size(ctypes.byref(a)) == 256  # lse and delta of 8 rows of 4 heads, rounded up
     a.dtype = N.VA_F16
-    assert size(ctypes.byref(a)) == 3 * 4 * 8 * 4
+    assert size(ctypes.byref(a)) == 512  # and the rows' largest |dout|
+    # Few blocks of keys that many queries see: their sums, a share of the queries each.
+    a.total_q = a.total_k = 2000
+    plain = 3 * 4 * 2000 * 4
+    parts, left = divmod(size(ctypes.byref(a)) - (plain + 255) // 256 * 256, (2000 // 64 + 2) * 2 * 2 * 64 * 64 * 4)
+    assert left == 0 and 2 <= parts <= 16
+    a.total_k = 0
+    assert size(ctypes.byref(a)) == (plain + 255) // 256 * 256
 
 
 def test_cpu_tensors_are_refused():

@@ -1,5 +1,6 @@
 // Host fast path of ops.paged_decode, ops.varlen_attention, ops.store_kvcache,
-// ops.qk_norm_rope, ops.load_kvcache and ops.batch_metadata.
+// ops.qk_norm_rope, ops.load_kvcache, ops.batch_metadata, ops.rotary_embedding
+// and the gradients ops.varlen_attention_backward and ops.qk_norm_rope_backward.
 //
 // The Python wrappers validate every argument and fill a ctypes struct on
 // each call, about 10 us of host time, which an eager engine step pays once
@@ -51,6 +52,18 @@ DecodeMx4Fn g_decode_mx4 = nullptr;
 DecodeWsFn g_decode_mx4_ws = nullptr;
 VarlenMx4Fn g_varlen_mx4 = nullptr;
 BatchFn g_batch = nullptr;
+
+// The training pass, and rotary positions alone.
+using VarlenBwdFn = int (*)(const va_varlen_bwd_args*, void*);
+using VarlenBwdWsFn = size_t (*)(const va_varlen_bwd_args*);
+using RopeBwdFn = int (*)(const va_qk_norm_rope_bwd_args*, void*);
+using RopeBwdWsFn = size_t (*)(const va_qk_norm_rope_bwd_args*);
+using RotaryFn = int (*)(const va_rotary_args*, void*);
+VarlenBwdFn g_varlen_bwd = nullptr;
+VarlenBwdWsFn g_varlen_bwd_ws = nullptr;
+RopeBwdFn g_rope_bwd = nullptr;
+RopeBwdWsFn g_rope_bwd_ws = nullptr;
+RotaryFn g_rotary = nullptr;
 
 constexpr int64_t kNotTaken = -1000;
 
@@ -692,6 +705,189 @@ int64_t qk_norm_rope(const at::Tensor& q, const at::Tensor& k, const at::Tensor&
   return g_rope(&a, reinterpret_cast<void*>(static_cast<intptr_t>(stream)));
 }
 
+// Rows [tokens, heads, head_dim] on `device`, contiguous in their last dimension.
+bool rows_on(const at::Tensor& t, int64_t device) {
+  return on(t, device) && t.dim() == 3 && t.stride(2) == 1 && fits_i32(t.size(0)) &&
+         fits_i32(t.size(1)) && fits_i32(t.size(2));
+}
+// Their strides (the wrappers' _row_strides: a dimension of one has none).
+int64_t tok_stride(const at::Tensor& t) { return t.size(0) > 1 ? t.stride(0) : 0; }
+int64_t head_stride(const at::Tensor& t) { return t.size(1) > 1 ? t.stride(1) : 0; }
+at::Tensor rows_like(const at::Tensor& t) { return at::empty(t.sizes(), t.options()); }
+
+// ops.varlen_attention_backward without given gradients: (status, [dq, dk, dv]).
+std::tuple<int64_t, std::vector<at::Tensor>> varlen_attention_backward(
+    const at::Tensor& dout, const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
+    const at::Tensor& out, const at::Tensor& cu_q, const at::Tensor& cu_k, double scale,
+    bool causal, int64_t device, int64_t stream) {
+  const std::tuple<int64_t, std::vector<at::Tensor>> none{kNotTaken, {}};
+  if (g_varlen_bwd == nullptr || !rows_on(dout, device) || !rows_on(q, device) ||
+      !rows_on(k, device) || !rows_on(v, device) || !rows_on(out, device) || !on(cu_q, device) ||
+      !on(cu_k, device))
+    return none;
+  const auto t = q.scalar_type();
+  if ((t != at::kBFloat16 && t != at::kHalf) || dout.scalar_type() != t || k.scalar_type() != t ||
+      v.scalar_type() != t || out.scalar_type() != t || out.sizes() != q.sizes() ||
+      dout.sizes() != q.sizes() || v.sizes() != k.sizes() || k.size(2) != q.size(2) ||
+      k.size(1) <= 0 || q.size(1) <= 0 || q.size(1) % k.size(1) != 0)
+    return none;
+  if (cu_q.scalar_type() != at::kInt || cu_k.scalar_type() != at::kInt || cu_q.dim() != 1 ||
+      cu_q.numel() < 2 || cu_k.sizes() != cu_q.sizes() || !cu_q.is_contiguous() ||
+      !cu_k.is_contiguous() || !fits_i32(cu_q.numel()))
+    return none;
+  const std::vector<at::Tensor> g{rows_like(q), rows_like(k), rows_like(k)};
+  va_varlen_bwd_args a{};
+  a.struct_size = sizeof(a);
+  a.dtype = dtype_code(t);
+  a.q = q.data_ptr();
+  a.q_stride_tok = tok_stride(q);
+  a.q_stride_head = head_stride(q);
+  a.k = k.data_ptr();
+  a.k_stride_tok = tok_stride(k);
+  a.k_stride_head = head_stride(k);
+  a.v = v.data_ptr();
+  a.v_stride_tok = tok_stride(v);
+  a.v_stride_head = head_stride(v);
+  a.out = out.data_ptr();
+  a.out_stride_tok = tok_stride(out);
+  a.out_stride_head = head_stride(out);
+  a.dout = dout.data_ptr();
+  a.dout_stride_tok = tok_stride(dout);
+  a.dout_stride_head = head_stride(dout);
+  a.dq = g[0].data_ptr();
+  a.dq_stride_tok = tok_stride(g[0]);
+  a.dq_stride_head = head_stride(g[0]);
+  a.dk = g[1].data_ptr();
+  a.dk_stride_tok = tok_stride(g[1]);
+  a.dk_stride_head = head_stride(g[1]);
+  a.dv = g[2].data_ptr();
+  a.dv_stride_tok = tok_stride(g[2]);
+  a.dv_stride_head = head_stride(g[2]);
+  a.cu_seqlens_q = static_cast<const int32_t*>(cu_q.data_ptr());
+  a.cu_seqlens_k = static_cast<const int32_t*>(cu_k.data_ptr());
+  a.num_seqs = (int32_t)(cu_q.numel() - 1);
+  a.total_q = (int32_t)q.size(0);
+  a.total_k = (int32_t)k.size(0);
+  a.num_heads = (int32_t)q.size(1);
+  a.num_kv_heads = (int32_t)k.size(1);
+  a.head_dim = (int32_t)q.size(2);
+  a.causal = causal ? 1 : 0;
+  a.scale = (float)scale;
+  const at::Tensor ws = at::empty({(int64_t)g_varlen_bwd_ws(&a)}, q.options().dtype(at::kByte));
+  a.workspace = ws.data_ptr();
+  a.workspace_bytes = (size_t)ws.numel();
+  return {g_varlen_bwd(&a, reinterpret_cast<void*>(static_cast<intptr_t>(stream))), g};
+}
+
+// ops.qk_norm_rope_backward of both sides, without given gradients: (status,
+// [dq, dk, dq_norm_weight, dk_norm_weight]).
+std::tuple<int64_t, std::vector<at::Tensor>> qk_norm_rope_backward(
+    const at::Tensor& dq_out, const at::Tensor& dk_out, const at::Tensor& q, const at::Tensor& k,
+    const at::Tensor& q_w, const at::Tensor& k_w, double eps, const at::Tensor& cos_sin,
+    const at::Tensor& positions, int64_t device, int64_t stream) {
+  const std::tuple<int64_t, std::vector<at::Tensor>> none{kNotTaken, {}};
+  if (g_rope_bwd == nullptr || !rows_on(dq_out, device) || !rows_on(dk_out, device) ||
+      !rows_on(q, device) || !rows_on(k, device))
+    return none;
+  const auto t = k.scalar_type();
+  const int64_t T = k.size(0), d = k.size(2);
+  if (dtype_code(t) < 0 || q.scalar_type() != t || dq_out.scalar_type() != t ||
+      dk_out.scalar_type() != t || q.size(0) != T || q.size(2) != d ||
+      dq_out.sizes() != q.sizes() || dk_out.sizes() != k.sizes() || q.size(1) <= 0)
+    return none;
+  va_qk_norm_rope_bwd_args a{};
+  a.struct_size = sizeof(a);
+  if (!fill_prologue(q_w, k_w, eps, cos_sin, positions, d, T, device, &a.prologue)) return none;
+  const std::vector<at::Tensor> g{rows_like(q), rows_like(k), at::empty({d}, q_w.options()),
+                                  at::empty({d}, k_w.options())};
+  a.dtype = dtype_code(t);
+  a.dq_out = dq_out.data_ptr();
+  a.dq_out_stride_tok = tok_stride(dq_out);
+  a.dq_out_stride_head = head_stride(dq_out);
+  a.dk_out = dk_out.data_ptr();
+  a.dk_out_stride_tok = tok_stride(dk_out);
+  a.dk_out_stride_head = head_stride(dk_out);
+  a.q = q.data_ptr();
+  a.q_stride_tok = tok_stride(q);
+  a.q_stride_head = head_stride(q);
+  a.k = k.data_ptr();
+  a.k_stride_tok = tok_stride(k);
+  a.k_stride_head = head_stride(k);
+  a.dq = g[0].data_ptr();
+  a.dq_stride_tok = tok_stride(g[0]);
+  a.dq_stride_head = head_stride(g[0]);
+  a.dk = g[1].data_ptr();
+  a.dk_stride_tok = tok_stride(g[1]);
+  a.dk_stride_head = head_stride(g[1]);
+  a.dq_weight = g[2].data_ptr();
+  a.dk_weight = g[3].data_ptr();
+  a.num_tokens = (int32_t)T;
+  a.num_heads = (int32_t)q.size(1);
+  a.num_kv_heads = (int32_t)k.size(1);
+  a.head_dim = (int32_t)d;
+  const at::Tensor ws = at::empty({(int64_t)g_rope_bwd_ws(&a)}, q.options().dtype(at::kByte));
+  a.workspace = ws.data_ptr();
+  a.workspace_bytes = (size_t)ws.numel();
+  return {g_rope_bwd(&a, reinterpret_cast<void*>(static_cast<intptr_t>(stream))), g};
+}
+
+// ops.rotary_embedding of q and k, without given outputs: (status, [q, k]).
+std::tuple<int64_t, std::vector<at::Tensor>> rotary(const at::Tensor& q, const at::Tensor& k,
+                                                    const at::Tensor& cos_sin,
+                                                    const at::Tensor& positions, bool interleaved,
+                                                    bool inverse, int64_t device, int64_t stream) {
+  const std::tuple<int64_t, std::vector<at::Tensor>> none{kNotTaken, {}};
+  if (g_rotary == nullptr || !rows_on(q, device) || !rows_on(k, device) || !on(cos_sin, device) ||
+      !on(positions, device))
+    return none;
+  const at::Tensor cs = cos_sin.dim() == 3 && cos_sin.size(1) == 1 ? cos_sin.select(1, 0) : cos_sin;
+  if (q.scalar_type() != k.scalar_type() || dtype_code(q.scalar_type()) < 0 ||
+      k.size(0) != q.size(0) || k.size(2) != q.size(2) || cs.dim() != 2 ||
+      cs.scalar_type() != at::kFloat || cs.stride(1) != 1 || cs.size(1) <= 0 ||
+      cs.size(1) > q.size(2) || cs.size(1) % 2 != 0 || !fits_i32(cs.size(0)) ||
+      positions.dim() != 1 || positions.numel() < q.size(0) || !positions.is_contiguous() ||
+      index_code(positions.scalar_type()) < 0)
+    return none;
+  const std::vector<at::Tensor> out{rows_like(q), rows_like(k)};
+  va_rotary_args a{};
+  a.struct_size = sizeof(a);
+  a.dtype = dtype_code(q.scalar_type());
+  a.q = q.data_ptr();
+  a.q_stride_tok = tok_stride(q);
+  a.q_stride_head = head_stride(q);
+  a.k = k.data_ptr();
+  a.k_stride_tok = tok_stride(k);
+  a.k_stride_head = head_stride(k);
+  a.q_out = out[0].data_ptr();
+  a.q_out_stride_tok = tok_stride(out[0]);
+  a.q_out_stride_head = head_stride(out[0]);
+  a.k_out = out[1].data_ptr();
+  a.k_out_stride_tok = tok_stride(out[1]);
+  a.k_out_stride_head = head_stride(out[1]);
+  a.num_tokens = (int32_t)q.size(0);
+  a.num_heads = (int32_t)q.size(1);
+  a.num_kv_heads = (int32_t)k.size(1);
+  a.head_dim = (int32_t)q.size(2);
+  a.rotary_dim = (int32_t)cs.size(1);
+  a.interleaved = interleaved;
+  a.inverse = inverse;
+  a.cos_sin_cache = static_cast<const float*>(cs.data_ptr());
+  a.cos_sin_stride = cs.stride(0);
+  a.max_position = (int32_t)cs.size(0);
+  a.positions_dtype = index_code(positions.scalar_type());
+  a.positions = positions.data_ptr();
+  return {g_rotary(&a, reinterpret_cast<void*>(static_cast<intptr_t>(stream))), out};
+}
+
+void set_train_entries(uintptr_t varlen_bwd, uintptr_t varlen_bwd_ws, uintptr_t rope_bwd,
+                       uintptr_t rope_bwd_ws, uintptr_t rotary_fn) {
+  g_varlen_bwd = reinterpret_cast<VarlenBwdFn>(varlen_bwd);
+  g_varlen_bwd_ws = reinterpret_cast<VarlenBwdWsFn>(varlen_bwd_ws);
+  g_rope_bwd = reinterpret_cast<RopeBwdFn>(rope_bwd);
+  g_rope_bwd_ws = reinterpret_cast<RopeBwdWsFn>(rope_bwd_ws);
+  g_rotary = reinterpret_cast<RotaryFn>(rotary_fn);
+}
+
 // ops.paged_decode over a 16-bit, fp32 or FP8 pool; ..._mx4: with an MXFP4
 // pool's scale tensors.  The same for ops.varlen_attention.
 using Opt = const c10::optional<at::Tensor>&;
@@ -757,4 +953,8 @@ PYBIND11_MODULE(_fast_calls, m) {
   m.def("store_kvcache_mx4", &store_kvcache_mx4);
   m.def("load_kvcache_mx4", &load_kvcache_mx4);
   m.def("batch_metadata", &batch_metadata);
+  m.def("set_train_entries", &set_train_entries);
+  m.def("varlen_attention_backward", &varlen_attention_backward);
+  m.def("qk_norm_rope_backward", &qk_norm_rope_backward);
+  m.def("rotary", &rotary);
 }

@@ -492,6 +492,17 @@ def qk_norm_rope_backward(
     roundings to the element type count as the identity.  ``dq`` / ``dk`` may be
     dq_out / dk_out or q / k themselves.  ``dq_out`` and ``q`` None: the keys
     alone (dq and dq_norm_weight are then None).  Two launches, no atomics."""
+    if q is not None and dq_out is not None and dq is None and dk is None:
+        fast, index = _fast_on(k, LAYOUT_NHD)
+        if fast is not None:
+            rc, made = fast.qk_norm_rope_backward(
+                dq_out, dk_out, q, k, prologue.q_norm_weight, prologue.k_norm_weight,
+                float(prologue.eps), prologue.cos_sin_cache, prologue.positions, index,
+                _raw_stream(index))
+            if rc == 0:
+                return tuple(made)
+            if _FAST_NOT_TAKEN < rc < 0:
+                N.check("va_qk_norm_rope_backward", rc)
     _require((q is None) == (dq_out is None), "q and dq_out must be given together")
     device = _check_gpu(dq_out, dk_out, q, k, dq, dk, prologue.q_norm_weight,
                         prologue.k_norm_weight, prologue.cos_sin_cache, prologue.positions)
@@ -605,6 +616,15 @@ def rotary_embedding(
     if (q_out is None and k_out is None and torch.is_grad_enabled() and
             ((q is not None and q.requires_grad) or (k is not None and k.requires_grad))):
         return _Rotary.apply(q, k, cos_sin_cache, positions, interleaved, inverse)
+    if q is not None and k is not None and q_out is None and k_out is None:
+        fast, index = _fast_on(q, LAYOUT_NHD)
+        if fast is not None:
+            rc, made = fast.rotary(q, k, cos_sin_cache, positions, bool(interleaved),
+                                   bool(inverse), index, _raw_stream(index))
+            if rc == 0:
+                return made[0], made[1]
+            if _FAST_NOT_TAKEN < rc < 0:
+                N.check("va_rotary", rc)
     device = _check_gpu(q, k, cos_sin_cache, positions, q_out, k_out)
     _require(q is not None or k is not None, "q or k must be given")
     like = k if q is None else q
@@ -726,7 +746,7 @@ _VARLEN_BWD_ARGS_SIZE = ctypes.sizeof(N.VarlenBwdArgs)
 # Host fast path (csrc/host/fast_calls.cpp, the ``_fast_calls`` module next
 # to the library): the same checks and the same C-ABI call in C++, for the
 # common paged_decode / varlen_attention / store_kvcache / qk_norm_rope /
-# load_kvcache / batch_metadata calls.  It launches nothing for a
+# load_kvcache / batch_metadata / rotary_embedding calls and the gradients.  It launches nothing for a
 # call it does not take, and the Python path below then runs (and raises the
 # error for a bad argument), so results and errors are the same either way.
 _FAST_NOT_TAKEN = -1000
@@ -764,6 +784,11 @@ def _fast_calls():
                                 addr(lib.va_paged_decode_mx4),
                                 addr(lib.va_paged_decode_mx4_workspace_bytes),
                                 addr(lib.va_varlen_attention_mx4), addr(lib.va_batch_metadata))
+            mod.set_train_entries(addr(lib.va_varlen_attention_backward),
+                                  addr(lib.va_varlen_attention_backward_workspace_bytes),
+                                  addr(lib.va_qk_norm_rope_backward),
+                                  addr(lib.va_qk_norm_rope_backward_workspace_bytes),
+                                  addr(lib.va_rotary))
             _FAST = mod
     return _FAST
 _POOLS: dict[tuple, N.KvPool] = {}  # pool descriptions by tensor identity and geometry
@@ -1270,8 +1295,18 @@ def varlen_attention_backward(
     call's arguments, and not read).  Rows outside every sequence, queries that
     see no key and keys that no query sees get zeros.  ``dq``, ``dk``, ``dv``:
     tensors to write into (views of one buffer, say); they may not overlap the
-    inputs.  Two launches on the current stream, no atomics: the results repeat
-    bit for bit."""
+    inputs.  Two or three launches on the current stream, no atomics: the
+    results repeat bit for bit."""
+    if dq is None and dk is None and dv is None:
+        fast, index = _fast_on(q, LAYOUT_NHD)
+        if fast is not None:
+            rc, made = fast.varlen_attention_backward(dout, q, k, v, out, cu_seqlens_q,
+                                                      cu_seqlens_k, float(scale), bool(causal),
+                                                      index, _raw_stream(index))
+            if rc == 0:
+                return tuple(made)
+            if _FAST_NOT_TAKEN < rc < 0:
+                N.check("va_varlen_attention_backward", rc)
     device = _check_gpu(dout, q, k, v, out, cu_seqlens_q, cu_seqlens_k, dq, dk, dv)
     _require(q.dim() == 3, "q must be [total_q, num_heads, head_dim]")
     _require(out.shape == q.shape and dout.shape == q.shape, "out and dout must match q")
