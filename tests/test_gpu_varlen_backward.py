@@ -76,6 +76,17 @@ def test_many_sequences(dev):
         _check(got, G.varlen_attention_backward(dout, q, k, v, out, cu_q, cu_k, 0.125, causal))
 
 
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("dtype,d", [(torch.bfloat16, 128), (torch.float16, 64)])
+def test_enough_blocks_to_fill_the_chip(dev, dtype, d, causal):
+    # (The cases above leave most of it idle, where blocks are smaller and their work shared.)
+    lens_q = [1, 31, 64, 65, 97, 127, 128, 129, 130, 161, 190, 192, 193, 255, 256, 257, 258]
+    lens_k = [n + e for n, e in zip(lens_q, [0, 3, -7, 64, 0, 129] * 3)]
+    q, k, v, dout, out, cu_q, cu_k = _inputs(lens_q, lens_k, 16, 16, d, dtype, 16)
+    got = _call(dev, q, k, v, dout, out, cu_q, cu_k, d ** -0.5, causal)
+    _check(got, G.varlen_attention_backward(dout, q, k, v, out, cu_q, cu_k, d ** -0.5, causal))
+
+
 @pytest.mark.parametrize("size", [2.0 ** -20, 1.0, 2.0 ** 8])
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
 def test_small_and_large_gradients(dev, dtype, size):

@@ -9,7 +9,12 @@ namespace va {
 
 // How many workgroups share the queries that see a block of keys.  Few blocks,
 // each of them seen by many queries (long sequences, or several query heads to a
-// kv head), leave most of the chip idle otherwise.
+// kv head), leave most of the chip idle otherwise: 4 sequences of 600 to 2000 rows,
+// 32 heads over 4 of 64, in f16 took 401 us, with 1, 2, 3 and 4 parts for each
+// place on the chip 401, 212, 192 and 199 with the parts' sum; a sequence of 420
+// rows 25, with parts of two steps at least 14.4 + 4.2, of one 12.0 + 8.  Where
+// blocks are many, parts only add the sum: 8 answers behind prompts of 700 rows
+// 31 us, in parts 35 + 15.
 static int dkv_parts(const va_varlen_bwd_args* a) {
   if (a->num_seqs <= 0 || a->num_kv_heads <= 0 || a->total_q <= 0 || a->total_k <= 0) return 1;
   const int64_t blocks = ((int64_t)a->total_k / kDkvKeys + a->num_seqs) * a->num_kv_heads;
@@ -17,6 +22,17 @@ static int dkv_parts(const va_varlen_bwd_args* a) {
   const int64_t tiles = ((int64_t)a->total_q / a->num_seqs + kDkvTile - 1) / kDkvTile;
   const int64_t steps = tiles * (a->num_heads / a->num_kv_heads) / (a->causal ? 2 : 1);
   return (int)std::max<int64_t>(1, std::min<int64_t>({3 * slots / blocks, steps / 2, 16}));
+}
+
+// Queries of a workgroup of the first launch: two workgroups fit a CU, and where
+// blocks of 128 queries would not fill them, blocks of 64, whose keys two waves
+// share, take less time: a sequence of 420 rows and 16 heads of 128 15.4 us
+// against 18.5, 8 answers of 40 to 260 rows behind 700 keys 27 against 31.  Where
+// they do fill them the tiles' copies, twice as many, cost more: windows of 104
+// rows 34 us against 27, a sequence of 8192 428 against 401.
+static int dq_rows(const va_varlen_bwd_args* a) {
+  const int64_t blocks = ((int64_t)a->total_q / 128 + a->num_seqs) * a->num_heads;
+  return blocks < 2 * (int64_t)current_device_cus() ? 64 : 128;
 }
 
 // Workspace: the first launch's results for the second (lse, delta and, for f16,
@@ -91,7 +107,8 @@ extern "C" int va_varlen_attention_backward(const va_varlen_bwd_args* a, void* s
   VA_CHECK_ARG(a->scale > 0.f && a->scale < INFINITY, "%s: scale must be > 0", fn);
   // A workgroup per block of every sequence; one more, which finds none, writes
   // the zeros of rows outside the sequences.
-  const int64_t q_tiles = (int64_t)a->total_q / kBwdRows + a->num_seqs + 1;
+  const int q_rows = dq_rows(a);
+  const int64_t q_tiles = (int64_t)a->total_q / q_rows + a->num_seqs + 1;
   const BwdLayout lay = backward_layout(a);
   VA_CHECK_ARG(q_tiles * a->num_heads <= INT32_MAX &&
                    lay.k_tiles * lay.parts * a->num_kv_heads <= INT32_MAX,
@@ -139,6 +156,7 @@ extern "C" int va_varlen_attention_backward(const va_varlen_bwd_args* a, void* s
   p.num_heads = a->num_heads;
   p.num_kv_heads = a->num_kv_heads;
   p.q_tiles = (int)q_tiles;
+  p.q_rows = q_rows;
   p.k_tiles = (int)lay.k_tiles;
   p.parts = lay.parts;
   p.lse = (float*)a->workspace;

@@ -8,21 +8,22 @@
 //     dq_i = c sum_j dS_ij k_j,   dk_j = c sum_i dS_ij q_i,   dv_j = sum_i P_ij dout_i
 // P is recomputed from q and k: nothing of the forward pass is kept but out.
 //
-// Two launches, neither with atomics, so that every call repeats bit for bit:
-//   1. varlen_dq_kernel: a workgroup per 128 queries of one head, one pass over
-//      their keys.  delta is known from out, so dq needs no softmax statistics
+// Two launches, or three, none with atomics, so that every call repeats bit for bit:
+//   1. varlen_dq_kernel: a workgroup per 128 (or 64) queries of one head, one pass
+//      over their keys.  delta is known from out, so dq needs no softmax statistics
 //      beforehand: with a running maximum m, dq gathers 2^(s c - m) (dP - delta) k
 //      and is divided by the sum at the end, rescaled where m rises.  It leaves
-//      lse_i = log2 sum_j 2^(c log2 e s_ij) and delta_i for the second launch.
-//   2. varlen_dkv_kernel: a workgroup per 128 keys of one kv head, over the
-//      queries that see them in every head of the group.
-// Each wave holds 32 queries (keys): their rows are B operands in registers
-// for the whole loop, their gradients accumulators.  The other side streams
-// through LDS in 64-row tiles, two stages filled by DMA, swizzled as in the
-// forward kernel.  S^T and dP^T (or S and dP) come from 32x32x16 MFMAs with the
-// tile's rows as A operands; their accumulators, rounded to 16 bits, are in
-// place the B operands of the gradients' products, whose A operands are the
-// same tile rows transposed by ds_read_b64_tr_b16.
+//      lse_i = log2 sum_j 2^(c log2 e s_ij) and -delta_i for the second launch.
+//   2. varlen_dkv_kernel: a workgroup per 64 keys of one kv head, over the queries
+//      that see them in every head of the group; or several, with a part of the
+//      queries each.
+//   3. varlen_dkv_sum_kernel: adds up the parts, where there are several.
+// A wave holds 32 queries (keys): their rows are B operands in registers for the
+// whole loop, their gradients accumulators.  The other side streams through LDS in
+// 64-row tiles, two stages filled by DMA, swizzled.  S^T and dP^T (or S and dP)
+// come from 32x32x16 MFMAs with the tile's rows as A operands; their accumulators,
+// rounded to 16 bits, are in place the B operands of the gradients' products, whose
+// A operands are the same tile rows transposed by ds_read_b64_tr_b16.
 #pragma once
 
 #include "varlen_kernel.h"
@@ -54,6 +55,7 @@ struct VarlenBwdParams {
   int32_t causal;
   int32_t num_seqs, total_q, total_k, num_heads, num_kv_heads;
   int32_t q_tiles, k_tiles;  // workgroups per head of the two launches (and part)
+  int32_t q_rows;            // queries of a workgroup of the first launch
   int32_t parts;             // workgroups that share a block of keys' queries
   float* part;               // parts > 1: their sums, [tile][part][kv head][wave][D / 8][64] x 4
   float* lse;                // [num_heads][total_q]: log2 sum 2^(c log2 e s), f16: - kF16Lift
@@ -62,7 +64,7 @@ struct VarlenBwdParams {
 };
 
 constexpr int kBwdThreads = 256;
-constexpr int kBwdRows = 128;  // queries (keys) of a workgroup, 32 a wave
+
 template <bool kBF16>
 __device__ inline f32x16_t mfma32(uint4 a, uint4 b, f32x16_t c) {
   if constexpr (kBF16)
@@ -225,6 +227,29 @@ __device__ inline uint4 pack_b(const f32x16_t& x, int half) {
                     pack_pair<kBF16>(x[8 * half + 6], x[8 * half + 7]));
 }
 
+// A wave's accumulators to LDS, 16 bytes a lane at a time, and a weighted sum with
+// what lies there.
+template <int DT>
+__device__ inline void put_acc(const f32x16_t (&acc)[DT], char* s, int lane) {
+#pragma unroll
+  for (int n = 0; n < 4 * DT; ++n) {
+    const f32x16_t& x = acc[n / 4];
+    const int i = n % 4 * 4;
+    *reinterpret_cast<f32x4_t*>(s + (n * 64 + lane) * 16) = f32x4_t{x[i], x[i + 1], x[i + 2], x[i + 3]};
+  }
+}
+template <int DT>
+__device__ inline void add_acc(f32x16_t (&acc)[DT], float mine, const char* s, float theirs,
+                               int lane) {
+#pragma unroll
+  for (int n = 0; n < 4 * DT; ++n) {
+    const f32x4_t x = *reinterpret_cast<const f32x4_t*>(s + (n * 64 + lane) * 16);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      acc[n / 4][n % 4 * 4 + i] = fmaf(x[i], theirs, acc[n / 4][n % 4 * 4 + i] * mine);
+  }
+}
+
 // Writes a wave's gradient, accumulators [D][32 rows] times `mul`, as rows of
 // 16 bits: through the wave's own 32 rows of LDS, so that each store
 // instruction writes whole rows.
@@ -267,9 +292,14 @@ constexpr int kF16Lift = 14;
 // a thousand keys would fall among f16's subnormals.  So P is scaled by 2^-e, e
 // the exponent of the row's largest |dout|, through the exponential's argument,
 // and the maximum is followed without slack, which keeps dS near v's size.
-template <bool kBF16, int D>
+//
+// kSplit: a wave takes 32 keys of each tile for its 32 queries, its neighbour the
+// other 32, and their sums meet in LDS at the end: launches whose blocks of 128
+// queries would leave the chip half idle take blocks of 64 in half the time.
+template <bool kBF16, int D, bool kSplit>
 __global__ __launch_bounds__(kBwdThreads, 2) void varlen_dq_kernel(VarlenBwdParams p) {
   constexpr int kTile = 64;  // keys
+  constexpr int kRows = kSplit ? 64 : 128;  // queries of a workgroup, 32 a wave
   constexpr int ROWB = D * 2, TILE_B = kTile * ROWB, DS = D / 16, DT = D / 32;
   __shared__ __align__(1024) char s_kv[2 * 2 * TILE_B];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -281,18 +311,17 @@ __global__ __launch_bounds__(kBwdThreads, 2) void varlen_dq_kernel(VarlenBwdPara
   const int pick = (int)(blockIdx.x % (unsigned)p.num_heads);
   const int group = p.num_heads / p.num_kv_heads;
   const int kv = pick % p.num_kv_heads, head = kv * group + pick / p.num_kv_heads;
-  const BwdBlock blk = find_block<kBwdRows>(p.cu_q, p.num_seqs, p.total_q, tile);
+  const BwdBlock blk = find_block<kRows>(p.cu_q, p.num_seqs, p.total_q, tile);
   if (!blk.found) {
-    zero_rest<D, kBwdThreads>(p.cu_q, p.num_seqs, p.total_q, p.dq, p.dq_st, head * p.dq_sh, tile - blk.first,
-                 p.q_tiles - blk.first);
+    zero_rest<D, kBwdThreads>(p.cu_q, p.num_seqs, p.total_q, p.dq, p.dq_st, head * p.dq_sh,
+                              tile - blk.first, p.q_tiles - blk.first);
     return;
   }
   const SeqRows qs = seq_rows(p.cu_q, blk.seq, p.total_q);
   const SeqRows ks = seq_rows(p.cu_k, blk.seq, p.total_k);
-  const int i0 = (tile - blk.first) * kBwdRows;  // the block's first query
-  const int ahead = ks.len - qs.len;             // causal: query i sees keys j <= i + ahead
-  const int kend =
-      p.causal ? min(max(ahead + min(i0 + kBwdRows, qs.len), 0), ks.len) : ks.len;
+  const int i0 = (tile - blk.first) * kRows;  // the block's first query
+  const int ahead = ks.len - qs.len;         // causal: query i sees keys j <= i + ahead
+  const int kend = p.causal ? min(max(ahead + min(i0 + kRows, qs.len), 0), ks.len) : ks.len;
   const int tiles = (kend + kTile - 1) / kTile;
   const char* const kp = p.k + (int64_t)ks.row * p.k_st + kv * p.k_sh;
   const char* const vp = p.v + (int64_t)ks.row * p.v_st + kv * p.v_sh;
@@ -318,7 +347,7 @@ __global__ __launch_bounds__(kBwdThreads, 2) void varlen_dq_kernel(VarlenBwdPara
   }
 
   // The wave's 32 queries (rows past the sequence repeat its last).
-  const int wrow = i0 + 32 * wave;
+  const int wrow = i0 + 32 * (kSplit ? wave >> 1 : wave);
   const int row = wrow + l32, at = qs.row + min(row, qs.len - 1);
   uint4 qreg[DS], doreg[DS];
   float delta = 0.f;
@@ -372,81 +401,99 @@ __global__ __launch_bounds__(kBwdThreads, 2) void varlen_dq_kernel(VarlenBwdPara
     const char* const sk = s_kv + (t & 1) * 2 * TILE_B;
     const char* const sv = sk + TILE_B;
 #pragma unroll
-    for (int sub = 0; sub < 2; ++sub) {
-    const int j0 = t * kTile + 32 * sub;
-    if (j0 >= lim_hi) {  // no query of the wave sees these
-      if (more) {
+    for (int turn = 0; turn < (kSplit ? 1 : 2); ++turn) {
+      const int sub = kSplit ? wave & 1 : turn;
+      constexpr int kTurnCopies = kSplit ? 2 * Copy::NI : Copy::NI;
+      const int j0 = t * kTile + 32 * sub;
+      if (j0 >= lim_hi) {  // no query of the wave sees these
+        if (more) {
 #pragma unroll
-        for (int n = 0; n < Copy::NI; ++n) issue(t + 1, sub * Copy::NI + n);
+          for (int n = 0; n < kTurnCopies; ++n) issue(t + 1, turn * Copy::NI + n);
+        }
+        continue;
       }
-      continue;
-    }
-    ta.rebuild();
-    // S and dP in turn, operands requested kAhead products before their own, the
-    // next tile's copies (K's beside the first 32 keys, V's beside the others)
-    // between them.
-    constexpr int kAhead = 4;
-    uint4 op[kAhead];
-    auto request = [&](int n) {
-      if (n < 2 * DS) op[n % kAhead] = ta.a(n & 1 ? sv : sk, sub, n / 2);
-    };
+      ta.rebuild();
+      // S and dP in turn, operands requested kAhead products before their own, the
+      // next tile's copies (K's beside the first 32 keys, V's beside the others)
+      // between them.
+      constexpr int kAhead = 4;
+      uint4 op[kAhead];
+      auto request = [&](int n) {
+        if (n < 2 * DS) op[n % kAhead] = ta.a(n & 1 ? sv : sk, sub, n / 2);
+      };
 #pragma unroll
-    for (int n = 0; n < kAhead; ++n) request(n);
-    f32x16_t s = {}, dp;
+      for (int n = 0; n < kAhead; ++n) request(n);
+      f32x16_t s = {}, dp;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) dp[i] = -delta;
+      for (int i = 0; i < 16; ++i) dp[i] = -delta;
 #pragma unroll
-    for (int n = 0; n < 2 * DS; ++n) {
-      if (n & 1)
-        dp = mfma32<kBF16>(op[n % kAhead], doreg[n / 2], dp);
-      else
-        s = mfma32<kBF16>(op[n % kAhead], qreg[n / 2], s);
-      request(n + kAhead);
-      constexpr int kEvery = 2 * DS / Copy::NI;
-      if (n % kEvery == kEvery - 1 && more) issue(t + 1, sub * Copy::NI + n / kEvery);
-    }
-    if (j0 + 32 > lim_lo) {
-      const int rel = lim - j0 - 4 * half;  // key 8 (i / 4) + i % 4 of the lane is seen iff < rel
+      for (int n = 0; n < 2 * DS; ++n) {
+        if (n & 1)
+          dp = mfma32<kBF16>(op[n % kAhead], doreg[n / 2], dp);
+        else
+          s = mfma32<kBF16>(op[n % kAhead], qreg[n / 2], s);
+        request(n + kAhead);
+        constexpr int kEvery = 2 * DS / kTurnCopies;
+        if (n % kEvery == kEvery - 1 && more) issue(t + 1, turn * Copy::NI + n / kEvery);
+      }
+      if (j0 + 32 > lim_lo) {
+        const int rel = lim - j0 - 4 * half;  // key 8 (i / 4) + i % 4 of the lane is seen iff < rel
 #pragma unroll
-      for (int i = 0; i < 16; ++i)
-        if (8 * (i / 4) + i % 4 >= rel) s[i] = -INFINITY;
-    }
-    float mx = s[0];
+        for (int i = 0; i < 16; ++i)
+          if (8 * (i / 4) + i % 4 >= rel) s[i] = -INFINITY;
+      }
+      float mx = s[0];
 #pragma unroll
-    for (int i = 1; i < 16; ++i) mx = fmaxf(mx, s[i]);
-    mx = max_xor32(mx) * p.scale_log2;
-    if (__builtin_amdgcn_ballot_w64(mx > m + kSlack) != 0) {
-      const float mn = fmaxf(m, mx);
-      const float alpha = fast_exp2(m - mn);
-      m = mn;
-      l *= alpha;
+      for (int i = 1; i < 16; ++i) mx = fmaxf(mx, s[i]);
+      mx = max_xor32(mx) * p.scale_log2;
+      if (__builtin_amdgcn_ballot_w64(mx > m + kSlack) != 0) {
+        const float mn = fmaxf(m, mx);
+        const float alpha = fast_exp2(m - mn);
+        m = mn;
+        l *= alpha;
 #pragma unroll
-      for (int dt = 0; dt < DT; ++dt) acc[dt] *= alpha;
-    }
-    const float base = kBF16 ? m : m + (float)e;
+        for (int dt = 0; dt < DT; ++dt) acc[dt] *= alpha;
+      }
+      const float base = kBF16 ? m : m + (float)e;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      s[i] = fast_exp2(fmaf(s[i], p.scale_log2, -base));
-      l += s[i];
-      dp[i] *= s[i];
-    }
+      for (int i = 0; i < 16; ++i) {
+        s[i] = fast_exp2(fmaf(s[i], p.scale_log2, -base));
+        l += s[i];
+        dp[i] *= s[i];
+      }
 #pragma unroll
-    for (int hf = 0; hf < 2; ++hf) {
-      const uint4 b = pack_b<kBF16>(dp, hf);
+      for (int hf = 0; hf < 2; ++hf) {
+        const uint4 b = pack_b<kBF16>(dp, hf);
 #pragma unroll
-      for (int dt = 0; dt < DT; ++dt) acc[dt] = mfma32<kBF16>(ta.at(sk, sub, hf, dt), b, acc[dt]);
-    }
+        for (int dt = 0; dt < DT; ++dt) acc[dt] = mfma32<kBF16>(ta.at(sk, sub, hf, dt), b, acc[dt]);
+      }
     }
   }
   l = sum_xor32(l);
+  __syncthreads();  // every wave is done with the tiles
+  // Where the wave's rows go out from, and in a split block its neighbour's sums lie.
+  char* const s_x = s_kv + (kSplit ? (wave >> 1) * (DT * 4 + 1) * 1024 : wave * 32 * ROWB);
+  if constexpr (kSplit) {
+    float2* const s_ml = reinterpret_cast<float2*>(s_x + DT * 4 * 1024);
+    if (wave & 1) {
+      put_acc<DT>(acc, s_x, lane);
+      s_ml[lane] = make_float2(m, l);
+    }
+    __syncthreads();
+    if (wave & 1) return;
+    const float2 o = s_ml[lane];
+    const float mn = fmaxf(m, o.x), mine = fast_exp2(m - mn), theirs = fast_exp2(o.x - mn);
+    m = mn;
+    l = l * mine + o.y * theirs;
+    add_acc<DT>(acc, mine, s_x, theirs, lane);
+  }
   const float base = kBF16 ? m : m + (float)e;
   if (half == 0 && row < qs.len) {
     const int64_t w = (int64_t)head * p.total_q + at;
     p.lse[w] = l > 0.f ? base + __builtin_amdgcn_logf(l) - (kBF16 ? 0.f : (float)kF16Lift) : INFINITY;
     p.delta[w] = -delta;
   }
-  __syncthreads();  // every wave is done with the tiles
-  write_rows<kBF16, D>(acc, l > 0.f ? p.scale / l : 0.f, s_kv + wave * 32 * ROWB,
+  write_rows<kBF16, D>(acc, l > 0.f ? p.scale / l : 0.f, s_x,
                        p.dq + (int64_t)qs.row * p.dq_st + head * p.dq_sh, p.dq_st, wrow, qs.len,
                        lane);
 }
@@ -501,12 +548,15 @@ __device__ inline void zero_rest_kv(const VarlenBwdParams& p, int kv, int nth, i
   zero_rest<D, 256>(p.cu_k, p.num_seqs, p.total_k, p.dv, p.dv_st, kv * p.dv_sh, nth, of);
 }
 
-// Two pairs of waves, 32 keys a pair.  Of a tile the first wave of a pair forms P and dS of the first 32 queries, the second of the
-// others; they exchange through LDS what the other one needs, and the first adds
-// up dv of all 64, the second dk.  So a wave holds one gradient beside its K and V
-// operands and has registers left for the next operands.  (A wave that adds up
-// both has none: at head_dim 128 its step of 32 queries took 3600 cycles for 1024
-// of matrix work, its operands requested one ahead.)
+// Two pairs of waves, 32 keys a pair.  Of a tile the first wave of a pair forms P
+// and dS of the first 32 queries, the second of the others; they exchange through
+// LDS what the other one needs, and the first adds up dv of all 64, the second dk.
+// So a wave holds one gradient beside its K and V operands and has registers left
+// for the operands ahead.  (A wave that adds up both has none at head_dim 128: its
+// step of 32 queries took 3600 cycles for 1024 of matrix work.)  Eight waves that
+// add up both gradients of 128 keys, two for each 32 keys, are faster on one long
+// sequence and slower where there are few blocks: 8192 rows 530 us against 578,
+// windows of 104 rows 56 against 30, one sequence of 420 rows 31 against 25.
 //
 // kParts: the block's steps are shared among several workgroups, whose sums a
 // third launch adds up (varlen_dkv_sum_kernel).
@@ -769,40 +819,41 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void varlen_dkv_kernel(Varlen
   write_dkv<kBF16, D>(p, acc, mul, s_qd + wave * 32 * ROWB, role, ks, kv, wkey, lane);
 }
 
-// Adds up the parts of a block's gradients, in their order: a wave the sums that
-// one wave of each part wrote.
+// Adds up the parts of a block's gradients, in their order: a thread 4 elements of
+// one key's dk or dv (256 of a wave's a workgroup; blockIdx.y counts them).
 template <bool kBF16, int D>
 __global__ __launch_bounds__(256) void varlen_dkv_sum_kernel(VarlenBwdParams p) {
-  constexpr int DT = D / 32;
-  __shared__ __align__(16) char s_w[4 * 32 * D * 2];
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int lane = threadIdx.x & 63;
   const int kv = (int)(blockIdx.x % (unsigned)p.num_kv_heads);
   const int tile = (int)(blockIdx.x / (unsigned)p.num_kv_heads);
   const DkvBlock blk = dkv_block(p, tile);
   if (!blk.found) {
-    zero_rest_kv<D>(p, kv, tile - blk.empty, p.k_tiles - blk.empty);
+    if (blockIdx.y == 0) zero_rest_kv<D>(p, kv, tile - blk.empty, p.k_tiles - blk.empty);
     return;
   }
-  f32x16_t acc[DT];
+  const int at = blockIdx.y * 256 + threadIdx.x;  // of the block's 4 waves x D / 8 x 64
+  const int wave = at / (D * 8), dt = at / 256 % (D / 32), j = at / 64 % 4, lane = at % 64;
+  const int key = blk.j0 + 32 * (wave >> 1) + lane % 32;
+  if (key >= blk.ks.len) return;
+  const int64_t unit = (int64_t)p.num_kv_heads * 4 * 32 * D;  // floats from part to part
+  const float* const from = p.part + (int64_t)tile * p.parts * unit + (int64_t)kv * 4 * 32 * D + at * 4;
+  f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
+  for (int n0 = 0; n0 < p.parts; n0 += 4) {
+    f32x4_t x[4];
 #pragma unroll
-  for (int dt = 0; dt < DT; ++dt) acc[dt] = f32x16_t{};
-  for (int n = 0; n < p.parts; ++n) {
-    if (part_begin(blk.steps, n, p.parts) == part_begin(blk.steps, n + 1, p.parts)) continue;
-    const float* const from =
-        p.part +
-        ((((int64_t)tile * p.parts + n) * p.num_kv_heads + kv) * 4 + wave) * (32 * D);
+    for (int i = 0; i < 4; ++i) {
+      // (A part without steps wrote nothing.)
+      const int n = n0 + i;
+      const bool any = n < p.parts && part_begin(blk.steps, n, p.parts) < part_begin(blk.steps, n + 1, p.parts);
+      x[i] = any ? *reinterpret_cast<const f32x4_t*>(from + n * unit) : f32x4_t{0.f, 0.f, 0.f, 0.f};
+    }
 #pragma unroll
-    for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const f32x4_t x = *reinterpret_cast<const f32x4_t*>(from + ((dt * 4 + j) * 64 + lane) * 4);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) acc[dt][4 * j + i] += x[i];
-      }
+    for (int i = 0; i < 4; ++i) acc += x[i];
   }
-  write_dkv<kBF16, D>(p, acc, 1.f, s_w + wave * 32 * D * 2, wave & 1, blk.ks, kv,
-                      blk.j0 + 32 * (wave >> 1), lane);
+  const bool is_k = wave & 1;
+  char* const to = is_k ? p.dk + (int64_t)(blk.ks.row + key) * p.dk_st + kv * p.dk_sh
+                        : p.dv + (int64_t)(blk.ks.row + key) * p.dv_st + kv * p.dv_sh;
+  *reinterpret_cast<uint2*>(to + (32 * dt + 8 * j + 4 * (lane / 32)) * 2) =
+      make_uint2(pack_pair<kBF16>(acc[0], acc[1]), pack_pair<kBF16>(acc[2], acc[3]));
 }
 
 // Both launches for one 16-bit type and head_dim, instantiated in
@@ -812,16 +863,19 @@ void launch_varlen_backward(const VarlenBwdParams& p, hipStream_t st);
 
 template <bool kBF16, int D>
 static void launch_varlen_backward_d(const VarlenBwdParams& p, hipStream_t st) {
-  hipLaunchKernelGGL((varlen_dq_kernel<kBF16, D>), dim3((unsigned)p.q_tiles * p.num_heads),
-                     dim3(kBwdThreads), 0, st, p);
+  const dim3 q_grid((unsigned)p.q_tiles * p.num_heads);
+  if (p.q_rows == 64)
+    hipLaunchKernelGGL((varlen_dq_kernel<kBF16, D, true>), q_grid, dim3(kBwdThreads), 0, st, p);
+  else
+    hipLaunchKernelGGL((varlen_dq_kernel<kBF16, D, false>), q_grid, dim3(kBwdThreads), 0, st, p);
   const dim3 grid((unsigned)p.k_tiles * p.parts * p.num_kv_heads);
   if (p.parts == 1) {
     hipLaunchKernelGGL((varlen_dkv_kernel<kBF16, D, false>), grid, dim3(256), 0, st, p);
     return;
   }
   hipLaunchKernelGGL((varlen_dkv_kernel<kBF16, D, true>), grid, dim3(256), 0, st, p);
-  hipLaunchKernelGGL((varlen_dkv_sum_kernel<kBF16, D>), dim3((unsigned)p.k_tiles * p.num_kv_heads),
-                     dim3(256), 0, st, p);
+  hipLaunchKernelGGL((varlen_dkv_sum_kernel<kBF16, D>),
+                     dim3((unsigned)p.k_tiles * p.num_kv_heads, D / 8), dim3(256), 0, st, p);
 }
 
 template <>
