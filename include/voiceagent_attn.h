@@ -166,7 +166,8 @@ int va_qk_norm_rope(const va_qk_norm_rope_args* args, void* stream);
  *   dx = r (dy weight - n mean(dy weight n)).
  * All in fp32, rounded once at the end; the forward's roundings to the element
  * type count as the identity.  No atomics: calls repeat bit for bit.  dq and dk
- * may be dq_out and dk_out or q and k themselves. */
+ * may be dq_out and dk_out or q and k themselves.  Norm weights and rows are
+ * 16-byte aligned. */
 typedef struct va_qk_norm_rope_bwd_args {
   uint32_t struct_size;   /* sizeof(va_qk_norm_rope_bwd_args)             */
   int32_t dtype;          /* VA_BF16 / VA_F16 / VA_F32, all rows          */

@@ -179,6 +179,14 @@ __device__ inline int64_t load_index(const void* p, int64_t i, int is_i64) {
                 : (int64_t)reinterpret_cast<const int32_t*>(p)[i];
 }
 
+// The same without a branch, whose join would hold up the loads behind it: the
+// low word, and the high one (or the low one again).
+__device__ inline int64_t load_index_words(const void* p, int64_t i, int is_i64) {
+  const int32_t* const w = reinterpret_cast<const int32_t*>(p) + (i << (is_i64 ? 1 : 0));
+  const int32_t lo = w[0], hi = w[is_i64 ? 1 : 0];
+  return is_i64 ? (int64_t)hi << 32 | (uint32_t)lo : (int64_t)lo;
+}
+
 // The 16-bit word u of 8 elements of ET (BF16 or F16), each multiplied by
 // inv in fp32, as 8 e4m3 codes (element i in byte i).
 template <typename ET>

@@ -8,10 +8,11 @@
 // 16-bit types.  Rows lie on lanes as in the forward kernel (prologue.h): the
 // two sums over a row are DPP reductions.  A lane adds up its own columns'
 // dy n of the rows it meets in registers; a workgroup's sums meet in LDS and
-// leave as one row of partials, and a second launch adds the partials of all
-// workgroups, in a fixed order: no atomics, so calls repeat bit for bit.
+// leave as one row of partials, and a second launch (3 to 4 us) adds the partials
+// of all workgroups, in a fixed order: no atomics, so calls repeat bit for bit.
 #include <algorithm>
 
+#include "fastdiv.h"
 #include "prologue.h"
 
 namespace va {
@@ -23,110 +24,112 @@ struct QkBwdParams {
   int64_t x_st[2], x_sh[2];
   char* dx[2];
   int64_t dx_st[2], dx_sh[2];
-  int32_t num_tokens, hq, hkv;
-  int32_t waves_per_token, groups_per_wave;
-  int64_t units;  // num_tokens * waves_per_token
+  int32_t hq, hkv;
+  uint32_t units;    // of work, unit_div.d a token
+  FastDiv unit_div;
   float* part;    // [blocks][2][D]
   PrologueParams pp;
 };
 
 constexpr int kQbThreads = 256;
 constexpr int kQbBlocks = 1024;  // rows of partials at most
-// Row groups whose loads (x and dz) a lane keeps in flight at once.
+// Row groups of a wave's unit of work, all of whose loads are in flight at once: of
+// 16 + 8 heads of 128 in bf16 8561 tokens take 31.8 us (158 MB, 5.0 TB/s) and 420 take
+// 5.6; two row groups 32.6 and 5.7, one 38.7 and 5.2 (and leaves three times the
+// partial sums).  Half the workgroups, 36 us.
 constexpr int kQbChunk = 3;
-constexpr int64_t kQbTargetWaves = 4096;
 
 template <typename ET, int D>
 __global__ __launch_bounds__(kQbThreads) void qk_norm_rope_backward_kernel(QkBwdParams p) {
   constexpr int E = ET::kPerVec;
   constexpr int LPR = D / E;
   constexpr int RPW = 64 / LPR;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane % LPR, sub = lane / LPR;
   const int heads = p.hq + p.hkv;
-  float w[2][E], dw[2][E];
+  // (With no query (key) heads the other side's weights stand in; unused.)
+  const WeightRaw<E> wqr = load_weights_raw<E>(p.hq > 0 ? p.pp.q_w : p.pp.k_w, p.pp.w_dtype, col * E);
+  const WeightRaw<E> wkr = load_weights_raw<E>(p.hkv > 0 ? p.pp.k_w : p.pp.q_w, p.pp.w_dtype, col * E);
+  float dw[2][E] = {};
+  for (uint32_t u = blockIdx.x * (kQbThreads / 64) + wave; u < p.units;
+       u += gridDim.x * (kQbThreads / 64)) {
+    const uint32_t tok = fast_div(u, p.unit_div);
+    const int h0 = (int)(u - tok * p.unit_div.d) * kQbChunk * RPW;
+    int64_t pos = load_index_words(p.pp.pos, tok, p.pp.pos_i64);
+    uint4 xr[kQbChunk], zr[kQbChunk];
 #pragma unroll
-  for (int e = 0; e < E; ++e) {
-    // (With no query (key) heads the other side's weights stand in; unused.)
-    w[0][e] = load_weight(p.hq > 0 ? p.pp.q_w : p.pp.k_w, p.pp.w_dtype, col * E + e);
-    w[1][e] = load_weight(p.hkv > 0 ? p.pp.k_w : p.pp.q_w, p.pp.w_dtype, col * E + e);
-    dw[0][e] = dw[1][e] = 0.f;
-  }
-  for (int64_t u = (int64_t)blockIdx.x * (kQbThreads / 64) + wave; u < p.units;
-       u += (int64_t)gridDim.x * (kQbThreads / 64)) {
-    const int64_t tok = u / p.waves_per_token;
-    const int r0 = (int)(u % p.waves_per_token) * p.groups_per_wave * RPW;
-    const int r1 = min(r0 + p.groups_per_wave * RPW, heads);
-    int64_t pos = load_index(p.pp.pos, tok, p.pp.pos_i64);
+    for (int j = 0; j < kQbChunk; ++j) {
+      const int hh = min(h0 + j * RPW + sub, heads - 1);
+      const int side = hh < p.hq ? 0 : 1, head = hh < p.hq ? hh : hh - p.hq;
+      const char* const xs = side ? p.x[1] + tok * p.x_st[1] + head * p.x_sh[1]
+                                  : p.x[0] + tok * p.x_st[0] + head * p.x_sh[0];
+      const char* const zs = side ? p.dz[1] + tok * p.dz_st[1] + head * p.dz_sh[1]
+                                  : p.dz[0] + tok * p.dz_st[0] + head * p.dz_sh[0];
+      xr[j] = ld16_nt(xs + col * 16);
+      zr[j] = ld16_nt(zs + col * 16);
+    }
+    pos = pos < 0 ? 0 : (pos >= p.pp.max_pos ? p.pp.max_pos - 1 : pos);
     float c[E], s[E];
-    for (int h0 = r0; h0 < r1; h0 += kQbChunk * RPW) {
-      uint4 xr[kQbChunk], zr[kQbChunk];
+    load_rotary<E, LPR>(p.pp, pos, col, D, c, s);
 #pragma unroll
-      for (int j = 0; j < kQbChunk; ++j) {
-        const int hh = min(h0 + j * RPW + sub, r1 - 1);
-        const int side = hh < p.hq ? 0 : 1, head = hh < p.hq ? hh : hh - p.hq;
-        const char* const xs = side ? p.x[1] + tok * p.x_st[1] + head * p.x_sh[1]
-                                    : p.x[0] + tok * p.x_st[0] + head * p.x_sh[0];
-        const char* const zs = side ? p.dz[1] + tok * p.dz_st[1] + head * p.dz_sh[1]
-                                    : p.dz[0] + tok * p.dz_st[0] + head * p.dz_sh[0];
-        xr[j] = ld16_nt(xs + col * 16);
-        zr[j] = ld16_nt(zs + col * 16);
+    for (int j = 0; j < kQbChunk; ++j) {
+      if (h0 + j * RPW >= heads) break;  // whole row groups past the token's last row
+      const int hh = h0 + j * RPW + sub;
+      const bool isq = hh < p.hq, live = hh < heads;
+      float x[E], z[E], w[E];
+      ET::unpack(xr[j], x);
+      ET::unpack(zr[j], z);
+      WeightRaw<E> wr;
+      wr.a = isq ? wqr.a : wkr.a;
+      wr.b = isq ? wqr.b : wkr.b;
+      convert_weights<E>(wr, p.pp.w_dtype, w);
+      float ss = 0.f;
+#pragma unroll
+      for (int e = 0; e < E; ++e) ss = fmaf(x[e], x[e], ss);
+      ss = group_sum<LPR>(ss);
+      const float r = 1.0f / sqrtf(ss / (float)D + p.pp.eps);
+      // s holds -sin in the row's first half, +sin in the second: the
+      // transposed rotation takes the partner's share with its sign turned.
+      float dot = 0.f;
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        const float dy = fmaf(-rotary_partner<LPR>(z[e]), s[e], z[e] * c[e]);
+        x[e] *= r;  // n
+        const float g = live ? dy * x[e] : 0.f;
+        dw[0][e] += isq ? g : 0.f;
+        dw[1][e] += isq ? 0.f : g;
+        z[e] = dy * w[e];
+        dot = fmaf(z[e], x[e], dot);
       }
-      if (h0 == r0) {
-        pos = pos < 0 ? 0 : (pos >= p.pp.max_pos ? p.pp.max_pos - 1 : pos);
-        load_rotary<E, LPR>(p.pp, pos, col, D, c, s);
-      }
+      dot = group_sum<LPR>(dot) / (float)D;
 #pragma unroll
-      for (int j = 0; j < kQbChunk; ++j) {
-        if (h0 + j * RPW >= r1) break;  // whole row groups past the wave's last row
-        const int hh = h0 + j * RPW + sub;
-        const bool isq = hh < p.hq, live = hh < r1;
-        float x[E], z[E];
-        ET::unpack(xr[j], x);
-        ET::unpack(zr[j], z);
-        float ss = 0.f;
-#pragma unroll
-        for (int e = 0; e < E; ++e) ss = fmaf(x[e], x[e], ss);
-        ss = group_sum<LPR>(ss);
-        const float r = 1.0f / sqrtf(ss / (float)D + p.pp.eps);
-        // s holds -sin in the row's first half, +sin in the second: the
-        // transposed rotation takes the partner's share with its sign turned.
-        float dot = 0.f;
-#pragma unroll
-        for (int e = 0; e < E; ++e) {
-          const float dy = fmaf(-rotary_partner<LPR>(z[e]), s[e], z[e] * c[e]);
-          x[e] *= r;  // n
-          const float g = live ? dy * x[e] : 0.f;
-          dw[0][e] += isq ? g : 0.f;
-          dw[1][e] += isq ? 0.f : g;
-          z[e] = dy * (isq ? w[0][e] : w[1][e]);
-          dot = fmaf(z[e], x[e], dot);
-        }
-        dot = group_sum<LPR>(dot) / (float)D;
-#pragma unroll
-        for (int e = 0; e < E; ++e) x[e] = r * fmaf(-x[e], dot, z[e]);
-        if (live) {
-          const int head = isq ? hh : hh - p.hq;
-          char* const to = isq ? p.dx[0] + tok * p.dx_st[0] + head * p.dx_sh[0]
-                               : p.dx[1] + tok * p.dx_st[1] + head * p.dx_sh[1];
-          st16_nt(to + col * 16, ET::pack(x));
-        }
+      for (int e = 0; e < E; ++e) x[e] = r * fmaf(-x[e], dot, z[e]);
+      if (live) {
+        const int head = isq ? hh : hh - p.hq;
+        char* const to = isq ? p.dx[0] + tok * p.dx_st[0] + head * p.dx_sh[0]
+                             : p.dx[1] + tok * p.dx_st[1] + head * p.dx_sh[1];
+        st16_nt(to + col * 16, ET::pack(x));
       }
     }
   }
-  // The workgroup's sums: over a wave's row groups, then over its waves.
-  __shared__ float s_dw[kQbThreads / 64][2][D];
+  // The workgroup's sums: every lane's go to LDS as they are, and a thread adds up
+  // those of one column.  (Summed over a wave's row groups by lane permutes first,
+  // 16 columns in turn, they cost a small call 2 us.)
+  constexpr int kRowsWg = kQbThreads / 64 * RPW;
+  __shared__ float s_dw[kRowsWg][2][D];
 #pragma unroll
   for (int side = 0; side < 2; ++side)
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-      const float v = strided_sum<LPR>(dw[side][e]);
-      if (sub == 0) s_dw[wave][side][col * E + e] = v;
-    }
+    for (int e = 0; e < E; e += 4)
+      *reinterpret_cast<float4*>(&s_dw[wave * RPW + sub][side][col * E + e]) =
+          make_float4(dw[side][e], dw[side][e + 1], dw[side][e + 2], dw[side][e + 3]);
   __syncthreads();
   for (int i = threadIdx.x; i < 2 * D; i += kQbThreads) {
-    const float* const v = &s_dw[0][0][0] + i;
-    p.part[(int64_t)blockIdx.x * 2 * D + i] = (v[0] + v[2 * D]) + (v[4 * D] + v[6 * D]);
+    float v = 0.f;
+#pragma unroll
+    for (int n = 0; n < kRowsWg; ++n) v += (&s_dw[n][0][0])[i];
+    p.part[(int64_t)blockIdx.x * 2 * D + i] = v;
   }
 }
 
@@ -139,9 +142,15 @@ __global__ __launch_bounds__(kQbSumThreads) void qk_weight_sum_kernel(const floa
   __shared__ float s_sum[STRANDS][kQbSumCols];
   const int c = threadIdx.x % kQbSumCols, strand = threadIdx.x / kQbSumCols;
   const int col = blockIdx.x * kQbSumCols + c;
-  float v = 0.f;
-#pragma unroll 4
-  for (int r = strand; r < rows; r += STRANDS) v += part[(int64_t)r * 2 * d + col];
+  // All of a strand's rows (1 to 16) are requested at once; the last stands in for
+  // those that are not there.
+  constexpr int kMost = kQbBlocks / STRANDS;
+  float x[kMost], v = 0.f;
+#pragma unroll
+  for (int i = 0; i < kMost; ++i)
+    x[i] = rows > 0 ? part[(int64_t)min(strand + i * STRANDS, rows - 1) * 2 * d + col] : 0.f;
+#pragma unroll
+  for (int i = 0; i < kMost; ++i) v += strand + i * STRANDS < rows ? x[i] : 0.f;
   s_sum[strand][c] = v;
   __syncthreads();
   for (int n = STRANDS / 2; n > 0; n /= 2) {
@@ -162,23 +171,16 @@ __global__ __launch_bounds__(kQbSumThreads) void qk_weight_sum_kernel(const floa
 }
 
 struct QkBwdPlan {
-  int wpt, gpw;
+  uint32_t per_token;  // units of a token
   int64_t units;
   int blocks;
 };
 static QkBwdPlan qk_bwd_plan(const va_qk_norm_rope_bwd_args* a) {
   const int e = a->dtype == VA_F32 ? 4 : 8;
-  const int rpw = 64 / (a->head_dim / e);
-  const int groups = (a->num_heads + a->num_kv_heads + rpw - 1) / rpw;
-  QkBwdPlan p{};
-  if (a->num_tokens == 0) return p;
-  // Waves per token as in the forward: several while the tokens alone would not
-  // fill the chip.
-  p.wpt = (int)std::min<int64_t>(
-      groups, std::max<int64_t>(1, (kQbTargetWaves + a->num_tokens - 1) / a->num_tokens));
-  p.gpw = (groups + p.wpt - 1) / p.wpt;
-  p.wpt = (groups + p.gpw - 1) / p.gpw;
-  p.units = (int64_t)a->num_tokens * p.wpt;
+  const int rows = kQbChunk * (64 / (a->head_dim / e));
+  QkBwdPlan p;
+  p.per_token = (uint32_t)((a->num_heads + a->num_kv_heads + rows - 1) / rows);
+  p.units = (int64_t)a->num_tokens * p.per_token;
   p.blocks = (int)std::min<int64_t>(kQbBlocks, (p.units + kQbThreads / 64 - 1) / (kQbThreads / 64));
   return p;
 }
@@ -242,7 +244,10 @@ extern "C" int va_qk_norm_rope_backward(const va_qk_norm_rope_bwd_args* a, void*
                             (uintptr_t)a->k, (uintptr_t)a->dq, (uintptr_t)a->dk};
   for (uintptr_t p : ptrs)
     VA_CHECK_ARG(p % 16 == 0, "%s: pointers must be 16-byte aligned", fn);
+  VA_CHECK_ARG((uintptr_t)pr.q_norm_weight % 16 == 0 && (uintptr_t)pr.k_norm_weight % 16 == 0,
+               "%s: norm weights must be 16-byte aligned", fn);
   const QkBwdPlan plan = qk_bwd_plan(a);
+  VA_CHECK_ARG(plan.units < ((int64_t)1 << 31), "%s: too many (token, head) rows", fn);
   const size_t need = (size_t)plan.blocks * 2 * a->head_dim * sizeof(float);
   if (need > 0 && (a->workspace == nullptr || a->workspace_bytes < need || (uintptr_t)a->workspace % 16 != 0)) {
     set_error("%s: needs a 16-byte aligned workspace of %zu bytes", fn, need);
@@ -267,12 +272,10 @@ extern "C" int va_qk_norm_rope_backward(const va_qk_norm_rope_bwd_args* a, void*
   p.dx[1] = (char*)a->dk;
   p.dx_st[1] = a->dk_stride_tok * eb;
   p.dx_sh[1] = a->dk_stride_head * eb;
-  p.num_tokens = a->num_tokens;
   p.hq = a->num_heads;
   p.hkv = a->num_kv_heads;
-  p.waves_per_token = plan.wpt;
-  p.groups_per_wave = plan.gpw;
-  p.units = plan.units;
+  p.units = (uint32_t)plan.units;
+  p.unit_div = make_fastdiv(plan.per_token);
   p.part = (float*)a->workspace;
   p.pp.q_w = pr.q_norm_weight;
   p.pp.k_w = pr.k_norm_weight;

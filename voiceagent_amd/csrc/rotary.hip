@@ -103,7 +103,7 @@ __global__ __launch_bounds__(kRotThreads) void rotary_kernel(RotaryParams p) {
       if (h0 + j < p.heads) rot_store<ET, CE>(target(j) + at, a[j]);
     return;
   }
-  int64_t pos = load_index(p.pos, tok, p.pos_i64);
+  int64_t pos = load_index_words(p.pos, tok, p.pos_i64);
   const int64_t at = (int64_t)u * E * ET::kBytes;
   const int64_t other = (int64_t)p.half * ET::kBytes;  // half-split: from a to b
   float a[kRotHeads][E], b[kRotHeads][kPairs ? 1 : E];
