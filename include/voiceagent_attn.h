@@ -408,9 +408,12 @@ size_t va_varlen_split_workspace_bytes(const va_varlen_args* args);
  * so that small gradients do not fall among f16's subnormals).
  * q, k, v, out and dout are as in the forward call (any group size); rows that
  * belong to no sequence get a gradient of zeros, as do queries that see no key
- * and keys that no query sees.  Lengths come from cu_seqlens alone, held to
- * the rows there are.  No atomics: calls repeat bit for bit.  The gradients
- * must not overlap the inputs or one another. */
+ * and keys that no query sees.  Lengths come from cu_seqlens, held to the rows
+ * there are; the maxima only choose the launch, and rows of a sequence past
+ * both may get zeros instead.  No atomics: calls repeat bit for bit.  The
+ * gradients must not overlap the inputs or one another.  Pointers and strides
+ * are 16-byte multiples; token strides of q, k, v and dout are from 0 to under
+ * 32 MiB. */
 typedef struct va_varlen_bwd_args {
   uint32_t struct_size;   /* sizeof(va_varlen_bwd_args)                   */
   int32_t dtype;          /* VA_BF16 / VA_F16                             */
@@ -434,6 +437,7 @@ typedef struct va_varlen_bwd_args {
   const int32_t* cu_seqlens_k; /* [num_seqs + 1]                          */
   int32_t num_seqs, total_q, total_k;
   int32_t num_heads, num_kv_heads, head_dim; /* head_dim 64 or 128        */
+  int32_t max_seqlen_q, max_seqlen_k; /* at least every length; 0: unknown */
   int32_t causal;         /* 1: bottom-right aligned causal mask          */
   float scale;
   void* workspace;        /* of va_varlen_attention_backward_workspace_bytes */

@@ -158,7 +158,7 @@ def test_training_fast_and_python_paths_agree(dev, python_path):
 
     first = run()
     assert ops._fast_calls().varlen_attention_backward(
-        dout, q, k.float(), v, out, cu, cu, 0.125, True, 0, 0)[0] == ops._FAST_NOT_TAKEN
+        dout, q, k.float(), v, out, cu, cu, 70, 70, 0.125, True, 0, 0)[0] == ops._FAST_NOT_TAKEN
     with pytest.raises(ops.AttentionArgumentError):
         ops.rotary_embedding(q, k.float(), table, pos)
     python_path()

@@ -65,6 +65,60 @@ def test_gradient_matches_the_definition(dev, lens, causal, dtype, d, hq, hkv):
     _check(got, G.varlen_attention_backward(dout, q, k, v, out, cu_q, cu_k, d ** -0.5, causal))
 
 
+WINDOWS = {
+    "encoder": ([104, 104, 33, 13], [104, 104, 33, 13], 104),
+    "tiles": ([31, 32, 33, 63, 64, 65], [31, 32, 33, 63, 64, 65], 65),
+    "most": ([128, 1, 0, 127, 96, 97], [128, 1, 0, 127, 96, 97], 128),
+    "tokens": ([1, 1, 2, 7], [1, 1, 2, 7], 7),
+    "sides": ([1, 40, 0, 100, 9, 3], [128, 7, 5, 0, 10, 99], 128),
+}
+
+
+@pytest.mark.parametrize("lens", WINDOWS)
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_short_sequences_in_one_launch(dev, lens, causal, dtype):
+    lens_q, lens_k, most = WINDOWS[lens]
+    q, k, v, dout, out, cu_q, cu_k = _inputs(lens_q, lens_k, 3, 3, 64, dtype, 17, before=3, behind=9)
+    on = [t.to(dev) for t in (dout, q, k, v, out, cu_q, cu_k)]
+    got = ops.varlen_attention_backward(*on, most, most, scale=0.125, causal=causal)
+    _check(got, G.varlen_attention_backward(dout, q, k, v, out, cu_q, cu_k, 0.125, causal))
+    for t in got:
+        assert not t[:3].any() and not t[-9:].any()
+
+
+def test_short_sequences_of_any_values(dev):
+    # Small and large gradients, rising maxima, strided rows, NaN outside and in another sequence.
+    lens, cu = [104, 50, 104], _cu([104, 50, 104], 7)
+    for dtype, size in ((torch.float16, 2.0 ** -20), (torch.float16, 2.0 ** 8), (torch.bfloat16, 2.0 ** -6)):
+        q, k, v, dout, out, _, _ = _inputs(lens, lens, 2, 2, 64, dtype, 18, grad=size, before=7, behind=5000)
+        q, k = q * 2, k * torch.linspace(0.1, 4, k.shape[0])[:, None, None].to(dtype)
+        want = G.varlen_attention_backward(dout, q, k, v, out, cu, cu, 0.125, False)
+        for t in (q, k, v, dout, out):
+            t[:7] = t[7 + 258:] = float("nan")
+        qkv = torch.cat((q, k, v), 1).to(dev).split([2, 2, 2], 1)
+        c, o, do = cu.to(dev), out.to(dev), dout.to(dev)
+        got = ops.varlen_attention_backward(do, *qkv, o, c, c, 104, 104, scale=0.125, causal=False)
+        _check(got, want)
+        do[7 + 104] = float("nan")  # the second sequence
+        for t, name in zip(ops.varlen_attention_backward(do, *qkv, o, c, c, 104, 104, scale=0.125,
+                                                         causal=False), NAMES):
+            for at in (slice(7, 111), slice(161, 265)):
+                err = (t[at].double().cpu() - want[name][at]).abs()
+                assert (err <= want[name + "_off"][at]).all()
+            assert not t[265:].any()
+
+
+def test_rows_past_the_maxima_get_zeros(dev):
+    q, k, v, dout, out, cu, _ = _inputs([100, 300], [100, 300], 2, 2, 64, torch.bfloat16, 19)
+    on = [t.to(dev) for t in (dout, q, k, v, out, cu, cu)]
+    got = ops.varlen_attention_backward(*on, 100, 100, scale=0.125, causal=False)
+    want = G.varlen_attention_backward(dout, q, k, v, out, cu, cu, 0.125, False)
+    for t, name in zip(got, NAMES):
+        assert ((t[:100].double().cpu() - want[name][:100]).abs() <= want[name + "_off"][:100]).all()
+        assert not t[200:].any()
+
+
 def test_many_sequences(dev):
     # More than a wave's lanes of sequences, some without queries.
     g = torch.Generator().manual_seed(5)

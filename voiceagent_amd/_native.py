@@ -294,6 +294,8 @@ class VarlenBwdArgs(ctypes.Structure):
         ("num_heads", c_int32),
         ("num_kv_heads", c_int32),
         ("head_dim", c_int32),
+        ("max_seqlen_q", c_int32),
+        ("max_seqlen_k", c_int32),
         ("causal", c_int32),
         ("scale", c_float),
         ("workspace", c_void_p),

@@ -718,10 +718,10 @@ at::Tensor rows_like(const at::Tensor& t) { return at::empty(t.sizes(), t.option
 // ops.varlen_attention_backward without given gradients: (status, [dq, dk, dv]).
 std::tuple<int64_t, std::vector<at::Tensor>> varlen_attention_backward(
     const at::Tensor& dout, const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
-    const at::Tensor& out, const at::Tensor& cu_q, const at::Tensor& cu_k, double scale,
-    bool causal, int64_t device, int64_t stream) {
+    const at::Tensor& out, const at::Tensor& cu_q, const at::Tensor& cu_k, int64_t max_q,
+    int64_t max_k, double scale, bool causal, int64_t device, int64_t stream) {
   const std::tuple<int64_t, std::vector<at::Tensor>> none{kNotTaken, {}};
-  if (g_varlen_bwd == nullptr || !rows_on(dout, device) || !rows_on(q, device) ||
+  if (g_varlen_bwd == nullptr || max_q < 0 || max_k < 0 || !fits_i32(max_q) || !fits_i32(max_k) || !rows_on(dout, device) || !rows_on(q, device) ||
       !rows_on(k, device) || !rows_on(v, device) || !rows_on(out, device) || !on(cu_q, device) ||
       !on(cu_k, device))
     return none;
@@ -771,6 +771,8 @@ std::tuple<int64_t, std::vector<at::Tensor>> varlen_attention_backward(
   a.num_heads = (int32_t)q.size(1);
   a.num_kv_heads = (int32_t)k.size(1);
   a.head_dim = (int32_t)q.size(2);
+  a.max_seqlen_q = (int32_t)max_q;
+  a.max_seqlen_k = (int32_t)max_k;
   a.causal = causal ? 1 : 0;
   a.scale = (float)scale;
   const at::Tensor ws = at::empty({(int64_t)g_varlen_bwd_ws(&a)}, q.options().dtype(at::kByte));

@@ -35,6 +35,16 @@ static int dq_rows(const va_varlen_bwd_args* a) {
   return blocks < 2 * (int64_t)current_device_cus() ? 64 : 128;
 }
 
+// The longest sequence, where one launch takes them whole (0: it does not; four tiles
+// of 128 rows of 64 are what LDS holds twice, and of 128 elements only once).
+static int window_rows(const va_varlen_bwd_args* a) {
+  const int most = std::max(a->max_seqlen_q, a->max_seqlen_k);
+  return a->head_dim == 64 && a->num_heads == a->num_kv_heads && a->max_seqlen_q > 0 &&
+                 a->max_seqlen_k > 0 && most <= kWindowMost
+             ? most
+             : 0;
+}
+
 // Workspace: the first launch's results for the second (lse, delta and, for f16,
 // the rows' largest |dout|), and the parts' sums.
 struct BwdLayout {
@@ -62,7 +72,7 @@ extern "C" size_t va_varlen_attention_backward_workspace_bytes(const va_varlen_b
       a->num_seqs < 0 || a->total_q <= 0 || a->total_k < 0 ||
       (a->head_dim != 64 && a->head_dim != 128))
     return 0;
-  return va::backward_layout(a).total;
+  return va::window_rows(a) > 0 ? 0 : va::backward_layout(a).total;
 }
 
 extern "C" int va_varlen_attention_backward(const va_varlen_bwd_args* a, void* stream) {
@@ -110,10 +120,13 @@ extern "C" int va_varlen_attention_backward(const va_varlen_bwd_args* a, void* s
   const int q_rows = dq_rows(a);
   const int64_t q_tiles = (int64_t)a->total_q / q_rows + a->num_seqs + 1;
   const BwdLayout lay = backward_layout(a);
-  VA_CHECK_ARG(q_tiles * a->num_heads <= INT32_MAX &&
+  VA_CHECK_ARG(a->max_seqlen_q >= 0 && a->max_seqlen_k >= 0, "%s: negative max_seqlen", fn);
+  const int window = window_rows(a);
+  VA_CHECK_ARG(((int64_t)a->num_seqs + 1 + std::max(a->total_q, a->total_k) / kWindowExtra) *
+                       a->num_heads <= INT32_MAX && q_tiles * a->num_heads <= INT32_MAX &&
                    lay.k_tiles * lay.parts * a->num_kv_heads <= INT32_MAX,
                "%s: too many (sequence, head, block) items", fn);
-  const size_t need = a->total_q > 0 ? lay.total : 0;
+  const size_t need = a->total_q > 0 && window == 0 ? lay.total : 0;
   if (need > 0 && (a->workspace == nullptr || a->workspace_bytes < need ||
                    (uintptr_t)a->workspace % 16 != 0)) {
     set_error("%s: needs a 16-byte aligned workspace of %zu bytes", fn, need);
@@ -157,6 +170,7 @@ extern "C" int va_varlen_attention_backward(const va_varlen_bwd_args* a, void* s
   p.num_kv_heads = a->num_kv_heads;
   p.q_tiles = (int)q_tiles;
   p.q_rows = q_rows;
+  p.window = window;
   p.k_tiles = (int)lay.k_tiles;
   p.parts = lay.parts;
   p.lse = (float*)a->workspace;

@@ -8,7 +8,8 @@
 //     dq_i = c sum_j dS_ij k_j,   dk_j = c sum_i dS_ij q_i,   dv_j = sum_i P_ij dout_i
 // P is recomputed from q and k: nothing of the forward pass is kept but out.
 //
-// Two launches, or three, none with atomics, so that every call repeats bit for bit:
+// Two launches, or three (or one, for short sequences: varlen_window_kernel), none
+// with atomics, so that every call repeats bit for bit:
 //   1. varlen_dq_kernel: a workgroup per 128 (or 64) queries of one head, one pass
 //      over their keys.  delta is known from out, so dq needs no softmax statistics
 //      beforehand: with a running maximum m, dq gathers 2^(s c - m) (dP - delta) k
@@ -25,6 +26,8 @@
 // rounded to 16 bits, are in place the B operands of the gradients' products, whose
 // A operands are the same tile rows transposed by ds_read_b64_tr_b16.
 #pragma once
+
+#include <algorithm>
 
 #include "varlen_kernel.h"
 
@@ -56,6 +59,7 @@ struct VarlenBwdParams {
   int32_t num_seqs, total_q, total_k, num_heads, num_kv_heads;
   int32_t q_tiles, k_tiles;  // workgroups per head of the two launches (and part)
   int32_t q_rows;            // queries of a workgroup of the first launch
+  int32_t window;            // > 0: one launch, no sequence is longer than this
   int32_t parts;             // workgroups that share a block of keys' queries
   float* part;               // parts > 1: their sums, [tile][part][kv head][wave][D / 8][64] x 4
   float* lse;                // [num_heads][total_q]: log2 sum 2^(c log2 e s), f16: - kF16Lift
@@ -82,39 +86,58 @@ __device__ inline void dma4(uint32_t off, const void* base, uint32_t lds) {
                : "memory");
 }
 
-// Sequence s's rows [row, row + len) of `total` packed rows: what cu says, held
-// to rows that there are.
+// A sequence's rows [row, row + len) of `total` packed rows: what cu says (a and
+// b, its ends), held to rows that there are.
 struct SeqRows {
   int row, len;
 };
-__device__ inline SeqRows seq_rows(const int32_t* cu, int s, int total) {
-  const int a = min(max(cu[s], 0), total);
-  return {a, min(max(cu[s + 1], a), total) - a};
+__device__ inline SeqRows seq_rows(int a, int b, int total) {
+  a = min(max(a, 0), total);
+  return {a, min(max(b, a), total) - a};
 }
 
-// The `tile`-th block of kRows rows, counting every sequence's blocks in
-// turn.  found: there is one; otherwise first is the number of blocks there are.
+// The `tile`-th block of kRows rows of one side, counting every sequence's blocks
+// in turn, with its sequence's rows on both.  found: there is one; otherwise first
+// is the number of blocks there are.  The ends of 128 sequences, both sides', are
+// requested at once (64 in turn, and the found sequence's again, took 160 sequences
+// of 14 heads 27.1 us for dq and 30.9 for dk and dv instead of 26.3 and 29.2).
 struct BwdBlock {
   bool found;
-  int seq, first;  // first: tile number of the sequence's first block
+  int first;  // tile number of the sequence's first block
+  SeqRows rows, other;
 };
 template <int kRows>
-__device__ inline BwdBlock find_block(const int32_t* cu, int num_seqs, int total, int tile) {
+__device__ inline BwdBlock find_block(const int32_t* cu, const int32_t* cu_other, int num_seqs,
+                                      int total, int total_other, int tile) {
   const int lane = threadIdx.x & 63;
   int before = 0;
-  for (int s0 = 0; s0 < num_seqs; s0 += 64) {
-    int nb = 0;
-    if (s0 + lane < num_seqs) nb = (seq_rows(cu, s0 + lane, total).len + kRows - 1) / kRows;
-    const int upto = wave_scan(nb);
-    const uint64_t past = __builtin_amdgcn_ballot_w64(before + upto > tile);
-    if (past != 0) {
-      const int at = __builtin_ctzll(past);
-      return {true, s0 + at,
-              before + __builtin_amdgcn_readlane(upto, at) - __builtin_amdgcn_readlane(nb, at)};
+  for (int s0 = 0; s0 < num_seqs; s0 += 128) {
+    int end[2][4];
+#pragma unroll
+    for (int n = 0; n < 2; ++n) {
+      const int s = min(s0 + 64 * n + lane, num_seqs - 1);
+      end[n][0] = cu[s];
+      end[n][1] = cu[s + 1];
+      end[n][2] = cu_other[s];
+      end[n][3] = cu_other[s + 1];
     }
-    before += __builtin_amdgcn_readlane(upto, 63);
+#pragma unroll
+    for (int n = 0; n < 2; ++n) {
+      const SeqRows mine = seq_rows(end[n][0], end[n][1], total);
+      const int nb = s0 + 64 * n + lane < num_seqs ? (mine.len + kRows - 1) / kRows : 0;
+      const int upto = wave_scan(nb);
+      const uint64_t past = __builtin_amdgcn_ballot_w64(before + upto > tile);
+      if (past != 0) {
+        const int at = __builtin_ctzll(past);
+        const SeqRows theirs = seq_rows(end[n][2], end[n][3], total_other);
+        auto pick = [at](int x) { return __builtin_amdgcn_readlane(x, at); };
+        return {true, before + pick(upto) - pick(nb), {pick(mine.row), pick(mine.len)},
+                {pick(theirs.row), pick(theirs.len)}};
+      }
+      before += __builtin_amdgcn_readlane(upto, 63);
+    }
   }
-  return {false, 0, before};
+  return {false, before, {}, {}};
 }
 
 // Zeros for one head of the rows that belong to no sequence (in front of the
@@ -311,14 +334,13 @@ __global__ __launch_bounds__(kBwdThreads, 2) void varlen_dq_kernel(VarlenBwdPara
   const int pick = (int)(blockIdx.x % (unsigned)p.num_heads);
   const int group = p.num_heads / p.num_kv_heads;
   const int kv = pick % p.num_kv_heads, head = kv * group + pick / p.num_kv_heads;
-  const BwdBlock blk = find_block<kRows>(p.cu_q, p.num_seqs, p.total_q, tile);
+  const BwdBlock blk = find_block<kRows>(p.cu_q, p.cu_k, p.num_seqs, p.total_q, p.total_k, tile);
   if (!blk.found) {
     zero_rest<D, kBwdThreads>(p.cu_q, p.num_seqs, p.total_q, p.dq, p.dq_st, head * p.dq_sh,
                               tile - blk.first, p.q_tiles - blk.first);
     return;
   }
-  const SeqRows qs = seq_rows(p.cu_q, blk.seq, p.total_q);
-  const SeqRows ks = seq_rows(p.cu_k, blk.seq, p.total_k);
+  const SeqRows qs = blk.rows, ks = blk.other;
   const int i0 = (tile - blk.first) * kRows;  // the block's first query
   const int ahead = ks.len - qs.len;         // causal: query i sees keys j <= i + ahead
   const int kend = p.causal ? min(max(ahead + min(i0 + kRows, qs.len), 0), ks.len) : ks.len;
@@ -524,13 +546,14 @@ struct DkvBlock {
   int empty;   // not found: the tiles that are there
 };
 __device__ inline DkvBlock dkv_block(const VarlenBwdParams& p, int tile) {
-  const BwdBlock blk = find_block<kDkvKeys>(p.cu_k, p.num_seqs, p.total_k, tile);
+  const BwdBlock blk =
+      find_block<kDkvKeys>(p.cu_k, p.cu_q, p.num_seqs, p.total_k, p.total_q, tile);
   DkvBlock b{};
   b.found = blk.found;
   b.empty = blk.first;
   if (!blk.found) return b;
-  b.qs = seq_rows(p.cu_q, blk.seq, p.total_q);
-  b.ks = seq_rows(p.cu_k, blk.seq, p.total_k);
+  b.qs = blk.other;
+  b.ks = blk.rows;
   b.j0 = (tile - blk.first) * kDkvKeys;
   b.t0 = p.causal ? max(b.j0 - (b.ks.len - b.qs.len), 0) / kDkvTile : 0;
   b.nt = max((b.qs.len + kDkvTile - 1) / kDkvTile - b.t0, 0);
@@ -856,13 +879,305 @@ __global__ __launch_bounds__(256) void varlen_dkv_sum_kernel(VarlenBwdParams p) 
       make_uint2(pack_pair<kBF16>(acc[0], acc[1]), pack_pair<kBF16>(acc[2], acc[3]));
 }
 
-// Both launches for one 16-bit type and head_dim, instantiated in
+// ------------------------------------------------------- short sequences, at once
+// Sequences of at most kWindowMost rows (an encoder's windows) at head_dim 64, a kv
+// head to each query head: one workgroup takes a sequence's head whole.  q, dout, k
+// and v come to LDS once, in as many rows as the longest sequence has (104 rows let
+// three workgroups share a CU); every wave forms dq of 32 queries, leaves lse and
+// -delta in LDS, and then dk and dv of 32 keys.  The launches above read the four
+// twice, and a launch waits for the other: 160 windows of 13 to 104 rows and 14 heads
+// take 36 us at once (134 MB, 3.7 TB/s) and 54 in two launches, 4 windows 10.9 and
+// 13.1.  What bounds many windows is HBM and each workgroup's own length, some 10 us
+// with three to a CU; few windows, that length alone.  Rows past the sequence's last
+// are never in LDS: what stands for them is the last row, and is masked.
+constexpr int kWindowMost = 128;
+constexpr int kWindowStats = 2 * kWindowMost * 4 + 4 * 4;  // bytes: lse, -delta, f16: largest |dout|s
+inline size_t window_lds(int rows) {
+  const size_t tile = (size_t)((rows + 7) / 8 * 8) * 128;
+  return std::max(4 * tile, 2 * tile + kWindowStats + 4 * 32 * 128);
+}
+constexpr int kWindowExtra = 2048;  // rows outside the sequences to a workgroup and head
+
+// LDS offsets in a tile of 64-element rows: of row r's chunk for the lane's half (8
+// elements from 16 step + 8 half: ^ step << 5), and of the transposed read of row r
+// (32 elements from 32 dt: ^ dt << 6).
+__device__ inline int window_row(int r, int half) { return r * 128 + ((half ^ bwd_swz<64>(r)) << 4); }
+__device__ inline int window_tr(int r, int lane) {
+  const int c = 2 * ((lane >> 4) & 1) + ((lane >> 1) & 1);
+  return r * 128 + ((lane & 1) << 3) + ((c ^ bwd_swz<64>(r)) << 4);
+}
+
+// Adds to acc the products of a tile's rows r0 ... r0 + 31 (transposed) and x.
+template <bool kBF16>
+__device__ inline void window_sum(f32x16_t (&acc)[2], const f32x16_t& x, const char* tile, int r0,
+                                  int last, int lane) {
+#pragma unroll
+  for (int hf = 0; hf < 2; ++hf) {
+    const int r = r0 + 16 * hf + 4 * (lane >> 5) + ((lane & 15) >> 2);
+    const int lo = window_tr(min(r, last), lane), hi = window_tr(min(r + 8, last), lane);
+    const uint4 b = pack_b<kBF16>(x, hf);
+#pragma unroll
+    for (int dt = 0; dt < 2; ++dt) {
+      const uint2 a = __builtin_bit_cast(uint2, lds_read_tr(tile, lo ^ (dt << 6)));
+      const uint2 c = __builtin_bit_cast(uint2, lds_read_tr(tile, hi ^ (dt << 6)));
+      acc[dt] = mfma32<kBF16>(make_uint4(a.x, a.y, c.x, c.y), b, acc[dt]);
+    }
+  }
+}
+
+template <bool kBF16>
+__global__ __launch_bounds__(kBwdThreads, 3) void varlen_window_kernel(VarlenBwdParams p) {
+  constexpr int D = 64, ROWB = D * 2, DS = D / 16, DT = D / 32, kAhead = 4;
+  extern __shared__ __align__(16) char s_all[];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63, l32 = lane & 31, half = lane >> 5;
+  const int seq = (int)(blockIdx.x / (unsigned)p.num_heads);
+  const int head = (int)(blockIdx.x % (unsigned)p.num_heads);
+  if (seq >= p.num_seqs) {
+    const int nth = seq - p.num_seqs, of = (int)(gridDim.x / (unsigned)p.num_heads) - p.num_seqs;
+    zero_rest<D, kBwdThreads>(p.cu_q, p.num_seqs, p.total_q, p.dq, p.dq_st, head * p.dq_sh, nth, of);
+    zero_rest_kv<D>(p, head, nth, of);
+    return;
+  }
+  SeqRows qs = seq_rows(p.cu_q[seq], p.cu_q[seq + 1], p.total_q);
+  SeqRows ks = seq_rows(p.cu_k[seq], p.cu_k[seq + 1], p.total_k);
+  char* const dq = p.dq + (int64_t)qs.row * p.dq_st + head * p.dq_sh;
+  char* const dk = p.dk + (int64_t)ks.row * p.dk_st + head * p.dk_sh;
+  char* const dv = p.dv + (int64_t)ks.row * p.dv_st + head * p.dv_sh;
+  // (Rows past the longest sequence that was spoken of get zeros.)
+  for (int i = p.window * 8 + threadIdx.x; i < max(qs.len, ks.len) * 8; i += kBwdThreads) {
+    const uint4 zero = make_uint4(0, 0, 0, 0);
+    if (i / 8 < qs.len) st16(dq + (i / 8) * p.dq_st + i % 8 * 16, zero);
+    if (i / 8 < ks.len) st16(dk + (i / 8) * p.dk_st + i % 8 * 16, zero);
+    if (i / 8 < ks.len) st16(dv + (i / 8) * p.dv_st + i % 8 * 16, zero);
+  }
+  qs.len = min(qs.len, p.window);
+  ks.len = min(ks.len, p.window);
+  const int ahead = ks.len - qs.len;
+  const int tile_b = (p.window + 7) / 8 * 8 * ROWB;
+  char* const sq = s_all;
+  char* const sd = sq + tile_b;
+  char* const sk = sd + tile_b;
+  char* const sv = sk + tile_b;
+  // In K's and V's place, once every wave has its keys in registers.
+  float* const s_lse = reinterpret_cast<float*>(sk);
+  float* const s_delta = s_lse + kWindowMost;
+  float* const s_top = s_delta + kWindowMost;
+  char* const s_out = sk + kWindowStats + wave * 32 * ROWB;  // the wave's rows on their way out
+  const uint32_t lds = __builtin_amdgcn_readfirstlane(
+      (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)s_all);
+  // 8 rows a copy, the waves in turn.
+  auto fetch = [&](const char* src, int64_t st, int len, int n) {
+    const int in8 = lane / 8;
+    for (int r0 = wave * 8; r0 < len; r0 += 32) {
+      const int r = r0 + in8;
+      const uint32_t chunk = (uint32_t)(((lane % 8) ^ bwd_swz<D>(r)) << 4);
+      dma16((uint32_t)min(in8, len - 1 - r0) * (uint32_t)st + chunk, src + r0 * st,
+            lds + (uint32_t)(n * tile_b + r0 * ROWB));
+    }
+  };
+  fetch(p.q + (int64_t)qs.row * p.q_st + head * p.q_sh, p.q_st, qs.len, 0);
+  fetch(p.dout + (int64_t)qs.row * p.do_st + head * p.do_sh, p.do_st, qs.len, 1);
+  fetch(p.k + (int64_t)ks.row * p.k_st + head * p.k_sh, p.k_st, ks.len, 2);
+  fetch(p.v + (int64_t)ks.row * p.v_st + head * p.v_sh, p.v_st, ks.len, 3);
+  const int first = 32 * wave, row = first + l32;  // the wave's queries, then its keys
+  uint4 oreg[DS] = {};
+  if (first < qs.len) {
+    const char* const op =
+        p.out + (int64_t)(qs.row + min(row, qs.len - 1)) * p.o_st + head * p.o_sh + half * 16;
+#pragma unroll
+    for (int ds = 0; ds < DS; ++ds) oreg[ds] = ld16(op + ds * 32);
+  }
+  wait_vmcnt<0>();
+  __syncthreads();
+
+  float top = 0.f, lse = 0.f, delta = 0.f, mul = 0.f;
+  f32x16_t acc[DT];  // dq
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt) acc[dt] = f32x16_t{};
+  if (first < qs.len) {
+    uint4 qreg[DS], doreg[DS];
+    const int own = window_row(min(row, qs.len - 1), half);
+#pragma unroll
+    for (int ds = 0; ds < DS; ++ds) {
+      qreg[ds] = lds_read16(sq, own ^ (ds << 5));
+      doreg[ds] = lds_read16(sd, own ^ (ds << 5));
+    }
+    using ET = std::conditional_t<kBF16, BF16, F16>;
+#pragma unroll
+    for (int ds = 0; ds < DS; ++ds) {
+      float a[8], b[8];
+      ET::unpack(doreg[ds], a);
+      ET::unpack(oreg[ds], b);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        delta = fmaf(a[i], b[i], delta);
+        if constexpr (!kBF16) top = fmaxf(top, fabsf(a[i]));
+      }
+    }
+    delta = sum_xor32(delta);
+    int e = 0;
+    if constexpr (!kBF16) {
+      top = max_xor32(top);
+      e = top_exponent(top);
+    }
+    const int lim = p.causal ? min(ks.len, ahead + row + 1) : ks.len;
+    const int lim_lo = p.causal ? min(ks.len, ahead + first + 1) : ks.len;
+    const int lim_hi = p.causal ? min(ks.len, ahead + min(first + 32, qs.len)) : ks.len;
+    constexpr float kSlack = kBF16 ? kLazy : 0.f;
+    float m = -1.0e30f, l = 0.f;
+    for (int j0 = 0; j0 < lim_hi; j0 += 32) {
+      const int ra = window_row(min(j0 + l32, ks.len - 1), half);
+      uint4 op[kAhead];
+      auto request = [&](int n) {
+        if (n < 2 * DS) op[n % kAhead] = lds_read16(n & 1 ? sv : sk, ra ^ (n / 2 << 5));
+      };
+#pragma unroll
+      for (int n = 0; n < kAhead; ++n) request(n);
+      f32x16_t s = {}, dp;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) dp[i] = -delta;
+#pragma unroll
+      for (int n = 0; n < 2 * DS; ++n) {
+        if (n & 1)
+          dp = mfma32<kBF16>(op[n % kAhead], doreg[n / 2], dp);
+        else
+          s = mfma32<kBF16>(op[n % kAhead], qreg[n / 2], s);
+        request(n + kAhead);
+      }
+      if (j0 + 32 > lim_lo) {
+        const int rel = lim - j0 - 4 * half;
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          if (8 * (i / 4) + i % 4 >= rel) s[i] = -INFINITY;
+      }
+      float mx = s[0];
+#pragma unroll
+      for (int i = 1; i < 16; ++i) mx = fmaxf(mx, s[i]);
+      mx = max_xor32(mx) * p.scale_log2;
+      if (__builtin_amdgcn_ballot_w64(mx > m + kSlack) != 0) {
+        const float mn = fmaxf(m, mx);
+        const float alpha = fast_exp2(m - mn);
+        m = mn;
+        l *= alpha;
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) acc[dt] *= alpha;
+      }
+      const float base = kBF16 ? m : m + (float)e;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        s[i] = fast_exp2(fmaf(s[i], p.scale_log2, -base));
+        l += s[i];
+        dp[i] *= s[i];
+      }
+      window_sum<kBF16>(acc, dp, sk, j0, ks.len - 1, lane);
+    }
+    l = sum_xor32(l);
+    lse = l > 0.f ? (kBF16 ? m : m + (float)e) + __builtin_amdgcn_logf(l) -
+                        (kBF16 ? 0.f : (float)kF16Lift)
+                  : INFINITY;
+    mul = l > 0.f ? p.scale / l : 0.f;
+  }
+  __syncthreads();  // every wave has been through K and V
+  uint4 kreg[DS] = {}, vreg[DS] = {};
+  if (first < ks.len) {
+    const int own = window_row(min(row, ks.len - 1), half);
+#pragma unroll
+    for (int ds = 0; ds < DS; ++ds) {
+      kreg[ds] = lds_read16(sk, own ^ (ds << 5));
+      vreg[ds] = lds_read16(sv, own ^ (ds << 5));
+    }
+  }
+  __syncthreads();
+  if constexpr (!kBF16) {
+    top = group_max<64>(top);
+    if (lane == 0) s_top[wave] = top;
+  }
+  if (first < qs.len) {
+    // Rows past the sequence's last, too: the queries' blocks below read them.
+    if (half == 0) {
+      s_lse[row] = lse;
+      s_delta[row] = -delta;
+    }
+    write_rows<kBF16, D>(acc, mul, s_out, dq, p.dq_st, first, qs.len, lane);
+  }
+  __syncthreads();
+  if (first >= ks.len) return;
+  float lift = 1.f, lower = 1.f;
+  if constexpr (!kBF16) {
+    const int e = top_exponent(fmaxf(fmaxf(s_top[0], s_top[1]), fmaxf(s_top[2], s_top[3])));
+    lift = pow2(-e - kF16Lift);
+    lower = pow2(e);
+  }
+
+  f32x16_t acc_k[DT], acc_v[DT];
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt) acc_k[dt] = acc_v[dt] = f32x16_t{};
+  // The first 32 queries of which one sees a key of the wave.
+  for (int i0 = p.causal ? max(first - ahead, 0) / 32 * 32 : 0; i0 < qs.len; i0 += 32) {
+    const int ra = window_row(min(i0 + l32, qs.len - 1), half);
+    uint4 op[kAhead];
+    auto request = [&](int n) {
+      if (n < 2 * DS) op[n % kAhead] = lds_read16(n & 1 ? sd : sq, ra ^ (n / 2 << 5));
+    };
+#pragma unroll
+    for (int n = 0; n < kAhead; ++n) request(n);
+    f32x16_t s = {}, dp;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const f32x4_t d = *reinterpret_cast<const f32x4_t*>(s_delta + i0 + 4 * half + 8 * j);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) dp[4 * j + i] = d[i];
+    }
+#pragma unroll
+    for (int n = 0; n < 2 * DS; ++n) {
+      if (n & 1)
+        dp = mfma32<kBF16>(op[n % kAhead], vreg[n / 2], dp);
+      else
+        s = mfma32<kBF16>(op[n % kAhead], kreg[n / 2], s);
+      request(n + kAhead);
+    }
+    const bool edge = p.causal && i0 + ahead < first + 31;
+    if (edge || i0 + 32 > qs.len) {
+      // Query 8 (i / 4) + i % 4 sees the lane's key iff >= rel, and is there iff < end.
+      const int rel = edge ? row - ahead - i0 - 4 * half : 0, end = qs.len - i0 - 4 * half;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const int c = 8 * (i / 4) + i % 4;
+        if (c < rel || c >= end) s[i] = -INFINITY;
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const f32x4_t at = *reinterpret_cast<const f32x4_t*>(s_lse + i0 + 4 * half + 8 * j);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        s[4 * j + i] = fast_exp2(fmaf(s[4 * j + i], p.scale_log2, -at[i]));
+        dp[4 * j + i] *= kBF16 ? s[4 * j + i] : s[4 * j + i] * lift;
+      }
+    }
+    window_sum<kBF16>(acc_v, s, sd, i0, qs.len - 1, lane);
+    window_sum<kBF16>(acc_k, dp, sq, i0, qs.len - 1, lane);
+  }
+  write_rows<kBF16, D>(acc_v, kBF16 ? 1.f : pow2(-kF16Lift), s_out, dv, p.dv_st, first, ks.len, lane);
+  write_rows<kBF16, D>(acc_k, p.scale * lower, s_out, dk, p.dk_st, first, ks.len, lane);
+}
+
+// The launches for one 16-bit type and head_dim, instantiated in
 // varlen_backward_<type>.hip.
 template <bool kBF16, int D>
 void launch_varlen_backward(const VarlenBwdParams& p, hipStream_t st);
 
 template <bool kBF16, int D>
 static void launch_varlen_backward_d(const VarlenBwdParams& p, hipStream_t st) {
+  if constexpr (D == 64) {
+    if (p.window > 0) {
+      const unsigned items = (unsigned)p.num_seqs + 1 + std::max(p.total_q, p.total_k) / kWindowExtra;
+      hipLaunchKernelGGL((varlen_window_kernel<kBF16>), dim3(items * p.num_heads),
+                         dim3(kBwdThreads), window_lds(p.window), st, p);
+      return;
+    }
+  }
   const dim3 q_grid((unsigned)p.q_tiles * p.num_heads);
   if (p.q_rows == 64)
     hipLaunchKernelGGL((varlen_dq_kernel<kBF16, D, true>), q_grid, dim3(kBwdThreads), 0, st, p);

@@ -1268,6 +1268,12 @@ def _apart(new: torch.Tensor, old: torch.Tensor) -> bool:
     return b <= c or d <= a
 
 
+def _length(n: int, name: str) -> int:
+    n = int(n)
+    _require(0 <= n < 2 ** 31, f"{name} must be a length")
+    return n
+
+
 def varlen_attention_backward(
     dout: torch.Tensor,
     q: torch.Tensor,
@@ -1290,19 +1296,22 @@ def varlen_attention_backward(
 
     q, k, v, cu_seqlens, scale and causal are those of the forward call (16-bit
     rows, head_dim 64 or 128; any group size); k and v of ``cu_seqlens_k``'s
-    rows, [total_k, Hkv, D].  The probabilities are recomputed.  Lengths come
-    from the cumulative lengths alone (the maxima are there for the forward
-    call's arguments, and not read).  Rows outside every sequence, queries that
-    see no key and keys that no query sees get zeros.  ``dq``, ``dk``, ``dv``:
-    tensors to write into (views of one buffer, say); they may not overlap the
-    inputs.  Two or three launches on the current stream, no atomics: the
-    results repeat bit for bit."""
+    rows, [total_k, Hkv, D].  The probabilities are recomputed.  The maxima
+    must be at least every length, as in the forward call, or 0 if they are not
+    known: sequences of at most 128 rows at head_dim 64, with as many kv heads as
+    heads, take one launch, which leaves zeros in rows past the maxima; others
+    take two or three and go by the cumulative lengths.  Rows outside every
+    sequence, queries that see no key and keys that no query sees get zeros.
+    ``dq``, ``dk``, ``dv``: tensors to write into (views of one buffer, say); they
+    may not overlap the inputs.  All launches are on the current stream, without
+    atomics: the results repeat bit for bit."""
     if dq is None and dk is None and dv is None:
         fast, index = _fast_on(q, LAYOUT_NHD)
         if fast is not None:
             rc, made = fast.varlen_attention_backward(dout, q, k, v, out, cu_seqlens_q,
-                                                      cu_seqlens_k, float(scale), bool(causal),
-                                                      index, _raw_stream(index))
+                                                      cu_seqlens_k, int(max_seqlen_q),
+                                                      int(max_seqlen_k), float(scale),
+                                                      bool(causal), index, _raw_stream(index))
             if rc == 0:
                 return tuple(made)
             if _FAST_NOT_TAKEN < rc < 0:
@@ -1339,7 +1348,9 @@ def varlen_attention_backward(
         struct_size=_VARLEN_BWD_ARGS_SIZE, dtype=_dtype_code(q),
         cu_seqlens_q=cu_seqlens_q.data_ptr(), cu_seqlens_k=cu_seqlens_k.data_ptr(),
         num_seqs=cu_seqlens_q.numel() - 1, total_q=total_q, total_k=total_k, num_heads=hq,
-        num_kv_heads=hkv, head_dim=d, causal=1 if causal else 0, scale=float(scale))
+        num_kv_heads=hkv, head_dim=d, max_seqlen_q=_length(max_seqlen_q, "max_seqlen_q"),
+        max_seqlen_k=_length(max_seqlen_k, "max_seqlen_k"), causal=1 if causal else 0,
+        scale=float(scale))
     for name, t in (("q", q), ("k", k), ("v", v), ("out", out), ("dout", dout), ("dq", dq),
                     ("dk", dk), ("dv", dv)):
         _require(t.stride(2) == 1, f"{name}: the last dimension must be contiguous")
