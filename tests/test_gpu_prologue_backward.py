@@ -116,6 +116,10 @@ def test_refusals(dev):
             ops.qk_norm_rope_backward(*bad, pro)
     with pytest.raises(ops.AttentionArgumentError, match="match"):
         ops.qk_norm_rope_backward(dq, dk, q, k, pro, dk=q)
+    with pytest.raises(ops.AttentionArgumentError, match="dq may not overlap the inputs"):
+        ops.qk_norm_rope_backward(dq[:, :2], dk, q[:, :2], k, pro, dq=k)
+    with pytest.raises(ops.AttentionArgumentError, match="dq may not overlap the inputs"):
+        ops.qk_norm_rope_backward(dq[:, :2], dk, q[:, :2], k, pro, dq=q[:, 1:3])
 
 
 # ------------------------------------------------------------- the training pass of the core

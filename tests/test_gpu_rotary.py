@@ -98,6 +98,29 @@ def test_no_tokens_and_refusals(dev):
             ops.rotary_embedding(*bad)
     with pytest.raises(ops.AttentionArgumentError, match="q_out"):
         ops.rotary_embedding(None, x, table, pos, q_out=x)
+    y = torch.zeros_like(x)
+    with pytest.raises(ops.AttentionArgumentError, match="overlap the inputs"):
+        ops.rotary_embedding(x, y, table, pos, q_out=y)
+    with pytest.raises(ops.AttentionArgumentError, match="overlap the inputs"):
+        ops.rotary_embedding(x[:4], y[:4], table, pos, q_out=x[1:5])
+    with pytest.raises(ops.AttentionArgumentError, match="k_out may not overlap q_out"):
+        ops.rotary_embedding(x, x, table, pos, q_out=y, k_out=y)
+
+
+def test_offsets_past_32_bits(dev):
+    # 300 tokens 16 MiB apart, the heads' rows side by side, into the columns behind them.
+    n, step = 300, 8 << 20
+    buf = torch.empty(n * step, dtype=torch.bfloat16, device=dev)
+    view = lambda heads, at: buf.as_strided((n, heads, 64), (step, 64, 1), at * 64)  # noqa: E731
+    g = torch.Generator().manual_seed(9)
+    x = torch.randn(n, 3, 64, generator=g).to(torch.bfloat16)
+    q, k, qo, ko = view(2, 0), view(1, 2), view(2, 3), view(1, 5)
+    q.copy_(x[:, :2])
+    k.copy_(x[:, 2:])
+    table, pos = _table(64), torch.randint(0, 300, (n,), generator=g)
+    ops.rotary_embedding(q, k, table.to(dev), pos.to(dev), interleaved=True, q_out=qo, k_out=ko)
+    _check(qo, x[:, :2], table, pos, True, False)
+    _check(ko, x[:, 2:], table, pos, True, False)
 
 
 @pytest.mark.parametrize("interleaved", [False, True])

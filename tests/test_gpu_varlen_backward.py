@@ -200,6 +200,11 @@ def test_no_sequences_no_rows(dev):
     assert not dk.any() and not dv.any() and dq.numel() == 0
     dq, dk, dv = _call(dev, q, k[:0], v[:0], dout, out, cu, cu * 0, 0.125, True)
     assert not dq.any() and dk.numel() == 0
+    on = [t.to(dev) for t in (dout, q, q, q, out, cu * 0, cu)]
+    for a, b in ((slice(0), slice(5)), (slice(5), slice(0))):  # the same of short sequences
+        call = [on[0][a], on[1][a], on[2][b], on[3][b], on[4][a]]
+        for t in ops.varlen_attention_backward(*call, on[5], on[5], 3, 3, scale=0.125, causal=True):
+            assert not t.any()
 
 
 def test_strided_rows_and_gradients_into_one_buffer(dev):
@@ -219,6 +224,31 @@ def test_strided_rows_and_gradients_into_one_buffer(dev):
     major = [t.to(dev).transpose(0, 1).contiguous().transpose(0, 1) for t in (dout, q, k, v, out)]
     _check(ops.varlen_attention_backward(*major, cu.to(dev), cu.to(dev), 90, 90, scale=0.09,
                                          causal=True), want)
+
+
+@pytest.mark.parametrize("d,hkv,most", [(128, 1, 150), (64, 2, 0), (64, 2, 110)])
+def test_offsets_past_32_bits(dev, d, hkv, most):
+    # Tokens 24 MiB apart in one buffer of 6.6 GB: a tile's last row lies 1.5 GB behind its first.
+    lens, step = [110, 150], 12 << 20
+    if most == 110:
+        lens = [110, 110]
+    n = sum(lens)
+    buf = torch.empty(n * step + 4096, dtype=torch.bfloat16, device=dev)
+    q, k, v, dout, out, cu, _ = _inputs(lens, lens, 2, hkv, d, torch.bfloat16, 21)
+    at = 0
+
+    def place(like, fill):
+        nonlocal at
+        t = buf.as_strided((n, like.shape[1], d), (step, d, 1), at)
+        at += like.shape[1] * d
+        return t.copy_(like) if fill else t
+
+    on = [place(t, True) for t in (dout, q, k, v, out)]
+    dq, dk, dv = (place(t, False) for t in (q, k, v))
+    c = cu.to(dev)
+    got = ops.varlen_attention_backward(*on, c, c, most, most, scale=0.125, causal=True, dq=dq, dk=dk,
+                                        dv=dv)
+    _check(got, G.varlen_attention_backward(dout, q, k, v, out, cu, cu, 0.125, True))
 
 
 def test_calls_repeat_bit_for_bit_on_any_stream(dev):
@@ -271,6 +301,11 @@ def test_refusals(dev):
         call(dout, q, k, v, out, dq=dout)
     with pytest.raises(ops.AttentionArgumentError, match="match"):
         call(dout, q, k, v, out, dk=q)
+    new = torch.zeros_like(k)
+    with pytest.raises(ops.AttentionArgumentError, match="dv may not overlap dk"):
+        call(dout, q, k, v, out, dk=new, dv=new)
+    with pytest.raises(ops.AttentionArgumentError, match="length"):
+        ops.varlen_attention_backward(dout, q, k, v, out, cu, cu, -1, 8, scale=1.0, causal=True)
     with pytest.raises(ops.AttentionArgumentError, match="int32"):
         ops.varlen_attention_backward(dout, q, k, v, out, cu.long(), cu, 8, 8, scale=1.0, causal=True)
     wide = torch.zeros(8, 4, 65, dtype=torch.bfloat16, device=dev)[:, :, :64]
@@ -310,3 +345,34 @@ def test_autograd_of_the_decoder_layer_without_a_cache(dev):
     out.backward(dout.to(dev))
     want = G.varlen_attention_backward(dout, q, k, v, out.detach().cpu(), cu, cu, d ** -0.5, True)
     _check([t.grad for t in leaves], want)
+
+
+@pytest.mark.parametrize("heads", [(3, 3), (4, 2)])
+def test_a_captured_training_step(dev, heads):
+    """Forward and gradient in one graph, several replays with eager steps between them."""
+    lens, (hq, hkv), d = [104, 60, 1], heads, 64
+    q, k, v, dout, _, cu, _ = _inputs(lens, lens, hq, hkv, d, torch.bfloat16, 22, grad=1.0)
+    on, do = cu.to(dev), dout.to(dev)
+    leaves = [t.to(dev).requires_grad_() for t in (q, k, v)]
+
+    def step(xs):
+        out = ops.varlen_attention(*xs, on, on, 104, 104, scale=0.125, causal=True)
+        return torch.autograd.grad(out, xs, do)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            step(leaves)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step(leaves)
+    for i in range(4):
+        with torch.no_grad():
+            leaves[0].copy_(torch.roll(q, i, 1))
+        graph.replay()
+        torch.cuda.synchronize()
+        want = step([t.detach().clone().requires_grad_() for t in leaves])
+        for a, b in zip(got, want):
+            assert torch.equal(a, b), i

@@ -123,6 +123,11 @@ def test_attention_gradient_without_rows_is_no_call():
     assert left == 0 and 2 <= parts <= 16
     a.total_k = 0
     assert size(ctypes.byref(a)) == (plain + 255) // 256 * 256
+    # Short sequences with a kv head to each head take one launch and none.
+    a = _bwd_args(num_kv_heads=4, max_seqlen_q=128, max_seqlen_k=5)
+    assert size(ctypes.byref(a)) == 0
+    for name, x in (("max_seqlen_k", 129), ("max_seqlen_q", 0), ("num_kv_heads", 2)):
+        assert size(ctypes.byref(_bwd_args(**{**dict(num_kv_heads=4, max_seqlen_q=128, max_seqlen_k=5), name: x}))) > 0
 
 
 def test_cpu_tensors_are_refused():
@@ -134,9 +139,21 @@ def test_cpu_tensors_are_refused():
 
 def test_overlap_is_seen():
     x = torch.zeros(4, 6, 8)
-    assert not ops._apart(x[:, :2], x[:, 2:])  # views of one buffer's rows: within one another
     assert ops._apart(x[:2], x[2:]) and not ops._apart(x[:3], x[2:])
-    assert ops._apart(x[:0], x) and ops._apart(torch.zeros(3), x)
+    assert ops._apart(x[:0], x) and ops._apart(torch.zeros(4, 6, 8), x)
+    # Views of one buffer's rows: side by side, or sharing a head, or of other strides.
+    assert ops._apart(x[:, :2], x[:, 2:]) and ops._apart(x[:, 3:], x[1:, :3])
+    assert not ops._apart(x[:, :3], x[:, 2:]) and not ops._apart(x, x[:, 5:])
+    assert not ops._apart(x[:, :2], x.view(8, 3, 8)[:, 2:])
+    major = x.view(6, 4, 8).transpose(0, 1)  # heads far apart
+    assert ops._apart(major[:2], major[2:]) and not ops._apart(major, major[:, 2:])
+    # In place is the same memory, element for element, and only where it is allowed.
+    assert ops._in_place(x, x[:]) and not ops._in_place(x[:3], x[1:])
+    ops._outputs_apart([("a", x[:, :2], (x[:, :2],))], (x[:, 2:],))
+    for given, inputs in (([("a", x, ())], (x,)), ([("a", x[1:], (x[:3],))], (x[:3],)),
+                          ([("a", x, ()), ("b", x, ())], ())):
+        with pytest.raises(ops.AttentionArgumentError, match="overlap"):
+            ops._outputs_apart(given, inputs)
 
 
 def _rotary_args(**over):
@@ -192,6 +209,7 @@ def _prologue_args(**over):
     (dict(q_norm_weight=None), "norm weights"), (dict(weight_dtype=5), "weight_dtype"),
     (dict(positions_dtype=-1), "positions_dtype"), (dict(dk_stride_tok=4), "strides"),
     (dict(dq=(1 << 20) + 4), "aligned"), (dict(workspace=None), "workspace"), (dict(workspace_bytes=8), "workspace"),
+    (dict(q_norm_weight=(1 << 20) + 8), "norm weights"), (dict(num_tokens=2 ** 31 - 1, num_heads=50), "too many"),
 ])
 def test_c_abi_refuses_bad_prologue_gradients(over, says):
     assert N.lib().va_qk_norm_rope_backward(ctypes.byref(_prologue_args(**over)), None) < 0

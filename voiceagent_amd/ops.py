@@ -476,6 +476,45 @@ def _k_norm_rope(k: torch.Tensor, prologue: QKPrologue,
     return k_out
 
 
+def _apart(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether two [rows, heads, elements] tensors are seen to share no memory: one ends before
+    the other begins, or their rows (or heads) lie side by side in one buffer's."""
+    if a.numel() == 0 or b.numel() == 0:
+        return True
+    size = a.element_size()
+
+    def reach(t, but=-1):  # bytes from the first element to behind the last, of all dimensions but one
+        return sum((n - 1) * st for i, (n, st) in enumerate(zip(t.shape, t.stride())) if i != but
+                   ) * t.element_size() + t.element_size()
+
+    pa, pb = a.data_ptr(), b.data_ptr()
+    if pa + reach(a) <= pb or pb + reach(b) <= pa:
+        return True
+    for dim in (0, 1):
+        step = a.stride(dim) * size
+        if step > 0 and b.stride(dim) * b.element_size() == step:
+            wa, wb, at = reach(a, dim), reach(b, dim), (pb - pa) % step
+            if wa <= at and at + wb <= step:
+                return True
+    return False
+
+
+def _in_place(new: torch.Tensor, old: torch.Tensor) -> bool:
+    """Whether two tensors of one shape are the same memory, element for element."""
+    return new.data_ptr() == old.data_ptr() and new.stride() == old.stride()
+
+
+def _outputs_apart(given, inputs) -> None:
+    """Refuses outputs that share memory with one another or with an input, but for what may be
+    written in place.  given: (name, tensor, the inputs it may replace)."""
+    for i, (name, t, own) in enumerate(given):
+        for x in inputs:
+            _require(_apart(t, x) or (any(x is o for o in own) and _in_place(t, x)),
+                     f"{name} may not overlap the inputs")
+        for other, u, _ in given[:i]:
+            _require(_apart(t, u), f"{name} may not overlap {other}")
+
+
 def qk_norm_rope_backward(
     dq_out: torch.Tensor | None,
     dk_out: torch.Tensor,
@@ -490,7 +529,7 @@ def qk_norm_rope_backward(
     gradients of its outputs and its inputs q [T, Hq, D], k [T, Hkv, D]; the
     weights' sum over all tokens and heads.  fp32, rounded once: the forward's
     roundings to the element type count as the identity.  ``dq`` / ``dk`` may be
-    dq_out / dk_out or q / k themselves.  ``dq_out`` and ``q`` None: the keys
+    dq_out / dk_out or q / k themselves, and share no memory otherwise.  ``dq_out`` and ``q`` None: the keys
     alone (dq and dq_norm_weight are then None).  Two launches, no atomics."""
     if q is not None and dq_out is not None and dq is None and dk is None:
         fast, index = _fast_on(k, LAYOUT_NHD)
@@ -513,13 +552,16 @@ def qk_norm_rope_backward(
     args.dtype = _dtype_code(k)
     args.num_tokens, args.num_kv_heads, args.head_dim = T, hkv, d
     results = {"q": None, "k": None, "qw": None, "kw": None}
+    given = []
     for name, dz, x, dx in sides:
         _require(x.dim() == 3 and x.shape[0] == T and x.shape[2] == d and x.dtype == k.dtype,
                  "q must be [T, Hq, D] and k [T, Hkv, D] of one dtype")
         _require(dz.shape == x.shape and dz.dtype == x.dtype, f"d{name}_out must match {name}")
         if dx is None:
             dx = torch.empty(x.shape, dtype=x.dtype, device=device)
-        _require(dx.shape == x.shape and dx.dtype == x.dtype, f"d{name} must match {name}")
+        else:
+            _require(dx.shape == x.shape and dx.dtype == x.dtype, f"d{name} must match {name}")
+            given.append((f"d{name}", dx, (dz, x)))
         for field, t in ((f"d{name}_out", dz), (name, x), (f"d{name}", dx)):
             _rows(t, field)
             tok, head = _row_strides(t)
@@ -529,6 +571,7 @@ def qk_norm_rope_backward(
         weight = prologue.q_norm_weight if name == "q" else prologue.k_norm_weight
         results[name], results[name + "w"] = dx, torch.empty(d, dtype=weight.dtype, device=device)
         setattr(args, f"d{name}_weight", results[name + "w"].data_ptr())
+    _outputs_apart(given, [t for _, dz, x, _ in sides for t in (dz, x)])
     args.num_heads = 0 if q is None else int(q.shape[1])
     args.prologue = _prologue_struct(prologue, d, T)
     lib = N.lib()
@@ -612,7 +655,8 @@ def rotary_embedding(
     transposed rotation, the gradient of the other.  fp32, rounded once (16-bit
     or fp32 rows, any head_dim and strides; rows of 16-byte multiples go 16
     bytes at a time).  Positions are held to the table.  Outputs may be q / k
-    themselves; without outputs the call is differentiable in q and k."""
+    themselves, and share no memory otherwise; without outputs the call is
+    differentiable in q and k (the table is a constant)."""
     if (q_out is None and k_out is None and torch.is_grad_enabled() and
             ((q is not None and q.requires_grad) or (k is not None and k.requires_grad))):
         return _Rotary.apply(q, k, cos_sin_cache, positions, interleaved, inverse)
@@ -633,7 +677,7 @@ def rotary_embedding(
     args = N.new_args(N.RotaryArgs)
     args.dtype = _dtype_code(like)
     args.num_tokens, args.head_dim = T, d
-    outs = []
+    outs, given = [], []
     for name, x, y in (("q", q, q_out), ("k", k, k_out)):
         if x is None:
             _require(y is None, f"{name}_out without {name}")
@@ -643,7 +687,9 @@ def rotary_embedding(
                  "q must be [T, Hq, D] and k [T, Hkv, D] of one dtype")
         if y is None:
             y = torch.empty(x.shape, dtype=x.dtype, device=device)
-        _require(y.shape == x.shape and y.dtype == x.dtype, f"{name}_out must match {name}")
+        else:
+            _require(y.shape == x.shape and y.dtype == x.dtype, f"{name}_out must match {name}")
+            given.append((f"{name}_out", y, (x,)))
         for field, t in ((name, x), (name + "_out", y)):
             _require(t.stride(2) == 1 or d == 1, f"{field}: the last dimension must be contiguous")
             tok, head = _row_strides(t)
@@ -651,6 +697,7 @@ def rotary_embedding(
             setattr(args, field + "_stride_tok", tok)
             setattr(args, field + "_stride_head", head)
         outs.append(y)
+    _outputs_apart(given, [x for x in (q, k) if x is not None])
     args.num_heads = 0 if q is None else int(q.shape[1])
     args.num_kv_heads = 0 if k is None else int(k.shape[1])
     cs = cos_sin_cache
@@ -1255,19 +1302,6 @@ def _row_strides(t: torch.Tensor) -> tuple[int, int]:
     return (t.stride(0) if n > 1 else 0), (t.stride(1) if h > 1 else 0)
 
 
-def _apart(new: torch.Tensor, old: torch.Tensor) -> bool:
-    """Whether two tensors' memory, first to last element, does not overlap."""
-    def span(t):
-        reach = [(n - 1) * st * t.element_size() for n, st in zip(t.shape, t.stride())]
-        return (t.data_ptr() + sum(r for r in reach if r < 0),
-                t.data_ptr() + sum(r for r in reach if r > 0) + t.element_size())
-
-    if new.numel() == 0 or old.numel() == 0:
-        return True
-    (a, b), (c, d) = span(new), span(old)
-    return b <= c or d <= a
-
-
 def _length(n: int, name: str) -> int:
     n = int(n)
     _require(0 <= n < 2 ** 31, f"{name} must be a length")
@@ -1337,10 +1371,8 @@ def varlen_attention_backward(
     for name, t, like in (("dq", dq, q), ("dk", dk, k), ("dv", dv, v)):
         if t is not None:
             _require(t.shape == like.shape and t.dtype == like.dtype, f"{name} must match {name[1]}")
-            given.append((name, t))
-    for name, t in given:
-        _require(all(_apart(t, x) for x in (dout, q, k, v, out)),
-                 f"{name} may not overlap the inputs")
+            given.append((name, t, ()))
+    _outputs_apart(given, (dout, q, k, v, out))
     dq = torch.empty(q.shape, dtype=q.dtype, device=device) if dq is None else dq
     dk = torch.empty(k.shape, dtype=k.dtype, device=device) if dk is None else dk
     dv = torch.empty(k.shape, dtype=k.dtype, device=device) if dv is None else dv
