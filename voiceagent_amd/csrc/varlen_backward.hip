@@ -10,11 +10,11 @@ namespace va {
 // How many workgroups share the queries that see a block of keys.  Few blocks,
 // each of them seen by many queries (long sequences, or several query heads to a
 // kv head), leave most of the chip idle otherwise: 4 sequences of 600 to 2000 rows,
-// 32 heads over 4 of 64, in f16 took 401 us, with 1, 2, 3 and 4 parts for each
-// place on the chip 401, 212, 192 and 199 with the parts' sum; a sequence of 420
-// rows 25, with parts of two steps at least 14.4 + 4.2, of one 12.0 + 8.  Where
+// 32 heads over 4 of 64, in f16 take 336 us whole, in 2, 3 and 4 workgroups for each
+// place on the chip 183 + 11 (the parts' sum), 166 + 14 and 171 + 17; a sequence of
+// 420 rows 26, in parts of two steps at least 14.5 + 4.3, of one 11.8 + 6.2.  Where
 // blocks are many, parts only add the sum: 8 answers behind prompts of 700 rows
-// 31 us, in parts 35 + 15.
+// 32 us, in parts 36 + 20.
 static int dkv_parts(const va_varlen_bwd_args* a) {
   if (a->num_seqs <= 0 || a->num_kv_heads <= 0 || a->total_q <= 0 || a->total_k <= 0) return 1;
   const int64_t blocks = ((int64_t)a->total_k / kDkvKeys + a->num_seqs) * a->num_kv_heads;
