@@ -721,9 +721,9 @@ std::tuple<int64_t, std::vector<at::Tensor>> varlen_attention_backward(
     const at::Tensor& out, const at::Tensor& cu_q, const at::Tensor& cu_k, int64_t max_q,
     int64_t max_k, double scale, bool causal, int64_t device, int64_t stream) {
   const std::tuple<int64_t, std::vector<at::Tensor>> none{kNotTaken, {}};
-  if (g_varlen_bwd == nullptr || max_q < 0 || max_k < 0 || !fits_i32(max_q) || !fits_i32(max_k) || !rows_on(dout, device) || !rows_on(q, device) ||
-      !rows_on(k, device) || !rows_on(v, device) || !rows_on(out, device) || !on(cu_q, device) ||
-      !on(cu_k, device))
+  if (g_varlen_bwd == nullptr || max_q < 0 || max_k < 0 || !fits_i32(max_q) || !fits_i32(max_k) ||
+      !rows_on(dout, device) || !rows_on(q, device) || !rows_on(k, device) || !rows_on(v, device) ||
+      !rows_on(out, device) || !on(cu_q, device) || !on(cu_k, device))
     return none;
   const auto t = q.scalar_type();
   if ((t != at::kBFloat16 && t != at::kHalf) || dout.scalar_type() != t || k.scalar_type() != t ||

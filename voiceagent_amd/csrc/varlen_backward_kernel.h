@@ -61,7 +61,7 @@ struct VarlenBwdParams {
   int32_t q_rows;            // queries of a workgroup of the first launch
   int32_t window;            // > 0: one launch, no sequence is longer than this
   int32_t parts;             // workgroups that share a block of keys' queries
-  float* part;               // parts > 1: their sums, [tile][part][kv head][wave][D / 8][64] x 4
+  float* part;               // parts > 1: their sums, [block][part][kv head][wave][D / 8][64] x 4
   float* lse;                // [num_heads][total_q]: log2 sum 2^(c log2 e s), f16: - kF16Lift
   float* delta;              // [num_heads][total_q]: -delta
   float* top;                // f16: [num_heads][total_q], largest |dout| of the row
@@ -96,23 +96,34 @@ __device__ inline SeqRows seq_rows(int a, int b, int total) {
   return {a, min(max(b, a), total) - a};
 }
 
-// The `tile`-th block of kRows rows of one side, counting every sequence's blocks
-// in turn, with its sequence's rows on both.  found: there is one; otherwise first
-// is the number of blocks there are.  The ends of 128 sequences, both sides', are
-// requested at once (64 in turn, and the found sequence's again, took 160 sequences
-// of 14 heads 27.1 us for dq and 30.9 for dk and dv instead of 26.3 and 29.2).
+// Orders of a launch's blocks.  kInTurn: sequence after sequence.  The others, up to
+// 128 sequences, are by the work under a causal mask, the most first, so that no
+// long block starts late: a sequence's n-th block has the keys of n blocks
+// (kByIndex: dq), and its n-th from the end the queries of n (kFromEnd: dk, dv).  32
+// sequences of 50 to 450 rows take 46 us for dk and dv so and 53.5 in turn; 4 of 600
+// to 2000 in f16 107 for dq and 119 (with a sequence's last block first).
+enum BwdOrder { kInTurn, kByIndex, kFromEnd };
+
+// The `tile`-th block of kRows rows of one side in that order, with its sequence's
+// rows on both.  found: there is one; otherwise `blocks` is how many there are.  The
+// ends of 128 sequences, both sides', are requested at once (64 in turn, and the
+// found sequence's again, took 160 sequences of 14 heads 27.1 us for dq and 30.9
+// for dk and dv instead of 26.3 and 29.2).
 struct BwdBlock {
   bool found;
-  int first;  // tile number of the sequence's first block
+  int index;   // of the block in its sequence
+  int blocks;
+  int place;   // found: its number in turn
   SeqRows rows, other;
 };
-template <int kRows>
+template <int kRows, BwdOrder kOrder>
 __device__ inline BwdBlock find_block(const int32_t* cu, const int32_t* cu_other, int num_seqs,
                                       int total, int total_other, int tile) {
   const int lane = threadIdx.x & 63;
+  auto pick = [](int x, int at) { return __builtin_amdgcn_readlane(x, at); };
   int before = 0;
   for (int s0 = 0; s0 < num_seqs; s0 += 128) {
-    int end[2][4];
+    int end[2][4], nb[2], upto[2];
 #pragma unroll
     for (int n = 0; n < 2; ++n) {
       const int s = min(s0 + 64 * n + lane, num_seqs - 1);
@@ -121,23 +132,63 @@ __device__ inline BwdBlock find_block(const int32_t* cu, const int32_t* cu_other
       end[n][2] = cu_other[s];
       end[n][3] = cu_other[s + 1];
     }
+    SeqRows mine[2], theirs[2];
 #pragma unroll
     for (int n = 0; n < 2; ++n) {
-      const SeqRows mine = seq_rows(end[n][0], end[n][1], total);
-      const int nb = s0 + 64 * n + lane < num_seqs ? (mine.len + kRows - 1) / kRows : 0;
-      const int upto = wave_scan(nb);
-      const uint64_t past = __builtin_amdgcn_ballot_w64(before + upto > tile);
-      if (past != 0) {
-        const int at = __builtin_ctzll(past);
-        const SeqRows theirs = seq_rows(end[n][2], end[n][3], total_other);
-        auto pick = [at](int x) { return __builtin_amdgcn_readlane(x, at); };
-        return {true, before + pick(upto) - pick(nb), {pick(mine.row), pick(mine.len)},
-                {pick(theirs.row), pick(theirs.len)}};
-      }
-      before += __builtin_amdgcn_readlane(upto, 63);
+      mine[n] = seq_rows(end[n][0], end[n][1], total);
+      theirs[n] = seq_rows(end[n][2], end[n][3], total_other);
+      nb[n] = s0 + 64 * n + lane < num_seqs ? (mine[n].len + kRows - 1) / kRows : 0;
+      upto[n] = wave_scan(nb[n]);
     }
+    const int c0 = pick(upto[0], 63), here = c0 + pick(upto[1], 63);
+    if (tile >= before + here) {
+      before += here;
+      continue;
+    }
+    int left = tile - before, n, at, index;
+    if (kOrder == kInTurn || num_seqs > 128) {
+      n = left >= c0;
+      left -= n ? c0 : 0;
+      at = __builtin_ctzll(__builtin_amdgcn_ballot_w64((n ? upto[1] : upto[0]) > left));
+      index = left - pick(n ? upto[1] : upto[0], at) + pick(n ? nb[1] : nb[0], at);
+    } else {
+      // Level by level of blocks that sequences have, those with the same sequences
+      // at once.
+      // (Floats hold the counts: 2^24 blocks of a sequence are 2^30 rows.)
+      int level = __builtin_amdgcn_readfirstlane((int)group_max<64>((float)max(nb[0], nb[1])));
+      uint64_t m[2];
+      int c[2];
+      while (true) {
+        int under = 0;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          m[i] = __builtin_amdgcn_ballot_w64(nb[i] >= level);
+          c[i] = __builtin_popcountll(m[i]);
+          under = max(under, nb[i] < level ? nb[i] : 0);
+        }
+        under = __builtin_amdgcn_readfirstlane((int)group_max<64>((float)under));
+        const int run = (c[0] + c[1]) * (level - under);
+        if (left < run) break;
+        left -= run;
+        level = under;
+      }
+      level -= left / (c[0] + c[1]);
+      left %= c[0] + c[1];
+      n = left >= c[0];
+      left -= n ? c[0] : 0;
+      const uint64_t in = n ? m[1] : m[0];
+      const int rank = __builtin_amdgcn_mbcnt_hi((uint32_t)(in >> 32),
+                                                 __builtin_amdgcn_mbcnt_lo((uint32_t)in, 0));
+      at = __builtin_ctzll(__builtin_amdgcn_ballot_w64((in >> lane & 1) != 0 && rank == left));
+      index = kOrder == kByIndex ? level - 1 : pick(n ? nb[1] : nb[0], at) - level;
+    }
+    const SeqRows& a = n ? mine[1] : mine[0];
+    const SeqRows& b = n ? theirs[1] : theirs[0];
+    return {true, index, 0,
+            before + (n ? c0 : 0) + pick(n ? upto[1] : upto[0], at) - pick(n ? nb[1] : nb[0], at) + index,
+            {pick(a.row, at), pick(a.len, at)}, {pick(b.row, at), pick(b.len, at)}};
   }
-  return {false, before, {}, {}};
+  return {false, 0, before, 0, {}, {}};
 }
 
 // Zeros for one head of the rows that belong to no sequence (in front of the
@@ -327,21 +378,19 @@ __global__ __launch_bounds__(kBwdThreads, 2) void varlen_dq_kernel(VarlenBwdPara
   __shared__ __align__(1024) char s_kv[2 * 2 * TILE_B];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int lane = threadIdx.x & 63, l32 = lane & 31, half = lane >> 5;
-  // Tiles run from the last to the first: under a causal mask a sequence's
-  // later blocks have more keys.  Consecutive workgroups, which run on
-  // different XCDs, take different kv heads.
-  const int tile = p.q_tiles - 1 - (int)(blockIdx.x / (unsigned)p.num_heads);
+  // Consecutive workgroups, which run on different XCDs, take different kv heads.
+  const int tile = (int)(blockIdx.x / (unsigned)p.num_heads);
   const int pick = (int)(blockIdx.x % (unsigned)p.num_heads);
   const int group = p.num_heads / p.num_kv_heads;
   const int kv = pick % p.num_kv_heads, head = kv * group + pick / p.num_kv_heads;
-  const BwdBlock blk = find_block<kRows>(p.cu_q, p.cu_k, p.num_seqs, p.total_q, p.total_k, tile);
+  const BwdBlock blk = find_block<kRows, kByIndex>(p.cu_q, p.cu_k, p.num_seqs, p.total_q, p.total_k, tile);
   if (!blk.found) {
     zero_rest<D, kBwdThreads>(p.cu_q, p.num_seqs, p.total_q, p.dq, p.dq_st, head * p.dq_sh,
-                              tile - blk.first, p.q_tiles - blk.first);
+                              tile - blk.blocks, p.q_tiles - blk.blocks);
     return;
   }
   const SeqRows qs = blk.rows, ks = blk.other;
-  const int i0 = (tile - blk.first) * kRows;  // the block's first query
+  const int i0 = blk.index * kRows;  // the block's first query
   const int ahead = ks.len - qs.len;         // causal: query i sees keys j <= i + ahead
   const int kend = p.causal ? min(max(ahead + min(i0 + kRows, qs.len), 0), ks.len) : ks.len;
   const int tiles = (kend + kTile - 1) / kTile;
@@ -544,17 +593,20 @@ struct DkvBlock {
   int t0, nt;  // tiles of queries that see it
   int steps;   // nt, for every head of the group
   int empty;   // not found: the tiles that are there
+  int place;   // its number in turn
 };
+template <BwdOrder kOrder>
 __device__ inline DkvBlock dkv_block(const VarlenBwdParams& p, int tile) {
   const BwdBlock blk =
-      find_block<kDkvKeys>(p.cu_k, p.cu_q, p.num_seqs, p.total_k, p.total_q, tile);
+      find_block<kDkvKeys, kOrder>(p.cu_k, p.cu_q, p.num_seqs, p.total_k, p.total_q, tile);
   DkvBlock b{};
   b.found = blk.found;
-  b.empty = blk.first;
+  b.empty = blk.blocks;
+  b.place = blk.place;
   if (!blk.found) return b;
   b.qs = blk.other;
   b.ks = blk.rows;
-  b.j0 = (tile - blk.first) * kDkvKeys;
+  b.j0 = blk.index * kDkvKeys;
   b.t0 = p.causal ? max(b.j0 - (b.ks.len - b.qs.len), 0) / kDkvTile : 0;
   b.nt = max((b.qs.len + kDkvTile - 1) / kDkvTile - b.t0, 0);
   b.steps = b.nt * (p.num_heads / p.num_kv_heads);
@@ -595,13 +647,12 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void varlen_dkv_kernel(Varlen
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int lane = threadIdx.x & 63, l32 = lane & 31, half = lane >> 5;
   const int pair = wave >> 1, role = wave & 1;  // role 0: first 32 queries, dv
-  // (Under a causal mask a sequence's earlier blocks are seen by more queries.)
   const int kv = (int)(blockIdx.x % (unsigned)p.num_kv_heads);
   const int unit = (int)(blockIdx.x / (unsigned)p.num_kv_heads);
   const int parts = kParts ? p.parts : 1;
   const int tile = unit / parts, part = unit % parts;
   const int group = p.num_heads / p.num_kv_heads;
-  const DkvBlock blk = dkv_block(p, tile);
+  const DkvBlock blk = dkv_block<kFromEnd>(p, tile);
   if (!blk.found) {
     if constexpr (!kParts) zero_rest_kv<D>(p, kv, tile - blk.empty, p.k_tiles - blk.empty);
     return;
@@ -828,7 +879,8 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void varlen_dkv_kernel(Varlen
   }
   const float mul = role == 1 ? p.scale * lower : kBF16 ? 1.f : pow2(-kF16Lift);
   if constexpr (kParts) {
-    float* const to = p.part + (((int64_t)unit * p.num_kv_heads + kv) * kWaves + wave) * (32 * D);
+    float* const to =
+        p.part + ((((int64_t)blk.place * parts + part) * p.num_kv_heads + kv) * kWaves + wave) * (32 * D);
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
@@ -848,7 +900,7 @@ template <bool kBF16, int D>
 __global__ __launch_bounds__(256) void varlen_dkv_sum_kernel(VarlenBwdParams p) {
   const int kv = (int)(blockIdx.x % (unsigned)p.num_kv_heads);
   const int tile = (int)(blockIdx.x / (unsigned)p.num_kv_heads);
-  const DkvBlock blk = dkv_block(p, tile);
+  const DkvBlock blk = dkv_block<kInTurn>(p, tile);
   if (!blk.found) {
     if (blockIdx.y == 0) zero_rest_kv<D>(p, kv, tile - blk.empty, p.k_tiles - blk.empty);
     return;
