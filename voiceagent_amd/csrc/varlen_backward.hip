@@ -9,19 +9,35 @@ namespace va {
 
 // How many workgroups share the queries that see a block of keys.  Few blocks,
 // each of them seen by many queries (long sequences, or several query heads to a
-// kv head), leave most of the chip idle otherwise: 4 sequences of 600 to 2000 rows,
-// 32 heads over 4 of 64, in f16 take 336 us whole, in 2, 3 and 4 workgroups for each
-// place on the chip 183 + 11 (the parts' sum), 166 + 14 and 171 + 17; a sequence of
-// 420 rows 26, in parts of two steps at least 14.5 + 4.3, of one 11.8 + 6.2.  Where
-// blocks are many, parts only add the sum: 8 answers behind prompts of 700 rows
-// 32 us, in parts 36 + 20.
+// kv head), leave most of the chip idle otherwise, and a block's steps (a tile of
+// queries of one head) come one after the other.  Parts save a block that all
+// queries see its share of them, about 1.5 us each at head_dim 128 and 1.2 at 64,
+// and cost a launch and their sums' way to memory and back.  At head_dim 128, 16
+// heads over 8, whole and in parts by this rule's estimate, us a gradient: one
+// sequence of 512 rows 43.7 and 34.0 (4 parts), two 44.2 and 42.1 (3), four 48.4
+// (whole; in 3 parts 57); one of 2000 142.7 and 108.1 (4); 4 of 600 to 2000, 32
+// heads over 4 of 64, dk and dv 291 and 165 (4 parts).  More than two workgroups
+// for each place on the chip, that one: 184 (6).
 static int dkv_parts(const va_varlen_bwd_args* a) {
   if (a->num_seqs <= 0 || a->num_kv_heads <= 0 || a->total_q <= 0 || a->total_k <= 0) return 1;
   const int64_t blocks = ((int64_t)a->total_k / kDkvKeys + a->num_seqs) * a->num_kv_heads;
   const int64_t slots = (a->head_dim == 64 ? 3 : 2) * (int64_t)current_device_cus();
   const int64_t tiles = ((int64_t)a->total_q / a->num_seqs + kDkvTile - 1) / kDkvTile;
-  const int64_t steps = tiles * (a->num_heads / a->num_kv_heads) / (a->causal ? 2 : 1);
-  return (int)std::max<int64_t>(1, std::min<int64_t>({3 * slots / blocks, steps / 2, 16}));
+  const int64_t steps = tiles * (a->num_heads / a->num_kv_heads);
+  const int64_t most =
+      std::min<int64_t>({2 * slots / blocks, steps / (a->causal ? 4 : 2), 16});  // (two steps a part)
+  const double step = a->head_dim == 64 ? 1.2 : 1.5;  // us
+  const double sums = 2.0 * (2 * kDkvKeys * a->head_dim * 4) / 8e6;  // us a block and part, at 8 TB/s
+  int parts = 1;
+  double best = 0;
+  for (int n = 2; n <= most; ++n) {
+    const double saved = step * (double)steps * (n - 1) / n - (4.0 + sums * (double)blocks * n);
+    if (saved > best) {
+      best = saved;
+      parts = n;
+    }
+  }
+  return parts;
 }
 
 // Queries of a workgroup of the first launch: two workgroups fit a CU, and where
