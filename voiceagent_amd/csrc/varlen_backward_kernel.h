@@ -514,6 +514,9 @@ __global__ __launch_bounds__(kBwdThreads, 2) void varlen_dq_kernel(VarlenBwdPara
       f32x16_t s = {}, dp;
 #pragma unroll
       for (int i = 0; i < 16; ++i) dp[i] = -delta;
+      // (The products ahead of the exponentials of the SIMD's other waves: a sequence of
+      // 8192 rows 388 us instead of 402, and 550 instead of 578 for dk and dv.)
+      __builtin_amdgcn_s_setprio(1);
 #pragma unroll
       for (int n = 0; n < 2 * DS; ++n) {
         if (n & 1)
@@ -524,6 +527,7 @@ __global__ __launch_bounds__(kBwdThreads, 2) void varlen_dq_kernel(VarlenBwdPara
         constexpr int kEvery = 2 * DS / kTurnCopies;
         if (n % kEvery == kEvery - 1 && more) issue(t + 1, turn * Copy::NI + n / kEvery);
       }
+      __builtin_amdgcn_s_setprio(0);
       if (j0 + 32 > lim_lo) {
         const int rel = lim - j0 - 4 * half;  // key 8 (i / 4) + i % 4 of the lane is seen iff < rel
 #pragma unroll
@@ -817,6 +821,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void varlen_dkv_kernel(Varlen
 #pragma unroll
         for (int i = 0; i < 4; ++i) dp[4 * j + i] = d[i];
       }
+      __builtin_amdgcn_s_setprio(1);
 #pragma unroll
       for (int n = 0; n < 2 * DS; ++n) {
         if (n & 1)
@@ -830,6 +835,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void varlen_dkv_kernel(Varlen
           if (n % kEvery == kEvery - 1) issue(kStage ^ 1, 1 + n / kEvery);
         }
       }
+      __builtin_amdgcn_s_setprio(0);
       // The first operands of the sums, past the exponentials.
 #pragma unroll
       for (int n = 0; n < kAhead && n < 2 * DT; ++n) op[n] = sums(n, 0);
