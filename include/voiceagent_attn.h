@@ -409,8 +409,8 @@ size_t va_varlen_split_workspace_bytes(const va_varlen_args* args);
  * q, k, v, out and dout are as in the forward call (any group size); rows that
  * belong to no sequence get a gradient of zeros, as do queries that see no key
  * and keys that no query sees.  Lengths come from cu_seqlens, held to the rows
- * there are; the maxima only choose the launch, and rows of a sequence past
- * both may get zeros instead.  No atomics: calls repeat bit for bit.  The
+ * there are; the maxima only choose the launch, and a sequence longer than a
+ * maximum of at most 128 may get NaN.  No atomics: calls repeat bit for bit.  The
  * gradients must not overlap the inputs or one another.  Pointers and strides
  * are 16-byte multiples; token strides of q, k, v and dout are from 0 to under
  * 32 MiB. */

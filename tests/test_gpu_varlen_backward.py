@@ -109,14 +109,18 @@ def test_short_sequences_of_any_values(dev):
             assert not t[265:].any()
 
 
-def test_rows_past_the_maxima_get_zeros(dev):
-    q, k, v, dout, out, cu, _ = _inputs([100, 300], [100, 300], 2, 2, 64, torch.bfloat16, 19)
-    on = [t.to(dev) for t in (dout, q, k, v, out, cu, cu)]
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_a_sequence_longer_than_the_maxima_gets_nan(dev, dtype):
+    lens_q, lens_k = [100, 300, 9, 20], [100, 300, 101, 20]
+    q, k, v, dout, out, cu_q, cu_k = _inputs(lens_q, lens_k, 2, 2, 64, dtype, 19)
+    on = [t.to(dev) for t in (dout, q, k, v, out, cu_q, cu_k)]
     got = ops.varlen_attention_backward(*on, 100, 100, scale=0.125, causal=False)
-    want = G.varlen_attention_backward(dout, q, k, v, out, cu, cu, 0.125, False)
-    for t, name in zip(got, NAMES):
-        assert ((t[:100].double().cpu() - want[name][:100]).abs() <= want[name + "_off"][:100]).all()
-        assert not t[200:].any()
+    want = G.varlen_attention_backward(dout, q, k, v, out, cu_q, cu_k, 0.125, False)
+    for t, name, cu in zip(got, NAMES, (cu_q, cu_k, cu_k)):
+        off = (t.double().cpu() - want[name]).abs() <= want[name + "_off"]
+        for i, right in enumerate((True, False, False, True)):
+            rows = slice(int(cu[i]), int(cu[i + 1]))
+            assert off[rows].all() if right else t[rows].isnan().all(), (name, i)
 
 
 def test_many_sequences(dev):

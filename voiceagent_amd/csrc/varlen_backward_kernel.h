@@ -651,8 +651,9 @@ __device__ inline void zero_rest_kv(const VarlenBwdParams& p, int kv, int nth, i
 // for the operands ahead.  (A wave that adds up both has none at head_dim 128: its
 // step of 32 queries took 3600 cycles for 1024 of matrix work.)  Eight waves that
 // add up both gradients of 128 keys, two for each 32 keys, are faster on one long
-// sequence and slower where there are few blocks: 8192 rows 530 us against 578,
-// windows of 104 rows 56 against 30, one sequence of 420 rows 31 against 25.
+// sequence and slower where there are few blocks: 8192 rows 530 us against 578 (550
+// with the priorities below), windows of 104 rows 56 against 30, one sequence of 420
+// rows 31 against 25.
 //
 // kParts: the block's steps are shared among several workgroups, whose sums a
 // third launch adds up (varlen_dkv_sum_kernel).
@@ -1016,20 +1017,21 @@ __global__ __launch_bounds__(kBwdThreads, 3) void varlen_window_kernel(VarlenBwd
     zero_rest_kv<D>(p, head, nth, of);
     return;
   }
-  SeqRows qs = seq_rows(p.cu_q[seq], p.cu_q[seq + 1], p.total_q);
-  SeqRows ks = seq_rows(p.cu_k[seq], p.cu_k[seq + 1], p.total_k);
+  const SeqRows qs = seq_rows(p.cu_q[seq], p.cu_q[seq + 1], p.total_q);
+  const SeqRows ks = seq_rows(p.cu_k[seq], p.cu_k[seq + 1], p.total_k);
   char* const dq = p.dq + (int64_t)qs.row * p.dq_st + head * p.dq_sh;
   char* const dk = p.dk + (int64_t)ks.row * p.dk_st + head * p.dk_sh;
   char* const dv = p.dv + (int64_t)ks.row * p.dv_st + head * p.dv_sh;
-  // (Rows past the longest sequence that was spoken of get zeros.)
-  for (int i = p.window * 8 + threadIdx.x; i < max(qs.len, ks.len) * 8; i += kBwdThreads) {
-    const uint4 zero = make_uint4(0, 0, 0, 0);
-    if (i / 8 < qs.len) st16(dq + (i / 8) * p.dq_st + i % 8 * 16, zero);
-    if (i / 8 < ks.len) st16(dk + (i / 8) * p.dk_st + i % 8 * 16, zero);
-    if (i / 8 < ks.len) st16(dv + (i / 8) * p.dv_st + i % 8 * 16, zero);
+  if (max(qs.len, ks.len) > p.window) {  // longer than the caller said: NaN, not some of it
+    const uint4 nan = make_uint4(0x7fff7fff, 0x7fff7fff, 0x7fff7fff, 0x7fff7fff);
+    for (int i = threadIdx.x / 8; i < max(qs.len, ks.len); i += kBwdThreads / 8) {
+      const int at = threadIdx.x % 8 * 16;
+      if (i < qs.len) st16(dq + i * p.dq_st + at, nan);
+      if (i < ks.len) st16(dk + i * p.dk_st + at, nan);
+      if (i < ks.len) st16(dv + i * p.dv_st + at, nan);
+    }
+    return;
   }
-  qs.len = min(qs.len, p.window);
-  ks.len = min(ks.len, p.window);
   const int ahead = ks.len - qs.len;
   const int tile_b = (p.window + 7) / 8 * 8 * ROWB;
   char* const sq = s_all;

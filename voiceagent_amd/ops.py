@@ -1333,8 +1333,8 @@ def varlen_attention_backward(
     rows, [total_k, Hkv, D].  The probabilities are recomputed.  The maxima
     must be at least every length, as in the forward call, or 0 if they are not
     known: sequences of at most 128 rows at head_dim 64, with as many kv heads as
-    heads, take one launch, which leaves zeros in rows past the maxima; others
-    take two or three and go by the cumulative lengths.  Rows outside every
+    heads, take one launch, in which a longer sequence than the maxima say gets
+    NaN; others take two or three and go by the cumulative lengths.  Rows outside every
     sequence, queries that see no key and keys that no query sees get zeros.
     ``dq``, ``dk``, ``dv``: tensors to write into (views of one buffer, say); they
     may not overlap the inputs.  All launches are on the current stream, without
