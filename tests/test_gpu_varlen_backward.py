@@ -3,10 +3,13 @@
 Every element is held to the bound that oracle.gradients derives for it (P and dS rounded to the
 element type once, sums in fp32, the result rounded)."""
 
+import ctypes
+
 import pytest
 import torch
 
 from oracle import gradients as G
+from voiceagent_amd import _native as N
 from voiceagent_amd import ops
 from voiceagent_amd._native import NativeError
 from voiceagent_amd.layers import (AttentionContext, PagedAttention, VarlenSelfAttention,
@@ -189,6 +192,32 @@ def test_lengths_past_the_rows_are_held(dev):
     held = torch.tensor([0, 40, 64, 64], dtype=torch.int32)
     got = _call(dev, q, k, v, dout, out, cu, cu, 0.125, True)
     _check(got, G.varlen_attention_backward(dout, q, k, v, out, held, held, 0.125, True))
+
+
+def test_lengths_that_fall_and_rise_stay_in_the_workspace(dev):
+    # More blocks than the rows make: results mean nothing, memory behind the workspace stays.
+    q, k, v, dout, out, _, _ = (None if t is None else t.to(dev) for t in
+                                _inputs([300], [300], 16, 1, 64, torch.bfloat16, 24))
+    cu = torch.tensor([0, 300] * 20 + [0], dtype=torch.int32, device=dev)
+    grads = [torch.empty_like(t) for t in (q, k, v)]
+    a = N.new_args(N.VarlenBwdArgs)
+    a.dtype = N.VA_BF16
+    for name, t in zip(("q", "k", "v", "out", "dout", "dq", "dk", "dv"), (q, k, v, out, dout, *grads)):
+        setattr(a, name, t.data_ptr())
+        setattr(a, name + "_stride_tok", t.stride(0))
+        setattr(a, name + "_stride_head", t.stride(1))
+    a.cu_seqlens_q = a.cu_seqlens_k = cu.data_ptr()
+    a.num_seqs, a.total_q, a.total_k = 40, 300, 300
+    a.num_heads, a.num_kv_heads, a.head_dim, a.scale = 16, 1, 64, 0.125
+    lib = N.lib()
+    need = lib.va_varlen_attention_backward_workspace_bytes(ctypes.byref(a))
+    assert need > 2 * 16 * 300 * 4 + 256  # the launch has parts
+    ws = torch.full((need + (8 << 20),), 85, dtype=torch.uint8, device=dev)
+    a.workspace, a.workspace_bytes = ws.data_ptr(), need
+    stream = torch.cuda.current_stream().cuda_stream
+    assert lib.va_varlen_attention_backward(ctypes.byref(a), stream) == 0
+    torch.cuda.synchronize()
+    assert (ws[need:] == 85).all()
 
 
 def test_no_sequences_no_rows(dev):

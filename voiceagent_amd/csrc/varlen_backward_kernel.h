@@ -381,7 +381,7 @@ constexpr int kF16Lift = 14;
 //
 // kSplit: a wave takes 32 keys of each tile for its 32 queries, its neighbour the
 // other 32, and their sums meet in LDS at the end: launches whose blocks of 128
-// queries would leave the chip half idle take blocks of 64 in half the time.
+// queries would leave the chip half idle take blocks of 64 in less time.
 template <bool kBF16, int D, bool kSplit>
 __global__ __launch_bounds__(kBwdThreads, 2) void varlen_dq_kernel(VarlenBwdParams p) {
   constexpr int kTile = 64;  // keys
@@ -684,7 +684,8 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void varlen_dkv_kernel(Varlen
   const int ahead = ks.len - qs.len;
   const int begin = kParts ? part_begin(blk.steps, part, parts) : 0;
   const int steps = (kParts ? part_begin(blk.steps, part + 1, parts) : blk.steps) - begin;
-  if (kParts && steps == 0) return;
+  // (Lengths that fall and rise again make more blocks than there is room for.)
+  if (kParts && (steps == 0 || blk.place >= p.k_tiles)) return;
 
   const uint32_t lds = __builtin_amdgcn_readfirstlane(
       (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)s_qd);
