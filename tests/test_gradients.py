@@ -98,6 +98,8 @@ def _bwd_args(**over):
     (dict(dv=None), "key side"), (dict(cu_seqlens_k=None), "cu_seqlens"), (dict(dq_stride_tok=4), "strides"),
     (dict(dout=(1 << 20) + 8), "aligned"), (dict(scale=0.0), "scale"),
     (dict(total_q=2 ** 31 - 1, total_k=2 ** 31 - 1, num_heads=1024, num_kv_heads=1024), "too many"),
+    (dict(num_seqs=1 << 20, num_heads=32, num_kv_heads=32), "too many"),
+    (dict(num_seqs=1 << 20, num_heads=32, num_kv_heads=32, max_seqlen_q=1, max_seqlen_k=1), "too many"),
     (dict(workspace=None), "workspace"), (dict(workspace_bytes=63), "workspace"),
 ])
 def test_c_abi_refuses_bad_attention_gradients(over, says):
@@ -150,7 +152,7 @@ def test_overlap_is_seen():
     # In place is the same memory, element for element, and only where it is allowed.
     assert ops._in_place(x, x[:]) and not ops._in_place(x[:3], x[1:])
     ops._outputs_apart([("a", x[:, :2], (x[:, :2],))], (x[:, 2:],))
-    for given, inputs in (([("a", x, ())], (x,)), ([("a", x[1:], (x[:3],))], (x[:3],)),
+    for given, inputs in (([("a", x[:1].expand(4, 6, 8), ())], ()), ([("a", x, ())], (x,)), ([("a", x[1:], (x[:3],))], (x[:3],)),
                           ([("a", x, ()), ("b", x, ())], ())):
         with pytest.raises(ops.AttentionArgumentError, match="overlap"):
             ops._outputs_apart(given, inputs)

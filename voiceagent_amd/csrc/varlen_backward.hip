@@ -61,6 +61,9 @@ static int window_rows(const va_varlen_bwd_args* a) {
              : 0;
 }
 
+// Workgroups of a launch: 256 threads each, 2^32 in all.
+constexpr int64_t kMostItems = (1 << 24) - 1;
+
 // Workspace: the first launch's results for the second (lse, delta and, for f16,
 // the rows' largest |dout|), and the parts' sums.
 struct BwdLayout {
@@ -139,8 +142,8 @@ extern "C" int va_varlen_attention_backward(const va_varlen_bwd_args* a, void* s
   VA_CHECK_ARG(a->max_seqlen_q >= 0 && a->max_seqlen_k >= 0, "%s: negative max_seqlen", fn);
   const int window = window_rows(a);
   VA_CHECK_ARG(((int64_t)a->num_seqs + 1 + std::max(a->total_q, a->total_k) / kWindowExtra) *
-                       a->num_heads <= INT32_MAX && q_tiles * a->num_heads <= INT32_MAX &&
-                   lay.k_tiles * lay.parts * a->num_kv_heads <= INT32_MAX,
+                       a->num_heads <= kMostItems && q_tiles * a->num_heads <= kMostItems &&
+                   lay.k_tiles * lay.parts * a->num_kv_heads <= kMostItems,
                "%s: too many (sequence, head, block) items", fn);
   const size_t need = a->total_q > 0 && window == 0 ? lay.total : 0;
   if (need > 0 && (a->workspace == nullptr || a->workspace_bytes < need ||

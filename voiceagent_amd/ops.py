@@ -508,6 +508,8 @@ def _outputs_apart(given, inputs) -> None:
     """Refuses outputs that share memory with one another or with an input, but for what may be
     written in place.  given: (name, tensor, the inputs it may replace)."""
     for i, (name, t, own) in enumerate(given):
+        _require(all(st > 0 for n, st in zip(t.shape, t.stride()) if n > 1),
+                 f"{name}'s rows may not overlap")
         for x in inputs:
             _require(_apart(t, x) or (any(x is o for o in own) and _in_place(t, x)),
                      f"{name} may not overlap the inputs")
