@@ -1,0 +1,60 @@
+"""CPU checks of the layers' host logic in a training pass: which calls a layer makes, and in
+which grad mode, with the operators stood in for."""
+
+import pytest
+import torch
+
+from voiceagent_amd import ops
+from voiceagent_amd.layers import (AttentionContext, PagedAttention, Qwen3AttentionCore,
+                                   attention_context)
+
+HQ, HKV, D, T = 4, 2, 128, 6
+
+
+@pytest.fixture
+def calls(monkeypatch):
+    """The operators a layer calls: (name, whether grad mode was on, whether a prologue went along)."""
+    made = []
+
+    def stand_in(name, result):
+        def call(*args, prologue=None, **kw):
+            made.append((name, torch.is_grad_enabled(), prologue is not None))
+            return result(*args)
+        monkeypatch.setattr(ops, name, call)
+
+    stand_in("qk_norm_rope", lambda q, k, pro: (q, k))
+    stand_in("rotary_embedding", lambda q, k, *rest: (q, k))
+    stand_in("varlen_attention", lambda q, k, v, *rest: q)
+    stand_in("paged_decode", lambda q, *rest: q)
+    stand_in("store_kvcache", lambda *rest: None)
+    return made
+
+
+def _rows(*asks):
+    rows = [torch.zeros(T, h, D, dtype=torch.bfloat16) for h in (HQ, HKV, HKV)]
+    for t, ask in zip(rows, asks):
+        t.requires_grad_(ask)
+    return rows
+
+
+def _context(slots=None):
+    cu = torch.tensor([0, T], dtype=torch.int32)
+    return attention_context(AttentionContext(cu, cu, T, T, slots, None))
+
+
+@pytest.mark.parametrize("asks", ["none", "q", "k", "v", "q weight", "k weight"])
+def test_a_launch_with_the_prologue_takes_nothing_that_asks_for_a_gradient(calls, asks):
+    """A launch that applies the query prologue has no gradient: whatever asks for one goes through
+    the prologue's own call, v alone too."""
+    core = Qwen3AttentionCore(HQ, D, HKV, max_position=16)
+    core.varlen_fuse_prologue = True
+    core.q_norm_weight.requires_grad_(asks == "q weight")
+    core.k_norm_weight.requires_grad_(asks == "k weight")
+    with _context():
+        core(torch.arange(T), *_rows(*(asks == name for name in "qkv")))
+    fused = asks == "none"
+    assert calls == [("qk_norm_rope", True, False), ("varlen_attention", True, fused)]
+    calls.clear()
+    with torch.no_grad(), _context():
+        core(torch.arange(T), *_rows(*(asks == name for name in "qkv")))
+    assert calls == [("qk_norm_rope", False, False), ("varlen_attention", False, True)]

@@ -144,7 +144,7 @@ class PagedAttention(nn.Module):
                 if isinstance(prologue, ops.Rotary):
                     q, k = ops.rotary_embedding(q, k, prologue.cos_sin_cache, prologue.positions,
                                                 interleaved=prologue.interleaved)
-                elif not decode and self._varlen_takes_prologue(q, k, prologue):
+                elif not decode and self._varlen_takes_prologue(q, k, v, prologue):
                     _, k = ops.qk_norm_rope(None, k, prologue)
                     q_pro = prologue
                 else:
@@ -221,7 +221,7 @@ class PagedAttention(nn.Module):
             prologue=q_pro,
         )
 
-    def _varlen_takes_prologue(self, q: torch.Tensor, k: torch.Tensor,
+    def _varlen_takes_prologue(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
                                prologue: ops.QKPrologue) -> bool:
         """Whether the varlen launch can apply the query prologue itself:
         head_dim 128, 16-bit q, a 16-bit pool or none, and nothing that asks for
@@ -230,7 +230,7 @@ class PagedAttention(nn.Module):
                 q.dtype in (torch.bfloat16, torch.float16) and
                 (not self.k_cache.numel() or self.k_cache.dtype == q.dtype) and
                 not (torch.is_grad_enabled() and
-                     (q.requires_grad or k.requires_grad or
+                     (q.requires_grad or k.requires_grad or v.requires_grad or
                       prologue.q_norm_weight.requires_grad or
                       prologue.k_norm_weight.requires_grad)))
 
