@@ -3,6 +3,7 @@
 import pytest
 import torch
 
+from voiceagent_amd import ops
 from voiceagent_amd.layers import AttentionContext, Qwen3AttentionCore, attention_context
 
 pytestmark = pytest.mark.gpu
@@ -28,3 +29,33 @@ def test_a_gradient_of_v_alone(dev):
             core(pos, q, k, leaf).backward(dout)
         grads.append(leaf.grad)
     assert grads[0].any() and torch.equal(*grads)
+
+
+def _prologue(dev, T, d, grad=False):
+    g = torch.Generator().manual_seed(9)
+    w = torch.ones(d, dtype=torch.bfloat16, device=dev, requires_grad=grad)
+    table = torch.rand(T, d, generator=g).to(dev)
+    return ops.QKPrologue(w, w, 1e-6, table, torch.arange(T, device=dev))
+
+
+def test_given_outputs_are_outside_the_graph(dev):
+    """In place on rows of a graph: refused in grad mode; otherwise written."""
+    T, d = 12, 64
+    q, k, v, _ = _rows(dev, T, 2, 2, d, 2)
+    pro, cu = _prologue(dev, T, d, grad=True), torch.tensor([0, T], dtype=torch.int32, device=dev)
+    table, pos = pro.cos_sin_cache, pro.positions
+    leaf = q.clone().requires_grad_()
+    x = leaf * 1
+    for call in (lambda: ops.rotary_embedding(x, None, table, pos, q_out=x),
+                 lambda: ops.qk_norm_rope(x, k, pro, q_out=x, k_out=k),
+                 lambda: ops.varlen_attention(q, k, v, cu, cu, T, T, scale=1.0, causal=True, out=x)):
+        with pytest.raises(ops.AttentionArgumentError, match="requires a gradient"):
+            call()
+    assert torch.equal(x, q)
+    # Rows outside the graph are written as before, weights that ask for a gradient or not.
+    a, b = q.clone(), k.clone()
+    got = ops.qk_norm_rope(a, b, pro, q_out=a, k_out=b)
+    with torch.no_grad():
+        want = ops.qk_norm_rope(q, k, pro)
+    assert got[0] is a and torch.equal(a, want[0]) and torch.equal(b, want[1])
+    assert not a.requires_grad

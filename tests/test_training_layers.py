@@ -58,3 +58,31 @@ def test_a_launch_with_the_prologue_takes_nothing_that_asks_for_a_gradient(calls
     with torch.no_grad(), _context():
         core(torch.arange(T), *_rows(*(asks == name for name in "qkv")))
     assert calls == [("qk_norm_rope", False, False), ("varlen_attention", False, True)]
+
+
+# ------------------------------------------------------------------ given outputs in grad mode
+def test_outputs_that_require_a_gradient_are_refused():
+    """Written through its pointer, such an output would keep its old place in the graph: the
+    gradient of what is written flowed on as if nothing had been done to it."""
+    leaf = torch.zeros(4, 2, 64, requires_grad=True)
+    x, table, pos, w = leaf * 1, torch.zeros(9, 64), torch.zeros(4, dtype=torch.int64), torch.ones(64)
+    y, cu = torch.zeros(4, 2, 64), torch.tensor([0, 4], dtype=torch.int32)
+    pro = ops.QKPrologue(w, w, 1e-6, table, pos)
+    bad = [lambda: ops.rotary_embedding(x, y, table, pos, q_out=x),
+           lambda: ops.rotary_embedding(y, x, table, pos, q_out=y, k_out=x),
+           lambda: ops.rotary_embedding(leaf, None, table, pos, q_out=leaf),
+           lambda: ops.rotary_embedding(y, None, table, pos, q_out=x),
+           lambda: ops.qk_norm_rope(x, y, pro, q_out=x, k_out=y),
+           lambda: ops.qk_norm_rope(y, x, pro, k_out=x),
+           lambda: ops.qk_norm_rope(None, x, pro, k_out=x),
+           lambda: ops.varlen_attention(y, y, y, cu, cu, 4, 4, scale=1.0, causal=True, out=x),
+           lambda: ops._outputs_apart([("dq", x, ())], ())]
+    for call in bad:
+        with pytest.raises(ops.AttentionArgumentError, match="requires a gradient"):
+            call()
+    # Without a graph nothing is falsified: the next check is what refuses the CPU's tensors.
+    with torch.no_grad():
+        for call in bad[:-1]:
+            with pytest.raises(ops.AttentionArgumentError, match="GPU"):
+                call()
+        bad[-1]()

@@ -69,6 +69,14 @@ def _rows(t: torch.Tensor, what: str) -> None:
     _require(t.stride(-1) == 1, f"{what}: the last dimension must be contiguous")
 
 
+def _plain_output(t: torch.Tensor | None, what: str) -> None:
+    """Refuses a given output that would claim a gradient that the call does not have: written
+    through its pointer it keeps its place in autograd's graph."""
+    _require(t is None or not t.requires_grad or not torch.is_grad_enabled(),
+             f"{what} requires a gradient, and a call with outputs has none "
+             "(call without outputs, or in torch.no_grad())")
+
+
 def _pool_matches(pool: torch.Tensor, dtype: torch.dtype) -> bool:
     """A pool of `dtype` itself, or an FP8 pool for 16-bit data."""
     return pool.dtype == dtype or (pool.dtype == FP8_KV_DTYPE and
@@ -396,8 +404,12 @@ def qk_norm_rope(
     may be q / k themselves (in place).  ``q`` None: the keys alone (a
     prefill whose varlen launch applies the query prologue itself); the
     first result is then None.  Without outputs the call is differentiable in q,
-    k and the norm weights (:func:`qk_norm_rope_backward`)."""
-    if q_out is None and k_out is None and torch.is_grad_enabled():
+    k and the norm weights (:func:`qk_norm_rope_backward`); with outputs it has
+    no gradient, and in grad mode they may not require one."""
+    if q_out is not None or k_out is not None:
+        _plain_output(q_out, "q_out")
+        _plain_output(k_out, "k_out")
+    elif torch.is_grad_enabled():
         qw, kw = prologue.q_norm_weight, prologue.k_norm_weight
         if q is None:
             if k.requires_grad or kw.requires_grad:
@@ -508,6 +520,7 @@ def _outputs_apart(given, inputs) -> None:
     """Refuses outputs that share memory with one another or with an input, but for what may be
     written in place.  given: (name, tensor, the inputs it may replace)."""
     for i, (name, t, own) in enumerate(given):
+        _plain_output(t, name)
         _require(all(st > 0 for n, st in zip(t.shape, t.stride()) if n > 1),
                  f"{name}'s rows may not overlap")
         for x in inputs:
@@ -658,8 +671,12 @@ def rotary_embedding(
     or fp32 rows, any head_dim and strides; rows of 16-byte multiples go 16
     bytes at a time).  Positions are held to the table.  Outputs may be q / k
     themselves, and share no memory otherwise; without outputs the call is
-    differentiable in q and k (the table is a constant)."""
-    if (q_out is None and k_out is None and torch.is_grad_enabled() and
+    differentiable in q and k (the table is a constant), with outputs it has no
+    gradient, and in grad mode they may not require one."""
+    if q_out is not None or k_out is not None:
+        _plain_output(q_out, "q_out")
+        _plain_output(k_out, "k_out")
+    elif (torch.is_grad_enabled() and
             ((q is not None and q.requires_grad) or (k is not None and k.requires_grad))):
         return _Rotary.apply(q, k, cos_sin_cache, positions, interleaved, inverse)
     if q is not None and k is not None and q_out is None and k_out is None:
@@ -1157,8 +1174,10 @@ def varlen_attention(
 
     Without a pool, a prologue or ``out`` the call is differentiable in q, k
     and v (:func:`varlen_attention_backward`); the others return tensors without
-    a gradient.
+    a gradient (in grad mode ``out`` may not require one).
     """
+    if out is not None:
+        _plain_output(out, "out")
     if (k_cache is None and out is None and prologue is None and k is not None and v is not None
             and (q.requires_grad or k.requires_grad or v.requires_grad)
             and torch.is_grad_enabled()):
