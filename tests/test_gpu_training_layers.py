@@ -39,7 +39,7 @@ def _prologue(dev, T, d, grad=False):
 
 
 def test_given_outputs_are_outside_the_graph(dev):
-    """In place on rows of a graph: refused in grad mode; otherwise written."""
+    """In place on rows of a graph: refused in grad mode; otherwise written, and counted."""
     T, d = 12, 64
     q, k, v, _ = _rows(dev, T, 2, 2, d, 2)
     pro, cu = _prologue(dev, T, d, grad=True), torch.tensor([0, T], dtype=torch.int32, device=dev)
@@ -51,11 +51,48 @@ def test_given_outputs_are_outside_the_graph(dev):
                  lambda: ops.varlen_attention(q, k, v, cu, cu, T, T, scale=1.0, causal=True, out=x)):
         with pytest.raises(ops.AttentionArgumentError, match="requires a gradient"):
             call()
-    assert torch.equal(x, q)
+    assert x._version == 0 and torch.equal(x, q)
     # Rows outside the graph are written as before, weights that ask for a gradient or not.
     a, b = q.clone(), k.clone()
     got = ops.qk_norm_rope(a, b, pro, q_out=a, k_out=b)
     with torch.no_grad():
         want = ops.qk_norm_rope(q, k, pro)
     assert got[0] is a and torch.equal(a, want[0]) and torch.equal(b, want[1])
-    assert not a.requires_grad
+    assert not a.requires_grad and a._version == b._version == 1
+
+
+@pytest.mark.parametrize("write", ["rotary", "prologue", "keys", "varlen", "decode", "gradient", "metadata"])
+def test_saved_rows_that_are_written_over_are_seen(dev, write):
+    """A call that writes where a backward pass has saved rows: the pass raises."""
+    T, d = 12, 64
+    q, k, v, _ = _rows(dev, T, 2, 2, d, 3)
+    pro, cu = _prologue(dev, T, d), torch.tensor([0, T], dtype=torch.int32, device=dev)
+    k.requires_grad_()
+    if write == "metadata":
+        lens = torch.tensor([T], dtype=torch.int32, device=dev)
+        req = torch.zeros(1, 4, dtype=torch.int32, device=dev)
+        step = lambda out: ops.batch_metadata(lens, lens * 0, req, 16, max_tokens=T, out=out)  # noqa: E731
+        made = step(None)
+        out = ops.rotary_embedding(None, k, pro.cos_sin_cache, made.positions)[1]
+        step(made)
+    else:
+        out = ops.varlen_attention(q, k, v, cu, cu, T, T, scale=1.0, causal=True)
+    with torch.no_grad():
+        if write == "rotary":
+            ops.rotary_embedding(q, None, pro.cos_sin_cache, pro.positions, q_out=q)
+        elif write == "prologue":
+            ops.qk_norm_rope(q, v, pro, q_out=q, k_out=v)
+        elif write == "keys":
+            ops.qk_norm_rope(None, v, pro, k_out=v)
+        elif write == "varlen":
+            ops.varlen_attention(q, k, v, cu, cu, T, T, scale=1.0, causal=True, out=q)
+        elif write == "gradient":
+            rows = [torch.ones_like(q) for _ in range(5)]
+            ops.varlen_attention_backward(*rows, cu, cu, T, T, scale=1.0, causal=True, dv=v)
+        elif write == "decode":
+            pool = torch.zeros(2, T, 16, 2, d, dtype=torch.bfloat16, device=dev)
+            table = torch.arange(T, dtype=torch.int32, device=dev)[:, None]
+            ops.paged_decode(q, *pool, table, torch.ones(T, dtype=torch.int32, device=dev),
+                             max_seq_len=1, scale=1.0, out=q)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        out.sum().backward()

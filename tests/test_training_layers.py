@@ -86,3 +86,16 @@ def test_outputs_that_require_a_gradient_are_refused():
             with pytest.raises(ops.AttentionArgumentError, match="GPU"):
                 call()
         bad[-1]()
+
+
+def test_written_outputs_count_as_changed():
+    x = torch.zeros(3, requires_grad=True)
+    y = x * 1
+    z = y.square()  # saves y
+    with torch.no_grad():
+        ops._written(y, None)
+    assert y._version == 1
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        z.sum().backward()
+    with torch.inference_mode():
+        ops._written(torch.zeros(2))  # (has no count)

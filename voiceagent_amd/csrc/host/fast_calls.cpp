@@ -67,6 +67,12 @@ RotaryFn g_rotary = nullptr;
 
 constexpr int64_t kNotTaken = -1000;
 
+// A call's status; launched, its output counts as changed (the wrappers' _written).
+int64_t written(int64_t status, const at::Tensor& out) {
+  if (status == 0 && !out.is_inference()) out.unsafeGetTensorImpl()->bump_version();
+  return status;
+}
+
 int dtype_code(c10::ScalarType t) {
   switch (t) {
     case at::kBFloat16: return VA_BF16;
@@ -342,7 +348,7 @@ int64_t decode_call(const at::Tensor& q, const at::Tensor& kc, const at::Tensor&
     a.workspace_bytes = (size_t)ws.numel() * ws.element_size();
   }
   void* const st = reinterpret_cast<void*>(static_cast<intptr_t>(stream));
-  return mx4 ? g_decode_mx4(&a, &sc, st) : g_decode(&a, st);
+  return written(mx4 ? g_decode_mx4(&a, &sc, st) : g_decode(&a, st), out);
 }
 
 // ops.varlen_attention over a 16-bit pool or none (an FP8 pool needs a
@@ -463,7 +469,7 @@ int64_t varlen_call(const at::Tensor& q, const c10::optional<at::Tensor>& k,
     }
   }
   void* const st = reinterpret_cast<void*>(static_cast<intptr_t>(stream));
-  return mx4 ? g_varlen_mx4(&a, &sc, st) : g_varlen(&a, st);
+  return written(mx4 ? g_varlen_mx4(&a, &sc, st) : g_varlen(&a, st), out);
 }
 
 // ops.store_kvcache.  0: launched; VA_ERR_*: the library's status;
@@ -702,7 +708,8 @@ int64_t qk_norm_rope(const at::Tensor& q, const at::Tensor& k, const at::Tensor&
   a.num_heads = (int32_t)hq;
   a.num_kv_heads = (int32_t)hkv;
   a.head_dim = (int32_t)d;
-  return g_rope(&a, reinterpret_cast<void*>(static_cast<intptr_t>(stream)));
+  const int64_t status = g_rope(&a, reinterpret_cast<void*>(static_cast<intptr_t>(stream)));
+  return written(written(status, q_out), k_out);
 }
 
 // Rows [tokens, heads, head_dim] on `device`, contiguous in their last dimension.

@@ -77,6 +77,12 @@ def _plain_output(t: torch.Tensor | None, what: str) -> None:
              "(call without outputs, or in torch.no_grad())")
 
 
+def _written(*outs: torch.Tensor | None) -> None:
+    """Counts given outputs as changed, as torch's own in-place calls do, so that a backward pass
+    that saved their rows before raises instead of reading others."""
+    torch.autograd.graph.increment_version([t for t in outs if t is not None])
+
+
 def _pool_matches(pool: torch.Tensor, dtype: torch.dtype) -> bool:
     """A pool of `dtype` itself, or an FP8 pool for 16-bit data."""
     return pool.dtype == dtype or (pool.dtype == FP8_KV_DTYPE and
@@ -462,6 +468,7 @@ def qk_norm_rope(
     args.num_tokens, args.num_heads, args.num_kv_heads, args.head_dim = T, hq, hkv, d
     args.prologue = _prologue_struct(prologue, d, T)
     N.call("va_qk_norm_rope", args, device)
+    _written(q_out, k_out)
     return q_out, k_out
 
 
@@ -485,6 +492,7 @@ def _k_norm_rope(k: torch.Tensor, prologue: QKPrologue,
     args.num_tokens, args.num_heads, args.num_kv_heads, args.head_dim = T, 0, hkv, d
     args.prologue = _prologue_struct(prologue, d, T)
     N.call("va_qk_norm_rope", args, device)
+    _written(k_out)
     return k_out
 
 
@@ -598,6 +606,7 @@ def qk_norm_rope_backward(
         args.workspace_bytes = nbytes
         N.check("va_qk_norm_rope_backward",
                 lib.va_qk_norm_rope_backward(ctypes.byref(args), _raw_stream(index)))
+    _written(*(t for _, t, _ in given))
     return results["q"], results["k"], results["qw"], results["kw"]
 
 
@@ -735,6 +744,7 @@ def rotary_embedding(
     args.positions_dtype = _index_code(positions, "positions")
     args.positions = positions.data_ptr()
     N.call("va_rotary", args, device)
+    _written(*(t for _, t, _ in given))
     return outs[0], outs[1]
 
 
@@ -1126,6 +1136,7 @@ def paged_decode(
                                             _raw_stream(index)))
         else:
             N.check("va_paged_decode", lib.va_paged_decode(ctypes.byref(args), _raw_stream(index)))
+    _written(out)
     return out
 
 
@@ -1302,6 +1313,7 @@ def varlen_attention(
         else:
             N.check("va_varlen_attention",
                     lib.va_varlen_attention(ctypes.byref(args), _raw_stream(index)))
+    _written(out)
     return out
 
 
@@ -1422,6 +1434,7 @@ def varlen_attention_backward(
         args.workspace_bytes = nbytes
         N.check("va_varlen_attention_backward",
                 lib.va_varlen_attention_backward(ctypes.byref(args), _raw_stream(index)))
+    _written(*(t for _, t, _ in given))
     return dq, dk, dv
 
 
@@ -1584,6 +1597,8 @@ def batch_metadata(
     with _current(index):
         N.check("va_batch_metadata",
                 N.lib().va_batch_metadata(ctypes.byref(args), _raw_stream(index)))
+    _written(out.positions, out.slot_mapping, out.cu_seqlens_q, out.cu_seqlens_k, out.block_tables,
+             out.totals)
     return out
 
 
