@@ -31,6 +31,27 @@ def test_a_gradient_of_v_alone(dev):
     assert grads[0].any() and torch.equal(*grads)
 
 
+@pytest.mark.parametrize("fuse_prologue", [True, False])
+@pytest.mark.parametrize("T", [1, 20])
+def test_a_bound_cache_builds_no_graph(dev, monkeypatch, fuse_prologue, T):
+    """Prompts and single tokens, the prologue inside the launches or ahead of them."""
+    hq, hkv, d = 4, 2, 128
+    q, k, v, _ = _rows(dev, T, hq, hkv, d, 4)
+    core = Qwen3AttentionCore(hq, d, hkv, max_position=64).to(dev)
+    core.fuse_prologue = fuse_prologue
+    cu = torch.tensor([0, T], dtype=torch.int32, device=dev)
+    slots = torch.arange(T, dtype=torch.int32, device=dev)
+    table = torch.tensor([[0, 1]], dtype=torch.int32, device=dev)
+    context = AttentionContext(cu, cu, T, T, slots, table)
+    monkeypatch.setattr(ops._QkNormRope, "apply", None)  # (a graph would need it)
+    outs = []
+    for grad in (True, False):
+        core.k_cache, core.v_cache = torch.zeros(2, 4, 16, hkv, d, dtype=torch.bfloat16, device=dev)
+        with torch.set_grad_enabled(grad), attention_context(context):
+            outs.append(core(torch.arange(T, device=dev), q, k, v))
+    assert torch.equal(*outs) and not outs[0].requires_grad
+
+
 def _prologue(dev, T, d, grad=False):
     g = torch.Generator().manual_seed(9)
     w = torch.ones(d, dtype=torch.bfloat16, device=dev, requires_grad=grad)

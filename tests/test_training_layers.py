@@ -60,6 +60,25 @@ def test_a_launch_with_the_prologue_takes_nothing_that_asks_for_a_gradient(calls
     assert calls == [("qk_norm_rope", False, False), ("varlen_attention", False, True)]
 
 
+@pytest.mark.parametrize("fuse_prologue,fuse_store", [(True, True), (True, False), (False, True), (False, False)])
+@pytest.mark.parametrize("asks", ["weights", "rows"])
+def test_over_a_cache_the_prologue_runs_without_a_graph(calls, fuse_prologue, fuse_store, asks):
+    """Serving without torch.no_grad(): the prologue saves nothing for a backward pass that cannot
+    be, however the layer's launches are chosen."""
+    core = Qwen3AttentionCore(HQ, D, HKV, max_position=16)  # (its weights ask for a gradient)
+    core.requires_grad_(asks == "weights")
+    core.fuse_prologue, core.fuse_store = fuse_prologue, fuse_store
+    core.k_cache = core.v_cache = torch.zeros(4, 16, HKV, D, dtype=torch.bfloat16)
+    with _context(torch.arange(T)):
+        core(torch.arange(T), *_rows(*[asks == "rows"] * 3))
+    assert [on for name, on, _ in calls if name == "qk_norm_rope"] == [False]
+    core.k_cache = torch.tensor([])
+    calls.clear()
+    with _context():
+        core(torch.arange(T), *_rows(*[asks == "rows"] * 3))
+    assert [on for name, on, _ in calls if name == "qk_norm_rope"] == [True]
+
+
 # ------------------------------------------------------------------ given outputs in grad mode
 def test_outputs_that_require_a_gradient_are_refused():
     """Written through its pointer, such an output would keep its old place in the graph: the

@@ -143,5 +143,7 @@ class Qwen3AttentionCore(PagedAttention):
         if self.fuse_prologue:
             # (a decode step in one launch; prefill batches as varlen_fuse_prologue says)
             return super().forward(q, k, v, prologue=pro)
-        qn, kn = ops.qk_norm_rope(q, k, pro)
+        # (Over a cache nothing has a gradient, whatever the weights ask for.)
+        with torch.set_grad_enabled(torch.is_grad_enabled() and not self.k_cache.numel()):
+            qn, kn = ops.qk_norm_rope(q, k, pro)
         return super().forward(qn, kn, v)
