@@ -118,3 +118,22 @@ def test_written_outputs_count_as_changed():
         z.sum().backward()
     with torch.inference_mode():
         ops._written(torch.zeros(2))  # (has no count)
+
+
+# ------------------------------------------------------------------------------ given outputs
+def test_outputs_whose_rows_overlap_are_refused():
+    x = torch.zeros(4096)
+    for sizes, strides in (((8, 4, 64), (32, 8, 1)), ((8, 4, 64), (256, 32, 1)),  # heads
+                           ((8, 4, 64), (128, 64, 1)), ((8, 4, 64), (64, 512 - 64, 1)),  # tokens
+                           ((8, 4, 64), (256, 0, 1)), ((8, 4, 64), (0, 64, 1)), ((2, 1, 64), (63, 1, 1))):
+        t = x.as_strided(sizes, strides)
+        assert len({i for i in torch.arange(4096).as_strided(sizes, strides).flatten().tolist()}) < t.numel()
+        with pytest.raises(ops.AttentionArgumentError, match="dq's rows may not overlap"):
+            ops._outputs_apart([("dq", t, ())], ())
+    # Rows side by side, far apart, heads ahead of tokens, one of either, none.
+    for sizes, strides in (((8, 4, 64), (256, 64, 1)), ((8, 4, 64), (500, 100, 1)), ((8, 4, 64), (64, 512, 1)),
+                           ((8, 1, 64), (64, 0, 1)), ((1, 4, 64), (1, 64, 1)), ((1, 1, 64), (0, 0, 1)),
+                           ((0, 4, 64), (0, 64, 1))):
+        t = x.as_strided(sizes, strides)
+        assert len({i for i in torch.arange(4096).as_strided(sizes, strides).flatten().tolist()}) == t.numel()
+        ops._outputs_apart([("dq", t, ())], ())

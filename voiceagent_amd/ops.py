@@ -519,6 +519,17 @@ def _apart(a: torch.Tensor, b: torch.Tensor) -> bool:
     return False
 
 
+def _rows_apart(t: torch.Tensor) -> bool:
+    """Whether no two elements of a tensor are seen to share memory: from the smallest stride on,
+    a dimension steps past all that the ones before it reach."""
+    reach = 1
+    for st, n in sorted((st, n) for n, st in zip(t.shape, t.stride()) if n > 1):
+        if st < reach:
+            return False
+        reach += (n - 1) * st
+    return True
+
+
 def _in_place(new: torch.Tensor, old: torch.Tensor) -> bool:
     """Whether two tensors of one shape are the same memory, element for element."""
     return new.data_ptr() == old.data_ptr() and new.stride() == old.stride()
@@ -529,8 +540,7 @@ def _outputs_apart(given, inputs) -> None:
     written in place.  given: (name, tensor, the inputs it may replace)."""
     for i, (name, t, own) in enumerate(given):
         _plain_output(t, name)
-        _require(all(st > 0 for n, st in zip(t.shape, t.stride()) if n > 1),
-                 f"{name}'s rows may not overlap")
+        _require(_rows_apart(t), f"{name}'s rows may not overlap")
         for x in inputs:
             _require(_apart(t, x) or (any(x is o for o in own) and _in_place(t, x)),
                      f"{name} may not overlap the inputs")
