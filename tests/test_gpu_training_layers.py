@@ -117,3 +117,22 @@ def test_saved_rows_that_are_written_over_are_seen(dev, write):
                              max_seq_len=1, scale=1.0, out=q)
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         out.sum().backward()
+
+
+@pytest.mark.parametrize("d,most", [(128, 40), (64, 40)])
+def test_tokens_far_apart(dev, d, most):
+    """Rows that the forward takes and the gradient does not as they are: q's tokens 72 MiB apart,
+    k's and v's 48."""
+    T = 40
+    q, k, v, dout = _rows(dev, T, 2, 2, d, 5)
+    cu = torch.tensor([0, 25, T], dtype=torch.int32, device=dev)
+    buf = torch.empty(T * (36 << 20) + 4096, dtype=torch.bfloat16, device=dev)
+    far = [buf.as_strided(t.shape, (step << 20, d, 1), at * 2 * d)
+           for at, (t, step) in enumerate(((q, 36), (k, 24), (v, 24)))]
+    grads = []
+    for rows in ((q, k, v), [f.copy_(t) for f, t in zip(far, (q, k, v))]):
+        leaves = [t.detach().requires_grad_() for t in rows]
+        out = ops.varlen_attention(*leaves, cu, cu, most, most, scale=0.125, causal=True)
+        grads.append(torch.autograd.grad(out, leaves, dout))
+    for a, b in zip(*grads):
+        assert a.any() and torch.equal(a, b)

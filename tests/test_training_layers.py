@@ -137,3 +137,30 @@ def test_outputs_whose_rows_overlap_are_refused():
         t = x.as_strided(sizes, strides)
         assert len({i for i in torch.arange(4096).as_strided(sizes, strides).flatten().tolist()}) == t.numel()
         ops._outputs_apart([("dq", t, ())], ())
+
+
+# ------------------------------------------------------------- rows that only the forward takes
+def test_rows_far_apart_reach_the_gradient_as_copies(monkeypatch):
+    """The attention takes q at any distance between tokens and k and v up to 64 MiB, its gradient
+    under 32: autograd copies rows that are farther apart."""
+    step = 1 << 24  # elements of 2 bytes: 32 MiB
+    buf = torch.zeros(step + 4096, dtype=torch.bfloat16)
+    seen = {}
+
+    def backward(dout, q, k, v, out, *rest, **kw):
+        seen.update(dout=dout, q=q, k=k, v=v)
+        return q, k, v
+
+    monkeypatch.setattr(ops, "varlen_attention", lambda q, *rest, **kw: torch.zeros(q.shape, dtype=q.dtype))
+    monkeypatch.setattr(ops, "varlen_attention_backward", backward)
+    cu = torch.tensor([0, 2], dtype=torch.int32)
+    for st, copied in ((step, True), (step - 8, False)):
+        far = {n: buf.as_strided((2, 2, 64), (st, 64, 1), i * 128) for i, n in enumerate(("q", "k", "v", "dout"))}
+        rows = [far[n].detach().requires_grad_() for n in "qkv"]
+        out = ops._VarlenAttention.apply(*rows, cu, cu, 2, 2, 1.0, True)
+        out.backward(far["dout"])
+        for n, t in seen.items():
+            assert (t.data_ptr() != far[n].data_ptr()) == copied, n
+            assert t.stride(0) * 2 < 1 << 25 and torch.equal(t, far[n])
+    one = buf.as_strided((1, 2, 64), (step, 64, 1))  # a single row has no distance
+    assert ops._near_rows(one) is one

@@ -1338,6 +1338,14 @@ def _whole_rows(t: torch.Tensor) -> torch.Tensor:
     return t
 
 
+def _near_rows(t: torch.Tensor) -> torch.Tensor:
+    """t, or a copy of it where its tokens are farther apart than the attention's gradient takes
+    (32 MiB: lane offsets in a tile are 32-bit) and the attention itself does."""
+    if t.shape[0] > 1 and t.stride(0) * t.element_size() >= 1 << 25:
+        return t.clone(memory_format=torch.contiguous_format)
+    return t
+
+
 def _row_strides(t: torch.Tensor) -> tuple[int, int]:
     """Strides of tokens and heads; a dimension of one has none to speak of
     (torch leaves any number there)."""
@@ -1372,8 +1380,8 @@ def varlen_attention_backward(
     gradient ``dout`` and the output itself ([total_q, Hq, D]).
 
     q, k, v, cu_seqlens, scale and causal are those of the forward call (16-bit
-    rows, head_dim 64 or 128; any group size); k and v of ``cu_seqlens_k``'s
-    rows, [total_k, Hkv, D].  The probabilities are recomputed.  The maxima
+    rows, head_dim 64 or 128, tokens under 32 MiB apart; any group size); k and
+    v of ``cu_seqlens_k``'s rows, [total_k, Hkv, D].  The probabilities are recomputed.  The maxima
     must be at least every length, as in the forward call, or 0 if they are not
     known: sequences of at most 128 rows at head_dim 64, with as many kv heads as
     heads, take one launch, in which a longer sequence than the maxima say gets
@@ -1464,8 +1472,9 @@ class _VarlenAttention(torch.autograd.Function):
     def backward(ctx, dout):
         q, k, v, out, cu_q, cu_k = ctx.saved_tensors
         max_q, max_k, scale, causal = ctx.call
-        grads = varlen_attention_backward(_whole_rows(dout), q, k, v, out, cu_q, cu_k, max_q, max_k,
-                                          scale=scale, causal=causal)
+        dout, q, k, v = (_near_rows(t) for t in (_whole_rows(dout), q, k, v))
+        grads = varlen_attention_backward(dout, q, k, v, out, cu_q, cu_k, max_q, max_k, scale=scale,
+                                          causal=causal)
         wanted = (g if need else None for g, need in zip(grads, ctx.needs_input_grad))
         return (*wanted, None, None, None, None, None, None)
 
