@@ -405,7 +405,8 @@ size_t va_varlen_split_workspace_bytes(const va_varlen_args* args);
  * dk and dv summed over the query heads of their group.  P is recomputed, in
  * fp32; P and dS are rounded to the element type before the products with
  * dout, q and k, whose sums are fp32 (f16: both scaled by powers of two first,
- * so that small gradients do not fall among f16's subnormals).
+ * so that small gradients do not fall among f16's subnormals, nor values of v
+ * near f16's largest take dS beyond it).
  * q, k, v, out and dout are as in the forward call (any group size); rows that
  * belong to no sequence get a gradient of zeros, as do queries that see no key
  * and keys that no query sees.  Lengths come from cu_seqlens, held to the rows

@@ -36,8 +36,8 @@ def varlen_attention_backward(dout, q, k, v, out, cu_q, cu_k, scale, causal):
       division;
     * dP - delta by (d + 8) 2^-24 (sum |dout||v| + sum |dout||out|);
     * P and dS are rounded: u of each; in f16, where they are scaled by powers of two that keep the
-      row's (the sequences') largest |dout| in [1, 2) and P's unit at 2^14, also by half a step of
-      the subnormals;
+      row's (the sequences') largest |dout|, or 2^-14 of its largest |dP - delta| if that is more, in
+      [1, 2) and P's unit at 2^14, also by half a step of the subnormals;
     * the last sums by (rows + 8) 2^-24 of their magnitudes, and u of the result.
     """
     u, tiny = HALF[q.dtype], TINY[q.dtype]
@@ -53,8 +53,14 @@ def varlen_attention_backward(dout, q, k, v, out, cu_q, cu_k, scale, causal):
         some = see.any(1, keepdim=True)
         for kv in range(k.shape[1]):
             heads = range(kv * group, (kv + 1) * group)
-            top_all = float(dout[a:b, kv * group:(kv + 1) * group].abs().max())
             kk, vv = k[c:e, kv].to(F64), v[c:e, kv].to(F64)
+            tops = {}
+            for h in heads:
+                do, oo = dout[a:b, h].to(F64), out[a:b, h].to(F64)
+                dp = (do @ vv.T - (do * oo).sum(-1, keepdim=True)) * see
+                tops[h] = torch.maximum(do.abs().amax(1, keepdim=True),
+                                        dp.abs().amax(1, keepdim=True) * 2.0 ** -14)
+            top_all = max(float(t.max()) for t in tops.values())
             for h in heads:
                 qq, do, oo = (x[a:b, h].to(F64) for x in (q, dout, out))
                 x = (qq @ kk.T * scale).masked_fill(~see, -math.inf)
@@ -70,7 +76,7 @@ def varlen_attention_backward(dout, q, k, v, out, cu_q, cu_k, scale, causal):
                 dp_off = (d + 8) * FP32 * (do.abs() @ vv.abs().T + (do * oo).abs().sum(-1, keepdim=True))
                 ds_off = (u + rel) * ds.abs() + p * dp_off
                 low = TINY[torch.float16] if f16 else 0.0
-                dq_each = ds_off + low * do.abs().amax(1, keepdim=True) * see
+                dq_each = ds_off + low * tops[h] * see
                 sums = (e - c + 8) * FP32
                 off["dq"][a:b, h] = scale * ((dq_each + sums * ds.abs()) @ kk.abs())
                 sums = (b - a + 8) * group * FP32

@@ -64,7 +64,7 @@ struct VarlenBwdParams {
   float* part;               // parts > 1: their sums, [block][part][kv head][wave][D / 8][64] x 4
   float* lse;                // [num_heads][total_q]: log2 sum 2^(c log2 e s), f16: - kF16Lift
   float* delta;              // [num_heads][total_q]: -delta
-  float* top;                // f16: [num_heads][total_q], largest |dout| of the row
+  float* top;                // f16: [num_heads][total_q], largest |dout| of the row (held_top)
 };
 
 constexpr int kBwdThreads = 256;
@@ -373,11 +373,23 @@ __device__ inline float pow2(int e) { return __uint_as_float((uint32_t)(e + 127)
 // probabilities of long contexts out of its subnormals.
 constexpr int kF16Lift = 14;
 
+// f16: dS is held as P (dP - delta) 2^-e, e the exponent of the row's largest |dout|.
+// Values of v in the ten thousands would take that past 65504, to infinity, and a
+// finite gradient with it.  So |dP - delta| 2^-e is held below 2^15: where `big`, the
+// largest one a lane has met, is not, e is raised, as the maximum is; masked keys do not
+// count.  (The test takes 4 sequences of 600 to 2000 rows, 32 heads over 4 of 64, from
+// 239.5 to 244.5 us a gradient.)
+__device__ inline bool out_of_range(float big, int e) { return big >= pow2(e + 15); }
+__device__ inline int raised(float big, int e) { return max(e, top_exponent(max_xor32(big)) - 14); }
+// What stands for the row's largest |dout| where the exponent was raised.
+__device__ inline float held_top(float top, int e) { return e > top_exponent(top) ? pow2(e) : top; }
+
 // ---------------------------------------------------------------------- dq
 // f16 (as for dk): dS is rounded to 16 bits, and a gradient of 1e-4 spread over
 // a thousand keys would fall among f16's subnormals.  So P is scaled by 2^-e, e
-// the exponent of the row's largest |dout|, through the exponential's argument,
-// and the maximum is followed without slack, which keeps dS near v's size.
+// the exponent of the row's largest |dout| (or more: out_of_range), through the
+// exponential's argument, and the maximum is followed without slack, which keeps dS
+// near v's size.
 //
 // kSplit: a wave takes 32 keys of each tile for its 32 queries, its neighbour the
 // other 32, and their sums meet in LDS at the end: launches whose blocks of 128
@@ -433,7 +445,7 @@ __global__ __launch_bounds__(kBwdThreads, 2) void varlen_dq_kernel(VarlenBwdPara
   const int wrow = i0 + 32 * (kSplit ? wave >> 1 : wave);
   const int row = wrow + l32, at = qs.row + min(row, qs.len - 1);
   uint4 qreg[DS], doreg[DS];
-  float delta = 0.f;
+  float delta = 0.f, top = 0.f;
   int e = 0;
   {
     const char* const qp = p.q + at * p.q_st + head * p.q_sh + half * 16;
@@ -451,7 +463,6 @@ __global__ __launch_bounds__(kBwdThreads, 2) void varlen_dq_kernel(VarlenBwdPara
     // all of them now (left to itself the compiler requests q once delta is done).
     __builtin_amdgcn_sched_barrier(0);
     using ET = std::conditional_t<kBF16, BF16, F16>;
-    float top = 0.f;
 #pragma unroll
     for (int ds = 0; ds < DS; ++ds) {
       float a[8], b[8];
@@ -467,7 +478,6 @@ __global__ __launch_bounds__(kBwdThreads, 2) void varlen_dq_kernel(VarlenBwdPara
     if constexpr (!kBF16) {
       top = max_xor32(top);
       e = top_exponent(top);
-      if (half == 0 && row < qs.len) p.top[(int64_t)head * p.total_q + at] = top;
     }
   }
 
@@ -532,16 +542,31 @@ __global__ __launch_bounds__(kBwdThreads, 2) void varlen_dq_kernel(VarlenBwdPara
         const int rel = lim - j0 - 4 * half;  // key 8 (i / 4) + i % 4 of the lane is seen iff < rel
 #pragma unroll
         for (int i = 0; i < 16; ++i)
-          if (8 * (i / 4) + i % 4 >= rel) s[i] = -INFINITY;
+          if (8 * (i / 4) + i % 4 >= rel) {
+            s[i] = -INFINITY;
+            if constexpr (!kBF16) dp[i] = 0.f;
+          }
       }
-      float mx = s[0];
+      float mx = s[0], big = 0.f;
 #pragma unroll
       for (int i = 1; i < 16; ++i) mx = fmaxf(mx, s[i]);
       mx = max_xor32(mx) * p.scale_log2;
-      if (__builtin_amdgcn_ballot_w64(mx > m + kSlack) != 0) {
+      bool up = mx > m + kSlack;
+      if constexpr (!kBF16) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) big = fmaxf(big, fabsf(dp[i]));
+        up = up || out_of_range(big, e);
+      }
+      if (__builtin_amdgcn_ballot_w64(up) != 0) {
         const float mn = fmaxf(m, mx);
-        const float alpha = fast_exp2(m - mn);
+        float alpha = m - mn;
         m = mn;
+        if constexpr (!kBF16) {
+          const int en = raised(big, e);
+          alpha += (float)(e - en);
+          e = en;
+        }
+        alpha = fast_exp2(alpha);
         l *= alpha;
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt) acc[dt] *= alpha;
@@ -563,27 +588,29 @@ __global__ __launch_bounds__(kBwdThreads, 2) void varlen_dq_kernel(VarlenBwdPara
   }
   l = sum_xor32(l);
   __syncthreads();  // every wave is done with the tiles
+  float base = kBF16 ? m : m + (float)e;  // what the sums are relative to
   // Where the wave's rows go out from, and in a split block its neighbour's sums lie.
   char* const s_x = s_kv + (kSplit ? (wave >> 1) * (DT * 4 + 1) * 1024 : wave * 32 * ROWB);
   if constexpr (kSplit) {
-    float2* const s_ml = reinterpret_cast<float2*>(s_x + DT * 4 * 1024);
+    float4* const s_ml = reinterpret_cast<float4*>(s_x + DT * 4 * 1024);
     if (wave & 1) {
       put_acc<DT>(acc, s_x, lane);
-      s_ml[lane] = make_float2(m, l);
+      s_ml[lane] = make_float4(base, l, __int_as_float(e), 0.f);
     }
     __syncthreads();
     if (wave & 1) return;
-    const float2 o = s_ml[lane];
-    const float mn = fmaxf(m, o.x), mine = fast_exp2(m - mn), theirs = fast_exp2(o.x - mn);
-    m = mn;
+    const float4 o = s_ml[lane];
+    const float mn = fmaxf(base, o.x), mine = fast_exp2(base - mn), theirs = fast_exp2(o.x - mn);
+    base = mn;
     l = l * mine + o.y * theirs;
+    e = max(e, __float_as_int(o.z));
     add_acc<DT>(acc, mine, s_x, theirs, lane);
   }
-  const float base = kBF16 ? m : m + (float)e;
   if (half == 0 && row < qs.len) {
     const int64_t w = (int64_t)head * p.total_q + at;
     p.lse[w] = l > 0.f ? base + __builtin_amdgcn_logf(l) - (kBF16 ? 0.f : (float)kF16Lift) : INFINITY;
     p.delta[w] = -delta;
+    if constexpr (!kBF16) p.top[w] = held_top(top, e);
   }
   write_rows<kBF16, D>(acc, l > 0.f ? p.scale / l : 0.f, s_x,
                        p.dq + (int64_t)qs.row * p.dq_st + head * p.dq_sh, p.dq_st, wrow, qs.len,
@@ -1129,16 +1156,31 @@ __global__ __launch_bounds__(kBwdThreads, 3) void varlen_window_kernel(VarlenBwd
         const int rel = lim - j0 - 4 * half;
 #pragma unroll
         for (int i = 0; i < 16; ++i)
-          if (8 * (i / 4) + i % 4 >= rel) s[i] = -INFINITY;
+          if (8 * (i / 4) + i % 4 >= rel) {
+            s[i] = -INFINITY;
+            if constexpr (!kBF16) dp[i] = 0.f;
+          }
       }
-      float mx = s[0];
+      float mx = s[0], big = 0.f;
 #pragma unroll
       for (int i = 1; i < 16; ++i) mx = fmaxf(mx, s[i]);
       mx = max_xor32(mx) * p.scale_log2;
-      if (__builtin_amdgcn_ballot_w64(mx > m + kSlack) != 0) {
+      bool up = mx > m + kSlack;
+      if constexpr (!kBF16) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) big = fmaxf(big, fabsf(dp[i]));
+        up = up || out_of_range(big, e);
+      }
+      if (__builtin_amdgcn_ballot_w64(up) != 0) {
         const float mn = fmaxf(m, mx);
-        const float alpha = fast_exp2(m - mn);
+        float alpha = m - mn;
         m = mn;
+        if constexpr (!kBF16) {
+          const int en = raised(big, e);
+          alpha += (float)(e - en);
+          e = en;
+        }
+        alpha = fast_exp2(alpha);
         l *= alpha;
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt) acc[dt] *= alpha;
@@ -1157,6 +1199,7 @@ __global__ __launch_bounds__(kBwdThreads, 3) void varlen_window_kernel(VarlenBwd
                         (kBF16 ? 0.f : (float)kF16Lift)
                   : INFINITY;
     mul = l > 0.f ? p.scale / l : 0.f;
+    if constexpr (!kBF16) top = held_top(top, e);
   }
   __syncthreads();  // every wave has been through K and V
   uint4 kreg[DS] = {}, vreg[DS] = {};
