@@ -136,3 +136,25 @@ def test_tokens_far_apart(dev, d, most):
         grads.append(torch.autograd.grad(out, leaves, dout))
     for a, b in zip(*grads):
         assert a.any() and torch.equal(a, b)
+
+
+def test_gradients_between_one_anothers_heads(dev):
+    """dq, dk and dv into one buffer [tokens, heads, 3, elements], as a projection of all three has
+    it, and rows rotated there in place."""
+    T, h, d = 50, 3, 64
+    rows = _rows(dev, T, h, h, d, 6)
+    q, k, v, dout = rows
+    cu = torch.tensor([0, T], dtype=torch.int32, device=dev)
+    out = ops.varlen_attention(q, k, v, cu, cu, T, T, scale=0.125, causal=True)
+    want = ops.varlen_attention_backward(dout, q, k, v, out, cu, cu, T, T, scale=0.125, causal=True)
+    buf = torch.full((T, h, 3, d), 7.0, dtype=torch.bfloat16, device=dev)
+    dq, dk, dv = (buf[:, :, i] for i in range(3))
+    ops.varlen_attention_backward(dout, q, k, v, out, cu, cu, T, T, scale=0.125, causal=True, dq=dq,
+                                  dk=dk, dv=dv)
+    for i in range(3):
+        assert torch.equal(buf[:, :, i], want[i])
+    pro = _prologue(dev, T, d)
+    turned = ops.rotary_embedding(*want[:2], pro.cos_sin_cache, pro.positions)
+    ops.rotary_embedding(dq, dk, pro.cos_sin_cache, pro.positions, q_out=dq, k_out=dk)
+    for i, t in enumerate((*turned, want[2])):
+        assert torch.equal(buf[:, :, i], t)

@@ -164,3 +164,33 @@ def test_rows_far_apart_reach_the_gradient_as_copies(monkeypatch):
             assert t.stride(0) * 2 < 1 << 25 and torch.equal(t, far[n])
     one = buf.as_strided((1, 2, 64), (step, 64, 1))  # a single row has no distance
     assert ops._near_rows(one) is one
+
+
+def test_heads_between_one_anothers_are_apart():
+    """q, k and v of a buffer [tokens, heads, 3, elements] share nothing; whatever is called apart
+    is so, element by element."""
+    T, H, D3 = 5, 3, 8
+    for dims in ((T, H, 3, D3), (H, T, 3, D3)):
+        buf = torch.zeros(dims)
+        parts = [buf[:, :, i] for i in range(3)]
+        if dims[0] == H:
+            parts = [t.transpose(0, 1) for t in parts]
+        ops._outputs_apart([("dq", parts[0], ()), ("dk", parts[1], ()), ("dv", parts[2], ())], ())
+        assert not ops._apart(parts[0], parts[0]) and not ops._apart(parts[1], buf.view(T, H, 24) if dims[0] == T
+                                                                     else buf.view(H, T, 24).transpose(0, 1))
+    g = torch.Generator().manual_seed(0)
+    memory, at = torch.zeros(4000), torch.arange(4000)
+    pick = lambda *xs: xs[int(torch.randint(len(xs), (), generator=g))]  # noqa: E731
+    seen = [0, 0]
+    for _ in range(3000):
+        views, where = [], []
+        for _ in range(2):
+            sizes = (pick(1, 2, 5), pick(1, 3, 4), 8)
+            strides = (pick(8, 16, 24, 32, 64, 72, 96, 120, 7), pick(8, 16, 24, 40, 64, 7), 1)
+            offset = pick(0, 8, 16, 24, 32, 48, 96, 500, 3)
+            views.append(memory.as_strided(sizes, strides, offset))
+            where.append(set(at.as_strided(sizes, strides, offset).flatten().tolist()))
+        share = bool(where[0] & where[1])
+        seen[share] += 1
+        assert not (share and ops._apart(*views)), (views[0].shape, views[0].stride(), views[1].shape, views[1].stride())
+    assert min(seen) > 500

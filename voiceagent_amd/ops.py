@@ -503,9 +503,10 @@ def _apart(a: torch.Tensor, b: torch.Tensor) -> bool:
         return True
     size = a.element_size()
 
-    def reach(t, but=-1):  # bytes from the first element to behind the last, of all dimensions but one
-        return sum((n - 1) * st for i, (n, st) in enumerate(zip(t.shape, t.stride())) if i != but
-                   ) * t.element_size() + t.element_size()
+    def reach(t, step=0):  # bytes from the first element to behind the last, but for whole steps
+        return t.element_size() + sum(
+            (n - 1) * st * t.element_size() for n, st in zip(t.shape, t.stride())
+            if not step or st * t.element_size() % step)
 
     pa, pb = a.data_ptr(), b.data_ptr()
     if pa + reach(a) <= pb or pb + reach(b) <= pa:
@@ -513,7 +514,7 @@ def _apart(a: torch.Tensor, b: torch.Tensor) -> bool:
     for dim in (0, 1):
         step = a.stride(dim) * size
         if step > 0 and b.stride(dim) * b.element_size() == step:
-            wa, wb, at = reach(a, dim), reach(b, dim), (pb - pa) % step
+            wa, wb, at = reach(a, step), reach(b, step), (pb - pa) % step
             if wa <= at and at + wb <= step:
                 return True
     return False
