@@ -158,3 +158,24 @@ def test_gradients_between_one_anothers_heads(dev):
     ops.rotary_embedding(dq, dk, pro.cos_sin_cache, pro.positions, q_out=dq, k_out=dk)
     for i, t in enumerate((*turned, want[2])):
         assert torch.equal(buf[:, :, i], t)
+
+
+@pytest.mark.parametrize("dtype,wdtype", [(torch.bfloat16, torch.bfloat16), (torch.float32, torch.float32)])
+def test_the_keys_alone_through_autograd(dev, dtype, wdtype):
+    """qk_norm_rope(None, k, ...): k's and its weight's gradients, either alone, are those of the
+    direct call.  (With both sides the weight's terms are the same and their order another.)"""
+    T, d = 33, 128
+    q, k, dk = (t.to(dtype) for t in _rows(dev, T, 3, 3, d, 7)[:3])
+    pro = _prologue(dev, T, d)
+    w = (torch.rand(d, generator=torch.Generator().manual_seed(8)) + 0.5).to(wdtype).to(dev)
+    pro = ops.QKPrologue(w, w, 1e-6, pro.cos_sin_cache, pro.positions)
+    _, want, _, want_w = ops.qk_norm_rope_backward(None, dk, None, k, pro)
+    assert torch.equal(want, ops.qk_norm_rope_backward(dk, dk, q, k, pro)[1])
+    for ask_k, ask_w in ((True, True), (True, False), (False, True)):
+        kk, ww = k.clone().requires_grad_(ask_k), w.clone().requires_grad_(ask_w)
+        none, out = ops.qk_norm_rope(None, kk, ops.QKPrologue(w, ww, 1e-6, pro.cos_sin_cache, pro.positions))
+        assert none is None and torch.equal(out, ops.qk_norm_rope(q, k, pro)[1])
+        out.backward(dk)
+        assert (kk.grad is None) == (not ask_k) and (ww.grad is None) == (not ask_w)
+        assert not ask_k or torch.equal(kk.grad, want)
+        assert not ask_w or torch.equal(ww.grad, want_w)
