@@ -68,3 +68,24 @@ def test_varlen_workgroups_per_cu(varlen_kernels):
         if have < want:
             short[key] = (vgprs, lds)
     assert not short
+
+
+def test_gradient_workgroups_per_cu():
+    """The gradient of varlen attention: two workgroups a CU at head_dim 128 and three at 64, as the
+    launches' choices of blocks and parts assume, none with scratch."""
+    found = {}
+    for elf in _code_objects(LIB_PATH.read_bytes()):
+        for k in _metadata(elf):
+            m = re.match(r"_ZN2va\d+varlen_(dq|dkv|window)_kernelI(.*)EEvNS_15VarlenBwdParamsE", k[".name"])
+            if m:
+                key = (m.group(1), *(int(x) for x in re.findall(r"L[bi](\d+)E", m.group(2) + "E")))
+                found[key] = (k[".vgpr_count"] + k.get(".agpr_count", 0),
+                              k[".group_segment_fixed_size"], k[".private_segment_fixed_size"])
+    assert len(found) == 18
+    short = {}
+    for key, (vgprs, lds, scratch) in found.items():
+        want = 2 if 128 in key else 3
+        have = min(512 // (-(-vgprs // 8) * 8), 160 * 1024 // max(lds, 1))
+        if have < want or scratch:
+            short[key] = (vgprs, lds, scratch)
+    assert not short

@@ -395,7 +395,7 @@ __device__ inline float held_top(float top, int e) { return e > top_exponent(top
 // other 32, and their sums meet in LDS at the end: launches whose blocks of 128
 // queries would leave the chip half idle take blocks of 64 in less time.
 template <bool kBF16, int D, bool kSplit>
-__global__ __launch_bounds__(kBwdThreads, 2) void varlen_dq_kernel(VarlenBwdParams p) {
+__global__ __launch_bounds__(kBwdThreads, D == 64 ? 3 : 2) void varlen_dq_kernel(VarlenBwdParams p) {
   constexpr int kTile = 64;  // keys
   constexpr int kRows = kSplit ? 64 : 128;  // queries of a workgroup, 32 a wave
   constexpr int ROWB = D * 2, TILE_B = kTile * ROWB, DS = D / 16, DT = D / 32;
