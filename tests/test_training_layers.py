@@ -194,3 +194,10 @@ def test_heads_between_one_anothers_are_apart():
         seen[share] += 1
         assert not (share and ops._apart(*views)), (views[0].shape, views[0].stride(), views[1].shape, views[1].stride())
     assert min(seen) > 500
+
+
+def test_an_output_without_its_input_is_refused():
+    x, w = torch.zeros(4, 2, 64), torch.ones(64)
+    pro = ops.QKPrologue(w, w, 1e-6, torch.zeros(9, 64), torch.zeros(4, dtype=torch.int64))
+    with pytest.raises(ops.AttentionArgumentError, match="dq without q"):
+        ops.qk_norm_rope_backward(None, x, None, x, pro, dq=torch.zeros(4, 2, 64))

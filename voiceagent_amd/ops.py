@@ -577,6 +577,7 @@ def qk_norm_rope_backward(
             if _FAST_NOT_TAKEN < rc < 0:
                 N.check("va_qk_norm_rope_backward", rc)
     _require((q is None) == (dq_out is None), "q and dq_out must be given together")
+    _require(q is not None or dq is None, "dq without q")
     device = _check_gpu(dq_out, dk_out, q, k, dq, dk, prologue.q_norm_weight,
                         prologue.k_norm_weight, prologue.cos_sin_cache, prologue.positions)
     sides = [("k", dk_out, k, dk)] if q is None else [("q", dq_out, q, dq), ("k", dk_out, k, dk)]
