@@ -201,3 +201,18 @@ def test_an_output_without_its_input_is_refused():
     pro = ops.QKPrologue(w, w, 1e-6, torch.zeros(9, 64), torch.zeros(4, dtype=torch.int64))
     with pytest.raises(ops.AttentionArgumentError, match="dq without q"):
         ops.qk_norm_rope_backward(None, x, None, x, pro, dq=torch.zeros(4, 2, 64))
+
+
+def test_sizes_past_the_argument_blocks_32_bits_are_refused(monkeypatch):
+    """2^32 + 4 tokens would be 4 of them there."""
+    monkeypatch.setattr(ops, "_check_gpu", lambda *tensors: torch.device("cpu"))  # (host checks alone)
+    table, pos, cu = torch.zeros(9, 2), torch.zeros(4, dtype=torch.int64), torch.tensor([0, 4], dtype=torch.int32)
+    x, many = torch.zeros(4, 1, 2), torch.zeros(1, 1, 2).expand(2 ** 32 + 4, 1, 2)
+    for call in (lambda: ops.rotary_embedding(many, None, table, pos, q_out=many),
+                 lambda: ops.rotary_embedding(x, torch.zeros(1, 1, 1).expand(4, 2 ** 32 + 1, 2), table, pos, q_out=x),
+                 lambda: ops.rotary_embedding(x, None, torch.zeros(1, 2).expand(2 ** 32 + 1, 2), pos, q_out=x),
+                 lambda: ops.varlen_attention_backward(
+                     *[t.bfloat16() for t in (x, x)], *[torch.zeros(1, 1, 2, dtype=torch.bfloat16).expand(2 ** 32 + 4, 1, 2)] * 2,
+                     x.bfloat16(), cu, cu, 4, 4, scale=1.0, causal=True, dq=x.bfloat16())):
+        with pytest.raises(ops.AttentionArgumentError, match=r"under 2\^31"):
+            call()

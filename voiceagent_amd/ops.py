@@ -714,6 +714,8 @@ def rotary_embedding(
     like = k if q is None else q
     _require(like.dim() == 3, "q and k must be [T, heads, D]")
     T, _, d = (int(x) for x in like.shape)
+    for n in (*like.shape, *(() if k is None else k.shape), *cos_sin_cache.shape[:1]):
+        _length(n, "every size")  # (the argument block's are 32-bit)
     args = N.new_args(N.RotaryArgs)
     args.dtype = _dtype_code(like)
     args.num_tokens, args.head_dim = T, d
@@ -1357,7 +1359,7 @@ def _row_strides(t: torch.Tensor) -> tuple[int, int]:
 
 def _length(n: int, name: str) -> int:
     n = int(n)
-    _require(0 <= n < 2 ** 31, f"{name} must be a length")
+    _require(0 <= n < 2 ** 31, f"{name} must be a length, from 0 to under 2^31")
     return n
 
 
@@ -1420,6 +1422,8 @@ def varlen_attention_backward(
              cu_seqlens_k.shape == cu_seqlens_q.shape, "cu_seqlens must be [num_seqs + 1]")
     _require(cu_seqlens_q.is_contiguous() and cu_seqlens_k.is_contiguous(),
              "cu_seqlens must be contiguous")
+    for n in (*q.shape, *k.shape, cu_seqlens_q.numel()):
+        _length(n, "every size")
     given = []
     for name, t, like in (("dq", dq, q), ("dk", dk, k), ("dv", dv, v)):
         if t is not None:
