@@ -36,7 +36,12 @@ constexpr int kQbBlocks = 1024;  // rows of partials at most
 // Row groups of a wave's unit of work, all of whose loads are in flight at once: of
 // 16 + 8 heads of 128 in bf16 8561 tokens take 31.8 us (158 MB, 5.0 TB/s) and 420 take
 // 5.6; two row groups 32.6 and 5.7, one 38.7 and 5.2 (and leaves three times the
-// partial sums).  Half the workgroups, 36 us.
+// partial sums).  Half the workgroups, 36 us.  A unit past the last head loads its rows
+// again, so what suits depends on the heads: calls of 158 MB with three, two and one
+// row groups, both launches, take 37.3, 39.1 and 44.2 us at 16 + 8 heads of 128, 41.9,
+// 38.5 and 45.6 at 14 + 14 of 64, 52.5, 49.9 and 62.4 at 8 + 1 of 64, 38.1, 37.0 and
+// 42.7 at 8 key heads of 128 alone, 38.4, 39.0 and 42.4 at 7 + 3 of 256, and 34.0, 34.7
+// and 39.4 at 16 + 8 of 128 in fp32.
 constexpr int kQbChunk = 3;
 
 template <typename ET, int D>

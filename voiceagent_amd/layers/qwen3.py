@@ -51,7 +51,8 @@ class RotaryScaling:
     * ``"yarn"`` (Peng et al., 2023): frequencies that turn at least
       ``beta_fast`` times over ``original_max_position`` stay, those that turn
       ``beta_slow`` times or fewer are divided by ``factor``, with a linear ramp
-      over the pairs' indices between; cosines and sines times
+      between, over the pairs' indices (the paper states one over the turns;
+      checkpoints' tables have this one); cosines and sines times
       ``attention_factor`` (0.1 ln factor + 1 if not given)."""
 
     kind: str
