@@ -95,6 +95,7 @@ def test_outputs_that_require_a_gradient_are_refused():
            lambda: ops.qk_norm_rope(y, x, pro, k_out=x),
            lambda: ops.qk_norm_rope(None, x, pro, k_out=x),
            lambda: ops.varlen_attention(y, y, y, cu, cu, 4, 4, scale=1.0, causal=True, out=x),
+           lambda: ops.paged_decode(y, y[None], y[None], cu[None], cu, max_seq_len=1, scale=1.0, out=x),
            lambda: ops._outputs_apart([("dq", x, ())], ())]
     for call in bad:
         with pytest.raises(ops.AttentionArgumentError, match="requires a gradient"):

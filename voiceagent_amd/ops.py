@@ -1003,7 +1003,8 @@ def paged_decode(
 ) -> torch.Tensor:
     """One-token paged GQA attention.
 
-    q: [B, Hq, D]; out: [B, Hq, D] (allocated if None); lens: per-sequence
+    q: [B, Hq, D]; out: [B, Hq, D] (allocated if None; it has no gradient, and
+    in grad mode may not require one); lens: per-sequence
     context lengths [B], or cu_seqlens_k [B + 1] with ``lens_cumulative``.
     ``new_k``/``new_v`` ([B, Hkv, D]) are written at position len-1 (or at
     ``new_slots[b]``) and used for that position in the same launch.  With a
@@ -1029,6 +1030,8 @@ def paged_decode(
     that is the batch's exact longest context (partitions fixed from it); a
     positive value fixes the partition size.
     """
+    if out is not None:
+        _plain_output(out, "out")
     mx4 = k_cache.dtype is MXFP4_KV_DTYPE
     fast = _FAST if _FAST_LOADED else _fast_calls()
     if (fast is not None and not no_alloc and layout in (LAYOUT_NHD, LAYOUT_HND) and
